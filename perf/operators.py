@@ -225,7 +225,7 @@ def _plain_forward(s):
 def _plain_train(s):
     h, last, a, before = _plain_forward(s)
     full, first, end = s["full"], s["first"], s["end"]
-    grad = s["grad_out"].float()
+    grad = s["grad_out"].to(torch.float32, copy=True)
     grad[end] += s["grad_last"][full]
     follow = torch.cat([a[1:], a[:1]])
     follow[end] = 0
