@@ -57,6 +57,8 @@ typedef enum {
     LCPP_I64 = 3,
     LCPP_U64 = 4,
     LCPP_F64 = 5,
+    LCPP_F16 = 6,  /* IEEE half; sequence operators only     */
+    LCPP_BF16 = 7, /* bfloat16; sequence operators only      */
     LCPP_NONE = 15 /* "no values" for SortKeys */
 } lcpp_dtype;
 
@@ -66,7 +68,7 @@ typedef enum { LCPP_OP_SUM = 0, LCPP_OP_MIN = 1, LCPP_OP_MAX = 2 } lcpp_op;
 typedef enum { LCPP_SCAN_EXCLUSIVE = 0, LCPP_SCAN_INCLUSIVE = 1 } lcpp_scan_kind;
 
 const char* lcpp_status_string(lcpp_status s);
-size_t      lcpp_dtype_size(int dtype);
+size_t      lcpp_dtype_size(int dtype); /* 0 for LCPP_F16 / LCPP_BF16, which the scalar primitives do not serve */
 
 /* ---- DeviceReduce ------------------------------------------------------
  * out[0] = init (+) reduce(in[0..n)), init = 0 / +max / lowest for
@@ -236,6 +238,81 @@ lcpp_status lcpp_reduce_by_key(int op, int key_dtype, int value_dtype, const voi
                                uint32_t* num_runs_out, uint64_t n, void* temp, size_t temp_bytes,
                                void* stream);
 
+
+/* ---- Sequence operators --------------------------------------------------
+ * No counterpart in the reference, whose scans and sorts are over scalars:
+ * the scan a recurrent language model is made of, with its gradient and its
+ * single-token form, and the selection and state reordering that decode such
+ * a model with beams.  dtype: LCPP_F32, LCPP_F16 or LCPP_BF16; states, scores
+ * and every sum are float32.  Matrices are row-major with unit element stride
+ * and a row stride in elements (>= channels, < 2^31; any value for one row);
+ * no alignment beyond the element's own is required.
+ *
+ * Gated linear recurrence, per channel (rows = tokens):
+ *   LCPP_GATE_LINEAR   h_t = gate_t h_{t-1} + in_t
+ *   LCPP_GATE_SIGMOID  h_t = a_t h_{t-1} + (1 - a_t) in_t, a_t = sigmoid(gate_t)
+ * Sequence s is rows [s * length, (s+1) * length) when offsets is NULL
+ * (rows = num_sequences * length), else rows [offsets[s], offsets[s+1]) of
+ * num_sequences + 1 ascending offsets; sequences may be empty, and rows before
+ * offsets[0] or from the last offset on are padding, whose outputs and
+ * gradients are 0 whatever they hold.  h before the first row is
+ * init[s * init_stride + c] (init_stride 0: one state for all; NULL: zeros).
+ * last[s * channels + c] (NULL: not wanted) is h after the last row; an empty
+ * sequence passes init on.  saved (NULL: no backward pass follows) receives
+ * lcpp_linear_recurrence_saved_bytes() for the backward call.  out may be
+ * gate or in, and last may be init (stride = channels).
+ * With LCPP_GATE_LINEAR the products of the gates along a stretch of up to
+ * 128 rows must stay finite. */
+enum { LCPP_GATE_LINEAR = 0, LCPP_GATE_SIGMOID = 1 };
+size_t      lcpp_linear_recurrence_temp_bytes(uint64_t rows, uint64_t channels);
+size_t      lcpp_linear_recurrence_saved_bytes(uint64_t rows, uint64_t channels);
+lcpp_status lcpp_linear_recurrence_forward(int gate, int dtype, const void* gate_in, uint64_t gate_stride,
+                                           const void* in, uint64_t in_stride, void* out, uint64_t out_stride,
+                                           uint64_t rows, uint64_t channels, uint64_t num_sequences,
+                                           uint64_t length, const uint32_t* offsets, const float* init,
+                                           uint64_t init_stride, float* last, void* saved, void* temp,
+                                           size_t temp_bytes, void* stream);
+/* Gradients from those of out (grad_out; NULL: 0) and last (grad_last, [num_sequences][channels]; NULL: 0),
+ * given the forward call's gate_in, in, init and saved: grad_gate, grad_in and grad_init
+ * ([num_sequences][channels], NULL: not wanted; one row per sequence also when init_stride is 0).
+ * grad_gate and grad_in may be gate_in, in or grad_out (each with the same stride). */
+lcpp_status lcpp_linear_recurrence_backward(int gate, int dtype, const void* gate_in, uint64_t gate_stride,
+                                            const void* in, uint64_t in_stride, const void* saved,
+                                            const float* init, uint64_t init_stride, const void* grad_out,
+                                            uint64_t grad_out_stride, const float* grad_last, void* grad_gate,
+                                            uint64_t grad_gate_stride, void* grad_in, uint64_t grad_in_stride,
+                                            float* grad_init, uint64_t rows, uint64_t channels,
+                                            uint64_t num_sequences, uint64_t length, const uint32_t* offsets,
+                                            void* temp, size_t temp_bytes, void* stream);
+/* One token: row i goes on from states_in[parents[i]] (parents NULL: row i; a negative parent or states_in NULL:
+ * zeros; a parent >= rows_in: zeros, and LCPP_ERR_INVALID_ARG in the device error word) and writes states_out[i]
+ * and its rounding to dtype, out[i] (NULL: not wanted).  States are [rows][channels] float32.  states_out may be
+ * states_in when parents is NULL, else they must not overlap. */
+lcpp_status lcpp_linear_recurrence_step(int gate, int dtype, const void* gate_in, uint64_t gate_stride,
+                                        const void* in, uint64_t in_stride, const float* states_in,
+                                        uint64_t rows_in, const int32_t* parents, float* states_out, void* out,
+                                        uint64_t out_stride, uint64_t rows, uint64_t channels, void* stream);
+
+/* Beam search's selection.  Row b * beams + k of logits is beam k of batch entry b (vocab tokens).  The candidates
+ * of a beam are its `beams` best tokens (larger logit first, equal logits by token) with the score
+ * scores_in[row] + log_softmax(logits[row])[token]; a finished beam (finished_in[row] != 0; NULL: none) has one
+ * candidate, eos_token with its score unchanged.  The `beams` best candidates of an entry (larger score first,
+ * equal scores by beam, then by place among the beam's candidates) are written in that order: scores_out,
+ * tokens_out, parents_out (the candidate's row) and finished_out (NULL: not wanted; 1 where the parent was
+ * finished or the token is eos_token; eos_token < 0: there is none).  A logit or score of -inf or NaN offers no
+ * candidate; an output that no candidate is left for has score -inf, token max(eos_token, 0), its own row as parent
+ * and is finished.  beams <= 32; outputs must not overlap inputs. */
+size_t      lcpp_beam_select_temp_bytes(uint64_t batches, uint32_t beams, uint64_t vocab);
+lcpp_status lcpp_beam_select(int dtype, const void* logits, uint64_t logits_stride, const float* scores_in,
+                             const uint8_t* finished_in, float* scores_out, int32_t* tokens_out,
+                             int32_t* parents_out, uint8_t* finished_out, uint64_t batches, uint32_t beams,
+                             uint64_t vocab, int32_t eos_token, void* temp, size_t temp_bytes, void* stream);
+/* States follow their beams: out[l][i] = in[l][parents[i]] for rows of row_bytes bytes, with layer and row strides
+ * in bytes; a negative parent: zeros; a parent >= rows_in: zeros, and LCPP_ERR_INVALID_ARG in the device error
+ * word.  in and out must not overlap. */
+lcpp_status lcpp_beam_reorder(const void* in, uint64_t in_layer_bytes, uint64_t in_row_bytes, void* out,
+                              uint64_t out_layer_bytes, uint64_t out_row_bytes, const int32_t* parents,
+                              uint64_t layers, uint64_t rows_in, uint64_t rows, uint64_t row_bytes, void* stream);
 
 /* ---- Multi-GPU (one process per GPU, NCCL) -----------------------------
  * No counterpart in the reference, which is single-GPU and limits item

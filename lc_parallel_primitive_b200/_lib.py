@@ -14,10 +14,13 @@ DATAGEN_PATH = _PKG / "libpcg_datagen.so"
 
 # lcpp_dtype
 I32, U32, F32, I64, U64, F64, NONE = 0, 1, 2, 3, 4, 5, 15
+F16, BF16 = 6, 7  # sequence operators only
 # lcpp_op
 OP_SUM, OP_MIN, OP_MAX = 0, 1, 2
 # lcpp_scan_kind
 SCAN_EXCLUSIVE, SCAN_INCLUSIVE = 0, 1
+# lcpp_gate
+GATE_LINEAR, GATE_SIGMOID = 0, 1
 XF_IDENTITY, XF_SQUARE, XF_ABS, XF_NEGATE = 0, 1, 2, 3
 # lcpp_status
 OK = 0
@@ -58,6 +61,18 @@ SIGNATURES = {
     "lcpp_scan_by_key": (_i, [_i, _i, _i, _i, _vp, _vp, _vp, _u64, _vp, _vp, _sz, _vp]),
     "lcpp_reduce_by_key_temp_bytes": (_sz, [_i, _i, _u64]),
     "lcpp_reduce_by_key": (_i, [_i, _i, _i, _vp, _vp, _vp, _vp, _vp, _u64, _vp, _sz, _vp]),
+    "lcpp_linear_recurrence_temp_bytes": (_sz, [_u64, _u64]),
+    "lcpp_linear_recurrence_saved_bytes": (_sz, [_u64, _u64]),
+    "lcpp_linear_recurrence_forward": (_i, [_i, _i, _vp, _u64, _vp, _u64, _vp, _u64, _u64, _u64, _u64, _u64, _vp,
+                                            _vp, _u64, _vp, _vp, _vp, _sz, _vp]),
+    "lcpp_linear_recurrence_backward": (_i, [_i, _i, _vp, _u64, _vp, _u64, _vp, _vp, _u64, _vp, _u64, _vp, _vp, _u64,
+                                             _vp, _u64, _vp, _u64, _u64, _u64, _u64, _vp, _vp, _sz, _vp]),
+    "lcpp_linear_recurrence_step": (_i, [_i, _i, _vp, _u64, _vp, _u64, _vp, _u64, _vp, _vp, _vp, _u64, _u64, _u64,
+                                         _vp]),
+    "lcpp_beam_select_temp_bytes": (_sz, [_u64, _u32, _u64]),
+    "lcpp_beam_select": (_i, [_i, _vp, _u64, _vp, _vp, _vp, _vp, _vp, _vp, _u64, _u32, _u64, C.c_int32, _vp, _sz,
+                              _vp]),
+    "lcpp_beam_reorder": (_i, [_vp, _u64, _u64, _vp, _u64, _u64, _vp, _u64, _u64, _u64, _u64, _vp]),
     "lcpp_mg_unique_id_bytes": (_sz, []),
     "lcpp_mg_get_unique_id": (_i, [_vp]),
     "lcpp_mg_comm_init_rank": (_i, [C.POINTER(_vp), _i, _vp, _i]),

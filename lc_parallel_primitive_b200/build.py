@@ -45,7 +45,7 @@ def _run(cmd, verbose):
     subprocess.run([str(c) for c in cmd], check=True)
 
 
-UNITS = ["unit_core", "unit_scan", "unit_sort", "unit_by_key"]
+UNITS = ["unit_core", "unit_scan", "unit_sort", "unit_by_key", "unit_sequence"]
 OBJDIR = PKG / "_build"
 
 

@@ -1,0 +1,33 @@
+// 2- and 4-byte floating element types of the sequence operators.  Arithmetic
+// is always float32; an element is widened when it is loaded and rounded to
+// nearest even once, when it is stored.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include "common.cuh"
+
+namespace lcpp {
+
+__device__ __forceinline__ float widen(float v) { return v; }
+__device__ __forceinline__ float widen(__half v) { return __half2float(v); }
+__device__ __forceinline__ float widen(__nv_bfloat16 v) { return __bfloat162float(v); }
+
+template <typename T> __device__ __forceinline__ T narrow(float v);
+template <> __device__ __forceinline__ float narrow<float>(float v) { return v; }
+template <> __device__ __forceinline__ __half narrow<__half>(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 narrow<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// Dispatch a functor over the three floating element types.
+template <typename F>
+inline lcpp_status dispatch_float(int dtype, F&& f) {
+    switch (dtype) {
+        case LCPP_F32: return f((float)0);
+        case LCPP_F16: return f(__half());
+        case LCPP_BF16: return f(__nv_bfloat16());
+        default: return LCPP_ERR_INVALID_ARG;
+    }
+}
+
+inline bool is_float_dtype(int dtype) { return dtype == LCPP_F32 || dtype == LCPP_F16 || dtype == LCPP_BF16; }
+
+}  // namespace lcpp
