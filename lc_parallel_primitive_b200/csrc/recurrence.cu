@@ -13,22 +13,39 @@
 // h_{t-1} is recomputed from one saved float32 state per LR_TILE rows, which
 // the forward pass writes: 4 / LR_TILE bytes an element instead of reading the
 // outputs back, and no rounding of h_{t-1} to the element type.
+//
+// Both passes read each operand once and write each result once.  A tile is
+// LR_TILE rows x one lane word (4 bytes) per lane of a warp; the compute warps
+// of a CTA take LR_ROWS rows each and turn them into the affine map
+// h_after = A h_before + H that the rows are.  Look-back warps join the maps of
+// the CTA's warps and of the tiles before (a decoupled look-back, Merrill &
+// Garland 2016, over affine maps) while the compute warps already turn the next
+// tile into its maps, so that the chain from tile to tile has a whole tile's
+// time to arrive.
 #include "float_types.cuh"
 
 namespace lcpp {
 
-constexpr int LR_TILE = 128;                  // rows of a tile, and rows between two saved states
-constexpr int LR_WARPS = 8;
-constexpr int LR_THREADS = LR_WARPS * 32;
-constexpr int LR_ROWS = LR_TILE / LR_WARPS;   // consecutive rows of one warp
+constexpr int LR_TILE = 128;                    // rows of a tile, and rows between two saved states
+constexpr int LR_WARPS = 16;                    // compute warps
+constexpr int LR_ROWS = LR_TILE / LR_WARPS;     // consecutive rows of one warp
 constexpr uint32_t LR_ALL = (1u << LR_ROWS) - 1;
-constexpr int LR_LANE_BYTES = 4;              // of one row, per lane: 1 float or 2 halves
-constexpr int LR_ROW_BYTES = 32 * LR_LANE_BYTES;
-constexpr int LR_BUF = LR_TILE * LR_ROW_BYTES;  // 16 KiB: one matrix of a tile
+constexpr int LR_ROW_BYTES = 128;               // a row of a tile: 4 bytes per lane, 1 float or 2 halves
+constexpr int LR_WARP_BUF = LR_ROWS * LR_ROW_BYTES;  // one warp's rows of one matrix
+
+// Division of 32-bit numbers by a fixed one: the high half of n * ceil(2^64 / d) is n / d for all n, d < 2^32
+// (the error n / 2^64 cannot reach the next quotient, 1 / d away).
+struct LrDivisor {
+    uint32_t d;
+    uint64_t m;
+    explicit LrDivisor(uint64_t v) : d((uint32_t)v), m(v > 1 ? ~0ull / v + 1 : 0) {}
+    __device__ __forceinline__ uint32_t div(uint32_t n) const { return m ? (uint32_t)__umul64hi(m, n) : n; }
+};
 
 struct LrShape {
-    uint64_t rows, channels, sequences, length;  // length: rows of a sequence when offsets is null
-    const uint32_t* offsets;                     // sequences + 1 row offsets, or null
+    uint64_t rows, channels, sequences;
+    LrDivisor length;         // rows of a sequence when offsets is null
+    const uint32_t* offsets;  // sequences + 1 row offsets, or null
 };
 
 // Sigmoid: a = 1 / (1 + e) and 1 - a = e a with e = exp(-g), so that
@@ -58,10 +75,9 @@ struct Gate {
         }
     }
     __device__ __forceinline__ float add(float x) const { return GATE == LCPP_GATE_SIGMOID ? na * x : x; }  // b
-    __device__ __forceinline__ float grad_gate(float lam, float before, float x) const {
-        return GATE == LCPP_GATE_SIGMOID ? lam * (before - x) * (a * na) : lam * before;
+    __device__ __forceinline__ float grad_gate(float before, float x) const {  // of h, by the gate
+        return GATE == LCPP_GATE_SIGMOID ? (before - x) * (a * na) : before;
     }
-    __device__ __forceinline__ float grad_in(float lam) const { return GATE == LCPP_GATE_SIGMOID ? na * lam : lam; }
 };
 
 struct LrForward {
@@ -83,12 +99,10 @@ struct LrBackward {
 };
 
 // ---- Which rows begin and end sequences ------------------------------------
-// Found by each warp for its LR_ROWS rows; bit i stands for row first + i.
-struct LrMarks {
-    uint32_t head, tail, valid;  // first / last row of a sequence; row of any sequence
-    int64_t base;                // offsets: sequence of lane 0's offset
-    uint32_t off;                // offsets: offsets[base + lane]
-};
+// Every row has a code: LR_OUTSIDE (of all sequences), or LR_HEAD and LR_TAIL
+// bits with the row's sequence (0 where neither bit is set).  Computed where
+// all sequences have one length, else written by lr_prepare_kernel.
+constexpr uint32_t LR_OUTSIDE = 1u << 31, LR_HEAD = 1u << 30, LR_TAIL = 1u << 29, LR_SEQUENCE = LR_TAIL - 1;
 
 // Number of offsets[0 .. count) that are <= row, minus 1 (-1: none); the warp narrows the range 32-fold a step.
 __device__ __forceinline__ int64_t lr_search(const uint32_t* offsets, uint64_t count, uint64_t row) {
@@ -104,632 +118,687 @@ __device__ __forceinline__ int64_t lr_search(const uint32_t* offsets, uint64_t c
     return (int64_t)lo - 1;
 }
 
-__device__ __forceinline__ LrMarks lr_marks(const LrShape& sh, uint64_t first) {
-    const int lane = threadIdx.x & 31;
-    LrMarks m;
-    m.base = 0;
-    m.off = 0;
-    if (!sh.offsets) {
-        const uint32_t row = (uint32_t)first + lane, length = (uint32_t)sh.length;
-        const uint32_t at = __ballot_sync(0xffffffffu, row % length == 0);
-        m.valid = __ballot_sync(0xffffffffu, lane < LR_ROWS && first + lane < sh.rows);
-        m.head = at & m.valid;
-        m.tail = (at >> 1) & m.valid;
-        return m;
+// The codes of a warp's rows, lane r holding row r's, and masks of them.
+struct LrMarks {
+    uint32_t code, head, tail, valid;
+    __device__ __forceinline__ explicit LrMarks(uint32_t c) : code(c) {
+        const bool mine = (threadIdx.x & 31) < LR_ROWS;
+        head = __ballot_sync(0xffffffffu, mine && (c & LR_HEAD));
+        tail = __ballot_sync(0xffffffffu, mine && (c & LR_TAIL));
+        valid = __ballot_sync(0xffffffffu, mine && !(c & LR_OUTSIDE));
     }
-    const uint64_t S = sh.sequences;
-    const uint64_t lo = sh.offsets[0], hi = min((uint64_t)sh.offsets[S], sh.rows);
-    m.valid = __ballot_sync(0xffffffffu, lane < LR_ROWS && first + lane >= lo && first + lane < hi);
-    uint32_t head = 0, tail = 0;
-    const int64_t at = max(lr_search(sh.offsets, S + 1, first), (int64_t)0);
-    m.base = at;
-    for (uint64_t i = at; ; i += 32) {
-        const uint32_t off = i + lane <= S ? sh.offsets[i + lane] : 0xffffffffu;
-        if (i == (uint64_t)at) m.off = off;
-        if (off >= first && off < first + LR_ROWS) head |= 1u << (off - first);
-        if (off > first && off <= first + LR_ROWS && off > lo) tail |= 1u << (off - first - 1);
-        if (i + 32 > S || __any_sync(0xffffffffu, off > first + LR_ROWS)) break;
+    // Sequence of row r, which is a head or tail.
+    __device__ __forceinline__ uint64_t sequence(const LrShape& sh, int r) const {
+        return min((uint64_t)(__shfl_sync(0xffffffffu, code, r) & LR_SEQUENCE), sh.sequences - 1);
     }
-    m.head = __reduce_or_sync(0xffffffffu, head) & m.valid;
-    m.tail = __reduce_or_sync(0xffffffffu, tail) & m.valid;
-    return m;
-}
-
-// Sequence of a valid row of the warp (warp-uniform call).
-__device__ __forceinline__ uint64_t lr_sequence(const LrShape& sh, const LrMarks& m, uint64_t row) {
-    if (!sh.offsets) return (uint32_t)row / (uint32_t)sh.length;
-    const uint32_t le = __ballot_sync(0xffffffffu, m.off <= row);
-    int64_t s = m.base + __popc(le) - 1;
-    if (le == 0xffffffffu) s = lr_search(sh.offsets, sh.sequences + 1, row);
-    return (uint64_t)min(max(s, (int64_t)0), (int64_t)sh.sequences - 1);
+};
+__device__ __forceinline__ uint32_t lr_code(const LrShape& sh, uint64_t row, const uint32_t* fetched) {
+    if (row >= sh.rows) return LR_OUTSIDE;
+    if (sh.offsets) return *fetched;
+    const uint32_t r = (uint32_t)row, s = sh.length.div(r), at = r - s * sh.length.d;
+    return (at == 0 ? LR_HEAD : 0) | (at + 1 == sh.length.d ? LR_TAIL : 0) | s;
 }
 
 // ---- Look-back between the tiles of a column -----------------------------------
-// A tile maps the state before it to the state after it, h -> A h + H.  Words
-// are float32 and their own flag: LR_NONE (a NaN that arithmetic does not make)
-// until published, so no status word and no ordering is needed.  pair[tile]
-// [channel] = (A, H) of the tile alone, state[tile][channel] = the state after it.
+// A tile maps the state before it to the state after it, h -> A h + H.  A tile's
+// record for a channel is (A, H, state after it, -).  Words are float32 and their
+// own flag: LR_NONE (a NaN that arithmetic does not make) until published, so no
+// status word and no ordering is needed.
 constexpr uint32_t LR_NONE = 0xffffffffu;
 
 struct LrChain {
-    uint32_t* ticket;  // starts at LR_NONE
-    float2* pair;
-    float* state;
+    float4* record;  // [row tile][width]
     uint64_t width;  // channels, rounded up to whole column tiles
 };
 __device__ __forceinline__ float lr_word(float v) { return __float_as_uint(v) == LR_NONE ? __uint_as_float(0x7fffffffu) : v; }
 __device__ __forceinline__ bool lr_there(float v) { return __float_as_uint(v) != LR_NONE; }
-__device__ __forceinline__ void lr_put(float* p, float v) {
-    asm volatile("st.relaxed.gpu.global.f32 [%0], %1;" ::"l"(p), "f"(lr_word(v)) : "memory");
+__device__ __forceinline__ void lr_put_state(float4* r, float v) {
+    asm volatile("st.relaxed.gpu.global.f32 [%0], %1;" ::"l"(&r->z), "f"(lr_word(v)) : "memory");
 }
-__device__ __forceinline__ void lr_put(float2* p, float2 v) {
-    asm volatile("st.relaxed.gpu.global.v2.f32 [%0], {%1, %2};" ::"l"(p), "f"(lr_word(v.x)), "f"(lr_word(v.y)) : "memory");
+__device__ __forceinline__ void lr_put_map(float4* r, float a, float h) {
+    asm volatile("st.relaxed.gpu.global.v2.f32 [%0], {%1, %2};" ::"l"(r), "f"(lr_word(a)), "f"(lr_word(h)) : "memory");
 }
-__device__ __forceinline__ float lr_get(const float* p) {
-    float v;
-    asm volatile("ld.relaxed.gpu.global.f32 %0, [%1];" : "=f"(v) : "l"(p) : "memory");
-    return v;
-}
-__device__ __forceinline__ float2 lr_get(const float2* p) {
-    float2 v;
-    asm volatile("ld.relaxed.gpu.global.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "l"(p) : "memory");
+__device__ __forceinline__ float4 lr_get(const float4* r) {
+    float4 v;
+    asm volatile("ld.relaxed.gpu.global.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(r) : "memory");
     return v;
 }
 
-// The next tile's number, for all threads of the CTA.
-__device__ __forceinline__ uint32_t lr_ticket(const LrChain& ch, uint32_t* shared) {
-    __syncthreads();
-    if (threadIdx.x == 0) *shared = atomicAdd(ch.ticket, 1u) + 1u;
-    __syncthreads();
-    return *shared;
+// The state of one channel behind the nearest of `left` tiles, whose records
+// are at r, r + step, ... (with none left, the state is 0).  The lane reads W
+// of them until one shows its state and all nearer ones their maps, and goes
+// from there down the tiles, state = A state + H, as those tiles do themselves:
+// the result does not depend on how far back the state was found.  Bounded by
+// the spin limit, after which the error word is set.
+template <int W>
+__device__ __forceinline__ float lr_lookback(const float4* r, int64_t step, uint32_t left, bool active) {
+    const uint32_t limit = g_spin_limit;
+    for (uint32_t spins = 0;; ++spins) {
+        float4 v[W];
+#pragma unroll
+        for (int j = 0; j < W; ++j) {
+            v[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (j < left) v[j] = lr_get(r + j * step);
+        }
+        uint32_t states = 0, maps = 0;
+#pragma unroll
+        for (int j = 0; j < W; ++j) {
+            states |= lr_there(v[j].z) ? 1u << j : 0;
+            maps |= lr_there(v[j].x) && lr_there(v[j].y) ? 1u << j : 0;
+        }
+        const int from = __ffs(states) - 1;
+        const bool found = from >= 0 && (~maps & ((1u << from) - 1)) == 0;
+        if (__all_sync(0xffffffffu, found || !active)) {
+            float carry = 0.0f;
+#pragma unroll
+            for (int j = W - 1; j >= 0; --j) carry = j >= from ? v[j].z : fmaf(v[j].x, carry, v[j].y);
+            return carry;
+        }
+        if (spins >= limit) {
+            if (!found && active) set_error(LCPP_ERR_LOOKBACK_TIMEOUT);
+            return 0.0f;
+        }
+        if (spins > 64) __nanosleep(32);
+    }
 }
 
-// ---- Tiles in shared memory ----------------------------------------------------
+// ---- Warps and their barriers ---------------------------------------------------
+// A CTA has LR_WARPS compute warps, and for each 32 channels one publishing and
+// one look-back warp, a channel a lane.  Tile i of a CTA (its i-th) uses buffer
+// i & 1.  The compute warps write their maps and arrive at barriers 1 + (i & 1),
+// on which the publishing warps wait, and 5 + (i & 1), for the look-back warps.
+// The publishing warps join the maps and publish the tile's, a tile ahead of its
+// outputs and whatever the look-back warps still wait for; these find the state
+// before the tile meanwhile, and write every warp's start.  Both then arrive at
+// 3 + (i & 1), on which the compute warps wait.  A compute warp writes the maps
+// of tile i + 2 after it has waited for the starts of tile i, so two buffers do.
+__device__ __forceinline__ void lr_sync(int barrier, int threads) {
+    asm volatile("bar.sync %0, %1;" ::"r"(barrier), "r"(threads) : "memory");
+}
+__device__ __forceinline__ void lr_arrive(int barrier, int threads) {
+    asm volatile("bar.arrive %0, %1;" ::"r"(barrier), "r"(threads) : "memory");
+}
+
+// ---- Rows in shared memory -------------------------------------------------------
 // How rows can be copied: by 16-byte or 4-byte asynchronous copies, or element
 // by element (2-byte elements on odd addresses or strides).
 enum { LR_COPY16 = 0, LR_COPY4 = 1, LR_COPY_ELEMENT = 2 };
 
-// Copies rows [row0, row0 + LR_TILE) x one column tile of a matrix to buf
-// (LR_ROW_BYTES a row); rows from `rows` on and channels from `channels` on are
-// left as they are.  Asynchronous copies are part of the caller's next commit.
+// Copies a warp's rows, first .., of one column tile of a matrix to buf; rows
+// from `rows` on and channels from `channels` on are left as they are.
+// Asynchronous copies are part of the warp's next commit.
 template <typename T, int COPY>
-__device__ __forceinline__ void lr_fetch(char* buf, const T* m, uint64_t stride, uint64_t row0, uint64_t rows,
+__device__ __forceinline__ void lr_fetch(char* buf, const T* m, uint64_t stride, uint64_t first, uint64_t rows,
                                          uint32_t channel0, uint32_t channels) {
-    const int tid = threadIdx.x;
-    const uint32_t left = (uint32_t)min((uint64_t)LR_TILE, rows - row0);
+    const int lane = threadIdx.x & 31;
+    const int n = (int)min((uint64_t)LR_ROWS, rows - min(rows, first));
+    m += first * stride + channel0;
     if constexpr (COPY == LR_COPY16) {
-        constexpr int PER_ROW = LR_ROW_BYTES / 16, STEP = LR_THREADS / PER_ROW, V = 16 / sizeof(T);
-        const uint32_t r0 = tid / PER_ROW, c = (tid % PER_ROW) * V;
+        constexpr int V = 16 / sizeof(T);
+        const int r0 = lane / 8, c = (lane % 8) * V;
         if (channel0 + c >= channels) return;
-        const T* src = m + (row0 + r0) * stride + channel0 + c;
-        char* dst = buf + tid * 16;
 #pragma unroll
-        for (int j = 0; j < LR_TILE / STEP; ++j, src += STEP * stride)
-            if (r0 + j * STEP < left) cp_async16(dst + j * LR_THREADS * 16, src);
+        for (int r = r0; r < LR_ROWS + r0; r += 4)
+            if (r < n) cp_async16(buf + r * LR_ROW_BYTES + lane % 8 * 16, m + r * stride + c);
     } else if constexpr (COPY == LR_COPY4) {
         constexpr int V = 4 / sizeof(T);
-        const uint32_t r0 = tid / 32, c = (tid % 32) * V;
-        if (channel0 + c >= channels) return;
-        const T* src = m + (row0 + r0) * stride + channel0 + c;
-        char* dst = buf + tid * 4;
-#pragma unroll 8
-        for (int j = 0; j < LR_TILE / LR_WARPS; ++j, src += LR_WARPS * stride)
-            if (r0 + j * LR_WARPS < left) cp_async4(dst + j * LR_THREADS * 4, src);
+        if (channel0 + lane * V >= channels) return;
+#pragma unroll
+        for (int r = 0; r < LR_ROWS; ++r)
+            if (r < n) cp_async4(buf + r * LR_ROW_BYTES + lane * 4, m + r * stride + lane * V);
     } else {
-        constexpr int PER_ROW = LR_ROW_BYTES / sizeof(T), STEP = LR_THREADS / PER_ROW;
-        const uint32_t r0 = tid / PER_ROW, c = tid % PER_ROW;
-        if (channel0 + c >= channels) return;
-        const T* src = m + (row0 + r0) * stride + channel0 + c;
-        T* dst = (T*)buf + tid;
-#pragma unroll 16
-        for (int j = 0; j < LR_TILE / STEP; ++j, src += STEP * stride)
-            if (r0 + j * STEP < left) dst[j * LR_THREADS] = *src;
+        T v[LR_ROWS][2];
+#pragma unroll
+        for (int r = 0; r < LR_ROWS; ++r)
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                if (r < n && channel0 + i * 32 + lane < channels) v[r][i] = m[r * stride + i * 32 + lane];
+#pragma unroll
+        for (int r = 0; r < LR_ROWS; ++r)
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                if (r < n && channel0 + i * 32 + lane < channels)
+                    ((T*)(buf + r * LR_ROW_BYTES))[i * 32 + lane] = v[r][i];
     }
 }
 
-// One lane's channels of one row, in shared memory.
-template <typename T> struct LrLane;
-template <> struct LrLane<float> {
+// One lane's word of a row: its channels widened, and narrowed again.
+template <typename T> struct LrWord;
+template <> struct LrWord<float> {
     static constexpr int N = 1;
-    static __device__ __forceinline__ void load(const char* row, float* v) { v[0] = ((const float*)row)[threadIdx.x & 31]; }
+    static __device__ __forceinline__ void widen(uint32_t w, float* v) { v[0] = __uint_as_float(w); }
+    static __device__ __forceinline__ uint32_t narrow(const float* v) { return __float_as_uint(v[0]); }
 };
-template <> struct LrLane<__half> {
+template <> struct LrWord<__half> {
     static constexpr int N = 2;
-    static __device__ __forceinline__ void load(const char* row, float* v) {
-        const float2 f = __half22float2(((const __half2*)row)[threadIdx.x & 31]);
+    static __device__ __forceinline__ void widen(uint32_t w, float* v) {
+        __half2 h;
+        memcpy(&h, &w, 4);
+        const float2 f = __half22float2(h);
         v[0] = f.x, v[1] = f.y;
     }
-};
-template <> struct LrLane<__nv_bfloat16> {
-    static constexpr int N = 2;
-    static __device__ __forceinline__ void load(const char* row, float* v) {
-        const uint32_t b = ((const uint32_t*)row)[threadIdx.x & 31];
-        v[0] = __uint_as_float(b << 16), v[1] = __uint_as_float(b & 0xffff0000u);
+    static __device__ __forceinline__ uint32_t narrow(const float* v) {
+        const __half2 h = __floats2half2_rn(v[0], v[1]);
+        uint32_t w;
+        memcpy(&w, &h, 4);
+        return w;
     }
 };
-// Stores one lane's channels (`left` of them in range; wide: 4-byte stores are aligned).
-template <typename T, bool WIDE>
+template <> struct LrWord<__nv_bfloat16> {
+    static constexpr int N = 2;
+    static __device__ __forceinline__ void widen(uint32_t w, float* v) {
+        v[0] = __uint_as_float(w << 16), v[1] = __uint_as_float(w & 0xffff0000u);
+    }
+    static __device__ __forceinline__ uint32_t narrow(const float* v) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(v[0], v[1]);
+        uint32_t w;
+        memcpy(&w, &h, 4);
+        return w;
+    }
+};
+__device__ __forceinline__ uint32_t lr_load(const char* rows, int r) {
+    return ((const uint32_t*)(rows + r * LR_ROW_BYTES))[threadIdx.x & 31];
+}
+// Stores one lane's channels, `left` of them in range.
+template <typename T, int COPY>
 __device__ __forceinline__ void lr_store(T* p, const float* v, int left) {
-    if constexpr (sizeof(T) == 4) {
-        if (left > 0) *p = v[0];
-    } else if constexpr (WIDE) {
-        if (left > 0) {
-            uint32_t b;
-            if constexpr (std::is_same_v<T, __half>) {
-                const __half2 h = __floats2half2_rn(v[0], v[1]);
-                memcpy(&b, &h, 4);
-            } else {
-                const __nv_bfloat162 h = __floats2bfloat162_rn(v[0], v[1]);
-                memcpy(&b, &h, 4);
-            }
-            *(uint32_t*)p = b;
-        }
+    if constexpr (sizeof(T) == 4 || COPY != LR_COPY_ELEMENT) {
+        if (left > 0) *(uint32_t*)p = LrWord<T>::narrow(v);
     } else {
         if (left > 0) p[0] = narrow<T>(v[0]);
         if (left > 1) p[1] = narrow<T>(v[1]);
     }
 }
 
-// The state before tile k of a column (REVERSE: behind it), from the LR_WINDOW
-// tiles before it, two of which each warp reads.  The CTA reads the window
-// again until every channel finds a state in it, and goes from the nearest one
-// down the tiles, state = A state + H, just as those tiles do themselves: the
-// result does not depend on how far back the state was found.
-constexpr int LR_WINDOW = 2 * LR_WARPS;
+// Whether row is the first of a sequence, or outside (nothing passes it from before).
+__device__ __forceinline__ bool lr_starts(const LrShape& sh, const uint32_t* codes, uint64_t row) {
+    return lr_code(sh, row, codes + row) & (LR_HEAD | LR_OUTSIDE);
+}
+__device__ __forceinline__ bool lr_ends(const LrShape& sh, const uint32_t* codes, uint64_t row) {
+    return lr_code(sh, row, codes + row) & (LR_TAIL | LR_OUTSIDE);
+}
 
-template <int N, bool REVERSE>
-__device__ __forceinline__ void lr_lookback(const LrChain& ch, int64_t k, int64_t tiles, uint32_t channel0,
-                                            uint32_t channels, float2* s_win, float* carry) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const uint32_t limit = g_spin_limit;
-    uint32_t spins = 0;
-    while (true) {
-        float st[2][N];
-        float2 pr[2][N];
-        bool there;
-        do {  // until each of this warp's tiles shows its map or its state
-            there = true;
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const int64_t d = 1 + warp + j * LR_WARPS, p = REVERSE ? k + d : k - d;
-#pragma unroll
-                for (int i = 0; i < N; ++i) {
-                    const uint32_t c = channel0 + lane * N + i;
-                    st[j][i] = 0.0f;  // before the first tile the state is 0
-                    pr[j][i] = make_float2(0.0f, 0.0f);
-                    if (p >= 0 && p < tiles && c < channels) {
-                        st[j][i] = lr_get(ch.state + (uint64_t)p * ch.width + c);
-                        pr[j][i] = lr_get(ch.pair + (uint64_t)p * ch.width + c);
-                        there &= lr_there(st[j][i]) || (lr_there(pr[j][i].x) && lr_there(pr[j][i].y));
-                    }
-                }
-            }
-            if (!there) {
-                if (++spins > limit) {
-                    set_error(LCPP_ERR_LOOKBACK_TIMEOUT);
-                    break;
-                }
-                if (spins > 16) __nanosleep(32);
-            }
-        } while (!there);
-        // a state is handed over as (LR_NONE, state)
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int i = 0; i < N; ++i)
-                s_win[(warp + j * LR_WARPS) * 32 * N + lane * N + i] =
-                    lr_there(st[j][i]) ? make_float2(__uint_as_float(LR_NONE), st[j][i]) : pr[j][i];
-        __syncthreads();
-        bool open = false;
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            int j = 0;
-            while (j < LR_WINDOW && lr_there(s_win[j * 32 * N + lane * N + i].x)) ++j;
-            open |= j == LR_WINDOW;
-            carry[i] = j < LR_WINDOW ? s_win[j * 32 * N + lane * N + i].y : 0.0f;
-            while (j-- > 0) {
-                const float2 w = s_win[j * 32 * N + lane * N + i];
-                carry[i] = fmaf(w.x, carry[i], w.y);
-            }
-        }
-        if (!__syncthreads_or(open && spins <= limit)) return;
-        if (++spins > limit) set_error(LCPP_ERR_LOOKBACK_TIMEOUT);
+// What a kernel of this file knows about its tiles: CTA b takes tiles b, b + grid, ..., numbered along the
+// channels first.  All CTAs of a chained launch are resident (a cooperative launch), so a tile may wait for the
+// tiles before it wherever they are.
+struct LrTiles {
+    uint32_t row_tiles;
+    LrDivisor col_tiles;
+    const uint32_t* codes;  // of the rows (with offsets)
+    bool narrow;            // many tiles of a column are under way at a time
+    __device__ __forceinline__ uint32_t count() const {
+        const uint32_t total = row_tiles * col_tiles.d;
+        return blockIdx.x < total ? (total - blockIdx.x - 1) / gridDim.x + 1 : 0;
     }
+    // Tile i of this CTA: its row tile, counted from the first (or last) one, and its column tile.
+    __device__ __forceinline__ uint2 tile(uint32_t i) const {
+        const uint32_t t = blockIdx.x + i * gridDim.x, k = col_tiles.div(t);
+        return make_uint2(k, t - k * col_tiles.d);
+    }
+};
+// Which warps of a CTA cut the chain, as bits, from one word each.
+__device__ __forceinline__ uint32_t lr_cuts(const uint32_t* cut, uint32_t bit) {
+    const int lane = threadIdx.x & 31;
+    return __ballot_sync(0xffffffffu, lane < LR_WARPS && (cut[lane % LR_WARPS] & bit));
 }
 
 // ---- Forward ---------------------------------------------------------------------
-template <typename T, int GATE, int COPY>
-__global__ void __launch_bounds__(LR_THREADS, 3) lr_forward_kernel(LrForward p, LrChain ch, uint32_t row_tiles, uint32_t col_tiles) {
-    constexpr int N = LrLane<T>::N, C = 32 * N;
-    extern __shared__ __align__(128) char smem[];  // [2 stages][gate, in][LR_BUF]
-    __shared__ float2 s_agg[LR_WARPS * C], s_win[LR_WINDOW * C];
-    __shared__ uint32_t s_reset[LR_WARPS], s_ticket;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const uint32_t channels = (uint32_t)p.sh.channels;
-    const uint64_t total = (uint64_t)row_tiles * col_tiles;
-    const bool chained = row_tiles > 1;
+template <typename T>
+struct LrForwardSmem {
+    static constexpr int STAGES = 4, C = 32 * LrWord<T>::N;
+    char rows[STAGES][LR_WARPS][2][LR_WARP_BUF];  // gate, in
+    uint32_t code[STAGES][LR_WARPS][LR_ROWS];
+    float2 map[2][LR_WARPS][C];  // (A, H) of a warp's rows
+    float start[2][LR_WARPS][C];
+    uint32_t cut[2][LR_WARPS];   // nothing from before a warp's rows passes them
+};
 
-    auto fetch = [&](uint64_t t, int stage) {
-        if (t < total) {
-            const uint64_t row0 = t / col_tiles * LR_TILE;
-            const uint32_t c0 = (uint32_t)(t % col_tiles) * C;
-            char* buf = smem + stage * 2 * LR_BUF;
-            lr_fetch<T, COPY>(buf, (const T*)p.gate, p.gate_stride, row0, p.sh.rows, c0, channels);
-            lr_fetch<T, COPY>(buf + LR_BUF, (const T*)p.in, p.in_stride, row0, p.sh.rows, c0, channels);
+template <typename T>
+constexpr int LR_THREADS = (LR_WARPS + 2 * LrWord<T>::N) * 32;
+
+template <typename T, int GATE, int COPY>
+__global__ void __launch_bounds__(LR_THREADS<T>, 1) lr_forward_kernel(LrForward p, LrChain ch, LrTiles tl) {
+    constexpr int N = LrWord<T>::N, C = 32 * N, THREADS = LR_THREADS<T>;
+    using Smem = LrForwardSmem<T>;
+    extern __shared__ __align__(128) char smem_raw[];
+    Smem& sm = *(Smem*)smem_raw;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const uint32_t channels = (uint32_t)p.sh.channels, count = tl.count();
+
+    if (warp >= LR_WARPS) {
+        const bool publishes = warp >= LR_WARPS + N;
+        const int cc = (warp - LR_WARPS) % N * 32 + lane;
+        for (uint32_t i = 0; i < count; ++i) {
+            const int b = i & 1;
+            const uint2 t = tl.tile(i);
+            const uint32_t k = t.x, c = t.y * C + cc;
+            float4* record = ch.record + (uint64_t)k * ch.width + c;
+            const bool active = c < channels, more = active && k + 1 < tl.row_tiles;
+            float carry = 0.0f;
+            if (!publishes && k > 0 && !lr_starts(p.sh, tl.codes, (uint64_t)k * LR_TILE)) {
+                const int64_t step = -(int64_t)ch.width;
+                carry = tl.narrow ? lr_lookback<16>(record + step, step, k, active)
+                                  : lr_lookback<8>(record + step, step, k, active);
+            }
+            lr_sync((publishes ? 1 : 5) + b, THREADS - 32 * N);
+            const uint32_t cuts = lr_cuts(sm.cut[b], 1);
+            float A = 1.0f, H = 0.0f, a[LR_WARPS], h[LR_WARPS];
+#pragma unroll
+            for (int w = 0; w < LR_WARPS; ++w) {
+                const float2 v = sm.map[b][w][cc];
+                a[w] = v.x, h[w] = v.y;
+                H = cuts >> w & 1 ? h[w] : fmaf(a[w], H, h[w]);
+                A *= a[w];
+            }
+            if (publishes) {
+                if (more) {
+                    if (cuts || k == 0) lr_put_state(record, H);
+                    else lr_put_map(record, A, H);
+                }
+            } else {
+                if (more && !cuts && k > 0) lr_put_state(record, fmaf(A, carry, H));
+                if (p.saved && active) p.saved[(uint64_t)k * channels + c] = carry;
+#pragma unroll
+                for (int w = 0; w < LR_WARPS; ++w) {
+                    sm.start[b][w][cc] = carry;
+                    carry = cuts >> w & 1 ? h[w] : fmaf(a[w], carry, h[w]);
+                }
+            }
+            lr_arrive(3 + b, THREADS);
+        }
+        return;
+    }
+
+    auto fetch = [&](uint32_t i) {
+        if (i < count) {
+            const uint32_t st = i % Smem::STAGES;
+            const uint2 t = tl.tile(i);
+            const uint64_t first = (uint64_t)t.x * LR_TILE + warp * LR_ROWS;
+            const uint32_t c0 = t.y * C;
+            lr_fetch<T, COPY>(sm.rows[st][warp][0], (const T*)p.gate, p.gate_stride, first, p.sh.rows, c0, channels);
+            lr_fetch<T, COPY>(sm.rows[st][warp][1], (const T*)p.in, p.in_stride, first, p.sh.rows, c0, channels);
+            if (p.sh.offsets && lane < LR_ROWS && first + lane < p.sh.rows)
+                cp_async4(&sm.code[st][warp][lane], tl.codes + first + lane);
         }
         cp_async_commit();
     };
-    // Tiles in the order of their tickets, down the rows: a tile waits only for tiles of smaller tickets, which
-    // CTAs take in ascending order, so the smallest unfinished one never waits.
-    uint64_t cur = blockIdx.x, next = (uint64_t)blockIdx.x + gridDim.x;
-    if (chained) {
-        cur = lr_ticket(ch, &s_ticket);
-        fetch(cur, 0);
-        next = lr_ticket(ch, &s_ticket);
-    } else {
-        fetch(cur, 0);
-    }
-    fetch(next, 1);
-    for (int stage = 0; cur < total; stage ^= 1) {
-        const uint32_t k = (uint32_t)(cur / col_tiles), c0 = (uint32_t)(cur % col_tiles) * C;
-        const uint64_t first = (uint64_t)k * LR_TILE + warp * LR_ROWS;
-        const uint32_t c = c0 + lane * N;
-        const int left = (int)min((uint32_t)N, channels - min(channels, c));
-        const LrMarks m = lr_marks(p.sh, first);
-        cp_async_wait_prior1();
-        __syncthreads();
-        uint32_t taken = 0;
-        if (chained && tid == 0) taken = atomicAdd(ch.ticket, 1u) + 1u;
-        // ---- this warp's rows alone: h_after = A h_before + H ---------------------
-        const char* buf = smem + stage * 2 * LR_BUF + warp * LR_ROWS * LR_ROW_BYTES;
-        const bool plain = m.valid == LR_ALL && m.head == 0;
-        float pre[LR_ROWS][N], loc[LR_ROWS][N], A[N], H[N];  // row r: h = pre h_before + loc
-        auto init = [&](int r, float* h) {  // state before the first row of a sequence
-            const uint64_t s = lr_sequence(p.sh, m, first + r);
+    struct Rows {  // a tile between its two halves: row r is h = pre h_before + loc
+        float pre[LR_ROWS][N], loc[LR_ROWS][N];
+        uint32_t code;
+    };
+    auto init = [&](const LrMarks& m, int r, uint32_t c, float* h) {  // state before a sequence's first row
+        const uint64_t s = m.sequence(p.sh, r);
 #pragma unroll
-            for (int i = 0; i < N; ++i) h[i] = p.init && i < left ? p.init[s * p.init_stride + c + i] : 0.0f;
-        };
+        for (int i = 0; i < N; ++i) h[i] = p.init && c + i < channels ? p.init[s * p.init_stride + c + i] : 0.0f;
+    };
+    auto maps = [&](uint32_t i, Rows& w) {
+        const uint32_t st = i % Smem::STAGES;
+        const uint2 t = tl.tile(i);
+        const uint64_t first = (uint64_t)t.x * LR_TILE + warp * LR_ROWS;
+        const uint32_t c = t.y * C + lane * N;
+        cp_async_wait_prior<Smem::STAGES - 1>();
+        __syncwarp();
+        w.code = lane < LR_ROWS ? lr_code(p.sh, first + lane, &sm.code[st][warp][lane]) : 0;
+        const LrMarks m(w.code);
+        const bool plain = m.valid == LR_ALL && m.head == 0;
+        float A[N], H[N];
 #pragma unroll
         for (int i = 0; i < N; ++i) A[i] = 1.0f, H[i] = 0.0f;
+        auto rows = [&](auto tag) {
+            constexpr bool marked = decltype(tag)::value;
 #pragma unroll
-        for (int r = 0; r < LR_ROWS; ++r) {
-            float g[N], x[N];
-            LrLane<T>::load(buf + r * LR_ROW_BYTES, g);
-            LrLane<T>::load(buf + LR_BUF + r * LR_ROW_BYTES, x);
-            if (!plain) {
-                if (m.head >> r & 1) {
-                    init(r, H);
+            for (int r = 0; r < LR_ROWS; ++r) {
+                float g[N], x[N];
+                LrWord<T>::widen(lr_load(sm.rows[st][warp][0], r), g);
+                LrWord<T>::widen(lr_load(sm.rows[st][warp][1], r), x);
+                if (marked && (m.head >> r & 1)) {
+                    init(m, r, c, H);
 #pragma unroll
                     for (int i = 0; i < N; ++i) A[i] = 0.0f;
                 }
-            }
 #pragma unroll
-            for (int i = 0; i < N; ++i) {
-                const Gate<GATE> gt(g[i]);
-                H[i] = fmaf(gt.a, H[i], gt.add(x[i]));
-                A[i] *= gt.a;
-                if (!plain && !(m.valid >> r & 1)) A[i] = 0.0f, H[i] = 0.0f;
-                pre[r][i] = A[i], loc[r][i] = H[i];
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < N; ++i) s_agg[warp * C + lane * N + i] = make_float2(A[i], H[i]);
-        if (lane == 0) s_reset[warp] = !plain;  // nothing from before the warp's rows passes them
-        if (chained && tid == 0) s_ticket = taken;
-        __syncthreads();
-        const uint64_t after = chained ? s_ticket : next + gridDim.x;
-        // ---- the tile as a whole is published --------------------------------------
-        bool reset = false;
-        float before[N], tA[N], tH[N];  // (A, H) of the warps before this one; of the tile
-        float bA[N];
-        bool breset = false;
-#pragma unroll
-        for (int i = 0; i < N; ++i) tA[i] = 1.0f, tH[i] = 0.0f, bA[i] = 1.0f, before[i] = 0.0f;
-#pragma unroll
-        for (int w = 0; w < LR_WARPS; ++w) {
-            if (w == warp) {
-                breset = reset;
-#pragma unroll
-                for (int i = 0; i < N; ++i) bA[i] = tA[i], before[i] = tH[i];
-            }
-            const bool cuts = s_reset[w];
-            reset |= cuts;
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-                const float2 a = s_agg[w * C + lane * N + i];
-                tH[i] = cuts ? a.y : fmaf(a.x, tH[i], a.y);
-                tA[i] = cuts ? 0.0f : tA[i] * a.x;
-            }
-        }
-        const uint64_t at = (uint64_t)k * ch.width + c;
-        const bool more = k + 1 < row_tiles;
-        if (more && warp == 0) {
-#pragma unroll
-            for (int i = 0; i < N; ++i)
-                if (i < left) {
-                    if (reset) lr_put(ch.state + at + i, tH[i]);
-                    else if (k > 0) lr_put(ch.pair + at + i, make_float2(tA[i], tH[i]));
-                    else lr_put(ch.state + at + i, tH[i]);
+                for (int i = 0; i < N; ++i) {
+                    const Gate<GATE> gt(g[i]);
+                    H[i] = fmaf(gt.a, H[i], gt.add(x[i]));
+                    A[i] *= gt.a;
+                    if (marked && !(m.valid >> r & 1)) A[i] = 0.0f, H[i] = 0.0f;
+                    w.pre[r][i] = A[i], w.loc[r][i] = H[i];
                 }
-        }
-        fetch(after, stage);  // every warp has read this stage
-        // ---- the state before the tile ----------------------------------------------
-        float carry[N];
+            }
+        };
+        if (plain) rows(std::false_type{});
+        else rows(std::true_type{});
+        const int b = i & 1;
 #pragma unroll
-        for (int i = 0; i < N; ++i) carry[i] = 0.0f;
-        if (k > 0) {
-            lr_lookback<N, false>(ch, k, row_tiles, c0, channels, s_win, carry);
-            if (more && warp == 0 && !reset)
+        for (int i = 0; i < N; ++i) sm.map[b][warp][lane * N + i] = make_float2(A[i], H[i]);
+        if (lane == 0) sm.cut[b][warp] = !plain;
+        lr_arrive(1 + b, THREADS - 32 * N);
+        lr_arrive(5 + b, THREADS - 32 * N);
+        __syncwarp();  // the stage is read
+        fetch(i + Smem::STAGES);
+    };
+    auto finish = [&](uint32_t i, const Rows& w) {
+        const int b = i & 1;
+        const uint2 t = tl.tile(i);
+        const uint64_t first = (uint64_t)t.x * LR_TILE + warp * LR_ROWS;
+        const uint32_t c = t.y * C + lane * N;
+        const int left = (int)min((uint32_t)N, channels - min(channels, c));
+        T* out = (T*)p.out + first * p.out_stride + c;
+        const LrMarks m(w.code);
+        float start[N];
+        lr_sync(3 + b, THREADS);
+#pragma unroll
+        for (int i = 0; i < N; ++i) start[i] = sm.start[b][warp][lane * N + i];
+        if (m.valid == LR_ALL && m.head == 0 && m.tail == 0) {
+#pragma unroll
+            for (int r = 0; r < LR_ROWS; ++r, out += p.out_stride) {
+                float h[N];
+#pragma unroll
+                for (int i = 0; i < N; ++i) h[i] = fmaf(w.pre[r][i], start[i], w.loc[r][i]);
+                lr_store<T, COPY>(out, h, left);
+            }
+            return;
+        }
+        // From the first head or outside row on nothing depends on the state before the warp's rows (not even as 0
+        // times it, which an infinity or NaN of another sequence would survive).
+        const int reach = __ffs(m.head | ~m.valid) - 1;
+#pragma unroll
+        for (int r = 0; r < LR_ROWS; ++r) {
+            float h[N];
+#pragma unroll
+            for (int i = 0; i < N; ++i) h[i] = r < reach ? fmaf(w.pre[r][i], start[i], w.loc[r][i]) : w.loc[r][i];
+            if (first + r < p.sh.rows) lr_store<T, COPY>(out + r * p.out_stride, h, left);
+            if ((m.tail >> r & 1) && p.last) {
+                const uint64_t s = m.sequence(p.sh, r);
 #pragma unroll
                 for (int i = 0; i < N; ++i)
-                    if (i < left) lr_put(ch.state + at + i, fmaf(tA[i], carry[i], tH[i]));
-        }
-        if (p.saved && warp == 0)
-#pragma unroll
-            for (int i = 0; i < N; ++i)
-                if (i < left) p.saved[(uint64_t)k * channels + c + i] = carry[i];
-        // ---- outputs -------------------------------------------------------------------
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-            if (!breset) before[i] = fmaf(bA[i], carry[i], before[i]);
-        T* out = (T*)p.out + first * p.out_stride + c;
-        if (plain && m.tail == 0) {
-#pragma unroll
-            for (int r = 0; r < LR_ROWS; ++r) {
-                float h[N];
-#pragma unroll
-                for (int i = 0; i < N; ++i) h[i] = fmaf(pre[r][i], before[i], loc[r][i]);
-                lr_store<T, COPY != LR_COPY_ELEMENT>(out + r * p.out_stride, h, left);
-            }
-        } else {
-            // From the first head or padding row on nothing depends on the state before the warp's rows (not even as
-            // 0 times it, which an infinity or NaN of another sequence would survive).
-            const int reach = __ffs(m.head | ~m.valid) - 1;
-#pragma unroll
-            for (int r = 0; r < LR_ROWS; ++r) {
-                float h[N];
-#pragma unroll
-                for (int i = 0; i < N; ++i) h[i] = r < reach ? fmaf(pre[r][i], before[i], loc[r][i]) : loc[r][i];
-                if (first + r < p.sh.rows) lr_store<T, COPY != LR_COPY_ELEMENT>(out + r * p.out_stride, h, left);
-                if ((m.tail >> r & 1) && p.last) {
-                    const uint64_t s = lr_sequence(p.sh, m, first + r);
-#pragma unroll
-                    for (int i = 0; i < N; ++i)
-                        if (i < left) p.last[s * channels + c + i] = h[i];
-                }
+                    if (i < left) p.last[s * channels + c + i] = h[i];
             }
         }
-        cur = next, next = after;
+    };
+#pragma unroll
+    for (int i = 0; i < Smem::STAGES; ++i) fetch(i);
+    Rows even, odd;
+    if (count > 0) maps(0, even);
+    for (uint32_t i = 0; i < count; i += 2) {
+        if (i + 1 < count) maps(i + 1, odd);
+        finish(i, even);
+        if (i + 2 < count) maps(i + 2, even);
+        if (i + 1 < count) finish(i + 1, odd);
     }
     cp_async_wait_all();
 }
 
-// Before a chained or packed call: the chain's words are LR_NONE, and sequences without rows pass their state
-// on, to[s] = from[s] (0 without from).
-__global__ void __launch_bounds__(256)
-lr_prepare_kernel(uint4* words, uint64_t count, LrShape sh, const float* from, uint64_t from_stride, float* to) {
-    for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < count; i += (uint64_t)gridDim.x * 256)
-        words[i] = make_uint4(LR_NONE, LR_NONE, LR_NONE, LR_NONE);
-    if (!to) return;
-    for (uint64_t s = blockIdx.x; s < sh.sequences; s += gridDim.x) {
-        if (sh.offsets ? min((uint64_t)sh.offsets[s], sh.rows) < min((uint64_t)sh.offsets[s + 1], sh.rows) : sh.length > 0)
-            continue;
-        for (uint64_t c = threadIdx.x; c < sh.channels; c += 256)
-            to[s * sh.channels + c] = from ? from[s * from_stride + c] : 0.0f;
-    }
-}
-
 // ---- Backward --------------------------------------------------------------------
-// Tiles from the last to the first: the chain carries mu, mu_before = A mu_after + M.
-template <typename T, int GATE, int COPY>
-__global__ void __launch_bounds__(LR_THREADS, 2) lr_backward_kernel(LrBackward p, LrChain ch, uint32_t row_tiles, uint32_t col_tiles) {
-    constexpr int N = LrLane<T>::N, C = 32 * N;
-    extern __shared__ __align__(128) char smem[];  // [2 stages][gate, in, grad_out][LR_BUF]
-    __shared__ float2 s_agg[LR_WARPS * C], s_win[LR_WINDOW * C];
-    __shared__ float s_mu[LR_WARPS * C];
-    __shared__ uint32_t s_cut[LR_WARPS], s_ticket;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const uint32_t channels = (uint32_t)p.sh.channels;
-    const uint64_t total = (uint64_t)row_tiles * col_tiles;
-    const bool chained = row_tiles > 1;
+// Tiles from the last to the first: the chain carries mu, mu_before = A mu_behind + M.
+template <typename T>
+struct LrBackwardSmem {
+    static constexpr int STAGES = 3, C = 32 * LrWord<T>::N;
+    char rows[STAGES][LR_WARPS][3][LR_WARP_BUF];  // gate, in, grad_out
+    uint32_t code[STAGES][LR_WARPS][LR_ROWS];
+    float2 map[2][LR_WARPS][C];                   // (A, H) of a warp's rows, and M
+    float grad_map[2][LR_WARPS][C];
+    float start[2][LR_WARPS][C], grad_start[2][LR_WARPS][C];
+    // bit 0: no state from before a warp's rows passes them; bit 1: no gradient from behind them does
+    uint32_t cut[2][LR_WARPS];
+};
 
-    auto fetch = [&](uint64_t t, int stage) {
-        if (t < total) {
-            const uint64_t row0 = (row_tiles - 1 - t / col_tiles) * LR_TILE;
-            const uint32_t c0 = (uint32_t)(t % col_tiles) * C;
-            char* buf = smem + stage * 3 * LR_BUF;
-            lr_fetch<T, COPY>(buf, (const T*)p.gate, p.gate_stride, row0, p.sh.rows, c0, channels);
-            lr_fetch<T, COPY>(buf + LR_BUF, (const T*)p.in, p.in_stride, row0, p.sh.rows, c0, channels);
+template <typename T, int GATE, int COPY>
+__global__ void __launch_bounds__(LR_THREADS<T>, 1) lr_backward_kernel(LrBackward p, LrChain ch, LrTiles tl) {
+    constexpr int N = LrWord<T>::N, C = 32 * N, THREADS = LR_THREADS<T>;
+    using Smem = LrBackwardSmem<T>;
+    extern __shared__ __align__(128) char smem_raw[];
+    Smem& sm = *(Smem*)smem_raw;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const uint32_t channels = (uint32_t)p.sh.channels, count = tl.count();
+    auto row_tile = [&](uint2 t) { return tl.row_tiles - 1 - t.x; };
+
+    if (warp >= LR_WARPS) {
+        const bool publishes = warp >= LR_WARPS + N;
+        const int cc = (warp - LR_WARPS) % N * 32 + lane;
+        for (uint32_t i = 0; i < count; ++i) {
+            const int b = i & 1;
+            const uint2 t = tl.tile(i);
+            const uint32_t k = row_tile(t), c = t.y * C + cc;
+            float4* record = ch.record + (uint64_t)k * ch.width + c;
+            const bool active = c < channels, more = active && k > 0, chained = k + 1 < tl.row_tiles;
+            // the publishing warps also carry the states on, from the saved one
+            float carry = 0.0f, state = publishes && active ? p.saved[(uint64_t)k * channels + c] : 0.0f;
+            if (!publishes && chained && !lr_ends(p.sh, tl.codes, (uint64_t)(k + 1) * LR_TILE - 1)) {
+                const int64_t step = ch.width;
+                carry = tl.narrow ? lr_lookback<16>(record + step, step, t.x, active)
+                                  : lr_lookback<8>(record + step, step, t.x, active);
+            }
+            lr_sync((publishes ? 1 : 5) + b, THREADS - 32 * N);
+            const uint32_t cuts = lr_cuts(sm.cut[b], 2);
+            float A = 1.0f, M = 0.0f, a[LR_WARPS], v[LR_WARPS];
+#pragma unroll
+            for (int w = LR_WARPS - 1; w >= 0; --w) {
+                a[w] = sm.map[b][w][cc].x, v[w] = sm.grad_map[b][w][cc];
+                M = cuts >> w & 1 ? v[w] : fmaf(a[w], M, v[w]);
+                A *= a[w];
+            }
+            if (publishes) {
+                if (more) {
+                    if (cuts || !chained) lr_put_state(record, M);
+                    else lr_put_map(record, A, M);
+                }
+                const uint32_t heads = lr_cuts(sm.cut[b], 1);
+#pragma unroll
+                for (int w = 0; w < LR_WARPS; ++w) {
+                    sm.start[b][w][cc] = state;
+                    const float h = sm.map[b][w][cc].y;
+                    state = heads >> w & 1 ? h : fmaf(a[w], state, h);
+                }
+            } else {
+                if (more && !cuts && chained) lr_put_state(record, fmaf(A, carry, M));
+#pragma unroll
+                for (int w = LR_WARPS - 1; w >= 0; --w) {
+                    sm.grad_start[b][w][cc] = carry;
+                    carry = cuts >> w & 1 ? v[w] : fmaf(a[w], carry, v[w]);
+                }
+            }
+            lr_arrive(3 + b, THREADS);
+        }
+        return;
+    }
+
+    auto fetch = [&](uint32_t i) {
+        if (i < count) {
+            const uint32_t st = i % Smem::STAGES;
+            const uint2 t = tl.tile(i);
+            const uint64_t first = (uint64_t)row_tile(t) * LR_TILE + warp * LR_ROWS;
+            const uint32_t c0 = t.y * C;
+            lr_fetch<T, COPY>(sm.rows[st][warp][0], (const T*)p.gate, p.gate_stride, first, p.sh.rows, c0, channels);
+            lr_fetch<T, COPY>(sm.rows[st][warp][1], (const T*)p.in, p.in_stride, first, p.sh.rows, c0, channels);
             if (p.grad_out)
-                lr_fetch<T, COPY>(buf + 2 * LR_BUF, (const T*)p.grad_out, p.grad_out_stride, row0, p.sh.rows, c0, channels);
+                lr_fetch<T, COPY>(sm.rows[st][warp][2], (const T*)p.grad_out, p.grad_out_stride, first, p.sh.rows, c0,
+                                  channels);
+            if (p.sh.offsets && lane < LR_ROWS && first + lane < p.sh.rows)
+                cp_async4(&sm.code[st][warp][lane], tl.codes + first + lane);
         }
         cp_async_commit();
     };
-    uint64_t cur = blockIdx.x, next = (uint64_t)blockIdx.x + gridDim.x;  // as in the forward kernel
-    if (chained) {
-        cur = lr_ticket(ch, &s_ticket);
-        fetch(cur, 0);
-        next = lr_ticket(ch, &s_ticket);
-    } else {
-        fetch(cur, 0);
-    }
-    fetch(next, 1);
-    for (int stage = 0; cur < total; stage ^= 1) {
-        const uint32_t k = row_tiles - 1 - (uint32_t)(cur / col_tiles), c0 = (uint32_t)(cur % col_tiles) * C;
-        const uint64_t first = (uint64_t)k * LR_TILE + warp * LR_ROWS;
-        const uint32_t c = c0 + lane * N;
-        const int left = (int)min((uint32_t)N, channels - min(channels, c));
-        float start[N];  // state before the tile
+    auto init = [&](const LrMarks& m, int r, uint32_t c, float* h) {  // state before a sequence's first row
+        const uint64_t s = m.sequence(p.sh, r);
 #pragma unroll
-        for (int i = 0; i < N; ++i) start[i] = i < left ? p.saved[(uint64_t)k * channels + c + i] : 0.0f;
-        const LrMarks m = lr_marks(p.sh, first);
-        cp_async_wait_prior1();
-        __syncthreads();
-        uint32_t taken = 0;
-        if (chained && tid == 0) taken = atomicAdd(ch.ticket, 1u) + 1u;
-        const char* buf = smem + stage * 3 * LR_BUF + warp * LR_ROWS * LR_ROW_BYTES;
-        const bool plain = m.valid == LR_ALL && m.head == 0 && m.tail == 0;
-        auto init = [&](int r, float* h) {
-            const uint64_t s = lr_sequence(p.sh, m, first + r);
+        for (int i = 0; i < N; ++i) h[i] = p.init && c + i < channels ? p.init[s * p.init_stride + c + i] : 0.0f;
+    };
+    auto last = [&](const LrMarks& m, int r, uint32_t c, float* mu) {  // gradient behind a sequence's last row
+        const uint64_t s = m.sequence(p.sh, r);
 #pragma unroll
-            for (int i = 0; i < N; ++i) h[i] = p.init && i < left ? p.init[s * p.init_stride + c + i] : 0.0f;
-        };
-        auto last = [&](int r, float* mu) {
-            const uint64_t s = lr_sequence(p.sh, m, first + r);
-#pragma unroll
-            for (int i = 0; i < N; ++i) mu[i] = p.grad_last && i < left ? p.grad_last[s * channels + c + i] : 0.0f;
-        };
-        // ---- this warp's rows alone, in both directions ------------------------------
-        float a[LR_ROWS][N], h[LR_ROWS][N], A[N], H[N], M[N];  // h: b first, the state before the row later
+        for (int i = 0; i < N; ++i) mu[i] = p.grad_last && c + i < channels ? p.grad_last[s * channels + c + i] : 0.0f;
+    };
+    auto marks = [&](uint32_t st, uint64_t first) {
+        return LrMarks(lane < LR_ROWS ? lr_code(p.sh, first + lane, &sm.code[st][warp][lane]) : 0);
+    };
+    auto maps = [&](uint32_t i) {
+        const uint32_t st = i % Smem::STAGES;
+        const uint2 t = tl.tile(i);
+        const uint64_t first = (uint64_t)row_tile(t) * LR_TILE + warp * LR_ROWS;
+        const uint32_t c = t.y * C + lane * N;
+        cp_async_wait_prior<Smem::STAGES - 2>();
+        __syncwarp();
+        const LrMarks m = marks(st, first);
+        const char(*rows)[LR_WARP_BUF] = sm.rows[st][warp];
+        float A[N], H[N], M[N];
 #pragma unroll
         for (int i = 0; i < N; ++i) A[i] = 1.0f, H[i] = 0.0f, M[i] = 0.0f;
+        auto both = [&](auto tag) {
+            constexpr bool marked = decltype(tag)::value;
+            float a[LR_ROWS][N];
 #pragma unroll
-        for (int r = 0; r < LR_ROWS; ++r) {
-            float g[N], x[N];
-            LrLane<T>::load(buf + r * LR_ROW_BYTES, g);
-            LrLane<T>::load(buf + LR_BUF + r * LR_ROW_BYTES, x);
-            if (!plain && (m.head >> r & 1)) init(r, H);
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-                const Gate<GATE> gt(g[i]);
-                a[r][i] = gt.a, h[r][i] = gt.add(x[i]);
-                H[i] = fmaf(a[r][i], H[i], h[r][i]);
-                A[i] *= a[r][i];
-            }
-        }
-        auto grad = [&](int r, float* v) {
-#pragma unroll
-            for (int i = 0; i < N; ++i) v[i] = 0.0f;
-            if (p.grad_out) LrLane<T>::load(buf + 2 * LR_BUF + r * LR_ROW_BYTES, v);
-        };
-#pragma unroll
-        for (int r = LR_ROWS - 1; r >= 0; --r) {
-            float v[N];
-            grad(r, v);
-            if (!plain && (m.tail >> r & 1)) last(r, M);
-#pragma unroll
-            for (int i = 0; i < N; ++i) M[i] = a[r][i] * (v[i] + M[i]);
-            if (!plain && !(m.valid >> r & 1))
-#pragma unroll
-                for (int i = 0; i < N; ++i) M[i] = 0.0f;
-        }
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            s_agg[warp * C + lane * N + i] = make_float2(A[i], H[i]);
-            s_mu[warp * C + lane * N + i] = M[i];
-        }
-        // bit 0: no state from before the warp's rows passes them; bit 1: no gradient from behind them does
-        if (lane == 0) s_cut[warp] = (m.valid != LR_ALL || m.head ? 1u : 0u) | (m.valid != LR_ALL || m.tail ? 2u : 0u);
-        if (chained && tid == 0) s_ticket = taken;
-        __syncthreads();
-        const uint64_t after = chained ? s_ticket : next + gridDim.x;
-        // ---- the state before this warp's rows ------------------------------------------
-#pragma unroll
-        for (int w = 0; w < LR_WARPS - 1; ++w)
-            if (w < warp) {
-                const bool cuts = s_cut[w] & 1u;
+            for (int r = 0; r < LR_ROWS; ++r) {
+                float g[N], x[N];
+                LrWord<T>::widen(lr_load(rows[0], r), g);
+                LrWord<T>::widen(lr_load(rows[1], r), x);
+                if (marked && (m.head >> r & 1)) init(m, r, c, H);
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
-                    const float2 v = s_agg[w * C + lane * N + i];
-                    start[i] = cuts ? v.y : fmaf(v.x, start[i], v.y);
+                    const Gate<GATE> gt(g[i]);
+                    a[r][i] = gt.a;
+                    H[i] = fmaf(gt.a, H[i], gt.add(x[i]));
+                    A[i] *= gt.a;
                 }
             }
-        // ---- the tile's gradient map is published ---------------------------------------
-        bool cut = false, behind_cut = false;
-        float tA[N], tM[N], bA[N], mu[N];  // of the tile; of the warps behind this one
 #pragma unroll
-        for (int i = 0; i < N; ++i) tA[i] = 1.0f, tM[i] = 0.0f, bA[i] = 1.0f, mu[i] = 0.0f;
+            for (int r = LR_ROWS - 1; r >= 0; --r) {
+                float v[N];
+                LrWord<T>::widen(p.grad_out ? lr_load(rows[2], r) : 0, v);
+                if (marked && (m.tail >> r & 1)) last(m, r, c, M);
 #pragma unroll
-        for (int w = LR_WARPS - 1; w >= 0; --w) {
-            if (w == warp) {
-                behind_cut = cut;
-#pragma unroll
-                for (int i = 0; i < N; ++i) bA[i] = tA[i], mu[i] = tM[i];
+                for (int i = 0; i < N; ++i) {
+                    M[i] = a[r][i] * (v[i] + M[i]);
+                    if (marked && !(m.valid >> r & 1)) M[i] = 0.0f;
+                }
             }
-            const bool cuts = s_cut[w] & 2u;
-            cut |= cuts;
+        };
+        if (m.valid == LR_ALL && m.head == 0 && m.tail == 0) both(std::false_type{});
+        else both(std::true_type{});
+        const int b = i & 1;
 #pragma unroll
-            for (int i = 0; i < N; ++i) {
-                const float Aw = s_agg[w * C + lane * N + i].x, Mw = s_mu[w * C + lane * N + i];
-                tM[i] = cuts ? Mw : fmaf(Aw, tM[i], Mw);
-                tA[i] = cuts ? 0.0f : tA[i] * Aw;
-            }
+        for (int i = 0; i < N; ++i) {
+            sm.map[b][warp][lane * N + i] = make_float2(A[i], H[i]);
+            sm.grad_map[b][warp][lane * N + i] = M[i];
         }
-        const uint64_t at = (uint64_t)k * ch.width + c;
-        const bool more = k > 0;
-        if (more && warp == 0) {
+        if (lane == 0)
+            sm.cut[b][warp] = (m.valid != LR_ALL || m.head ? 1u : 0u) | (m.valid != LR_ALL || m.tail ? 2u : 0u);
+        lr_arrive(1 + b, THREADS - 32 * N);
+        lr_arrive(5 + b, THREADS - 32 * N);
+    };
+    auto finish = [&](uint32_t i) {
+        const int b = i & 1;
+        const uint32_t st = i % Smem::STAGES;
+        const uint2 t = tl.tile(i);
+        const uint64_t first = (uint64_t)row_tile(t) * LR_TILE + warp * LR_ROWS;
+        const uint32_t c = t.y * C + lane * N;
+        const int left = (int)min((uint32_t)N, channels - min(channels, c));
+        const LrMarks m = marks(st, first);
+        const char(*rows)[LR_WARP_BUF] = sm.rows[st][warp];
+        lr_sync(3 + b, THREADS);
+        auto both = [&](auto tag) {
+            constexpr bool marked = decltype(tag)::value;
+            float h[N], mu[N], a[LR_ROWS][N], na[LR_ROWS][N], dgate[LR_ROWS][N];  // dgate: of the gate, per unit of lam
 #pragma unroll
             for (int i = 0; i < N; ++i)
-                if (i < left) {
-                    if (cut || k + 1 == row_tiles) lr_put(ch.state + at + i, tM[i]);
-                    else lr_put(ch.pair + at + i, make_float2(tA[i], tM[i]));
+                h[i] = sm.start[b][warp][lane * N + i], mu[i] = sm.grad_start[b][warp][lane * N + i];
+#pragma unroll
+            for (int r = 0; r < LR_ROWS; ++r) {
+                float g[N], x[N];
+                LrWord<T>::widen(lr_load(rows[0], r), g);
+                LrWord<T>::widen(lr_load(rows[1], r), x);
+                if (marked && (m.head >> r & 1)) init(m, r, c, h);
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    const Gate<GATE> gt(g[i]);
+                    a[r][i] = gt.a, na[r][i] = gt.na;
+                    dgate[r][i] = gt.grad_gate(h[i], x[i]);
+                    h[i] = fmaf(gt.a, h[i], gt.add(x[i]));
                 }
-        }
-        // ---- states before each row: while the chain is on its way ----------------------
-#pragma unroll
-        for (int r = 0; r < LR_ROWS; ++r) {
-            if (!plain && (m.head >> r & 1)) init(r, start);
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-                const float b = h[r][i];
-                h[r][i] = start[i];
-                start[i] = fmaf(a[r][i], start[i], b);
             }
-        }
-        if (k + 1 < row_tiles) {
-            float carry[N];
-            lr_lookback<N, true>(ch, k, row_tiles, c0, channels, s_win, carry);
-            if (more && warp == 0 && !cut)
+            T* out_gate = (T*)p.grad_gate + (first + LR_ROWS - 1) * p.grad_gate_stride + c;
+            T* out_in = (T*)p.grad_in + (first + LR_ROWS - 1) * p.grad_in_stride + c;
 #pragma unroll
-                for (int i = 0; i < N; ++i)
-                    if (i < left) lr_put(ch.state + at + i, fmaf(tA[i], carry[i], tM[i]));
-            if (!behind_cut)
+            for (int r = LR_ROWS - 1; r >= 0; --r, out_gate -= p.grad_gate_stride, out_in -= p.grad_in_stride) {
+                float v[N], dg[N], dx[N];
+                LrWord<T>::widen(p.grad_out ? lr_load(rows[2], r) : 0, v);
+                if (marked && (m.tail >> r & 1)) last(m, r, c, mu);
 #pragma unroll
-                for (int i = 0; i < N; ++i) mu[i] = fmaf(bA[i], carry[i], mu[i]);
-        }
-        // ---- gradients ---------------------------------------------------------------------
-        T* out_gate = (T*)p.grad_gate + first * p.grad_gate_stride + c;
-        T* out_in = (T*)p.grad_in + first * p.grad_in_stride + c;
-        constexpr bool WIDE = COPY != LR_COPY_ELEMENT;
-#pragma unroll
-        for (int r = LR_ROWS - 1; r >= 0; --r) {
-            float g[N], x[N], v[N], dg[N], dx[N];
-            LrLane<T>::load(buf + r * LR_ROW_BYTES, g);
-            LrLane<T>::load(buf + LR_BUF + r * LR_ROW_BYTES, x);
-            grad(r, v);
-            if (!plain && (m.tail >> r & 1)) last(r, mu);
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-                const Gate<GATE> gt(g[i]);
-                const float lam = v[i] + mu[i];
-                dg[i] = gt.grad_gate(lam, h[r][i], x[i]);
-                dx[i] = gt.grad_in(lam);
-                mu[i] = a[r][i] * lam;
-            }
-            if (plain) {
-                lr_store<T, WIDE>(out_gate + r * p.grad_gate_stride, dg, left);
-                lr_store<T, WIDE>(out_in + r * p.grad_in_stride, dx, left);
-            } else {
-                if (!(m.valid >> r & 1))
-#pragma unroll
-                    for (int i = 0; i < N; ++i) dg[i] = dx[i] = mu[i] = 0.0f;
-                if (first + r < p.sh.rows) {
-                    lr_store<T, WIDE>(out_gate + r * p.grad_gate_stride, dg, left);
-                    lr_store<T, WIDE>(out_in + r * p.grad_in_stride, dx, left);
+                for (int i = 0; i < N; ++i) {
+                    const float lam = v[i] + mu[i];
+                    dg[i] = lam * dgate[r][i];
+                    dx[i] = GATE == LCPP_GATE_SIGMOID ? na[r][i] * lam : lam;
+                    mu[i] = a[r][i] * lam;
+                    if (marked && !(m.valid >> r & 1)) dg[i] = dx[i] = mu[i] = 0.0f;
                 }
-                if ((m.head >> r & 1) && p.grad_init) {
-                    const uint64_t s = lr_sequence(p.sh, m, first + r);
+                if (!marked || first + r < p.sh.rows) {
+                    lr_store<T, COPY>(out_gate, dg, left);
+                    lr_store<T, COPY>(out_in, dx, left);
+                }
+                if (marked && (m.head >> r & 1) && p.grad_init) {
+                    const uint64_t s = m.sequence(p.sh, r);
 #pragma unroll
                     for (int i = 0; i < N; ++i)
                         if (i < left) p.grad_init[s * channels + c + i] = mu[i];
                 }
             }
-        }
-        __syncthreads();  // the stage is free
-        fetch(after, stage);
-        cur = next, next = after;
+        };
+        if (m.valid == LR_ALL && m.head == 0 && m.tail == 0) both(std::false_type{});
+        else both(std::true_type{});
+        __syncwarp();  // the stage is read
+        fetch(i + Smem::STAGES);
+    };
+#pragma unroll
+    for (int i = 0; i < Smem::STAGES; ++i) fetch(i);
+    if (count > 0) maps(0);
+    for (uint32_t i = 0; i < count; ++i) {
+        if (i + 1 < count) maps(i + 1);
+        finish(i);
     }
     cp_async_wait_all();
+}
+
+// ---- Before a chained or packed call ------------------------------------------------
+// The chain's words become LR_NONE, the rows get their codes (with offsets, a
+// warp a tile), and sequences without rows pass their state on, to[s] = from[s]
+// (0 without from).
+__global__ void __launch_bounds__(128)
+lr_prepare_kernel(uint4* words, uint64_t count, uint32_t* codes, LrShape sh, const float* from, uint64_t from_stride, float* to) {
+    __shared__ uint32_t s_code[4][LR_TILE];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    for (uint64_t i = (uint64_t)blockIdx.x * 128 + threadIdx.x; i < count; i += (uint64_t)gridDim.x * 128)
+        words[i] = make_uint4(LR_NONE, LR_NONE, LR_NONE, LR_NONE);
+    if (sh.offsets) {
+        const uint64_t S = sh.sequences, tiles = (sh.rows + LR_TILE - 1) / LR_TILE;
+        for (uint64_t k = (uint64_t)blockIdx.x * 4 + warp; k < tiles; k += (uint64_t)gridDim.x * 4) {
+            const uint64_t first = k * LR_TILE, end = min(first + LR_TILE, sh.rows);
+            const uint64_t lo = sh.offsets[0], hi = sh.offsets[S];
+            const int64_t base = max(lr_search(sh.offsets, S + 1, first), (int64_t)0);
+            for (int r = lane; r < LR_TILE; r += 32) s_code[warp][r] = first + r >= lo && first + r < hi ? 0 : LR_OUTSIDE;
+            __syncwarp();
+            for (uint64_t i = base;; i += 32) {
+                const uint64_t s = i + lane;
+                uint64_t begin = ~0ull, stop = 0;
+                if (s < S) begin = sh.offsets[s], stop = min((uint64_t)sh.offsets[s + 1], sh.rows);
+                if (begin < stop) {
+                    if (begin >= first && begin < end) atomicOr(&s_code[warp][begin - first], LR_HEAD | (uint32_t)s);
+                    if (stop > first && stop <= end) atomicOr(&s_code[warp][stop - 1 - first], LR_TAIL | (uint32_t)s);
+                }
+                if (__any_sync(0xffffffffu, begin >= end)) break;
+            }
+            __syncwarp();
+            for (int r = lane; r < (int)(end - first); r += 32) codes[first + r] = s_code[warp][r];
+            __syncwarp();
+        }
+    }
+    if (!to) return;
+    for (uint64_t s = blockIdx.x; s < sh.sequences; s += gridDim.x) {
+        if (sh.offsets ? min((uint64_t)sh.offsets[s], sh.rows) < min((uint64_t)sh.offsets[s + 1], sh.rows) : sh.length.d > 0)
+            continue;
+        for (uint64_t c = threadIdx.x; c < sh.channels; c += 128)
+            to[s * sh.channels + c] = from ? from[s * from_stride + c] : 0.0f;
+    }
 }
 
 // One token: row i continues the state of row parents[i] (itself without
@@ -759,8 +828,8 @@ constexpr uint64_t LR_MAX_CHANNELS = 1ull << 20;
 
 static lcpp_status lr_check(int gate, int dtype, const LrShape& sh, const void* gate_in, const void* in) {
     if ((gate != LCPP_GATE_LINEAR && gate != LCPP_GATE_SIGMOID) || !is_float_dtype(dtype)) return LCPP_ERR_INVALID_ARG;
-    if (sh.rows > LR_MAX_ROWS || sh.channels > LR_MAX_CHANNELS || sh.sequences > LR_MAX_ROWS) return LCPP_ERR_INVALID_ARG;
-    if (!sh.offsets && (sh.length > LR_MAX_ROWS || sh.sequences * sh.length != sh.rows)) return LCPP_ERR_INVALID_ARG;
+    if (sh.rows > LR_MAX_ROWS || sh.channels > LR_MAX_CHANNELS || sh.sequences > LR_SEQUENCE) return LCPP_ERR_INVALID_ARG;
+    if (!sh.offsets && sh.sequences * sh.length.d != sh.rows) return LCPP_ERR_INVALID_ARG;
     if (sh.rows && sh.channels && (!gate_in || !in || !sh.sequences)) return LCPP_ERR_INVALID_ARG;
     return LCPP_OK;
 }
@@ -769,16 +838,15 @@ static bool lr_stride_ok(uint64_t stride, uint64_t rows, uint64_t channels) {
     return rows <= 1 || (stride >= channels && stride < (1ull << 31));
 }
 
-// Temp: [ticket | pad to 256][pair: row tiles x width float2][state: row tiles x width float], all LR_NONE at the start.
+// Temp: [row codes u32][records: row tiles x width float4].
 static uint64_t lr_width(uint64_t channels) { return align_up(channels, 64); }
 static size_t lr_chain_bytes(uint64_t rows, uint64_t channels) {
     const uint64_t tiles = ceil_div(rows, LR_TILE);
-    return tiles > 1 ? 256 + tiles * lr_width(channels) * 12 : 0;
+    return tiles > 1 ? tiles * lr_width(channels) * 16 : 0;
 }
+static size_t lr_code_bytes(uint64_t rows) { return align_up(rows * 4, 256); }
 static LrChain lr_chain(void* temp, uint64_t rows, uint64_t channels) {
-    const uint64_t n = ceil_div(rows, LR_TILE) * lr_width(channels);
-    char* t = (char*)temp;
-    return LrChain{(uint32_t*)t, (float2*)(t + 256), (float*)(t + 256 + n * 8), lr_width(channels)};
+    return LrChain{(float4*)((char*)temp + lr_code_bytes(rows)), lr_width(channels)};
 }
 
 // How the rows of these matrices can be copied.
@@ -795,27 +863,38 @@ struct LrCopy {
 static lcpp_status lr_prepare(const LrShape& sh, void* temp, const float* from, uint64_t from_stride, float* to,
                               cudaStream_t s) {
     const uint64_t words = lr_chain_bytes(sh.rows, sh.channels) / 16;
-    if (!sh.offsets && sh.length) to = nullptr;  // no sequence is empty
-    if (!words && !to) return LCPP_OK;
-    const uint64_t grid = max(ceil_div(words, 256 * 4), to ? min(sh.sequences, (uint64_t)1024) : 0);
+    if (!sh.offsets && sh.length.d) to = nullptr;  // no sequence is empty
+    if (!words && !to && !sh.offsets) return LCPP_OK;
+    uint64_t grid = max(ceil_div(words, 128 * 4), to ? min(sh.sequences, (uint64_t)1024) : 1);
+    if (sh.offsets) grid = max(grid, ceil_div(ceil_div(sh.rows, LR_TILE), 4));
     ProfScope prof("lr_prepare", s);
-    lr_prepare_kernel<<<(unsigned)min(grid, (uint64_t)device_info().sms * 8), 256, 0, s>>>((uint4*)temp, words, sh, from,
-                                                                                       from_stride, to);
+    lr_prepare_kernel<<<(unsigned)min(grid, (uint64_t)device_info().sms * 16), 128, 0, s>>>(
+        (uint4*)lr_chain(temp, sh.rows, sh.channels).record, words, (uint32_t*)temp, sh, from, from_stride, to);
     count_launch();
     return check_launch();
 }
 
-template <typename K, typename P>
-static lcpp_status lr_launch(K kernel, const char* name, const P& p, const LrShape& sh, int channels_per_tile,
-                             size_t smem, int ctas_per_sm, void* temp, cudaStream_t s) {
-    const uint64_t row_tiles = ceil_div(sh.rows, LR_TILE), col_tiles = ceil_div(sh.channels, channels_per_tile);
+template <typename T, typename Smem, typename K, typename P>
+static lcpp_status lr_launch(K kernel, const char* name, const P& p, const LrShape& sh, void* temp, cudaStream_t s) {
+    constexpr int N = LrWord<T>::N;
+    const uint64_t row_tiles = ceil_div(sh.rows, LR_TILE), col_tiles = ceil_div(sh.channels, 32 * N);
     if (row_tiles * col_tiles > 0x7fffffffull) return LCPP_ERR_INVALID_ARG;
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+    const uint64_t grid = min(row_tiles * col_tiles, (uint64_t)device_info().sms);
+    const LrTiles tl{(uint32_t)row_tiles, LrDivisor(col_tiles), (const uint32_t*)temp, grid > 6 * col_tiles};
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(Smem)) != cudaSuccess)
         return LCPP_ERR_CUDA;
-    const uint64_t grid = min(row_tiles * col_tiles, (uint64_t)device_info().sms * ctas_per_sm);
+    cudaLaunchAttribute together{};  // tiles wait for one another
+    together.id = cudaLaunchAttributeCooperative;
+    together.val.cooperative = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)grid);
+    cfg.blockDim = dim3(LR_THREADS<T>);
+    cfg.dynamicSmemBytes = sizeof(Smem);
+    cfg.stream = s;
+    cfg.attrs = &together;
+    cfg.numAttrs = row_tiles > 1 ? 1 : 0;
     ProfScope prof(name, s);
-    kernel<<<(unsigned)grid, LR_THREADS, smem, s>>>(p, lr_chain(temp, sh.rows, sh.channels), (uint32_t)row_tiles,
-                                                    (uint32_t)col_tiles);
+    if (cudaLaunchKernelEx(&cfg, kernel, p, lr_chain(temp, sh.rows, sh.channels), tl) != cudaSuccess) return LCPP_ERR_CUDA;
     count_launch();
     return check_launch();
 }
@@ -833,7 +912,7 @@ static lcpp_status lr_dispatch(int gate, int dtype, F&& f) {
 using namespace lcpp;
 
 extern "C" size_t lcpp_linear_recurrence_temp_bytes(uint64_t rows, uint64_t channels) {
-    return max(lr_chain_bytes(rows, channels), (size_t)256);
+    return max(lr_code_bytes(rows) + lr_chain_bytes(rows, channels), (size_t)256);
 }
 
 extern "C" size_t lcpp_linear_recurrence_saved_bytes(uint64_t rows, uint64_t channels) {
@@ -845,7 +924,8 @@ extern "C" lcpp_status lcpp_linear_recurrence_forward(
     uint64_t out_stride, uint64_t rows, uint64_t channels, uint64_t num_sequences, uint64_t length,
     const uint32_t* offsets, const float* init, uint64_t init_stride, float* last, void* saved, void* temp,
     size_t temp_bytes, void* stream) {
-    const LrShape sh{rows, channels, num_sequences, length, offsets};
+    if (!offsets && length > LR_MAX_ROWS) return LCPP_ERR_INVALID_ARG;
+    const LrShape sh{rows, channels, num_sequences, LrDivisor(offsets ? 0 : length), offsets};
     const lcpp_status ok = lr_check(gate, dtype, sh, gate_in, in);
     if (ok != LCPP_OK) return ok;
     if (!channels || !num_sequences) return LCPP_OK;
@@ -859,10 +939,10 @@ extern "C" lcpp_status lcpp_linear_recurrence_forward(
     if (ready != LCPP_OK || !rows) return ready;
     return lr_dispatch(gate, dtype, [&](auto t, auto g) -> lcpp_status {
         using T = decltype(t);
-        constexpr int G = decltype(g)::value, C = 32 * LR_LANE_BYTES / sizeof(T);
+        constexpr int G = decltype(g)::value;
         const int copy = LrCopy(channels, sizeof(T)).add(gate_in, gate_stride, sizeof(T)).add(in, in_stride, sizeof(T))
                              .add(out, out_stride, sizeof(T)).kind();
-        auto launch = [&](auto kernel) { return lr_launch(kernel, "lr_forward", p, sh, C, 4 * LR_BUF, 3, temp, s); };
+        auto launch = [&](auto kernel) { return lr_launch<T, LrForwardSmem<T>>(kernel, "lr_forward", p, sh, temp, s); };
         if (copy == LR_COPY16) return launch(lr_forward_kernel<T, G, LR_COPY16>);
         if (copy == LR_COPY4) return launch(lr_forward_kernel<T, G, LR_COPY4>);
         return launch(lr_forward_kernel<T, G, LR_COPY_ELEMENT>);
@@ -875,7 +955,8 @@ extern "C" lcpp_status lcpp_linear_recurrence_backward(
     const float* grad_last, void* grad_gate, uint64_t grad_gate_stride, void* grad_in, uint64_t grad_in_stride,
     float* grad_init, uint64_t rows, uint64_t channels, uint64_t num_sequences, uint64_t length,
     const uint32_t* offsets, void* temp, size_t temp_bytes, void* stream) {
-    const LrShape sh{rows, channels, num_sequences, length, offsets};
+    if (!offsets && length > LR_MAX_ROWS) return LCPP_ERR_INVALID_ARG;
+    const LrShape sh{rows, channels, num_sequences, LrDivisor(offsets ? 0 : length), offsets};
     const lcpp_status ok = lr_check(gate, dtype, sh, gate_in, in);
     if (ok != LCPP_OK) return ok;
     if (!channels || !num_sequences) return LCPP_OK;
@@ -892,13 +973,13 @@ extern "C" lcpp_status lcpp_linear_recurrence_backward(
     if (ready != LCPP_OK || !rows) return ready;
     return lr_dispatch(gate, dtype, [&](auto t, auto g) -> lcpp_status {
         using T = decltype(t);
-        constexpr int G = decltype(g)::value, C = 32 * LR_LANE_BYTES / sizeof(T);
+        constexpr int G = decltype(g)::value;
         LrCopy align(channels, sizeof(T));
         align.add(gate_in, gate_stride, sizeof(T)).add(in, in_stride, sizeof(T))
             .add(grad_gate, grad_gate_stride, sizeof(T)).add(grad_in, grad_in_stride, sizeof(T));
         if (grad_out) align.add(grad_out, grad_out_stride, sizeof(T));
         const int copy = align.kind();
-        auto launch = [&](auto kernel) { return lr_launch(kernel, "lr_backward", p, sh, C, 6 * LR_BUF, 2, temp, s); };
+        auto launch = [&](auto kernel) { return lr_launch<T, LrBackwardSmem<T>>(kernel, "lr_backward", p, sh, temp, s); };
         if (copy == LR_COPY16) return launch(lr_backward_kernel<T, G, LR_COPY16>);
         if (copy == LR_COPY4) return launch(lr_backward_kernel<T, G, LR_COPY4>);
         return launch(lr_backward_kernel<T, G, LR_COPY_ELEMENT>);
