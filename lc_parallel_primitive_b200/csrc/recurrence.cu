@@ -26,12 +26,17 @@
 
 namespace lcpp {
 
-constexpr int LR_TILE = 128;                    // rows of a tile, and rows between two saved states
-constexpr int LR_WARPS = 16;                    // compute warps
-constexpr int LR_ROWS = LR_TILE / LR_WARPS;     // consecutive rows of one warp
-constexpr uint32_t LR_ALL = (1u << LR_ROWS) - 1;
-constexpr int LR_ROW_BYTES = 128;               // a row of a tile: 4 bytes per lane, 1 float or 2 halves
-constexpr int LR_WARP_BUF = LR_ROWS * LR_ROW_BYTES;  // one warp's rows of one matrix
+constexpr int LR_WARPS = 16;                             // compute warps
+constexpr int LR_LANES = 32;                             // lanes across a row, 4 bytes each: 1 float or 2 halves
+constexpr int LR_GROUPS = 32 / LR_LANES;                 // of a warp, one under the other
+constexpr int LR_ROWS = 8;                               // consecutive rows of a group
+constexpr int LR_WARP_ROWS = LR_ROWS * LR_GROUPS;
+constexpr int LR_TILE = LR_WARPS * LR_WARP_ROWS;         // rows of a tile, and rows between two saved states
+constexpr int LR_ROW_BYTES = LR_LANES * 4;
+// Groups are a row further apart in shared memory than their rows take, so that a load of the whole warp meets all
+// banks once.
+constexpr int LR_GROUP_BUF = LR_ROWS * LR_ROW_BYTES + (LR_GROUPS > 1 ? LR_ROW_BYTES : 0);
+constexpr int LR_WARP_BUF = LR_GROUPS * LR_GROUP_BUF;    // one warp's rows of one matrix
 
 // Division of 32-bit numbers by a fixed one: the high half of n * ceil(2^64 / d) is n / d for all n, d < 2^32
 // (the error n / 2^64 cannot reach the next quotient, 1 / d away).
@@ -104,6 +109,33 @@ struct LrBackward {
 // all sequences have one length, else written by lr_prepare_kernel.
 constexpr uint32_t LR_OUTSIDE = 1u << 31, LR_HEAD = 1u << 30, LR_TAIL = 1u << 29, LR_SEQUENCE = LR_TAIL - 1;
 
+__device__ __forceinline__ uint32_t lr_code(const LrShape& sh, uint64_t row, const uint32_t* fetched) {
+    if (row >= sh.rows) return LR_OUTSIDE;
+    if (sh.offsets) return *fetched;
+    const uint32_t r = (uint32_t)row, s = sh.length.div(r), at = r - s * sh.length.d;
+    return (at == 0 ? LR_HEAD : 0) | (at + 1 == sh.length.d ? LR_TAIL : 0) | s;
+}
+// What one lane needs of them: masks over its group's rows.
+struct LrMarks {
+    uint32_t code, head, tail, valid;
+    __device__ __forceinline__ explicit LrMarks(uint32_t c) : code(c) {
+        const int lane = threadIdx.x & 31, shift = lane / LR_LANES * LR_ROWS;
+        const bool mine = lane < LR_WARP_ROWS;
+        constexpr uint32_t ALL = (1u << LR_ROWS) - 1;
+        head = __ballot_sync(0xffffffffu, mine && (c & LR_HEAD)) >> shift & ALL;
+        tail = __ballot_sync(0xffffffffu, mine && (c & LR_TAIL)) >> shift & ALL;
+        valid = __ballot_sync(0xffffffffu, mine && !(c & LR_OUTSIDE)) >> shift & ALL;
+    }
+    // Sequence of the group's row r, if that is a head or tail (a call of the whole warp).
+    __device__ __forceinline__ uint64_t sequence(const LrShape& sh, int r) const {
+        const uint32_t s = __shfl_sync(0xffffffffu, code, (threadIdx.x & 31) / LR_LANES * LR_ROWS + r) & LR_SEQUENCE;
+        return min((uint64_t)s, sh.sequences - 1);
+    }
+    // Nothing from before the group's rows passes them; nothing from behind them does.
+    __device__ __forceinline__ bool cuts() const { return head || valid != (1u << LR_ROWS) - 1; }
+    __device__ __forceinline__ bool cuts_back() const { return tail || valid != (1u << LR_ROWS) - 1; }
+};
+
 // Number of offsets[0 .. count) that are <= row, minus 1 (-1: none); the warp narrows the range 32-fold a step.
 __device__ __forceinline__ int64_t lr_search(const uint32_t* offsets, uint64_t count, uint64_t row) {
     const int lane = threadIdx.x & 31;
@@ -116,27 +148,6 @@ __device__ __forceinline__ int64_t lr_search(const uint32_t* offsets, uint64_t c
         n = min(step - 1, full * step < n ? n - full * step : 0);
     }
     return (int64_t)lo - 1;
-}
-
-// The codes of a warp's rows, lane r holding row r's, and masks of them.
-struct LrMarks {
-    uint32_t code, head, tail, valid;
-    __device__ __forceinline__ explicit LrMarks(uint32_t c) : code(c) {
-        const bool mine = (threadIdx.x & 31) < LR_ROWS;
-        head = __ballot_sync(0xffffffffu, mine && (c & LR_HEAD));
-        tail = __ballot_sync(0xffffffffu, mine && (c & LR_TAIL));
-        valid = __ballot_sync(0xffffffffu, mine && !(c & LR_OUTSIDE));
-    }
-    // Sequence of row r, which is a head or tail.
-    __device__ __forceinline__ uint64_t sequence(const LrShape& sh, int r) const {
-        return min((uint64_t)(__shfl_sync(0xffffffffu, code, r) & LR_SEQUENCE), sh.sequences - 1);
-    }
-};
-__device__ __forceinline__ uint32_t lr_code(const LrShape& sh, uint64_t row, const uint32_t* fetched) {
-    if (row >= sh.rows) return LR_OUTSIDE;
-    if (sh.offsets) return *fetched;
-    const uint32_t r = (uint32_t)row, s = sh.length.div(r), at = r - s * sh.length.d;
-    return (at == 0 ? LR_HEAD : 0) | (at + 1 == sh.length.d ? LR_TAIL : 0) | s;
 }
 
 // ---- Look-back between the tiles of a column -----------------------------------
@@ -225,43 +236,58 @@ __device__ __forceinline__ void lr_arrive(int barrier, int threads) {
 // by element (2-byte elements on odd addresses or strides).
 enum { LR_COPY16 = 0, LR_COPY4 = 1, LR_COPY_ELEMENT = 2 };
 
-// Copies a warp's rows, first .., of one column tile of a matrix to buf; rows
-// from `rows` on and channels from `channels` on are left as they are.
-// Asynchronous copies are part of the warp's next commit.
+// One lane's part of copying a warp's rows of a column tile: constant offsets.
 template <typename T, int COPY>
-__device__ __forceinline__ void lr_fetch(char* buf, const T* m, uint64_t stride, uint64_t first, uint64_t rows,
-                                         uint32_t channel0, uint32_t channels) {
-    const int lane = threadIdx.x & 31;
-    const int n = (int)min((uint64_t)LR_ROWS, rows - min(rows, first));
-    m += first * stride + channel0;
-    if constexpr (COPY == LR_COPY16) {
-        constexpr int V = 16 / sizeof(T);
-        const int r0 = lane / 8, c = (lane % 8) * V;
-        if (channel0 + c >= channels) return;
-#pragma unroll
-        for (int r = r0; r < LR_ROWS + r0; r += 4)
-            if (r < n) cp_async16(buf + r * LR_ROW_BYTES + lane % 8 * 16, m + r * stride + c);
-    } else if constexpr (COPY == LR_COPY4) {
-        constexpr int V = 4 / sizeof(T);
-        if (channel0 + lane * V >= channels) return;
-#pragma unroll
-        for (int r = 0; r < LR_ROWS; ++r)
-            if (r < n) cp_async4(buf + r * LR_ROW_BYTES + lane * 4, m + r * stride + lane * V);
-    } else {
-        T v[LR_ROWS][2];
-#pragma unroll
-        for (int r = 0; r < LR_ROWS; ++r)
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-                if (r < n && channel0 + i * 32 + lane < channels) v[r][i] = m[r * stride + i * 32 + lane];
-#pragma unroll
-        for (int r = 0; r < LR_ROWS; ++r)
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-                if (r < n && channel0 + i * 32 + lane < channels)
-                    ((T*)(buf + r * LR_ROW_BYTES))[i * 32 + lane] = v[r][i];
+struct LrFetch {
+    static constexpr int PER_ROW = COPY == LR_COPY16 ? LR_ROW_BYTES / 16 : LR_LANES;  // lanes a row
+    static constexpr int STEP = 32 / PER_ROW;                                        // rows a step
+    static constexpr int V = (COPY == LR_COPY16 ? 16 : 4) / sizeof(T);               // elements a lane
+    const char* m;       // this lane's part of the warp's first rows
+    uint64_t row_bytes;
+    __device__ __forceinline__ LrFetch(const void* matrix, uint64_t stride, int warp) {
+        const int lane = threadIdx.x & 31;
+        row_bytes = stride * sizeof(T);
+        m = (const char*)matrix + (warp * LR_WARP_ROWS + lane / PER_ROW) * row_bytes + lane % PER_ROW * V * sizeof(T);
     }
-}
+    static __device__ __forceinline__ char* at(char* buf, int r) {
+        return buf + r / LR_ROWS * LR_GROUP_BUF + r % LR_ROWS * LR_ROW_BYTES;
+    }
+    // Copies the warp's rows (n of them in range) of the tile `offset` bytes into the matrix, `channels` of whose
+    // channels are in range, to buf; what is out of range is left as it is.  Asynchronous copies are part of the
+    // warp's next commit.
+    __device__ __forceinline__ void copy(char* buf, uint64_t offset, int n, uint32_t channels) const {
+        const int lane = threadIdx.x & 31, r0 = lane / PER_ROW;
+        const uint32_t c = lane % PER_ROW * V;
+        const uint64_t step_bytes = row_bytes * STEP;
+        const char* src = m + offset;
+        if constexpr (COPY != LR_COPY_ELEMENT) {
+            char* dst = at(buf, r0) + c * sizeof(T);
+            if (c >= channels) return;
+#pragma unroll
+            for (int j = 0; j < LR_WARP_ROWS / STEP; ++j, src += step_bytes) {
+                // rows r0 + j STEP of one group follow one another; STEP divides LR_ROWS or the reverse
+                char* d = dst + (STEP <= LR_ROWS ? j * STEP / LR_ROWS * LR_GROUP_BUF + j * STEP % LR_ROWS * LR_ROW_BYTES
+                                                 : j * (STEP / LR_ROWS) * LR_GROUP_BUF);
+                if (r0 + j * STEP < n) {
+                    if constexpr (COPY == LR_COPY16) cp_async16(d, src);
+                    else cp_async4(d, src);
+                }
+            }
+        } else {
+            T v[LR_WARP_ROWS / STEP][V];
+#pragma unroll
+            for (int j = 0; j < LR_WARP_ROWS / STEP; ++j, src += step_bytes)
+#pragma unroll
+                for (int i = 0; i < V; ++i)
+                    if (r0 + j * STEP < n && c + i < channels) v[j][i] = ((const T*)src)[i];
+#pragma unroll
+            for (int j = 0; j < LR_WARP_ROWS / STEP; ++j)
+#pragma unroll
+                for (int i = 0; i < V; ++i)
+                    if (r0 + j * STEP < n && c + i < channels) ((T*)at(buf, r0 + j * STEP))[c + i] = v[j][i];
+        }
+    }
+};
 
 // One lane's word of a row: its channels widened, and narrowed again.
 template <typename T> struct LrWord;
@@ -297,9 +323,12 @@ template <> struct LrWord<__nv_bfloat16> {
         return w;
     }
 };
-__device__ __forceinline__ uint32_t lr_load(const char* rows, int r) {
-    return ((const uint32_t*)(rows + r * LR_ROW_BYTES))[threadIdx.x & 31];
+// One lane's words of a matrix in shared memory: row r of its group.
+__device__ __forceinline__ const uint32_t* lr_words(const char* buf) {
+    const int lane = threadIdx.x & 31;
+    return (const uint32_t*)(buf + lane / LR_LANES * LR_GROUP_BUF) + lane % LR_LANES;
 }
+constexpr int LR_ROW_WORDS = LR_ROW_BYTES / 4;
 // Stores one lane's channels, `left` of them in range.
 template <typename T, int COPY>
 __device__ __forceinline__ void lr_store(T* p, const float* v, int left) {
@@ -343,45 +372,95 @@ __device__ __forceinline__ uint32_t lr_cuts(const uint32_t* cut, uint32_t bit) {
     return __ballot_sync(0xffffffffu, lane < LR_WARPS && (cut[lane % LR_WARPS] & bit));
 }
 
+// What the compute warps have to know about a tile, worked out by a publishing warp a few tiles ahead: eight slots,
+// of which tile i's is written before the arrival for the starts of tile i - 6 and read until tile i is finished.
+struct alignas(16) LrSlot {
+    uint64_t offset[5];      // of the tile in each matrix, in bytes
+    uint32_t row, channel;   // its first
+    uint32_t rows, channels; // that are in range
+    uint32_t plain;          // a bit a warp: its rows are all inside a sequence (where all have one length)
+    uint32_t pad;
+};
+constexpr int LR_SLOTS = 8, LR_AHEAD = 6;
+
+template <int M>
+__device__ __forceinline__ void lr_slot(LrSlot& slot, const LrShape& sh, uint64_t row, uint64_t channel, uint32_t columns,
+                                        int element, const uint64_t (&stride)[M]) {
+    const int lane = threadIdx.x & 31;
+    bool plain = false;
+    if (!sh.offsets && lane < LR_WARPS) {
+        const uint64_t first = row + lane * LR_WARP_ROWS;
+        const uint32_t r = (uint32_t)first, at = r - sh.length.div(r) * sh.length.d;
+        plain = at > 0 && at + LR_WARP_ROWS < sh.length.d && first + LR_WARP_ROWS <= sh.rows;
+    }
+    const uint32_t bits = __ballot_sync(0xffffffffu, plain);
+    if (lane == 0) {
+#pragma unroll
+        for (int i = 0; i < M; ++i) slot.offset[i] = (row * stride[i] + channel) * element;
+        slot.row = (uint32_t)row, slot.channel = (uint32_t)channel;
+        slot.rows = (uint32_t)min(sh.rows - row, (uint64_t)LR_TILE);
+        slot.channels = (uint32_t)min(sh.channels - channel, (uint64_t)columns);
+        slot.plain = bits;
+    }
+}
+
 // ---- Forward ---------------------------------------------------------------------
 template <typename T>
-struct LrForwardSmem {
-    static constexpr int STAGES = 4, C = 32 * LrWord<T>::N;
-    char rows[STAGES][LR_WARPS][2][LR_WARP_BUF];  // gate, in
-    uint32_t code[STAGES][LR_WARPS][LR_ROWS];
-    float2 map[2][LR_WARPS][C];  // (A, H) of a warp's rows
-    float start[2][LR_WARPS][C];
-    uint32_t cut[2][LR_WARPS];   // nothing from before a warp's rows passes them
+struct LrConfig {
+    static constexpr int N = LrWord<T>::N;       // channels a lane
+    static constexpr int C = LR_LANES * N;       // channels of a tile
+    static constexpr int HELPERS = (C + 31) / 32;  // publishing warps, and look-back warps
+    static constexpr int THREADS = (LR_WARPS + 2 * HELPERS) * 32;
+    static constexpr int MAPPED = THREADS - 32 * HELPERS;  // of a barrier that the compute warps and one kind share
 };
 
 template <typename T>
-constexpr int LR_THREADS = (LR_WARPS + 2 * LrWord<T>::N) * 32;
+struct LrForwardSmem {
+    static constexpr int STAGES = 4, C = LrConfig<T>::C;
+    char rows[STAGES][LR_WARPS][2][LR_WARP_BUF];  // gate, in
+    uint32_t code[STAGES][LR_WARPS][LR_WARP_ROWS];
+    float2 map[2][LR_WARPS][C];  // (A, H) of a warp's rows
+    float start[2][LR_WARPS][C];
+    uint32_t cut[2][LR_WARPS];   // nothing from before a warp's rows passes them
+    LrSlot slot[LR_SLOTS];
+};
 
 template <typename T, int GATE, int COPY>
-__global__ void __launch_bounds__(LR_THREADS<T>, 1) lr_forward_kernel(LrForward p, LrChain ch, LrTiles tl) {
-    constexpr int N = LrWord<T>::N, C = 32 * N, THREADS = LR_THREADS<T>;
+__global__ void __launch_bounds__(LrConfig<T>::THREADS, 1) lr_forward_kernel(LrForward p, LrChain ch, LrTiles tl) {
+    using Config = LrConfig<T>;
     using Smem = LrForwardSmem<T>;
+    constexpr int N = Config::N, C = Config::C;
     extern __shared__ __align__(128) char smem_raw[];
     Smem& sm = *(Smem*)smem_raw;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31, warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
     const uint32_t channels = (uint32_t)p.sh.channels, count = tl.count();
 
+    const uint64_t strides[3] = {p.gate_stride, p.in_stride, p.out_stride};
+    auto slot = [&](uint32_t i) {
+        if (i >= count) return;
+        const uint2 t = tl.tile(i);
+        lr_slot(sm.slot[i % LR_SLOTS], p.sh, (uint64_t)t.x * LR_TILE, (uint64_t)t.y * C, C, sizeof(T), strides);
+    };
+    if (warp < LR_AHEAD) slot(warp);
+    __syncthreads();
+
     if (warp >= LR_WARPS) {
-        const bool publishes = warp >= LR_WARPS + N;
-        const int cc = (warp - LR_WARPS) % N * 32 + lane;
+        const bool publishes = warp >= LR_WARPS + Config::HELPERS;
+        const int cc = min((warp - LR_WARPS) % Config::HELPERS * 32 + lane, C - 1);  // a channel a lane
+        const bool lanes = (warp - LR_WARPS) % Config::HELPERS * 32 + lane < C;
         for (uint32_t i = 0; i < count; ++i) {
             const int b = i & 1;
             const uint2 t = tl.tile(i);
             const uint32_t k = t.x, c = t.y * C + cc;
             float4* record = ch.record + (uint64_t)k * ch.width + c;
-            const bool active = c < channels, more = active && k + 1 < tl.row_tiles;
+            const bool active = lanes && c < channels, more = active && k + 1 < tl.row_tiles;
             float carry = 0.0f;
             if (!publishes && k > 0 && !lr_starts(p.sh, tl.codes, (uint64_t)k * LR_TILE)) {
                 const int64_t step = -(int64_t)ch.width;
                 carry = tl.narrow ? lr_lookback<16>(record + step, step, k, active)
                                   : lr_lookback<8>(record + step, step, k, active);
             }
-            lr_sync((publishes ? 1 : 5) + b, THREADS - 32 * N);
+            lr_sync((publishes ? 1 : 5) + b, Config::MAPPED);
             const uint32_t cuts = lr_cuts(sm.cut[b], 1);
             float A = 1.0f, H = 0.0f, a[LR_WARPS], h[LR_WARPS];
 #pragma unroll
@@ -396,101 +475,144 @@ __global__ void __launch_bounds__(LR_THREADS<T>, 1) lr_forward_kernel(LrForward 
                     if (cuts || k == 0) lr_put_state(record, H);
                     else lr_put_map(record, A, H);
                 }
+                if (warp == LR_WARPS + Config::HELPERS) slot(i + LR_AHEAD);
             } else {
                 if (more && !cuts && k > 0) lr_put_state(record, fmaf(A, carry, H));
                 if (p.saved && active) p.saved[(uint64_t)k * channels + c] = carry;
+                if (lanes) {
 #pragma unroll
-                for (int w = 0; w < LR_WARPS; ++w) {
-                    sm.start[b][w][cc] = carry;
-                    carry = cuts >> w & 1 ? h[w] : fmaf(a[w], carry, h[w]);
+                    for (int w = 0; w < LR_WARPS; ++w) {
+                        sm.start[b][w][cc] = carry;
+                        carry = cuts >> w & 1 ? h[w] : fmaf(a[w], carry, h[w]);
+                    }
                 }
             }
-            lr_arrive(3 + b, THREADS);
+            lr_arrive(3 + b, Config::THREADS);
         }
         return;
     }
 
+    const int group = lane / LR_LANES, column = lane % LR_LANES * N;
+    const LrFetch<T, COPY> fetch_gate(p.gate, p.gate_stride, warp), fetch_in(p.in, p.in_stride, warp);
+    T* const out0 = (T*)p.out + (uint64_t)(warp * LR_WARP_ROWS + group * LR_ROWS) * p.out_stride + column;
     auto fetch = [&](uint32_t i) {
         if (i < count) {
             const uint32_t st = i % Smem::STAGES;
-            const uint2 t = tl.tile(i);
-            const uint64_t first = (uint64_t)t.x * LR_TILE + warp * LR_ROWS;
-            const uint32_t c0 = t.y * C;
-            lr_fetch<T, COPY>(sm.rows[st][warp][0], (const T*)p.gate, p.gate_stride, first, p.sh.rows, c0, channels);
-            lr_fetch<T, COPY>(sm.rows[st][warp][1], (const T*)p.in, p.in_stride, first, p.sh.rows, c0, channels);
-            if (p.sh.offsets && lane < LR_ROWS && first + lane < p.sh.rows)
-                cp_async4(&sm.code[st][warp][lane], tl.codes + first + lane);
+            const LrSlot& sl = sm.slot[i % LR_SLOTS];
+            const int n = (int)sl.rows - warp * LR_WARP_ROWS;
+            fetch_gate.copy(sm.rows[st][warp][0], sl.offset[0], n, sl.channels);
+            fetch_in.copy(sm.rows[st][warp][1], sl.offset[1], n, sl.channels);
+            if (p.sh.offsets && lane < min(n, LR_WARP_ROWS))
+                cp_async4(&sm.code[st][warp][lane], tl.codes + sl.row + warp * LR_WARP_ROWS + lane);
         }
         cp_async_commit();
+    };
+    // Whether a warp's rows are all inside a sequence, and their codes if not.
+    auto codes = [&](const LrSlot& sl, uint32_t st, bool* plain) -> uint32_t {
+        *plain = sl.plain >> warp & 1;
+        if (*plain) return 0;
+        const uint32_t code = lane < LR_WARP_ROWS ? lr_code(p.sh, (uint64_t)sl.row + warp * LR_WARP_ROWS + lane,
+                                                            &sm.code[st][warp][lane]) : 0;
+        *plain = !__any_sync(0xffffffffu, code & (LR_OUTSIDE | LR_HEAD | LR_TAIL));
+        return code;
     };
     struct Rows {  // a tile between its two halves: row r is h = pre h_before + loc
         float pre[LR_ROWS][N], loc[LR_ROWS][N];
         uint32_t code;
-    };
-    auto init = [&](const LrMarks& m, int r, uint32_t c, float* h) {  // state before a sequence's first row
-        const uint64_t s = m.sequence(p.sh, r);
-#pragma unroll
-        for (int i = 0; i < N; ++i) h[i] = p.init && c + i < channels ? p.init[s * p.init_stride + c + i] : 0.0f;
+        bool plain;
     };
     auto maps = [&](uint32_t i, Rows& w) {
         const uint32_t st = i % Smem::STAGES;
-        const uint2 t = tl.tile(i);
-        const uint64_t first = (uint64_t)t.x * LR_TILE + warp * LR_ROWS;
-        const uint32_t c = t.y * C + lane * N;
+        const LrSlot& sl = sm.slot[i % LR_SLOTS];
         cp_async_wait_prior<Smem::STAGES - 1>();
         __syncwarp();
-        w.code = lane < LR_ROWS ? lr_code(p.sh, first + lane, &sm.code[st][warp][lane]) : 0;
-        const LrMarks m(w.code);
-        const bool plain = m.valid == LR_ALL && m.head == 0;
+        w.code = codes(sl, st, &w.plain);
+        const uint32_t *gate = lr_words(sm.rows[st][warp][0]), *in = lr_words(sm.rows[st][warp][1]);
         float A[N], H[N];
 #pragma unroll
         for (int i = 0; i < N; ++i) A[i] = 1.0f, H[i] = 0.0f;
-        auto rows = [&](auto tag) {
-            constexpr bool marked = decltype(tag)::value;
+        bool cuts = false;
+        if (w.plain) {
 #pragma unroll
             for (int r = 0; r < LR_ROWS; ++r) {
                 float g[N], x[N];
-                LrWord<T>::widen(lr_load(sm.rows[st][warp][0], r), g);
-                LrWord<T>::widen(lr_load(sm.rows[st][warp][1], r), x);
-                if (marked && (m.head >> r & 1)) {
-                    init(m, r, c, H);
-#pragma unroll
-                    for (int i = 0; i < N; ++i) A[i] = 0.0f;
-                }
+                LrWord<T>::widen(gate[r * LR_ROW_WORDS], g);
+                LrWord<T>::widen(in[r * LR_ROW_WORDS], x);
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
                     const Gate<GATE> gt(g[i]);
                     H[i] = fmaf(gt.a, H[i], gt.add(x[i]));
                     A[i] *= gt.a;
-                    if (marked && !(m.valid >> r & 1)) A[i] = 0.0f, H[i] = 0.0f;
                     w.pre[r][i] = A[i], w.loc[r][i] = H[i];
                 }
             }
-        };
-        if (plain) rows(std::false_type{});
-        else rows(std::true_type{});
-        const int b = i & 1;
+        } else {
+            const LrMarks m(w.code);
+            const uint32_t c = sl.channel + column;
+            cuts = m.cuts();
 #pragma unroll
-        for (int i = 0; i < N; ++i) sm.map[b][warp][lane * N + i] = make_float2(A[i], H[i]);
-        if (lane == 0) sm.cut[b][warp] = !plain;
-        lr_arrive(1 + b, THREADS - 32 * N);
-        lr_arrive(5 + b, THREADS - 32 * N);
+            for (int r = 0; r < LR_ROWS; ++r) {
+                float g[N], x[N];
+                LrWord<T>::widen(gate[r * LR_ROW_WORDS], g);
+                LrWord<T>::widen(in[r * LR_ROW_WORDS], x);
+                const uint64_t s = m.sequence(p.sh, r);
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    if (m.head >> r & 1) {
+                        A[i] = 0.0f;
+                        H[i] = p.init && c + i < channels ? p.init[s * p.init_stride + c + i] : 0.0f;
+                    }
+                    const Gate<GATE> gt(g[i]);
+                    H[i] = fmaf(gt.a, H[i], gt.add(x[i]));
+                    A[i] *= gt.a;
+                    if (!(m.valid >> r & 1)) A[i] = 0.0f, H[i] = 0.0f;
+                    w.pre[r][i] = A[i], w.loc[r][i] = H[i];
+                }
+            }
+        }
+        // the groups' maps one after the other are the warp's
+        const int b = i & 1;
+        bool any = cuts;
+#pragma unroll
+        for (int s = 1; s < LR_GROUPS; ++s) {
+            const bool cut = __shfl_down_sync(0xffffffffu, cuts, s * LR_LANES);
+            any |= cut;
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const float a = __shfl_down_sync(0xffffffffu, w.pre[LR_ROWS - 1][i], s * LR_LANES);
+                const float h = __shfl_down_sync(0xffffffffu, w.loc[LR_ROWS - 1][i], s * LR_LANES);
+                H[i] = cut ? h : fmaf(a, H[i], h);
+                A[i] *= a;
+            }
+        }
+        if (group == 0) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) sm.map[b][warp][column + i] = make_float2(A[i], H[i]);
+            if (lane == 0) sm.cut[b][warp] = any;
+        }
+        lr_arrive(1 + b, Config::MAPPED);
+        lr_arrive(5 + b, Config::MAPPED);
         __syncwarp();  // the stage is read
         fetch(i + Smem::STAGES);
     };
     auto finish = [&](uint32_t i, const Rows& w) {
         const int b = i & 1;
-        const uint2 t = tl.tile(i);
-        const uint64_t first = (uint64_t)t.x * LR_TILE + warp * LR_ROWS;
-        const uint32_t c = t.y * C + lane * N;
-        const int left = (int)min((uint32_t)N, channels - min(channels, c));
-        T* out = (T*)p.out + first * p.out_stride + c;
-        const LrMarks m(w.code);
+        const LrSlot& sl = sm.slot[i % LR_SLOTS];
+        const int left = (int)sl.channels - column;
+        T* out = (T*)((char*)out0 + sl.offset[2]);
         float start[N];
-        lr_sync(3 + b, THREADS);
+        lr_sync(3 + b, Config::THREADS);
 #pragma unroll
-        for (int i = 0; i < N; ++i) start[i] = sm.start[b][warp][lane * N + i];
-        if (m.valid == LR_ALL && m.head == 0 && m.tail == 0) {
+        for (int i = 0; i < N; ++i) start[i] = sm.start[b][warp][column + i];
+        if (w.plain) {
+#pragma unroll
+            for (int s = 1; s < LR_GROUPS; ++s)
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    const float behind = fmaf(w.pre[LR_ROWS - 1][i], start[i], w.loc[LR_ROWS - 1][i]);
+                    const float up = __shfl_up_sync(0xffffffffu, behind, LR_LANES);
+                    if (group == s) start[i] = up;
+                }
 #pragma unroll
             for (int r = 0; r < LR_ROWS; ++r, out += p.out_stride) {
                 float h[N];
@@ -500,17 +622,29 @@ __global__ void __launch_bounds__(LR_THREADS<T>, 1) lr_forward_kernel(LrForward 
             }
             return;
         }
-        // From the first head or outside row on nothing depends on the state before the warp's rows (not even as 0
+        // From the first head or outside row on nothing depends on the state before the group's rows (not even as 0
         // times it, which an infinity or NaN of another sequence would survive).
+        const LrMarks m(w.code);
+        const uint32_t c = sl.channel + column;
+        const int rows = (int)sl.rows - warp * LR_WARP_ROWS - group * LR_ROWS;
         const int reach = __ffs(m.head | ~m.valid) - 1;
 #pragma unroll
-        for (int r = 0; r < LR_ROWS; ++r) {
+        for (int s = 1; s < LR_GROUPS; ++s)
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const float loc = w.loc[LR_ROWS - 1][i];
+                const float behind = reach < LR_ROWS ? loc : fmaf(w.pre[LR_ROWS - 1][i], start[i], loc);
+                const float up = __shfl_up_sync(0xffffffffu, behind, LR_LANES);
+                if (group == s) start[i] = up;
+            }
+#pragma unroll
+        for (int r = 0; r < LR_ROWS; ++r, out += p.out_stride) {
             float h[N];
 #pragma unroll
             for (int i = 0; i < N; ++i) h[i] = r < reach ? fmaf(w.pre[r][i], start[i], w.loc[r][i]) : w.loc[r][i];
-            if (first + r < p.sh.rows) lr_store<T, COPY>(out + r * p.out_stride, h, left);
+            if (r < rows) lr_store<T, COPY>(out, h, left);
+            const uint64_t s = m.sequence(p.sh, r);
             if ((m.tail >> r & 1) && p.last) {
-                const uint64_t s = m.sequence(p.sh, r);
 #pragma unroll
                 for (int i = 0; i < N; ++i)
                     if (i < left) p.last[s * channels + c + i] = h[i];
@@ -534,35 +668,48 @@ __global__ void __launch_bounds__(LR_THREADS<T>, 1) lr_forward_kernel(LrForward 
 // Tiles from the last to the first: the chain carries mu, mu_before = A mu_behind + M.
 template <typename T>
 struct LrBackwardSmem {
-    static constexpr int STAGES = 3, C = 32 * LrWord<T>::N;
+    static constexpr int STAGES = 3, C = LrConfig<T>::C, N = LrConfig<T>::N;
     char rows[STAGES][LR_WARPS][3][LR_WARP_BUF];  // gate, in, grad_out
-    uint32_t code[STAGES][LR_WARPS][LR_ROWS];
+    uint32_t code[STAGES][LR_WARPS][LR_WARP_ROWS];
     float2 map[2][LR_WARPS][C];                   // (A, H) of a warp's rows, and M
     float grad_map[2][LR_WARPS][C];
     float start[2][LR_WARPS][C], grad_start[2][LR_WARPS][C];
+    float group[2][LR_WARPS][3 * N][32];          // (A, H, M) of a group's rows, a lane's own
     // bit 0: no state from before a warp's rows passes them; bit 1: no gradient from behind them does
     uint32_t cut[2][LR_WARPS];
+    LrSlot slot[LR_SLOTS];
 };
 
 template <typename T, int GATE, int COPY>
-__global__ void __launch_bounds__(LR_THREADS<T>, 1) lr_backward_kernel(LrBackward p, LrChain ch, LrTiles tl) {
-    constexpr int N = LrWord<T>::N, C = 32 * N, THREADS = LR_THREADS<T>;
+__global__ void __launch_bounds__(LrConfig<T>::THREADS, 1) lr_backward_kernel(LrBackward p, LrChain ch, LrTiles tl) {
+    using Config = LrConfig<T>;
     using Smem = LrBackwardSmem<T>;
+    constexpr int N = Config::N, C = Config::C;
     extern __shared__ __align__(128) char smem_raw[];
     Smem& sm = *(Smem*)smem_raw;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31, warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
     const uint32_t channels = (uint32_t)p.sh.channels, count = tl.count();
     auto row_tile = [&](uint2 t) { return tl.row_tiles - 1 - t.x; };
 
+    const uint64_t strides[5] = {p.gate_stride, p.in_stride, p.grad_out_stride, p.grad_gate_stride, p.grad_in_stride};
+    auto slot = [&](uint32_t i) {
+        if (i >= count) return;
+        const uint2 t = tl.tile(i);
+        lr_slot(sm.slot[i % LR_SLOTS], p.sh, (uint64_t)row_tile(t) * LR_TILE, (uint64_t)t.y * C, C, sizeof(T), strides);
+    };
+    if (warp < LR_AHEAD) slot(warp);
+    __syncthreads();
+
     if (warp >= LR_WARPS) {
-        const bool publishes = warp >= LR_WARPS + N;
-        const int cc = (warp - LR_WARPS) % N * 32 + lane;
+        const bool publishes = warp >= LR_WARPS + Config::HELPERS;
+        const int cc = min((warp - LR_WARPS) % Config::HELPERS * 32 + lane, C - 1);  // a channel a lane
+        const bool lanes = (warp - LR_WARPS) % Config::HELPERS * 32 + lane < C;
         for (uint32_t i = 0; i < count; ++i) {
             const int b = i & 1;
             const uint2 t = tl.tile(i);
             const uint32_t k = row_tile(t), c = t.y * C + cc;
             float4* record = ch.record + (uint64_t)k * ch.width + c;
-            const bool active = c < channels, more = active && k > 0, chained = k + 1 < tl.row_tiles;
+            const bool active = lanes && c < channels, more = active && k > 0, chained = k + 1 < tl.row_tiles;
             // the publishing warps also carry the states on, from the saved one
             float carry = 0.0f, state = publishes && active ? p.saved[(uint64_t)k * channels + c] : 0.0f;
             if (!publishes && chained && !lr_ends(p.sh, tl.codes, (uint64_t)(k + 1) * LR_TILE - 1)) {
@@ -570,7 +717,7 @@ __global__ void __launch_bounds__(LR_THREADS<T>, 1) lr_backward_kernel(LrBackwar
                 carry = tl.narrow ? lr_lookback<16>(record + step, step, t.x, active)
                                   : lr_lookback<8>(record + step, step, t.x, active);
             }
-            lr_sync((publishes ? 1 : 5) + b, THREADS - 32 * N);
+            lr_sync((publishes ? 1 : 5) + b, Config::MAPPED);
             const uint32_t cuts = lr_cuts(sm.cut[b], 2);
             float A = 1.0f, M = 0.0f, a[LR_WARPS], v[LR_WARPS];
 #pragma unroll
@@ -584,76 +731,84 @@ __global__ void __launch_bounds__(LR_THREADS<T>, 1) lr_backward_kernel(LrBackwar
                     if (cuts || !chained) lr_put_state(record, M);
                     else lr_put_map(record, A, M);
                 }
+                if (warp == LR_WARPS + Config::HELPERS) slot(i + LR_AHEAD);
                 const uint32_t heads = lr_cuts(sm.cut[b], 1);
+                if (lanes) {
 #pragma unroll
-                for (int w = 0; w < LR_WARPS; ++w) {
-                    sm.start[b][w][cc] = state;
-                    const float h = sm.map[b][w][cc].y;
-                    state = heads >> w & 1 ? h : fmaf(a[w], state, h);
+                    for (int w = 0; w < LR_WARPS; ++w) {
+                        sm.start[b][w][cc] = state;
+                        const float h = sm.map[b][w][cc].y;
+                        state = heads >> w & 1 ? h : fmaf(a[w], state, h);
+                    }
                 }
             } else {
                 if (more && !cuts && chained) lr_put_state(record, fmaf(A, carry, M));
+                if (lanes) {
 #pragma unroll
-                for (int w = LR_WARPS - 1; w >= 0; --w) {
-                    sm.grad_start[b][w][cc] = carry;
-                    carry = cuts >> w & 1 ? v[w] : fmaf(a[w], carry, v[w]);
+                    for (int w = LR_WARPS - 1; w >= 0; --w) {
+                        sm.grad_start[b][w][cc] = carry;
+                        carry = cuts >> w & 1 ? v[w] : fmaf(a[w], carry, v[w]);
+                    }
                 }
             }
-            lr_arrive(3 + b, THREADS);
+            lr_arrive(3 + b, Config::THREADS);
         }
         return;
     }
 
+    const int group = lane / LR_LANES, column = lane % LR_LANES * N;
+    const LrFetch<T, COPY> fetch_gate(p.gate, p.gate_stride, warp), fetch_in(p.in, p.in_stride, warp),
+        fetch_grad(p.grad_out, p.grad_out_stride, warp);
+    const uint64_t bottom = warp * LR_WARP_ROWS + group * LR_ROWS + LR_ROWS - 1;  // the group's last row
+    T* const out_gate0 = (T*)p.grad_gate + bottom * p.grad_gate_stride + column;
+    T* const out_in0 = (T*)p.grad_in + bottom * p.grad_in_stride + column;
     auto fetch = [&](uint32_t i) {
         if (i < count) {
             const uint32_t st = i % Smem::STAGES;
-            const uint2 t = tl.tile(i);
-            const uint64_t first = (uint64_t)row_tile(t) * LR_TILE + warp * LR_ROWS;
-            const uint32_t c0 = t.y * C;
-            lr_fetch<T, COPY>(sm.rows[st][warp][0], (const T*)p.gate, p.gate_stride, first, p.sh.rows, c0, channels);
-            lr_fetch<T, COPY>(sm.rows[st][warp][1], (const T*)p.in, p.in_stride, first, p.sh.rows, c0, channels);
-            if (p.grad_out)
-                lr_fetch<T, COPY>(sm.rows[st][warp][2], (const T*)p.grad_out, p.grad_out_stride, first, p.sh.rows, c0,
-                                  channels);
-            if (p.sh.offsets && lane < LR_ROWS && first + lane < p.sh.rows)
-                cp_async4(&sm.code[st][warp][lane], tl.codes + first + lane);
+            const LrSlot& sl = sm.slot[i % LR_SLOTS];
+            const int n = (int)sl.rows - warp * LR_WARP_ROWS;
+            fetch_gate.copy(sm.rows[st][warp][0], sl.offset[0], n, sl.channels);
+            fetch_in.copy(sm.rows[st][warp][1], sl.offset[1], n, sl.channels);
+            if (p.grad_out) fetch_grad.copy(sm.rows[st][warp][2], sl.offset[2], n, sl.channels);
+            if (p.sh.offsets && lane < min(n, LR_WARP_ROWS))
+                cp_async4(&sm.code[st][warp][lane], tl.codes + sl.row + warp * LR_WARP_ROWS + lane);
         }
         cp_async_commit();
     };
-    auto init = [&](const LrMarks& m, int r, uint32_t c, float* h) {  // state before a sequence's first row
-        const uint64_t s = m.sequence(p.sh, r);
-#pragma unroll
-        for (int i = 0; i < N; ++i) h[i] = p.init && c + i < channels ? p.init[s * p.init_stride + c + i] : 0.0f;
+    // Whether a warp's rows are all inside a sequence, and their codes if not.
+    auto codes = [&](const LrSlot& sl, uint32_t st, bool* plain) -> uint32_t {
+        *plain = sl.plain >> warp & 1;
+        if (*plain) return 0;
+        const uint32_t code = lane < LR_WARP_ROWS ? lr_code(p.sh, (uint64_t)sl.row + warp * LR_WARP_ROWS + lane,
+                                                            &sm.code[st][warp][lane]) : 0;
+        *plain = !__any_sync(0xffffffffu, code & (LR_OUTSIDE | LR_HEAD | LR_TAIL));
+        return code;
     };
-    auto last = [&](const LrMarks& m, int r, uint32_t c, float* mu) {  // gradient behind a sequence's last row
-        const uint64_t s = m.sequence(p.sh, r);
-#pragma unroll
-        for (int i = 0; i < N; ++i) mu[i] = p.grad_last && c + i < channels ? p.grad_last[s * channels + c + i] : 0.0f;
-    };
-    auto marks = [&](uint32_t st, uint64_t first) {
-        return LrMarks(lane < LR_ROWS ? lr_code(p.sh, first + lane, &sm.code[st][warp][lane]) : 0);
-    };
+    if (!p.grad_out) {  // zeros that stay
+        for (int st = 0; st < Smem::STAGES; ++st)
+            for (int j = lane; j < LR_WARP_BUF / 4; j += 32) ((uint32_t*)sm.rows[st][warp][2])[j] = 0;
+        __syncwarp();
+    }
     auto maps = [&](uint32_t i) {
         const uint32_t st = i % Smem::STAGES;
-        const uint2 t = tl.tile(i);
-        const uint64_t first = (uint64_t)row_tile(t) * LR_TILE + warp * LR_ROWS;
-        const uint32_t c = t.y * C + lane * N;
+        const LrSlot& sl = sm.slot[i % LR_SLOTS];
         cp_async_wait_prior<Smem::STAGES - 2>();
         __syncwarp();
-        const LrMarks m = marks(st, first);
-        const char(*rows)[LR_WARP_BUF] = sm.rows[st][warp];
+        bool plain;
+        const uint32_t code = codes(sl, st, &plain);
+        const uint32_t *gate = lr_words(sm.rows[st][warp][0]), *in = lr_words(sm.rows[st][warp][1]),
+                       *grad = lr_words(sm.rows[st][warp][2]);
         float A[N], H[N], M[N];
 #pragma unroll
         for (int i = 0; i < N; ++i) A[i] = 1.0f, H[i] = 0.0f, M[i] = 0.0f;
-        auto both = [&](auto tag) {
-            constexpr bool marked = decltype(tag)::value;
+        bool cuts = false, cuts_back = false;
+        if (plain) {
             float a[LR_ROWS][N];
 #pragma unroll
             for (int r = 0; r < LR_ROWS; ++r) {
                 float g[N], x[N];
-                LrWord<T>::widen(lr_load(rows[0], r), g);
-                LrWord<T>::widen(lr_load(rows[1], r), x);
-                if (marked && (m.head >> r & 1)) init(m, r, c, H);
+                LrWord<T>::widen(gate[r * LR_ROW_WORDS], g);
+                LrWord<T>::widen(in[r * LR_ROW_WORDS], x);
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
                     const Gate<GATE> gt(g[i]);
@@ -665,50 +820,131 @@ __global__ void __launch_bounds__(LR_THREADS<T>, 1) lr_backward_kernel(LrBackwar
 #pragma unroll
             for (int r = LR_ROWS - 1; r >= 0; --r) {
                 float v[N];
-                LrWord<T>::widen(p.grad_out ? lr_load(rows[2], r) : 0, v);
-                if (marked && (m.tail >> r & 1)) last(m, r, c, M);
+                LrWord<T>::widen(grad[r * LR_ROW_WORDS], v);
+#pragma unroll
+                for (int i = 0; i < N; ++i) M[i] = a[r][i] * (v[i] + M[i]);
+            }
+        } else {
+            const LrMarks m(code);
+            const uint32_t c = sl.channel + column;
+            cuts = m.cuts(), cuts_back = m.cuts_back();
+            float a[LR_ROWS][N];
+#pragma unroll
+            for (int r = 0; r < LR_ROWS; ++r) {
+                float g[N], x[N];
+                LrWord<T>::widen(gate[r * LR_ROW_WORDS], g);
+                LrWord<T>::widen(in[r * LR_ROW_WORDS], x);
+                const uint64_t s = m.sequence(p.sh, r);
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
-                    M[i] = a[r][i] * (v[i] + M[i]);
-                    if (marked && !(m.valid >> r & 1)) M[i] = 0.0f;
+                    if (m.head >> r & 1) H[i] = p.init && c + i < channels ? p.init[s * p.init_stride + c + i] : 0.0f;
+                    const Gate<GATE> gt(g[i]);
+                    a[r][i] = gt.a;
+                    H[i] = fmaf(gt.a, H[i], gt.add(x[i]));
+                    A[i] *= gt.a;
                 }
             }
-        };
-        if (m.valid == LR_ALL && m.head == 0 && m.tail == 0) both(std::false_type{});
-        else both(std::true_type{});
-        const int b = i & 1;
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            sm.map[b][warp][lane * N + i] = make_float2(A[i], H[i]);
-            sm.grad_map[b][warp][lane * N + i] = M[i];
+            for (int r = LR_ROWS - 1; r >= 0; --r) {
+                float v[N];
+                LrWord<T>::widen(grad[r * LR_ROW_WORDS], v);
+                const uint64_t s = m.sequence(p.sh, r);
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    if (m.tail >> r & 1) M[i] = p.grad_last && c + i < channels ? p.grad_last[s * channels + c + i] : 0.0f;
+                    M[i] = m.valid >> r & 1 ? a[r][i] * (v[i] + M[i]) : 0.0f;
+                }
+            }
         }
-        if (lane == 0)
-            sm.cut[b][warp] = (m.valid != LR_ALL || m.head ? 1u : 0u) | (m.valid != LR_ALL || m.tail ? 2u : 0u);
-        lr_arrive(1 + b, THREADS - 32 * N);
-        lr_arrive(5 + b, THREADS - 32 * N);
+        const int b = i & 1;
+        bool any = cuts, any_back = cuts_back;
+        if constexpr (LR_GROUPS > 1) {
+            float a[N], h[N], m[N];
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                a[i] = A[i], h[i] = H[i], m[i] = M[i];
+                sm.group[b][warp][i][lane] = A[i];
+                sm.group[b][warp][N + i][lane] = H[i];
+                sm.group[b][warp][2 * N + i][lane] = M[i];
+            }
+            // states go down the groups, gradients up
+#pragma unroll
+            for (int s = 1; s < LR_GROUPS; ++s) {
+                const bool cut = __shfl_down_sync(0xffffffffu, cuts, s * LR_LANES);
+                any |= cut;
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    const float as = __shfl_down_sync(0xffffffffu, a[i], s * LR_LANES);
+                    const float hs = __shfl_down_sync(0xffffffffu, h[i], s * LR_LANES);
+                    H[i] = cut ? hs : fmaf(as, H[i], hs);
+                    A[i] *= as;
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < N; ++i) M[i] = 0.0f;
+#pragma unroll
+            for (int s = LR_GROUPS - 1; s >= 0; --s) {
+                const bool cut = __shfl_down_sync(0xffffffffu, cuts_back, s * LR_LANES);
+                any_back |= cut;
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    const float as = __shfl_down_sync(0xffffffffu, a[i], s * LR_LANES);
+                    const float ms = __shfl_down_sync(0xffffffffu, m[i], s * LR_LANES);
+                    M[i] = cut ? ms : fmaf(as, M[i], ms);
+                }
+            }
+        }
+        if (group == 0) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                sm.map[b][warp][column + i] = make_float2(A[i], H[i]);
+                sm.grad_map[b][warp][column + i] = M[i];
+            }
+            if (lane == 0) sm.cut[b][warp] = (any ? 1u : 0u) | (any_back ? 2u : 0u);
+        }
+        lr_arrive(1 + b, Config::MAPPED);
+        lr_arrive(5 + b, Config::MAPPED);
     };
     auto finish = [&](uint32_t i) {
         const int b = i & 1;
         const uint32_t st = i % Smem::STAGES;
-        const uint2 t = tl.tile(i);
-        const uint64_t first = (uint64_t)row_tile(t) * LR_TILE + warp * LR_ROWS;
-        const uint32_t c = t.y * C + lane * N;
-        const int left = (int)min((uint32_t)N, channels - min(channels, c));
-        const LrMarks m = marks(st, first);
-        const char(*rows)[LR_WARP_BUF] = sm.rows[st][warp];
-        lr_sync(3 + b, THREADS);
-        auto both = [&](auto tag) {
-            constexpr bool marked = decltype(tag)::value;
-            float h[N], mu[N], a[LR_ROWS][N], na[LR_ROWS][N], dgate[LR_ROWS][N];  // dgate: of the gate, per unit of lam
+        const LrSlot& sl = sm.slot[i % LR_SLOTS];
+        const int left = (int)sl.channels - column;
+        bool plain;
+        const uint32_t code = codes(sl, st, &plain);
+        const uint32_t *gate = lr_words(sm.rows[st][warp][0]), *in = lr_words(sm.rows[st][warp][1]),
+                       *grad = lr_words(sm.rows[st][warp][2]);
+        T* out_gate = (T*)((char*)out_gate0 + sl.offset[3]);
+        T* out_in = (T*)((char*)out_in0 + sl.offset[4]);
+        float h[N], mu[N], a[LR_ROWS][N], na[LR_ROWS][N], dgate[LR_ROWS][N];  // dgate: of the gate, per unit of lam
+        lr_sync(3 + b, Config::THREADS);
 #pragma unroll
-            for (int i = 0; i < N; ++i)
-                h[i] = sm.start[b][warp][lane * N + i], mu[i] = sm.grad_start[b][warp][lane * N + i];
+        for (int i = 0; i < N; ++i) h[i] = sm.start[b][warp][column + i], mu[i] = sm.grad_start[b][warp][column + i];
+        // the groups' starts, from the group before (behind) each
+        auto starts = [&](bool cuts, bool cuts_back) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const float A = sm.group[b][warp][i][lane], H = sm.group[b][warp][N + i][lane],
+                            M = sm.group[b][warp][2 * N + i][lane];
+#pragma unroll
+                for (int s = 1; s < LR_GROUPS; ++s) {
+                    const float up = __shfl_up_sync(0xffffffffu, cuts ? H : fmaf(A, h[i], H), LR_LANES);
+                    if (group == s) h[i] = up;
+                }
+#pragma unroll
+                for (int s = LR_GROUPS - 2; s >= 0; --s) {
+                    const float down = __shfl_down_sync(0xffffffffu, cuts_back ? M : fmaf(A, mu[i], M), LR_LANES);
+                    if (group == s) mu[i] = down;
+                }
+            }
+        };
+        if (plain) {
+            if constexpr (LR_GROUPS > 1) starts(false, false);
 #pragma unroll
             for (int r = 0; r < LR_ROWS; ++r) {
                 float g[N], x[N];
-                LrWord<T>::widen(lr_load(rows[0], r), g);
-                LrWord<T>::widen(lr_load(rows[1], r), x);
-                if (marked && (m.head >> r & 1)) init(m, r, c, h);
+                LrWord<T>::widen(gate[r * LR_ROW_WORDS], g);
+                LrWord<T>::widen(in[r * LR_ROW_WORDS], x);
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
                     const Gate<GATE> gt(g[i]);
@@ -717,35 +953,61 @@ __global__ void __launch_bounds__(LR_THREADS<T>, 1) lr_backward_kernel(LrBackwar
                     h[i] = fmaf(gt.a, h[i], gt.add(x[i]));
                 }
             }
-            T* out_gate = (T*)p.grad_gate + (first + LR_ROWS - 1) * p.grad_gate_stride + c;
-            T* out_in = (T*)p.grad_in + (first + LR_ROWS - 1) * p.grad_in_stride + c;
 #pragma unroll
             for (int r = LR_ROWS - 1; r >= 0; --r, out_gate -= p.grad_gate_stride, out_in -= p.grad_in_stride) {
                 float v[N], dg[N], dx[N];
-                LrWord<T>::widen(p.grad_out ? lr_load(rows[2], r) : 0, v);
-                if (marked && (m.tail >> r & 1)) last(m, r, c, mu);
+                LrWord<T>::widen(grad[r * LR_ROW_WORDS], v);
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
                     const float lam = v[i] + mu[i];
                     dg[i] = lam * dgate[r][i];
                     dx[i] = GATE == LCPP_GATE_SIGMOID ? na[r][i] * lam : lam;
                     mu[i] = a[r][i] * lam;
-                    if (marked && !(m.valid >> r & 1)) dg[i] = dx[i] = mu[i] = 0.0f;
                 }
-                if (!marked || first + r < p.sh.rows) {
+                lr_store<T, COPY>(out_gate, dg, left);
+                lr_store<T, COPY>(out_in, dx, left);
+            }
+        } else {
+            const LrMarks m(code);
+            const uint32_t c = sl.channel + column;
+            const int rows = (int)sl.rows - warp * LR_WARP_ROWS - group * LR_ROWS;
+            if constexpr (LR_GROUPS > 1) starts(m.cuts(), m.cuts_back());
+#pragma unroll
+            for (int r = 0; r < LR_ROWS; ++r) {
+                float g[N], x[N];
+                LrWord<T>::widen(gate[r * LR_ROW_WORDS], g);
+                LrWord<T>::widen(in[r * LR_ROW_WORDS], x);
+                const uint64_t s = m.sequence(p.sh, r);
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    if (m.head >> r & 1) h[i] = p.init && c + i < channels ? p.init[s * p.init_stride + c + i] : 0.0f;
+                    const Gate<GATE> gt(g[i]);
+                    a[r][i] = gt.a, na[r][i] = gt.na;
+                    dgate[r][i] = gt.grad_gate(h[i], x[i]);
+                    h[i] = fmaf(gt.a, h[i], gt.add(x[i]));
+                }
+            }
+#pragma unroll
+            for (int r = LR_ROWS - 1; r >= 0; --r, out_gate -= p.grad_gate_stride, out_in -= p.grad_in_stride) {
+                float v[N], dg[N], dx[N];
+                LrWord<T>::widen(grad[r * LR_ROW_WORDS], v);
+                const uint64_t s = m.sequence(p.sh, r);
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    if (m.tail >> r & 1) mu[i] = p.grad_last && c + i < channels ? p.grad_last[s * channels + c + i] : 0.0f;
+                    const float lam = v[i] + mu[i];
+                    const bool valid = m.valid >> r & 1;
+                    dg[i] = valid ? lam * dgate[r][i] : 0.0f;
+                    dx[i] = valid ? GATE == LCPP_GATE_SIGMOID ? na[r][i] * lam : lam : 0.0f;
+                    mu[i] = valid ? a[r][i] * lam : 0.0f;
+                    if ((m.head >> r & 1) && p.grad_init && i < left) p.grad_init[s * channels + c + i] = mu[i];
+                }
+                if (r < rows) {
                     lr_store<T, COPY>(out_gate, dg, left);
                     lr_store<T, COPY>(out_in, dx, left);
                 }
-                if (marked && (m.head >> r & 1) && p.grad_init) {
-                    const uint64_t s = m.sequence(p.sh, r);
-#pragma unroll
-                    for (int i = 0; i < N; ++i)
-                        if (i < left) p.grad_init[s * channels + c + i] = mu[i];
-                }
             }
-        };
-        if (m.valid == LR_ALL && m.head == 0 && m.tail == 0) both(std::false_type{});
-        else both(std::true_type{});
+        }
         __syncwarp();  // the stage is read
         fetch(i + Smem::STAGES);
     };
@@ -876,8 +1138,7 @@ static lcpp_status lr_prepare(const LrShape& sh, void* temp, const float* from, 
 
 template <typename T, typename Smem, typename K, typename P>
 static lcpp_status lr_launch(K kernel, const char* name, const P& p, const LrShape& sh, void* temp, cudaStream_t s) {
-    constexpr int N = LrWord<T>::N;
-    const uint64_t row_tiles = ceil_div(sh.rows, LR_TILE), col_tiles = ceil_div(sh.channels, 32 * N);
+    const uint64_t row_tiles = ceil_div(sh.rows, LR_TILE), col_tiles = ceil_div(sh.channels, LrConfig<T>::C);
     if (row_tiles * col_tiles > 0x7fffffffull) return LCPP_ERR_INVALID_ARG;
     const uint64_t grid = min(row_tiles * col_tiles, (uint64_t)device_info().sms);
     const LrTiles tl{(uint32_t)row_tiles, LrDivisor(col_tiles), (const uint32_t*)temp, grid > 6 * col_tiles};
@@ -888,7 +1149,7 @@ static lcpp_status lr_launch(K kernel, const char* name, const P& p, const LrSha
     together.val.cooperative = 1;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)grid);
-    cfg.blockDim = dim3(LR_THREADS<T>);
+    cfg.blockDim = dim3(LrConfig<T>::THREADS);
     cfg.dynamicSmemBytes = sizeof(Smem);
     cfg.stream = s;
     cfg.attrs = &together;
@@ -916,7 +1177,7 @@ extern "C" size_t lcpp_linear_recurrence_temp_bytes(uint64_t rows, uint64_t chan
 }
 
 extern "C" size_t lcpp_linear_recurrence_saved_bytes(uint64_t rows, uint64_t channels) {
-    return align_up(ceil_div(rows, LR_TILE) * channels * sizeof(float), 256);
+    return align_up(ceil_div(rows, 128) * channels * sizeof(float), 256);  // a state per tile, of 128 rows at least
 }
 
 extern "C" lcpp_status lcpp_linear_recurrence_forward(
