@@ -382,6 +382,7 @@ struct alignas(16) LrSlot {
     uint32_t pad;
 };
 constexpr int LR_SLOTS = 8, LR_AHEAD = 6;
+static_assert(LR_SLOTS >= LR_AHEAD + 2, "a slot is rewritten after its tile is finished");
 
 template <int M>
 __device__ __forceinline__ void lr_slot(LrSlot& slot, const LrShape& sh, uint64_t row, uint64_t channel, uint32_t columns,
@@ -430,6 +431,7 @@ __global__ void __launch_bounds__(LrConfig<T>::THREADS, 1) lr_forward_kernel(LrF
     using Config = LrConfig<T>;
     using Smem = LrForwardSmem<T>;
     constexpr int N = Config::N, C = Config::C;
+    static_assert(Smem::STAGES + 2 <= LR_AHEAD, "tile i + STAGES is fetched after the starts of tile i - 2");
     extern __shared__ __align__(128) char smem_raw[];
     Smem& sm = *(Smem*)smem_raw;
     const int lane = threadIdx.x & 31, warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
@@ -685,6 +687,7 @@ __global__ void __launch_bounds__(LrConfig<T>::THREADS, 1) lr_backward_kernel(Lr
     using Config = LrConfig<T>;
     using Smem = LrBackwardSmem<T>;
     constexpr int N = Config::N, C = Config::C;
+    static_assert(Smem::STAGES <= LR_AHEAD, "tile i + STAGES is fetched after the starts of tile i");
     extern __shared__ __align__(128) char smem_raw[];
     Smem& sm = *(Smem*)smem_raw;
     const int lane = threadIdx.x & 31, warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
@@ -1063,26 +1066,70 @@ lr_prepare_kernel(uint4* words, uint64_t count, uint32_t* codes, LrShape sh, con
     }
 }
 
-// One token: row i continues the state of row parents[i] (itself without
-// parents; zero for a negative parent).
-template <typename T, int GATE>
-__global__ void __launch_bounds__(256)
+// ---- One token ---------------------------------------------------------------------
+// Row i continues the state of row parents[i] (itself without parents; zero for
+// a negative parent).  Bound by the bytes; a warp takes U x 32 vectors of V
+// channels of a row, so that enough loads are under way at any alignment.
+constexpr int LR_STEP_WARPS = 4;
+
+template <typename T, int V>
+struct alignas(V * sizeof(T)) LrVector {
+    T v[V];
+};
+
+template <typename T, int GATE, int V, int U>
+__global__ void __launch_bounds__(LR_STEP_WARPS * 32)
 lr_step_kernel(const T* gate, uint64_t gate_stride, const T* in, uint64_t in_stride, const float* states_in,
-               uint64_t rows_in, const int32_t* parents, float* states_out, T* out, uint64_t out_stride,
-               uint64_t rows, uint64_t channels) {
-    const uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= rows * channels) return;
-    const uint64_t r = i / channels, c = i - r * channels;
+               uint32_t rows_in, const int32_t* parents, float* states_out, T* out, uint64_t out_stride,
+               uint32_t rows, uint32_t channels, uint32_t parts) {
+    constexpr int VS = V > 4 ? 4 : V;  // states a load
+    using Vector = LrVector<T, V>;
+    using States = LrVector<float, VS>;
+    const uint32_t unit = blockIdx.x * LR_STEP_WARPS + (threadIdx.x >> 5), r = unit / parts;
+    if (r >= rows) return;
+    const uint32_t c0 = (unit - r * parts) * (32 * V * U) + (threadIdx.x & 31) * V;
     int64_t from = parents ? (int64_t)parents[r] : (int64_t)r;
-    if (from >= (int64_t)rows_in) {
+    Vector g[U], x[U];
+    States h[U][V / VS];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const uint32_t c = c0 + u * 32 * V;
+        if (c < channels) {
+            g[u] = *(const Vector*)(gate + r * gate_stride + c);
+            x[u] = *(const Vector*)(in + r * in_stride + c);
+        }
+    }
+    if (!states_in) {
+        from = -1;
+    } else if (from >= (int64_t)rows_in) {
         set_error(LCPP_ERR_INVALID_ARG);
         from = -1;
     }
-    const float before = states_in && from >= 0 ? states_in[from * channels + c] : 0.0f;
-    const Gate<GATE> g(widen(gate[r * gate_stride + c]));
-    const float h = fmaf(g.a, before, g.add(widen(in[r * in_stride + c])));
-    states_out[i] = h;
-    if (out) out[r * out_stride + c] = narrow<T>(h);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int j = 0; j < V / VS; ++j) {
+            const uint32_t c = c0 + u * 32 * V;
+#pragma unroll
+            for (int i = 0; i < VS; ++i) h[u][j].v[i] = 0.0f;
+            if (from >= 0 && c < channels) h[u][j] = *(const States*)(states_in + from * channels + c + j * VS);
+        }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const uint32_t c = c0 + u * 32 * V;
+        if (c >= channels) break;
+        Vector y;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            float& s = h[u][i / VS].v[i % VS];
+            const Gate<GATE> gt(widen(g[u].v[i]));
+            s = fmaf(gt.a, s, gt.add(widen(x[u].v[i])));
+            y.v[i] = narrow<T>(s);
+        }
+#pragma unroll
+        for (int j = 0; j < V / VS; ++j) *(States*)(states_out + (uint64_t)r * channels + c + j * VS) = h[u][j];
+        if (out) *(Vector*)(out + r * out_stride + c) = y;
+    }
 }
 
 constexpr uint64_t LR_MAX_ROWS = 0xffffffffull;  // offsets are 32-bit
@@ -1267,11 +1314,24 @@ extern "C" lcpp_status lcpp_linear_recurrence_step(int gate, int dtype, const vo
     cudaStream_t s = (cudaStream_t)stream;
     return lr_dispatch(gate, dtype, [&](auto t, auto g) -> lcpp_status {
         using T = decltype(t);
-        ProfScope prof("lr_step", s);
-        lr_step_kernel<T, decltype(g)::value><<<(unsigned)ceil_div(rows * channels, 256), 256, 0, s>>>(
-            (const T*)gate_in, gate_stride, (const T*)in, in_stride, states_in, rows_in, parents, states_out, (T*)out,
-            out_stride, rows, channels);
-        count_launch();
-        return check_launch();
+        constexpr int G = decltype(g)::value, WIDE = 16 / sizeof(T);
+        // the widest vectors that every row of every operand is a whole number of
+        uint64_t bits = (uint64_t)(uintptr_t)gate_in | (uint64_t)(uintptr_t)in | (uint64_t)(uintptr_t)out;
+        if (rows > 1) bits |= (gate_stride | in_stride | (out ? out_stride : 0)) * sizeof(T);
+        const uint64_t states = (uint64_t)(uintptr_t)states_in | (uint64_t)(uintptr_t)states_out;
+        auto fits = [&](int v) { return channels % v == 0 && bits % (v * sizeof(T)) == 0 && states % (v > 4 ? 16 : v * 4) == 0; };
+        auto launch = [&](auto kernel, int span) -> lcpp_status {
+            const uint64_t parts = ceil_div(channels, span), units = parts * rows;
+            if (ceil_div(units, LR_STEP_WARPS) > 0x3fffffffull) return LCPP_ERR_INVALID_ARG;
+            ProfScope prof("lr_step", s);
+            kernel<<<(unsigned)ceil_div(units, LR_STEP_WARPS), LR_STEP_WARPS * 32, 0, s>>>(
+                (const T*)gate_in, gate_stride, (const T*)in, in_stride, states_in, (uint32_t)rows_in, parents, states_out,
+                (T*)out, out_stride, (uint32_t)rows, (uint32_t)channels, (uint32_t)parts);
+            count_launch();
+            return check_launch();
+        };
+        if (fits(WIDE)) return launch(lr_step_kernel<T, G, WIDE, 1>, 32 * WIDE);
+        if (fits(2)) return launch(lr_step_kernel<T, G, 2, 2>, 32 * 2 * 2);
+        return launch(lr_step_kernel<T, G, 1, 4>, 32 * 4);
     });
 }
