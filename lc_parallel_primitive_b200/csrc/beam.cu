@@ -72,7 +72,7 @@ __device__ __forceinline__ uint64_t warp_top(const uint64_t* keys, int n) {
 // element).
 constexpr int BEAM_VECS = 4;
 constexpr int BEAM_TILE = BEAM_THREADS * BEAM_VECS;  // vectors of a tile of a part
-constexpr int BEAM_TILES = 16;                       // tiles of a part at most
+constexpr int BEAM_TILES = 32;                       // tiles of a part at most
 constexpr int BEAM_KEYS = 1024;                      // logits that may reach the threads' bound
 
 // Results of one part: its `beams` best keys (ordered logit << 32 | ~token, 0: none), largest logit, and the sum of
@@ -82,46 +82,28 @@ struct BeamTemp {
     float2* total;   // [rows][parts]
 };
 
-// The vector at address `at`, of which elements [lo, hi) belong to the row; the others, and NaN, read as -inf.
+// 16 bytes of a row.
 template <typename T>
 struct BeamVector {
     static constexpr int E = 16 / sizeof(T);
     uint4 w;
+    // The vector at address `at`, of which elements [lo, hi) belong to the row; the others read as -inf.
     __device__ __forceinline__ void load(const T* at, int64_t lo, int64_t hi) {
-        if (lo <= 0 && hi >= E) {
-            w = ld_stream((const uint4*)at);
-            return;
-        }
-        float v[E];
-#pragma unroll
-        for (int e = 0; e < E; ++e) v[e] = e >= lo && e < hi ? widen(at[e]) : -INFINITY;
-        pack(v);
-    }
-    __device__ __forceinline__ void pack(const float* v) {
         T t[E];
 #pragma unroll
-        for (int e = 0; e < E; ++e) t[e] = narrow<T>(v[e]);
+        for (int e = 0; e < E; ++e) t[e] = e >= lo && e < hi ? at[e] : narrow<T>(-INFINITY);
         memcpy(&w, t, 16);
     }
-    // No NaN from here on; the largest element.
-    __device__ __forceinline__ float clean_max() {
+    // The largest element that is not NaN (-inf if there is none).
+    __device__ __forceinline__ float max() const {
         if constexpr (sizeof(T) == 4) {
-            float v[4];
-            memcpy(v, &w, 16);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = fmaxf(v[e], -INFINITY);
-            memcpy(&w, v, 16);
-            return fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3]));
+            return fmaxf(fmaxf(get(0), get(1)), fmaxf(fmaxf(get(2), get(3)), -INFINITY));
         } else {
             using T2 = std::conditional_t<std::is_same_v<T, __half>, __half2, __nv_bfloat162>;
-            T2 v[4], low;
+            T2 v[4];
             memcpy(v, &w, 16);
-            low.x = low.y = narrow<T>(-INFINITY);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = __hmax2(v[e], low);
-            memcpy(&w, v, 16);
             const T2 m = __hmax2(__hmax2(v[0], v[1]), __hmax2(v[2], v[3]));
-            return fmaxf(widen(m.x), widen(m.y));
+            return fmaxf(fmaxf(widen(m.x), widen(m.y)), -INFINITY);
         }
     }
     __device__ __forceinline__ float get(int e) const {
@@ -152,47 +134,56 @@ __device__ __forceinline__ bool beam_live(const float* scores, const uint8_t* fi
     return scores[row] > -INFINITY && !(finished && finished[row]);
 }
 
+struct BeamRow {
+    int beams;
+    uint32_t vocab, part, parts;
+};
+
 template <typename T>
-__global__ void __launch_bounds__(BEAM_THREADS, 4)
-beam_rows_kernel(const T* logits, uint64_t stride, const float* scores, const uint8_t* finished, int beams,
-                 uint32_t vocab, uint32_t parts, BeamTemp tmp) {
+struct BeamPartSmem {
+    float chunk[BEAM_TILES][BEAM_THREADS];
+    uint64_t key[BEAM_KEYS];
+    float top[BEAM_THREADS / 32][32], scale[BEAM_THREADS / 32], sum[BEAM_THREADS / 32];
+    int count;
+};
+
+// Part p.part of the row z: the calling CTA's first warp returns its `beams` best keys, a lane each, and all threads
+// (largest, total).
+template <typename T>
+__device__ __forceinline__ uint64_t beam_part(const T* z, const BeamRow& p, BeamPartSmem<T>& sm, float2* out) {
     constexpr int E = BeamVector<T>::E, WARPS = BEAM_THREADS / 32;
-    __shared__ float s_chunk[BEAM_TILES][BEAM_THREADS];
-    __shared__ uint64_t s_key[BEAM_KEYS];
-    __shared__ float s_top[WARPS][32], s_scale[WARPS], s_sum[WARPS];
-    __shared__ int s_count;
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const uint64_t row = blockIdx.x / parts;
-    const uint32_t part = blockIdx.x - (uint32_t)row * parts;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    if (!beam_live(scores, finished, row)) return;
-    const T* z = logits + row * stride;
-    const int64_t shift = ((uintptr_t)z & 15) / sizeof(T);  // elements between the first vector's address and z
+    const int shift = (int)(((uintptr_t)z & 15) / sizeof(T));  // elements between the first vector's address and z
     const T* base = z - shift;
-    const uint32_t vectors = (uint32_t)((shift + vocab + E - 1) / E);
+    const uint32_t end = shift + p.vocab, vectors = (end + E - 1) / E;  // vocab < 2^31
     const uint32_t tiles = (vectors + BEAM_TILE - 1) / BEAM_TILE;
-    const uint32_t tile0 = (uint32_t)((uint64_t)tiles * part / parts), tile1 = (uint32_t)((uint64_t)tiles * (part + 1) / parts);
+    const uint32_t tile0 = (uint32_t)((uint64_t)tiles * p.part / p.parts);
+    const uint32_t tile1 = (uint32_t)((uint64_t)tiles * (p.part + 1) / p.parts);
     const int n = (int)(tile1 - tile0);
-    auto load = [&](BeamVector<T>* v, uint32_t tile) {
+    using Chunk = BeamVector<T>[BEAM_VECS];
+    auto load = [&](Chunk& v, uint32_t tile) {
+        const uint32_t at0 = tile * BEAM_TILE + tid;
+        if ((tile > 0 || shift == 0) && (tile + 1) * BEAM_TILE <= end / E) {  // all inside the row
+            const uint4* src = (const uint4*)base + at0;
 #pragma unroll
-        for (int q = 0; q < BEAM_VECS; ++q) {
-            const uint32_t at = tile * BEAM_TILE + q * BEAM_THREADS + tid;
-            // elements of the vector before the row's first and behind its last
-            const int64_t first = shift - (int64_t)at * E, end = first + vocab;
-            if (at < vectors) v[q].load(base + (int64_t)at * E, first, end);
-            else v[q].load(base, E, 0);
+            for (int q = 0; q < BEAM_VECS; ++q) v[q].w = ld_stream(src + q * BEAM_THREADS);
+        } else {
+#pragma unroll
+            for (int q = 0; q < BEAM_VECS; ++q) {
+                const uint32_t at = at0 + q * BEAM_THREADS;
+                const int64_t first = (int64_t)at * E;  // element of the vectors' count
+                if (at < vectors) v[q].load(base + first, shift - first, (int64_t)end - first);
+                else v[q].load(base, E, 0);
+            }
         }
     };
-    if (tid == 0) s_count = 0;
+    if (tid == 0) sm.count = 0;
     float top = -INFINITY, scale = -1e30f, sum = 0.0f;  // sum of 2^(z log2e - scale)
-    BeamVector<T> v[BEAM_VECS], ahead[BEAM_VECS];
-    if (n > 0) load(v, tile0);
-    for (int j = 0; j < n; ++j) {
-        if (j + 1 < n) load(ahead, tile0 + j + 1);
-        float m = v[0].clean_max();
+    auto add = [&](const Chunk& v, int j) {
+        float m = v[0].max();
 #pragma unroll
-        for (int q = 1; q < BEAM_VECS; ++q) m = fmaxf(m, v[q].clean_max());
-        s_chunk[j][tid] = m;
+        for (int q = 1; q < BEAM_VECS; ++q) m = fmaxf(m, v[q].max());
+        sm.chunk[j][tid] = m;
         top = fmaxf(top, m);
         const float k = ceilf(m * BEAM_LOG2E);
         if (k > scale) {
@@ -206,147 +197,225 @@ beam_rows_kernel(const T* logits, uint64_t stride, const float* scores, const ui
             for (int e = 0; e < E; ++e) part_sum += beam_ex2(fmaf(v[q].get(e), BEAM_LOG2E, -scale));
             sum += part_sum;
         }
-#pragma unroll
-        for (int q = 0; q < BEAM_VECS; ++q) v[q] = ahead[q];
+    };
+    Chunk v, ahead;
+    if (n > 0) load(v, tile0);
+    for (int j = 0; j < n; j += 2) {
+        if (j + 1 < n) load(ahead, tile0 + j + 1);
+        add(v, j);
+        if (j + 1 < n) {
+            if (j + 2 < n) load(v, tile0 + j + 2);
+            add(ahead, j + 1);
+        }
     }
     // ---- the part's maximum and sum, and the beams-th largest of the threads' maxima ----
     float sorted = warp_sort(top);
-    s_top[warp][lane] = sorted;
+    sm.top[warp][lane] = sorted;
     float warp_scale = scale;
     for (int o = 16; o; o >>= 1) warp_scale = fmaxf(warp_scale, __shfl_xor_sync(0xffffffffu, warp_scale, o));
     float warp_sum = sum * beam_ex2(scale - warp_scale);
     for (int o = 16; o; o >>= 1) warp_sum += __shfl_xor_sync(0xffffffffu, warp_sum, o);
-    if (lane == 0) s_scale[warp] = warp_scale, s_sum[warp] = warp_sum;
+    if (lane == 0) sm.scale[warp] = warp_scale, sm.sum[warp] = warp_sum;
     for (int half = WARPS / 2; half; half >>= 1) {
         __syncthreads();
         if (warp < half) {
-            sorted = warp_merge(sorted, s_top[warp + half][lane]);
-            s_top[warp][lane] = sorted;
+            sorted = warp_merge(sorted, sm.top[warp + half][lane]);
+            sm.top[warp][lane] = sorted;
         }
     }
     __syncthreads();
-    const float largest = s_top[0][0], bound = s_top[0][beams - 1];
+    const float largest = sm.top[0][0], bound = sm.top[0][p.beams - 1];
     // ---- what reaches the bound ------------------------------------------------------
-    for (int j = 0; j < n; ++j) {
-        if (!(s_chunk[j][tid] >= bound && s_chunk[j][tid] > -INFINITY)) continue;
-        load(v, tile0 + j);
-        for (int q = 0; q < BEAM_VECS; ++q) {
-            v[q].clean_max();
-            for (int e = 0; e < E; ++e) {
-                const float x = v[q].get(e);
-                if (x >= bound && x > -INFINITY) {
-                    const int at = atomicAdd(&s_count, 1);
-                    const uint32_t token = (uint32_t)(((int64_t)(tile0 + j) * BEAM_TILE + q * BEAM_THREADS + tid) * E + e - shift);
-                    if (at < BEAM_KEYS) s_key[at] = (uint64_t)ordered(x) << 32 | (uint32_t)~token;
-                }
+    if (top >= bound && top > -INFINITY) {
+        for (int j = 0; j < n; ++j) {
+            const float m = sm.chunk[j][tid];
+            if (!(m >= bound && m > -INFINITY)) continue;
+            if (n > 2) {
+                load(v, tile0 + j);
+            } else if (j == 1) {  // both are still here, the first in v
+#pragma unroll
+                for (int q = 0; q < BEAM_VECS; ++q) v[q] = ahead[q];
             }
+#pragma unroll
+            for (int q = 0; q < BEAM_VECS; ++q)
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    const float x = v[q].get(e);
+                    if (x >= bound && x > -INFINITY) {
+                        const int at = atomicAdd(&sm.count, 1);
+                        const uint32_t token = ((tile0 + j) * BEAM_TILE + q * BEAM_THREADS + tid) * E + e - shift;
+                        if (at < BEAM_KEYS) sm.key[at] = (uint64_t)ordered(x) << 32 | (uint32_t)~token;
+                    }
+                }
         }
     }
     __syncthreads();
-    uint64_t* out = tmp.key + (row * parts + part) * beams;
-    const uint32_t first = (uint32_t)max((int64_t)tile0 * BEAM_TILE * E - shift, (int64_t)0);
-    const uint32_t end = (uint32_t)min((int64_t)tile1 * BEAM_TILE * E - shift, (int64_t)vocab);
-    if (s_count <= BEAM_KEYS) {
-        if (warp == 0) {
-            const uint64_t key = warp_top(s_key, s_count);
-            if (lane < beams) out[lane] = key;
-        }
+    const uint32_t first = max((int64_t)tile0 * BEAM_TILE * E - shift, (int64_t)0);
+    const uint32_t stop = min((int64_t)tile1 * BEAM_TILE * E - shift, (int64_t)p.vocab);
+    uint64_t mine = 0;
+    if (sm.count <= BEAM_KEYS) {
+        if (warp == 0) mine = warp_top(sm.key, sm.count);
     } else {  // many equal logits: the best below the last one found, `beams` times over
         uint64_t below = ~0ull;
-        for (int j = 0; j < beams; ++j) {
+        for (int j = 0; j < p.beams; ++j) {
             uint64_t best = 0;
-            for (uint32_t t = first + tid; t < end; t += BEAM_THREADS) {
+            for (uint32_t t = first + tid; t < stop; t += BEAM_THREADS) {
                 const float x = widen(z[t]);
                 const uint64_t key = (uint64_t)ordered(x) << 32 | (uint32_t)~t;
                 if (x >= bound && x > -INFINITY && key < below && key > best) best = key;
             }
             for (int o = 16; o; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
             __syncthreads();
-            if (lane == 0) s_key[warp] = best;
+            if (lane == 0) sm.key[warp] = best;
             __syncthreads();
-            for (int w = 0; w < WARPS; ++w) best = max(best, s_key[w]);
+            for (int w = 0; w < WARPS; ++w) best = max(best, sm.key[w]);
             below = best;
-            if (tid == 0) out[j] = best;
+            if (tid == j) mine = best;
         }
     }
-    float all_scale = s_scale[0], total = 0.0f;
-    for (int w = 1; w < WARPS; ++w) all_scale = fmaxf(all_scale, s_scale[w]);
-    for (int w = 0; w < WARPS; ++w) total += s_sum[w] * beam_ex2(s_scale[w] - all_scale);
+    float all_scale = sm.scale[0], total = 0.0f;
+#pragma unroll
+    for (int w = 1; w < WARPS; ++w) all_scale = fmaxf(all_scale, sm.scale[w]);
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) total += sm.sum[w] * beam_ex2(sm.scale[w] - all_scale);
     // relative to the largest term, which went through the same product
     total /= beam_ex2(fmaf(largest, BEAM_LOG2E, -all_scale));
     if (!(total >= 0.5f && total < INFINITY) && largest > -INFINITY) {
-        // a maximum of +inf or one whose scaled value is out of range: term by term
+        // NaN among the logits, a maximum of +inf, or one whose scaled value is out of range: term by term
         total = 0.0f;
-        for (uint32_t t = first + tid; t < end; t += BEAM_THREADS) {
+        for (uint32_t t = first + tid; t < stop; t += BEAM_THREADS) {
             const float x = fmaxf(widen(z[t]), -INFINITY);
             total += x == largest ? 1.0f : __expf(x - largest);
         }
         for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
         __syncthreads();
-        if (lane == 0) s_sum[warp] = total;
+        if (lane == 0) sm.sum[warp] = total;
         __syncthreads();
         total = 0.0f;
-        for (int w = 0; w < WARPS; ++w) total += s_sum[w];
+        for (int w = 0; w < WARPS; ++w) total += sm.sum[w];
     }
-    if (tid == 0) tmp.total[row * parts + part] = make_float2(largest, total);
+    *out = make_float2(largest, total);
+    return mine;
 }
 
 // ---- One batch entry ----------------------------------------------------------------
 // A warp a beam joins the parts of its row; then the first warp takes the best
-// of all beams' candidates.
-template <int WARPS>
-__global__ void __launch_bounds__(WARPS * 32)
-beam_merge_kernel(BeamTemp tmp, const float* scores, const uint8_t* finished, int beams, uint32_t parts, int eos,
-                  float* scores_out, int32_t* tokens_out, int32_t* parents_out, uint8_t* finished_out) {
-    __shared__ uint64_t s_key[BEAM_MAX * BEAM_MAX];
-    __shared__ float s_score[BEAM_MAX * BEAM_MAX];
-    __shared__ int32_t s_token[BEAM_MAX * BEAM_MAX];
-    const uint64_t first = (uint64_t)blockIdx.x * beams;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    for (int k = warp; k < beams; k += WARPS) {
+// of all beams' candidates.  key: [beam][part][beams], total: [beam][part].
+struct BeamOut {
+    float* scores;
+    int32_t *tokens, *parents;
+    uint8_t* finished;
+};
+struct BeamMergeSmem {
+    uint64_t key[BEAM_MAX * BEAM_MAX];
+    float score[BEAM_MAX * BEAM_MAX];
+    int32_t token[BEAM_MAX * BEAM_MAX];
+};
+
+__device__ __forceinline__ void beam_merge(const uint64_t* key, const float2* total, uint64_t first, const float* scores,
+                                           const uint8_t* finished, int beams, uint32_t parts, int eos,
+                                           const BeamOut& out, BeamMergeSmem& sm) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    for (int k = warp; k < beams; k += warps) {
         const uint64_t row = first + k;
         const float score = scores[row];
         float best = -INFINITY;
         int32_t token = max(eos, 0);
         if (beam_live(scores, finished, row)) {
-            const uint64_t key = warp_top(tmp.key + row * parts * beams, (int)(parts * beams));
-            float largest = -INFINITY, total = 0.0f;
-            for (uint32_t i = lane; i < parts; i += 32) largest = fmaxf(largest, tmp.total[row * parts + i].x);
+            const uint64_t mine = warp_top(key + (uint64_t)k * parts * beams, (int)(parts * beams));
+            float largest = -INFINITY, sum = 0.0f;
+            for (uint32_t i = lane; i < parts; i += 32) largest = fmaxf(largest, total[(uint64_t)k * parts + i].x);
             for (int o = 16; o; o >>= 1) largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, o));
             for (uint32_t i = lane; i < parts; i += 32) {
-                const float2 t = tmp.total[row * parts + i];
-                if (t.x > -INFINITY) total += t.x == largest ? t.y : t.y * __expf(t.x - largest);
+                const float2 t = total[(uint64_t)k * parts + i];
+                if (t.x > -INFINITY) sum += t.x == largest ? t.y : t.y * __expf(t.x - largest);
             }
-            for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-            if (key) {
-                const float z = unordered((uint32_t)(key >> 32));
-                best = score + ((z == largest ? 0.0f : z - largest) - logf(total));
-                token = (int32_t)~(uint32_t)key;
+            for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            if (mine) {
+                const float z = unordered((uint32_t)(mine >> 32));
+                best = score + ((z == largest ? 0.0f : z - largest) - logf(sum));
+                token = (int32_t)~(uint32_t)mine;
             }
         } else if (lane == 0 && score > -INFINITY) {
             best = score;  // finished: it stays
         }
         if (lane < beams) {
             const int at = k * beams + lane;
-            s_score[at] = best, s_token[at] = token;
-            s_key[at] = best > -INFINITY ? (uint64_t)ordered(best) << 32 | (uint32_t)~at : 0;
+            sm.score[at] = best, sm.token[at] = token;
+            sm.key[at] = best > -INFINITY ? (uint64_t)ordered(best) << 32 | (uint32_t)~at : 0;
         }
     }
     __syncthreads();
     if (warp == 0) {
-        const uint64_t key = warp_top(s_key, beams * beams);
+        const uint64_t mine = warp_top(sm.key, beams * beams);
         if (lane < beams) {
-            const uint32_t at = ~(uint32_t)key;
-            const bool any = key != 0;
+            const uint32_t at = ~(uint32_t)mine;
+            const bool any = mine != 0;
             const uint64_t parent = any ? first + at / beams : first + lane;
-            const int32_t token = any ? s_token[at] : max(eos, 0);
-            scores_out[first + lane] = any ? s_score[at] : -INFINITY;
-            tokens_out[first + lane] = token;
-            parents_out[first + lane] = (int32_t)parent;
-            if (finished_out) finished_out[first + lane] = !any || (finished && finished[parent]) || token == eos;
+            const int32_t token = any ? sm.token[at] : max(eos, 0);
+            out.scores[first + lane] = any ? sm.score[at] : -INFINITY;
+            out.tokens[first + lane] = token;
+            out.parents[first + lane] = (int32_t)parent;
+            if (out.finished) out.finished[first + lane] = !any || (finished && finished[parent]) || token == eos;
         }
     }
+}
+
+// Two kernels: parts of all rows, joined through `tmp`.
+template <typename T>
+__global__ void __launch_bounds__(BEAM_THREADS, 4)
+beam_rows_kernel(const T* logits, uint64_t stride, const float* scores, const uint8_t* finished, int beams,
+                 uint32_t vocab, uint32_t parts, BeamTemp tmp) {
+    __shared__ BeamPartSmem<T> sm;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const uint64_t row = blockIdx.x / parts;
+    const uint32_t part = blockIdx.x - (uint32_t)row * parts;
+    if (!beam_live(scores, finished, row)) return;
+    float2 total;
+    const uint64_t key = beam_part(logits + row * stride, BeamRow{beams, vocab, part, parts}, sm, &total);
+    if (threadIdx.x < beams) tmp.key[(row * parts + part) * beams + threadIdx.x] = key;
+    if (threadIdx.x == 0) tmp.total[row * parts + part] = total;
+}
+__global__ void __launch_bounds__(256)
+beam_merge_kernel(BeamTemp tmp, const float* scores, const uint8_t* finished, int beams, uint32_t parts, int eos, BeamOut out) {
+    __shared__ BeamMergeSmem sm;
+    const uint64_t first = (uint64_t)blockIdx.x * beams;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    beam_merge(tmp.key + first * parts * beams, tmp.total + first * parts, first, scores, finished, beams, parts, eos, out, sm);
+}
+
+// One kernel: a cluster takes a batch entry, a CTA a part of one of its rows; the first CTA joins them from its
+// shared memory.  For few and short rows, where a second launch and the way through L2 are what counts.
+constexpr int BEAM_CLUSTER = 8;
+
+template <typename T>
+__global__ void __launch_bounds__(BEAM_THREADS)
+beam_cluster_kernel(const T* logits, uint64_t stride, const float* scores, const uint8_t* finished, int beams,
+                    uint32_t vocab, uint32_t parts, int eos, BeamOut out) {
+    __shared__ union {
+        BeamPartSmem<T> part;
+        BeamMergeSmem merge;
+    } sm;
+    __shared__ uint64_t s_key[BEAM_CLUSTER * BEAM_CLUSTER];
+    __shared__ float2 s_total[BEAM_CLUSTER];
+    asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");
+    const uint32_t size = beams * parts, rank = blockIdx.x % size, part = rank % parts;
+    const uint64_t first = (uint64_t)(blockIdx.x / size) * beams, row = first + rank / parts;
+    float2 total = make_float2(-INFINITY, 0.0f);
+    uint64_t key = 0;
+    if (beam_live(scores, finished, row))
+        key = beam_part(logits + row * stride, BeamRow{beams, vocab, part, parts}, sm.part, &total);
+    asm volatile("barrier.cluster.wait;" ::: "memory");  // the first CTA has started
+    uint32_t key_at, total_at;
+    asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(key_at) : "r"((uint32_t)__cvta_generic_to_shared(s_key)));
+    asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(total_at) : "r"((uint32_t)__cvta_generic_to_shared(s_total)));
+    if (threadIdx.x < beams)
+        asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(key_at + (rank * beams + threadIdx.x) * 8), "l"(key) : "memory");
+    if (threadIdx.x == 0)
+        asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(total_at + rank * 8), "f"(total.x), "f"(total.y) : "memory");
+    asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+    if (rank == 0) beam_merge(s_key, s_total, first, scores, finished, beams, parts, eos, out, sm.merge);
 }
 
 // ---- Reordering ------------------------------------------------------------------------
@@ -424,10 +493,14 @@ beam_reorder_kernel(const char* in, uint64_t in_layer, uint64_t in_row, char* ou
 
 // Parts of a row: whole tiles, at least as many as keep a part within BEAM_TILES of them, and as many more as give
 // every SM BEAM_PARTS_PER_SM parts.
-constexpr int BEAM_PARTS_PER_SM = 8;
-static uint32_t beam_parts(uint64_t rows, uint64_t vocab, size_t element, uint64_t sms) {
+constexpr int BEAM_PARTS_PER_SM = 3;
+constexpr int BEAM_SHORT = 4;
+static uint64_t beam_tiles(uint64_t vocab, size_t element) {  // at any alignment
     const uint64_t per_vector = 16 / element;
-    const uint64_t tiles = ceil_div(ceil_div(vocab + per_vector - 1, per_vector), BEAM_TILE);  // at any alignment
+    return ceil_div(ceil_div(vocab + per_vector - 1, per_vector), BEAM_TILE);
+}
+static uint32_t beam_parts(uint64_t rows, uint64_t vocab, size_t element, uint64_t sms) {
+    const uint64_t tiles = beam_tiles(vocab, element);
     const uint64_t least = ceil_div(tiles, BEAM_TILES);
     const uint64_t wanted = ceil_div(sms * BEAM_PARTS_PER_SM, rows ? rows : 1);
     return (uint32_t)std::max(least, std::min(wanted, tiles));
@@ -462,7 +535,31 @@ extern "C" lcpp_status lcpp_beam_select(int dtype, const void* logits, uint64_t 
     cudaStream_t s = (cudaStream_t)stream;
     return dispatch_float(dtype, [&](auto t) -> lcpp_status {
         using T = decltype(t);
-        const uint32_t parts = beam_parts(rows, vocab, sizeof(T), device_info().sms);
+        const BeamOut out{scores_out, tokens_out, parents_out, finished_out};
+        const uint64_t sms = device_info().sms;
+        uint32_t parts = beam_parts(rows, vocab, sizeof(T), sms);
+        // A cluster an entry, where that fills the SMs or leaves a CTA little to read.
+        const uint32_t split = BEAM_CLUSTER / beams;
+        const uint64_t tiles = beam_tiles(vocab, sizeof(T)), span = split ? ceil_div(tiles, std::min(split, parts)) : ~0ull;
+        if (span <= BEAM_SHORT || (span <= BEAM_TILES && rows * std::min(split, parts) >= 2 * sms)) {
+            parts = std::min(split, parts);
+            cudaLaunchAttribute cluster{};
+            cluster.id = cudaLaunchAttributeClusterDimension;
+            cluster.val.clusterDim.x = beams * parts;
+            cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
+            cudaLaunchConfig_t cfg{};
+            cfg.gridDim = dim3((unsigned)(rows * parts));
+            cfg.blockDim = dim3(BEAM_THREADS);
+            cfg.stream = s;
+            cfg.attrs = &cluster;
+            cfg.numAttrs = 1;
+            ProfScope prof("beam_cluster", s);
+            if (cudaLaunchKernelEx(&cfg, beam_cluster_kernel<T>, (const T*)logits, logits_stride, scores_in, finished_in,
+                                   (int)beams, (uint32_t)vocab, parts, (int)eos_token, out) != cudaSuccess)
+                return LCPP_ERR_CUDA;
+            count_launch();
+            return check_launch();
+        }
         if (rows * parts > 0x7fffffffull) return LCPP_ERR_INVALID_ARG;
         const BeamTemp tmp{(uint64_t*)temp, (float2*)((char*)temp + align_up(rows * parts * beams * 8, 256))};
         {
@@ -481,9 +578,8 @@ extern "C" lcpp_status lcpp_beam_select(int dtype, const void* logits, uint64_t 
         cfg.stream = s;
         cfg.attrs = &early;
         cfg.numAttrs = 1;
-        const auto kernel = beams > 1 ? beam_merge_kernel<8> : beam_merge_kernel<1>;
-        if (cudaLaunchKernelEx(&cfg, kernel, tmp, scores_in, finished_in, (int)beams, parts, eos_token, scores_out,
-                               tokens_out, parents_out, finished_out) != cudaSuccess)
+        if (cudaLaunchKernelEx(&cfg, beam_merge_kernel, tmp, scores_in, finished_in, (int)beams, parts, (int)eos_token,
+                               out) != cudaSuccess)
             return LCPP_ERR_CUDA;
         count_launch(2);
         return check_launch();
