@@ -26,17 +26,10 @@
 
 namespace lcpp {
 
-constexpr int LR_WARPS = 16;                             // compute warps
-constexpr int LR_LANES = 32;                             // lanes across a row, 4 bytes each: 1 float or 2 halves
-constexpr int LR_GROUPS = 32 / LR_LANES;                 // of a warp, one under the other
-constexpr int LR_ROWS = 8;                               // consecutive rows of a group
-constexpr int LR_WARP_ROWS = LR_ROWS * LR_GROUPS;
-constexpr int LR_TILE = LR_WARPS * LR_WARP_ROWS;         // rows of a tile, and rows between two saved states
-constexpr int LR_ROW_BYTES = LR_LANES * 4;
-// Groups are a row further apart in shared memory than their rows take, so that a load of the whole warp meets all
-// banks once.
-constexpr int LR_GROUP_BUF = LR_ROWS * LR_ROW_BYTES + (LR_GROUPS > 1 ? LR_ROW_BYTES : 0);
-constexpr int LR_WARP_BUF = LR_GROUPS * LR_GROUP_BUF;    // one warp's rows of one matrix
+constexpr int LR_WARPS = 16;                    // compute warps
+constexpr int LR_ROWS = 8;                      // consecutive rows of one warp
+constexpr int LR_TILE = LR_WARPS * LR_ROWS;     // rows of a tile, and rows between two saved states
+constexpr uint32_t LR_ALL = (1u << LR_ROWS) - 1;
 
 // Division of 32-bit numbers by a fixed one: the high half of n * ceil(2^64 / d) is n / d for all n, d < 2^32
 // (the error n / 2^64 cannot reach the next quotient, 1 / d away).
@@ -115,25 +108,23 @@ __device__ __forceinline__ uint32_t lr_code(const LrShape& sh, uint64_t row, con
     const uint32_t r = (uint32_t)row, s = sh.length.div(r), at = r - s * sh.length.d;
     return (at == 0 ? LR_HEAD : 0) | (at + 1 == sh.length.d ? LR_TAIL : 0) | s;
 }
-// What one lane needs of them: masks over its group's rows.
+// The codes of a warp's rows, lane r holding row r's, and masks of them.
 struct LrMarks {
     uint32_t code, head, tail, valid;
+    __device__ __forceinline__ LrMarks() : code(0), head(0), tail(0), valid(LR_ALL) {}  // all inside a sequence
     __device__ __forceinline__ explicit LrMarks(uint32_t c) : code(c) {
-        const int lane = threadIdx.x & 31, shift = lane / LR_LANES * LR_ROWS;
-        const bool mine = lane < LR_WARP_ROWS;
-        constexpr uint32_t ALL = (1u << LR_ROWS) - 1;
-        head = __ballot_sync(0xffffffffu, mine && (c & LR_HEAD)) >> shift & ALL;
-        tail = __ballot_sync(0xffffffffu, mine && (c & LR_TAIL)) >> shift & ALL;
-        valid = __ballot_sync(0xffffffffu, mine && !(c & LR_OUTSIDE)) >> shift & ALL;
+        const bool mine = (threadIdx.x & 31) < LR_ROWS;
+        head = __ballot_sync(0xffffffffu, mine && (c & LR_HEAD));
+        tail = __ballot_sync(0xffffffffu, mine && (c & LR_TAIL));
+        valid = __ballot_sync(0xffffffffu, mine && !(c & LR_OUTSIDE));
     }
-    // Sequence of the group's row r, if that is a head or tail (a call of the whole warp).
+    // Sequence of row r, which is a head or tail.
     __device__ __forceinline__ uint64_t sequence(const LrShape& sh, int r) const {
-        const uint32_t s = __shfl_sync(0xffffffffu, code, (threadIdx.x & 31) / LR_LANES * LR_ROWS + r) & LR_SEQUENCE;
-        return min((uint64_t)s, sh.sequences - 1);
+        return min((uint64_t)(__shfl_sync(0xffffffffu, code, r) & LR_SEQUENCE), sh.sequences - 1);
     }
-    // Nothing from before the group's rows passes them; nothing from behind them does.
-    __device__ __forceinline__ bool cuts() const { return head || valid != (1u << LR_ROWS) - 1; }
-    __device__ __forceinline__ bool cuts_back() const { return tail || valid != (1u << LR_ROWS) - 1; }
+    // Nothing from before the rows passes them; nothing from behind them does.
+    __device__ __forceinline__ bool cuts() const { return head || valid != LR_ALL; }
+    __device__ __forceinline__ bool cuts_back() const { return tail || valid != LR_ALL; }
 };
 
 // Number of offsets[0 .. count) that are <= row, minus 1 (-1: none); the warp narrows the range 32-fold a step.
@@ -232,60 +223,96 @@ __device__ __forceinline__ void lr_arrive(int barrier, int threads) {
 }
 
 // ---- Rows in shared memory -------------------------------------------------------
-// How rows can be copied: by 16-byte or 4-byte asynchronous copies, or element
-// by element (2-byte elements on odd addresses or strides).
-enum { LR_COPY16 = 0, LR_COPY4 = 1, LR_COPY_ELEMENT = 2 };
+// A row of a tile is 32 words of 4 bytes, one a lane: 1 float or 2 halves.  How
+// rows are copied, all asynchronously: 16 or 4 bytes at a time where rows are
+// aligned so, else (2-byte elements on odd addresses or strides) the 33 aligned
+// words around a row's elements, which the reader shifts.
+enum { LR_COPY16 = 0, LR_COPY4 = 1, LR_COPY_ODD = 2 };
 
-// One lane's part of copying a warp's rows of a column tile: constant offsets.
+// One lane's part of copying a warp's rows of a column tile.
 template <typename T, int COPY>
 struct LrFetch {
-    static constexpr int PER_ROW = COPY == LR_COPY16 ? LR_ROW_BYTES / 16 : LR_LANES;  // lanes a row
-    static constexpr int STEP = 32 / PER_ROW;                                        // rows a step
-    static constexpr int V = (COPY == LR_COPY16 ? 16 : 4) / sizeof(T);               // elements a lane
-    const char* m;       // this lane's part of the warp's first rows
+    static constexpr int PER_ROW = COPY == LR_COPY16 ? 8 : 32;          // lanes a row
+    static constexpr int STEP = 32 / PER_ROW;                           // rows a step
+    static constexpr int BYTES = COPY == LR_COPY16 ? 16 : 4;            // a copy
+    static constexpr int PITCH = COPY == LR_COPY_ODD ? 132 : 128;       // of rows in shared memory, in bytes
+    static constexpr int BUF = LR_ROWS * PITCH;                         // a warp's rows
+    const char* m;  // this lane's part of the warp's first rows
     uint64_t row_bytes;
-    __device__ __forceinline__ LrFetch(const void* matrix, uint64_t stride, int warp) {
+    const char *begin, *end;  // of the matrix (LR_COPY_ODD)
+    __device__ __forceinline__ LrFetch(const void* matrix, uint64_t stride, int warp, const LrShape& sh) {
         const int lane = threadIdx.x & 31;
         row_bytes = stride * sizeof(T);
-        m = (const char*)matrix + (warp * LR_WARP_ROWS + lane / PER_ROW) * row_bytes + lane % PER_ROW * V * sizeof(T);
-    }
-    static __device__ __forceinline__ char* at(char* buf, int r) {
-        return buf + r / LR_ROWS * LR_GROUP_BUF + r % LR_ROWS * LR_ROW_BYTES;
+        m = (const char*)matrix + (warp * LR_ROWS + lane / PER_ROW) * row_bytes + lane % PER_ROW * BYTES;
+        begin = (const char*)matrix;
+        end = begin + ((sh.rows - 1) * stride + sh.channels) * sizeof(T);
     }
     // Copies the warp's rows (n of them in range) of the tile `offset` bytes into the matrix, `channels` of whose
-    // channels are in range, to buf; what is out of range is left as it is.  Asynchronous copies are part of the
-    // warp's next commit.
+    // channels are in range, to buf; what is out of range is left as it is.  Part of the warp's next commit.
     __device__ __forceinline__ void copy(char* buf, uint64_t offset, int n, uint32_t channels) const {
-        const int lane = threadIdx.x & 31, r0 = lane / PER_ROW;
-        const uint32_t c = lane % PER_ROW * V;
+        const int lane = threadIdx.x & 31, r0 = lane / PER_ROW, at = lane % PER_ROW * BYTES;
         const uint64_t step_bytes = row_bytes * STEP;
         const char* src = m + offset;
-        if constexpr (COPY != LR_COPY_ELEMENT) {
-            char* dst = at(buf, r0) + c * sizeof(T);
-            if (c >= channels) return;
+        char* dst = buf + r0 * PITCH + at;
+        if constexpr (COPY != LR_COPY_ODD) {
+            if (at >= channels * (int)sizeof(T)) return;
 #pragma unroll
-            for (int j = 0; j < LR_WARP_ROWS / STEP; ++j, src += step_bytes) {
-                // rows r0 + j STEP of one group follow one another; STEP divides LR_ROWS or the reverse
-                char* d = dst + (STEP <= LR_ROWS ? j * STEP / LR_ROWS * LR_GROUP_BUF + j * STEP % LR_ROWS * LR_ROW_BYTES
-                                                 : j * (STEP / LR_ROWS) * LR_GROUP_BUF);
+            for (int j = 0; j < LR_ROWS / STEP; ++j, src += step_bytes)
                 if (r0 + j * STEP < n) {
-                    if constexpr (COPY == LR_COPY16) cp_async16(d, src);
-                    else cp_async4(d, src);
+                    if constexpr (COPY == LR_COPY16) cp_async16(dst + j * STEP * PITCH, src);
+                    else cp_async4(dst + j * STEP * PITCH, src);
                 }
-            }
         } else {
-            T v[LR_WARP_ROWS / STEP][V];
+            // words 0 .. 31 of the rows, a row a step, of those that hold one of its channels; then the 33rd words, a
+            // row a lane
+            const int bytes = channels * (int)sizeof(T);
+            const char* row0 = src - at;
+            const char* tail = row0 + lane * row_bytes + 128;
+            const bool tails = lane < min(n, LR_ROWS) && bytes == 128 && ((uintptr_t)tail & 2);
+            if (n >= LR_ROWS && row0 >= begin + 4 && row0 + (LR_ROWS - 1) * row_bytes + 136 <= end) {
 #pragma unroll
-            for (int j = 0; j < LR_WARP_ROWS / STEP; ++j, src += step_bytes)
-#pragma unroll
-                for (int i = 0; i < V; ++i)
-                    if (r0 + j * STEP < n && c + i < channels) v[j][i] = ((const T*)src)[i];
-#pragma unroll
-            for (int j = 0; j < LR_WARP_ROWS / STEP; ++j)
-#pragma unroll
-                for (int i = 0; i < V; ++i)
-                    if (r0 + j * STEP < n && c + i < channels) ((T*)at(buf, r0 + j * STEP))[c + i] = v[j][i];
+                for (int j = 0; j < LR_ROWS; ++j, src += step_bytes) {
+                    const int odd = (int)((uintptr_t)src & 2);
+                    if (at < bytes + odd) cp_async4(dst + j * PITCH, src - odd);
+                }
+                if (tails) cp_async4(buf + lane * PITCH + 128, tail - 2);
+            } else {
+                for (int j = 0; j < min(n, LR_ROWS); ++j, src += step_bytes) {
+                    const int odd = (int)((uintptr_t)src & 2);
+                    if (at < bytes + odd) word(dst + j * PITCH, src - odd);
+                }
+                if (tails) word(buf + lane * PITCH + 128, tail - 2);
+            }
         }
+    }
+    // One aligned word, which at the matrix's ends is half outside it.
+    __device__ __forceinline__ void word(char* dst, const char* src) const {
+        if (src >= begin && src + 4 <= end) cp_async4(dst, src);
+        else if (src >= begin) *(uint16_t*)dst = *(const uint16_t*)src;
+        else *(uint16_t*)(dst + 2) = *(const uint16_t*)(src + 2);
+    }
+};
+
+// Which of a warp's rows of a matrix start in the middle of a word (2-byte elements), as bits.
+__device__ __forceinline__ uint32_t lr_odd_rows(const void* matrix, uint64_t offset, uint64_t stride) {
+    return ((uintptr_t)matrix + offset & 2 ? 0xffu : 0u) ^ (stride & 1 ? 0xaau : 0u);  // a warp's first row is even
+}
+
+// A warp's rows of a matrix, as copied: one lane's word of row r.
+template <typename T, int COPY>
+struct LrRows {
+    const uint32_t* words;
+    uint32_t odd;  // LR_COPY_ODD: bit r: row r starts in the middle of a word
+    __device__ __forceinline__ LrRows(const char* buf, const void* matrix, uint64_t offset, uint64_t stride)
+        : words((const uint32_t*)buf + (threadIdx.x & 31)), odd(0) {
+        if constexpr (COPY == LR_COPY_ODD) {
+            odd = lr_odd_rows(matrix, offset, stride);
+        }
+    }
+    __device__ __forceinline__ uint32_t operator[](int r) const {
+        const uint32_t* w = words + r * (LrFetch<T, COPY>::PITCH / 4);
+        if constexpr (COPY == LR_COPY_ODD) return __funnelshift_r(w[0], w[1], odd >> r & 1 ? 16 : 0);
+        else return w[0];
     }
 };
 
@@ -323,23 +350,28 @@ template <> struct LrWord<__nv_bfloat16> {
         return w;
     }
 };
-// One lane's words of a matrix in shared memory: row r of its group.
-__device__ __forceinline__ const uint32_t* lr_words(const char* buf) {
-    const int lane = threadIdx.x & 31;
-    return (const uint32_t*)(buf + lane / LR_LANES * LR_GROUP_BUF) + lane % LR_LANES;
-}
-constexpr int LR_ROW_WORDS = LR_ROW_BYTES / 4;
-// Stores one lane's channels, `left` of them in range.
+// Stores one row, a lane its channels, `left` of them (if positive) in range.  A call of the whole warp; odd
+// (LR_COPY_ODD): the row starts in the middle of a word, so that a lane's second and the next lane's first channel
+// share one.
 template <typename T, int COPY>
-__device__ __forceinline__ void lr_store(T* p, const float* v, int left) {
-    if constexpr (sizeof(T) == 4 || COPY != LR_COPY_ELEMENT) {
-        if (left > 0) *(uint32_t*)p = LrWord<T>::narrow(v);
+__device__ __forceinline__ void lr_store(T* p, const float* v, int left, bool odd) {
+    const uint32_t w = LrWord<T>::narrow(v);
+    if constexpr (COPY != LR_COPY_ODD) {
+        if (left > 0) *(uint32_t*)p = w;
     } else {
-        if (left > 0) p[0] = narrow<T>(v[0]);
-        if (left > 1) p[1] = narrow<T>(v[1]);
+        const uint32_t next = __shfl_down_sync(0xffffffffu, w, 1);
+        const int lane = threadIdx.x & 31;
+        uint16_t* h = (uint16_t*)p;
+        if (odd) {
+            if (lane == 0 && left > 0) h[0] = (uint16_t)w;
+            if (left > 2 && lane < 31) *(uint32_t*)(h + 1) = __funnelshift_r(w, next, 16);
+            else if (left > 1) h[1] = (uint16_t)(w >> 16);
+        } else {
+            if (left > 1) *(uint32_t*)h = w;
+            else if (left > 0) h[0] = (uint16_t)w;
+        }
     }
 }
-
 // Whether row is the first of a sequence, or outside (nothing passes it from before).
 __device__ __forceinline__ bool lr_starts(const LrShape& sh, const uint32_t* codes, uint64_t row) {
     return lr_code(sh, row, codes + row) & (LR_HEAD | LR_OUTSIDE);
@@ -390,9 +422,9 @@ __device__ __forceinline__ void lr_slot(LrSlot& slot, const LrShape& sh, uint64_
     const int lane = threadIdx.x & 31;
     bool plain = false;
     if (!sh.offsets && lane < LR_WARPS) {
-        const uint64_t first = row + lane * LR_WARP_ROWS;
+        const uint64_t first = row + lane * LR_ROWS;
         const uint32_t r = (uint32_t)first, at = r - sh.length.div(r) * sh.length.d;
-        plain = at > 0 && at + LR_WARP_ROWS < sh.length.d && first + LR_WARP_ROWS <= sh.rows;
+        plain = at > 0 && at + LR_ROWS < sh.length.d && first + LR_ROWS <= sh.rows;
     }
     const uint32_t bits = __ballot_sync(0xffffffffu, plain);
     if (lane == 0) {
@@ -408,18 +440,17 @@ __device__ __forceinline__ void lr_slot(LrSlot& slot, const LrShape& sh, uint64_
 // ---- Forward ---------------------------------------------------------------------
 template <typename T>
 struct LrConfig {
-    static constexpr int N = LrWord<T>::N;       // channels a lane
-    static constexpr int C = LR_LANES * N;       // channels of a tile
-    static constexpr int HELPERS = (C + 31) / 32;  // publishing warps, and look-back warps
-    static constexpr int THREADS = (LR_WARPS + 2 * HELPERS) * 32;
-    static constexpr int MAPPED = THREADS - 32 * HELPERS;  // of a barrier that the compute warps and one kind share
+    static constexpr int N = LrWord<T>::N;                 // channels a lane; publishing warps, and look-back warps
+    static constexpr int C = 32 * N;                       // channels of a tile
+    static constexpr int THREADS = (LR_WARPS + 2 * N) * 32;
+    static constexpr int MAPPED = THREADS - 32 * N;        // of a barrier of the compute warps and one kind of helpers
 };
 
-template <typename T>
+template <typename T, int COPY>
 struct LrForwardSmem {
     static constexpr int STAGES = 4, C = LrConfig<T>::C;
-    char rows[STAGES][LR_WARPS][2][LR_WARP_BUF];  // gate, in
-    uint32_t code[STAGES][LR_WARPS][LR_WARP_ROWS];
+    char rows[STAGES][LR_WARPS][2][LrFetch<T, COPY>::BUF];  // gate, in
+    uint32_t code[STAGES][LR_WARPS][LR_ROWS];
     float2 map[2][LR_WARPS][C];  // (A, H) of a warp's rows
     float start[2][LR_WARPS][C];
     uint32_t cut[2][LR_WARPS];   // nothing from before a warp's rows passes them
@@ -429,7 +460,7 @@ struct LrForwardSmem {
 template <typename T, int GATE, int COPY>
 __global__ void __launch_bounds__(LrConfig<T>::THREADS, 1) lr_forward_kernel(LrForward p, LrChain ch, LrTiles tl) {
     using Config = LrConfig<T>;
-    using Smem = LrForwardSmem<T>;
+    using Smem = LrForwardSmem<T, COPY>;
     constexpr int N = Config::N, C = Config::C;
     static_assert(Smem::STAGES + 2 <= LR_AHEAD, "tile i + STAGES is fetched after the starts of tile i - 2");
     extern __shared__ __align__(128) char smem_raw[];
@@ -447,15 +478,14 @@ __global__ void __launch_bounds__(LrConfig<T>::THREADS, 1) lr_forward_kernel(LrF
     __syncthreads();
 
     if (warp >= LR_WARPS) {
-        const bool publishes = warp >= LR_WARPS + Config::HELPERS;
-        const int cc = min((warp - LR_WARPS) % Config::HELPERS * 32 + lane, C - 1);  // a channel a lane
-        const bool lanes = (warp - LR_WARPS) % Config::HELPERS * 32 + lane < C;
+        const bool publishes = warp >= LR_WARPS + N;
+        const int cc = (warp - LR_WARPS) % N * 32 + lane;
         for (uint32_t i = 0; i < count; ++i) {
             const int b = i & 1;
             const uint2 t = tl.tile(i);
             const uint32_t k = t.x, c = t.y * C + cc;
             float4* record = ch.record + (uint64_t)k * ch.width + c;
-            const bool active = lanes && c < channels, more = active && k + 1 < tl.row_tiles;
+            const bool active = c < channels, more = active && k + 1 < tl.row_tiles;
             float carry = 0.0f;
             if (!publishes && k > 0 && !lr_starts(p.sh, tl.codes, (uint64_t)k * LR_TILE)) {
                 const int64_t step = -(int64_t)ch.width;
@@ -477,16 +507,14 @@ __global__ void __launch_bounds__(LrConfig<T>::THREADS, 1) lr_forward_kernel(LrF
                     if (cuts || k == 0) lr_put_state(record, H);
                     else lr_put_map(record, A, H);
                 }
-                if (warp == LR_WARPS + Config::HELPERS) slot(i + LR_AHEAD);
+                if (warp == LR_WARPS + N) slot(i + LR_AHEAD);
             } else {
                 if (more && !cuts && k > 0) lr_put_state(record, fmaf(A, carry, H));
                 if (p.saved && active) p.saved[(uint64_t)k * channels + c] = carry;
-                if (lanes) {
 #pragma unroll
-                    for (int w = 0; w < LR_WARPS; ++w) {
-                        sm.start[b][w][cc] = carry;
-                        carry = cuts >> w & 1 ? h[w] : fmaf(a[w], carry, h[w]);
-                    }
+                for (int w = 0; w < LR_WARPS; ++w) {
+                    sm.start[b][w][cc] = carry;
+                    carry = cuts >> w & 1 ? h[w] : fmaf(a[w], carry, h[w]);
                 }
             }
             lr_arrive(3 + b, Config::THREADS);
@@ -494,18 +522,18 @@ __global__ void __launch_bounds__(LrConfig<T>::THREADS, 1) lr_forward_kernel(LrF
         return;
     }
 
-    const int group = lane / LR_LANES, column = lane % LR_LANES * N;
-    const LrFetch<T, COPY> fetch_gate(p.gate, p.gate_stride, warp), fetch_in(p.in, p.in_stride, warp);
-    T* const out0 = (T*)p.out + (uint64_t)(warp * LR_WARP_ROWS + group * LR_ROWS) * p.out_stride + column;
+    const int column = lane * N;
+    const LrFetch<T, COPY> fetch_gate(p.gate, p.gate_stride, warp, p.sh), fetch_in(p.in, p.in_stride, warp, p.sh);
+    T* const out0 = (T*)p.out + (uint64_t)(warp * LR_ROWS) * p.out_stride + column;
     auto fetch = [&](uint32_t i) {
         if (i < count) {
             const uint32_t st = i % Smem::STAGES;
             const LrSlot& sl = sm.slot[i % LR_SLOTS];
-            const int n = (int)sl.rows - warp * LR_WARP_ROWS;
+            const int n = (int)sl.rows - warp * LR_ROWS;
             fetch_gate.copy(sm.rows[st][warp][0], sl.offset[0], n, sl.channels);
             fetch_in.copy(sm.rows[st][warp][1], sl.offset[1], n, sl.channels);
-            if (p.sh.offsets && lane < min(n, LR_WARP_ROWS))
-                cp_async4(&sm.code[st][warp][lane], tl.codes + sl.row + warp * LR_WARP_ROWS + lane);
+            if (p.sh.offsets && lane < min(n, LR_ROWS))
+                cp_async4(&sm.code[st][warp][lane], tl.codes + sl.row + warp * LR_ROWS + lane);
         }
         cp_async_commit();
     };
@@ -513,7 +541,7 @@ __global__ void __launch_bounds__(LrConfig<T>::THREADS, 1) lr_forward_kernel(LrF
     auto codes = [&](const LrSlot& sl, uint32_t st, bool* plain) -> uint32_t {
         *plain = sl.plain >> warp & 1;
         if (*plain) return 0;
-        const uint32_t code = lane < LR_WARP_ROWS ? lr_code(p.sh, (uint64_t)sl.row + warp * LR_WARP_ROWS + lane,
+        const uint32_t code = lane < LR_ROWS ? lr_code(p.sh, (uint64_t)sl.row + warp * LR_ROWS + lane,
                                                             &sm.code[st][warp][lane]) : 0;
         *plain = !__any_sync(0xffffffffu, code & (LR_OUTSIDE | LR_HEAD | LR_TAIL));
         return code;
@@ -529,17 +557,17 @@ __global__ void __launch_bounds__(LrConfig<T>::THREADS, 1) lr_forward_kernel(LrF
         cp_async_wait_prior<Smem::STAGES - 1>();
         __syncwarp();
         w.code = codes(sl, st, &w.plain);
-        const uint32_t *gate = lr_words(sm.rows[st][warp][0]), *in = lr_words(sm.rows[st][warp][1]);
+        const LrRows<T, COPY> gate(sm.rows[st][warp][0], p.gate, sl.offset[0], p.gate_stride),
+            in(sm.rows[st][warp][1], p.in, sl.offset[1], p.in_stride);
         float A[N], H[N];
 #pragma unroll
         for (int i = 0; i < N; ++i) A[i] = 1.0f, H[i] = 0.0f;
-        bool cuts = false;
         if (w.plain) {
 #pragma unroll
             for (int r = 0; r < LR_ROWS; ++r) {
                 float g[N], x[N];
-                LrWord<T>::widen(gate[r * LR_ROW_WORDS], g);
-                LrWord<T>::widen(in[r * LR_ROW_WORDS], x);
+                LrWord<T>::widen(gate[r], g);
+                LrWord<T>::widen(in[r], x);
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
                     const Gate<GATE> gt(g[i]);
@@ -551,12 +579,11 @@ __global__ void __launch_bounds__(LrConfig<T>::THREADS, 1) lr_forward_kernel(LrF
         } else {
             const LrMarks m(w.code);
             const uint32_t c = sl.channel + column;
-            cuts = m.cuts();
 #pragma unroll
             for (int r = 0; r < LR_ROWS; ++r) {
                 float g[N], x[N];
-                LrWord<T>::widen(gate[r * LR_ROW_WORDS], g);
-                LrWord<T>::widen(in[r * LR_ROW_WORDS], x);
+                LrWord<T>::widen(gate[r], g);
+                LrWord<T>::widen(in[r], x);
                 const uint64_t s = m.sequence(p.sh, r);
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
@@ -572,26 +599,10 @@ __global__ void __launch_bounds__(LrConfig<T>::THREADS, 1) lr_forward_kernel(LrF
                 }
             }
         }
-        // the groups' maps one after the other are the warp's
         const int b = i & 1;
-        bool any = cuts;
 #pragma unroll
-        for (int s = 1; s < LR_GROUPS; ++s) {
-            const bool cut = __shfl_down_sync(0xffffffffu, cuts, s * LR_LANES);
-            any |= cut;
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-                const float a = __shfl_down_sync(0xffffffffu, w.pre[LR_ROWS - 1][i], s * LR_LANES);
-                const float h = __shfl_down_sync(0xffffffffu, w.loc[LR_ROWS - 1][i], s * LR_LANES);
-                H[i] = cut ? h : fmaf(a, H[i], h);
-                A[i] *= a;
-            }
-        }
-        if (group == 0) {
-#pragma unroll
-            for (int i = 0; i < N; ++i) sm.map[b][warp][column + i] = make_float2(A[i], H[i]);
-            if (lane == 0) sm.cut[b][warp] = any;
-        }
+        for (int i = 0; i < N; ++i) sm.map[b][warp][column + i] = make_float2(A[i], H[i]);
+        if (lane == 0) sm.cut[b][warp] = !w.plain;
         lr_arrive(1 + b, Config::MAPPED);
         lr_arrive(5 + b, Config::MAPPED);
         __syncwarp();  // the stage is read
@@ -602,49 +613,33 @@ __global__ void __launch_bounds__(LrConfig<T>::THREADS, 1) lr_forward_kernel(LrF
         const LrSlot& sl = sm.slot[i % LR_SLOTS];
         const int left = (int)sl.channels - column;
         T* out = (T*)((char*)out0 + sl.offset[2]);
+        const uint32_t odd = COPY == LR_COPY_ODD ? lr_odd_rows(p.out, sl.offset[2], p.out_stride) : 0;
         float start[N];
         lr_sync(3 + b, Config::THREADS);
 #pragma unroll
         for (int i = 0; i < N; ++i) start[i] = sm.start[b][warp][column + i];
         if (w.plain) {
 #pragma unroll
-            for (int s = 1; s < LR_GROUPS; ++s)
-#pragma unroll
-                for (int i = 0; i < N; ++i) {
-                    const float behind = fmaf(w.pre[LR_ROWS - 1][i], start[i], w.loc[LR_ROWS - 1][i]);
-                    const float up = __shfl_up_sync(0xffffffffu, behind, LR_LANES);
-                    if (group == s) start[i] = up;
-                }
-#pragma unroll
             for (int r = 0; r < LR_ROWS; ++r, out += p.out_stride) {
                 float h[N];
 #pragma unroll
                 for (int i = 0; i < N; ++i) h[i] = fmaf(w.pre[r][i], start[i], w.loc[r][i]);
-                lr_store<T, COPY>(out, h, left);
+                lr_store<T, COPY>(out, h, left, odd >> r & 1);
             }
             return;
         }
-        // From the first head or outside row on nothing depends on the state before the group's rows (not even as 0
+        // From the first head or outside row on nothing depends on the state before the warp's rows (not even as 0
         // times it, which an infinity or NaN of another sequence would survive).
         const LrMarks m(w.code);
         const uint32_t c = sl.channel + column;
-        const int rows = (int)sl.rows - warp * LR_WARP_ROWS - group * LR_ROWS;
+        const int rows = (int)sl.rows - warp * LR_ROWS;
         const int reach = __ffs(m.head | ~m.valid) - 1;
-#pragma unroll
-        for (int s = 1; s < LR_GROUPS; ++s)
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-                const float loc = w.loc[LR_ROWS - 1][i];
-                const float behind = reach < LR_ROWS ? loc : fmaf(w.pre[LR_ROWS - 1][i], start[i], loc);
-                const float up = __shfl_up_sync(0xffffffffu, behind, LR_LANES);
-                if (group == s) start[i] = up;
-            }
 #pragma unroll
         for (int r = 0; r < LR_ROWS; ++r, out += p.out_stride) {
             float h[N];
 #pragma unroll
             for (int i = 0; i < N; ++i) h[i] = r < reach ? fmaf(w.pre[r][i], start[i], w.loc[r][i]) : w.loc[r][i];
-            if (r < rows) lr_store<T, COPY>(out, h, left);
+            if (r < rows) lr_store<T, COPY>(out, h, left, odd >> r & 1);
             const uint64_t s = m.sequence(p.sh, r);
             if ((m.tail >> r & 1) && p.last) {
 #pragma unroll
@@ -668,15 +663,14 @@ __global__ void __launch_bounds__(LrConfig<T>::THREADS, 1) lr_forward_kernel(LrF
 
 // ---- Backward --------------------------------------------------------------------
 // Tiles from the last to the first: the chain carries mu, mu_before = A mu_behind + M.
-template <typename T>
+template <typename T, int COPY>
 struct LrBackwardSmem {
-    static constexpr int STAGES = 3, C = LrConfig<T>::C, N = LrConfig<T>::N;
-    char rows[STAGES][LR_WARPS][3][LR_WARP_BUF];  // gate, in, grad_out
-    uint32_t code[STAGES][LR_WARPS][LR_WARP_ROWS];
+    static constexpr int STAGES = 3, C = LrConfig<T>::C;
+    char rows[STAGES][LR_WARPS][3][LrFetch<T, COPY>::BUF];  // gate, in, grad_out
+    uint32_t code[STAGES][LR_WARPS][LR_ROWS];
     float2 map[2][LR_WARPS][C];                   // (A, H) of a warp's rows, and M
     float grad_map[2][LR_WARPS][C];
     float start[2][LR_WARPS][C], grad_start[2][LR_WARPS][C];
-    float group[2][LR_WARPS][3 * N][32];          // (A, H, M) of a group's rows, a lane's own
     // bit 0: no state from before a warp's rows passes them; bit 1: no gradient from behind them does
     uint32_t cut[2][LR_WARPS];
     LrSlot slot[LR_SLOTS];
@@ -685,7 +679,7 @@ struct LrBackwardSmem {
 template <typename T, int GATE, int COPY>
 __global__ void __launch_bounds__(LrConfig<T>::THREADS, 1) lr_backward_kernel(LrBackward p, LrChain ch, LrTiles tl) {
     using Config = LrConfig<T>;
-    using Smem = LrBackwardSmem<T>;
+    using Smem = LrBackwardSmem<T, COPY>;
     constexpr int N = Config::N, C = Config::C;
     static_assert(Smem::STAGES <= LR_AHEAD, "tile i + STAGES is fetched after the starts of tile i");
     extern __shared__ __align__(128) char smem_raw[];
@@ -704,15 +698,14 @@ __global__ void __launch_bounds__(LrConfig<T>::THREADS, 1) lr_backward_kernel(Lr
     __syncthreads();
 
     if (warp >= LR_WARPS) {
-        const bool publishes = warp >= LR_WARPS + Config::HELPERS;
-        const int cc = min((warp - LR_WARPS) % Config::HELPERS * 32 + lane, C - 1);  // a channel a lane
-        const bool lanes = (warp - LR_WARPS) % Config::HELPERS * 32 + lane < C;
+        const bool publishes = warp >= LR_WARPS + N;
+        const int cc = (warp - LR_WARPS) % N * 32 + lane;
         for (uint32_t i = 0; i < count; ++i) {
             const int b = i & 1;
             const uint2 t = tl.tile(i);
             const uint32_t k = row_tile(t), c = t.y * C + cc;
             float4* record = ch.record + (uint64_t)k * ch.width + c;
-            const bool active = lanes && c < channels, more = active && k > 0, chained = k + 1 < tl.row_tiles;
+            const bool active = c < channels, more = active && k > 0, chained = k + 1 < tl.row_tiles;
             // the publishing warps also carry the states on, from the saved one
             float carry = 0.0f, state = publishes && active ? p.saved[(uint64_t)k * channels + c] : 0.0f;
             if (!publishes && chained && !lr_ends(p.sh, tl.codes, (uint64_t)(k + 1) * LR_TILE - 1)) {
@@ -734,24 +727,20 @@ __global__ void __launch_bounds__(LrConfig<T>::THREADS, 1) lr_backward_kernel(Lr
                     if (cuts || !chained) lr_put_state(record, M);
                     else lr_put_map(record, A, M);
                 }
-                if (warp == LR_WARPS + Config::HELPERS) slot(i + LR_AHEAD);
+                if (warp == LR_WARPS + N) slot(i + LR_AHEAD);
                 const uint32_t heads = lr_cuts(sm.cut[b], 1);
-                if (lanes) {
 #pragma unroll
-                    for (int w = 0; w < LR_WARPS; ++w) {
-                        sm.start[b][w][cc] = state;
-                        const float h = sm.map[b][w][cc].y;
-                        state = heads >> w & 1 ? h : fmaf(a[w], state, h);
-                    }
+                for (int w = 0; w < LR_WARPS; ++w) {
+                    sm.start[b][w][cc] = state;
+                    const float h = sm.map[b][w][cc].y;
+                    state = heads >> w & 1 ? h : fmaf(a[w], state, h);
                 }
             } else {
                 if (more && !cuts && chained) lr_put_state(record, fmaf(A, carry, M));
-                if (lanes) {
 #pragma unroll
-                    for (int w = LR_WARPS - 1; w >= 0; --w) {
-                        sm.grad_start[b][w][cc] = carry;
-                        carry = cuts >> w & 1 ? v[w] : fmaf(a[w], carry, v[w]);
-                    }
+                for (int w = LR_WARPS - 1; w >= 0; --w) {
+                    sm.grad_start[b][w][cc] = carry;
+                    carry = cuts >> w & 1 ? v[w] : fmaf(a[w], carry, v[w]);
                 }
             }
             lr_arrive(3 + b, Config::THREADS);
@@ -759,22 +748,22 @@ __global__ void __launch_bounds__(LrConfig<T>::THREADS, 1) lr_backward_kernel(Lr
         return;
     }
 
-    const int group = lane / LR_LANES, column = lane % LR_LANES * N;
-    const LrFetch<T, COPY> fetch_gate(p.gate, p.gate_stride, warp), fetch_in(p.in, p.in_stride, warp),
-        fetch_grad(p.grad_out, p.grad_out_stride, warp);
-    const uint64_t bottom = warp * LR_WARP_ROWS + group * LR_ROWS + LR_ROWS - 1;  // the group's last row
+    const int column = lane * N;
+    const LrFetch<T, COPY> fetch_gate(p.gate, p.gate_stride, warp, p.sh), fetch_in(p.in, p.in_stride, warp, p.sh),
+        fetch_grad(p.grad_out, p.grad_out_stride, warp, p.sh);
+    const uint64_t bottom = warp * LR_ROWS + LR_ROWS - 1;  // the warp's last row
     T* const out_gate0 = (T*)p.grad_gate + bottom * p.grad_gate_stride + column;
     T* const out_in0 = (T*)p.grad_in + bottom * p.grad_in_stride + column;
     auto fetch = [&](uint32_t i) {
         if (i < count) {
             const uint32_t st = i % Smem::STAGES;
             const LrSlot& sl = sm.slot[i % LR_SLOTS];
-            const int n = (int)sl.rows - warp * LR_WARP_ROWS;
+            const int n = (int)sl.rows - warp * LR_ROWS;
             fetch_gate.copy(sm.rows[st][warp][0], sl.offset[0], n, sl.channels);
             fetch_in.copy(sm.rows[st][warp][1], sl.offset[1], n, sl.channels);
             if (p.grad_out) fetch_grad.copy(sm.rows[st][warp][2], sl.offset[2], n, sl.channels);
-            if (p.sh.offsets && lane < min(n, LR_WARP_ROWS))
-                cp_async4(&sm.code[st][warp][lane], tl.codes + sl.row + warp * LR_WARP_ROWS + lane);
+            if (p.sh.offsets && lane < min(n, LR_ROWS))
+                cp_async4(&sm.code[st][warp][lane], tl.codes + sl.row + warp * LR_ROWS + lane);
         }
         cp_async_commit();
     };
@@ -782,14 +771,14 @@ __global__ void __launch_bounds__(LrConfig<T>::THREADS, 1) lr_backward_kernel(Lr
     auto codes = [&](const LrSlot& sl, uint32_t st, bool* plain) -> uint32_t {
         *plain = sl.plain >> warp & 1;
         if (*plain) return 0;
-        const uint32_t code = lane < LR_WARP_ROWS ? lr_code(p.sh, (uint64_t)sl.row + warp * LR_WARP_ROWS + lane,
+        const uint32_t code = lane < LR_ROWS ? lr_code(p.sh, (uint64_t)sl.row + warp * LR_ROWS + lane,
                                                             &sm.code[st][warp][lane]) : 0;
         *plain = !__any_sync(0xffffffffu, code & (LR_OUTSIDE | LR_HEAD | LR_TAIL));
         return code;
     };
     if (!p.grad_out) {  // zeros that stay
         for (int st = 0; st < Smem::STAGES; ++st)
-            for (int j = lane; j < LR_WARP_BUF / 4; j += 32) ((uint32_t*)sm.rows[st][warp][2])[j] = 0;
+            for (int j = lane; j < LrFetch<T, COPY>::BUF / 4; j += 32) ((uint32_t*)sm.rows[st][warp][2])[j] = 0;
         __syncwarp();
     }
     auto maps = [&](uint32_t i) {
@@ -799,8 +788,9 @@ __global__ void __launch_bounds__(LrConfig<T>::THREADS, 1) lr_backward_kernel(Lr
         __syncwarp();
         bool plain;
         const uint32_t code = codes(sl, st, &plain);
-        const uint32_t *gate = lr_words(sm.rows[st][warp][0]), *in = lr_words(sm.rows[st][warp][1]),
-                       *grad = lr_words(sm.rows[st][warp][2]);
+        const LrRows<T, COPY> gate(sm.rows[st][warp][0], p.gate, sl.offset[0], p.gate_stride),
+            in(sm.rows[st][warp][1], p.in, sl.offset[1], p.in_stride),
+            grad(sm.rows[st][warp][2], p.grad_out, sl.offset[2], p.grad_out_stride);
         float A[N], H[N], M[N];
 #pragma unroll
         for (int i = 0; i < N; ++i) A[i] = 1.0f, H[i] = 0.0f, M[i] = 0.0f;
@@ -810,8 +800,8 @@ __global__ void __launch_bounds__(LrConfig<T>::THREADS, 1) lr_backward_kernel(Lr
 #pragma unroll
             for (int r = 0; r < LR_ROWS; ++r) {
                 float g[N], x[N];
-                LrWord<T>::widen(gate[r * LR_ROW_WORDS], g);
-                LrWord<T>::widen(in[r * LR_ROW_WORDS], x);
+                LrWord<T>::widen(gate[r], g);
+                LrWord<T>::widen(in[r], x);
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
                     const Gate<GATE> gt(g[i]);
@@ -823,7 +813,7 @@ __global__ void __launch_bounds__(LrConfig<T>::THREADS, 1) lr_backward_kernel(Lr
 #pragma unroll
             for (int r = LR_ROWS - 1; r >= 0; --r) {
                 float v[N];
-                LrWord<T>::widen(grad[r * LR_ROW_WORDS], v);
+                LrWord<T>::widen(grad[r], v);
 #pragma unroll
                 for (int i = 0; i < N; ++i) M[i] = a[r][i] * (v[i] + M[i]);
             }
@@ -835,8 +825,8 @@ __global__ void __launch_bounds__(LrConfig<T>::THREADS, 1) lr_backward_kernel(Lr
 #pragma unroll
             for (int r = 0; r < LR_ROWS; ++r) {
                 float g[N], x[N];
-                LrWord<T>::widen(gate[r * LR_ROW_WORDS], g);
-                LrWord<T>::widen(in[r * LR_ROW_WORDS], x);
+                LrWord<T>::widen(gate[r], g);
+                LrWord<T>::widen(in[r], x);
                 const uint64_t s = m.sequence(p.sh, r);
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
@@ -850,7 +840,7 @@ __global__ void __launch_bounds__(LrConfig<T>::THREADS, 1) lr_backward_kernel(Lr
 #pragma unroll
             for (int r = LR_ROWS - 1; r >= 0; --r) {
                 float v[N];
-                LrWord<T>::widen(grad[r * LR_ROW_WORDS], v);
+                LrWord<T>::widen(grad[r], v);
                 const uint64_t s = m.sequence(p.sh, r);
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
@@ -860,51 +850,12 @@ __global__ void __launch_bounds__(LrConfig<T>::THREADS, 1) lr_backward_kernel(Lr
             }
         }
         const int b = i & 1;
-        bool any = cuts, any_back = cuts_back;
-        if constexpr (LR_GROUPS > 1) {
-            float a[N], h[N], m[N];
 #pragma unroll
-            for (int i = 0; i < N; ++i) {
-                a[i] = A[i], h[i] = H[i], m[i] = M[i];
-                sm.group[b][warp][i][lane] = A[i];
-                sm.group[b][warp][N + i][lane] = H[i];
-                sm.group[b][warp][2 * N + i][lane] = M[i];
-            }
-            // states go down the groups, gradients up
-#pragma unroll
-            for (int s = 1; s < LR_GROUPS; ++s) {
-                const bool cut = __shfl_down_sync(0xffffffffu, cuts, s * LR_LANES);
-                any |= cut;
-#pragma unroll
-                for (int i = 0; i < N; ++i) {
-                    const float as = __shfl_down_sync(0xffffffffu, a[i], s * LR_LANES);
-                    const float hs = __shfl_down_sync(0xffffffffu, h[i], s * LR_LANES);
-                    H[i] = cut ? hs : fmaf(as, H[i], hs);
-                    A[i] *= as;
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < N; ++i) M[i] = 0.0f;
-#pragma unroll
-            for (int s = LR_GROUPS - 1; s >= 0; --s) {
-                const bool cut = __shfl_down_sync(0xffffffffu, cuts_back, s * LR_LANES);
-                any_back |= cut;
-#pragma unroll
-                for (int i = 0; i < N; ++i) {
-                    const float as = __shfl_down_sync(0xffffffffu, a[i], s * LR_LANES);
-                    const float ms = __shfl_down_sync(0xffffffffu, m[i], s * LR_LANES);
-                    M[i] = cut ? ms : fmaf(as, M[i], ms);
-                }
-            }
+        for (int i = 0; i < N; ++i) {
+            sm.map[b][warp][column + i] = make_float2(A[i], H[i]);
+            sm.grad_map[b][warp][column + i] = M[i];
         }
-        if (group == 0) {
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-                sm.map[b][warp][column + i] = make_float2(A[i], H[i]);
-                sm.grad_map[b][warp][column + i] = M[i];
-            }
-            if (lane == 0) sm.cut[b][warp] = (any ? 1u : 0u) | (any_back ? 2u : 0u);
-        }
+        if (lane == 0) sm.cut[b][warp] = (cuts ? 1u : 0u) | (cuts_back ? 2u : 0u);
         lr_arrive(1 + b, Config::MAPPED);
         lr_arrive(5 + b, Config::MAPPED);
     };
@@ -915,39 +866,23 @@ __global__ void __launch_bounds__(LrConfig<T>::THREADS, 1) lr_backward_kernel(Lr
         const int left = (int)sl.channels - column;
         bool plain;
         const uint32_t code = codes(sl, st, &plain);
-        const uint32_t *gate = lr_words(sm.rows[st][warp][0]), *in = lr_words(sm.rows[st][warp][1]),
-                       *grad = lr_words(sm.rows[st][warp][2]);
+        const LrRows<T, COPY> gate(sm.rows[st][warp][0], p.gate, sl.offset[0], p.gate_stride),
+            in(sm.rows[st][warp][1], p.in, sl.offset[1], p.in_stride),
+            grad(sm.rows[st][warp][2], p.grad_out, sl.offset[2], p.grad_out_stride);
         T* out_gate = (T*)((char*)out_gate0 + sl.offset[3]);
         T* out_in = (T*)((char*)out_in0 + sl.offset[4]);
+        const uint32_t odd_gate = COPY == LR_COPY_ODD ? lr_odd_rows(p.grad_gate, sl.offset[3], p.grad_gate_stride) : 0;
+        const uint32_t odd_in = COPY == LR_COPY_ODD ? lr_odd_rows(p.grad_in, sl.offset[4], p.grad_in_stride) : 0;
         float h[N], mu[N], a[LR_ROWS][N], na[LR_ROWS][N], dgate[LR_ROWS][N];  // dgate: of the gate, per unit of lam
         lr_sync(3 + b, Config::THREADS);
 #pragma unroll
         for (int i = 0; i < N; ++i) h[i] = sm.start[b][warp][column + i], mu[i] = sm.grad_start[b][warp][column + i];
-        // the groups' starts, from the group before (behind) each
-        auto starts = [&](bool cuts, bool cuts_back) {
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-                const float A = sm.group[b][warp][i][lane], H = sm.group[b][warp][N + i][lane],
-                            M = sm.group[b][warp][2 * N + i][lane];
-#pragma unroll
-                for (int s = 1; s < LR_GROUPS; ++s) {
-                    const float up = __shfl_up_sync(0xffffffffu, cuts ? H : fmaf(A, h[i], H), LR_LANES);
-                    if (group == s) h[i] = up;
-                }
-#pragma unroll
-                for (int s = LR_GROUPS - 2; s >= 0; --s) {
-                    const float down = __shfl_down_sync(0xffffffffu, cuts_back ? M : fmaf(A, mu[i], M), LR_LANES);
-                    if (group == s) mu[i] = down;
-                }
-            }
-        };
         if (plain) {
-            if constexpr (LR_GROUPS > 1) starts(false, false);
 #pragma unroll
             for (int r = 0; r < LR_ROWS; ++r) {
                 float g[N], x[N];
-                LrWord<T>::widen(gate[r * LR_ROW_WORDS], g);
-                LrWord<T>::widen(in[r * LR_ROW_WORDS], x);
+                LrWord<T>::widen(gate[r], g);
+                LrWord<T>::widen(in[r], x);
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
                     const Gate<GATE> gt(g[i]);
@@ -959,7 +894,7 @@ __global__ void __launch_bounds__(LrConfig<T>::THREADS, 1) lr_backward_kernel(Lr
 #pragma unroll
             for (int r = LR_ROWS - 1; r >= 0; --r, out_gate -= p.grad_gate_stride, out_in -= p.grad_in_stride) {
                 float v[N], dg[N], dx[N];
-                LrWord<T>::widen(grad[r * LR_ROW_WORDS], v);
+                LrWord<T>::widen(grad[r], v);
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
                     const float lam = v[i] + mu[i];
@@ -967,19 +902,18 @@ __global__ void __launch_bounds__(LrConfig<T>::THREADS, 1) lr_backward_kernel(Lr
                     dx[i] = GATE == LCPP_GATE_SIGMOID ? na[r][i] * lam : lam;
                     mu[i] = a[r][i] * lam;
                 }
-                lr_store<T, COPY>(out_gate, dg, left);
-                lr_store<T, COPY>(out_in, dx, left);
+                lr_store<T, COPY>(out_gate, dg, left, odd_gate >> r & 1);
+                lr_store<T, COPY>(out_in, dx, left, odd_in >> r & 1);
             }
         } else {
             const LrMarks m(code);
             const uint32_t c = sl.channel + column;
-            const int rows = (int)sl.rows - warp * LR_WARP_ROWS - group * LR_ROWS;
-            if constexpr (LR_GROUPS > 1) starts(m.cuts(), m.cuts_back());
+            const int rows = (int)sl.rows - warp * LR_ROWS;
 #pragma unroll
             for (int r = 0; r < LR_ROWS; ++r) {
                 float g[N], x[N];
-                LrWord<T>::widen(gate[r * LR_ROW_WORDS], g);
-                LrWord<T>::widen(in[r * LR_ROW_WORDS], x);
+                LrWord<T>::widen(gate[r], g);
+                LrWord<T>::widen(in[r], x);
                 const uint64_t s = m.sequence(p.sh, r);
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
@@ -993,7 +927,7 @@ __global__ void __launch_bounds__(LrConfig<T>::THREADS, 1) lr_backward_kernel(Lr
 #pragma unroll
             for (int r = LR_ROWS - 1; r >= 0; --r, out_gate -= p.grad_gate_stride, out_in -= p.grad_in_stride) {
                 float v[N], dg[N], dx[N];
-                LrWord<T>::widen(grad[r * LR_ROW_WORDS], v);
+                LrWord<T>::widen(grad[r], v);
                 const uint64_t s = m.sequence(p.sh, r);
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
@@ -1006,8 +940,8 @@ __global__ void __launch_bounds__(LrConfig<T>::THREADS, 1) lr_backward_kernel(Lr
                     if ((m.head >> r & 1) && p.grad_init && i < left) p.grad_init[s * channels + c + i] = mu[i];
                 }
                 if (r < rows) {
-                    lr_store<T, COPY>(out_gate, dg, left);
-                    lr_store<T, COPY>(out_in, dx, left);
+                    lr_store<T, COPY>(out_gate, dg, left, odd_gate >> r & 1);
+                    lr_store<T, COPY>(out_in, dx, left, odd_in >> r & 1);
                 }
             }
         }
@@ -1166,7 +1100,7 @@ struct LrCopy {
         bits |= (uint64_t)(uintptr_t)p | stride * e;
         return *this;
     }
-    int kind() const { return bits % 16 == 0 ? LR_COPY16 : bits % 4 == 0 ? LR_COPY4 : LR_COPY_ELEMENT; }
+    int kind() const { return bits % 16 == 0 ? LR_COPY16 : bits % 4 == 0 ? LR_COPY4 : LR_COPY_ODD; }
 };
 
 static lcpp_status lr_prepare(const LrShape& sh, void* temp, const float* from, uint64_t from_stride, float* to,
@@ -1183,13 +1117,13 @@ static lcpp_status lr_prepare(const LrShape& sh, void* temp, const float* from, 
     return check_launch();
 }
 
-template <typename T, typename Smem, typename K, typename P>
-static lcpp_status lr_launch(K kernel, const char* name, const P& p, const LrShape& sh, void* temp, cudaStream_t s) {
+template <typename T, typename K, typename P>
+static lcpp_status lr_launch(size_t smem, K kernel, const char* name, const P& p, const LrShape& sh, void* temp, cudaStream_t s) {
     const uint64_t row_tiles = ceil_div(sh.rows, LR_TILE), col_tiles = ceil_div(sh.channels, LrConfig<T>::C);
     if (row_tiles * col_tiles > 0x7fffffffull) return LCPP_ERR_INVALID_ARG;
     const uint64_t grid = min(row_tiles * col_tiles, (uint64_t)device_info().sms);
     const LrTiles tl{(uint32_t)row_tiles, LrDivisor(col_tiles), (const uint32_t*)temp, grid > 6 * col_tiles};
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(Smem)) != cudaSuccess)
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
         return LCPP_ERR_CUDA;
     cudaLaunchAttribute together{};  // tiles wait for one another
     together.id = cudaLaunchAttributeCooperative;
@@ -1197,7 +1131,7 @@ static lcpp_status lr_launch(K kernel, const char* name, const P& p, const LrSha
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)grid);
     cfg.blockDim = dim3(LrConfig<T>::THREADS);
-    cfg.dynamicSmemBytes = sizeof(Smem);
+    cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
     cfg.attrs = &together;
     cfg.numAttrs = row_tiles > 1 ? 1 : 0;
@@ -1250,10 +1184,14 @@ extern "C" lcpp_status lcpp_linear_recurrence_forward(
         constexpr int G = decltype(g)::value;
         const int copy = LrCopy(channels, sizeof(T)).add(gate_in, gate_stride, sizeof(T)).add(in, in_stride, sizeof(T))
                              .add(out, out_stride, sizeof(T)).kind();
-        auto launch = [&](auto kernel) { return lr_launch<T, LrForwardSmem<T>>(kernel, "lr_forward", p, sh, temp, s); };
-        if (copy == LR_COPY16) return launch(lr_forward_kernel<T, G, LR_COPY16>);
-        if (copy == LR_COPY4) return launch(lr_forward_kernel<T, G, LR_COPY4>);
-        return launch(lr_forward_kernel<T, G, LR_COPY_ELEMENT>);
+        auto launch = [&](auto copies, auto kernel) {
+            return lr_launch<T>(sizeof(LrForwardSmem<T, decltype(copies)::value>), kernel, "lr_forward", p, sh, temp, s);
+        };
+        if (copy == LR_COPY16) return launch(std::integral_constant<int, LR_COPY16>{}, lr_forward_kernel<T, G, LR_COPY16>);
+        if constexpr (sizeof(T) == 2) {
+            if (copy == LR_COPY_ODD) return launch(std::integral_constant<int, LR_COPY_ODD>{}, lr_forward_kernel<T, G, LR_COPY_ODD>);
+        }
+        return launch(std::integral_constant<int, LR_COPY4>{}, lr_forward_kernel<T, G, LR_COPY4>);
     });
 }
 
@@ -1287,10 +1225,14 @@ extern "C" lcpp_status lcpp_linear_recurrence_backward(
             .add(grad_gate, grad_gate_stride, sizeof(T)).add(grad_in, grad_in_stride, sizeof(T));
         if (grad_out) align.add(grad_out, grad_out_stride, sizeof(T));
         const int copy = align.kind();
-        auto launch = [&](auto kernel) { return lr_launch<T, LrBackwardSmem<T>>(kernel, "lr_backward", p, sh, temp, s); };
-        if (copy == LR_COPY16) return launch(lr_backward_kernel<T, G, LR_COPY16>);
-        if (copy == LR_COPY4) return launch(lr_backward_kernel<T, G, LR_COPY4>);
-        return launch(lr_backward_kernel<T, G, LR_COPY_ELEMENT>);
+        auto launch = [&](auto copies, auto kernel) {
+            return lr_launch<T>(sizeof(LrBackwardSmem<T, decltype(copies)::value>), kernel, "lr_backward", p, sh, temp, s);
+        };
+        if (copy == LR_COPY16) return launch(std::integral_constant<int, LR_COPY16>{}, lr_backward_kernel<T, G, LR_COPY16>);
+        if constexpr (sizeof(T) == 2) {
+            if (copy == LR_COPY_ODD) return launch(std::integral_constant<int, LR_COPY_ODD>{}, lr_backward_kernel<T, G, LR_COPY_ODD>);
+        }
+        return launch(std::integral_constant<int, LR_COPY4>{}, lr_backward_kernel<T, G, LR_COPY4>);
     });
 }
 
