@@ -437,6 +437,9 @@ __device__ __forceinline__ void lr_slot(LrSlot& slot, const LrShape& sh, uint64_
     }
 }
 
+// The kernels are launched while lr_prepare_kernel runs: what reads the rows' codes or touches records waits for it.
+__device__ __forceinline__ void lr_prepared() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // ---- Forward ---------------------------------------------------------------------
 template <typename T>
 struct LrConfig {
@@ -466,6 +469,7 @@ __global__ void __launch_bounds__(LrConfig<T>::THREADS, 1) lr_forward_kernel(LrF
     extern __shared__ __align__(128) char smem_raw[];
     Smem& sm = *(Smem*)smem_raw;
     const int lane = threadIdx.x & 31, warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
+    if (p.sh.offsets || warp >= LR_WARPS) lr_prepared();
     const uint32_t channels = (uint32_t)p.sh.channels, count = tl.count();
 
     const uint64_t strides[3] = {p.gate_stride, p.in_stride, p.out_stride};
@@ -685,6 +689,7 @@ __global__ void __launch_bounds__(LrConfig<T>::THREADS, 1) lr_backward_kernel(Lr
     extern __shared__ __align__(128) char smem_raw[];
     Smem& sm = *(Smem*)smem_raw;
     const int lane = threadIdx.x & 31, warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
+    if (p.sh.offsets || warp >= LR_WARPS) lr_prepared();
     const uint32_t channels = (uint32_t)p.sh.channels, count = tl.count();
     auto row_tile = [&](uint2 t) { return tl.row_tiles - 1 - t.x; };
 
@@ -965,6 +970,7 @@ __global__ void __launch_bounds__(LrConfig<T>::THREADS, 1) lr_backward_kernel(Lr
 __global__ void __launch_bounds__(128)
 lr_prepare_kernel(uint4* words, uint64_t count, uint32_t* codes, LrShape sh, const float* from, uint64_t from_stride, float* to) {
     __shared__ uint32_t s_code[4][LR_TILE];
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     for (uint64_t i = (uint64_t)blockIdx.x * 128 + threadIdx.x; i < count; i += (uint64_t)gridDim.x * 128)
         words[i] = make_uint4(LR_NONE, LR_NONE, LR_NONE, LR_NONE);
@@ -1104,10 +1110,11 @@ struct LrCopy {
 };
 
 static lcpp_status lr_prepare(const LrShape& sh, void* temp, const float* from, uint64_t from_stride, float* to,
-                              cudaStream_t s) {
+                              bool* prepared, cudaStream_t s) {
     const uint64_t words = lr_chain_bytes(sh.rows, sh.channels) / 16;
     if (!sh.offsets && sh.length.d) to = nullptr;  // no sequence is empty
-    if (!words && !to && !sh.offsets) return LCPP_OK;
+    *prepared = words || to || sh.offsets;
+    if (!*prepared) return LCPP_OK;
     uint64_t grid = max(ceil_div(words, 128 * 4), to ? min(sh.sequences, (uint64_t)1024) : 1);
     if (sh.offsets) grid = max(grid, ceil_div(ceil_div(sh.rows, LR_TILE), 4));
     ProfScope prof("lr_prepare", s);
@@ -1118,23 +1125,26 @@ static lcpp_status lr_prepare(const LrShape& sh, void* temp, const float* from, 
 }
 
 template <typename T, typename K, typename P>
-static lcpp_status lr_launch(size_t smem, K kernel, const char* name, const P& p, const LrShape& sh, void* temp, cudaStream_t s) {
+static lcpp_status lr_launch(size_t smem, K kernel, const char* name, const P& p, const LrShape& sh, void* temp, bool prepared,
+                             cudaStream_t s) {
     const uint64_t row_tiles = ceil_div(sh.rows, LR_TILE), col_tiles = ceil_div(sh.channels, LrConfig<T>::C);
     if (row_tiles * col_tiles > 0x7fffffffull) return LCPP_ERR_INVALID_ARG;
     const uint64_t grid = min(row_tiles * col_tiles, (uint64_t)device_info().sms);
     const LrTiles tl{(uint32_t)row_tiles, LrDivisor(col_tiles), (const uint32_t*)temp, grid > 6 * col_tiles};
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
         return LCPP_ERR_CUDA;
-    cudaLaunchAttribute together{};  // tiles wait for one another
-    together.id = cudaLaunchAttributeCooperative;
-    together.val.cooperative = 1;
+    cudaLaunchAttribute how[2] = {};
+    how[0].id = cudaLaunchAttributeCooperative;  // tiles wait for one another
+    how[0].val.cooperative = row_tiles > 1;
+    how[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // launched while lr_prepare_kernel runs
+    how[1].val.programmaticStreamSerializationAllowed = prepared;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)grid);
     cfg.blockDim = dim3(LrConfig<T>::THREADS);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
-    cfg.attrs = &together;
-    cfg.numAttrs = row_tiles > 1 ? 1 : 0;
+    cfg.attrs = how;
+    cfg.numAttrs = 2;
     ProfScope prof(name, s);
     if (cudaLaunchKernelEx(&cfg, kernel, p, lr_chain(temp, sh.rows, sh.channels), tl) != cudaSuccess) return LCPP_ERR_CUDA;
     count_launch();
@@ -1177,7 +1187,8 @@ extern "C" lcpp_status lcpp_linear_recurrence_forward(
     if (!temp || temp_bytes < lcpp_linear_recurrence_temp_bytes(rows, channels)) return LCPP_ERR_TEMP_TOO_SMALL;
     const LrForward p{sh, gate_in, in, out, gate_stride, in_stride, out_stride, init_stride, init, last, (float*)saved};
     cudaStream_t s = (cudaStream_t)stream;
-    const lcpp_status ready = lr_prepare(sh, temp, init, init_stride, last, s);
+    bool prepared = false;
+    const lcpp_status ready = lr_prepare(sh, temp, init, init_stride, last, &prepared, s);
     if (ready != LCPP_OK || !rows) return ready;
     return lr_dispatch(gate, dtype, [&](auto t, auto g) -> lcpp_status {
         using T = decltype(t);
@@ -1185,7 +1196,7 @@ extern "C" lcpp_status lcpp_linear_recurrence_forward(
         const int copy = LrCopy(channels, sizeof(T)).add(gate_in, gate_stride, sizeof(T)).add(in, in_stride, sizeof(T))
                              .add(out, out_stride, sizeof(T)).kind();
         auto launch = [&](auto copies, auto kernel) {
-            return lr_launch<T>(sizeof(LrForwardSmem<T, decltype(copies)::value>), kernel, "lr_forward", p, sh, temp, s);
+            return lr_launch<T>(sizeof(LrForwardSmem<T, decltype(copies)::value>), kernel, "lr_forward", p, sh, temp, prepared, s);
         };
         if (copy == LR_COPY16) return launch(std::integral_constant<int, LR_COPY16>{}, lr_forward_kernel<T, G, LR_COPY16>);
         if constexpr (sizeof(T) == 2) {
@@ -1215,7 +1226,8 @@ extern "C" lcpp_status lcpp_linear_recurrence_backward(
     const LrBackward p{sh, gate_in, in, grad_out, grad_gate, grad_in, gate_stride, in_stride, grad_out_stride,
                        grad_gate_stride, grad_in_stride, init_stride, init, grad_last, (const float*)saved, grad_init};
     cudaStream_t s = (cudaStream_t)stream;
-    const lcpp_status ready = lr_prepare(sh, temp, grad_last, channels, grad_init, s);
+    bool prepared = false;
+    const lcpp_status ready = lr_prepare(sh, temp, grad_last, channels, grad_init, &prepared, s);
     if (ready != LCPP_OK || !rows) return ready;
     return lr_dispatch(gate, dtype, [&](auto t, auto g) -> lcpp_status {
         using T = decltype(t);
@@ -1226,7 +1238,7 @@ extern "C" lcpp_status lcpp_linear_recurrence_backward(
         if (grad_out) align.add(grad_out, grad_out_stride, sizeof(T));
         const int copy = align.kind();
         auto launch = [&](auto copies, auto kernel) {
-            return lr_launch<T>(sizeof(LrBackwardSmem<T, decltype(copies)::value>), kernel, "lr_backward", p, sh, temp, s);
+            return lr_launch<T>(sizeof(LrBackwardSmem<T, decltype(copies)::value>), kernel, "lr_backward", p, sh, temp, prepared, s);
         };
         if (copy == LR_COPY16) return launch(std::integral_constant<int, LR_COPY16>{}, lr_backward_kernel<T, G, LR_COPY16>);
         if constexpr (sizeof(T) == 2) {
