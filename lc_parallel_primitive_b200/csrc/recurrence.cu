@@ -108,6 +108,10 @@ __device__ __forceinline__ uint32_t lr_code(const LrShape& sh, uint64_t row, con
     const uint32_t r = (uint32_t)row, s = sh.length.div(r), at = r - s * sh.length.d;
     return (at == 0 ? LR_HEAD : 0) | (at + 1 == sh.length.d ? LR_TAIL : 0) | s;
 }
+// A warp's rows: no mark; one head and one tail at most (their states are read before the loop over the rows, which
+// only selects); anything else.
+enum { LR_PLAIN = 0, LR_SINGLE = 1, LR_MANY = 2 };
+
 // The codes of a warp's rows, lane r holding row r's, and masks of them.
 struct LrMarks {
     uint32_t code, head, tail, valid;
@@ -121,6 +125,10 @@ struct LrMarks {
     // Sequence of row r, which is a head or tail.
     __device__ __forceinline__ uint64_t sequence(const LrShape& sh, int r) const {
         return min((uint64_t)(__shfl_sync(0xffffffffu, code, r) & LR_SEQUENCE), sh.sequences - 1);
+    }
+    __device__ __forceinline__ int kind() const {
+        if (valid != LR_ALL || (head & (head - 1)) || (tail & (tail - 1))) return LR_MANY;
+        return head | tail ? LR_SINGLE : LR_PLAIN;
     }
     // Nothing from before the rows passes them; nothing from behind them does.
     __device__ __forceinline__ bool cuts() const { return head || valid != LR_ALL; }
@@ -372,14 +380,6 @@ __device__ __forceinline__ void lr_store(T* p, const float* v, int left, bool od
         }
     }
 }
-// Whether row is the first of a sequence, or outside (nothing passes it from before).
-__device__ __forceinline__ bool lr_starts(const LrShape& sh, const uint32_t* codes, uint64_t row) {
-    return lr_code(sh, row, codes + row) & (LR_HEAD | LR_OUTSIDE);
-}
-__device__ __forceinline__ bool lr_ends(const LrShape& sh, const uint32_t* codes, uint64_t row) {
-    return lr_code(sh, row, codes + row) & (LR_TAIL | LR_OUTSIDE);
-}
-
 // What a kernel of this file knows about its tiles: CTA b takes tiles b, b + grid, ..., numbered along the
 // channels first.  All CTAs of a chained launch are resident (a cooperative launch), so a tile may wait for the
 // tiles before it wherever they are.
@@ -437,6 +437,26 @@ __device__ __forceinline__ void lr_slot(LrSlot& slot, const LrShape& sh, uint64_
     }
 }
 
+// Asks for the states (C floats from `channel` on) of the sequences that begin (LR_HEAD) or end (LR_TAIL) in a warp's
+// rows of the next tile, so that they will be found in L1: a warp that waits for them there holds up its whole CTA
+// (backward, 32768 x 1536 f16 in 300 sequences: 184 us against 200 without).
+template <int C>
+__device__ __forceinline__ void lr_touch(const LrShape& sh, uint32_t code, uint32_t mark, const float* from, uint64_t stride,
+                                         uint32_t channel) {
+    if (!from) return;
+    const int lane = threadIdx.x & 31;
+    for (uint32_t rows = __ballot_sync(0xffffffffu, code & mark); rows; rows &= rows - 1) {
+        const uint32_t s = __shfl_sync(0xffffffffu, code, __ffs(rows) - 1) & LR_SEQUENCE;
+        const float* at = from + min((uint64_t)s, sh.sequences - 1) * stride + channel;
+#pragma unroll
+        for (int i = 0; i < C; i += 32)
+            if (channel + i + lane < sh.channels) {
+                float v;
+                asm volatile("ld.global.ca.f32 %0, [%1];" : "=f"(v) : "l"(at + i + lane));
+            }
+    }
+}
+
 // The kernels are launched while lr_prepare_kernel runs: what reads the rows' codes or touches records waits for it.
 __device__ __forceinline__ void lr_prepared() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
@@ -484,14 +504,22 @@ __global__ void __launch_bounds__(LrConfig<T>::THREADS, 1) lr_forward_kernel(LrF
     if (warp >= LR_WARPS) {
         const bool publishes = warp >= LR_WARPS + N;
         const int cc = (warp - LR_WARPS) % N * 32 + lane;
+        // the code of a tile's first row, read a tile ahead: nothing passes a head or enters outside a sequence
+        auto first_code = [&](uint32_t i) -> uint32_t {
+            const uint64_t row = (uint64_t)tl.tile(min(i, count - 1)).x * LR_TILE;
+            return lr_code(p.sh, row, tl.codes + row);
+        };
+        uint32_t code = first_code(0);
         for (uint32_t i = 0; i < count; ++i) {
             const int b = i & 1;
             const uint2 t = tl.tile(i);
             const uint32_t k = t.x, c = t.y * C + cc;
             float4* record = ch.record + (uint64_t)k * ch.width + c;
             const bool active = c < channels, more = active && k + 1 < tl.row_tiles;
+            const bool enters = !publishes && k > 0 && !(code & (LR_HEAD | LR_OUTSIDE));
+            code = first_code(i + 1);
             float carry = 0.0f;
-            if (!publishes && k > 0 && !lr_starts(p.sh, tl.codes, (uint64_t)k * LR_TILE)) {
+            if (enters) {
                 const int64_t step = -(int64_t)ch.width;
                 carry = tl.narrow ? lr_lookback<16>(record + step, step, k, active)
                                   : lr_lookback<8>(record + step, step, k, active);
@@ -541,76 +569,90 @@ __global__ void __launch_bounds__(LrConfig<T>::THREADS, 1) lr_forward_kernel(LrF
         }
         cp_async_commit();
     };
-    // Whether a warp's rows are all inside a sequence, and their codes if not.
-    auto codes = [&](const LrSlot& sl, uint32_t st, bool* plain) -> uint32_t {
-        *plain = sl.plain >> warp & 1;
-        if (*plain) return 0;
-        const uint32_t code = lane < LR_ROWS ? lr_code(p.sh, (uint64_t)sl.row + warp * LR_ROWS + lane,
-                                                            &sm.code[st][warp][lane]) : 0;
-        *plain = !__any_sync(0xffffffffu, code & (LR_OUTSIDE | LR_HEAD | LR_TAIL));
-        return code;
+    // The codes of this warp's rows of tile i (0 if it is known that none has a mark), a tile ahead of their use.
+    auto codes_ahead = [&](uint32_t i) -> uint32_t {
+        const LrSlot& sl = sm.slot[i % LR_SLOTS];
+        if (i >= count || (sl.plain >> warp & 1) || lane >= LR_ROWS) return 0;
+        const uint64_t row = (uint64_t)sl.row + warp * LR_ROWS + lane;
+        return lr_code(p.sh, row, tl.codes + row);
+    };
+    uint32_t ahead = codes_ahead(1);
+    // The marks of a warp's rows in a tile, and what the loops over the rows have to do about them.
+    auto marks = [&](const LrSlot& sl, uint32_t st, int* kind) -> LrMarks {
+        *kind = LR_PLAIN;
+        if (sl.plain >> warp & 1) return LrMarks();
+        const uint64_t row = (uint64_t)sl.row + warp * LR_ROWS + lane;
+        const uint32_t code = lane < LR_ROWS ? lr_code(p.sh, row, &sm.code[st][warp][lane]) : 0;
+        if (!__any_sync(0xffffffffu, code & (LR_OUTSIDE | LR_HEAD | LR_TAIL))) return LrMarks();
+        const LrMarks m(code);
+        *kind = m.kind();
+        return m;
+    };
+    // The state of the sequence that begins (ends) in row r of a warp's rows: `from` [sequence][stride].
+    auto edge = [&](const LrMarks& m, const LrSlot& sl, int r, const float* from, uint64_t stride, float* v) {
+        const uint64_t s = m.sequence(p.sh, r);
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            v[i] = from && column + i < sl.channels ? from[s * stride + sl.channel + column + i] : 0.0f;
     };
     struct Rows {  // a tile between its two halves: row r is h = pre h_before + loc
         float pre[LR_ROWS][N], loc[LR_ROWS][N];
-        uint32_t code;
-        bool plain;
+        LrMarks m;
+        int kind;
     };
     auto maps = [&](uint32_t i, Rows& w) {
         const uint32_t st = i % Smem::STAGES;
         const LrSlot& sl = sm.slot[i % LR_SLOTS];
         cp_async_wait_prior<Smem::STAGES - 1>();
         __syncwarp();
-        w.code = codes(sl, st, &w.plain);
+        w.m = marks(sl, st, &w.kind);
         const LrRows<T, COPY> gate(sm.rows[st][warp][0], p.gate, sl.offset[0], p.gate_stride),
             in(sm.rows[st][warp][1], p.in, sl.offset[1], p.in_stride);
         float A[N], H[N];
 #pragma unroll
         for (int i = 0; i < N; ++i) A[i] = 1.0f, H[i] = 0.0f;
-        if (w.plain) {
+        auto rows = [&](auto tag) {
+            constexpr int kind = decltype(tag)::value;
+            const LrMarks& m = w.m;
+            const int head = __ffs(m.head) - 1;
+            float init[N];
+            if (kind == LR_SINGLE && head >= 0) edge(m, sl, head, p.init, p.init_stride, init);
 #pragma unroll
             for (int r = 0; r < LR_ROWS; ++r) {
                 float g[N], x[N];
                 LrWord<T>::widen(gate[r], g);
                 LrWord<T>::widen(in[r], x);
+                if (kind == LR_MANY) edge(m, sl, r, p.init, p.init_stride, init);
+                if (kind == LR_SINGLE ? r == head : kind == LR_MANY && (m.head >> r & 1))
+#pragma unroll
+                    for (int i = 0; i < N; ++i) A[i] = 0.0f, H[i] = init[i];
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
                     const Gate<GATE> gt(g[i]);
                     H[i] = fmaf(gt.a, H[i], gt.add(x[i]));
                     A[i] *= gt.a;
-                    w.pre[r][i] = A[i], w.loc[r][i] = H[i];
                 }
-            }
-        } else {
-            const LrMarks m(w.code);
-            const uint32_t c = sl.channel + column;
+                if (kind == LR_MANY && !(m.valid >> r & 1))
 #pragma unroll
-            for (int r = 0; r < LR_ROWS; ++r) {
-                float g[N], x[N];
-                LrWord<T>::widen(gate[r], g);
-                LrWord<T>::widen(in[r], x);
-                const uint64_t s = m.sequence(p.sh, r);
+                    for (int i = 0; i < N; ++i) A[i] = H[i] = 0.0f;
 #pragma unroll
-                for (int i = 0; i < N; ++i) {
-                    if (m.head >> r & 1) {
-                        A[i] = 0.0f;
-                        H[i] = p.init && c + i < channels ? p.init[s * p.init_stride + c + i] : 0.0f;
-                    }
-                    const Gate<GATE> gt(g[i]);
-                    H[i] = fmaf(gt.a, H[i], gt.add(x[i]));
-                    A[i] *= gt.a;
-                    if (!(m.valid >> r & 1)) A[i] = 0.0f, H[i] = 0.0f;
-                    w.pre[r][i] = A[i], w.loc[r][i] = H[i];
-                }
+                for (int i = 0; i < N; ++i) w.pre[r][i] = A[i], w.loc[r][i] = H[i];
             }
-        }
+        };
+        if (w.kind == LR_PLAIN) rows(std::integral_constant<int, LR_PLAIN>{});
+        else if (w.kind == LR_SINGLE) rows(std::integral_constant<int, LR_SINGLE>{});
+        else rows(std::integral_constant<int, LR_MANY>{});
         const int b = i & 1;
 #pragma unroll
         for (int i = 0; i < N; ++i) sm.map[b][warp][column + i] = make_float2(A[i], H[i]);
-        if (lane == 0) sm.cut[b][warp] = !w.plain;
+        if (lane == 0) sm.cut[b][warp] = w.m.cuts();
         lr_arrive(1 + b, Config::MAPPED);
         lr_arrive(5 + b, Config::MAPPED);
         __syncwarp();  // the stage is read
         fetch(i + Smem::STAGES);
+        if (__any_sync(0xffffffffu, ahead & (LR_HEAD | LR_TAIL)))
+            lr_touch<C>(p.sh, ahead, LR_HEAD, p.init, p.init_stride, sm.slot[(i + 1) % LR_SLOTS].channel);
+        ahead = codes_ahead(i + 2);
     };
     auto finish = [&](uint32_t i, const Rows& w) {
         const int b = i & 1;
@@ -622,7 +664,7 @@ __global__ void __launch_bounds__(LrConfig<T>::THREADS, 1) lr_forward_kernel(LrF
         lr_sync(3 + b, Config::THREADS);
 #pragma unroll
         for (int i = 0; i < N; ++i) start[i] = sm.start[b][warp][column + i];
-        if (w.plain) {
+        if (w.kind == LR_PLAIN) {
 #pragma unroll
             for (int r = 0; r < LR_ROWS; ++r, out += p.out_stride) {
                 float h[N];
@@ -634,8 +676,7 @@ __global__ void __launch_bounds__(LrConfig<T>::THREADS, 1) lr_forward_kernel(LrF
         }
         // From the first head or outside row on nothing depends on the state before the warp's rows (not even as 0
         // times it, which an infinity or NaN of another sequence would survive).
-        const LrMarks m(w.code);
-        const uint32_t c = sl.channel + column;
+        const LrMarks& m = w.m;
         const int rows = (int)sl.rows - warp * LR_ROWS;
         const int reach = __ffs(m.head | ~m.valid) - 1;
 #pragma unroll
@@ -644,17 +685,17 @@ __global__ void __launch_bounds__(LrConfig<T>::THREADS, 1) lr_forward_kernel(LrF
 #pragma unroll
             for (int i = 0; i < N; ++i) h[i] = r < reach ? fmaf(w.pre[r][i], start[i], w.loc[r][i]) : w.loc[r][i];
             if (r < rows) lr_store<T, COPY>(out, h, left, odd >> r & 1);
-            const uint64_t s = m.sequence(p.sh, r);
             if ((m.tail >> r & 1) && p.last) {
+                float* last = p.last + m.sequence(p.sh, r) * channels + sl.channel + column;
 #pragma unroll
                 for (int i = 0; i < N; ++i)
-                    if (i < left) p.last[s * channels + c + i] = h[i];
+                    if (i < left) last[i] = h[i];
             }
         }
     };
 #pragma unroll
     for (int i = 0; i < Smem::STAGES; ++i) fetch(i);
-    Rows even, odd;
+    Rows even, odd;  // the maps of tile i + 1, then the outputs of tile i
     if (count > 0) maps(0, even);
     for (uint32_t i = 0; i < count; i += 2) {
         if (i + 1 < count) maps(i + 1, odd);
@@ -705,6 +746,12 @@ __global__ void __launch_bounds__(LrConfig<T>::THREADS, 1) lr_backward_kernel(Lr
     if (warp >= LR_WARPS) {
         const bool publishes = warp >= LR_WARPS + N;
         const int cc = (warp - LR_WARPS) % N * 32 + lane;
+        // the code of a tile's last row, read a tile ahead: nothing passes a tail or enters outside a sequence
+        auto last_code = [&](uint32_t i) -> uint32_t {
+            const uint64_t row = (uint64_t)(tl.row_tiles - tl.tile(min(i, count - 1)).x) * LR_TILE - 1;
+            return lr_code(p.sh, row, tl.codes + row);
+        };
+        uint32_t code = last_code(0);
         for (uint32_t i = 0; i < count; ++i) {
             const int b = i & 1;
             const uint2 t = tl.tile(i);
@@ -713,7 +760,9 @@ __global__ void __launch_bounds__(LrConfig<T>::THREADS, 1) lr_backward_kernel(Lr
             const bool active = c < channels, more = active && k > 0, chained = k + 1 < tl.row_tiles;
             // the publishing warps also carry the states on, from the saved one
             float carry = 0.0f, state = publishes && active ? p.saved[(uint64_t)k * channels + c] : 0.0f;
-            if (!publishes && chained && !lr_ends(p.sh, tl.codes, (uint64_t)(k + 1) * LR_TILE - 1)) {
+            const bool enters = !publishes && chained && !(code & (LR_TAIL | LR_OUTSIDE));
+            code = last_code(i + 1);
+            if (enters) {
                 const int64_t step = ch.width;
                 carry = tl.narrow ? lr_lookback<16>(record + step, step, t.x, active)
                                   : lr_lookback<8>(record + step, step, t.x, active);
@@ -772,41 +821,65 @@ __global__ void __launch_bounds__(LrConfig<T>::THREADS, 1) lr_backward_kernel(Lr
         }
         cp_async_commit();
     };
-    // Whether a warp's rows are all inside a sequence, and their codes if not.
-    auto codes = [&](const LrSlot& sl, uint32_t st, bool* plain) -> uint32_t {
-        *plain = sl.plain >> warp & 1;
-        if (*plain) return 0;
-        const uint32_t code = lane < LR_ROWS ? lr_code(p.sh, (uint64_t)sl.row + warp * LR_ROWS + lane,
-                                                            &sm.code[st][warp][lane]) : 0;
-        *plain = !__any_sync(0xffffffffu, code & (LR_OUTSIDE | LR_HEAD | LR_TAIL));
-        return code;
+    // The codes of this warp's rows of tile i (0 if it is known that none has a mark), a tile ahead of their use.
+    auto codes_ahead = [&](uint32_t i) -> uint32_t {
+        const LrSlot& sl = sm.slot[i % LR_SLOTS];
+        if (i >= count || (sl.plain >> warp & 1) || lane >= LR_ROWS) return 0;
+        const uint64_t row = (uint64_t)sl.row + warp * LR_ROWS + lane;
+        return lr_code(p.sh, row, tl.codes + row);
+    };
+    uint32_t ahead = codes_ahead(1);
+    // The marks of a warp's rows in a tile, and what the loops over the rows have to do about them.
+    auto marks = [&](const LrSlot& sl, uint32_t st, int* kind) -> LrMarks {
+        *kind = LR_PLAIN;
+        if (sl.plain >> warp & 1) return LrMarks();
+        const uint64_t row = (uint64_t)sl.row + warp * LR_ROWS + lane;
+        const uint32_t code = lane < LR_ROWS ? lr_code(p.sh, row, &sm.code[st][warp][lane]) : 0;
+        if (!__any_sync(0xffffffffu, code & (LR_OUTSIDE | LR_HEAD | LR_TAIL))) return LrMarks();
+        const LrMarks m(code);
+        *kind = m.kind();
+        return m;
+    };
+    // The state of the sequence that begins (ends) in row r of a warp's rows: `from` [sequence][stride].
+    auto edge = [&](const LrMarks& m, const LrSlot& sl, int r, const float* from, uint64_t stride, float* v) {
+        const uint64_t s = m.sequence(p.sh, r);
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            v[i] = from && column + i < sl.channels ? from[s * stride + sl.channel + column + i] : 0.0f;
     };
     if (!p.grad_out) {  // zeros that stay
         for (int st = 0; st < Smem::STAGES; ++st)
             for (int j = lane; j < LrFetch<T, COPY>::BUF / 4; j += 32) ((uint32_t*)sm.rows[st][warp][2])[j] = 0;
         __syncwarp();
     }
-    auto maps = [&](uint32_t i) {
+    auto maps = [&](uint32_t i) -> int {
         const uint32_t st = i % Smem::STAGES;
         const LrSlot& sl = sm.slot[i % LR_SLOTS];
         cp_async_wait_prior<Smem::STAGES - 2>();
         __syncwarp();
-        bool plain;
-        const uint32_t code = codes(sl, st, &plain);
+        int what;
+        const LrMarks m = marks(sl, st, &what);
         const LrRows<T, COPY> gate(sm.rows[st][warp][0], p.gate, sl.offset[0], p.gate_stride),
             in(sm.rows[st][warp][1], p.in, sl.offset[1], p.in_stride),
             grad(sm.rows[st][warp][2], p.grad_out, sl.offset[2], p.grad_out_stride);
         float A[N], H[N], M[N];
 #pragma unroll
         for (int i = 0; i < N; ++i) A[i] = 1.0f, H[i] = 0.0f, M[i] = 0.0f;
-        bool cuts = false, cuts_back = false;
-        if (plain) {
-            float a[LR_ROWS][N];
+        auto rows = [&](auto tag) {
+            constexpr int kind = decltype(tag)::value;
+            float a[LR_ROWS][N], init[N], last[N];
+            const int head = __ffs(m.head) - 1, tail = __ffs(m.tail) - 1;
+            if (kind == LR_SINGLE && head >= 0) edge(m, sl, head, p.init, p.init_stride, init);
+            if (kind == LR_SINGLE && tail >= 0) edge(m, sl, tail, p.grad_last, channels, last);
 #pragma unroll
             for (int r = 0; r < LR_ROWS; ++r) {
                 float g[N], x[N];
                 LrWord<T>::widen(gate[r], g);
                 LrWord<T>::widen(in[r], x);
+                if (kind == LR_MANY) edge(m, sl, r, p.init, p.init_stride, init);
+                if (kind == LR_SINGLE ? r == head : kind == LR_MANY && (m.head >> r & 1))
+#pragma unroll
+                    for (int i = 0; i < N; ++i) H[i] = init[i];
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
                     const Gate<GATE> gt(g[i]);
@@ -819,75 +892,77 @@ __global__ void __launch_bounds__(LrConfig<T>::THREADS, 1) lr_backward_kernel(Lr
             for (int r = LR_ROWS - 1; r >= 0; --r) {
                 float v[N];
                 LrWord<T>::widen(grad[r], v);
+                if (kind == LR_MANY) edge(m, sl, r, p.grad_last, channels, last);
+                if (kind == LR_SINGLE ? r == tail : kind == LR_MANY && (m.tail >> r & 1))
+#pragma unroll
+                    for (int i = 0; i < N; ++i) M[i] = last[i];
 #pragma unroll
                 for (int i = 0; i < N; ++i) M[i] = a[r][i] * (v[i] + M[i]);
+                if (kind == LR_MANY && !(m.valid >> r & 1))
+#pragma unroll
+                    for (int i = 0; i < N; ++i) M[i] = 0.0f;
             }
-        } else {
-            const LrMarks m(code);
-            const uint32_t c = sl.channel + column;
-            cuts = m.cuts(), cuts_back = m.cuts_back();
-            float a[LR_ROWS][N];
-#pragma unroll
-            for (int r = 0; r < LR_ROWS; ++r) {
-                float g[N], x[N];
-                LrWord<T>::widen(gate[r], g);
-                LrWord<T>::widen(in[r], x);
-                const uint64_t s = m.sequence(p.sh, r);
-#pragma unroll
-                for (int i = 0; i < N; ++i) {
-                    if (m.head >> r & 1) H[i] = p.init && c + i < channels ? p.init[s * p.init_stride + c + i] : 0.0f;
-                    const Gate<GATE> gt(g[i]);
-                    a[r][i] = gt.a;
-                    H[i] = fmaf(gt.a, H[i], gt.add(x[i]));
-                    A[i] *= gt.a;
-                }
-            }
-#pragma unroll
-            for (int r = LR_ROWS - 1; r >= 0; --r) {
-                float v[N];
-                LrWord<T>::widen(grad[r], v);
-                const uint64_t s = m.sequence(p.sh, r);
-#pragma unroll
-                for (int i = 0; i < N; ++i) {
-                    if (m.tail >> r & 1) M[i] = p.grad_last && c + i < channels ? p.grad_last[s * channels + c + i] : 0.0f;
-                    M[i] = m.valid >> r & 1 ? a[r][i] * (v[i] + M[i]) : 0.0f;
-                }
-            }
-        }
+        };
+        if (what == LR_PLAIN) rows(std::integral_constant<int, LR_PLAIN>{});
+        else if (what == LR_SINGLE) rows(std::integral_constant<int, LR_SINGLE>{});
+        else rows(std::integral_constant<int, LR_MANY>{});
         const int b = i & 1;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             sm.map[b][warp][column + i] = make_float2(A[i], H[i]);
             sm.grad_map[b][warp][column + i] = M[i];
         }
-        if (lane == 0) sm.cut[b][warp] = (cuts ? 1u : 0u) | (cuts_back ? 2u : 0u);
+        if (lane == 0) sm.cut[b][warp] = (m.cuts() ? 1u : 0u) | (m.cuts_back() ? 2u : 0u);
         lr_arrive(1 + b, Config::MAPPED);
         lr_arrive(5 + b, Config::MAPPED);
+        if (__any_sync(0xffffffffu, ahead & (LR_HEAD | LR_TAIL))) {
+            const uint32_t channel = sm.slot[(i + 1) % LR_SLOTS].channel;
+            lr_touch<C>(p.sh, ahead, LR_HEAD, p.init, p.init_stride, channel);
+            lr_touch<C>(p.sh, ahead, LR_TAIL, p.grad_last, channels, channel);
+        }
+        ahead = codes_ahead(i + 2);
+        return what;
     };
-    auto finish = [&](uint32_t i) {
+    auto finish = [&](uint32_t i, int what) {
         const int b = i & 1;
         const uint32_t st = i % Smem::STAGES;
         const LrSlot& sl = sm.slot[i % LR_SLOTS];
         const int left = (int)sl.channels - column;
-        bool plain;
-        const uint32_t code = codes(sl, st, &plain);
+        const LrMarks m = what == LR_PLAIN ? LrMarks() : marks(sl, st, &what);
         const LrRows<T, COPY> gate(sm.rows[st][warp][0], p.gate, sl.offset[0], p.gate_stride),
             in(sm.rows[st][warp][1], p.in, sl.offset[1], p.in_stride),
             grad(sm.rows[st][warp][2], p.grad_out, sl.offset[2], p.grad_out_stride);
         T* out_gate = (T*)((char*)out_gate0 + sl.offset[3]);
         T* out_in = (T*)((char*)out_in0 + sl.offset[4]);
         const uint32_t odd_gate = COPY == LR_COPY_ODD ? lr_odd_rows(p.grad_gate, sl.offset[3], p.grad_gate_stride) : 0;
-        const uint32_t odd_in = COPY == LR_COPY_ODD ? lr_odd_rows(p.grad_in, sl.offset[4], p.grad_in_stride) : 0;
-        float h[N], mu[N], a[LR_ROWS][N], na[LR_ROWS][N], dgate[LR_ROWS][N];  // dgate: of the gate, per unit of lam
-        lr_sync(3 + b, Config::THREADS);
+        auto keep = [&](int r, const float* v) {  // the gradient of the initial state
+            if (!p.grad_init) return;
+            float* to = p.grad_init + m.sequence(p.sh, r) * channels + sl.channel + column;
 #pragma unroll
-        for (int i = 0; i < N; ++i) h[i] = sm.start[b][warp][column + i], mu[i] = sm.grad_start[b][warp][column + i];
-        if (plain) {
+            for (int i = 0; i < N; ++i)
+                if (i < left) to[i] = v[i];
+        };
+        const uint32_t odd_in = COPY == LR_COPY_ODD ? lr_odd_rows(p.grad_in, sl.offset[4], p.grad_in_stride) : 0;
+        auto rows = [&](auto tag) {
+            constexpr int kind = decltype(tag)::value;
+            float h[N], mu[N], a[LR_ROWS][N], na[LR_ROWS][N], dgate[LR_ROWS][N];  // dgate: of the gate, per unit of lam
+            float init[N], last[N], first[N] = {};
+            const int head = __ffs(m.head) - 1, tail = __ffs(m.tail) - 1;
+            if (kind == LR_SINGLE && head >= 0) edge(m, sl, head, p.init, p.init_stride, init);
+            if (kind == LR_SINGLE && tail >= 0) edge(m, sl, tail, p.grad_last, channels, last);
+            const int n = kind == LR_MANY ? (int)sl.rows - warp * LR_ROWS : LR_ROWS;
+            lr_sync(3 + b, Config::THREADS);
+#pragma unroll
+            for (int i = 0; i < N; ++i) h[i] = sm.start[b][warp][column + i], mu[i] = sm.grad_start[b][warp][column + i];
 #pragma unroll
             for (int r = 0; r < LR_ROWS; ++r) {
                 float g[N], x[N];
                 LrWord<T>::widen(gate[r], g);
                 LrWord<T>::widen(in[r], x);
+                if (kind == LR_MANY) edge(m, sl, r, p.init, p.init_stride, init);
+                if (kind == LR_SINGLE ? r == head : kind == LR_MANY && (m.head >> r & 1))
+#pragma unroll
+                    for (int i = 0; i < N; ++i) h[i] = init[i];
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
                     const Gate<GATE> gt(g[i]);
@@ -900,6 +975,10 @@ __global__ void __launch_bounds__(LrConfig<T>::THREADS, 1) lr_backward_kernel(Lr
             for (int r = LR_ROWS - 1; r >= 0; --r, out_gate -= p.grad_gate_stride, out_in -= p.grad_in_stride) {
                 float v[N], dg[N], dx[N];
                 LrWord<T>::widen(grad[r], v);
+                if (kind == LR_MANY) edge(m, sl, r, p.grad_last, channels, last);
+                if (kind == LR_SINGLE ? r == tail : kind == LR_MANY && (m.tail >> r & 1))
+#pragma unroll
+                    for (int i = 0; i < N; ++i) mu[i] = last[i];
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
                     const float lam = v[i] + mu[i];
@@ -907,58 +986,32 @@ __global__ void __launch_bounds__(LrConfig<T>::THREADS, 1) lr_backward_kernel(Lr
                     dx[i] = GATE == LCPP_GATE_SIGMOID ? na[r][i] * lam : lam;
                     mu[i] = a[r][i] * lam;
                 }
-                lr_store<T, COPY>(out_gate, dg, left, odd_gate >> r & 1);
-                lr_store<T, COPY>(out_in, dx, left, odd_in >> r & 1);
-            }
-        } else {
-            const LrMarks m(code);
-            const uint32_t c = sl.channel + column;
-            const int rows = (int)sl.rows - warp * LR_ROWS;
+                if (kind == LR_MANY && !(m.valid >> r & 1))
 #pragma unroll
-            for (int r = 0; r < LR_ROWS; ++r) {
-                float g[N], x[N];
-                LrWord<T>::widen(gate[r], g);
-                LrWord<T>::widen(in[r], x);
-                const uint64_t s = m.sequence(p.sh, r);
-#pragma unroll
-                for (int i = 0; i < N; ++i) {
-                    if (m.head >> r & 1) h[i] = p.init && c + i < channels ? p.init[s * p.init_stride + c + i] : 0.0f;
-                    const Gate<GATE> gt(g[i]);
-                    a[r][i] = gt.a, na[r][i] = gt.na;
-                    dgate[r][i] = gt.grad_gate(h[i], x[i]);
-                    h[i] = fmaf(gt.a, h[i], gt.add(x[i]));
-                }
-            }
-#pragma unroll
-            for (int r = LR_ROWS - 1; r >= 0; --r, out_gate -= p.grad_gate_stride, out_in -= p.grad_in_stride) {
-                float v[N], dg[N], dx[N];
-                LrWord<T>::widen(grad[r], v);
-                const uint64_t s = m.sequence(p.sh, r);
-#pragma unroll
-                for (int i = 0; i < N; ++i) {
-                    if (m.tail >> r & 1) mu[i] = p.grad_last && c + i < channels ? p.grad_last[s * channels + c + i] : 0.0f;
-                    const float lam = v[i] + mu[i];
-                    const bool valid = m.valid >> r & 1;
-                    dg[i] = valid ? lam * dgate[r][i] : 0.0f;
-                    dx[i] = valid ? GATE == LCPP_GATE_SIGMOID ? na[r][i] * lam : lam : 0.0f;
-                    mu[i] = valid ? a[r][i] * lam : 0.0f;
-                    if ((m.head >> r & 1) && p.grad_init && i < left) p.grad_init[s * channels + c + i] = mu[i];
-                }
-                if (r < rows) {
+                    for (int i = 0; i < N; ++i) dg[i] = dx[i] = mu[i] = 0.0f;
+                if (r < n) {
                     lr_store<T, COPY>(out_gate, dg, left, odd_gate >> r & 1);
                     lr_store<T, COPY>(out_in, dx, left, odd_in >> r & 1);
                 }
+                if (kind == LR_SINGLE)
+#pragma unroll
+                    for (int i = 0; i < N; ++i) first[i] = r == head ? mu[i] : first[i];
+                if (kind == LR_MANY && (m.head >> r & 1)) keep(r, mu);
             }
-        }
+            if (kind == LR_SINGLE && head >= 0) keep(head, first);
+        };
+        if (what == LR_PLAIN) rows(std::integral_constant<int, LR_PLAIN>{});
+        else if (what == LR_SINGLE) rows(std::integral_constant<int, LR_SINGLE>{});
+        else rows(std::integral_constant<int, LR_MANY>{});
         __syncwarp();  // the stage is read
         fetch(i + Smem::STAGES);
     };
 #pragma unroll
     for (int i = 0; i < Smem::STAGES; ++i) fetch(i);
-    if (count > 0) maps(0);
-    for (uint32_t i = 0; i < count; ++i) {
-        if (i + 1 < count) maps(i + 1);
-        finish(i);
+    int kind = LR_PLAIN, before = LR_PLAIN;
+    for (uint32_t i = 0; i <= count; ++i, before = kind) {  // each compiled once: the instruction cache counts here
+        if (i < count) kind = maps(i);
+        if (i > 0) finish(i - 1, before);
     }
     cp_async_wait_all();
 }
