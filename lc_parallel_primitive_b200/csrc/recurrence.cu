@@ -1177,31 +1177,41 @@ static lcpp_status lr_prepare(const LrShape& sh, void* temp, const float* from, 
     return check_launch();
 }
 
-template <typename T, typename K, typename P>
-static lcpp_status lr_launch(size_t smem, K kernel, const char* name, const P& p, const LrShape& sh, void* temp, bool prepared,
+// Launches KERNEL over all tiles.
+template <typename T, auto KERNEL, typename P>
+static lcpp_status lr_launch(size_t smem, const char* name, const P& p, const LrShape& sh, void* temp, bool prepared,
                              cudaStream_t s) {
     const uint64_t row_tiles = ceil_div(sh.rows, LR_TILE), col_tiles = ceil_div(sh.channels, LrConfig<T>::C);
     if (row_tiles * col_tiles > 0x7fffffffull) return LCPP_ERR_INVALID_ARG;
-    const uint64_t grid = min(row_tiles * col_tiles, (uint64_t)device_info().sms);
+    const DeviceInfo device = device_info();
+    const uint64_t grid = min(row_tiles * col_tiles, (uint64_t)device.sms);
     const LrTiles tl{(uint32_t)row_tiles, LrDivisor(col_tiles), (const uint32_t*)temp, grid > 6 * col_tiles};
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
-        return LCPP_ERR_CUDA;
-    cudaLaunchAttribute how[2] = {};
-    how[0].id = cudaLaunchAttributeCooperative;  // tiles wait for one another
-    how[0].val.cooperative = row_tiles > 1;
-    how[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // launched while lr_prepare_kernel runs
-    how[1].val.programmaticStreamSerializationAllowed = prepared;
+    static std::atomic<uint64_t> sized{0};  // devices on which the kernel may have this much shared memory
+    const uint64_t bit = 1ull << device.device;
+    if (!(sized.load(std::memory_order_relaxed) & bit)) {
+        if (cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+            return LCPP_ERR_CUDA;
+        sized.fetch_or(bit, std::memory_order_relaxed);
+    }
+    cudaLaunchAttribute how[2];
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)grid);
     cfg.blockDim = dim3(LrConfig<T>::THREADS);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
     cfg.attrs = how;
-    cfg.numAttrs = 2;
+    if (row_tiles > 1) {  // tiles wait for one another
+        how[cfg.numAttrs].id = cudaLaunchAttributeCooperative;
+        how[cfg.numAttrs++].val.cooperative = 1;
+    }
+    if (prepared) {  // launched while lr_prepare_kernel runs
+        how[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        how[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+    }
     ProfScope prof(name, s);
-    if (cudaLaunchKernelEx(&cfg, kernel, p, lr_chain(temp, sh.rows, sh.channels), tl) != cudaSuccess) return LCPP_ERR_CUDA;
+    if (cudaLaunchKernelEx(&cfg, KERNEL, p, lr_chain(temp, sh.rows, sh.channels), tl) != cudaSuccess) return LCPP_ERR_CUDA;
     count_launch();
-    return check_launch();
+    return LCPP_OK;
 }
 
 template <typename F>
@@ -1248,14 +1258,15 @@ extern "C" lcpp_status lcpp_linear_recurrence_forward(
         constexpr int G = decltype(g)::value;
         const int copy = LrCopy(channels, sizeof(T)).add(gate_in, gate_stride, sizeof(T)).add(in, in_stride, sizeof(T))
                              .add(out, out_stride, sizeof(T)).kind();
-        auto launch = [&](auto copies, auto kernel) {
-            return lr_launch<T>(sizeof(LrForwardSmem<T, decltype(copies)::value>), kernel, "lr_forward", p, sh, temp, prepared, s);
+        auto launch = [&](auto c) {
+            constexpr int COPY = decltype(c)::value;
+            return lr_launch<T, lr_forward_kernel<T, G, COPY>>(sizeof(LrForwardSmem<T, COPY>), "lr_forward", p, sh, temp, prepared, s);
         };
-        if (copy == LR_COPY16) return launch(std::integral_constant<int, LR_COPY16>{}, lr_forward_kernel<T, G, LR_COPY16>);
+        if (copy == LR_COPY16) return launch(std::integral_constant<int, LR_COPY16>{});
         if constexpr (sizeof(T) == 2) {
-            if (copy == LR_COPY_ODD) return launch(std::integral_constant<int, LR_COPY_ODD>{}, lr_forward_kernel<T, G, LR_COPY_ODD>);
+            if (copy == LR_COPY_ODD) return launch(std::integral_constant<int, LR_COPY_ODD>{});
         }
-        return launch(std::integral_constant<int, LR_COPY4>{}, lr_forward_kernel<T, G, LR_COPY4>);
+        return launch(std::integral_constant<int, LR_COPY4>{});
     });
 }
 
@@ -1290,14 +1301,15 @@ extern "C" lcpp_status lcpp_linear_recurrence_backward(
             .add(grad_gate, grad_gate_stride, sizeof(T)).add(grad_in, grad_in_stride, sizeof(T));
         if (grad_out) align.add(grad_out, grad_out_stride, sizeof(T));
         const int copy = align.kind();
-        auto launch = [&](auto copies, auto kernel) {
-            return lr_launch<T>(sizeof(LrBackwardSmem<T, decltype(copies)::value>), kernel, "lr_backward", p, sh, temp, prepared, s);
+        auto launch = [&](auto c) {
+            constexpr int COPY = decltype(c)::value;
+            return lr_launch<T, lr_backward_kernel<T, G, COPY>>(sizeof(LrBackwardSmem<T, COPY>), "lr_backward", p, sh, temp, prepared, s);
         };
-        if (copy == LR_COPY16) return launch(std::integral_constant<int, LR_COPY16>{}, lr_backward_kernel<T, G, LR_COPY16>);
+        if (copy == LR_COPY16) return launch(std::integral_constant<int, LR_COPY16>{});
         if constexpr (sizeof(T) == 2) {
-            if (copy == LR_COPY_ODD) return launch(std::integral_constant<int, LR_COPY_ODD>{}, lr_backward_kernel<T, G, LR_COPY_ODD>);
+            if (copy == LR_COPY_ODD) return launch(std::integral_constant<int, LR_COPY_ODD>{});
         }
-        return launch(std::integral_constant<int, LR_COPY4>{}, lr_backward_kernel<T, G, LR_COPY4>);
+        return launch(std::integral_constant<int, LR_COPY4>{});
     });
 }
 

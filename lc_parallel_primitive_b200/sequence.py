@@ -78,10 +78,12 @@ def _matrix(t: torch.Tensor, name: str):
     return t.data_ptr(), row, rows, channels
 
 
-def _like(t: Optional[torch.Tensor], rows: int, channels: int, name: str):
-    """(pointer, row stride) of a matrix of this size (None: a null pointer)."""
+def _like(t: Optional[torch.Tensor], first: torch.Tensor, rows: int, channels: int, name: str):
+    """(pointer, row stride) of a matrix of the first one's size (None: a null pointer)."""
     if t is None:
         return None, 0
+    if t.shape == first.shape and t.is_contiguous():  # the usual one
+        return t.data_ptr(), channels
     pointer, row, r, c = _matrix(t, name)
     if r != rows or c != channels:
         raise ValueError(f"{name} must have the same shape as the call's other matrices, "
@@ -173,8 +175,8 @@ class DeviceLinearRecurrence(_Recorded):
         keep = (d_gate, d_in, d_out, d_init, d_last, d_saved, temp_storage, offsets)
         _one_device(*keep)
         pg, sg, rows, channels = _matrix(d_gate, "d_gate")
-        pi, si = _like(d_in, rows, channels, "d_in")
-        po, so = _like(d_out, rows, channels, "d_out")
+        pi, si = _like(d_in, d_gate, rows, channels, "d_in")
+        po, so = _like(d_out, d_gate, rows, channels, "d_out")
         count, length, off = self._sequences(offsets_or_length, rows)
         p0, s0 = self._init(d_init, count, channels)
         pl = _dense(d_last, (count, channels), _F32, "d_last")
@@ -197,10 +199,10 @@ class DeviceLinearRecurrence(_Recorded):
                 temp_storage, offsets)
         _one_device(*keep)
         pg, sg, rows, channels = _matrix(d_gate, "d_gate")
-        pi, si = _like(d_in, rows, channels, "d_in")
-        pgo, sgo = _like(d_grad_out, rows, channels, "d_grad_out")
-        pgg, sgg = _like(d_grad_gate, rows, channels, "d_grad_gate")
-        pgi, sgi = _like(d_grad_in, rows, channels, "d_grad_in")
+        pi, si = _like(d_in, d_gate, rows, channels, "d_in")
+        pgo, sgo = _like(d_grad_out, d_gate, rows, channels, "d_grad_out")
+        pgg, sgg = _like(d_grad_gate, d_gate, rows, channels, "d_grad_gate")
+        pgi, sgi = _like(d_grad_in, d_gate, rows, channels, "d_grad_in")
         count, length, off = self._sequences(offsets_or_length, rows)
         p0, s0 = self._init(d_init, count, channels)
         pgl = _dense(d_grad_last, (count, channels), _F32, "d_grad_last")
@@ -218,8 +220,8 @@ class DeviceLinearRecurrence(_Recorded):
         keep = (d_gate, d_in, d_states_in, d_states_out, d_out, d_parents)
         _one_device(*keep)
         pg, sg, rows, channels = _matrix(d_gate, "d_gate")
-        pi, si = _like(d_in, rows, channels, "d_in")
-        po, so = _like(d_out, rows, channels, "d_out")
+        pi, si = _like(d_in, d_gate, rows, channels, "d_in")
+        po, so = _like(d_out, d_gate, rows, channels, "d_out")
         rows_in = 0 if d_states_in is None else d_states_in.shape[0]
         psi = _dense(d_states_in, (rows_in, channels), _F32, "d_states_in")
         pso = _dense(d_states_out, (rows, channels), _F32, "d_states_out")
