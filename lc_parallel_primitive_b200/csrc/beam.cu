@@ -61,6 +61,16 @@ __device__ __forceinline__ uint64_t warp_top(const uint64_t* keys, int n) {
     return top;
 }
 
+// The 32 largest of `lists` sorted lists of n <= 32 keys one behind the other: list by list where they are long, else
+// all keys sorted.
+__device__ __forceinline__ uint64_t warp_top_lists(const uint64_t* keys, int lists, int n) {
+    const int lane = threadIdx.x & 31;
+    if (lists > 1 && n < 8) return warp_top(keys, lists * n);
+    uint64_t top = lane < n ? keys[lane] : 0;
+    for (int i = 1; i < lists; ++i) top = warp_merge(top, lane < n ? keys[i * n + lane] : 0);
+    return top;
+}
+
 // ---- One part of one row ---------------------------------------------------------
 // A CTA reads its part of a row once: each thread takes vectors of 16 bytes,
 // BEAM_VECS of them a chunk, and keeps the sum of 2^(z log2(e) - K) with a whole
@@ -131,7 +141,9 @@ __device__ __forceinline__ float beam_ex2(float v) {
 }
 // A row takes part if its beam has a score and is not finished.
 __device__ __forceinline__ bool beam_live(const float* scores, const uint8_t* finished, uint64_t row) {
-    return scores[row] > -INFINITY && !(finished && finished[row]);
+    const float score = scores[row];  // both are asked for before either is looked at
+    const uint8_t done = finished ? finished[row] : 0;
+    return score > -INFINITY && !done;
 }
 
 struct BeamRow {
@@ -148,9 +160,9 @@ struct BeamPartSmem {
 };
 
 // Part p.part of the row z: the calling CTA's first warp returns its `beams` best keys, a lane each, and all threads
-// (largest, total).
-template <typename T>
-__device__ __forceinline__ uint64_t beam_part(const T* z, const BeamRow& p, BeamPartSmem<T>& sm, float2* out) {
+// (largest, total).  live(): whether the row takes part at all; if not, there are no keys and (-inf, 0).
+template <typename T, typename Live>
+__device__ __forceinline__ uint64_t beam_part(const T* z, const BeamRow& p, BeamPartSmem<T>& sm, float2* out, Live live) {
     constexpr int E = BeamVector<T>::E, WARPS = BEAM_THREADS / 32;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int shift = (int)(((uintptr_t)z & 15) / sizeof(T));  // elements between the first vector's address and z
@@ -199,6 +211,10 @@ __device__ __forceinline__ uint64_t beam_part(const T* z, const BeamRow& p, Beam
         }
     };
     Chunk v, ahead;
+    if (!live()) {
+        *out = make_float2(-INFINITY, 0.0f);
+        return 0;
+    }
     if (n > 0) load(v, tile0);
     for (int j = 0; j < n; j += 2) {
         if (j + 1 < n) load(ahead, tile0 + j + 1);
@@ -307,7 +323,7 @@ struct BeamOut {
     uint8_t* finished;
 };
 struct BeamMergeSmem {
-    uint64_t key[BEAM_MAX * BEAM_MAX];
+    uint64_t top[BEAM_THREADS / 32][32];
     float score[BEAM_MAX * BEAM_MAX];
     int32_t token[BEAM_MAX * BEAM_MAX];
 };
@@ -316,13 +332,14 @@ __device__ __forceinline__ void beam_merge(const uint64_t* key, const float2* to
                                            const uint8_t* finished, int beams, uint32_t parts, int eos,
                                            const BeamOut& out, BeamMergeSmem& sm) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    uint64_t top = 0;  // the best candidates of this warp's beams
     for (int k = warp; k < beams; k += warps) {
         const uint64_t row = first + k;
         const float score = scores[row];
         float best = -INFINITY;
         int32_t token = max(eos, 0);
         if (beam_live(scores, finished, row)) {
-            const uint64_t mine = warp_top(key + (uint64_t)k * parts * beams, (int)(parts * beams));
+            const uint64_t mine = warp_top_lists(key + (uint64_t)k * parts * beams, (int)parts, beams);
             float largest = -INFINITY, sum = 0.0f;
             for (uint32_t i = lane; i < parts; i += 32) largest = fmaxf(largest, total[(uint64_t)k * parts + i].x);
             for (int o = 16; o; o >>= 1) largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, o));
@@ -339,25 +356,35 @@ __device__ __forceinline__ void beam_merge(const uint64_t* key, const float2* to
         } else if (lane == 0 && score > -INFINITY) {
             best = score;  // finished: it stays
         }
+        // a beam's candidates are in order: larger scores first, equal ones by place
+        const int at = k * beams + lane;
+        uint64_t list = 0;
         if (lane < beams) {
-            const int at = k * beams + lane;
             sm.score[at] = best, sm.token[at] = token;
-            sm.key[at] = best > -INFINITY ? (uint64_t)ordered(best) << 32 | (uint32_t)~at : 0;
+            if (best > -INFINITY) list = (uint64_t)ordered(best) << 32 | (uint32_t)~at;
+        }
+        top = k == warp ? list : warp_merge(top, list);
+    }
+    sm.top[warp][lane] = top;
+    int half = 1;
+    while (2 * half < min(warps, beams)) half *= 2;
+    for (; half && beams > 1; half >>= 1) {
+        __syncthreads();
+        if (warp < half && warp + half < warps) {
+            top = warp_merge(top, sm.top[warp + half][lane]);
+            sm.top[warp][lane] = top;
         }
     }
     __syncthreads();
-    if (warp == 0) {
-        const uint64_t mine = warp_top(sm.key, beams * beams);
-        if (lane < beams) {
-            const uint32_t at = ~(uint32_t)mine;
-            const bool any = mine != 0;
-            const uint64_t parent = any ? first + at / beams : first + lane;
-            const int32_t token = any ? sm.token[at] : max(eos, 0);
-            out.scores[first + lane] = any ? sm.score[at] : -INFINITY;
-            out.tokens[first + lane] = token;
-            out.parents[first + lane] = (int32_t)parent;
-            if (out.finished) out.finished[first + lane] = !any || (finished && finished[parent]) || token == eos;
-        }
+    if (warp == 0 && lane < beams) {
+        const uint32_t at = ~(uint32_t)top;
+        const bool any = top != 0;
+        const uint64_t parent = any ? first + at / beams : first + lane;
+        const int32_t token = any ? sm.token[at] : max(eos, 0);
+        out.scores[first + lane] = any ? sm.score[at] : -INFINITY;
+        out.tokens[first + lane] = token;
+        out.parents[first + lane] = (int32_t)parent;
+        if (out.finished) out.finished[first + lane] = !any || (finished && finished[parent]) || token == eos;
     }
 }
 
@@ -370,9 +397,9 @@ beam_rows_kernel(const T* logits, uint64_t stride, const float* scores, const ui
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const uint64_t row = blockIdx.x / parts;
     const uint32_t part = blockIdx.x - (uint32_t)row * parts;
-    if (!beam_live(scores, finished, row)) return;
     float2 total;
-    const uint64_t key = beam_part(logits + row * stride, BeamRow{beams, vocab, part, parts}, sm, &total);
+    const uint64_t key = beam_part(logits + row * stride, BeamRow{beams, vocab, part, parts}, sm, &total,
+                                   [&] { return beam_live(scores, finished, row); });
     if (threadIdx.x < beams) tmp.key[(row * parts + part) * beams + threadIdx.x] = key;
     if (threadIdx.x == 0) tmp.total[row * parts + part] = total;
 }
@@ -389,7 +416,7 @@ beam_merge_kernel(BeamTemp tmp, const float* scores, const uint8_t* finished, in
 constexpr int BEAM_CLUSTER = 8;
 
 template <typename T>
-__global__ void __launch_bounds__(BEAM_THREADS)
+__global__ void __launch_bounds__(BEAM_THREADS, 4)
 beam_cluster_kernel(const T* logits, uint64_t stride, const float* scores, const uint8_t* finished, int beams,
                     uint32_t vocab, uint32_t parts, int eos, BeamOut out) {
     __shared__ union {
@@ -401,10 +428,9 @@ beam_cluster_kernel(const T* logits, uint64_t stride, const float* scores, const
     asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");
     const uint32_t size = beams * parts, rank = blockIdx.x % size, part = rank % parts;
     const uint64_t first = (uint64_t)(blockIdx.x / size) * beams, row = first + rank / parts;
-    float2 total = make_float2(-INFINITY, 0.0f);
-    uint64_t key = 0;
-    if (beam_live(scores, finished, row))
-        key = beam_part(logits + row * stride, BeamRow{beams, vocab, part, parts}, sm.part, &total);
+    float2 total;
+    const uint64_t key = beam_part(logits + row * stride, BeamRow{beams, vocab, part, parts}, sm.part, &total,
+                                   [&] { return beam_live(scores, finished, row); });
     asm volatile("barrier.cluster.wait;" ::: "memory");  // the first CTA has started
     uint32_t key_at, total_at;
     asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(key_at) : "r"((uint32_t)__cvta_generic_to_shared(s_key)));
