@@ -10,3 +10,5 @@
 #include "lcpp/device/device_radix_sort.h"
 #include "lcpp/device/device_segment_reduce.h"
 #include "lcpp/device/device_multi_gpu.h"
+#include "lcpp/device/device_linear_recurrence.h"
+#include "lcpp/device/device_beam_search.h"
