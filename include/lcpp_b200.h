@@ -405,7 +405,9 @@ lcpp_status lcpp_lookback_probe(const uint64_t* descriptors, uint64_t tile,
  * kernel with CUDA events on the launching stream (0 turns it off); both
  * calls reset the totals.  lcpp_profile_read() waits for the recorded events
  * and returns, for one kernel kind ("reduce", "scan", "rs_memset",
- * "rs_histogram", "rs_bins_scan", "rs_onesweep", "seg_warp", "seg_block"),
+ * "rs_histogram", "rs_bins_scan", "rs_onesweep", "seg_warp", "seg_block",
+ * "lr_prepare", "lr_forward", "lr_backward", "lr_step", "beam_cluster",
+ * "beam_rows", "beam_merge", "beam_reorder"),
  * the number of timed launches and their summed duration in ms. */
 lcpp_status lcpp_profile_enable(int on);
 lcpp_status lcpp_profile_read(const char* kernel, uint64_t* launches, double* total_ms);

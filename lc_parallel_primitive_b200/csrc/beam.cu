@@ -79,7 +79,9 @@ __device__ __forceinline__ uint64_t warp_top_lists(const uint64_t* keys, int lis
 // the beams-th best logit of the part: only the few chunks that reach it are read
 // again (from L2), and what reaches it there is sorted.  The streaming loop thus
 // spends nothing on the selection but a maximum (half an instruction a 2-byte
-// element).
+// element).  512 rows of 100003 f32: 42.6 us on one B200 (4.8 TB/s, 73 % of the
+// copy rate), the rest being the end of each CTA, which all reach at about the
+// same time; 131072 bf16 41 us (4.5 instructions an element).
 constexpr int BEAM_VECS = 4;
 constexpr int BEAM_TILE = BEAM_THREADS * BEAM_VECS;  // vectors of a tile of a part
 constexpr int BEAM_TILES = 32;                       // tiles of a part at most
@@ -446,7 +448,9 @@ beam_cluster_kernel(const T* logits, uint64_t stride, const float* scores, const
 
 // ---- Reordering ------------------------------------------------------------------------
 // out[l][i] = in[l][parents[i]], rows of bytes; a negative parent: zeros.  A warp
-// copies BEAM_COPY vectors a lane of one row, all loads before the first store.
+// copies BEAM_COPY vectors a lane of one row, all loads before the first store
+// (268 MB of f32 states in 69 us, 7.8 TB/s of bytes asked for: repeated parents
+// come from L2).
 // V: 16- or 4-byte vectors where everything is a whole number of them, else
 // (V = 1) 4-byte words of out put together from the two words of in they lie
 // in, with single bytes at the row's ends.

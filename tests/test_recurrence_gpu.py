@@ -339,6 +339,25 @@ def test_graph_capture(cuda):
         assert np.array_equal(host(c.out), want)
 
 
+def test_look_back_gives_up(cuda):
+    # waits cut to two polls run out somewhere in a long chain: a status, and the context goes on
+    import torch
+
+    c = Case([20000], 64, "f32", "sigmoid", seed=24)
+    want = host(c.forward()[0])
+    lib = L.lib()
+    L.check(lib.lcpp_set_spin_limit(1))
+    try:
+        with pytest.raises(L.LcppError) as e:
+            for _ in range(20):
+                c.forward()
+        assert e.value.status == L.ERR_LOOKBACK_TIMEOUT
+    finally:
+        torch.cuda.synchronize()
+        L.check(lib.lcpp_set_spin_limit(0))
+    assert np.array_equal(host(c.forward()[0]), want)
+
+
 def test_long_cache_offsets_pass_32_bits(cuda):
     # element offsets beyond 2^32: rows of a wide buffer
     import torch
