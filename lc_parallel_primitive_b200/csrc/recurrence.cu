@@ -189,6 +189,13 @@ __device__ __forceinline__ float4 lr_get(const float4* r) {
 // from there down the tiles, state = A state + H, as those tiles do themselves:
 // the result does not depend on how far back the state was found.  Bounded by
 // the spin limit, after which the error word is set.
+// More records a read reach further where many tiles of a column are under way,
+// but take time and registers: 16 instead of LR_FAR (LR_NEAR) spill, and the
+// backward pass over 65536 x 1000 f32 takes 345 us instead of 238, though the
+// forward pass over 65536 x 128 bf16, with 74 tiles under way, 42 instead of 49;
+// 8 everywhere 60 there.
+constexpr int LR_NEAR = 6, LR_FAR = 12;
+
 template <int W>
 __device__ __forceinline__ float lr_lookback(const float4* r, int64_t step, uint32_t left, bool active) {
     const uint32_t limit = g_spin_limit;
@@ -205,12 +212,12 @@ __device__ __forceinline__ float lr_lookback(const float4* r, int64_t step, uint
             states |= lr_there(v[j].z) ? 1u << j : 0;
             maps |= lr_there(v[j].x) && lr_there(v[j].y) ? 1u << j : 0;
         }
-        const int from = __ffs(states) - 1;
+        const int from = __ffs(states) - 1;  // the nearest with a state, if all nearer ones have maps
         const bool found = from >= 0 && (~maps & ((1u << from) - 1)) == 0;
         if (__all_sync(0xffffffffu, found || !active)) {
             float carry = 0.0f;
 #pragma unroll
-            for (int j = W - 1; j >= 0; --j) carry = j >= from ? v[j].z : fmaf(v[j].x, carry, v[j].y);
+            for (int j = W - 1; j >= 0; --j) carry = j > from ? carry : j == from ? v[j].z : fmaf(v[j].x, carry, v[j].y);
             return carry;
         }
         if (spins >= limit) {
@@ -532,8 +539,8 @@ __global__ void __launch_bounds__(LrConfig<T>::THREADS, 1) lr_forward_kernel(LrF
             float carry = 0.0f;
             if (enters) {
                 const int64_t step = -(int64_t)ch.width;
-                carry = tl.narrow ? lr_lookback<16>(record + step, step, k, active)
-                                  : lr_lookback<8>(record + step, step, k, active);
+                carry = tl.narrow ? lr_lookback<LR_FAR>(record + step, step, k, active)
+                                  : lr_lookback<LR_NEAR>(record + step, step, k, active);
             }
             lr_sync((publishes ? 1 : 5) + b, Config::MAPPED);
             const uint32_t cuts = lr_cuts(sm.cut[b], 1);
@@ -779,8 +786,8 @@ __global__ void __launch_bounds__(LrConfig<T>::THREADS, 1) lr_backward_kernel(Lr
             code = last_code(i + 1);
             if (enters) {
                 const int64_t step = ch.width;
-                carry = tl.narrow ? lr_lookback<16>(record + step, step, t.x, active)
-                                  : lr_lookback<8>(record + step, step, t.x, active);
+                carry = tl.narrow ? lr_lookback<LR_FAR>(record + step, step, t.x, active)
+                                  : lr_lookback<LR_NEAR>(record + step, step, t.x, active);
             }
             lr_sync((publishes ? 1 : 5) + b, Config::MAPPED);
             const uint32_t cuts = lr_cuts(sm.cut[b], 2);
@@ -1201,7 +1208,7 @@ static lcpp_status lr_launch(size_t smem, const char* name, const P& p, const Lr
     if (row_tiles * col_tiles > 0x7fffffffull) return LCPP_ERR_INVALID_ARG;
     const DeviceInfo device = device_info();
     const uint64_t grid = min(row_tiles * col_tiles, (uint64_t)device.sms);
-    const LrTiles tl{(uint32_t)row_tiles, LrDivisor(col_tiles), (const uint32_t*)temp, grid > 6 * col_tiles};
+    const LrTiles tl{(uint32_t)row_tiles, LrDivisor(col_tiles), (const uint32_t*)temp, grid > LR_NEAR * col_tiles};
     static std::atomic<uint64_t> sized{0};  // devices on which the kernel may have this much shared memory
     const uint64_t bit = 1ull << device.device;
     if (!(sized.load(std::memory_order_relaxed) & bit)) {
