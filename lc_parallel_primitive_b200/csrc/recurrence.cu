@@ -23,10 +23,10 @@
 // tile into its maps, so that the chain from tile to tile has a whole tile's
 // time to arrive.
 //
-// Measured on one B200: forward 65536 x 2048 bf16 197 us (4.1 TB/s, 62 % of the
-// copy rate; 160 us with the chain's result dropped), f32 16384 x 2048 93 us;
-// backward 65536 x 2048 bf16 317 us (65 %).  Bound by instructions (33 and 68 an
-// element, 64-70 % of the issue slots), of which address and tile bookkeeping is
+// Measured on one B200: forward 65536 x 2048 bf16 196 us (4.1 TB/s, 63 % of the
+// copy rate; 160 us with the chain's result dropped), f32 16384 x 2048 87 us;
+// backward 65536 x 2048 bf16 316 us (65 %).  Bound by instructions (34 and 67 an
+// element, 64 and 77 % of the issue slots), of which address and tile bookkeeping is
 // half: 8 rows a lane do not amortise it, but 16 rows (with half the warps, or
 // two CTAs of 8 warps an SM) take 229-235 / 379-398 us, since either the warps
 // or the registers for two tiles at once run out.
@@ -454,7 +454,7 @@ __device__ __forceinline__ void lr_slot(LrSlot& slot, const LrShape& sh, uint64_
 
 // Asks for the states (C floats from `channel` on) of the sequences that begin (LR_HEAD) or end (LR_TAIL) in a warp's
 // rows of the next tile, so that they will be found in L1: a warp that waits for them there holds up its whole CTA
-// (backward, 32768 x 1536 f16 in 300 sequences: 184 us against 200 without).
+// (backward, 32768 x 1536 f16 in 300 sequences: 176 us against 188 without).
 template <int C>
 __device__ __forceinline__ void lr_touch(const LrShape& sh, uint32_t code, uint32_t mark, const float* from, uint64_t stride,
                                          uint32_t channel) {
