@@ -562,12 +562,20 @@ extern "C" lcpp_status lcpp_beam_select(int dtype, const void* logits, uint64_t 
     if (batches * beams > 1 && (logits_stride < vocab || logits_stride > 0x7fffffffull)) return LCPP_ERR_INVALID_ARG;
     if (!temp || temp_bytes < lcpp_beam_select_temp_bytes(batches, beams, vocab)) return LCPP_ERR_TEMP_TOO_SMALL;
     const uint64_t rows = batches * beams;
+    if (!elements_aligned(dtype, logits) || !elements_aligned(LCPP_F32, scores_in, scores_out, tokens_out, parents_out))
+        return LCPP_ERR_INVALID_ARG;
+    // outputs are written while inputs of the same entry may still be read
+    for (const void* o : {(const void*)scores_out, (const void*)tokens_out, (const void*)parents_out})
+        if (overlap(o, rows * 4, scores_in, rows * 4) || overlap(o, rows * 4, finished_in, rows)) return LCPP_ERR_INVALID_ARG;
+    if (overlap(finished_out, rows, scores_in, rows * 4) || overlap(finished_out, rows, finished_in, rows))
+        return LCPP_ERR_INVALID_ARG;
     cudaStream_t s = (cudaStream_t)stream;
     return dispatch_float(dtype, [&](auto t) -> lcpp_status {
         using T = decltype(t);
         const BeamOut out{scores_out, tokens_out, parents_out, finished_out};
         const uint64_t sms = device_info().sms;
         uint32_t parts = beam_parts(rows, vocab, sizeof(T), sms);
+        if (rows * parts > 0x7fffffffull) return LCPP_ERR_INVALID_ARG;
         // A cluster an entry, where that fills the SMs or leaves a CTA little to read.
         const uint32_t split = BEAM_CLUSTER / beams;
         const uint64_t tiles = beam_tiles(vocab, sizeof(T)), span = split ? ceil_div(tiles, std::min(split, parts)) : ~0ull;
@@ -586,11 +594,10 @@ extern "C" lcpp_status lcpp_beam_select(int dtype, const void* logits, uint64_t 
             ProfScope prof("beam_cluster", s);
             if (cudaLaunchKernelEx(&cfg, beam_cluster_kernel<T>, (const T*)logits, logits_stride, scores_in, finished_in,
                                    (int)beams, (uint32_t)vocab, parts, (int)eos_token, out) != cudaSuccess)
-                return LCPP_ERR_CUDA;
+                return check_launch();
             count_launch();
             return check_launch();
         }
-        if (rows * parts > 0x7fffffffull) return LCPP_ERR_INVALID_ARG;
         const BeamTemp tmp{(uint64_t*)temp, (float2*)((char*)temp + align_up(rows * parts * beams * 8, 256))};
         {
             ProfScope prof("beam_rows", s);
@@ -610,7 +617,7 @@ extern "C" lcpp_status lcpp_beam_select(int dtype, const void* logits, uint64_t 
         cfg.numAttrs = 1;
         if (cudaLaunchKernelEx(&cfg, beam_merge_kernel, tmp, scores_in, finished_in, (int)beams, parts, (int)eos_token,
                                out) != cudaSuccess)
-            return LCPP_ERR_CUDA;
+            return check_launch();
         count_launch(2);
         return check_launch();
     });
@@ -624,12 +631,13 @@ extern "C" lcpp_status lcpp_beam_reorder(const void* in, uint64_t in_layer_bytes
         return LCPP_ERR_INVALID_ARG;
     if (!rows || !layers || !row_bytes) return LCPP_OK;
     if (!in || !out || !parents || rows * layers > 0x7fffffffull) return LCPP_ERR_INVALID_ARG;
-    if ((rows_in > 1 && in_row_bytes < row_bytes) || (rows > 1 && out_row_bytes < row_bytes)) return LCPP_ERR_INVALID_ARG;
+    if ((rows_in > 1 && in_row_bytes < row_bytes) || (rows > 1 && out_row_bytes < row_bytes) ||
+        (layers > 1 && out_layer_bytes < row_bytes) || !elements_aligned(LCPP_I32, parents))
+        return LCPP_ERR_INVALID_ARG;
     // a row may be read after another row's copy took its place
-    const char *i0 = (const char*)in, *o0 = (const char*)out;
     const uint64_t in_span = (layers - 1) * in_layer_bytes + (rows_in ? rows_in - 1 : 0) * in_row_bytes + row_bytes;
     const uint64_t out_span = (layers - 1) * out_layer_bytes + (rows - 1) * out_row_bytes + row_bytes;
-    if (o0 < i0 + in_span && i0 < o0 + out_span) return LCPP_ERR_INVALID_ARG;
+    if (overlap(in, in_span, out, out_span)) return LCPP_ERR_INVALID_ARG;
     cudaStream_t s = (cudaStream_t)stream;
     uint64_t bits = (uint64_t)(uintptr_t)in | (uint64_t)(uintptr_t)out | row_bytes;
     if (layers > 1) bits |= in_layer_bytes | out_layer_bytes;

@@ -30,4 +30,15 @@ inline lcpp_status dispatch_float(int dtype, F&& f) {
 
 inline bool is_float_dtype(int dtype) { return dtype == LCPP_F32 || dtype == LCPP_F16 || dtype == LCPP_BF16; }
 
+// Every pointer is a whole number of elements (of 2 bytes for the half types, else 4).
+template <typename... P>
+inline bool elements_aligned(int dtype, const P*... p) {
+    return ((uintptr_t)0 | ... | (uintptr_t)p) % (dtype == LCPP_F16 || dtype == LCPP_BF16 ? 2 : 4) == 0;
+}
+
+inline bool overlap(const void* a, uint64_t a_bytes, const void* b, uint64_t b_bytes) {
+    const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
+    return a && b && a_bytes && b_bytes && x < y + b_bytes && y < x + a_bytes;
+}
+
 }  // namespace lcpp

@@ -1213,7 +1213,7 @@ static lcpp_status lr_launch(size_t smem, const char* name, const P& p, const Lr
     const uint64_t bit = 1ull << device.device;
     if (!(sized.load(std::memory_order_relaxed) & bit)) {
         if (cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
-            return LCPP_ERR_CUDA;
+            return check_launch();
         sized.fetch_or(bit, std::memory_order_relaxed);
     }
     cudaLaunchAttribute how[2];
@@ -1232,7 +1232,7 @@ static lcpp_status lr_launch(size_t smem, const char* name, const P& p, const Lr
         how[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
     }
     ProfScope prof(name, s);
-    if (cudaLaunchKernelEx(&cfg, KERNEL, p, lr_chain(temp, sh.rows, sh.channels), tl) != cudaSuccess) return LCPP_ERR_CUDA;
+    if (cudaLaunchKernelEx(&cfg, KERNEL, p, lr_chain(temp, sh.rows, sh.channels), tl) != cudaSuccess) return check_launch();
     count_launch();
     return LCPP_OK;
 }
@@ -1267,6 +1267,7 @@ extern "C" lcpp_status lcpp_linear_recurrence_forward(
     const lcpp_status ok = lr_check(gate, dtype, sh, gate_in, in);
     if (ok != LCPP_OK) return ok;
     if (!channels || !num_sequences) return LCPP_OK;
+    if (!elements_aligned(dtype, gate_in, in, out) || !elements_aligned(LCPP_F32, init, last, saved)) return LCPP_ERR_INVALID_ARG;
     if (rows && (!out || !lr_stride_ok(gate_stride, rows, channels) || !lr_stride_ok(in_stride, rows, channels) ||
                  !lr_stride_ok(out_stride, rows, channels)))
         return LCPP_ERR_INVALID_ARG;
@@ -1304,6 +1305,9 @@ extern "C" lcpp_status lcpp_linear_recurrence_backward(
     const lcpp_status ok = lr_check(gate, dtype, sh, gate_in, in);
     if (ok != LCPP_OK) return ok;
     if (!channels || !num_sequences) return LCPP_OK;
+    if (!elements_aligned(dtype, gate_in, in, grad_out, grad_gate, grad_in) ||
+        !elements_aligned(LCPP_F32, saved, init, grad_last, grad_init))
+        return LCPP_ERR_INVALID_ARG;
     if (rows && (!saved || !grad_gate || !grad_in || !lr_stride_ok(gate_stride, rows, channels) ||
                  !lr_stride_ok(in_stride, rows, channels) || !lr_stride_ok(grad_gate_stride, rows, channels) ||
                  !lr_stride_ok(grad_in_stride, rows, channels) ||
@@ -1347,10 +1351,11 @@ extern "C" lcpp_status lcpp_linear_recurrence_step(int gate, int dtype, const vo
     if (!gate_in || !in || !states_out || !lr_stride_ok(gate_stride, rows, channels) ||
         !lr_stride_ok(in_stride, rows, channels) || (out && !lr_stride_ok(out_stride, rows, channels)))
         return LCPP_ERR_INVALID_ARG;
+    if (!elements_aligned(dtype, gate_in, in, out) || !elements_aligned(LCPP_F32, states_in, parents, states_out))
+        return LCPP_ERR_INVALID_ARG;
     if (states_in && !parents && rows_in < rows) return LCPP_ERR_INVALID_ARG;
     if (parents && states_in) {  // a row may be read after another row's new state took its place
-        const char *i0 = (const char*)states_in, *o0 = (const char*)states_out;
-        if (o0 < i0 + rows_in * channels * sizeof(float) && i0 < o0 + rows * channels * sizeof(float))
+        if (overlap(states_in, rows_in * channels * sizeof(float), states_out, rows * channels * sizeof(float)))
             return LCPP_ERR_INVALID_ARG;
     }
     cudaStream_t s = (cudaStream_t)stream;

@@ -84,6 +84,34 @@ def test_reorder_refuses(kw):
     assert reorder(**kw) == L.ERR_INVALID_ARG
 
 
+ODD = ctypes.c_void_p(257)
+
+
+@pytest.mark.parametrize("call", [
+    lambda: forward(g=ODD), lambda: forward(out=ODD), lambda: forward(dtype=L.F32, x=ctypes.c_void_p(258)),
+    lambda: backward(gg=ODD), lambda: backward(saved=ctypes.c_void_p(258)), lambda: backward(go=ODD),
+    lambda: step(g=ODD), lambda: step(states=ctypes.c_void_p(258)), lambda: step(out=ODD),
+    lambda: select(z=ODD), lambda: select(scores=ctypes.c_void_p(258)), lambda: reorder(parents=ODD)])
+def test_a_part_of_an_element_is_no_address(call):
+    assert call() == L.ERR_INVALID_ARG
+
+
+@pytest.mark.parametrize("place", ["scores", "tokens", "parents", "finished"])
+@pytest.mark.parametrize("onto", ["scores", "finished"])
+def test_select_refuses_outputs_over_inputs(place, onto):
+    at = {n: ctypes.c_void_p((i + 2) << 16) for i, n in enumerate(["scores", "tokens", "parents", "finished"])}
+    inputs = dict(scores=ctypes.c_void_p(1 << 12), finished=ctypes.c_void_p(1 << 13))
+    at[place] = ctypes.c_void_p(inputs[onto].value + 4)
+    assert L.lib().lcpp_beam_select(L.BF16, ctypes.c_void_p(1 << 30), 100, inputs["scores"], inputs["finished"], at["scores"],
+                                    at["tokens"], at["parents"], at["finished"], 2, 4, 100, -1, BAD, BIG,
+                                    None) == L.ERR_INVALID_ARG
+
+
+def test_reorder_refuses_layers_over_each_other():
+    out = ctypes.c_void_p(1 << 30)
+    assert L.lib().lcpp_beam_reorder(BAD, 256, 64, out, 63, 64, BAD, 2, 4, 4, 64, None) == L.ERR_INVALID_ARG
+
+
 def test_sizes():
     lib = L.lib()
     assert lib.lcpp_linear_recurrence_saved_bytes(129, 64) >= 2 * 64 * 4
