@@ -561,6 +561,7 @@ extern "C" lcpp_status lcpp_beam_select(int dtype, const void* logits, uint64_t 
     if (!logits || !scores_in || !scores_out || !tokens_out || !parents_out) return LCPP_ERR_INVALID_ARG;
     if (batches * beams > 1 && (logits_stride < vocab || logits_stride > 0x7fffffffull)) return LCPP_ERR_INVALID_ARG;
     if (!temp || temp_bytes < lcpp_beam_select_temp_bytes(batches, beams, vocab)) return LCPP_ERR_TEMP_TOO_SMALL;
+    if ((uintptr_t)temp % sizeof(uint64_t)) return LCPP_ERR_INVALID_ARG;
     const uint64_t rows = batches * beams;
     if (!elements_aligned(dtype, logits) || !elements_aligned(LCPP_F32, scores_in, scores_out, tokens_out, parents_out))
         return LCPP_ERR_INVALID_ARG;

@@ -1272,6 +1272,7 @@ extern "C" lcpp_status lcpp_linear_recurrence_forward(
                  !lr_stride_ok(out_stride, rows, channels)))
         return LCPP_ERR_INVALID_ARG;
     if (!temp || temp_bytes < lcpp_linear_recurrence_temp_bytes(rows, channels)) return LCPP_ERR_TEMP_TOO_SMALL;
+    if ((uintptr_t)temp % sizeof(float4)) return LCPP_ERR_INVALID_ARG;
     const LrForward p{sh, gate_in, in, out, gate_stride, in_stride, out_stride, init_stride, init, last, (float*)saved};
     cudaStream_t s = (cudaStream_t)stream;
     bool prepared = false;
@@ -1314,6 +1315,7 @@ extern "C" lcpp_status lcpp_linear_recurrence_backward(
                  (grad_out && !lr_stride_ok(grad_out_stride, rows, channels))))
         return LCPP_ERR_INVALID_ARG;
     if (!temp || temp_bytes < lcpp_linear_recurrence_temp_bytes(rows, channels)) return LCPP_ERR_TEMP_TOO_SMALL;
+    if ((uintptr_t)temp % sizeof(float4)) return LCPP_ERR_INVALID_ARG;
     const LrBackward p{sh, gate_in, in, grad_out, grad_gate, grad_in, gate_stride, in_stride, grad_out_stride,
                        grad_gate_stride, grad_in_stride, init_stride, init, grad_last, (const float*)saved, grad_init};
     cudaStream_t s = (cudaStream_t)stream;
