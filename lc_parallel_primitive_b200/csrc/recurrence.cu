@@ -1267,7 +1267,8 @@ extern "C" lcpp_status lcpp_linear_recurrence_forward(
     const lcpp_status ok = lr_check(gate, dtype, sh, gate_in, in);
     if (ok != LCPP_OK) return ok;
     if (!channels || !num_sequences) return LCPP_OK;
-    if (!elements_aligned(dtype, gate_in, in, out) || !elements_aligned(LCPP_F32, init, last, saved)) return LCPP_ERR_INVALID_ARG;
+    if (!elements_aligned(dtype, gate_in, in, out) || !elements_aligned(LCPP_F32, offsets, init, last, saved))
+        return LCPP_ERR_INVALID_ARG;
     if (rows && (!out || !lr_stride_ok(gate_stride, rows, channels) || !lr_stride_ok(in_stride, rows, channels) ||
                  !lr_stride_ok(out_stride, rows, channels)))
         return LCPP_ERR_INVALID_ARG;
@@ -1307,7 +1308,7 @@ extern "C" lcpp_status lcpp_linear_recurrence_backward(
     if (ok != LCPP_OK) return ok;
     if (!channels || !num_sequences) return LCPP_OK;
     if (!elements_aligned(dtype, gate_in, in, grad_out, grad_gate, grad_in) ||
-        !elements_aligned(LCPP_F32, saved, init, grad_last, grad_init))
+        !elements_aligned(LCPP_F32, saved, offsets, init, grad_last, grad_init))
         return LCPP_ERR_INVALID_ARG;
     if (rows && (!saved || !grad_gate || !grad_in || !lr_stride_ok(gate_stride, rows, channels) ||
                  !lr_stride_ok(in_stride, rows, channels) || !lr_stride_ok(grad_gate_stride, rows, channels) ||

@@ -47,3 +47,8 @@ def test_recurrence_temp_holds_vectors(call, shift):
 def test_selection_temp_holds_keys(shift):
     # keys are 8 bytes
     assert select(temp=place(8, shift)) == L.ERR_INVALID_ARG
+
+
+@pytest.mark.parametrize("call", [forward, backward])
+def test_offsets_are_whole_words(call):
+    assert call(offsets=place(11, 2)) == L.ERR_INVALID_ARG
