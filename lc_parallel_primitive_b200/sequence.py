@@ -104,6 +104,15 @@ def _dense(t: Optional[torch.Tensor], shape, dtypes, name: str) -> Optional[int]
     return t.data_ptr()
 
 
+def _temp(t: Optional[torch.Tensor]):
+    """(pointer, bytes) of the temp buffer."""
+    if t is None:
+        return None, 0
+    if not t.is_contiguous():
+        raise ValueError("temp_storage must be contiguous")
+    return t.data_ptr(), _nbytes(t)
+
+
 class _Recorded(_Module):
     def _call(self, cmdlist, entry, args, keep, what) -> None:
         """Record entry(*args, stream); `keep`: the tensors that it uses."""
@@ -172,6 +181,7 @@ class DeviceLinearRecurrence(_Recorded):
         d_gate or d_in, and d_last may be d_init."""
         dt, gate = _float_dtype(d_gate, d_in, d_out), _gate(mode)
         offsets = offsets_or_length if isinstance(offsets_or_length, torch.Tensor) else None
+        temp, temp_bytes = _temp(temp_storage)
         keep = (d_gate, d_in, d_out, d_init, d_last, d_saved, temp_storage, offsets)
         _one_device(*keep)
         pg, sg, rows, channels = _matrix(d_gate, "d_gate")
@@ -183,7 +193,7 @@ class DeviceLinearRecurrence(_Recorded):
         ps = _saved(d_saved, rows, channels)
         self._call(cmdlist, L.lib().lcpp_linear_recurrence_forward,
                    (gate, dt, pg, sg, pi, si, po, so, rows, channels, count, length, off, p0, s0, pl, ps,
-                    temp_storage.data_ptr(), _nbytes(temp_storage)),
+                    temp, temp_bytes),
                    keep, "DeviceLinearRecurrence.Forward")
 
     def Backward(self, cmdlist, temp_storage, d_gate, d_in, d_saved, d_grad_out, d_grad_gate, d_grad_in,
@@ -195,6 +205,7 @@ class DeviceLinearRecurrence(_Recorded):
             raise ValueError("d_saved is needed: give it to Forward first")
         dt, gate = _float_dtype(d_gate, d_in, d_grad_out, d_grad_gate, d_grad_in), _gate(mode)
         offsets = offsets_or_length if isinstance(offsets_or_length, torch.Tensor) else None
+        temp, temp_bytes = _temp(temp_storage)
         keep = (d_gate, d_in, d_saved, d_grad_out, d_grad_gate, d_grad_in, d_init, d_grad_last, d_grad_init,
                 temp_storage, offsets)
         _one_device(*keep)
@@ -209,7 +220,7 @@ class DeviceLinearRecurrence(_Recorded):
         pg0 = _dense(d_grad_init, (count, channels), _F32, "d_grad_init")
         self._call(cmdlist, L.lib().lcpp_linear_recurrence_backward,
                    (gate, dt, pg, sg, pi, si, _saved(d_saved, rows, channels), p0, s0, pgo, sgo, pgl, pgg, sgg, pgi,
-                    sgi, pg0, rows, channels, count, length, off, temp_storage.data_ptr(), _nbytes(temp_storage)),
+                    sgi, pg0, rows, channels, count, length, off, temp, temp_bytes),
                    keep, "DeviceLinearRecurrence.Backward")
 
     def Step(self, cmdlist, d_gate, d_in, d_states_in, d_states_out, d_out=None, d_parents=None, mode="sigmoid"):
@@ -257,6 +268,7 @@ class DeviceBeamSearch(_Recorded):
         the token eos_token).  A finished beam offers itself, with eos_token and its score.  d_finished and
         d_finished_out may be None."""
         dt = _float_dtype(d_logits)
+        temp, temp_bytes = _temp(temp_storage)
         keep = (d_logits, d_scores, d_finished, d_scores_out, d_tokens_out, d_parents_out, d_finished_out, temp_storage)
         _one_device(*keep)
         shape = d_scores.shape
@@ -270,8 +282,7 @@ class DeviceBeamSearch(_Recorded):
         pt, pp = _dense(d_tokens_out, shape, _I32, "d_tokens_out"), _dense(d_parents_out, shape, _I32, "d_parents_out")
         pf, pfo = _dense(d_finished, shape, _U8, "d_finished"), _dense(d_finished_out, shape, _U8, "d_finished_out")
         self._call(cmdlist, L.lib().lcpp_beam_select,
-                   (dt, pz, sz, pi, pf, po, pt, pp, pfo, batches, beams, vocab, eos_token, temp_storage.data_ptr(),
-                    _nbytes(temp_storage)),
+                   (dt, pz, sz, pi, pf, po, pt, pp, pfo, batches, beams, vocab, eos_token, temp, temp_bytes),
                    keep, "DeviceBeamSearch.Select")
 
     def Reorder(self, cmdlist, d_in, d_out, d_parents):

@@ -52,3 +52,23 @@ def test_selection_temp_holds_keys(shift):
 @pytest.mark.parametrize("call", [forward, backward])
 def test_offsets_are_whole_words(call):
     assert call(offsets=place(11, 2)) == L.ERR_INVALID_ARG
+
+
+@pytest.mark.parametrize("view", ["strided", "expanded"])
+def test_python_temp_is_one_piece(view):
+    # its size is the number of bytes from its address on, which a view with gaps or repeats does not have
+    import torch
+    from lc_parallel_primitive_b200 import CommandList, DeviceBeamSearch, DeviceLinearRecurrence
+
+    temp = {"strided": torch.zeros(1 << 16, dtype=torch.int32)[::2],
+            "expanded": torch.zeros(1, dtype=torch.int32).expand(1 << 16)}[view]
+    x, c = torch.zeros((4, 8)), CommandList()
+    s, i = torch.zeros((1, 4)), torch.zeros((1, 4), dtype=torch.int32)
+    m = DeviceLinearRecurrence()
+    with pytest.raises(ValueError, match="temp_storage must be contiguous"):
+        m.Forward(c, temp, x, x, x, 4)
+    with pytest.raises(ValueError, match="temp_storage must be contiguous"):
+        m.Backward(c, temp, x, x, x, x, x, x, 4)
+    with pytest.raises(ValueError, match="temp_storage must be contiguous"):
+        DeviceBeamSearch().Select(c, temp, x, s, None, s, i, i, None)
+    assert len(c) == 0
