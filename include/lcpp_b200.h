@@ -260,7 +260,8 @@ lcpp_status lcpp_reduce_by_key(int op, int key_dtype, int value_dtype, const voi
  * last[s * channels + c] (NULL: not wanted) is h after the last row; an empty
  * sequence passes init on.  saved (NULL: no backward pass follows) receives
  * lcpp_linear_recurrence_saved_bytes() for the backward call.  out may be
- * gate or in, and last may be init (stride = channels).
+ * gate or in (with the same stride), and last may be init (stride = channels);
+ * what is written must not overlap anything else.
  * With LCPP_GATE_LINEAR the products of the gates along a stretch of up to
  * 128 rows must stay finite. */
 enum { LCPP_GATE_LINEAR = 0, LCPP_GATE_SIGMOID = 1 };

@@ -4,6 +4,7 @@
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+#include <utility>
 #include "common.cuh"
 
 namespace lcpp {
@@ -35,6 +36,39 @@ template <typename... P>
 inline bool elements_aligned(int dtype, const P*... p) {
     return ((uintptr_t)0 | ... | (uintptr_t)p) % (dtype == LCPP_F16 || dtype == LCPP_BF16 ? 2 : 4) == 0;
 }
+
+// Memory that a call reads or writes: `rows` pieces of `bytes` bytes, `stride` bytes from one to the next.
+struct Region {
+    uintptr_t at;
+    uint64_t rows, stride, bytes;
+    Region(const void* p, uint64_t n) : Region(p, 1, n, n) {}
+    Region(const void* p, uint64_t r, uint64_t s, uint64_t b)
+        : at((uintptr_t)p), rows(p && b ? r : 0), stride(r > 1 ? s : b), bytes(b) {}
+    // One piece lies on the other's, each row on its own.
+    bool same(const Region& o) const { return at == o.at && rows == o.rows && stride == o.stride && bytes == o.bytes; }
+    // Whether they have a byte in common.  Exact for one piece or equal strides (columns of one buffer, say); two
+    // matrices of different strides within each other's bounds count as overlapping.
+    bool meets(const Region& o) const {
+        if (!rows || !o.rows) return false;
+        Region a = joined(), b = o.joined();
+        if (b.at < a.at) std::swap(a, b);
+        const uint64_t d = b.at - a.at;
+        if (d >= (a.rows - 1) * a.stride + a.bytes) return false;
+        if (a.rows == 1 || (b.rows > 1 && b.stride != a.stride) || !a.stride) return true;
+        return d % a.stride < a.bytes || (d % a.stride + b.bytes > a.stride && d / a.stride + 1 < a.rows);
+    }
+    template <typename... R>
+    bool apart(const R&... others) const { return (!meets(others) && ...); }
+    template <typename... R>
+    bool apart_or_same(const R&... others) const { return ((same(others) || !meets(others)) && ...); }
+
+  private:
+    Region joined() const {  // rows without gaps are one piece
+        Region r = *this;
+        if (r.stride == r.bytes) r.bytes *= r.rows, r.stride = r.bytes, r.rows = 1;
+        return r;
+    }
+};
 
 inline bool overlap(const void* a, uint64_t a_bytes, const void* b, uint64_t b_bytes) {
     const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;

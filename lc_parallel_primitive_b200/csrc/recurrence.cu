@@ -1174,6 +1174,20 @@ static LrChain lr_chain(void* temp, uint64_t rows, uint64_t channels) {
     return LrChain{(float4*)((char*)temp + lr_code_bytes(rows)), lr_width(channels)};
 }
 
+// The operands' memory.  Tiles read and write at different times, so an output may be an input only where each element
+// is written by the lane that has read it: in the same place of the matrix.
+static Region lr_scratch(const LrShape& sh, const void* temp) {
+    return Region(temp, lr_code_bytes(sh.rows) + lr_chain_bytes(sh.rows, sh.channels));
+}
+static Region lr_matrix(const void* p, const LrShape& sh, uint64_t stride, uint64_t element) {
+    return Region(p, sh.rows, stride * element, sh.channels * element);
+}
+static Region lr_states(const float* p, const LrShape& sh, uint64_t stride) {
+    return Region(p, stride ? sh.sequences : 1, stride * 4, sh.channels * 4);
+}
+static Region lr_offsets(const LrShape& sh) { return Region(sh.offsets, (sh.sequences + 1) * 4); }
+static Region lr_saved(const void* p, const LrShape& sh) { return Region(p, ceil_div(sh.rows, LR_TILE) * sh.channels * 4); }
+
 // How the rows of these matrices can be copied.
 struct LrCopy {
     uint64_t bits;  // all addresses and byte strides or-ed together
@@ -1274,6 +1288,14 @@ extern "C" lcpp_status lcpp_linear_recurrence_forward(
         return LCPP_ERR_INVALID_ARG;
     if (!temp || temp_bytes < lcpp_linear_recurrence_temp_bytes(rows, channels)) return LCPP_ERR_TEMP_TOO_SMALL;
     if ((uintptr_t)temp % sizeof(float4)) return LCPP_ERR_INVALID_ARG;
+    const uint64_t e = dtype == LCPP_F32 ? 4 : 2;
+    const Region rg = lr_matrix(gate_in, sh, gate_stride, e), ri = lr_matrix(in, sh, in_stride, e),
+                 ro = lr_matrix(out, sh, out_stride, e), r0 = lr_states(init, sh, init_stride),
+                 rl = lr_states(last, sh, channels), rs = lr_saved(saved, sh), rt = lr_scratch(sh, temp),
+                 rf = lr_offsets(sh);
+    if (!ro.apart_or_same(rg, ri) || !ro.apart(r0, rl, rs, rt, rf) || !rl.apart_or_same(r0) ||
+        !rl.apart(rg, ri, rs, rt, rf) || !rs.apart(rg, ri, r0, rt, rf) || !rt.apart(rg, ri, r0, rf))
+        return LCPP_ERR_INVALID_ARG;
     const LrForward p{sh, gate_in, in, out, gate_stride, in_stride, out_stride, init_stride, init, last, (float*)saved};
     cudaStream_t s = (cudaStream_t)stream;
     bool prepared = false;

@@ -72,3 +72,39 @@ def test_python_temp_is_one_piece(view):
     with pytest.raises(ValueError, match="temp_storage must be contiguous"):
         DeviceBeamSearch().Select(c, temp, x, s, None, s, i, i, None)
     assert len(c) == 0
+
+
+# Matrices of 300 rows x 64 float32 elements, 76800 bytes; a row is 256 bytes.
+ROW, MATRIX, STATES = 256, 300 * 256, 3 * 256
+
+
+@pytest.mark.parametrize("kw", [
+    dict(out=place(1, ROW)), dict(out=place(2, 4)), dict(out=place(1, MATRIX - 4)),  # shifted against an input
+    dict(out=place(1), os=128), dict(out=place(2), gs=128, xs=128),                  # another stride
+    dict(out=place(1, 128), os=128, gs=128),                                         # half a row aside, strided
+    dict(last=place(4), ins=0), dict(last=place(4), ins=128), dict(last=place(4, ROW)),
+    dict(last=place(1)), dict(last=place(3, MATRIX - 4)), dict(out=place(4)),
+    dict(saved=place(1)), dict(saved=place(3)), dict(saved=place(4)), dict(saved=place(5, STATES - 4)),
+    dict(temp=place(3)), dict(temp=place(6)), dict(temp=place(1, MATRIX - 16)),
+    dict(offsets=place(3), out=place(3)), dict(offsets=place(5, 4)), dict(offsets=place(7, 4)),
+    dict(dtype=L.BF16, out=place(1, 2))])
+def test_forward_refuses_overlaps(kw):
+    assert forward(**kw) == L.ERR_INVALID_ARG
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_forward_within_one_buffer(cuda, dtype):
+    # gate, input and output as columns of one buffer do not overlap
+    import torch
+    from tests import sequence_reference as R
+    from tests.test_recurrence_gpu import Case, host
+
+    c = Case([150, 150], 64, dtype, "sigmoid", seed=40)
+    f = c.reference()
+    buf = torch.full((300, 192), 77.0, dtype=c.gate.dtype, device="cuda")
+    buf[:, :64], buf[:, 128:] = c.gate, c.x
+    c.gate, c.x = buf[:, :64], buf[:, 128:]
+    out, last = c.forward(out=buf[:, 64:128])
+    R.assert_within(host(out), f["out"], f["out_err"], dtype, "out")
+    R.assert_within(host(last), f["last"], f["last_err"], "f32", "last")
