@@ -276,7 +276,8 @@ lcpp_status lcpp_linear_recurrence_forward(int gate, int dtype, const void* gate
 /* Gradients from those of out (grad_out; NULL: 0) and last (grad_last, [num_sequences][channels]; NULL: 0),
  * given the forward call's gate_in, in, init and saved: grad_gate, grad_in and grad_init
  * ([num_sequences][channels], NULL: not wanted; one row per sequence also when init_stride is 0).
- * grad_gate and grad_in may be gate_in, in or grad_out (each with the same stride). */
+ * grad_gate and grad_in may be gate_in, in or grad_out (each with the same stride), and grad_init may be init
+ * (init_stride = channels); what is written must not overlap anything else, grad_last neither. */
 lcpp_status lcpp_linear_recurrence_backward(int gate, int dtype, const void* gate_in, uint64_t gate_stride,
                                             const void* in, uint64_t in_stride, const void* saved,
                                             const float* init, uint64_t init_stride, const void* grad_out,

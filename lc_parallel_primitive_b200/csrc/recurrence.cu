@@ -1339,6 +1339,16 @@ extern "C" lcpp_status lcpp_linear_recurrence_backward(
         return LCPP_ERR_INVALID_ARG;
     if (!temp || temp_bytes < lcpp_linear_recurrence_temp_bytes(rows, channels)) return LCPP_ERR_TEMP_TOO_SMALL;
     if ((uintptr_t)temp % sizeof(float4)) return LCPP_ERR_INVALID_ARG;
+    const uint64_t e = dtype == LCPP_F32 ? 4 : 2;
+    const Region rg = lr_matrix(gate_in, sh, gate_stride, e), ri = lr_matrix(in, sh, in_stride, e),
+                 ro = lr_matrix(grad_out, sh, grad_out_stride, e), rgg = lr_matrix(grad_gate, sh, grad_gate_stride, e),
+                 rgi = lr_matrix(grad_in, sh, grad_in_stride, e), r0 = lr_states(init, sh, init_stride),
+                 rl = lr_states(grad_last, sh, channels), rg0 = lr_states(grad_init, sh, channels),
+                 rs = lr_saved(saved, sh), rt = lr_scratch(sh, temp), rf = lr_offsets(sh);
+    if (!rgg.apart_or_same(rg, ri, ro) || !rgg.apart(rgi, r0, rl, rg0, rs, rt, rf) || !rgi.apart_or_same(rg, ri, ro) ||
+        !rgi.apart(r0, rl, rg0, rs, rt, rf) || !rg0.apart_or_same(r0) || !rg0.apart(rg, ri, ro, rl, rs, rt, rf) ||
+        !rt.apart(rg, ri, ro, r0, rl, rs, rf))
+        return LCPP_ERR_INVALID_ARG;
     const LrBackward p{sh, gate_in, in, grad_out, grad_gate, grad_in, gate_stride, in_stride, grad_out_stride,
                        grad_gate_stride, grad_in_stride, init_stride, init, grad_last, (const float*)saved, grad_init};
     cudaStream_t s = (cudaStream_t)stream;

@@ -178,7 +178,7 @@ class DeviceLinearRecurrence(_Recorded):
     def Forward(self, cmdlist, temp_storage, d_gate, d_in, d_out, offsets_or_length, d_init=None, d_last=None,
                 d_saved=None, mode="sigmoid"):
         """d_out = h; d_last = h after each sequence's last row (d_init for an empty sequence).  d_out may be
-        d_gate or d_in, and d_last may be d_init."""
+        d_gate or d_in (with the same row stride), and d_last may be d_init; other overlaps are refused."""
         dt, gate = _float_dtype(d_gate, d_in, d_out), _gate(mode)
         offsets = offsets_or_length if isinstance(offsets_or_length, torch.Tensor) else None
         temp, temp_bytes = _temp(temp_storage)
@@ -200,7 +200,8 @@ class DeviceLinearRecurrence(_Recorded):
                  offsets_or_length, d_init=None, d_grad_last=None, d_grad_init=None, mode="sigmoid"):
         """Gradients of d_gate, d_in and d_init from those of d_out (None: zero) and d_last (None: zero); d_gate,
         d_in, d_saved and d_init are the Forward call's.  d_grad_init has one row per sequence, also for an
-        expanded d_init (whose gradient is the sum of the rows)."""
+        expanded d_init (whose gradient is the sum of the rows).  d_grad_gate and d_grad_in may be d_gate, d_in or
+        d_grad_out (with the same row stride), and d_grad_init may be d_init; other overlaps are refused."""
         if d_saved is None:
             raise ValueError("d_saved is needed: give it to Forward first")
         dt, gate = _float_dtype(d_gate, d_in, d_grad_out, d_grad_gate, d_grad_in), _gate(mode)

@@ -108,3 +108,63 @@ def test_forward_within_one_buffer(cuda, dtype):
     out, last = c.forward(out=buf[:, 64:128])
     R.assert_within(host(out), f["out"], f["out_err"], dtype, "out")
     R.assert_within(host(last), f["last"], f["last_err"], "f32", "last")
+
+
+@pytest.mark.parametrize("kw", [
+    dict(gg=place(1, ROW)), dict(gi=place(2, 4)), dict(gg=place(3, MATRIX - 4)),  # shifted against an input
+    dict(gg=place(1), ggs=128), dict(gi=place(3), gs=128, xs=128, gos=128),       # another stride
+    dict(gg=place(9)), dict(gi=place(8, ROW)),                                    # one gradient over the other
+    dict(g0=place(5)), dict(g0=place(5, ROW)), dict(g0=place(4), ins=0), dict(g0=place(4, 4)),
+    dict(g0=place(8)), dict(g0=place(1)), dict(g0=place(6)),
+    dict(gg=place(6)), dict(gi=place(4)), dict(gg=place(5)),
+    dict(temp=place(3)), dict(temp=place(6)), dict(temp=place(10)), dict(temp=place(4)),
+    dict(offsets=place(8)), dict(offsets=place(10, 4)), dict(offsets=place(7, 4)),
+    dict(dtype=L.BF16, gg=place(1, 2))])
+def test_backward_refuses_overlaps(kw):
+    assert backward(**kw) == L.ERR_INVALID_ARG
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_backward_within_one_buffer(cuda, dtype):
+    # operands and gradients as columns of one buffer
+    import torch
+    from tests import sequence_reference as R
+    from tests.test_recurrence_gpu import Case, host
+
+    c = Case([150, 150], 64, dtype, "sigmoid", seed=41)
+    f = c.reference()
+    want = R.backward(f, host(c.grad_out), host(c.grad_last))
+    buf = torch.full((300, 320), 77.0, dtype=c.gate.dtype, device="cuda")
+    for name, at in (("gate", 0), ("x", 128), ("grad_out", 256)):
+        buf[:, at:at + 64] = getattr(c, name)
+        setattr(c, name, buf[:, at:at + 64])
+    c.forward()
+    gg, gi, g0 = c.backward(grad_gate=buf[:, 64:128], grad_in=buf[:, 192:256])
+    R.assert_within(host(gg), want["grad_gate"], want["grad_gate_err"], dtype, "grad_gate")
+    R.assert_within(host(gi), want["grad_in"], want["grad_in_err"], dtype, "grad_in")
+    R.assert_within(host(g0), want["grad_init"], want["grad_init_err"], "f32", "grad_init")
+
+
+@pytest.mark.gpu
+def test_grad_init_in_the_place_of_init(cuda):
+    # a state is read by the lanes that write its gradient later, and by no others
+    import torch
+    from lc_parallel_primitive_b200 import CommandList, DeviceLinearRecurrence, Stream
+    from tests import sequence_reference as R
+    from tests.test_recurrence_gpu import Case, host
+
+    c = Case([3, 0, 300, 1, 1, 150], 72, "f32", "sigmoid", seed=42, packed=True)
+    f = c.reference()
+    want = R.backward(f, host(c.grad_out), host(c.grad_last))
+    c.forward()
+    m, cl = DeviceLinearRecurrence(), CommandList()
+    m.create()
+    gg, gi = c.matrix(), c.matrix()
+    m.Backward(cl, c.temp, c.gate, c.x, c.saved, c.grad_out, gg, gi, c.sequences, d_init=c.init,
+               d_grad_last=c.grad_last, d_grad_init=c.init)
+    Stream() << cl.commit()
+    torch.cuda.synchronize()
+    R.assert_within(host(gg), want["grad_gate"], want["grad_gate_err"], "f32", "grad_gate")
+    R.assert_within(host(gi), want["grad_in"], want["grad_in_err"], "f32", "grad_in")
+    R.assert_within(host(c.init), want["grad_init"], want["grad_init_err"], "f32", "grad_init")
