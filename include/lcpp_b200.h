@@ -289,7 +289,8 @@ lcpp_status lcpp_linear_recurrence_backward(int gate, int dtype, const void* gat
 /* One token: row i goes on from states_in[parents[i]] (parents NULL: row i; a negative parent or states_in NULL:
  * zeros; a parent >= rows_in: zeros, and LCPP_ERR_INVALID_ARG in the device error word) and writes states_out[i]
  * and its rounding to dtype, out[i] (NULL: not wanted).  States are [rows][channels] float32.  states_out may be
- * states_in when parents is NULL, else they must not overlap. */
+ * states_in when parents is NULL, and out may be gate_in or in (with the same stride); what is written must not
+ * overlap anything else. */
 lcpp_status lcpp_linear_recurrence_step(int gate, int dtype, const void* gate_in, uint64_t gate_stride,
                                         const void* in, uint64_t in_stride, const float* states_in,
                                         uint64_t rows_in, const int32_t* parents, float* states_out, void* out,

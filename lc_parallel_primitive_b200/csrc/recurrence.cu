@@ -1389,10 +1389,14 @@ extern "C" lcpp_status lcpp_linear_recurrence_step(int gate, int dtype, const vo
     if (!elements_aligned(dtype, gate_in, in, out) || !elements_aligned(LCPP_F32, states_in, parents, states_out))
         return LCPP_ERR_INVALID_ARG;
     if (states_in && !parents && rows_in < rows) return LCPP_ERR_INVALID_ARG;
-    if (parents && states_in) {  // a row may be read after another row's new state took its place
-        if (overlap(states_in, rows_in * channels * sizeof(float), states_out, rows * channels * sizeof(float)))
-            return LCPP_ERR_INVALID_ARG;
-    }
+    const uint64_t e = dtype == LCPP_F32 ? 4 : 2;
+    const Region rg(gate_in, rows, gate_stride * e, channels * e), ri(in, rows, in_stride * e, channels * e),
+        ro(out, rows, out_stride * e, channels * e), rn(states_out, rows, channels * 4, channels * 4),
+        rs(states_in, parents ? rows_in : rows, channels * 4, channels * 4), rp(parents, rows * 4);
+    if (!rn.apart_or_same(rg, ri, ro) || !rn.apart(rp) || !ro.apart_or_same(rg, ri) || !ro.apart(rp))
+        return LCPP_ERR_INVALID_ARG;
+    // with parents a row may be read after another row's new state took its place
+    if (parents ? !rs.apart(rn, ro) : !rs.apart_or_same(rn, ro)) return LCPP_ERR_INVALID_ARG;
     cudaStream_t s = (cudaStream_t)stream;
     return lr_dispatch(gate, dtype, [&](auto t, auto g) -> lcpp_status {
         using T = decltype(t);

@@ -227,7 +227,8 @@ class DeviceLinearRecurrence(_Recorded):
     def Step(self, cmdlist, d_gate, d_in, d_states_in, d_states_out, d_out=None, d_parents=None, mode="sigmoid"):
         """One token for each row: row i goes on from d_states_in[d_parents[i]] (without d_parents row i, a negative
         parent from zeros) to d_states_out[i], and d_out[i] is its rounding.  d_states_out may be d_states_in when
-        there are no parents."""
+        there are no parents, and d_out may be d_gate or d_in (with the same row stride); other overlaps are
+        refused."""
         dt, gate = _float_dtype(d_gate, d_in, d_out), _gate(mode)
         keep = (d_gate, d_in, d_states_in, d_states_out, d_out, d_parents)
         _one_device(*keep)

@@ -168,3 +168,65 @@ def test_grad_init_in_the_place_of_init(cuda):
     R.assert_within(host(gg), want["grad_gate"], want["grad_gate_err"], "f32", "grad_gate")
     R.assert_within(host(gi), want["grad_in"], want["grad_in_err"], "f32", "grad_in")
     R.assert_within(host(c.init), want["grad_init"], want["grad_init_err"], "f32", "grad_init")
+
+
+def step(gate=L.GATE_SIGMOID, dtype=L.F32, g=place(1), gs=64, x=place(2), xs=64, states=place(3), rows_in=300, parents=None,
+         new=place(4), out=place(5), os=64, rows=300, d=64):
+    return L.lib().lcpp_linear_recurrence_step(gate, dtype, g, gs, x, xs, states, rows_in, parents, new, out, os, rows, d,
+                                               None)
+
+
+@pytest.mark.parametrize("kw", [
+    dict(new=place(3, ROW)), dict(new=place(3, 4)), dict(states=place(4, MATRIX - 4)),  # shifted states
+    dict(out=place(3, ROW)), dict(out=place(3), os=128), dict(out=place(4, 4)),
+    dict(dtype=L.BF16, out=place(3)), dict(dtype=L.BF16, out=place(4)),
+    dict(out=place(1, ROW)), dict(out=place(2), os=128), dict(new=place(1, 4)),
+    dict(parents=place(6), new=place(3)), dict(parents=place(6), out=place(3)),
+    dict(parents=place(5, 4)), dict(parents=place(4, 4)),
+    dict(parents=place(6), rows_in=400, out=place(3, MATRIX))])
+def test_step_refuses_overlaps(kw):
+    assert step(**kw) == L.ERR_INVALID_ARG
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("out", ["gate", "in", "states", "new"])
+def test_step_outputs_in_the_place_of_operands(cuda, out):
+    # float32 without parents: every operand has the same layout, and each lane reads what it writes before
+    import torch
+    from lc_parallel_primitive_b200 import CommandList, DeviceLinearRecurrence, Stream
+    from tests import sequence_reference as R
+    from tests.test_recurrence_gpu import Case, host
+
+    c = Case([1] * 33, 100, "f32", "sigmoid", seed=43)
+    f = c.reference()
+    new = torch.empty((33, 100), device="cuda")
+    o = {"gate": c.gate, "in": c.x, "states": c.init, "new": new}[out]
+    m, cl = DeviceLinearRecurrence(), CommandList()
+    m.create()
+    m.Step(cl, c.gate, c.x, c.init, new, o)
+    Stream() << cl.commit()
+    torch.cuda.synchronize()
+    R.assert_within(host(new), f["out"], f["out_err"], "f32", "states")
+    R.assert_within(host(o), f["out"], f["out_err"], "f32", "out")
+
+
+@pytest.mark.gpu
+def test_step_within_one_buffer(cuda):
+    # old and new states as the halves of one buffer, gate, input and output as columns of another
+    import torch
+    from lc_parallel_primitive_b200 import CommandList, DeviceLinearRecurrence, Stream
+    from tests import sequence_reference as R
+    from tests.test_recurrence_gpu import Case, host
+
+    c = Case([1] * 9, 72, "bf16", "sigmoid", seed=44)
+    f = c.reference()
+    states = torch.cat([c.init, torch.zeros_like(c.init)])
+    buf = torch.cat([c.gate, c.x, torch.zeros_like(c.x)], dim=1)
+    m, cl = DeviceLinearRecurrence(), CommandList()
+    m.create()
+    m.Step(cl, buf[:, :72], buf[:, 72:144], states[:9], states[9:], buf[:, 144:],
+           d_parents=torch.arange(9, dtype=torch.int32, device="cuda"))
+    Stream() << cl.commit()
+    torch.cuda.synchronize()
+    R.assert_within(host(states[9:]), f["out"], f["out_err"], "f32", "states")
+    R.assert_within(host(buf[:, 144:]), f["out"], f["out_err"], "bf16", "out")
