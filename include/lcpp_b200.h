@@ -304,7 +304,7 @@ lcpp_status lcpp_linear_recurrence_step(int gate, int dtype, const void* gate_in
  * tokens_out, parents_out (the candidate's row) and finished_out (NULL: not wanted; 1 where the parent was
  * finished or the token is eos_token; eos_token < 0: there is none).  A logit or score of -inf or NaN offers no
  * candidate; an output that no candidate is left for has score -inf, token max(eos_token, 0), its own row as parent
- * and is finished.  beams <= 32; outputs must not overlap inputs. */
+ * and is finished.  beams <= 32; outputs and temp must not overlap inputs or one another. */
 size_t      lcpp_beam_select_temp_bytes(uint64_t batches, uint32_t beams, uint64_t vocab);
 lcpp_status lcpp_beam_select(int dtype, const void* logits, uint64_t logits_stride, const float* scores_in,
                              const uint8_t* finished_in, float* scores_out, int32_t* tokens_out,

@@ -566,9 +566,12 @@ extern "C" lcpp_status lcpp_beam_select(int dtype, const void* logits, uint64_t 
     if (!elements_aligned(dtype, logits) || !elements_aligned(LCPP_F32, scores_in, scores_out, tokens_out, parents_out))
         return LCPP_ERR_INVALID_ARG;
     // outputs are written while inputs of the same entry may still be read
-    for (const void* o : {(const void*)scores_out, (const void*)tokens_out, (const void*)parents_out})
-        if (overlap(o, rows * 4, scores_in, rows * 4) || overlap(o, rows * 4, finished_in, rows)) return LCPP_ERR_INVALID_ARG;
-    if (overlap(finished_out, rows, scores_in, rows * 4) || overlap(finished_out, rows, finished_in, rows))
+    const uint64_t e = dtype == LCPP_F32 ? 4 : 2;
+    const Region rz(logits, rows, logits_stride * e, vocab * e), rs(scores_in, rows * 4), rf(finished_in, rows),
+        so(scores_out, rows * 4), to(tokens_out, rows * 4), po(parents_out, rows * 4), fo(finished_out, rows),
+        rt(temp, lcpp_beam_select_temp_bytes(batches, beams, vocab));
+    if (!so.apart(rz, rs, rf, to, po, fo, rt) || !to.apart(rz, rs, rf, po, fo, rt) || !po.apart(rz, rs, rf, fo, rt) ||
+        !fo.apart(rz, rs, rf, rt) || !rt.apart(rz, rs, rf))
         return LCPP_ERR_INVALID_ARG;
     cudaStream_t s = (cudaStream_t)stream;
     return dispatch_float(dtype, [&](auto t) -> lcpp_status {

@@ -268,7 +268,7 @@ class DeviceBeamSearch(_Recorded):
         `beams` best of an entry come out, best first, with their token, their parent (a row of d_logits, for
         Reorder and DeviceLinearRecurrence.Step) and whether they are finished (d_finished of the parent, or
         the token eos_token).  A finished beam offers itself, with eos_token and its score.  d_finished and
-        d_finished_out may be None."""
+        d_finished_out may be None.  Outputs that overlap an input or one another are refused."""
         dt = _float_dtype(d_logits)
         temp, temp_bytes = _temp(temp_storage)
         keep = (d_logits, d_scores, d_finished, d_scores_out, d_tokens_out, d_parents_out, d_finished_out, temp_storage)

@@ -230,3 +230,38 @@ def test_step_within_one_buffer(cuda):
     torch.cuda.synchronize()
     R.assert_within(host(states[9:]), f["out"], f["out_err"], "f32", "states")
     R.assert_within(host(buf[:, 144:]), f["out"], f["out_err"], "bf16", "out")
+
+
+@pytest.mark.parametrize("kw", [
+    dict(so=place(5)), dict(so=place(6, 28)), dict(to=place(6, 4)), dict(fo=place(4, 31)), dict(fo=place(5, 4)),
+    dict(so=place(1)), dict(to=place(1, 3196)), dict(po=place(1, 1600)), dict(fo=place(1, 3199)),
+    dict(temp=place(4)), dict(temp=place(1)), dict(temp=place(2)), dict(temp=place(3)), dict(fo=place(8)),
+    dict(stride=200, to=place(1, 800 + 396))])
+def test_select_refuses_overlaps(kw):
+    # 8 rows of 100 float32 logits, 3200 bytes; outputs of 32 bytes (8 of finished)
+    assert select(**kw) == L.ERR_INVALID_ARG
+
+
+@pytest.mark.gpu
+def test_select_within_one_buffer(cuda):
+    # scores and choices as rows of one buffer, logits as columns of another
+    import numpy as np
+    import torch
+    from lc_parallel_primitive_b200 import CommandList, DeviceBeamSearch, Stream, temp_buffer
+    from tests import sequence_reference as R
+
+    wide = torch.randn((8, 500), generator=torch.Generator().manual_seed(45)).cuda()
+    logits = wide[:, 100:400]
+    scores = torch.zeros((2, 4), device="cuda")
+    scores[:] = torch.tensor([0.0, -0.5, -1.0, -1.5])
+    words = torch.zeros((2, 2, 4), dtype=torch.int32, device="cuda")
+    both = torch.stack([scores, torch.zeros_like(scores)])
+    m, c = DeviceBeamSearch(), CommandList()
+    m.create()
+    m.Select(c, temp_buffer(m.GetTempStorageBytes(2, 4, 300)), logits, both[0], None, both[1], words[0], words[1], None)
+    Stream() << c.commit()
+    torch.cuda.synchronize()
+    s, t, p, _, gap = R.beam_select(logits.cpu().numpy(), scores.cpu().numpy(), None, -1)
+    assert (gap > 1e-4).all()  # no two choices of this seed that rounding could swap
+    assert np.allclose(both[1].cpu().numpy(), s, rtol=0, atol=1e-5)
+    assert np.array_equal(words[0].cpu().numpy(), t) and np.array_equal(words[1].cpu().numpy(), p)
