@@ -638,10 +638,18 @@ extern "C" lcpp_status lcpp_beam_reorder(const void* in, uint64_t in_layer_bytes
     if ((rows_in > 1 && in_row_bytes < row_bytes) || (rows > 1 && out_row_bytes < row_bytes) ||
         (layers > 1 && out_layer_bytes < row_bytes) || !elements_aligned(LCPP_I32, parents))
         return LCPP_ERR_INVALID_ARG;
-    // a row may be read after another row's copy took its place
-    const uint64_t in_span = (layers - 1) * in_layer_bytes + (rows_in ? rows_in - 1 : 0) * in_row_bytes + row_bytes;
-    const uint64_t out_span = (layers - 1) * out_layer_bytes + (rows - 1) * out_row_bytes + row_bytes;
-    if (overlap(in, in_span, out, out_span)) return LCPP_ERR_INVALID_ARG;
+    // A row may be read after another row's copy took its place.  Apart as they lie, as layers (halves of each layer of
+    // one buffer, say) or as rows a stride apart.
+    const uint64_t in_block = rows_in ? (rows_in - 1) * in_row_bytes + row_bytes : 0;
+    const uint64_t out_block = (rows - 1) * out_row_bytes + row_bytes;
+    bool apart = Region(in, layers, in_layer_bytes, in_block).apart(Region(out, layers, out_layer_bytes, out_block));
+    if (!apart && rows_in > 1 && rows > 1 && in_row_bytes == out_row_bytes &&
+        (layers == 1 || (in_layer_bytes | out_layer_bytes) % in_row_bytes == 0)) {
+        const uint64_t l = layers - 1, r = in_row_bytes;
+        apart = Region(in, l * (in_layer_bytes / r) + rows_in, r, row_bytes)
+                    .apart(Region(out, l * (out_layer_bytes / r) + rows, r, row_bytes));
+    }
+    if (!apart) return LCPP_ERR_INVALID_ARG;
     cudaStream_t s = (cudaStream_t)stream;
     uint64_t bits = (uint64_t)(uintptr_t)in | (uint64_t)(uintptr_t)out | row_bytes;
     if (layers > 1) bits |= in_layer_bytes | out_layer_bytes;

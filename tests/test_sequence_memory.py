@@ -265,3 +265,39 @@ def test_select_within_one_buffer(cuda):
     assert (gap > 1e-4).all()  # no two choices of this seed that rounding could swap
     assert np.allclose(both[1].cpu().numpy(), s, rtol=0, atol=1e-5)
     assert np.array_equal(words[0].cpu().numpy(), t) and np.array_equal(words[1].cpu().numpy(), p)
+
+
+def reorder(x=place(1), lin=256, rin=64, out=place(2), lout=256, rout=64, parents=place(3), layers=2, rows_in=4, rows=4,
+            width=64):
+    return L.lib().lcpp_beam_reorder(x, lin, rin, out, lout, rout, parents, layers, rows_in, rows, width, None)
+
+
+@pytest.mark.parametrize("kw", [
+    dict(out=place(1)), dict(out=place(1, 448)), dict(x=place(2, 255)), dict(out=place(1, 64), lin=512, lout=512),
+    dict(out=place(1, 200), lin=512, lout=512), dict(out=place(1, 300), lin=512, lout=512),  # into the next layer
+    dict(out=place(1, 63), lin=512, lout=512, rin=128, rout=128), dict(out=place(1, 65), lin=512, lout=512, rin=128, rout=128),
+    dict(out=place(1, 256), lin=512, lout=256), dict(out=place(1, 64), lin=0)])
+def test_reorder_refuses_overlaps(kw):
+    assert reorder(**kw) == L.ERR_INVALID_ARG
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("split", [1, 2])
+@pytest.mark.parametrize("width", [16, 33])
+def test_reorder_between_halves_of_one_buffer(cuda, split, width):
+    # (layers, 2, rows, width) and (layers, rows, 2, width): old and new states alternate, and do not overlap
+    import torch
+    from lc_parallel_primitive_b200 import CommandList, DeviceBeamSearch, Stream
+
+    shape = (3, 2, 5, width) if split == 1 else (3, 5, 2, width)
+    buf = torch.randn(shape, device="cuda")
+    old, new = buf.unbind(split)
+    parents = torch.tensor([4, 0, 0, -1, 2], dtype=torch.int32, device="cuda")
+    want = torch.where(parents[:, None] >= 0, old[:, parents.clamp(min=0).long()], torch.zeros((), device="cuda"))
+    before = old.clone()
+    m, c = DeviceBeamSearch(), CommandList()
+    m.create()
+    m.Reorder(c, old, new, parents)
+    Stream() << c.commit()
+    torch.cuda.synchronize()
+    assert torch.equal(new, want) and torch.equal(old, before)
