@@ -638,6 +638,15 @@ extern "C" lcpp_status lcpp_beam_reorder(const void* in, uint64_t in_layer_bytes
     if ((rows_in > 1 && in_row_bytes < row_bytes) || (rows > 1 && out_row_bytes < row_bytes) ||
         (layers > 1 && out_layer_bytes < row_bytes) || !elements_aligned(LCPP_I32, parents))
         return LCPP_ERR_INVALID_ARG;
+    // no two rows of out in one place: with neither all of a layer nor all of a row's layers together, layers that are
+    // dl apart must not come as near as row_bytes to rows that are di apart
+    if (layers > 1 && rows > 1 && out_layer_bytes < (rows - 1) * out_row_bytes + row_bytes &&
+        out_row_bytes < (layers - 1) * out_layer_bytes + row_bytes)
+        for (uint64_t dl = 1; dl < layers && dl * out_layer_bytes < (rows - 1) * out_row_bytes + row_bytes; ++dl) {
+            const uint64_t at = dl * out_layer_bytes, di = at / out_row_bytes, past = at % out_row_bytes;
+            if ((di >= 1 && di < rows && past < row_bytes) || (di + 1 < rows && out_row_bytes - past < row_bytes))
+                return LCPP_ERR_INVALID_ARG;
+        }
     // A row may be read after another row's copy took its place.  Apart as they lie, as layers (halves of each layer of
     // one buffer, say) or as rows a stride apart.
     const uint64_t in_block = rows_in ? (rows_in - 1) * in_row_bytes + row_bytes : 0;

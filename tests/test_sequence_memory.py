@@ -301,3 +301,30 @@ def test_reorder_between_halves_of_one_buffer(cuda, split, width):
     Stream() << c.commit()
     torch.cuda.synchronize()
     assert torch.equal(new, want) and torch.equal(old, before)
+
+
+@pytest.mark.parametrize("kw", [
+    dict(lout=64), dict(lout=128), dict(lout=192), dict(lout=191, rout=128), dict(lout=100, rout=70, layers=3),
+    dict(lout=130, rout=64, layers=3, rows=3)])
+def test_reorder_refuses_rows_of_layers_over_each_other(kw):
+    # two layers' rows in one place would be written in any order
+    assert reorder(**kw) == L.ERR_INVALID_ARG
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("layer,row", [(64, 192), (64, 200), (320, 64), (96, 224), (160, 64), (192, 128)])
+def test_reorder_to_interleaved_layers(cuda, layer, row):
+    # 3 layers x 4 rows of 32 bytes whose places are apart, though not all one behind the other
+    import torch
+    from lc_parallel_primitive_b200 import CommandList, DeviceBeamSearch, Stream
+
+    layers, rows = (2, 2) if (layer, row) == (96, 224) else (3, 4)
+    x = torch.randint(0, 255, (layers, rows, 32), device="cuda", dtype=torch.uint8)
+    buf = torch.full((2 * layer + 3 * row + 32,), 7, dtype=torch.uint8, device="cuda")
+    out = buf.as_strided((layers, rows, 32), (layer, row, 1))
+    m, c = DeviceBeamSearch(), CommandList()
+    m.create()
+    m.Reorder(c, x, out, torch.arange(rows - 1, -1, -1, dtype=torch.int32, device="cuda"))
+    Stream() << c.commit()
+    torch.cuda.synchronize()
+    assert torch.equal(out, x.flip(1))
