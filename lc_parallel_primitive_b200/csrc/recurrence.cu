@@ -1155,7 +1155,7 @@ static lcpp_status lr_check(int gate, int dtype, const LrShape& sh, const void* 
     if ((gate != LCPP_GATE_LINEAR && gate != LCPP_GATE_SIGMOID) || !is_float_dtype(dtype)) return LCPP_ERR_INVALID_ARG;
     if (sh.rows > LR_MAX_ROWS || sh.channels > LR_MAX_CHANNELS || sh.sequences > LR_SEQUENCE) return LCPP_ERR_INVALID_ARG;
     if (!sh.offsets && sh.sequences * sh.length.d != sh.rows) return LCPP_ERR_INVALID_ARG;
-    if (sh.rows && sh.channels && (!gate_in || !in || !sh.sequences)) return LCPP_ERR_INVALID_ARG;
+    if (sh.rows && sh.channels && (!gate_in || !in || (!sh.sequences && !sh.offsets))) return LCPP_ERR_INVALID_ARG;
     return LCPP_OK;
 }
 // A row stride must reach past the channels (one row may have any).
@@ -1280,7 +1280,8 @@ extern "C" lcpp_status lcpp_linear_recurrence_forward(
     const LrShape sh{rows, channels, num_sequences, LrDivisor(offsets ? 0 : length), offsets};
     const lcpp_status ok = lr_check(gate, dtype, sh, gate_in, in);
     if (ok != LCPP_OK) return ok;
-    if (!channels || !num_sequences) return LCPP_OK;
+    if (!channels || (!num_sequences && !rows)) return LCPP_OK;
+    if (!num_sequences) init = nullptr, last = nullptr;  // all rows are padding, and no state exists
     if (!elements_aligned(dtype, gate_in, in, out) || !elements_aligned(LCPP_F32, offsets, init, last, saved))
         return LCPP_ERR_INVALID_ARG;
     if (rows && (!out || !lr_stride_ok(gate_stride, rows, channels) || !lr_stride_ok(in_stride, rows, channels) ||
@@ -1328,7 +1329,8 @@ extern "C" lcpp_status lcpp_linear_recurrence_backward(
     const LrShape sh{rows, channels, num_sequences, LrDivisor(offsets ? 0 : length), offsets};
     const lcpp_status ok = lr_check(gate, dtype, sh, gate_in, in);
     if (ok != LCPP_OK) return ok;
-    if (!channels || !num_sequences) return LCPP_OK;
+    if (!channels || (!num_sequences && !rows)) return LCPP_OK;
+    if (!num_sequences) init = grad_last = nullptr, grad_init = nullptr;
     if (!elements_aligned(dtype, gate_in, in, grad_out, grad_gate, grad_in) ||
         !elements_aligned(LCPP_F32, saved, offsets, init, grad_last, grad_init))
         return LCPP_ERR_INVALID_ARG;
