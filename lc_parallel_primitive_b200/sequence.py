@@ -280,6 +280,8 @@ class DeviceBeamSearch(_Recorded):
         pz, sz, rows, vocab = _matrix(d_logits, "d_logits")
         if rows != batches * beams:
             raise ValueError("d_logits must have a row for each score")
+        if not -0x80000000 <= eos_token <= 0x7fffffff:  # the entry's is 32 bits wide
+            raise ValueError("eos_token must be a token (or negative: there is none)")
         pi, po = _dense(d_scores, shape, _F32, "d_scores"), _dense(d_scores_out, shape, _F32, "d_scores_out")
         pt, pp = _dense(d_tokens_out, shape, _I32, "d_tokens_out"), _dense(d_parents_out, shape, _I32, "d_parents_out")
         pf, pfo = _dense(d_finished, shape, _U8, "d_finished"), _dense(d_finished_out, shape, _U8, "d_finished_out")

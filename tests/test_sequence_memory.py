@@ -328,3 +328,17 @@ def test_reorder_to_interleaved_layers(cuda, layer, row):
     Stream() << c.commit()
     torch.cuda.synchronize()
     assert torch.equal(out, x.flip(1))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("eos", [1 << 32, (1 << 32) + 2, 1 << 31, -(1 << 40)])
+def test_select_refuses_an_end_token_that_is_none(cuda, eos):
+    # not the token that its lowest 32 bits are
+    import torch
+    from lc_parallel_primitive_b200 import CommandList, DeviceBeamSearch, temp_buffer
+
+    z, s = torch.zeros((4, 10), device="cuda"), torch.zeros((1, 4), device="cuda")
+    i, m, c = torch.zeros((1, 4), dtype=torch.int32, device="cuda"), DeviceBeamSearch(), CommandList()
+    with pytest.raises(ValueError, match="eos_token"):
+        m.Select(c, temp_buffer(m.GetTempStorageBytes(1, 4, 10)), z, s, None, s.clone(), i, i.clone(), None, eos_token=eos)
+    assert len(c) == 0
