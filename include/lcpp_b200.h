@@ -312,7 +312,8 @@ lcpp_status lcpp_beam_select(int dtype, const void* logits, uint64_t logits_stri
                              uint64_t vocab, int32_t eos_token, void* temp, size_t temp_bytes, void* stream);
 /* States follow their beams: out[l][i] = in[l][parents[i]] for rows of row_bytes bytes, with layer and row strides
  * in bytes; a negative parent: zeros; a parent >= rows_in: zeros, and LCPP_ERR_INVALID_ARG in the device error
- * word.  in and out must not overlap, nor two rows of out; layers may be interleaved. */
+ * word.  out must not overlap in or parents, nor its rows one another; layers may be
+ * interleaved. */
 lcpp_status lcpp_beam_reorder(const void* in, uint64_t in_layer_bytes, uint64_t in_row_bytes, void* out,
                               uint64_t out_layer_bytes, uint64_t out_row_bytes, const int32_t* parents,
                               uint64_t layers, uint64_t rows_in, uint64_t rows, uint64_t row_bytes, void* stream);

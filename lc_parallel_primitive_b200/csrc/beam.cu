@@ -658,7 +658,7 @@ extern "C" lcpp_status lcpp_beam_reorder(const void* in, uint64_t in_layer_bytes
         apart = Region(in, l * (in_layer_bytes / r) + rows_in, r, row_bytes)
                     .apart(Region(out, l * (out_layer_bytes / r) + rows, r, row_bytes));
     }
-    if (!apart) return LCPP_ERR_INVALID_ARG;
+    if (!apart || !Region(out, layers, out_layer_bytes, out_block).apart(Region(parents, rows * 4))) return LCPP_ERR_INVALID_ARG;
     cudaStream_t s = (cudaStream_t)stream;
     uint64_t bits = (uint64_t)(uintptr_t)in | (uint64_t)(uintptr_t)out | row_bytes;
     if (layers > 1) bits |= in_layer_bytes | out_layer_bytes;

@@ -342,3 +342,8 @@ def test_select_refuses_an_end_token_that_is_none(cuda, eos):
     with pytest.raises(ValueError, match="eos_token"):
         m.Select(c, temp_buffer(m.GetTempStorageBytes(1, 4, 10)), z, s, None, s.clone(), i, i.clone(), None, eos_token=eos)
     assert len(c) == 0
+
+
+@pytest.mark.parametrize("kw", [dict(parents=place(2)), dict(parents=place(2, 500)), dict(out=place(3, 8))])
+def test_reorder_refuses_outputs_over_parents(kw):
+    assert reorder(**kw) == L.ERR_INVALID_ARG
