@@ -634,7 +634,7 @@ extern "C" lcpp_status lcpp_beam_reorder(const void* in, uint64_t in_layer_bytes
     if (rows > 0x7fffffffull || rows_in > 0x7fffffffull || layers > 0x7fffffffull || row_bytes > (1ull << 40))
         return LCPP_ERR_INVALID_ARG;
     if (!rows || !layers || !row_bytes) return LCPP_OK;
-    if (!in || !out || !parents || rows * layers > 0x7fffffffull) return LCPP_ERR_INVALID_ARG;
+    if ((!in && rows_in) || !out || !parents || rows * layers > 0x7fffffffull) return LCPP_ERR_INVALID_ARG;
     if ((rows_in > 1 && in_row_bytes < row_bytes) || (rows > 1 && out_row_bytes < row_bytes) ||
         (layers > 1 && out_layer_bytes < row_bytes) || !elements_aligned(LCPP_I32, parents))
         return LCPP_ERR_INVALID_ARG;

@@ -347,3 +347,18 @@ def test_select_refuses_an_end_token_that_is_none(cuda, eos):
 @pytest.mark.parametrize("kw", [dict(parents=place(2)), dict(parents=place(2, 500)), dict(out=place(3, 8))])
 def test_reorder_refuses_outputs_over_parents(kw):
     assert reorder(**kw) == L.ERR_INVALID_ARG
+
+
+@pytest.mark.gpu
+def test_reorder_from_no_rows(cuda):
+    # an empty pool has no memory; its negative parents give zeros, as everywhere
+    import torch
+    from lc_parallel_primitive_b200 import CommandList, DeviceBeamSearch, Stream, last_device_error
+
+    out = torch.full((2, 3, 40), 7.0, device="cuda")
+    m, c = DeviceBeamSearch(), CommandList()
+    m.create()
+    m.Reorder(c, torch.empty((2, 0, 40), device="cuda"), out, torch.full((3,), -1, dtype=torch.int32, device="cuda"))
+    Stream() << c.commit()
+    torch.cuda.synchronize()
+    assert (out == 0).all() and last_device_error() == L.OK
