@@ -59,7 +59,7 @@ class DeviceLinearRecurrence : public LuisaModule {
                  BufferView<T> d_out, size_t num_rows, size_t num_channels, Sequences sequences, Gate,
                  BufferView<float> d_init = {}, BufferView<float> d_last = {}, BufferView<uint> d_saved = {}) {
         cmdlist << [=](cudaStream_t s) -> int {
-            if (!fits(d_gate, num_rows, num_channels) || !fits(d_in, num_rows, num_channels) ||
+            if (!whole(sequences) || !fits(d_gate, num_rows, num_channels) || !fits(d_in, num_rows, num_channels) ||
                 !fits(d_out, num_rows, num_channels) || !states(d_init, sequences, num_channels) ||
                 !states(d_last, sequences, num_channels) || !saved(d_saved, num_rows, num_channels))
                 return LCPP_ERR_INVALID_ARG;
@@ -79,7 +79,7 @@ class DeviceLinearRecurrence : public LuisaModule {
                   BufferView<float> d_init = {}, BufferView<float> d_grad_last = {},
                   BufferView<float> d_grad_init = {}) {
         cmdlist << [=](cudaStream_t s) -> int {
-            if (!fits(d_gate, num_rows, num_channels) || !fits(d_in, num_rows, num_channels) ||
+            if (!whole(sequences) || !fits(d_gate, num_rows, num_channels) || !fits(d_in, num_rows, num_channels) ||
                 !fits(d_grad_gate, num_rows, num_channels) || !fits(d_grad_in, num_rows, num_channels) ||
                 (d_grad_out.data() && !fits(d_grad_out, num_rows, num_channels)) ||
                 !states(d_init, sequences, num_channels) || !states(d_grad_last, sequences, num_channels) ||
@@ -116,6 +116,9 @@ class DeviceLinearRecurrence : public LuisaModule {
   private:
     template <typename T>
     static bool fits(BufferView<T> m, size_t rows, size_t channels) { return m.size() >= rows * channels; }
+    static bool whole(const Sequences& sequences) {
+        return !sequences.offsets.data() || sequences.offsets.size() > sequences.count;
+    }
     static bool states(BufferView<float> v, const Sequences& sequences, size_t channels) {
         return !v.data() || v.size() >= sequences.count * channels;
     }
