@@ -1268,7 +1268,7 @@ extern "C" size_t lcpp_linear_recurrence_temp_bytes(uint64_t rows, uint64_t chan
 }
 
 extern "C" size_t lcpp_linear_recurrence_saved_bytes(uint64_t rows, uint64_t channels) {
-    return align_up(ceil_div(rows, 128) * channels * sizeof(float), 256);  // a state per tile, of 128 rows at least
+    return align_up(ceil_div(rows, LR_TILE) * channels * sizeof(float), 256);  // a state per tile
 }
 
 extern "C" lcpp_status lcpp_linear_recurrence_forward(
