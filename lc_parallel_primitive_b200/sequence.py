@@ -71,7 +71,7 @@ def _matrix(t: torch.Tensor, name: str):
             raise ValueError(f"{name}: the batch stride must be the row stride times the length")
     else:
         raise ValueError(f"{name} must have the shape (rows, channels) or (batch, time, channels)")
-    if unit != 1 and channels > 1:
+    if unit != 1 and channels > 1 and rows:
         raise ValueError(f"{name}: the channels of a row must be adjacent")
     if row < channels and rows > 1:
         raise ValueError(f"{name}: rows must not overlap")
@@ -171,7 +171,7 @@ class DeviceLinearRecurrence(_Recorded):
             raise TypeError("d_init must have the element type torch.float32")
         if d_init.shape != (count, channels):
             raise ValueError(f"d_init must have the shape {(count, channels)}, not {tuple(d_init.shape)}")
-        if channels > 1 and d_init.stride(1) != 1:
+        if channels > 1 and count and d_init.stride(1) != 1:
             raise ValueError("d_init: the channels of a state must be adjacent")
         return d_init.data_ptr(), d_init.stride(0)
 

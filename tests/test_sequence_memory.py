@@ -362,3 +362,20 @@ def test_reorder_from_no_rows(cuda):
     Stream() << c.commit()
     torch.cuda.synchronize()
     assert (out == 0).all() and last_device_error() == L.OK
+
+
+@pytest.mark.gpu
+def test_empty_tensors_have_no_strides(cuda):
+    # as they come from numpy, where an empty array's strides say nothing
+    import numpy as np
+    import torch
+    from lc_parallel_primitive_b200 import CommandList, DeviceLinearRecurrence, Stream, temp_buffer
+
+    def empty():
+        return torch.from_numpy(np.empty((0, 8), np.float32)).as_strided((0, 8), (1, 0)).cuda().as_strided((0, 8), (1, 0))
+
+    m, c = DeviceLinearRecurrence(), CommandList()
+    m.create()
+    m.Forward(c, temp_buffer(m.GetTempStorageBytes(0, 8)), empty(), empty(), empty(), 4, d_init=empty())
+    Stream() << c.commit()
+    torch.cuda.synchronize()
