@@ -312,13 +312,15 @@ def test_reorder_refuses_rows_of_layers_over_each_other(kw):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("layer,row", [(64, 192), (64, 200), (320, 64), (96, 224), (160, 64), (192, 128)])
-def test_reorder_to_interleaved_layers(cuda, layer, row):
-    # 3 layers x 4 rows of 32 bytes whose places are apart, though not all one behind the other
+@pytest.mark.parametrize("layers,rows,layer,row", [(3, 4, 64, 192), (3, 4, 64, 200), (3, 4, 320, 64), (2, 2, 96, 224),
+                                                   (3, 4, 160, 64), (2, 4, 192, 128)])
+def test_reorder_to_interleaved_layers(cuda, layers, rows, layer, row):
+    # rows of 32 bytes whose places are apart, though not all one behind the other
     import torch
     from lc_parallel_primitive_b200 import CommandList, DeviceBeamSearch, Stream
 
-    layers, rows = (2, 2) if (layer, row) == (96, 224) else (3, 4)
+    places = sorted(l * layer + i * row for l in range(layers) for i in range(rows))
+    assert all(b - a >= 32 for a, b in zip(places, places[1:]))
     x = torch.randint(0, 255, (layers, rows, 32), device="cuda", dtype=torch.uint8)
     buf = torch.full((2 * layer + 3 * row + 32,), 7, dtype=torch.uint8, device="cuda")
     out = buf.as_strided((layers, rows, 32), (layer, row, 1))
