@@ -26,7 +26,8 @@ constexpr int lcpp_float_dtype_of() {
 template <typename T>
 concept SequenceFloatT = lcpp_float_dtype_of<T>() >= 0;
 
-struct LinearGate { static constexpr int lcpp_gate = LCPP_GATE_LINEAR; };    // h = gate h' + in
+// h = gate h' + in; the product of the gates along up to 128 rows must stay finite
+struct LinearGate { static constexpr int lcpp_gate = LCPP_GATE_LINEAR; };
 struct SigmoidGate { static constexpr int lcpp_gate = LCPP_GATE_SIGMOID; };  // h = a h' + (1 - a) in, a = sigmoid(gate)
 
 // Rows of equal sequences, or CSR row offsets (num_sequences + 1 on the device).

@@ -246,7 +246,10 @@ lcpp_status lcpp_reduce_by_key(int op, int key_dtype, int value_dtype, const voi
  * a model with beams.  dtype: LCPP_F32, LCPP_F16 or LCPP_BF16; states, scores
  * and every sum are float32.  Matrices are row-major with unit element stride
  * and a row stride in elements (>= channels, < 2^31; any value for one row);
- * no alignment beyond the element's own is required.
+ * no alignment beyond the element's own is required, and any other address is
+ * refused.  temp is refused where it is not 16-byte (selection: 8-byte) aligned.
+ * Matrices may be columns of one buffer; two of different strides whose bounds
+ * meet count as overlapping.
  *
  * Gated linear recurrence, per channel (rows = tokens):
  *   LCPP_GATE_LINEAR   h_t = gate_t h_{t-1} + in_t
@@ -257,6 +260,7 @@ lcpp_status lcpp_reduce_by_key(int op, int key_dtype, int value_dtype, const voi
  * offsets[0] or from the last offset on are padding, whose outputs and
  * gradients are 0 whatever they hold.  h before the first row is
  * init[s * init_stride + c] (init_stride 0: one state for all; NULL: zeros).
+ * offsets of no sequence (num_sequences 0) make every row padding.
  * last[s * channels + c] (NULL: not wanted) is h after the last row; an empty
  * sequence passes init on.  saved (NULL: no backward pass follows) receives
  * lcpp_linear_recurrence_saved_bytes() for the backward call.  out may be

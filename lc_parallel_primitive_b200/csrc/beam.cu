@@ -414,7 +414,8 @@ beam_merge_kernel(BeamTemp tmp, const float* scores, const uint8_t* finished, in
 }
 
 // One kernel: a cluster takes a batch entry, a CTA a part of one of its rows; the first CTA joins them from its
-// shared memory.  For few and short rows, where a second launch and the way through L2 are what counts.
+// shared memory.  For short rows, where a second launch and the way through L2 are what counts, and for batches whose
+// CTAs fill the SMs by themselves.
 constexpr int BEAM_CLUSTER = 8;
 
 template <typename T>

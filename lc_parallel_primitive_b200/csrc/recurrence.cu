@@ -190,10 +190,11 @@ __device__ __forceinline__ float4 lr_get(const float4* r) {
 // the result does not depend on how far back the state was found.  Bounded by
 // the spin limit, after which the error word is set.
 // More records a read reach further where many tiles of a column are under way,
-// but take time and registers: 16 instead of LR_FAR (LR_NEAR) spill, and the
-// backward pass over 65536 x 1000 f32 takes 345 us instead of 238, though the
-// forward pass over 65536 x 128 bf16, with 74 tiles under way, 42 instead of 49;
-// 8 everywhere 60 there.
+// but take time and registers: with 16 (8) instead of LR_FAR (LR_NEAR) the
+// backward pass over 65536 x 1000 f32 spills and takes 345 us instead of 238,
+// though the forward pass over 65536 x 128 bf16, with 74 tiles under way, 42
+// instead of 49; 8 everywhere 60 there.  At 12 and 6 the forward kernels of 2-byte
+// elements at odd addresses still spill 156 bytes, four backward ones 4 or 8.
 constexpr int LR_NEAR = 6, LR_FAR = 12;
 
 template <int W>

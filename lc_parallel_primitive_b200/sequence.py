@@ -130,13 +130,13 @@ class _Recorded(_Module):
 class DeviceLinearRecurrence(_Recorded):
     """h_t = a_t h_{t-1} + b_t per channel, along the rows of each sequence.
 
-    mode "linear":  d_gate = a, d_in = b
+    mode "linear":  d_gate = a, d_in = b; the product of the gates along up to 128 rows must stay finite
     mode "sigmoid": a = sigmoid(d_gate), b = (1 - a) d_in
 
     Matrices are (rows, channels) or (batch, time, channels), channels adjacent, any row stride.
     offsets_or_length: the length of every sequence (rows must be a multiple of it), or S + 1 ascending int32 /
     uint32 row offsets on the device (CSR) of S sequences; rows outside them are padding (zeros come out).
-    States are float32 of the shape (S, channels).
+    States are float32 of the shape (S, channels).  temp_storage is contiguous and 16-byte aligned, as temp_buffer's is.
     """
 
     @staticmethod
