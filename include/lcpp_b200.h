@@ -322,6 +322,31 @@ lcpp_status lcpp_beam_reorder(const void* in, uint64_t in_layer_bytes, uint64_t 
                               uint64_t out_layer_bytes, uint64_t out_row_bytes, const int32_t* parents,
                               uint64_t layers, uint64_t rows_in, uint64_t rows, uint64_t row_bytes, void* stream);
 
+/* Softmax cross entropy over a vocabulary from hidden states, without the logits in memory:
+ *   z = hidden weight^T,  logsum[i] = log sum_v exp(z_iv),  loss[i] = logsum[i] - z_i,targets[i]
+ * hidden is [rows][channels], weight [vocab][channels], both of dtype; products are summed in float32 (float32 operands
+ * as three bf16 parts each, products to about 2^-24).  A row with a negative target takes no part: its loss, logsum and
+ * gradient are 0, it adds nothing to the weight's gradient, and its hidden state may hold anything; a target >= vocab
+ * does the same and leaves LCPP_ERR_INVALID_ARG in the device error word.  loss or logsum may be NULL.
+ * rows <= 2^24, vocab <= 2^30.  What is written, temp included, must not overlap anything else.
+ * temp bytes: for the forward call, or (backward != 0) for both; aligned = 0 where a row of weight may start off a
+ * 16-byte boundary (it is copied then, as it is for channels that are no multiple of 8 and for float32). */
+size_t      lcpp_cross_entropy_temp_bytes(int dtype, uint64_t rows, uint64_t channels, uint64_t vocab, int backward,
+                                          int aligned);
+lcpp_status lcpp_cross_entropy_forward(int dtype, const void* hidden, uint64_t hidden_stride, const void* weight,
+                                       uint64_t weight_stride, const int32_t* targets, float* loss, float* logsum,
+                                       uint64_t rows, uint64_t channels, uint64_t vocab, void* temp, size_t temp_bytes,
+                                       void* stream);
+/* Gradients from those of loss (grad_loss[i * grad_loss_stride]; stride 0: one for all rows), given the forward call's
+ * logsum: grad_hidden [rows][channels] and grad_weight [vocab][channels] (NULL: not wanted), both of dtype.  The
+ * logits' gradient is rounded to dtype between the two products (float32: to three bf16 parts). */
+lcpp_status lcpp_cross_entropy_backward(int dtype, const void* hidden, uint64_t hidden_stride, const void* weight,
+                                        uint64_t weight_stride, const int32_t* targets, const float* logsum,
+                                        const float* grad_loss, uint64_t grad_loss_stride, void* grad_hidden,
+                                        uint64_t grad_hidden_stride, void* grad_weight, uint64_t grad_weight_stride,
+                                        uint64_t rows, uint64_t channels, uint64_t vocab, void* temp, size_t temp_bytes,
+                                        void* stream);
+
 /* ---- Multi-GPU (one process per GPU, NCCL) -----------------------------
  * No counterpart in the reference, which is single-GPU and limits item
  * counts to 32 bits (device_radix_sort.h:136, details/scan.h:72).  These

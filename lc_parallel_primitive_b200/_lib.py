@@ -73,6 +73,10 @@ SIGNATURES = {
     "lcpp_beam_select": (_i, [_i, _vp, _u64, _vp, _vp, _vp, _vp, _vp, _vp, _u64, _u32, _u64, C.c_int32, _vp, _sz,
                               _vp]),
     "lcpp_beam_reorder": (_i, [_vp, _u64, _u64, _vp, _u64, _u64, _vp, _u64, _u64, _u64, _u64, _vp]),
+    "lcpp_cross_entropy_temp_bytes": (_sz, [_i, _u64, _u64, _u64, _i, _i]),
+    "lcpp_cross_entropy_forward": (_i, [_i, _vp, _u64, _vp, _u64, _vp, _vp, _vp, _u64, _u64, _u64, _vp, _sz, _vp]),
+    "lcpp_cross_entropy_backward": (_i, [_i, _vp, _u64, _vp, _u64, _vp, _vp, _vp, _u64, _vp, _u64, _vp, _u64, _u64, _u64,
+                                         _u64, _vp, _sz, _vp]),
     "lcpp_mg_unique_id_bytes": (_sz, []),
     "lcpp_mg_get_unique_id": (_i, [_vp]),
     "lcpp_mg_comm_init_rank": (_i, [C.POINTER(_vp), _i, _vp, _i]),

@@ -308,6 +308,85 @@ class DeviceBeamSearch(_Recorded):
                    keep, "DeviceBeamSearch.Reorder")
 
 
+class DeviceCrossEntropy(_Recorded):
+    """Softmax cross entropy over a vocabulary from hidden states, without the logits in memory.
+
+    loss[i] = log sum_v exp(z_iv) - z_i,target(i) with z = d_hidden d_weight^T.  d_hidden: (rows, channels) or
+    (batch, time, channels), any row stride; d_weight: (vocab, channels) of the same type; d_targets: int32, one for
+    each row.  A row with a negative target takes no part: loss, logsum and gradient 0, whatever its hidden state
+    holds.  Sums are float32; float32 operands are multiplied in three bf16 parts.
+    """
+
+    @staticmethod
+    def GetTempStorageBytes(num_rows: int, num_channels: int, vocab: int, dtype=torch.bfloat16, backward: bool = True,
+                            aligned: bool = True) -> int:
+        """For Forward, or for both calls; aligned=False: rows of d_weight may start off a 16-byte boundary."""
+        if dtype not in _FLOATS:
+            raise TypeError(f"unsupported element type {dtype}")
+        return int(L.lib().lcpp_cross_entropy_temp_bytes(_FLOATS[dtype], num_rows, num_channels, vocab, backward, aligned))
+
+    @staticmethod
+    def _operands(d_hidden, d_weight, d_targets):
+        """(hidden pointer, stride, weight pointer, stride, targets pointer, rows, channels, vocab)."""
+        ph, sh, rows, channels = _matrix(d_hidden, "d_hidden")
+        if d_weight.dim() != 2 or d_weight.shape[1] != channels:
+            raise ValueError(f"d_weight must have the shape (vocab, {channels}), not {tuple(d_weight.shape)}")
+        pw, sw, vocab, _ = _matrix(d_weight, "d_weight")
+        if d_targets.dtype != torch.int32:
+            raise TypeError("d_targets must have the element type torch.int32")
+        if d_targets.numel() != rows or not d_targets.is_contiguous():
+            raise ValueError("d_targets must be contiguous, one for each row of d_hidden")
+        return ph, sh, pw, sw, d_targets.data_ptr(), rows, channels, vocab
+
+    def Forward(self, cmdlist, temp_storage, d_hidden, d_weight, d_targets, d_loss, d_logsum=None):
+        """d_loss and d_logsum (for Backward): float32, one for each row; either may be None."""
+        dt = _float_dtype(d_hidden, d_weight)
+        temp, temp_bytes = _temp(temp_storage)
+        keep = (d_hidden, d_weight, d_targets, d_loss, d_logsum, temp_storage)
+        _one_device(*keep)
+        ph, sh, pw, sw, pt, rows, channels, vocab = self._operands(d_hidden, d_weight, d_targets)
+        pl, ps = _per_row(d_loss, rows, "d_loss"), _per_row(d_logsum, rows, "d_logsum")
+        self._call(cmdlist, L.lib().lcpp_cross_entropy_forward,
+                   (dt, ph, sh, pw, sw, pt, pl, ps, rows, channels, vocab, temp, temp_bytes),
+                   keep, "DeviceCrossEntropy.Forward")
+
+    def Backward(self, cmdlist, temp_storage, d_hidden, d_weight, d_targets, d_logsum, d_grad_loss, d_grad_hidden,
+                 d_grad_weight):
+        """Gradients of d_hidden and d_weight (None: not wanted) from that of the loss: float32, one for each row, or
+        one expanded over the rows (stride 0); d_logsum is the Forward call's.  Outputs must not overlap anything
+        else."""
+        dt = _float_dtype(d_hidden, d_weight, d_grad_hidden, d_grad_weight)
+        temp, temp_bytes = _temp(temp_storage)
+        keep = (d_hidden, d_weight, d_targets, d_logsum, d_grad_loss, d_grad_hidden, d_grad_weight, temp_storage)
+        _one_device(*keep)
+        ph, sh, pw, sw, pt, rows, channels, vocab = self._operands(d_hidden, d_weight, d_targets)
+        ps = _per_row(d_logsum, rows, "d_logsum")
+        if d_grad_loss.dtype != torch.float32:
+            raise TypeError("d_grad_loss must have the element type torch.float32")
+        if d_grad_loss.numel() != rows:
+            raise ValueError("d_grad_loss must hold one value for each row")
+        one = rows > 0 and all(n == 1 or st == 0 for n, st in zip(d_grad_loss.shape, d_grad_loss.stride()))
+        if not one and not d_grad_loss.is_contiguous():
+            raise ValueError("d_grad_loss must be contiguous or one value expanded")
+        pgh, sgh = _like(d_grad_hidden, d_hidden, rows, channels, "d_grad_hidden")
+        pgw, sgw = _like(d_grad_weight, d_weight, vocab, channels, "d_grad_weight")
+        self._call(cmdlist, L.lib().lcpp_cross_entropy_backward,
+                   (dt, ph, sh, pw, sw, pt, ps, d_grad_loss.data_ptr(), 0 if one else 1, pgh, sgh, pgw, sgw, rows,
+                    channels, vocab, temp, temp_bytes),
+                   keep, "DeviceCrossEntropy.Backward")
+
+
+def _per_row(t, rows, name):
+    """Pointer of a contiguous float32 tensor with one value for each row (None stays None)."""
+    if t is None:
+        return None
+    if t.dtype != torch.float32:
+        raise TypeError(f"{name} must have the element type torch.float32")
+    if t.numel() != rows or not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous, one value for each row")
+    return t.data_ptr()
+
+
 def _layers(t, name):
     """(pointer, layer stride, row stride, layers, rows, row bytes) of states, strides in bytes."""
     shape, stride, e = t.shape, t.stride(), t.element_size()
