@@ -322,6 +322,56 @@ lcpp_status lcpp_beam_reorder(const void* in, uint64_t in_layer_bytes, uint64_t 
                               uint64_t out_layer_bytes, uint64_t out_row_bytes, const int32_t* parents,
                               uint64_t layers, uint64_t rows_in, uint64_t rows, uint64_t row_bytes, void* stream);
 
+/* Gated delta rule: per sequence and head a state S of [value_dim][key_dim] float32, and for each row (token)
+ *   S' = exp(decay_t) S,  u = beta_t (v_t - S' k_t),  S = S' + u k_t^T,  out_t = scale S q_t
+ * q and k are [rows][key_heads][key_dim], v and out [rows][heads][value_dim] of dtype (LCPP_F32, LCPP_F16, LCPP_BF16),
+ * decay (log of the factor, <= 0; -inf: the state starts anew; NULL: 0) and beta [rows][heads] float32, each with a
+ * row stride in elements; head h reads key head h / (heads / key_heads).  key_dim and value_dim <= 128.  Sequences are
+ * as above (length, or offsets); rows outside them give zeros.  init and last are [num_sequences][heads][value_dim]
+ * [key_dim] (init NULL: zeros, last NULL: not wanted; last may be init).  The work goes by chunks of 64 rows, so a value
+ * that is not finite reaches the rows of its sequence up to 63 before it, too, but no other sequence or head. */
+typedef struct {
+    uint64_t rows, num_sequences, length; /* length: of every sequence, where offsets is NULL */
+    const uint32_t* offsets;              /* num_sequences + 1 ascending row offsets */
+    uint32_t heads, key_heads, key_dim, value_dim;
+    float scale;
+} lcpp_delta_shape;
+typedef struct {
+    const void *q, *k, *v;
+    uint64_t q_stride, k_stride, v_stride;
+    const float *decay, *beta;
+    uint64_t decay_stride, beta_stride;
+    const float* init;
+} lcpp_delta_inputs;
+/* Only rows, num_sequences and the heads and dimensions of the shape are looked at.  backward != 0: for both calls;
+ * aligned = 0 where q, k, v or grad_out may have rows that start off a 16-byte boundary. */
+size_t      lcpp_delta_rule_temp_bytes(int dtype, const lcpp_delta_shape* shape, int backward, int aligned);
+size_t      lcpp_delta_rule_saved_bytes(const lcpp_delta_shape* shape);
+/* saved (16-byte aligned; NULL: no backward pass follows) is filled for the backward call.  What is written must not
+ * overlap anything else, but last may be init. */
+lcpp_status lcpp_delta_rule_forward(int dtype, const lcpp_delta_shape* shape, const lcpp_delta_inputs* in, void* out,
+                                    uint64_t out_stride, float* last, void* saved, void* temp, size_t temp_bytes,
+                                    void* stream);
+/* Gradients from those of out (NULL: 0) and last (NULL: 0), given the forward call's inputs and saved: of q, k and v
+ * ([rows][...] of dtype, rows adjacent), of decay and beta ([rows][heads] float32) and of init (NULL: not wanted).
+ * Heads that share a key head add up in grad_q and grad_k.  What is written must not overlap anything else. */
+typedef struct {
+    const void* out;
+    uint64_t out_stride;
+    const float* last;
+    void *q, *k, *v;
+    float *decay, *beta, *init;
+} lcpp_delta_grads;
+lcpp_status lcpp_delta_rule_backward(int dtype, const lcpp_delta_shape* shape, const lcpp_delta_inputs* in,
+                                     const void* saved, const lcpp_delta_grads* grads, void* temp, size_t temp_bytes,
+                                     void* stream);
+/* One token: row i goes on from states_in[parents[i]] (in->init; parents NULL: row i; a negative parent or in->init
+ * NULL: zeros; a parent >= rows_in: zeros, and LCPP_ERR_INVALID_ARG in the device error word) and writes states_out[i]
+ * and out[i].  Of the shape rows, heads, key_heads, key_dim, value_dim and scale are looked at.  states_out may be the
+ * states read when parents is NULL; nothing else that is written may overlap anything. */
+lcpp_status lcpp_delta_rule_step(int dtype, const lcpp_delta_shape* shape, const lcpp_delta_inputs* in, uint64_t rows_in,
+                                 const int32_t* parents, float* states_out, void* out, uint64_t out_stride, void* stream);
+
 /* Softmax cross entropy over a vocabulary from hidden states, without the logits in memory:
  *   z = hidden weight^T,  logsum[i] = log sum_v exp(z_iv),  loss[i] = logsum[i] - z_i,targets[i]
  * hidden is [rows][channels], weight [vocab][channels], both of dtype; products are summed in float32 (float32 operands

@@ -16,4 +16,4 @@ from .primitives import (  # noqa: F401
     synchronize,
     temp_buffer,
 )
-from .sequence import DeviceBeamSearch, DeviceCrossEntropy, DeviceLinearRecurrence  # noqa: F401
+from .sequence import DeviceBeamSearch, DeviceCrossEntropy, DeviceDeltaRule, DeviceLinearRecurrence  # noqa: F401

@@ -34,6 +34,23 @@ ERR_CAPACITY = -7
 
 _vp, _u64, _sz, _i, _u32 = C.c_void_p, C.c_uint64, C.c_size_t, C.c_int, C.c_uint32
 
+
+
+class DeltaShape(C.Structure):
+    _fields_ = [("rows", _u64), ("num_sequences", _u64), ("length", _u64), ("offsets", _vp), ("heads", _u32),
+                ("key_heads", _u32), ("key_dim", _u32), ("value_dim", _u32), ("scale", C.c_float)]
+
+
+class DeltaInputs(C.Structure):
+    _fields_ = [("q", _vp), ("k", _vp), ("v", _vp), ("q_stride", _u64), ("k_stride", _u64), ("v_stride", _u64),
+                ("decay", _vp), ("beta", _vp), ("decay_stride", _u64), ("beta_stride", _u64), ("init", _vp)]
+
+
+class DeltaGrads(C.Structure):
+    _fields_ = [("out", _vp), ("out_stride", _u64), ("last", _vp), ("q", _vp), ("k", _vp), ("v", _vp), ("decay", _vp),
+                ("beta", _vp), ("init", _vp)]
+
+
 # name -> (restype, argtypes); the complete list of symbols of include/lcpp_b200.h
 SIGNATURES = {
     "lcpp_status_string": (C.c_char_p, [_i]),
@@ -73,6 +90,12 @@ SIGNATURES = {
     "lcpp_beam_select": (_i, [_i, _vp, _u64, _vp, _vp, _vp, _vp, _vp, _vp, _u64, _u32, _u64, C.c_int32, _vp, _sz,
                               _vp]),
     "lcpp_beam_reorder": (_i, [_vp, _u64, _u64, _vp, _u64, _u64, _vp, _u64, _u64, _u64, _u64, _vp]),
+    "lcpp_delta_rule_temp_bytes": (_sz, [_i, C.POINTER(DeltaShape), _i, _i]),
+    "lcpp_delta_rule_saved_bytes": (_sz, [C.POINTER(DeltaShape)]),
+    "lcpp_delta_rule_forward": (_i, [_i, C.POINTER(DeltaShape), C.POINTER(DeltaInputs), _vp, _u64, _vp, _vp, _vp, _sz, _vp]),
+    "lcpp_delta_rule_backward": (_i, [_i, C.POINTER(DeltaShape), C.POINTER(DeltaInputs), _vp, C.POINTER(DeltaGrads), _vp,
+                                      _sz, _vp]),
+    "lcpp_delta_rule_step": (_i, [_i, C.POINTER(DeltaShape), C.POINTER(DeltaInputs), _u64, _vp, _vp, _vp, _u64, _vp]),
     "lcpp_cross_entropy_temp_bytes": (_sz, [_i, _u64, _u64, _u64, _i, _i]),
     "lcpp_cross_entropy_forward": (_i, [_i, _vp, _u64, _vp, _u64, _vp, _vp, _vp, _u64, _u64, _u64, _vp, _sz, _vp]),
     "lcpp_cross_entropy_backward": (_i, [_i, _vp, _u64, _vp, _u64, _vp, _vp, _vp, _u64, _vp, _u64, _vp, _u64, _u64, _u64,

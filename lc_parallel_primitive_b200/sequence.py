@@ -254,6 +254,174 @@ def _saved(d_saved, rows, channels):
     return d_saved.data_ptr()
 
 
+class DeviceDeltaRule(_Recorded):
+    """Gated delta rule: per sequence and head a state S (value_dim, key_dim), and for each token
+
+        S' = exp(decay) S,  u = beta (v - S' k),  S = S' + u k^T,  out = scale S q
+
+    d_q, d_k: (rows, key_heads, key_dim) or (batch, time, key_heads, key_dim), d_v and d_out the same with heads and
+    value_dim; heads of a row adjacent, any row stride; head h reads key head h // (heads // key_heads).  d_decay (log
+    of the factor, <= 0; None: 0) and d_beta: float32 (rows, heads), any row stride.  Dimensions up to 128.  scale:
+    None for 1 / sqrt(key_dim).  offsets_or_length as in DeviceLinearRecurrence; states are contiguous float32
+    (sequences, heads, value_dim, key_dim).  temp_storage is contiguous and 16-byte aligned, as temp_buffer's is.
+    Inputs are finite: the work goes by 64 rows, so a NaN reaches up to 63 rows of its sequence and head before it too.
+    """
+
+    @staticmethod
+    def _shape(num_rows, num_sequences, heads, key_heads, key_dim, value_dim, length=0, offsets=None, scale=0.0):
+        return L.DeltaShape(num_rows, num_sequences, length, offsets, heads, key_heads, key_dim, value_dim, scale)
+
+    @staticmethod
+    def GetTempStorageBytes(num_rows: int, num_sequences: int, heads: int, key_heads: int, key_dim: int, value_dim: int,
+                            dtype=torch.bfloat16, backward: bool = True, aligned: bool = True) -> int:
+        """For Forward, or for both calls; aligned=False: rows of d_q, d_k, d_v or d_grad_out may start off a 16-byte
+        boundary."""
+        if dtype not in _FLOATS:
+            raise TypeError(f"unsupported element type {dtype}")
+        shape = DeviceDeltaRule._shape(num_rows, num_sequences, heads, key_heads, key_dim, value_dim)
+        return int(L.lib().lcpp_delta_rule_temp_bytes(_FLOATS[dtype], shape, backward, aligned))
+
+    @staticmethod
+    def GetSavedStateBytes(num_rows: int, num_sequences: int, heads: int, key_heads: int, key_dim: int, value_dim: int) -> int:
+        """Bytes of d_saved, which Forward fills for Backward."""
+        shape = DeviceDeltaRule._shape(num_rows, num_sequences, heads, key_heads, key_dim, value_dim)
+        return int(L.lib().lcpp_delta_rule_saved_bytes(shape))
+
+    @staticmethod
+    def _inputs(d_q, d_k, d_v, d_decay, d_beta):
+        """(inputs without states, rows, heads, key_heads, key_dim, value_dim)."""
+        pq, sq, rows, key_heads, key_dim = _heads(d_q, "d_q")
+        pk, sk, rk, hk, dk = _heads(d_k, "d_k")
+        pv, sv, rv, heads, value_dim = _heads(d_v, "d_v")
+        if (rk, hk, dk) != (rows, key_heads, key_dim):
+            raise ValueError("d_q and d_k must have the same shape")
+        if rv != rows:
+            raise ValueError("d_v must have the rows of d_q")
+        if not key_heads or heads % key_heads:
+            raise ValueError(f"{heads} heads are no whole number for each of {key_heads} key heads")
+        if key_dim > 128 or value_dim > 128 or not key_dim or not value_dim:
+            raise ValueError("key_dim and value_dim must be from 1 to 128")
+        if d_beta.dtype != torch.float32 or (d_decay is not None and d_decay.dtype != torch.float32):
+            raise TypeError("d_decay and d_beta must have the element type torch.float32")
+        pb, sb, rb, hb = _matrix(d_beta, "d_beta")
+        pd, sd, rd, hd = (None, 0, rb, hb) if d_decay is None else _matrix(d_decay, "d_decay")
+        if (rb, hb) != (rows, heads) or (rd, hd) != (rows, heads):
+            raise ValueError(f"d_decay and d_beta must have the shape {(rows, heads)}")
+        return L.DeltaInputs(pq, pk, pv, sq, sk, sv, pd, pb, sd, sb, None), rows, heads, key_heads, key_dim, value_dim
+
+    def _sequences(self, inputs, offsets_or_length, rows, heads, key_heads, key_dim, value_dim, d_init, scale):
+        """(shape, shape of the states)."""
+        count, length, off = DeviceLinearRecurrence._sequences(offsets_or_length, rows)
+        states = (count, heads, value_dim, key_dim)
+        inputs.init = _dense(d_init, states, _F32, "d_init")
+        if scale is None:
+            scale = key_dim ** -0.5
+        return self._shape(rows, count, heads, key_heads, key_dim, value_dim, length, off, scale), states
+
+    def Forward(self, cmdlist, temp_storage, d_q, d_k, d_v, d_decay, d_beta, d_out, offsets_or_length, d_init=None,
+                d_last=None, d_saved=None, scale=None):
+        """d_out, and d_last = the states after each sequence's last row (d_init for an empty sequence).  d_last may be
+        d_init; other overlaps are refused."""
+        dt = _float_dtype(d_q, d_k, d_v, d_out)
+        offsets = offsets_or_length if isinstance(offsets_or_length, torch.Tensor) else None
+        temp, temp_bytes = _temp(temp_storage)
+        keep = (d_q, d_k, d_v, d_decay, d_beta, d_out, d_init, d_last, d_saved, temp_storage, offsets)
+        _one_device(*keep)
+        inputs, *sizes = self._inputs(d_q, d_k, d_v, d_decay, d_beta)
+        shape, states = self._sequences(inputs, offsets_or_length, *sizes, d_init, scale)
+        po, so, *like = _heads(d_out, "d_out")
+        if like != [sizes[0], sizes[1], sizes[4]]:
+            raise ValueError("d_out must have the shape of d_v")
+        pl = _dense(d_last, states, _F32, "d_last")
+        self._call(cmdlist, L.lib().lcpp_delta_rule_forward,
+                   (dt, shape, inputs, po, so, pl, self._saved(d_saved, shape), temp, temp_bytes),
+                   keep, "DeviceDeltaRule.Forward")
+
+    @staticmethod
+    def _saved(d_saved, shape):
+        if d_saved is None:
+            return None
+        if not d_saved.is_contiguous():
+            raise ValueError("d_saved must be contiguous")
+        if _nbytes(d_saved) < L.lib().lcpp_delta_rule_saved_bytes(shape):
+            raise ValueError("d_saved must hold GetSavedStateBytes(...) bytes")
+        return d_saved.data_ptr()
+
+    def Backward(self, cmdlist, temp_storage, d_q, d_k, d_v, d_decay, d_beta, d_saved, d_grad_out, d_grad_q, d_grad_k,
+                 d_grad_v, d_grad_decay, d_grad_beta, offsets_or_length, d_init=None, d_grad_last=None, d_grad_init=None,
+                 scale=None):
+        """Gradients of the inputs from those of d_out (None: zero) and d_last (None: zero); the inputs, d_init, scale
+        and d_saved are the Forward call's.  Gradients are contiguous, of the inputs' shapes and types; d_grad_decay
+        and d_grad_init may be None.  Outputs must not overlap anything else."""
+        if d_saved is None:
+            raise ValueError("d_saved is needed: give it to Forward first")
+        dt = _float_dtype(d_q, d_k, d_v, d_grad_out, d_grad_q, d_grad_k, d_grad_v)
+        offsets = offsets_or_length if isinstance(offsets_or_length, torch.Tensor) else None
+        temp, temp_bytes = _temp(temp_storage)
+        keep = (d_q, d_k, d_v, d_decay, d_beta, d_saved, d_grad_out, d_grad_q, d_grad_k, d_grad_v, d_grad_decay,
+                d_grad_beta, d_init, d_grad_last, d_grad_init, temp_storage, offsets)
+        _one_device(*keep)
+        inputs, *sizes = self._inputs(d_q, d_k, d_v, d_decay, d_beta)
+        shape, states = self._sequences(inputs, offsets_or_length, *sizes, d_init, scale)
+        pgo, sgo = None, 0
+        if d_grad_out is not None:
+            pgo, sgo, *like = _heads(d_grad_out, "d_grad_out")
+            if like != [sizes[0], sizes[1], sizes[4]]:
+                raise ValueError("d_grad_out must have the shape of d_v")
+        own = (d_q.dtype,)
+        grads = L.DeltaGrads(pgo, sgo, _dense(d_grad_last, states, _F32, "d_grad_last"),
+                             _dense(d_grad_q, d_q.shape, own, "d_grad_q"), _dense(d_grad_k, d_k.shape, own, "d_grad_k"),
+                             _dense(d_grad_v, d_v.shape, own, "d_grad_v"),
+                             _dense(d_grad_decay, d_beta.shape, _F32, "d_grad_decay"),
+                             _dense(d_grad_beta, d_beta.shape, _F32, "d_grad_beta"),
+                             _dense(d_grad_init, states, _F32, "d_grad_init"))
+        self._call(cmdlist, L.lib().lcpp_delta_rule_backward,
+                   (dt, shape, inputs, self._saved(d_saved, shape), grads, temp, temp_bytes),
+                   keep, "DeviceDeltaRule.Backward")
+
+    def Step(self, cmdlist, d_q, d_k, d_v, d_decay, d_beta, d_states_in, d_states_out, d_out, d_parents=None, scale=None):
+        """One token for each row: row i goes on from d_states_in[d_parents[i]] (without d_parents row i; a negative
+        parent, or d_states_in None, from zeros) to d_states_out[i] (rows, heads, value_dim, key_dim).  d_states_out may
+        be d_states_in when there are no parents; other overlaps are refused."""
+        dt = _float_dtype(d_q, d_k, d_v, d_out)
+        keep = (d_q, d_k, d_v, d_decay, d_beta, d_states_in, d_states_out, d_out, d_parents)
+        _one_device(*keep)
+        inputs, rows, heads, key_heads, key_dim, value_dim = self._inputs(d_q, d_k, d_v, d_decay, d_beta)
+        rows_in = 0 if d_states_in is None else d_states_in.shape[0]
+        inputs.init = _dense(d_states_in, (rows_in, heads, value_dim, key_dim), _F32, "d_states_in")
+        pn = _dense(d_states_out, (rows, heads, value_dim, key_dim), _F32, "d_states_out")
+        pp = _dense(d_parents, (rows,), _I32, "d_parents")
+        po, so, *like = _heads(d_out, "d_out")
+        if like != [rows, heads, value_dim]:
+            raise ValueError("d_out must have the shape of d_v")
+        shape = self._shape(rows, 0, heads, key_heads, key_dim, value_dim, scale=key_dim ** -0.5 if scale is None else scale)
+        self._call(cmdlist, L.lib().lcpp_delta_rule_step, (dt, shape, inputs, rows_in, pp, pn, po, so), keep,
+                   "DeviceDeltaRule.Step")
+
+
+def _heads(t, name):
+    """(pointer, row stride, rows, heads, dim) of a (rows, heads, dim) or (batch, time, heads, dim) tensor whose rows are
+    one stride apart and whose heads are adjacent."""
+    shape, stride = t.shape, t.stride()
+    if len(shape) == 4:
+        batch, time, heads, dim = shape
+        rows, row = batch * time, stride[1]
+        if time == 1:
+            row = stride[0]
+        elif batch > 1 and rows and stride[0] != time * row:
+            raise ValueError(f"{name}: the batch stride must be the row stride times the length")
+    elif len(shape) == 3:
+        rows, heads, dim = shape
+        row = stride[0]
+    else:
+        raise ValueError(f"{name} must have the shape (rows, heads, dim) or (batch, time, heads, dim)")
+    if rows and ((dim > 1 and stride[-1] != 1) or (heads > 1 and stride[-2] != dim)):
+        raise ValueError(f"{name}: the heads of a row must be adjacent")
+    if row < heads * dim and rows > 1:
+        raise ValueError(f"{name}: rows must not overlap")
+    return t.data_ptr(), row, rows, heads, dim
+
+
 class DeviceBeamSearch(_Recorded):
     """Selection of the best continuations of every batch entry's beams, and states that follow them."""
 
