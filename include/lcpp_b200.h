@@ -343,9 +343,8 @@ typedef struct {
     uint64_t decay_stride, beta_stride;
     const float* init;
 } lcpp_delta_inputs;
-/* Only rows, num_sequences and the heads and dimensions of the shape are looked at.  backward != 0: for both calls;
- * aligned = 0 where q, k, v or grad_out may have rows that start off a 16-byte boundary. */
-size_t      lcpp_delta_rule_temp_bytes(int dtype, const lcpp_delta_shape* shape, int backward, int aligned);
+/* Only rows, num_sequences and the heads and dimensions of the shape are looked at.  backward != 0: for both calls. */
+size_t      lcpp_delta_rule_temp_bytes(int dtype, const lcpp_delta_shape* shape, int backward);
 size_t      lcpp_delta_rule_saved_bytes(const lcpp_delta_shape* shape);
 /* saved (16-byte aligned; NULL: no backward pass follows) is filled for the backward call.  What is written must not
  * overlap anything else, but last may be init. */

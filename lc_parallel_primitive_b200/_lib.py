@@ -90,7 +90,7 @@ SIGNATURES = {
     "lcpp_beam_select": (_i, [_i, _vp, _u64, _vp, _vp, _vp, _vp, _vp, _vp, _u64, _u32, _u64, C.c_int32, _vp, _sz,
                               _vp]),
     "lcpp_beam_reorder": (_i, [_vp, _u64, _u64, _vp, _u64, _u64, _vp, _u64, _u64, _u64, _u64, _vp]),
-    "lcpp_delta_rule_temp_bytes": (_sz, [_i, C.POINTER(DeltaShape), _i, _i]),
+    "lcpp_delta_rule_temp_bytes": (_sz, [_i, C.POINTER(DeltaShape), _i]),
     "lcpp_delta_rule_saved_bytes": (_sz, [C.POINTER(DeltaShape)]),
     "lcpp_delta_rule_forward": (_i, [_i, C.POINTER(DeltaShape), C.POINTER(DeltaInputs), _vp, _u64, _vp, _vp, _vp, _sz, _vp]),
     "lcpp_delta_rule_backward": (_i, [_i, C.POINTER(DeltaShape), C.POINTER(DeltaInputs), _vp, C.POINTER(DeltaGrads), _vp,

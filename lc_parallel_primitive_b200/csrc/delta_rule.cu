@@ -20,9 +20,9 @@
 // registers: a warp owns 16 of the value dimensions, for which the recurrence needs nothing of any other warp, and the
 // accumulators of one product are the operands of the next.  dr_gradient_kernel is parallel over chunks again.
 //
-// Products are of bf16 with float32 sums.  A float32 value enters as the sum of two bf16 (16 bits, 2^-18) in as many
-// products as that takes, so that states, which live for a whole sequence, keep float32's order of error; bf16 inputs
-// are exact as they are, float16 and float32 ones are split the same way (dr_pack_kernel).
+// Products are of float16 with float32 sums, and a float32 value enters as two float16 with a power of two taken out
+// (warp_mma.cuh), so that states, which live for a whole sequence, and gradients keep float32's order of error.  q and k
+// of 16 bits are exact in one float16 but for the scale of their tile; float32 ones are split too (PLANES 2).
 #include "float_types.cuh"
 #include "warp_mma.cuh"
 
@@ -30,8 +30,8 @@ namespace lcpp {
 
 constexpr int DR_CHUNK = 64;
 constexpr int DR_MAX_DIM = 128;
-constexpr int DR_TILE = DR_CHUNK * DR_CHUNK;  // elements of a chunk's square matrices
-constexpr float DR_LEAST_DECAY = -150.0f;     // exp of less is 0 in float32 anyway, and -inf has no differences
+constexpr int DR_BLOCK = DR_CHUNK * BLOCK_ROW;  // bytes of a 64 x 64 block
+constexpr float DR_LEAST_DECAY = -150.0f;       // exp of less is 0 in float32 anyway, and -inf has no differences
 
 struct DrShape {
     uint64_t rows, length;
@@ -46,15 +46,14 @@ struct DrShape {
 // The chunk in a slot: its first row and how many of its rows exist (0: none).
 struct DrChunk {
     uint64_t row;
-    uint32_t rows, sequence;
-    __device__ __forceinline__ DrChunk(const DrShape& sh, uint64_t slot) : row(0), rows(0), sequence(0) {
+    uint32_t rows;
+    __device__ __forceinline__ DrChunk(const DrShape& sh, uint64_t slot) : row(0), rows(0) {
         uint32_t lo = 0, hi = sh.sequences;  // the last sequence whose base is not past the slot
         while (hi - lo > 1) {
             const uint32_t mid = lo + (hi - lo) / 2;
             if (sh.base(mid) <= slot) lo = mid;
             else hi = mid;
         }
-        sequence = lo;
         const uint64_t from = sh.start(lo), to = min(sh.start(lo + 1), sh.rows), base = sh.base(lo);
         if (slot < base) return;
         row = from + (slot - base) * DR_CHUNK;
@@ -62,75 +61,62 @@ struct DrChunk {
     }
 };
 
-// A matrix [rows][heads][dim] as bf16: the caller's own, or two planes by slot (64 rows each, zeros where there are none).
-struct DrOperand {
-    const __nv_bfloat16* at;
-    uint64_t row;    // elements from a row to the next
-    uint64_t plane;
-    uint32_t head;   // and from a head to the next
-    uint32_t dim;    // columns to read, a multiple of 8
-    bool packed;
-    __device__ __forceinline__ const __nv_bfloat16* rows(uint64_t slot, const DrChunk& c, uint32_t h) const {
-        return at + (packed ? slot * DR_CHUNK : c.row) * row + (uint64_t)h * head;
-    }
-    __device__ __forceinline__ int have(const DrChunk& c) const { return packed ? DR_CHUNK : (int)c.rows; }
+// ---- images --------------------------------------------------------------------------------------
+// What the kernels leave for one another lies in blocks as shared memory holds them (warp_mma.cuh).
+// Of a slot and key head: K, then Q, each PLANES x (key columns / 64) blocks of 64 rows.
+template <int DK, int PLANES>
+constexpr int DR_KEYS = PLANES * (DK / 64) * DR_BLOCK;  // bytes of K, and of Q
+// Of a slot and head: the inverse, then A (two planes each), then the gates.
+struct DrGates {
+    float g[64], e[64], beta[64];
+    float back_k, back_q, back_inverse, back_read;  // inverses of the scales
+    float pad[60];
+    float total[64], rest[64];  // running sums of the decays, in two parts
+};
+constexpr int DR_UNIT = 4 * DR_BLOCK + (int)sizeof(DrGates);
+static_assert(DR_UNIT % 16 == 0, "a bulk copy");
+// Matrices of a slot and head with a row per value dimension, by 32 rows: two planes of blocks of 32 rows.  Every 16
+// rows have a scale of their own, since one warp writes them; its inverse is kept beside.
+constexpr int DR_PIECE = 32 * BLOCK_ROW;  // bytes of a block
+struct DrImage {
+    uint8_t* at;
+    float* back;        // 8 for each slot and head
+    uint32_t blocks;    // of 64 columns: 1 (tokens), or the key columns'
+    uint32_t rows;      // a multiple of 32
+    __host__ __device__ uint64_t bytes() const { return (uint64_t)rows / 32 * 2 * blocks * DR_PIECE; }
+    __device__ __forceinline__ uint8_t* of(uint64_t unit) const { return at + unit * bytes(); }
 };
 
-// What dr_prepare_kernel writes by slot and head.
-struct DrPrepared {
-    __nv_bfloat16 *inverse, *read;  // two planes of 64 x 64: (I + N B)^-1 or (I + B N)^-1, and A
-    float* gates;                   // g, e, beta (64 each)
-    __device__ __forceinline__ uint64_t at(const DrShape& sh, uint64_t slot, uint32_t h) const { return slot * sh.heads + h; }
-};
-// Matrices of two planes by slot and head: states [value_dim][key columns], values [value_dim][64].
-struct DrPlanes {
-    __nv_bfloat16* at;
-    uint64_t size;  // elements of one plane
-    __device__ __forceinline__ __nv_bfloat16* of(const DrShape& sh, uint64_t slot, uint32_t h) const {
-        return at + (slot * sh.heads + h) * 2 * size;
-    }
-};
-
-// ---- operands in two planes ---------------------------------------------------------------------
-template <typename T>
-__global__ void __launch_bounds__(256)
-dr_pack_kernel(DrShape sh, const T* from, uint64_t from_stride, uint32_t heads, uint32_t dim, __nv_bfloat16* to, uint64_t plane,
-               uint32_t pitch) {
-    const uint64_t slot = blockIdx.x;
-    const DrChunk c(sh, slot);
-    const uint32_t words = heads * pitch / 2;
-    for (uint32_t i = threadIdx.x; i < DR_CHUNK * words; i += blockDim.x) {
-        const uint32_t r = i / words, w = i % words, h = w * 2 / pitch, d = w * 2 % pitch;
-        float x = 0.0f, y = 0.0f;
-        if (r < c.rows) {
-            const T* const p = from + (c.row + r) * from_stride + (uint64_t)h * dim + d;
-            if (d < dim) x = widen(p[0]);
-            if (d + 1 < dim) y = widen(p[1]);
-        }
-        uint32_t hi, lo;
-        split_bf16(x, y, hi, lo);
-        uint32_t* const at = (uint32_t*)(to + (slot * DR_CHUNK + r) * (uint64_t)heads * pitch) + w;
-        at[0] = hi;
-        *(uint32_t*)((__nv_bfloat16*)at + plane) = lo;
-    }
+// Stores elements (row, col), (row, col + 1), col even, of a matrix with `blocks` blocks in its rows.
+__device__ __forceinline__ void dr_store(uint8_t* image, uint32_t blocks, uint32_t row, uint32_t col, uint32_t hi, uint32_t lo) {
+    uint8_t* const at = image + ((row >> 5) * 2 * blocks + (col >> 6)) * DR_PIECE + block_at(row & 31, col & 63);
+    *(uint32_t*)at = hi;
+    *(uint32_t*)(at + blocks * DR_PIECE) = lo;
 }
 
 // ---- what does not depend on the state ------------------------------------------------------------
 constexpr int DR_PREPARE_THREADS = 128;
-constexpr int DR_PITCH = DR_CHUNK + 1;
+constexpr int DR_PITCH = 68;
+struct DrInvert {
+    float m[64 * DR_PITCH], inv[64 * DR_PITCH], tmp[32 * 36];
+};
 template <int DK, int PLANES>
 struct DrPrepareSmem {
-    __nv_bfloat16 k[PLANES][DR_CHUNK * DK], q[PLANES][DR_CHUNK * DK];
-    float near[DR_CHUNK * DR_PITCH], read[DR_CHUNK * DR_PITCH];  // k_i.k_j and q_i.k_j
-    float m[DR_CHUNK * DR_PITCH], inv[DR_CHUNK * DR_PITCH], tmp[32 * 33];
-    double total[DR_CHUNK];
-    float beta[DR_CHUNK];
+    union alignas(128) {
+        uint8_t keys[2 * DR_KEYS<DK, PLANES>];
+        DrInvert invert;
+    };
+    alignas(128) uint8_t unit[DR_UNIT];
+    float most[2][4];
 };
 
+__device__ __forceinline__ void dr_fma4(float (&v)[4], float a, const float* b) {
+    const float4 x = *(const float4*)b;
+    v[0] = fmaf(a, x.x, v[0]), v[1] = fmaf(a, x.y, v[1]), v[2] = fmaf(a, x.z, v[2]), v[3] = fmaf(a, x.w, v[3]);
+}
 // inv = (I + m)^-1 of a strictly lower triangular m: the 16 x 16 blocks of the diagonal by substitution, a column a
 // lane, then blocks below from ones above: [X 0; -Y m21 X, Y].
-template <typename S>
-__device__ __forceinline__ void dr_invert(S& s) {
+__device__ __forceinline__ void dr_invert(DrInvert& s) {
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
     if (lane < 16) {
         const int b = warp * 16;
@@ -139,238 +125,326 @@ __device__ __forceinline__ void dr_invert(S& s) {
         for (int i = 0; i < 16; ++i) {
             float v = i == lane ? 1.0f : 0.0f;
 #pragma unroll
-            for (int k = 0; k < i; ++k) v = fmaf(-s.m[(b + i) * DR_PITCH + b + k], x[k], v);
+            for (int k = 0; k < i; k += 4) {
+                const float4 m = *(const float4*)&s.m[(b + i) * DR_PITCH + b + k];
+                v = fmaf(-m.x, x[k], v);
+                if (k + 1 < i) v = fmaf(-m.y, x[k + 1], v);
+                if (k + 2 < i) v = fmaf(-m.z, x[k + 2], v);
+                if (k + 3 < i) v = fmaf(-m.w, x[k + 3], v);
+            }
             x[i] = v;
         }
 #pragma unroll
         for (int i = 0; i < 16; ++i) s.inv[(b + i) * DR_PITCH + b + lane] = x[i];
     }
-    for (int i = t; i < DR_CHUNK * DR_CHUNK; i += DR_PREPARE_THREADS) {  // above the diagonal blocks
-        const int r = i >> 6, c = i & 63;
-        if ((c >> 4) > (r >> 4)) s.inv[r * DR_PITCH + c] = 0.0f;
+    for (int i = t; i < 64 * 16; i += DR_PREPARE_THREADS) {  // above the diagonal blocks
+        const int r = i >> 4, c = (i & 15) * 4;
+        if ((c >> 4) > (r >> 4)) *(float4*)&s.inv[r * DR_PITCH + c] = make_float4(0, 0, 0, 0);
     }
     __syncthreads();
     {
-        const int b = (t >> 6) * 32, r = (t & 63) >> 2, c = (t & 3) * 4;  // blocks (16, 0) and (48, 32)
+        const int half = t >> 6, b = half * 32, r = (t & 63) >> 2, c = (t & 3) * 4;  // blocks (16, 0) and (48, 32)
         float v[4] = {0, 0, 0, 0};
 #pragma unroll
-        for (int k = 0; k < 16; ++k) {
-            const float a = s.m[(b + 16 + r) * DR_PITCH + b + k];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) v[j] = fmaf(a, s.inv[(b + k) * DR_PITCH + b + c + j], v[j]);
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) s.tmp[((t >> 6) * 16 + r) * 33 + c + j] = v[j];
+        for (int k = 0; k < 16; ++k) dr_fma4(v, s.m[(b + 16 + r) * DR_PITCH + b + k], &s.inv[(b + k) * DR_PITCH + b + c]);
+        *(float4*)&s.tmp[(half * 16 + r) * 36 + c] = make_float4(v[0], v[1], v[2], v[3]);
         __syncthreads();
+        v[0] = v[1] = v[2] = v[3] = 0.0f;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = 0.0f;
-#pragma unroll
-        for (int k = 0; k < 16; ++k) {
-            const float a = s.inv[(b + 16 + r) * DR_PITCH + b + 16 + k];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) v[j] = fmaf(a, s.tmp[((t >> 6) * 16 + k) * 33 + c + j], v[j]);
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) s.inv[(b + 16 + r) * DR_PITCH + b + c + j] = -v[j];
+        for (int k = 0; k < 16; ++k) dr_fma4(v, s.inv[(b + 16 + r) * DR_PITCH + b + 16 + k], &s.tmp[(half * 16 + k) * 36 + c]);
+        *(float4*)&s.inv[(b + 16 + r) * DR_PITCH + b + c] = make_float4(-v[0], -v[1], -v[2], -v[3]);
     }
     __syncthreads();
     {
-        const int r = t >> 2, c = (t & 3) * 8;  // block (32, 0)
-        float v[8] = {};
+        const int r = t >> 2, c = (t & 3) * 4;  // block (32, 0), columns c .. and 16 + c ..
+        float v[4] = {0, 0, 0, 0}, u[4] = {0, 0, 0, 0};
 #pragma unroll 8
         for (int k = 0; k < 32; ++k) {
             const float a = s.m[(32 + r) * DR_PITCH + k];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = fmaf(a, s.inv[k * DR_PITCH + c + j], v[j]);
+            dr_fma4(v, a, &s.inv[k * DR_PITCH + c]), dr_fma4(u, a, &s.inv[k * DR_PITCH + 16 + c]);
         }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) s.tmp[r * 33 + c + j] = v[j];
+        *(float4*)&s.tmp[r * 36 + c] = make_float4(v[0], v[1], v[2], v[3]);
+        *(float4*)&s.tmp[r * 36 + 16 + c] = make_float4(u[0], u[1], u[2], u[3]);
         __syncthreads();
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = 0.0f;
+        v[0] = v[1] = v[2] = v[3] = u[0] = u[1] = u[2] = u[3] = 0.0f;
 #pragma unroll 8
         for (int k = 0; k < 32; ++k) {
             const float a = s.inv[(32 + r) * DR_PITCH + 32 + k];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = fmaf(a, s.tmp[k * 33 + c + j], v[j]);
+            dr_fma4(v, a, &s.tmp[k * 36 + c]), dr_fma4(u, a, &s.tmp[k * 36 + 16 + c]);
         }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) s.inv[(32 + r) * DR_PITCH + c + j] = -v[j];
+        *(float4*)&s.inv[(32 + r) * DR_PITCH + c] = make_float4(-v[0], -v[1], -v[2], -v[3]);
+        *(float4*)&s.inv[(32 + r) * DR_PITCH + 16 + c] = make_float4(-u[0], -u[1], -u[2], -u[3]);
     }
     __syncthreads();
 }
 
-template <int DK, int PLANES, bool BACKWARD>
+// The largest of the CTA's values >= 0; `room` 4 floats, between barriers of the caller.
+__device__ __forceinline__ float dr_max4(const float* room) { return fmaxf(fmaxf(room[0], room[1]), fmaxf(room[2], room[3])); }
+
+struct DrPrepare {
+    DrShape sh;
+    const void *q, *k;
+    uint64_t q_stride, k_stride;
+    const float *decay, *beta;
+    uint64_t decay_stride, beta_stride;
+    bool wide;  // rows of q and k are whole pieces of 8 elements on 16 bytes
+    uint8_t *keys, *units;
+};
+
+template <typename T, int DK, bool BACKWARD>
 __global__ void __launch_bounds__(DR_PREPARE_THREADS)
-dr_prepare_kernel(DrShape sh, DrOperand q, DrOperand k, const float* decay, uint64_t decay_stride, const float* beta,
-                  uint64_t beta_stride, DrPrepared to) {
+dr_prepare_kernel(const __grid_constant__ DrPrepare p) {
+    constexpr int PLANES = sizeof(T) == 4 ? 2 : 1, NB = DK / 64, ITEMS = DR_CHUNK * DK / 8 / DR_PREPARE_THREADS;
     extern __shared__ __align__(128) uint8_t dr_smem[];
-    using Smem = DrPrepareSmem<DK, PLANES>;
-    Smem& s = *(Smem*)dr_smem;
+    auto& s = *(DrPrepareSmem<DK, PLANES>*)dr_smem;
+    const DrShape& sh = p.sh;
     const uint64_t slot = blockIdx.x / sh.key_heads;
     const uint32_t hk = blockIdx.x % sh.key_heads, group = sh.heads / sh.key_heads;
     const DrChunk c(sh, slot);
     if (!c.rows) return;
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
-    uint32_t kt[PLANES], qt[PLANES];
-#pragma unroll
-    for (int p = 0; p < PLANES; ++p) {
-        kt[p] = smem_u32(s.k[p]), qt[p] = smem_u32(s.q[p]);
-        tile_load<DK>(kt[p], k.rows(slot, c, hk) + p * k.plane, k.row, DR_CHUNK, k.have(c), k.dim, t, DR_PREPARE_THREADS);
-        tile_load<DK>(qt[p], q.rows(slot, c, hk) + p * q.plane, q.row, DR_CHUNK, q.have(c), q.dim, t, DR_PREPARE_THREADS);
-    }
-    cp_async_commit();
-    cp_async_wait_all();
-    __syncthreads();
+    const LaneOffsets o(lane);
+    // K and Q into blocks, each with a scale
+    Scale scale[2];
     {
-        float nr[8][4] = {}, rd[8][4] = {};
+        alignas(16) T raw[2][ITEMS][8];
 #pragma unroll
-        for (int kk = 0; kk < DK / 16; ++kk) {
-            uint32_t ak[PLANES][4], aq[PLANES][4];
+        for (int x = 0; x < 2; ++x)
 #pragma unroll
-            for (int p = 0; p < PLANES; ++p) load_a<DK>(ak[p], kt[p], warp * 16, kk * 2, lane), load_a<DK>(aq[p], qt[p], warp * 16, kk * 2, lane);
+            for (int i = 0; i < ITEMS; ++i) {
+                const uint32_t item = i * DR_PREPARE_THREADS + t, r = item / (DK / 8), d = item % (DK / 8) * 8;
+                const T* const from = (const T*)(x ? p.q : p.k) + (c.row + r) * (x ? p.q_stride : p.k_stride) + (uint64_t)hk * sh.key_dim + d;
+                if (p.wide && r < c.rows && d < sh.key_dim) {
 #pragma unroll
-            for (int n = 0; n < 4; ++n) {
-                if (n > warp) break;  // columns past the warp's rows are masked
-                uint32_t b[4];
-                load_b<DK>(b, kt[0], n * 16, kk * 2, lane);
+                    for (int j = 0; j < (int)sizeof(T) / 2; ++j) ((uint4*)raw[x][i])[j] = ((const uint4*)from)[j];
+                } else {
 #pragma unroll
-                for (int p = 0; p < PLANES; ++p) {
-                    mma_bf16(nr[2 * n], ak[p], b[0], b[1]), mma_bf16(nr[2 * n + 1], ak[p], b[2], b[3]);
-                    mma_bf16(rd[2 * n], aq[p], b[0], b[1]), mma_bf16(rd[2 * n + 1], aq[p], b[2], b[3]);
-                }
-                if constexpr (PLANES == 2) {
-                    load_b<DK>(b, kt[1], n * 16, kk * 2, lane);
-                    mma_bf16(nr[2 * n], ak[0], b[0], b[1]), mma_bf16(nr[2 * n + 1], ak[0], b[2], b[3]);
-                    mma_bf16(rd[2 * n], aq[0], b[0], b[1]), mma_bf16(rd[2 * n + 1], aq[0], b[2], b[3]);
+                    for (int j = 0; j < 8; ++j) raw[x][i][j] = r < c.rows && d + j < sh.key_dim ? from[j] : narrow<T>(0.0f);
                 }
             }
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            float most = 0.0f;
+#pragma unroll
+            for (int i = 0; i < ITEMS; ++i)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) most = fmaxf(most, fabsf(widen(raw[x][i][j])));
+            most = warp_max(most);
+            if (lane == 0) s.most[x][warp] = most;
         }
-        const int r = warp * 16 + (lane >> 2), col = (lane & 3) * 2;
+        __syncthreads();
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            scale[x] = scale_for(dr_max4(s.most[x]));
+#pragma unroll
+            for (int i = 0; i < ITEMS; ++i) {
+                const uint32_t item = i * DR_PREPARE_THREADS + t, r = item / (DK / 8), d = item % (DK / 8) * 8;
+                uint32_t hi[4], lo[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) split_f16(widen(raw[x][i][2 * j]), widen(raw[x][i][2 * j + 1]), scale[x].by, hi[j], lo[j]);
+                uint8_t* const at = s.keys + x * DR_KEYS<DK, PLANES> + (d >> 6) * DR_BLOCK + block_at(r, d & 63);
+                *(uint4*)at = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                if constexpr (PLANES == 2) *(uint4*)(at + NB * DR_BLOCK) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+            }
+        }
+        fence_proxy_async_smem();
+        __syncthreads();
+    }
+    if (t == 0) {
+        bulk_store(p.keys + (slot * sh.key_heads + hk) * (2 * DR_KEYS<DK, PLANES>), s.keys, 2 * DR_KEYS<DK, PLANES>);
+        bulk_commit();
+    }
+    float nr[8][4] = {}, rd[8][4] = {};  // k_i.k_j and q_i.k_j: 16 rows a warp
+    const uint32_t kt = smem_u32(s.keys), qt = kt + DR_KEYS<DK, PLANES>;
+#pragma unroll
+    for (int kk = 0; kk < DK / 16; ++kk) {
+        const uint32_t block = (kk >> 2) * DR_BLOCK;
+        uint32_t ak[PLANES][4], aq[PLANES][4];
+#pragma unroll
+        for (int i = 0; i < PLANES; ++i) {
+            load_a(ak[i], kt + i * NB * DR_BLOCK + block, warp * 16, kk & 3, o);
+            load_a(aq[i], qt + i * NB * DR_BLOCK + block, warp * 16, kk & 3, o);
+        }
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+            if (n > warp) break;  // columns past the warp's rows are masked
+#pragma unroll
+            for (int i = 0; i < PLANES; ++i) {
+                uint32_t b[4];
+                load_b(b, kt + i * NB * DR_BLOCK + block, n * 16, kk & 3, o);
+#pragma unroll
+                for (int l = 0; l < PLANES - i; ++l) mma_f16_2(nr[2 * n], nr[2 * n + 1], ak[l], b), mma_f16_2(rd[2 * n], rd[2 * n + 1], aq[l], b);
+            }
+        }
+    }
+    const int r0 = warp * 16 + (lane >> 2), col = (lane & 3) * 2;
+    const float back_near = scale[0].back * scale[0].back, back_read = scale[0].back * scale[1].back * sh.scale;
+#pragma unroll
+    for (int n = 0; n < 8; ++n)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) nr[n][j] *= back_near, rd[n][j] *= back_read;
+    DrGates& gates = *(DrGates*)(s.unit + 4 * DR_BLOCK);
+    for (uint32_t h = hk * group; h < (hk + 1) * group; ++h) {
+        if (t == 0) bulk_wait_read_all();  // the keys, the head before's unit
+        __syncthreads();
+        if (warp == 0) {  // running sums of the decays, in 64 bits: differences of long sums matter
+            double v[2];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const uint32_t r = lane * 2 + j;
+                float d = r < c.rows && p.decay ? p.decay[(c.row + r) * p.decay_stride + h] : 0.0f;
+                d = d < DR_LEAST_DECAY ? DR_LEAST_DECAY : d;
+                v[j] = d;
+                gates.beta[r] = r < c.rows ? p.beta[(c.row + r) * p.beta_stride + h] : 0.0f;
+            }
+            double sum = v[0] + v[1];
+#pragma unroll
+            for (int i = 1; i < 32; i <<= 1) {
+                const double up = __shfl_up_sync(0xffffffffu, sum, i);
+                if (lane >= i) sum += up;
+            }
+            const double last = __shfl_sync(0xffffffffu, sum, 31), total[2] = {sum - v[1], sum};
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const int r = lane * 2 + j;
+                gates.total[r] = (float)total[j], gates.rest[r] = (float)(total[j] - (float)total[j]);
+                gates.g[r] = expf((float)total[j]), gates.e[r] = expf((float)(last - total[j]));
+            }
+            if (lane == 0) gates.back_k = scale[0].back, gates.back_q = scale[1].back;
+        }
+        __syncthreads();
+        float a[8][4], most = 0.0f;
 #pragma unroll
         for (int n = 0; n < 8; ++n)
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const int at = (r + (j >> 1) * 8) * DR_PITCH + n * 8 + col + (j & 1);
-                s.near[at] = nr[n][j], s.read[at] = rd[n][j];
+                const int r = r0 + (j >> 1) * 8, cc = n * 8 + col + (j & 1);
+                const float d = cc <= r ? expf((gates.total[r] - gates.total[cc]) + (gates.rest[r] - gates.rest[cc])) : 0.0f;
+                a[n][j] = cc <= r ? d * rd[n][j] : 0.0f;
+                most = fmaxf(most, fabsf(a[n][j]));
+                s.invert.m[r * DR_PITCH + cc] = cc < r ? d * nr[n][j] * gates.beta[BACKWARD ? r : cc] : 0.0f;
             }
-    }
-    for (uint32_t h = hk * group; h < (hk + 1) * group; ++h) {
+        most = warp_max(most);
+        if (lane == 0) s.most[0][warp] = most;
         __syncthreads();
-        const uint64_t at = to.at(sh, slot, h);
-        float* const gates = to.gates + at * 3 * DR_CHUNK;
-        if (warp == 0) {  // running sums of the decays, in 64 bits: differences of long sums matter
-            double v[2];
-            float b[2];
+        dr_invert(s.invert);
+        const Scale read = scale_for(dr_max4(s.most[0]));
+        float v[8][4];
+        most = 0.0f;
+#pragma unroll
+        for (int n = 0; n < 8; ++n)
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                const uint32_t r = lane * 2 + j;
-                float d = r < c.rows && decay ? decay[(c.row + r) * decay_stride + h] : 0.0f;
-                d = d < DR_LEAST_DECAY ? DR_LEAST_DECAY : d;
-                v[j] = d;
-                b[j] = r < c.rows ? beta[(c.row + r) * beta_stride + h] : 0.0f;
+                const float2 x = *(const float2*)&s.invert.inv[(r0 + j * 8) * DR_PITCH + n * 8 + col];
+                v[n][2 * j] = x.x, v[n][2 * j + 1] = x.y;
+                most = fmaxf(most, fmaxf(fabsf(x.x), fabsf(x.y)));
             }
-            double sum = v[0] + v[1];
+        most = warp_max(most);
+        if (lane == 0) s.most[1][warp] = most;
+        __syncthreads();
+        const Scale inverse = scale_for(dr_max4(s.most[1]));
+        if (t == 0) gates.back_inverse = inverse.back, gates.back_read = read.back;
 #pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const double up = __shfl_up_sync(0xffffffffu, sum, o);
-                if (lane >= o) sum += up;
-            }
-            const double last = __shfl_sync(0xffffffffu, sum, 31);
-            const double g[2] = {sum - v[1], sum};
+        for (int n = 0; n < 8; ++n)
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                const int r = lane * 2 + j;
-                s.total[r] = g[j], s.beta[r] = b[j];
-                gates[r] = expf((float)g[j]), gates[DR_CHUNK + r] = expf((float)(last - g[j])), gates[2 * DR_CHUNK + r] = b[j];
+                uint32_t hi, lo;
+                uint8_t* const at = s.unit + block_at(r0 + j * 8, n * 8 + col);
+                split_f16(v[n][2 * j], v[n][2 * j + 1], inverse.by, hi, lo);
+                *(uint32_t*)at = hi, *(uint32_t*)(at + DR_BLOCK) = lo;
+                split_f16(a[n][2 * j], a[n][2 * j + 1], read.by, hi, lo);
+                *(uint32_t*)(at + 2 * DR_BLOCK) = hi, *(uint32_t*)(at + 3 * DR_BLOCK) = lo;
             }
-        }
+        fence_proxy_async_smem();
         __syncthreads();
-        __nv_bfloat16* const read = to.read + at * 2 * DR_TILE;
-        for (int i = t; i < DR_TILE / 2; i += DR_PREPARE_THREADS) {
-            const int r = i >> 5, c0 = (i & 31) * 2;
-            float rd[2];
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const int col = c0 + j;
-                const float d = col <= r ? expf((float)(s.total[r] - s.total[col])) : 0.0f;
-                const float n = col < r ? d * s.near[r * DR_PITCH + col] * s.beta[BACKWARD ? r : col] : 0.0f;
-                s.m[r * DR_PITCH + col] = n;
-                rd[j] = col <= r ? sh.scale * d * s.read[r * DR_PITCH + col] : 0.0f;
-            }
-            uint32_t hi, lo;
-            split_bf16(rd[0], rd[1], hi, lo);
-            ((uint32_t*)read)[i] = hi;
-            ((uint32_t*)(read + DR_TILE))[i] = lo;
-        }
-        __syncthreads();
-        dr_invert(s);
-        __nv_bfloat16* const inverse = to.inverse + at * 2 * DR_TILE;
-        for (int i = t; i < DR_TILE / 2; i += DR_PREPARE_THREADS) {
-            const int r = i >> 5, c0 = (i & 31) * 2;
-            uint32_t hi, lo;
-            split_bf16(s.inv[r * DR_PITCH + c0], s.inv[r * DR_PITCH + c0 + 1], hi, lo);
-            ((uint32_t*)inverse)[i] = hi;
-            ((uint32_t*)(inverse + DR_TILE))[i] = lo;
+        if (t == 0) {
+            bulk_store(p.units + (slot * sh.heads + h) * DR_UNIT, s.unit, DR_UNIT);
+            bulk_commit();
         }
     }
+    if (t == 0) bulk_wait_read_all();
 }
 
 // ---- chunk after chunk ----------------------------------------------------------------------------
-// Rows [row, row + 2) x ... of a fragment's element pairs, to a matrix of two planes with `pitch` columns.
-__device__ __forceinline__ void dr_store_planes(__nv_bfloat16* to, uint64_t plane, int pitch, int row, int col, float x, float y) {
-    uint32_t hi, lo;
-    split_bf16(x, y, hi, lo);
-    __nv_bfloat16* const at = to + row * pitch + col;
-    *(uint32_t*)at = hi;
-    *(uint32_t*)(at + plane) = lo;
+// Values as the caller has them ([rows][heads][value_dim]): 64 tokens x 16 of a warp's value dimensions.  2-byte rows of
+// 32 bytes with their two pieces swapped every 4 rows, float32 rows of 80 bytes, against bank conflicts.
+template <typename T>
+constexpr int DR_RAW_ROW = sizeof(T) == 4 ? 80 : 32;
+template <typename T>
+constexpr int DR_RAW = DR_CHUNK * DR_RAW_ROW<T>;
+template <typename T>
+__device__ __forceinline__ uint32_t dr_raw_at(uint32_t tile, int row, int piece) {
+    if constexpr (sizeof(T) == 4) return tile + row * 80 + piece * 16;
+    else return tile + row * 32 + ((piece ^ (row >> 2 & 1)) << 4);
+}
+template <typename T>
+__device__ __forceinline__ void dr_raw_load(uint32_t tile, const T* from, uint64_t stride, int rows, int cols, bool wide, int lane) {
+    constexpr int PIECES = 2 * sizeof(T) / 2, E = 16 / sizeof(T);  // of a row; elements of one
+#pragma unroll
+    for (int i = 0; i < DR_CHUNK * PIECES / 32; ++i) {
+        const int item = i * 32 + lane, r = item / PIECES, c = item % PIECES;
+        const uint32_t at = dr_raw_at<T>(tile, r, c);
+        if (wide) {
+            const bool have = r < rows && c * E < cols;
+            cp_async16_fill(at, have ? from + r * stride + c * E : from, have ? 16 : 0);
+        } else {
+            alignas(16) T v[E];
+#pragma unroll
+            for (int j = 0; j < E; ++j) v[j] = r < rows && c * E + j < cols ? from[r * stride + c * E + j] : narrow<T>(0.0f);
+            const uint4 w = *(const uint4*)v;
+            asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(w.x), "r"(w.y), "r"(w.z), "r"(w.w) : "memory");
+        }
+    }
+}
+// Transposed, tokens [token, token + 16): v[x] are the value dimensions g + 8 (x & 1) and the tokens 8 (x >> 1) + col, + 1.
+template <typename T>
+__device__ __forceinline__ void dr_raw_get(float (&v)[4][2], uint32_t tile, int token, int lane) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+                v[x][j] = __uint_as_float(lds32(tile + (token + (x >> 1) * 8 + (lane & 3) * 2 + j) * 80 + ((lane >> 2) + (x & 1) * 8) * 4));
+    } else {
+        uint32_t r[4];
+        const int row = token + (lane & 7) + (lane >> 4) * 8;
+        ldmatrix4_t(r, dr_raw_at<T>(tile, row, lane >> 3 & 1));
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+            if constexpr (std::is_same_v<T, __half>) {
+                const float2 f = unpack_f16(r[x]);
+                v[x][0] = f.x, v[x][1] = f.y;
+            } else {
+                v[x][0] = __uint_as_float(r[x] << 16), v[x][1] = __uint_as_float(r[x] & 0xffff0000u);
+            }
+        }
+    }
 }
 
-template <int DK, int PLANES, int WARPS>
-struct DrChainStage {
-    __nv_bfloat16 k[PLANES][DR_CHUNK * DK], q[PLANES][DR_CHUNK * DK];
-    __nv_bfloat16 v[PLANES][DR_CHUNK * (WARPS > 4 ? 128 : 64)];  // V forward, dO backward: the CTA's columns
-    __nv_bfloat16 inverse[2][DR_TILE], read[2][DR_TILE];
-    float gates[3][DR_CHUNK];
-};
-template <int DK, int PLANES, int WARPS>
+template <typename T, int DK, int WARPS>
 struct DrChainSmem {
-    DrChainStage<DK, PLANES, WARPS> stage[2];
+    static constexpr int PLANES = sizeof(T) == 4 ? 2 : 1;
+    static constexpr int STAGE = 2 * DR_KEYS<DK, PLANES> + DR_UNIT;
+    // two stages but where they do not fit beside the values
+    static constexpr int STAGES = 2 * (STAGE + WARPS * DR_RAW<T>) + 64 <= 227 * 1024 ? 2 : 1;
+    alignas(128) uint8_t stage[STAGES][STAGE];
+    alignas(16) uint8_t raw[WARPS][2][DR_RAW<T>];
+    uint64_t full[STAGES], empty[STAGES];
 };
 
 struct DrChain {
     DrShape sh;
-    DrOperand q, k, v;  // v: dO in the backward pass
-    DrPrepared prepared;
-    const float* from;  // states before the first chunk (forward), gradients of the last ones (backward)
-    float* to;          // the states after; gradients of the first
-    void* out;          // forward
+    const uint8_t *keys, *units;
+    const void* values;  // V forward, dO backward (null: zeros)
+    uint64_t value_stride;
+    bool wide;           // rows of values are whole 16-byte pieces
+    const float* from;   // states before the first chunk (forward), gradients of the last ones (backward)
+    float* to;           // the states after; gradients of the first
+    void* out;           // forward
     uint64_t out_stride;
-    DrPlanes states, values;  // S0 and w (forward, if saved), X and z (backward)
-    uint32_t key_cols;        // columns of a saved state, key_dim up to a multiple of 16
+    DrImage states, kept;  // S0 and w (forward, if saved), X and z (backward)
+    float* back_values;    // backward: inverse scales of dO
 };
-
-template <int DK, int PLANES, int WARPS>
-__device__ __forceinline__ void dr_load(DrChainStage<DK, PLANES, WARPS>& st, const DrChain& p, const DrChunk& c, uint64_t slot,
-                                        uint32_t h, uint32_t hk, uint32_t v0, int t) {
-    constexpr int THREADS = WARPS * 32, VC = WARPS > 4 ? 128 : 64;
-#pragma unroll
-    for (int i = 0; i < PLANES; ++i) {
-        tile_load<DK>(smem_u32(st.k[i]), p.k.rows(slot, c, hk) + i * p.k.plane, p.k.row, DR_CHUNK, p.k.have(c), p.k.dim, t, THREADS);
-        tile_load<DK>(smem_u32(st.q[i]), p.q.rows(slot, c, hk) + i * p.q.plane, p.q.row, DR_CHUNK, p.q.have(c), p.q.dim, t, THREADS);
-        if (p.v.at)
-            tile_load<VC>(smem_u32(st.v[i]), p.v.rows(slot, c, h) + i * p.v.plane + v0, p.v.row, DR_CHUNK, p.v.have(c),
-                          (int)p.v.dim - (int)v0, t, THREADS);
-    }
-    const uint64_t at = p.prepared.at(p.sh, slot, h);
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        tile_load<64>(smem_u32(st.inverse[i]), p.prepared.inverse + (at * 2 + i) * DR_TILE, 64, 64, 64, 64, t, THREADS);
-        tile_load<64>(smem_u32(st.read[i]), p.prepared.read + (at * 2 + i) * DR_TILE, 64, 64, 64, 64, t, THREADS);
-    }
-    for (int i = t; i < 3 * DR_CHUNK / 4; i += THREADS)
-        cp_async16(&st.gates[0][0] + i * 4, p.prepared.gates + at * 3 * DR_CHUNK + i * 4);
-}
 
 // The state's 16 rows of this warp, from or to float32 [value_dim][key_dim].
 template <int NT>
@@ -384,53 +458,20 @@ __device__ __forceinline__ void dr_state_in(float (&s)[NT][4], const float* from
         }
 }
 template <int NT>
-__device__ __forceinline__ void dr_state_out(const float (&s)[NT][4], float* to, uint32_t row, uint32_t rows, uint32_t cols, int col) {
+__device__ __forceinline__ void dr_state_out(const float (&s)[NT][4], float by, float* to, uint32_t row, uint32_t rows, uint32_t cols, int col) {
     if (!to) return;
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const uint32_t r = row + (j >> 1) * 8, c = n * 8 + col + (j & 1);
-            if (r < rows && c < cols) to[(uint64_t)r * cols + c] = s[n][j];
+            if (r < rows && c < cols) to[(uint64_t)r * cols + c] = s[n][j] * by;
         }
-}
-
-// c (16 x 64: value x token) += s (16 x DK) K^T
-template <int DK, int PLANES>
-__device__ __forceinline__ void dr_times_keys(float (&c)[8][4], const uint32_t (&hi)[4], const uint32_t (&lo)[4],
-                                              const uint32_t (&k)[PLANES], int kk, int lane) {
-#pragma unroll
-    for (int n = 0; n < 4; ++n) {
-        uint32_t b[4];
-        load_b<DK>(b, k[0], n * 16, kk * 2, lane);
-        mma_bf16(c[2 * n], hi, b[0], b[1]), mma_bf16(c[2 * n + 1], hi, b[2], b[3]);
-        mma_bf16(c[2 * n], lo, b[0], b[1]), mma_bf16(c[2 * n + 1], lo, b[2], b[3]);
-        if constexpr (PLANES == 2) {
-            load_b<DK>(b, k[PLANES - 1], n * 16, kk * 2, lane);
-            mma_bf16(c[2 * n], hi, b[0], b[1]), mma_bf16(c[2 * n + 1], hi, b[2], b[3]);
-        }
-    }
-}
-// s (16 x DK) += a (16 x 16 tokens: hi + lo) times rows [16 kt, 16 kt + 16) of a tile of keys or queries
-template <int DK, int PLANES>
-__device__ __forceinline__ void dr_add_outer(float (&s)[DK / 8][4], const uint32_t (&hi)[4], const uint32_t (&lo)[4],
-                                             const uint32_t (&tile)[PLANES], int kt, int lane) {
-#pragma unroll
-    for (int n = 0; n < DK / 16; ++n) {
-        uint32_t b[4];
-        load_b_t<DK>(b, tile[0], kt * 16, n * 2, lane);
-        mma_bf16(s[2 * n], hi, b[0], b[1]), mma_bf16(s[2 * n + 1], hi, b[2], b[3]);
-        mma_bf16(s[2 * n], lo, b[0], b[1]), mma_bf16(s[2 * n + 1], lo, b[2], b[3]);
-        if constexpr (PLANES == 2) {
-            load_b_t<DK>(b, tile[PLANES - 1], kt * 16, n * 2, lane);
-            mma_bf16(s[2 * n], hi, b[0], b[1]), mma_bf16(s[2 * n + 1], hi, b[2], b[3]);
-        }
-    }
 }
 
 template <typename T>
-__device__ __forceinline__ void dr_store_pair(T* to, uint32_t col, uint32_t cols, bool even, float x, float y) {
-    if (even && col + 1 < cols) {
+__device__ __forceinline__ void dr_store_pair(T* to, uint32_t col, uint32_t cols, bool pairs, float x, float y) {
+    if (pairs && col + 1 < cols) {
         if constexpr (sizeof(T) == 4) *(float2*)(to + col) = make_float2(x, y);
         else if constexpr (std::is_same_v<T, __half>) *(__half2*)(to + col) = __floats2half2_rn(x, y);
         else *(__nv_bfloat162*)(to + col) = __floats2bfloat162_rn(x, y);
@@ -440,586 +481,848 @@ __device__ __forceinline__ void dr_store_pair(T* to, uint32_t col, uint32_t cols
     }
 }
 
-template <typename T, int DK, int PLANES, int WARPS>
+// What both directions share: where a CTA's warps are, the copies of the chunks' images, and products with them.
+template <typename T, int DK, int WARPS>
+struct DrChainCta {
+    using Smem = DrChainSmem<T, DK, WARPS>;
+    static constexpr int PLANES = Smem::PLANES, NB = DK / 64, NT = DK / 8, STAGES = Smem::STAGES, KEYS = DR_KEYS<DK, PLANES>;
+    const DrChain& p;
+    Smem& sm;
+    const int lane, warp, g, col;
+    const LaneOffsets o;
+    uint32_t h, hk, seq, v0, live, row, limit;
+    uint64_t start, end, base, state;
+    uint32_t chunks;
+    bool ok = true;
+
+    __device__ __forceinline__ DrChainCta(const DrChain& p_, Smem& sm_)
+        : p(p_), sm(sm_), lane(threadIdx.x & 31), warp(threadIdx.x >> 5), g((threadIdx.x & 31) >> 2), col((threadIdx.x & 3) * 2),
+          o(threadIdx.x & 31) {
+        const DrShape& sh = p.sh;
+        const uint32_t slices = (sh.value_dim + WARPS * 16 - 1) / (WARPS * 16);
+        h = blockIdx.x / slices % sh.heads, seq = blockIdx.x / slices / sh.heads;
+        hk = h / (sh.heads / sh.key_heads), v0 = blockIdx.x % slices * WARPS * 16;
+        live = min((uint32_t)WARPS, (sh.value_dim - v0 + 15) / 16);
+        row = v0 + warp * 16 + g;
+        start = sh.start(seq), end = min(sh.start(seq + 1), sh.rows), base = sh.base(seq);
+        chunks = end > start ? (uint32_t)((end - start + DR_CHUNK - 1) / DR_CHUNK) : 0;
+        state = ((uint64_t)seq * sh.heads + h) * sh.value_dim * sh.key_dim;
+        limit = g_spin_limit;
+        if (threadIdx.x == 0) {
+            for (int i = 0; i < STAGES; ++i) mbar_init(&sm.full[i], 1), mbar_init(&sm.empty[i], live);
+            fence_mbar_init();
+        }
+        __syncthreads();
+    }
+    __device__ __forceinline__ uint64_t unit(uint32_t chunk) const { return (base + chunk) * p.sh.heads + h; }
+    __device__ __forceinline__ uint32_t rows(uint32_t chunk) const {
+        return (uint32_t)min((uint64_t)DR_CHUNK, end - start - (uint64_t)chunk * DR_CHUNK);
+    }
+    __device__ __forceinline__ void load(uint32_t stage, uint32_t chunk) {  // one thread
+        mbar_arrive_expect_tx(&sm.full[stage], Smem::STAGE);
+        bulk_load(sm.stage[stage], p.keys + ((base + chunk) * p.sh.key_heads + hk) * (2 * KEYS), 2 * KEYS, &sm.full[stage]);
+        bulk_load(sm.stage[stage] + 2 * KEYS, p.units + unit(chunk) * DR_UNIT, DR_UNIT, &sm.full[stage]);
+    }
+    __device__ __forceinline__ void load_values(uint32_t buffer, uint32_t chunk) {
+        if (!p.values) return;
+        const T* const from = (const T*)p.values + (start + (uint64_t)chunk * DR_CHUNK) * p.value_stride + (uint64_t)h * p.sh.value_dim + v0 + warp * 16;
+        dr_raw_load<T>(smem_u32(sm.raw[warp][buffer]), from, p.value_stride, rows(chunk), (int)(p.sh.value_dim - v0) - warp * 16, p.wide, lane);
+    }
+    // Step `it` is chunk order(it).  Waits for its images, then for its values, and starts the next ones.
+    template <typename F>
+    __device__ __forceinline__ bool begin(uint32_t it, F&& order) {
+        cp_async_wait_all();
+        __syncwarp();
+        if (it + 1 < chunks) load_values((it + 1) & 1, order(it + 1));
+        cp_async_commit();
+        ok = __all_sync(0xffffffffu, mbar_wait(&sm.full[it % STAGES], (it / STAGES) & 1, limit));
+        return ok;
+    }
+    // Two stages: the next images are asked for amid a step, when the other warps have left the step before.
+    template <typename F>
+    __device__ __forceinline__ void ahead(uint32_t it, F&& order) {
+        if (STAGES == 2 && warp == 0 && lane == 0 && it + 1 < chunks && it >= 1) {
+            if (mbar_wait(&sm.empty[(it + 1) & 1], ((it - 1) / 2) & 1, limit)) load((it + 1) & 1, order(it + 1));
+            else set_error(LCPP_ERR_LOOKBACK_TIMEOUT);
+        }
+        __syncwarp();
+    }
+    template <typename F>
+    __device__ __forceinline__ void finish(uint32_t it, F&& order) {
+        __syncwarp();
+        if (lane == 0) {
+            asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&sm.empty[it % STAGES])) : "memory");
+            if (STAGES == 1 && warp == 0 && it + 1 < chunks) {
+                if (mbar_wait(&sm.empty[0], it & 1, limit)) load(0, order(it + 1));
+                else set_error(LCPP_ERR_LOOKBACK_TIMEOUT);
+            }
+        }
+        __syncwarp();
+    }
+    // c (16 x 64: value x token) += s (16 x 16 kk .. 16 kk + 16) K^T
+    __device__ __forceinline__ void times_keys(float (&c)[8][4], const uint32_t (&hi)[4], const uint32_t (&lo)[4], uint32_t k, int kk) const {
+#pragma unroll
+        for (int i = 0; i < PLANES; ++i)
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+                uint32_t b[4];
+                load_b(b, k + (i * NB + (kk >> 2)) * DR_BLOCK, n * 16, kk & 3, o);
+                mma_f16_2(c[2 * n], c[2 * n + 1], hi, b);
+                if (i == 0) mma_f16_2(c[2 * n], c[2 * n + 1], lo, b);
+            }
+    }
+    // s (16 x DK) += a (16 x tokens 16 kt .. 16 kt + 16) times the rows of K or Q
+    template <bool EXACT>
+    __device__ __forceinline__ void add_outer(float (&s)[NT][4], const uint32_t (&hi)[4], const uint32_t (&lo)[4], uint32_t tile, int kt) const {
+#pragma unroll
+        for (int i = 0; i < PLANES; ++i)
+#pragma unroll
+            for (int n = 0; n < DK / 16; ++n) {
+                uint32_t b[4];
+                load_b_t(b, tile + (i * NB + (n >> 2)) * DR_BLOCK, kt * 16, n & 3, o);
+                mma_f16_2(s[2 * n], s[2 * n + 1], hi, b);
+                if (i == 0 && !EXACT) mma_f16_2(s[2 * n], s[2 * n + 1], lo, b);
+            }
+    }
+    // The state's fragment kk to an image.
+    __device__ __forceinline__ void keep_state(uint8_t* image, const uint32_t (&hi)[4], const uint32_t (&lo)[4], int kk) const {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) dr_store(image, NB, row + (j & 1) * 8, kk * 16 + (j >> 1) * 8 + col, hi[j], lo[j]);
+    }
+    __device__ __forceinline__ void keep_values(uint8_t* image, const uint32_t (&hi)[4], const uint32_t (&lo)[4], int kt) const {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) dr_store(image, 1, row + (j & 1) * 8, kt * 16 + (j >> 1) * 8 + col, hi[j], lo[j]);
+    }
+    __device__ __forceinline__ void keep_back(float* back, uint64_t unit, float v) const {
+        if (lane == 0) back[unit * 8 + (v0 >> 4) + warp] = v;
+    }
+};
+
+template <typename T, int DK, int WARPS>
 __global__ void __launch_bounds__(WARPS * 32, 1)
 dr_forward_kernel(const __grid_constant__ DrChain p) {
-    constexpr int NT = DK / 8, VC = WARPS > 4 ? 128 : 64;
+    using Cta = DrChainCta<T, DK, WARPS>;
+    constexpr int NT = Cta::NT, NB = Cta::NB, PLANES = Cta::PLANES, KEYS = Cta::KEYS;
+    constexpr bool FINE = !std::is_same_v<T, __nv_bfloat16>;  // outputs of 8 bits need one part of the state and of u (11 bits)
     extern __shared__ __align__(128) uint8_t dr_smem[];
-    auto& smem = *(DrChainSmem<DK, PLANES, WARPS>*)dr_smem;
-    const uint32_t slices = (p.sh.value_dim + WARPS * 16 - 1) / (WARPS * 16);
-    const uint32_t slice = blockIdx.x % slices, h = blockIdx.x / slices % p.sh.heads, seq = blockIdx.x / slices / p.sh.heads;
-    const uint32_t hk = h / (p.sh.heads / p.sh.key_heads), v0 = slice * WARPS * 16;
-    const int t = threadIdx.x, lane = t & 31, warp = t >> 5, g = lane >> 2, col = (lane & 3) * 2;
-    const uint32_t row = v0 + warp * 16 + g;  // of the state: the thread's first
-    const uint64_t start = p.sh.start(seq), end = min(p.sh.start(seq + 1), p.sh.rows), base = p.sh.base(seq);
-    const uint32_t chunks = end > start ? (uint32_t)((end - start + DR_CHUNK - 1) / DR_CHUNK) : 0;
-    const uint64_t state = ((uint64_t)seq * p.sh.heads + h) * p.sh.value_dim * p.sh.key_dim;
-    float s[NT][4];
-    dr_state_in<NT>(s, p.from ? p.from + state : nullptr, row, p.sh.value_dim, p.sh.key_dim, col);
-    DrChunk c(p.sh, base);
-    auto chunk = [&](uint32_t i) {
-        c.row = start + (uint64_t)i * DR_CHUNK;
-        c.rows = (uint32_t)min((uint64_t)DR_CHUNK, end - c.row);
-        return c;
-    };
-    if (chunks) dr_load(smem.stage[0], p, chunk(0), base, h, hk, v0, t);
+    Cta cta(p, *(typename Cta::Smem*)dr_smem);
+    const int lane = cta.lane, warp = cta.warp, g = cta.g, col = cta.col;
+    const LaneOffsets& o = cta.o;
+    if (warp >= (int)cta.live) return;
+    auto order = [](uint32_t it) { return it; };
+    if (warp == 0 && lane == 0)
+        for (uint32_t i = 0; i < (uint32_t)Cta::STAGES && i < cta.chunks; ++i) cta.load(i, i);
+    __syncwarp();
+    if (cta.chunks) cta.load_values(0, 0);
     cp_async_commit();
-    T* const out = (T*)p.out;
-    const bool even = ((uintptr_t)out | p.out_stride * sizeof(T) | p.sh.value_dim * sizeof(T)) % (2 * sizeof(T)) == 0;
-    for (uint32_t i = 0; i < chunks; ++i) {
-        if (i + 1 < chunks) dr_load(smem.stage[(i + 1) & 1], p, chunk(i + 1), base + i + 1, h, hk, v0, t);
-        cp_async_commit();
-        cp_async_wait_prior1();
-        __syncthreads();
-        const DrChunk now = chunk(i);
-        auto& st = smem.stage[i & 1];
-        uint32_t k[PLANES], q[PLANES];
-#pragma unroll
-        for (int j = 0; j < PLANES; ++j) k[j] = smem_u32(st.k[j]), q[j] = smem_u32(st.q[j]);
-        const uint32_t inv[2] = {smem_u32(st.inverse[0]), smem_u32(st.inverse[1])},
-                       rd[2] = {smem_u32(st.read[0]), smem_u32(st.read[1])};
-        __nv_bfloat16* const saved = p.states.at ? p.states.of(p.sh, base + i, h) : nullptr;
-        // r = S0 K^T (value x token) and o = Q S0^T (token x value)
-        float r[8][4] = {}, o[4][2][4] = {};
+    float s[NT][4];  // the state times a power of two
+    float back_domain = 1.0f;
+    dr_state_in<NT>(s, p.from ? p.from + cta.state : nullptr, cta.row, p.sh.value_dim, p.sh.key_dim, col);
+    T* const out = (T*)p.out + (uint64_t)cta.h * p.sh.value_dim;
+    const bool pairs = ((uintptr_t)p.out | p.out_stride * sizeof(T) | p.sh.value_dim * sizeof(T)) % (2 * sizeof(T)) == 0;
+    for (uint32_t it = 0; it < cta.chunks; ++it) {
+        if (!cta.begin(it, order)) break;
+        const uint32_t stage = smem_u32(cta.sm.stage[it % Cta::STAGES]), k = stage, q = stage + KEYS, inv = stage + 2 * KEYS,
+                       rd = inv + 2 * DR_BLOCK;
+        const DrGates& gt = *(const DrGates*)(cta.sm.stage[it % Cta::STAGES] + 2 * KEYS + 4 * DR_BLOCK);
+        const uint64_t unit = cta.unit(it);
+        // r = S0 K^T (value x token) and out = Q S0^T (token x value)
+        float r[8][4] = {}, y[4][2][4] = {};
+        const Scale ss = scale_for(max_abs(s));
+        uint8_t* const states = p.states.at ? p.states.of(unit) : nullptr;
+        if (states) cta.keep_back(p.states.back, unit, ss.back * back_domain);
 #pragma unroll
         for (int kk = 0; kk < DK / 16; ++kk) {
             uint32_t hi[4], lo[4];
-            split_block(s[2 * kk], s[2 * kk + 1], hi, lo);
-            if (saved) {
+            split_block(s[2 * kk], s[2 * kk + 1], ss.by, hi, lo);
+            if (states) cta.keep_state(states, hi, lo, kk);
+            cta.times_keys(r, hi, lo, k, kk);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const uint32_t rr = row + (j & 1) * 8, cc = kk * 16 + (j >> 1) * 8 + col;
-                    if (rr < p.sh.value_dim && cc < p.key_cols) {
-                        __nv_bfloat16* const at = saved + rr * p.key_cols + cc;
-                        *(uint32_t*)at = hi[j];
-                        *(uint32_t*)(at + p.states.size) = lo[j];
-                    }
-                }
-            }
-            dr_times_keys<DK, PLANES>(r, hi, lo, k, kk, lane);
+            for (int i = 0; i < PLANES; ++i)
 #pragma unroll
-            for (int m = 0; m < 4; ++m) {
-                uint32_t a[4];
-                load_a<DK>(a, q[0], m * 16, kk * 2, lane);
-                mma_bf16(o[m][0], a, hi[0], hi[2]), mma_bf16(o[m][1], a, hi[1], hi[3]);
-                mma_bf16(o[m][0], a, lo[0], lo[2]), mma_bf16(o[m][1], a, lo[1], lo[3]);
-                if constexpr (PLANES == 2) {
-                    load_a<DK>(a, q[PLANES - 1], m * 16, kk * 2, lane);
-                    mma_bf16(o[m][0], a, hi[0], hi[2]), mma_bf16(o[m][1], a, hi[1], hi[3]);
+                for (int m = 0; m < 4; ++m) {
+                    uint32_t a[4];
+                    load_a(a, q + (i * NB + (kk >> 2)) * DR_BLOCK, m * 16, kk & 3, o);
+                    mma_f16(y[m][0], a, hi[0], hi[2]), mma_f16(y[m][1], a, hi[1], hi[3]);
+                    if (FINE && i == 0) mma_f16(y[m][0], a, lo[0], lo[2]), mma_f16(y[m][1], a, lo[1], lo[3]);
                 }
-            }
         }
+        const float back_state = ss.back * back_domain;
         // r = V - g S0 K^T
+        const uint32_t raw = smem_u32(cta.sm.raw[warp][it & 1]);
+        const float back_r = -back_state * gt.back_k;
 #pragma unroll
         for (int n = 0; n < 4; ++n) {
-            uint32_t v[PLANES][4];
+            float v[4][2];
+            dr_raw_get<T>(v, raw, n * 16, lane);
 #pragma unroll
-            for (int j = 0; j < PLANES; ++j) load_a_t<VC>(v[j], smem_u32(st.v[j]), n * 16, warp * 2, lane);
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {  // fragment register x: rows g + 8 (x & 1), tokens 16 n + 8 (x >> 1) + col
-                const float2 gate = *(const float2*)&st.gates[0][n * 16 + (x >> 1) * 8 + col];
-                float v0 = bf16_low(v[0][x]), v1 = bf16_high(v[0][x]);
-                if constexpr (PLANES == 2) v0 += bf16_low(v[PLANES - 1][x]), v1 += bf16_high(v[PLANES - 1][x]);
+            for (int x = 0; x < 4; ++x) {
+                const float2 gate = *(const float2*)&gt.g[n * 16 + (x >> 1) * 8 + col];
                 float* const d = &r[2 * n + (x >> 1)][(x & 1) * 2];
-                d[0] = fmaf(-gate.x, d[0], v0), d[1] = fmaf(-gate.y, d[1], v1);
+                d[0] = fmaf(gate.x * back_r, d[0], v[x][0]), d[1] = fmaf(gate.y * back_r, d[1], v[x][1]);
             }
         }
+        cta.ahead(it, order);
         // w = r inverse^T
+        const Scale sr = scale_for(max_abs(r));
         float w[8][4] = {};
 #pragma unroll
         for (int kt = 0; kt < 4; ++kt) {
             uint32_t hi[4], lo[4];
-            split_block(r[2 * kt], r[2 * kt + 1], hi, lo);
+            split_block(r[2 * kt], r[2 * kt + 1], sr.by, hi, lo);
 #pragma unroll
             for (int n = kt; n < 4; ++n) {
                 uint32_t b[4];
-                load_b<64>(b, inv[0], n * 16, kt * 2, lane);
-                mma_bf16(w[2 * n], hi, b[0], b[1]), mma_bf16(w[2 * n + 1], hi, b[2], b[3]);
-                mma_bf16(w[2 * n], lo, b[0], b[1]), mma_bf16(w[2 * n + 1], lo, b[2], b[3]);
-                load_b<64>(b, inv[1], n * 16, kt * 2, lane);
-                mma_bf16(w[2 * n], hi, b[0], b[1]), mma_bf16(w[2 * n + 1], hi, b[2], b[3]);
+                load_b(b, inv, n * 16, kt, o);
+                mma_f16_2(w[2 * n], w[2 * n + 1], hi, b);
+                mma_f16_2(w[2 * n], w[2 * n + 1], lo, b);
+                load_b(b, inv + DR_BLOCK, n * 16, kt, o);
+                mma_f16_2(w[2 * n], w[2 * n + 1], hi, b);
             }
         }
-        if (p.values.at) {
-            __nv_bfloat16* const values = p.values.of(p.sh, base + i, h);
+        const float back_w = sr.back * gt.back_inverse;
+        if (p.kept.at) {
+            const Scale sw = scale_for(max_abs(w));
+            uint8_t* const kept = p.kept.of(unit);
+            cta.keep_back(p.kept.back, unit, sw.back * back_w);
 #pragma unroll
-            for (int n = 0; n < 8; ++n)
-#pragma unroll
-                for (int j = 0; j < 2; ++j)
-                    if (row + j * 8 < p.sh.value_dim)
-                        dr_store_planes(values, p.values.size, DR_CHUNK, row + j * 8, n * 8 + col, w[n][2 * j], w[n][2 * j + 1]);
+            for (int kt = 0; kt < 4; ++kt) {
+                uint32_t hi[4], lo[4];
+                split_block(w[2 * kt], w[2 * kt + 1], sw.by, hi, lo);
+                cta.keep_values(kept, hi, lo, kt);
+            }
         }
 #pragma unroll
         for (int n = 0; n < 8; ++n) {  // u
-            const float2 b = *(const float2*)&st.gates[2][n * 8 + col];
-            w[n][0] *= b.x, w[n][1] *= b.y, w[n][2] *= b.x, w[n][3] *= b.y;
+            const float2 b = *(const float2*)&gt.beta[n * 8 + col];
+            w[n][0] *= b.x * back_w, w[n][1] *= b.y * back_w, w[n][2] *= b.x * back_w, w[n][3] *= b.y * back_w;
         }
-        // o = scale g o + A u
+        // out = scale g out + A u
+        const Scale su = scale_for(max_abs(w));
+        {
+            const float by = p.sh.scale * back_state * gt.back_q, into = su.by * __frcp_rn(gt.back_read);
 #pragma unroll
-        for (int m = 0; m < 4; ++m) {
-            const float g0 = st.gates[0][m * 16 + g] * p.sh.scale, g1 = st.gates[0][m * 16 + g + 8] * p.sh.scale;
+            for (int m = 0; m < 4; ++m) {
+                const float g0 = gt.g[m * 16 + g] * by * into, g1 = gt.g[m * 16 + g + 8] * by * into;
 #pragma unroll
-            for (int n = 0; n < 2; ++n) o[m][n][0] *= g0, o[m][n][1] *= g0, o[m][n][2] *= g1, o[m][n][3] *= g1;
+                for (int n = 0; n < 2; ++n) y[m][n][0] *= g0, y[m][n][1] *= g0, y[m][n][2] *= g1, y[m][n][3] *= g1;
+            }
         }
 #pragma unroll
         for (int kt = 0; kt < 4; ++kt) {
             uint32_t hi[4], lo[4];
-            split_block(w[2 * kt], w[2 * kt + 1], hi, lo);
+            split_block(w[2 * kt], w[2 * kt + 1], su.by, hi, lo);
 #pragma unroll
             for (int m = kt; m < 4; ++m) {
                 uint32_t a[4];
-                load_a<64>(a, rd[0], m * 16, kt * 2, lane);
-                mma_bf16(o[m][0], a, hi[0], hi[2]), mma_bf16(o[m][1], a, hi[1], hi[3]);
-                mma_bf16(o[m][0], a, lo[0], lo[2]), mma_bf16(o[m][1], a, lo[1], lo[3]);
-                load_a<64>(a, rd[1], m * 16, kt * 2, lane);
-                mma_bf16(o[m][0], a, hi[0], hi[2]), mma_bf16(o[m][1], a, hi[1], hi[3]);
+                load_a(a, rd, m * 16, kt, o);
+                mma_f16(y[m][0], a, hi[0], hi[2]), mma_f16(y[m][1], a, hi[1], hi[3]);
+                if constexpr (FINE) {
+                    mma_f16(y[m][0], a, lo[0], lo[2]), mma_f16(y[m][1], a, lo[1], lo[3]);
+                    load_a(a, rd + DR_BLOCK, m * 16, kt, o);
+                    mma_f16(y[m][0], a, hi[0], hi[2]), mma_f16(y[m][1], a, hi[1], hi[3]);
+                }
             }
         }
+        {
+            const float back = su.back * gt.back_read;
+            const uint32_t have = cta.rows(it);
+            T* const first = out + (cta.start + (uint64_t)it * DR_CHUNK + g) * p.out_stride;
 #pragma unroll
-        for (int m = 0; m < 4; ++m)
+            for (int m = 0; m < 4; ++m)
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const uint32_t token = m * 16 + g + j * 8;
-                if (token >= now.rows) continue;
-                T* const to = out + (now.row + token) * p.out_stride + (uint64_t)h * p.sh.value_dim;
+                for (int j = 0; j < 2; ++j) {
+                    if (m * 16 + j * 8 + g >= have) continue;
+                    T* const to = first + (m * 16 + j * 8) * p.out_stride;
 #pragma unroll
-                for (int n = 0; n < 2; ++n)
-                    dr_store_pair(to, v0 + warp * 16 + n * 8 + col, p.sh.value_dim, even, o[m][n][2 * j], o[m][n][2 * j + 1]);
-            }
-        // S = g_64 S + (e u)^T K
-        const float whole = st.gates[0][DR_CHUNK - 1];
+                    for (int n = 0; n < 2; ++n)
+                        dr_store_pair(to, cta.v0 + warp * 16 + n * 8 + col, p.sh.value_dim, pairs, y[m][n][2 * j] * back, y[m][n][2 * j + 1] * back);
+                }
+        }
+        // S = g_64 S + (e u)^T K, in the domain of the product
+#pragma unroll
+        for (int n = 0; n < 8; ++n) {
+            const float2 e = *(const float2*)&gt.e[n * 8 + col];
+            w[n][0] *= e.x, w[n][1] *= e.y, w[n][2] *= e.x, w[n][3] *= e.y;
+        }
+        const Scale se = scale_for(max_abs(w));
+        const float into = se.by * __frcp_rn(gt.back_k), whole = gt.g[DR_CHUNK - 1] * back_domain * into;
+        back_domain = se.back * gt.back_k;
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int j = 0; j < 4; ++j) s[n][j] *= whole;
 #pragma unroll
         for (int kt = 0; kt < 4; ++kt) {
-#pragma unroll
-            for (int n = 2 * kt; n < 2 * kt + 2; ++n) {
-                const float2 e = *(const float2*)&st.gates[1][n * 8 + col];
-                w[n][0] *= e.x, w[n][1] *= e.y, w[n][2] *= e.x, w[n][3] *= e.y;
-            }
             uint32_t hi[4], lo[4];
-            split_block(w[2 * kt], w[2 * kt + 1], hi, lo);
-            dr_add_outer<DK, PLANES>(s, hi, lo, k, kt, lane);
+            split_block(w[2 * kt], w[2 * kt + 1], se.by, hi, lo);
+            cta.template add_outer<false>(s, hi, lo, k, kt);
         }
-        __syncthreads();  // the stage is free
+        cta.finish(it, order);
     }
-    dr_state_out<NT>(s, p.to ? p.to + state : nullptr, row, p.sh.value_dim, p.sh.key_dim, col);
+    if (!cta.ok) set_error(LCPP_ERR_LOOKBACK_TIMEOUT);
+    dr_state_out<NT>(s, back_domain, p.to ? p.to + cta.state : nullptr, cta.row, p.sh.value_dim, p.sh.key_dim, col);
 }
 
-template <int DK, int PLANES, int WARPS>
+template <typename T, int DK, int WARPS>
 __global__ void __launch_bounds__(WARPS * 32, 1)
 dr_backward_kernel(const __grid_constant__ DrChain p) {
-    constexpr int NT = DK / 8, VC = WARPS > 4 ? 128 : 64;
+    using Cta = DrChainCta<T, DK, WARPS>;
+    constexpr int NT = Cta::NT, KEYS = Cta::KEYS;
+    constexpr bool EXACT = sizeof(T) == 2;  // dO in one part
     extern __shared__ __align__(128) uint8_t dr_smem[];
-    auto& smem = *(DrChainSmem<DK, PLANES, WARPS>*)dr_smem;
-    const uint32_t slices = (p.sh.value_dim + WARPS * 16 - 1) / (WARPS * 16);
-    const uint32_t slice = blockIdx.x % slices, h = blockIdx.x / slices % p.sh.heads, seq = blockIdx.x / slices / p.sh.heads;
-    const uint32_t hk = h / (p.sh.heads / p.sh.key_heads), v0 = slice * WARPS * 16;
-    const int t = threadIdx.x, lane = t & 31, warp = t >> 5, g = lane >> 2, col = (lane & 3) * 2;
-    const uint32_t row = v0 + warp * 16 + g;
-    const uint64_t start = p.sh.start(seq), end = min(p.sh.start(seq + 1), p.sh.rows), base = p.sh.base(seq);
-    const uint32_t chunks = end > start ? (uint32_t)((end - start + DR_CHUNK - 1) / DR_CHUNK) : 0;
-    const uint64_t state = ((uint64_t)seq * p.sh.heads + h) * p.sh.value_dim * p.sh.key_dim;
-    float x[NT][4];
-    dr_state_in<NT>(x, p.from ? p.from + state : nullptr, row, p.sh.value_dim, p.sh.key_dim, col);
-    DrChunk c(p.sh, base);
-    auto chunk = [&](uint32_t i) {
-        c.row = start + (uint64_t)i * DR_CHUNK;
-        c.rows = (uint32_t)min((uint64_t)DR_CHUNK, end - c.row);
-        return c;
-    };
-    if (chunks) dr_load(smem.stage[0], p, chunk(chunks - 1), base + chunks - 1, h, hk, v0, t);
+    Cta cta(p, *(typename Cta::Smem*)dr_smem);
+    const int lane = cta.lane, warp = cta.warp, col = cta.col;
+    const LaneOffsets& o = cta.o;
+    if (warp >= (int)cta.live) return;
+    const uint32_t last = cta.chunks - 1;
+    auto order = [last](uint32_t it) { return last - it; };
+    if (warp == 0 && lane == 0)
+        for (uint32_t i = 0; i < (uint32_t)Cta::STAGES && i < cta.chunks; ++i) cta.load(i, order(i));
+    __syncwarp();
+    if (cta.chunks) cta.load_values(0, last);
     cp_async_commit();
-    for (uint32_t i = 0; i < chunks; ++i) {
-        const uint64_t slot = base + chunks - 1 - i;
-        if (i + 1 < chunks) dr_load(smem.stage[(i + 1) & 1], p, chunk(chunks - 2 - i), slot - 1, h, hk, v0, t);
-        cp_async_commit();
-        cp_async_wait_prior1();
-        __syncthreads();
-        auto& st = smem.stage[i & 1];
-        uint32_t k[PLANES], q[PLANES], go[PLANES];
-#pragma unroll
-        for (int j = 0; j < PLANES; ++j) k[j] = smem_u32(st.k[j]), q[j] = smem_u32(st.q[j]), go[j] = smem_u32(st.v[j]);
-        const uint32_t inv[2] = {smem_u32(st.inverse[0]), smem_u32(st.inverse[1])},
-                       rd[2] = {smem_u32(st.read[0]), smem_u32(st.read[1])};
+    float x[NT][4];  // the state's gradient times a power of two
+    float back_domain = 1.0f;
+    dr_state_in<NT>(x, p.from ? p.from + cta.state : nullptr, cta.row, p.sh.value_dim, p.sh.key_dim, col);
+    for (uint32_t it = 0; it < cta.chunks; ++it) {
+        if (!cta.begin(it, order)) break;
+        const uint32_t stage = smem_u32(cta.sm.stage[it % Cta::STAGES]), k = stage, q = stage + KEYS, inv = stage + 2 * KEYS,
+                       rd = inv + 2 * DR_BLOCK;
+        const DrGates& gt = *(const DrGates*)(cta.sm.stage[it % Cta::STAGES] + 2 * KEYS + 4 * DR_BLOCK);
+        const uint64_t unit = cta.unit(order(it));
+        const uint32_t raw = smem_u32(cta.sm.raw[warp][it & 1]);
         // du = e X K^T (value x token)
         float du[8][4] = {};
-        __nv_bfloat16* const states = p.states.of(p.sh, slot, h);
+        const Scale sx = scale_for(max_abs(x));
+        uint8_t* const states = p.states.of(unit);
+        cta.keep_back(p.states.back, unit, sx.back * back_domain);
 #pragma unroll
         for (int kk = 0; kk < DK / 16; ++kk) {
             uint32_t hi[4], lo[4];
-            split_block(x[2 * kk], x[2 * kk + 1], hi, lo);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const uint32_t rr = row + (j & 1) * 8, cc = kk * 16 + (j >> 1) * 8 + col;
-                if (rr < p.sh.value_dim && cc < p.key_cols) {
-                    __nv_bfloat16* const at = states + rr * p.key_cols + cc;
-                    *(uint32_t*)at = hi[j];
-                    *(uint32_t*)(at + p.states.size) = lo[j];
-                }
-            }
-            dr_times_keys<DK, PLANES>(du, hi, lo, k, kk, lane);
-        }
-#pragma unroll
-        for (int n = 0; n < 8; ++n) {
-            const float2 e = *(const float2*)&st.gates[1][n * 8 + col];
-            du[n][0] *= e.x, du[n][1] *= e.y, du[n][2] *= e.x, du[n][3] *= e.y;
+            split_block(x[2 * kk], x[2 * kk + 1], sx.by, hi, lo);
+            cta.keep_state(states, hi, lo, kk);
+            cta.times_keys(du, hi, lo, k, kk);
         }
         // ... + dO^T A
-        if (p.v.at) {
+        float most = 0.0f, most_g = 0.0f;
+        if (p.values) {
 #pragma unroll
             for (int kt = 0; kt < 4; ++kt) {
-                uint32_t a[PLANES][4];
+                float v[4][2];
+                dr_raw_get<T>(v, raw, kt * 16, lane);
 #pragma unroll
-                for (int j = 0; j < PLANES; ++j) load_a_t<VC>(a[j], go[j], kt * 16, warp * 2, lane);
+                for (int j = 0; j < 4; ++j) {
+                    const float2 gate = *(const float2*)&gt.g[kt * 16 + (j >> 1) * 8 + col];
+                    most = fmaxf(most, fmaxf(fabsf(v[j][0]), fabsf(v[j][1])));
+                    most_g = fmaxf(most_g, fmaxf(fabsf(v[j][0] * gate.x), fabsf(v[j][1] * gate.y)));
+                }
+            }
+        }
+        const Scale so = scale_for(warp_max(most)), sg = scale_for(warp_max(most_g) * fabsf(p.sh.scale));
+        cta.keep_back(p.back_values, unit, so.back);
+        {
+            const float back = sx.back * back_domain * gt.back_k * so.by * __frcp_rn(gt.back_read);
+#pragma unroll
+            for (int n = 0; n < 8; ++n) {
+                const float2 e = *(const float2*)&gt.e[n * 8 + col];
+                du[n][0] *= e.x * back, du[n][1] *= e.y * back, du[n][2] *= e.x * back, du[n][3] *= e.y * back;
+            }
+        }
+        if (p.values) {
+#pragma unroll
+            for (int kt = 0; kt < 4; ++kt) {
+                float v[4][2];
+                uint32_t hi[4], lo[4];
+                dr_raw_get<T>(v, raw, kt * 16, lane);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) split_f16(v[j][0], v[j][1], so.by, hi[j], lo[j]);
 #pragma unroll
                 for (int n = 0; n <= kt; ++n) {
                     uint32_t b[4];
-                    load_b_t<64>(b, rd[0], kt * 16, n * 2, lane);
-#pragma unroll
-                    for (int j = 0; j < PLANES; ++j) mma_bf16(du[2 * n], a[j], b[0], b[1]), mma_bf16(du[2 * n + 1], a[j], b[2], b[3]);
-                    load_b_t<64>(b, rd[1], kt * 16, n * 2, lane);
-                    mma_bf16(du[2 * n], a[0], b[0], b[1]), mma_bf16(du[2 * n + 1], a[0], b[2], b[3]);
+                    load_b_t(b, rd, kt * 16, n, o);
+                    mma_f16_2(du[2 * n], du[2 * n + 1], hi, b);
+                    if constexpr (!EXACT) mma_f16_2(du[2 * n], du[2 * n + 1], lo, b);
+                    load_b_t(b, rd + DR_BLOCK, kt * 16, n, o);
+                    mma_f16_2(du[2 * n], du[2 * n + 1], hi, b);
                 }
             }
         }
+        cta.ahead(it, order);
         // z = du inverse
+        const Scale sd = scale_for(max_abs(du));
         float z[8][4] = {};
 #pragma unroll
         for (int kt = 0; kt < 4; ++kt) {
             uint32_t hi[4], lo[4];
-            split_block(du[2 * kt], du[2 * kt + 1], hi, lo);
+            split_block(du[2 * kt], du[2 * kt + 1], sd.by, hi, lo);
 #pragma unroll
             for (int n = 0; n <= kt; ++n) {
                 uint32_t b[4];
-                load_b_t<64>(b, inv[0], kt * 16, n * 2, lane);
-                mma_bf16(z[2 * n], hi, b[0], b[1]), mma_bf16(z[2 * n + 1], hi, b[2], b[3]);
-                mma_bf16(z[2 * n], lo, b[0], b[1]), mma_bf16(z[2 * n + 1], lo, b[2], b[3]);
-                load_b_t<64>(b, inv[1], kt * 16, n * 2, lane);
-                mma_bf16(z[2 * n], hi, b[0], b[1]), mma_bf16(z[2 * n + 1], hi, b[2], b[3]);
+                load_b_t(b, inv, kt * 16, n, o);
+                mma_f16_2(z[2 * n], z[2 * n + 1], hi, b);
+                mma_f16_2(z[2 * n], z[2 * n + 1], lo, b);
+                load_b_t(b, inv + DR_BLOCK, kt * 16, n, o);
+                mma_f16_2(z[2 * n], z[2 * n + 1], hi, b);
             }
         }
-        __nv_bfloat16* const values = p.values.of(p.sh, slot, h);
+        const float back_z = sd.back * gt.back_inverse * so.back * gt.back_read;
+        {
+            const Scale sz = scale_for(max_abs(z));
+            uint8_t* const kept = p.kept.of(unit);
+            cta.keep_back(p.kept.back, unit, sz.back * back_z);
 #pragma unroll
-        for (int n = 0; n < 8; ++n)
+            for (int kt = 0; kt < 4; ++kt) {
+                uint32_t hi[4], lo[4];
+                split_block(z[2 * kt], z[2 * kt + 1], sz.by, hi, lo);
+                cta.keep_values(kept, hi, lo, kt);
+            }
+        }
+        // X = g_64 X + (scale g dO)^T Q - (g beta z)^T K, each in the domain of its product
+        float into = gt.g[DR_CHUNK - 1] * back_domain;
+        if (p.values) {
+            into *= sg.by * __frcp_rn(gt.back_q);
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
-                if (row + j * 8 < p.sh.value_dim)
-                    dr_store_planes(values, p.values.size, DR_CHUNK, row + j * 8, n * 8 + col, z[n][2 * j], z[n][2 * j + 1]);
-        // X = g_64 X + (scale g dO)^T Q - (g beta z)^T K
-        const float whole = st.gates[0][DR_CHUNK - 1];
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) x[n][j] *= into;
+#pragma unroll
+            for (int kt = 0; kt < 4; ++kt) {
+                float v[4][2];
+                uint32_t hi[4], lo[4];
+                dr_raw_get<T>(v, raw, kt * 16, lane);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float2 gate = *(const float2*)&gt.g[kt * 16 + (j >> 1) * 8 + col];
+                    split_f16(v[j][0] * (gate.x * p.sh.scale), v[j][1] * (gate.y * p.sh.scale), sg.by, hi[j], lo[j]);
+                }
+                cta.template add_outer<false>(x, hi, lo, q, kt);
+            }
+            into = sg.back * gt.back_q;
+        }
+#pragma unroll
+        for (int n = 0; n < 8; ++n) {
+            const float2 gate = *(const float2*)&gt.g[n * 8 + col], b = *(const float2*)&gt.beta[n * 8 + col];
+            const float y0 = -gate.x * b.x * back_z, y1 = -gate.y * b.y * back_z;
+            z[n][0] *= y0, z[n][1] *= y1, z[n][2] *= y0, z[n][3] *= y1;
+        }
+        const Scale sy = scale_for(max_abs(z));
+        into *= sy.by * __frcp_rn(gt.back_k);
+        back_domain = sy.back * gt.back_k;
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) x[n][j] *= whole;
+            for (int j = 0; j < 4; ++j) x[n][j] *= into;
 #pragma unroll
         for (int kt = 0; kt < 4; ++kt) {
             uint32_t hi[4], lo[4];
-            if (p.v.at) {
-                uint32_t a[PLANES][4];
-#pragma unroll
-                for (int j = 0; j < PLANES; ++j) load_a_t<VC>(a[j], go[j], kt * 16, warp * 2, lane);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float2 gate = *(const float2*)&st.gates[0][kt * 16 + (j >> 1) * 8 + col];
-                    float v0 = bf16_low(a[0][j]), v1 = bf16_high(a[0][j]);
-                    if constexpr (PLANES == 2) v0 += bf16_low(a[PLANES - 1][j]), v1 += bf16_high(a[PLANES - 1][j]);
-                    split_bf16(v0 * gate.x * p.sh.scale, v1 * gate.y * p.sh.scale, hi[j], lo[j]);
-                }
-                dr_add_outer<DK, PLANES>(x, hi, lo, q, kt, lane);
-            }
-#pragma unroll
-            for (int n = 2 * kt; n < 2 * kt + 2; ++n) {
-                const float2 gate = *(const float2*)&st.gates[0][n * 8 + col], b = *(const float2*)&st.gates[2][n * 8 + col];
-                const float y0 = -gate.x * b.x, y1 = -gate.y * b.y;
-                z[n][0] *= y0, z[n][1] *= y1, z[n][2] *= y0, z[n][3] *= y1;
-            }
-            split_block(z[2 * kt], z[2 * kt + 1], hi, lo);
-            dr_add_outer<DK, PLANES>(x, hi, lo, k, kt, lane);
+            split_block(z[2 * kt], z[2 * kt + 1], sy.by, hi, lo);
+            cta.template add_outer<false>(x, hi, lo, k, kt);
         }
-        __syncthreads();
+        cta.finish(it, order);
     }
-    dr_state_out<NT>(x, p.to ? p.to + state : nullptr, row, p.sh.value_dim, p.sh.key_dim, col);
+    if (!cta.ok) set_error(LCPP_ERR_LOOKBACK_TIMEOUT);
+    dr_state_out<NT>(x, back_domain, p.to ? p.to + cta.state : nullptr, cta.row, p.sh.value_dim, p.sh.key_dim, col);
 }
 
 // ---- gradients of the inputs ------------------------------------------------------------------------
 constexpr int DR_GRAD_THREADS = 256;  // warps: 4 blocks of 16 tokens x 2 halves of the key columns
-template <int DK, int PLANES>
+// 64 tokens x 32 of the value dimensions of dO: rows of 64 bytes with permuted pieces, float32 rows of 144 bytes.
+template <typename T>
+constexpr int DR_SLAB_ROW = sizeof(T) == 4 ? 144 : 64;
+template <typename T>
+__device__ __forceinline__ uint32_t dr_slab_at(uint32_t slab, int row, int piece) {
+    if constexpr (sizeof(T) == 4) return slab + row * 144 + piece * 16;
+    else return slab + row * 64 + ((piece ^ (row >> 1 & 3)) << 4);
+}
+template <typename T, int DK>
 struct DrGradientSmem {
-    __nv_bfloat16 k[PLANES][DR_CHUNK * DK], q[PLANES][DR_CHUNK * DK];
-    __nv_bfloat16 s[2][64 * DK], x[2][64 * DK];       // 64 of the value dimensions
-    __nv_bfloat16 w[2][64 * DR_CHUNK], z[2][64 * DR_CHUNK], go[PLANES][DR_CHUNK * 64];
-    __nv_bfloat16 da[2][DR_TILE], dn[2][DR_TILE];
-    float gates[3][DR_CHUNK];
-    double total[DR_CHUNK];
-    float dot[2][DR_CHUNK], carry[2][DR_CHUNK], dbeta[4][DR_CHUNK], sx[8];
+    static constexpr int PLANES = sizeof(T) == 4 ? 2 : 1, NB = DK / 64;
+    static constexpr int STATE = 2 * NB * DR_PIECE, KEPT = 2 * DR_PIECE, STEP = 2 * STATE + 2 * KEPT;  // S, X, w, z
+    alignas(128) uint8_t keys[2 * DR_KEYS<DK, PLANES>];
+    alignas(128) uint8_t step[2][STEP];
+    alignas(128) uint8_t slab[2][DR_CHUNK * DR_SLAB_ROW<T>];
+    alignas(128) uint8_t da[2 * DR_BLOCK];  // two planes
+    uint8_t dn[2 * DR_BLOCK];
+    DrGates gates;
+    float factor[5][8], back[5], own[4][8];  // of 16 value dimensions: shares of the largest scale; scales; of S, X, w, z
+    float by_out[8];                         // scales of dO
+    alignas(16) float dbeta[4][DR_CHUNK];  // also read and written in pairs
+    float dot[2][DR_CHUNK], carry[2][DR_CHUNK], most[2][8], sx[8];
+    uint64_t full[2], keys_full;
 };
 
 struct DrGradient {
     DrShape sh;
-    DrOperand q, k, go;
-    DrPrepared prepared;
-    const float* decay;
-    uint64_t decay_stride;
-    DrPlanes s, w, x, z;
-    uint32_t key_cols;
+    const uint8_t *keys, *units;
+    const void* out;  // dO, or null
+    uint64_t out_stride;
+    bool wide;
+    DrImage s, w, x, z;
+    const float* back_out;
     void *dq, *dk, *dv;
     float *ddecay, *dbeta;
     bool pairs_k, pairs_v;  // elements 2 i and 2 i + 1 of a row can be stored together: of dq and dk, of dv
 };
 
-template <typename T, int DK, int PLANES>
+template <typename T, int DK, bool SHARED>  // SHARED: several heads a key head
 __global__ void __launch_bounds__(DR_GRAD_THREADS, 1)
 dr_gradient_kernel(const __grid_constant__ DrGradient p) {
-    constexpr int NT = DK / 16, NP = DK / 32;  // tiles and pairs of tiles of 8 key columns a warp has
+    using Smem = DrGradientSmem<T, DK>;
+    constexpr int PLANES = Smem::PLANES, NB = Smem::NB, NT = DK / 16, NP = DK / 32;  // (pairs of) tiles of 8 key columns a warp has
+    constexpr bool EXACT = sizeof(T) == 2;
     extern __shared__ __align__(128) uint8_t dr_smem[];
-    auto& sm = *(DrGradientSmem<DK, PLANES>*)dr_smem;
-    const uint64_t slot = blockIdx.x / p.sh.key_heads;
-    const uint32_t hk = blockIdx.x % p.sh.key_heads, group = p.sh.heads / p.sh.key_heads;
-    const DrChunk c(p.sh, slot);
+    auto& sm = *(Smem*)dr_smem;
+    const DrShape& sh = p.sh;
+    const uint64_t slot = blockIdx.x / sh.key_heads;
+    const uint32_t hk = blockIdx.x % sh.key_heads, group = sh.heads / sh.key_heads, h0 = hk * group;
+    const DrChunk c(sh, slot);
     if (!c.rows) return;
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5, rb = warp >> 1, ch = warp & 1, g = lane >> 2, col = (lane & 3) * 2;
-    uint32_t k[PLANES], q[PLANES], go[PLANES];
+    const LaneOffsets o(lane);
+    const uint32_t limit = g_spin_limit, groups = (sh.value_dim + 15) / 16, steps = (groups + 1) / 2, total = steps * group;
+    bool ok = true;
+    auto load = [&](uint32_t it) {  // one thread
+        const uint64_t unit = slot * sh.heads + h0 + it / steps;
+        const uint32_t v = it % steps;
+        uint8_t* const to = sm.step[it & 1];
+        mbar_arrive_expect_tx(&sm.full[it & 1], Smem::STEP);
+        bulk_load(to, p.s.of(unit) + v * Smem::STATE, Smem::STATE, &sm.full[it & 1]);
+        bulk_load(to + Smem::STATE, p.x.of(unit) + v * Smem::STATE, Smem::STATE, &sm.full[it & 1]);
+        bulk_load(to + 2 * Smem::STATE, p.w.of(unit) + v * Smem::KEPT, Smem::KEPT, &sm.full[it & 1]);
+        bulk_load(to + 2 * Smem::STATE + Smem::KEPT, p.z.of(unit) + v * Smem::KEPT, Smem::KEPT, &sm.full[it & 1]);
+    };
+    auto load_out = [&](uint32_t it) {
+        if (!p.out) return;
+        constexpr int E = 16 / sizeof(T), PIECES = 32 / E;
+        const uint32_t v0 = it % steps * 32, slab = smem_u32(sm.slab[it & 1]);
+        const T* const from = (const T*)p.out + c.row * p.out_stride + (uint64_t)(h0 + it / steps) * sh.value_dim + v0;
 #pragma unroll
-    for (int i = 0; i < PLANES; ++i) {
-        k[i] = smem_u32(sm.k[i]), q[i] = smem_u32(sm.q[i]), go[i] = smem_u32(sm.go[i]);
-        tile_load<DK>(k[i], p.k.rows(slot, c, hk) + i * p.k.plane, p.k.row, DR_CHUNK, p.k.have(c), p.k.dim, t, DR_GRAD_THREADS);
-        tile_load<DK>(q[i], p.q.rows(slot, c, hk) + i * p.q.plane, p.q.row, DR_CHUNK, p.q.have(c), p.q.dim, t, DR_GRAD_THREADS);
+        for (int i = 0; i < DR_CHUNK * PIECES / DR_GRAD_THREADS; ++i) {
+            const uint32_t item = i * DR_GRAD_THREADS + t, r = item / PIECES, e = item % PIECES * E;
+            const uint32_t at = dr_slab_at<T>(slab, r, item % PIECES);
+            if (p.wide) {
+                const bool have = r < c.rows && v0 + e < sh.value_dim;
+                cp_async16_fill(at, have ? from + r * p.out_stride + e : from, have ? 16 : 0);
+            } else {
+                alignas(16) T w[E];
+#pragma unroll
+                for (int j = 0; j < E; ++j) w[j] = r < c.rows && v0 + e + j < sh.value_dim ? from[r * p.out_stride + e + j] : narrow<T>(0.0f);
+                const uint4 q = *(const uint4*)w;
+                asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(q.x), "r"(q.y), "r"(q.z), "r"(q.w) : "memory");
+            }
+        }
+    };
+    if (t == 0) {
+        mbar_init(&sm.full[0], 1), mbar_init(&sm.full[1], 1), mbar_init(&sm.keys_full, 1);
+        fence_mbar_init();
+        mbar_arrive_expect_tx(&sm.keys_full, 2 * DR_KEYS<DK, PLANES>);
+        bulk_load(sm.keys, p.keys + (slot * sh.key_heads + hk) * (2 * DR_KEYS<DK, PLANES>), 2 * DR_KEYS<DK, PLANES>, &sm.keys_full);
+        load(0);
     }
-    const uint32_t s[2] = {smem_u32(sm.s[0]), smem_u32(sm.s[1])}, x[2] = {smem_u32(sm.x[0]), smem_u32(sm.x[1])},
-                   w[2] = {smem_u32(sm.w[0]), smem_u32(sm.w[1])}, z[2] = {smem_u32(sm.z[0]), smem_u32(sm.z[1])},
-                   da[2] = {smem_u32(sm.da[0]), smem_u32(sm.da[1])}, dn[2] = {smem_u32(sm.dn[0]), smem_u32(sm.dn[1])};
-    float all_q[NT][4] = {}, all_k[NT][4] = {};  // sums over the key head's heads
+    load_out(0);
+    cp_async_commit();
+    const uint32_t k = smem_u32(sm.keys), q = k + DR_KEYS<DK, PLANES>, da = smem_u32(sm.da), dn = smem_u32(sm.dn);
+    float all_q[SHARED ? NT : 1][4] = {}, all_k[SHARED ? NT : 1][4] = {};  // sums over the key head's heads
     const uint32_t token = rb * 16 + g;
-    for (uint32_t h = hk * group; h < (hk + 1) * group; ++h) {
-        const uint64_t at = p.prepared.at(p.sh, slot, h);
-        __syncthreads();
-        if (t < 3 * DR_CHUNK) (&sm.gates[0][0])[t] = p.prepared.gates[at * 3 * DR_CHUNK + t];
-        if (warp == 7) {
-            double v[2];
+    uint32_t it = 0;
+    for (uint32_t h = h0; h < h0 + group; ++h) {
+        const uint64_t unit = slot * sh.heads + h;
+        // the heads' gates and scales; what the head before read is read (barriers of its end)
+        for (int i = t; i < (int)sizeof(DrGates) / 4; i += DR_GRAD_THREADS)
+            ((float*)&sm.gates)[i] = ((const float*)(p.units + unit * DR_UNIT + 4 * DR_BLOCK))[i];
+        if (warp < 5 && lane < 8) {
+            const bool have = lane < (int)groups;
+            const float s = have ? p.s.back[unit * 8 + lane] : 0.0f, x = have ? p.x.back[unit * 8 + lane] : 0.0f,
+                        w = have ? p.w.back[unit * 8 + lane] : 0.0f, z = have ? p.z.back[unit * 8 + lane] : 0.0f,
+                        go = have ? p.back_out[unit * 8 + lane] : 0.0f;
+            const float mine = warp == 0 ? go * s : warp == 1 ? z * s : warp == 2 ? w * x : warp == 3 ? go * w : z * w;
+            float most = mine;
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const uint32_t r = lane * 2 + j;
-                const float d = r < c.rows && p.decay ? p.decay[(c.row + r) * p.decay_stride + h] : 0.0f;
-                v[j] = d < DR_LEAST_DECAY ? DR_LEAST_DECAY : d;
-            }
-            double sum = v[0] + v[1];
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const double up = __shfl_up_sync(0xffffffffu, sum, o);
-                if (lane >= o) sum += up;
-            }
-            sm.total[lane * 2] = sum - v[1], sm.total[lane * 2 + 1] = sum;
+            for (int i = 4; i > 0; i >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffu, most, i));
+            sm.factor[warp][lane] = most > 0.0f ? mine / most : 0.0f;
+            if (lane == 0) sm.back[warp] = most;
+            if (warp == 4) sm.own[0][lane] = s, sm.own[1][lane] = x, sm.own[2][lane] = w, sm.own[3][lane] = z;
+            if (warp == 0) sm.by_out[lane] = go > 0.0f ? 1.0f / go : 0.0f;
         }
         float dq[NT][4] = {}, er[NT][4] = {}, wr[NT][4] = {}, a[4][4] = {}, n[4][4] = {};
-        float sx = 0.0f;
-        for (uint32_t v0 = 0; v0 < p.sh.value_dim; v0 += 64) {
-            if (v0) __syncthreads();
-            const int have = min((int)(p.sh.value_dim - v0), 64);
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                tile_load<DK>(s[i], p.s.of(p.sh, slot, h) + i * p.s.size + v0 * p.key_cols, p.key_cols, 64, have, p.key_cols, t, DR_GRAD_THREADS);
-                tile_load<DK>(x[i], p.x.of(p.sh, slot, h) + i * p.x.size + v0 * p.key_cols, p.key_cols, 64, have, p.key_cols, t, DR_GRAD_THREADS);
-                tile_load<64>(w[i], p.w.of(p.sh, slot, h) + i * p.w.size + v0 * DR_CHUNK, DR_CHUNK, 64, have, 64, t, DR_GRAD_THREADS);
-                tile_load<64>(z[i], p.z.of(p.sh, slot, h) + i * p.z.size + v0 * DR_CHUNK, DR_CHUNK, 64, have, 64, t, DR_GRAD_THREADS);
-            }
-#pragma unroll
-            for (int i = 0; i < PLANES; ++i)
-                if (p.go.at)
-                    tile_load<64>(go[i], p.go.rows(slot, c, h) + i * p.go.plane + v0, p.go.row, DR_CHUNK, p.go.have(c),
-                                  (int)p.go.dim - (int)v0, t, DR_GRAD_THREADS);
-            cp_async_commit();
+        float sx = 0.0f, db0 = 0.0f, db1 = 0.0f;
+        for (uint32_t v = 0; v < steps; ++v, ++it) {
             cp_async_wait_all();
-            __syncthreads();
+            __syncthreads();  // dO is there, and the buffers of the step before are free
+            if (it + 1 < total) {
+                if (t == 0) load(it + 1);
+                load_out(it + 1);
+            }
+            cp_async_commit();
+            if (it == 0) ok = mbar_wait(&sm.keys_full, 0, limit) && ok;
+            ok = mbar_wait(&sm.full[it & 1], (it >> 1) & 1, limit) && ok;
+            const uint8_t* const step = sm.step[it & 1];
+            const uint32_t s = smem_u32(step), x = s + Smem::STATE, w = x + Smem::STATE, z = w + Smem::KEPT,
+                           slab = smem_u32(sm.slab[it & 1]);
 #pragma unroll
-            for (int kt = 0; kt < 4; ++kt) {
-                uint32_t ag[PLANES][4], aw[2][4], az[2][4];
-                if (p.go.at) {
+            for (int kt = 0; kt < 2; ++kt) {
+                const uint32_t at = v * 2 + kt;  // 16 value dimensions
+                if (at >= groups) break;
+                uint32_t gs[2][4], gw[2][4], aw[2][4], zs[2][4], zw[2][4];
+                if (p.out) {
+                    const float by = sm.by_out[at];
+                    if constexpr (sizeof(T) == 2) {
+                        uint32_t r[4];
+                        ldmatrix4(r, dr_slab_at<T>(slab, rb * 16 + (lane & 15), kt * 2 + (lane >> 4)));
 #pragma unroll
-                    for (int i = 0; i < PLANES; ++i) load_a<64>(ag[i], go[i], rb * 16, kt * 2, lane);
+                        for (int j = 0; j < 4; ++j) {
+                            float2 f;
+                            if constexpr (std::is_same_v<T, __half>) f = unpack_f16(r[j]);
+                            else f = make_float2(__uint_as_float(r[j] << 16), __uint_as_float(r[j] & 0xffff0000u));
+                            gs[0][j] = gw[0][j] = pack_f16(f.x * by, f.y * by);
+                        }
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const uint32_t f = slab + (rb * 16 + g + (j & 1) * 8) * 144 + (kt * 16 + (j >> 1) * 8 + col) * 4;
+                            split_f16(__uint_as_float(lds32(f)), __uint_as_float(lds32(f + 4)), by, gs[0][j], gs[1][j]);
+                            gw[0][j] = gs[0][j], gw[1][j] = gs[1][j];
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < (EXACT ? 1 : 2); ++i)
+                        scale_f16(gs[i], __float2half2_rn(sm.factor[0][at])), scale_f16(gw[i], __float2half2_rn(sm.factor[3][at]));
                 }
 #pragma unroll
-                for (int i = 0; i < 2; ++i) load_a_t<64>(aw[i], w[i], kt * 16, rb * 2, lane), load_a_t<64>(az[i], z[i], kt * 16, rb * 2, lane);
+                for (int i = 0; i < 2; ++i) {
+                    load_a_t(aw[i], w + i * DR_PIECE, kt * 16, rb, o);
+                    load_a_t(zs[i], z + i * DR_PIECE, kt * 16, rb, o);
+                }
                 if (ch == 0) {  // dv = beta z
-                    T* const to = (T*)p.dv + (c.row * p.sh.heads + h) * p.sh.value_dim;
+                    T* const to = (T*)p.dv + (c.row * sh.heads + h) * sh.value_dim;
+                    const float back = sm.own[3][at];
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         const uint32_t r = token + (j & 1) * 8;
-                        const float b = sm.gates[2][r];
+                        const float b = sm.gates.beta[r] * back;
+                        const float2 hi = unpack_f16(zs[0][j]), lo = unpack_f16(zs[1][j]);
                         if (r < c.rows)
-                            dr_store_pair(to + (uint64_t)r * p.sh.heads * p.sh.value_dim, v0 + kt * 16 + (j >> 1) * 8 + col, p.sh.value_dim,
-                                          p.pairs_v, b * (bf16_low(az[0][j]) + bf16_low(az[1][j])),
-                                          b * (bf16_high(az[0][j]) + bf16_high(az[1][j])));
+                            dr_store_pair(to + (uint64_t)r * sh.heads * sh.value_dim, at * 16 + (j >> 1) * 8 + col, sh.value_dim, p.pairs_v,
+                                          b * (hi.x + lo.x), b * (hi.y + lo.y));
                     }
+                }
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) zw[i][j] = zs[i][j];
+                    scale_f16(zs[i], __float2half2_rn(sm.factor[1][at])), scale_f16(zw[i], __float2half2_rn(sm.factor[4][at]));
+                    scale_f16(aw[i], __float2half2_rn(sm.factor[2][at]));
                 }
 #pragma unroll
                 for (int j = 0; j < NP; ++j) {
+                    const int first = ch * (DK / 2) + j * 16, block = first / 64 * DR_PIECE, jj = first % 64 / 16;
                     uint32_t b[4];
-                    const int piece = (ch * NP + j) * 2;
-                    load_b_t<DK>(b, s[0], kt * 16, piece, lane);
-                    if (p.go.at) {
-#pragma unroll
-                        for (int i = 0; i < PLANES; ++i) mma_bf16(dq[2 * j], ag[i], b[0], b[1]), mma_bf16(dq[2 * j + 1], ag[i], b[2], b[3]);
+                    load_b_t(b, s + block, kt * 16, jj, o);
+                    if (p.out) {
+                        mma_f16_2(dq[2 * j], dq[2 * j + 1], gs[0], b);
+                        if constexpr (!EXACT) mma_f16_2(dq[2 * j], dq[2 * j + 1], gs[1], b);
                     }
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) mma_bf16(er[2 * j], az[i], b[0], b[1]), mma_bf16(er[2 * j + 1], az[i], b[2], b[3]);
-                    load_b_t<DK>(b, s[1], kt * 16, piece, lane);
-                    if (p.go.at) mma_bf16(dq[2 * j], ag[0], b[0], b[1]), mma_bf16(dq[2 * j + 1], ag[0], b[2], b[3]);
-                    mma_bf16(er[2 * j], az[0], b[0], b[1]), mma_bf16(er[2 * j + 1], az[0], b[2], b[3]);
-                    load_b_t<DK>(b, x[0], kt * 16, piece, lane);
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) mma_bf16(wr[2 * j], aw[i], b[0], b[1]), mma_bf16(wr[2 * j + 1], aw[i], b[2], b[3]);
-                    load_b_t<DK>(b, x[1], kt * 16, piece, lane);
-                    mma_bf16(wr[2 * j], aw[0], b[0], b[1]), mma_bf16(wr[2 * j + 1], aw[0], b[2], b[3]);
+                    mma_f16_2(er[2 * j], er[2 * j + 1], zs[0], b);
+                    mma_f16_2(er[2 * j], er[2 * j + 1], zs[1], b);
+                    load_b_t(b, s + NB * DR_PIECE + block, kt * 16, jj, o);
+                    if (p.out) mma_f16_2(dq[2 * j], dq[2 * j + 1], gs[0], b);
+                    mma_f16_2(er[2 * j], er[2 * j + 1], zs[0], b);
+                    load_b_t(b, x + block, kt * 16, jj, o);
+                    mma_f16_2(wr[2 * j], wr[2 * j + 1], aw[0], b);
+                    mma_f16_2(wr[2 * j], wr[2 * j + 1], aw[1], b);
+                    load_b_t(b, x + NB * DR_PIECE + block, kt * 16, jj, o);
+                    mma_f16_2(wr[2 * j], wr[2 * j + 1], aw[0], b);
                 }
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {  // 32 of the other tokens
+                for (int j = 0; j < 2; ++j) {  // 32 of the other tokens, if there are earlier ones among them
+                    if (ch * 2 + j > rb) break;
                     uint32_t b[4];
-                    load_b_t<64>(b, w[0], kt * 16, (ch * 2 + j) * 2, lane);
-                    if (p.go.at) {
-#pragma unroll
-                        for (int i = 0; i < PLANES; ++i) mma_bf16(a[2 * j], ag[i], b[0], b[1]), mma_bf16(a[2 * j + 1], ag[i], b[2], b[3]);
+                    load_b_t(b, w, kt * 16, ch * 2 + j, o);
+                    if (p.out) {
+                        mma_f16_2(a[2 * j], a[2 * j + 1], gw[0], b);
+                        if constexpr (!EXACT) mma_f16_2(a[2 * j], a[2 * j + 1], gw[1], b);
                     }
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) mma_bf16(n[2 * j], az[i], b[0], b[1]), mma_bf16(n[2 * j + 1], az[i], b[2], b[3]);
-                    load_b_t<64>(b, w[1], kt * 16, (ch * 2 + j) * 2, lane);
-                    if (p.go.at) mma_bf16(a[2 * j], ag[0], b[0], b[1]), mma_bf16(a[2 * j + 1], ag[0], b[2], b[3]);
-                    mma_bf16(n[2 * j], az[0], b[0], b[1]), mma_bf16(n[2 * j + 1], az[0], b[2], b[3]);
+                    mma_f16_2(n[2 * j], n[2 * j + 1], zw[0], b);
+                    mma_f16_2(n[2 * j], n[2 * j + 1], zw[1], b);
+                    load_b_t(b, w + DR_PIECE, kt * 16, ch * 2 + j, o);
+                    if (p.out) mma_f16_2(a[2 * j], a[2 * j + 1], gw[0], b);
+                    mma_f16_2(n[2 * j], n[2 * j + 1], zw[0], b);
                 }
-            }
-            // <S0, X> and w.z
-            for (int i = t; i < 64 * DK / 2; i += DR_GRAD_THREADS) {
-                const uint32_t s0 = ((const uint32_t*)sm.s[0])[i], s1 = ((const uint32_t*)sm.s[1])[i],
-                               x0 = ((const uint32_t*)sm.x[0])[i], x1 = ((const uint32_t*)sm.x[1])[i];
-                sx = fmaf(bf16_low(s0) + bf16_low(s1), bf16_low(x0) + bf16_low(x1), sx);
-                sx = fmaf(bf16_high(s0) + bf16_high(s1), bf16_high(x0) + bf16_high(x1), sx);
-            }
-            {
-                const int j = (t & 31) * 2;  // two tokens, 8 of the value dimensions
+                // <S0, X>
+                const float both = sm.own[0][at] * sm.own[1][at];
+                float sum = 0.0f;
+#pragma unroll
+                for (int i = 0; i < NB * 16 * 32 / DR_GRAD_THREADS; ++i) {
+                    const uint32_t word = i * DR_GRAD_THREADS + t, off = word / 512 * DR_PIECE + kt * 2048 + word % 512 * 4;
+                    const float2 s0 = unpack_f16(lds32(s + off)), s1 = unpack_f16(lds32(s + NB * DR_PIECE + off)),
+                                 x0 = unpack_f16(lds32(x + off)), x1 = unpack_f16(lds32(x + NB * DR_PIECE + off));
+                    sum = fmaf(s0.x + s1.x, x0.x + x1.x, sum);
+                    sum = fmaf(s0.y + s1.y, x0.y + x1.y, sum);
+                }
+                sx = fmaf(sum, both, sx);
+                // w.z of two tokens a lane, 2 of the value dimensions a warp
+                const float wz = sm.own[2][at] * sm.own[3][at];
                 float d0 = 0.0f, d1 = 0.0f;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const int r = warp * 8 + i;
-                    const uint32_t w0 = tile_word<64>(w[0], r, j), w1 = tile_word<64>(w[1], r, j), z0 = tile_word<64>(z[0], r, j),
-                                   z1 = tile_word<64>(z[1], r, j);
-                    d0 = fmaf(bf16_low(w0) + bf16_low(w1), bf16_low(z0) + bf16_low(z1), d0);
-                    d1 = fmaf(bf16_high(w0) + bf16_high(w1), bf16_high(z0) + bf16_high(z1), d1);
+                for (int i = 0; i < 2; ++i) {
+                    const uint32_t off = block_at(kt * 16 + warp * 2 + i, lane * 2);
+                    const float2 w0 = unpack_f16(lds32(w + off)), w1 = unpack_f16(lds32(w + DR_PIECE + off)), z0 = unpack_f16(lds32(z + off)),
+                                 z1 = unpack_f16(lds32(z + DR_PIECE + off));
+                    d0 = fmaf(w0.x + w1.x, z0.x + z1.x, d0);
+                    d1 = fmaf(w0.y + w1.y, z0.y + z1.y, d1);
                 }
-                // warps 2 i and 2 i + 1 take turns with row i of the table
-                if (v0 == 0 && (warp & 1) == 0) sm.dbeta[warp >> 1][j] = 0.0f, sm.dbeta[warp >> 1][j + 1] = 0.0f;
-                __syncthreads();
-                if ((warp & 1) == 0) sm.dbeta[warp >> 1][j] += d0, sm.dbeta[warp >> 1][j + 1] += d1;
-                __syncthreads();
-                if ((warp & 1) == 1) sm.dbeta[warp >> 1][j] += d0, sm.dbeta[warp >> 1][j + 1] += d1;
+                db0 = fmaf(d0, wz, db0), db1 = fmaf(d1, wz, db1);
             }
         }
-        // scale D dA and D dN as operands: dA_ij = beta_j a_ij, dN_ij = -beta_i beta_j n_ij
+        // scale D dA and D dN: dA_ij = beta_j a_ij, dN_ij = -beta_i beta_j n_ij
+        float most_a = 0.0f, most_n = 0.0f;
+        {
+            const float back_a = sm.back[3] * sh.scale, back_n = -sm.back[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int m = 0; m < 4; ++m) {
+                    const int i = token + (m >> 1) * 8, cc = ch * 32 + j * 8 + col + (m & 1);
+                    const float d = cc <= i ? expf((sm.gates.total[i] - sm.gates.total[cc]) + (sm.gates.rest[i] - sm.gates.rest[cc])) * sm.gates.beta[cc] : 0.0f;
+                    a[j][m] = cc <= i ? a[j][m] * back_a * d : 0.0f;
+                    n[j][m] = cc < i ? n[j][m] * back_n * d * sm.gates.beta[i] : 0.0f;
+                    most_a = fmaxf(most_a, fabsf(a[j][m])), most_n = fmaxf(most_n, fabsf(n[j][m]));
+                }
+        }
+        most_a = warp_max(most_a), most_n = warp_max(most_n);
+        if (lane == 0) sm.most[0][warp] = most_a, sm.most[1][warp] = most_n;
+        if ((warp & 1) == 0) *(float2*)&sm.dbeta[warp >> 1][lane * 2] = make_float2(db0, db1);
+        __syncthreads();
+        if ((warp & 1) == 1) sm.dbeta[warp >> 1][lane * 2] += db0, sm.dbeta[warp >> 1][lane * 2 + 1] += db1;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) most_a = fmaxf(most_a, sm.most[0][i]), most_n = fmaxf(most_n, sm.most[1][i]);
+        const Scale sa = scale_for(most_a), sn = scale_for(most_n);
 #pragma unroll
         for (int j = 0; j < 4; ++j)
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
-                const int i = token + half * 8, c0 = ch * 32 + j * 8 + col;
-                float va[2], vn[2];
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const int cc = c0 + e;
-                    const float d = cc <= i ? expf((float)(sm.total[i] - sm.total[cc])) * sm.gates[2][cc] : 0.0f;
-                    va[e] = cc <= i ? p.sh.scale * d * a[j][half * 2 + e] : 0.0f;
-                    vn[e] = cc < i ? -d * sm.gates[2][i] * n[j][half * 2 + e] : 0.0f;
-                }
                 uint32_t hi, lo;
-                const uint32_t off = tile_at<64>(0, i, c0 >> 3) + (c0 & 7) * 2;
-                split_bf16(va[0], va[1], hi, lo);
-                *(uint32_t*)((char*)sm.da[0] + off) = hi, *(uint32_t*)((char*)sm.da[1] + off) = lo;
-                split_bf16(vn[0], vn[1], hi, lo);
-                *(uint32_t*)((char*)sm.dn[0] + off) = hi, *(uint32_t*)((char*)sm.dn[1] + off) = lo;
+                const uint32_t off = block_at(token + half * 8, ch * 32 + j * 8 + col);
+                split_f16(a[j][half * 2], a[j][half * 2 + 1], sa.by, hi, lo);
+                sts32(da + off, hi), sts32(da + DR_BLOCK + off, lo);
+                split_f16(n[j][half * 2], n[j][half * 2 + 1], sn.by, hi, lo);
+                sts32(dn + off, hi), sts32(dn + DR_BLOCK + off, lo);
             }
-        // row factors of the products with the states; k.(e u X) is needed by itself
+        // row factors of the products with the states, into the domains of the products that follow; k.(e u X) is needed by
+        // itself
+        const float back_k = sm.gates.back_k, back_q = sm.gates.back_q;
+        const float by_k = __frcp_rn(back_k), into_q = sa.by * by_k, into_n = sn.by * by_k;
         float carry[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
             const int i = token + half * 8;
-            const float g0 = sm.gates[0][i], e = sm.gates[1][i] * sm.gates[2][i], b = sm.gates[2][i];
+            const float g0 = sm.gates.g[i], b = sm.gates.beta[i];
+            const float fq = g0 * sh.scale * sm.back[0] * into_q, fe = -g0 * b * sm.back[1] * into_n, fw = sm.gates.e[i] * b * sm.back[2];
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
-                const int cc = ch * (DK / 2) + j * 8 + col;
-                uint32_t kw = tile_word<DK>(k[0], i, cc);
-                float k0 = bf16_low(kw), k1 = bf16_high(kw);
-                if constexpr (PLANES == 2) kw = tile_word<DK>(k[PLANES - 1], i, cc), k0 += bf16_low(kw), k1 += bf16_high(kw);
+                const int first = ch * (DK / 2) + j * 8 + col;
+                const uint32_t off = first / 64 * DR_BLOCK + block_at(i, first % 64);
+                float2 kv = unpack_f16(lds32(k + off));
+                if constexpr (PLANES == 2) {
+                    const float2 lo = unpack_f16(lds32(k + NB * DR_BLOCK + off));
+                    kv.x += lo.x, kv.y += lo.y;
+                }
 #pragma unroll
-                for (int m = half * 2; m < half * 2 + 2; ++m) dq[j][m] *= g0 * p.sh.scale, er[j][m] *= -g0 * b, wr[j][m] *= e;
-                carry[half] = fmaf(k0, wr[j][half * 2], fmaf(k1, wr[j][half * 2 + 1], carry[half]));
+                for (int m = half * 2; m < half * 2 + 2; ++m) dq[j][m] *= fq, er[j][m] *= fe, wr[j][m] *= fw;
+                carry[half] = fmaf(kv.x, wr[j][half * 2], fmaf(kv.y, wr[j][half * 2 + 1], carry[half]));
+                wr[j][half * 2] *= into_n, wr[j][half * 2 + 1] *= into_n;
             }
+            carry[half] *= back_k;
         }
         __syncthreads();
+        // rows of dA and dN against the keys before; then columns against the later ones: dN^T K, and in dA^T Q's domain that
 #pragma unroll
-        for (int kt = 0; kt < 4; ++kt) {
+        for (int part = 0; part < 3; ++part) {
+            if (part == 2) {
+                const float turn = sa.by * __frcp_rn(back_q) * sn.back * back_k;
 #pragma unroll
-            for (int side = 0; side < 2; ++side) {  // rows of dA, dN against earlier tokens; columns against later ones
-                if (side == 0 ? kt > rb : kt < rb) continue;
+                for (int j = 0; j < NT; ++j)
+#pragma unroll
+                    for (int m = 0; m < 4; ++m) wr[j][m] *= turn;
+            }
+#pragma unroll
+            for (int kt = 0; kt < 4; ++kt) {
+                if (part == 0 ? kt > rb : kt < rb) continue;
                 uint32_t fa[2][4], fn[2][4];
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    if (side == 0) load_a<64>(fa[i], da[i], rb * 16, kt * 2, lane), load_a<64>(fn[i], dn[i], rb * 16, kt * 2, lane);
-                    else load_a_t<64>(fa[i], da[i], kt * 16, rb * 2, lane), load_a_t<64>(fn[i], dn[i], kt * 16, rb * 2, lane);
+                    if (part == 0) load_a(fa[i], da + i * DR_BLOCK, rb * 16, kt, o), load_a(fn[i], dn + i * DR_BLOCK, rb * 16, kt, o);
+                    if (part == 1) load_a_t(fn[i], dn + i * DR_BLOCK, kt * 16, rb, o);
+                    if (part == 2) load_a_t(fa[i], da + i * DR_BLOCK, kt * 16, rb, o);
                 }
 #pragma unroll
                 for (int j = 0; j < NP; ++j) {
-                    const int piece = (ch * NP + j) * 2;
-                    uint32_t b[4];
+                    const int first = ch * (DK / 2) + j * 16, block = first / 64 * DR_BLOCK, jj = first % 64 / 16;
 #pragma unroll
                     for (int i = 0; i < PLANES; ++i) {
-                        load_b_t<DK>(b, k[i], kt * 16, piece, lane);
+                        uint32_t b[4];
+                        load_b_t(b, (part == 2 ? q : k) + i * NB * DR_BLOCK + block, kt * 16, jj, o);
 #pragma unroll
                         for (int l = 0; l < 2 - i; ++l) {
-                            if (side == 0) {
-                                mma_bf16(dq[2 * j], fa[l], b[0], b[1]), mma_bf16(dq[2 * j + 1], fa[l], b[2], b[3]);
-                                mma_bf16(er[2 * j], fn[l], b[0], b[1]), mma_bf16(er[2 * j + 1], fn[l], b[2], b[3]);
-                            } else {
-                                mma_bf16(wr[2 * j], fn[l], b[0], b[1]), mma_bf16(wr[2 * j + 1], fn[l], b[2], b[3]);
-                            }
-                        }
-                        if (side == 1) {
-                            load_b_t<DK>(b, q[i], kt * 16, piece, lane);
-#pragma unroll
-                            for (int l = 0; l < 2 - i; ++l) mma_bf16(wr[2 * j], fa[l], b[0], b[1]), mma_bf16(wr[2 * j + 1], fa[l], b[2], b[3]);
+                            if (part == 0) mma_f16_2(dq[2 * j], dq[2 * j + 1], fa[l], b), mma_f16_2(er[2 * j], er[2 * j + 1], fn[l], b);
+                            if (part == 1) mma_f16_2(wr[2 * j], wr[2 * j + 1], fn[l], b);
+                            if (part == 2) mma_f16_2(wr[2 * j], wr[2 * j + 1], fa[l], b);
                         }
                     }
                 }
             }
         }
         // q.dq + k.(erase - write)
+        const float out_q = sa.back * back_k, out_e = sn.back * back_k, out_w = sa.back * back_q;
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
             const int i = token + half * 8;
             float dot = 0.0f;
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
-                const int cc = ch * (DK / 2) + j * 8 + col;
+                const int first = ch * (DK / 2) + j * 8 + col;
+                const uint32_t off = first / 64 * DR_BLOCK + block_at(i, first % 64);
                 float kv[2] = {0, 0}, qv[2] = {0, 0};
 #pragma unroll
                 for (int l = 0; l < PLANES; ++l) {
-                    const uint32_t kw = tile_word<DK>(k[l], i, cc), qw = tile_word<DK>(q[l], i, cc);
-                    kv[0] += bf16_low(kw), kv[1] += bf16_high(kw), qv[0] += bf16_low(qw), qv[1] += bf16_high(qw);
+                    const float2 kw = unpack_f16(lds32(k + l * NB * DR_BLOCK + off)), qw = unpack_f16(lds32(q + l * NB * DR_BLOCK + off));
+                    kv[0] += kw.x, kv[1] += kw.y, qv[0] += qw.x, qv[1] += qw.y;
                 }
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                     const int m = half * 2 + e;
-                    dot = fmaf(qv[e], dq[j][m], fmaf(kv[e], er[j][m] - wr[j][m], dot));
-                    all_q[j][m] += dq[j][m], all_k[j][m] += er[j][m] + wr[j][m];
+                    const float fq = dq[j][m] * out_q, fe = er[j][m] * out_e, fw = wr[j][m] * out_w;
+                    dot = fmaf(qv[e] * back_q, fq, fmaf(kv[e] * back_k, fe - fw, dot));
+                    dq[j][m] = fq, er[j][m] = fe + fw;
+                    if constexpr (SHARED) all_q[j][m] += fq, all_k[j][m] += fe + fw;
                 }
             }
 #pragma unroll
-            for (int o = 1; o < 4; o <<= 1) {
-                dot += __shfl_xor_sync(0xffffffffu, dot, o);
-                carry[half] += __shfl_xor_sync(0xffffffffu, carry[half], o);
+            for (int i2 = 1; i2 < 4; i2 <<= 1) {
+                dot += __shfl_xor_sync(0xffffffffu, dot, i2);
+                carry[half] += __shfl_xor_sync(0xffffffffu, carry[half], i2);
             }
             if ((lane & 3) == 0) sm.dot[ch][i] = dot, sm.carry[ch][i] = carry[half];
         }
         sx = warp_reduce<OpSum>(sx);
         if (lane == 0) sm.sx[warp] = sx;
+        if (!SHARED || h + 1 == h0 + group) {
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const uint32_t i = token + half * 8;
+                if (i >= c.rows) continue;
+                const uint64_t to = ((c.row + i) * sh.key_heads + hk) * sh.key_dim;
+#pragma unroll
+                for (int j = 0; j < NT; ++j) {
+                    const uint32_t cc = ch * (DK / 2) + j * 8 + col;
+                    const float* const fq = SHARED ? all_q[SHARED ? j : 0] : dq[j];
+                    const float* const fk = SHARED ? all_k[SHARED ? j : 0] : er[j];
+                    dr_store_pair((T*)p.dq + to, cc, sh.key_dim, p.pairs_k, fq[half * 2], fq[half * 2 + 1]);
+                    dr_store_pair((T*)p.dk + to, cc, sh.key_dim, p.pairs_k, fk[half * 2], fk[half * 2 + 1]);
+                }
+            }
+        }
         __syncthreads();
         if (warp == 0) {
             double d[2], extra = 0.0;
@@ -1029,39 +1332,29 @@ dr_gradient_kernel(const __grid_constant__ DrGradient p) {
                 d[j] = (double)sm.dot[0][r] + sm.dot[1][r];
                 extra += (double)sm.carry[0][r] + sm.carry[1][r];
             }
-            if (lane < 8) extra += (double)sm.sx[lane] * sm.gates[0][DR_CHUNK - 1];
+            if (lane < 8) extra += (double)sm.sx[lane] * sm.gates.g[DR_CHUNK - 1];
 #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) extra += __shfl_xor_sync(0xffffffffu, extra, o);
+            for (int i = 16; i > 0; i >>= 1) extra += __shfl_xor_sync(0xffffffffu, extra, i);
             double sum = d[0] + d[1];  // from the lane's rows to the end
 #pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const double down = __shfl_down_sync(0xffffffffu, sum, o);
-                if (lane + o < 32) sum += down;
+            for (int i = 1; i < 32; i <<= 1) {
+                const double down = __shfl_down_sync(0xffffffffu, sum, i);
+                if (lane + i < 32) sum += down;
             }
             const double v[2] = {sum + extra, sum - d[0] + extra};
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 const uint32_t r = lane * 2 + j;
                 if (r < c.rows) {
-                    const uint64_t to = (c.row + r) * p.sh.heads + h;
+                    const uint64_t to = (c.row + r) * sh.heads + h;
                     if (p.ddecay) p.ddecay[to] = (float)v[j];
                     p.dbeta[to] = (sm.dbeta[0][r] + sm.dbeta[1][r]) + (sm.dbeta[2][r] + sm.dbeta[3][r]);
                 }
             }
         }
+        if (SHARED) __syncthreads();  // the gates and scales may be replaced
     }
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-        const uint32_t i = token + half * 8;
-        if (i >= c.rows) continue;
-        const uint64_t to = ((c.row + i) * p.sh.key_heads + hk) * p.sh.key_dim;
-#pragma unroll
-        for (int j = 0; j < NT; ++j) {
-            const uint32_t cc = ch * (DK / 2) + j * 8 + col;
-            dr_store_pair((T*)p.dq + to, cc, p.sh.key_dim, p.pairs_k, all_q[j][half * 2], all_q[j][half * 2 + 1]);
-            dr_store_pair((T*)p.dk + to, cc, p.sh.key_dim, p.pairs_k, all_k[j][half * 2], all_k[j][half * 2 + 1]);
-        }
-    }
+    if (!ok) set_error(LCPP_ERR_LOOKBACK_TIMEOUT);
 }
 
 // Rows outside all sequences: zeros.
@@ -1193,61 +1486,42 @@ static DrShape dr_shape(const lcpp_delta_shape& sh) {
     return DrShape{sh.rows, sh.offsets ? 0 : sh.length, sh.offsets, (uint32_t)sh.num_sequences, sh.heads, sh.key_heads,
                    sh.key_dim, sh.value_dim, sh.scale};
 }
-static uint64_t dr_key_cols(const lcpp_delta_shape& sh) { return align_up(sh.key_dim, 16); }
 
 struct DrLayout {
-    uint64_t slots, state, value;  // chunks; elements of a plane
-    size_t inverse, read, gates, x, z, q, k, v, bytes;
-    uint64_t key_pitch, value_pitch;
-    bool packed;
-    DrLayout(const lcpp_delta_shape& sh, bool backward, bool pack) : packed(pack) {
-        slots = sh.rows / DR_CHUNK + sh.num_sequences;
-        state = sh.value_dim * dr_key_cols(sh), value = sh.value_dim * DR_CHUNK;
-        key_pitch = align_up(sh.key_dim, 8), value_pitch = align_up(sh.value_dim, 8);
+    uint64_t slots, units;
+    uint32_t planes, key_cols, rows;  // rows of an image
+    size_t keys, unit, x, back_x, z, back_z, back_out, bytes;
+    DrLayout(int dtype, const lcpp_delta_shape& sh, bool backward) {
+        slots = sh.rows / DR_CHUNK + sh.num_sequences, units = slots * sh.heads;
+        planes = dtype == LCPP_F32 ? 2 : 1, key_cols = sh.key_dim <= 64 ? 64 : 128, rows = (uint32_t)align_up(sh.value_dim, 32);
         size_t at = 0;
         auto take = [&](uint64_t n) {
             const size_t here = at;
             at += align_up(n, 256);
             return here;
         };
-        const uint64_t units = slots * sh.heads;
-        inverse = take(units * 2 * DR_TILE * 2), read = take(units * 2 * DR_TILE * 2), gates = take(units * 3 * DR_CHUNK * 4);
-        x = z = q = k = v = 0;
-        if (backward) x = take(units * 2 * state * 2), z = take(units * 2 * value * 2);
-        if (pack) {
-            q = take(slots * DR_CHUNK * sh.key_heads * key_pitch * 4), k = take(slots * DR_CHUNK * sh.key_heads * key_pitch * 4);
-            v = take(slots * DR_CHUNK * sh.heads * value_pitch * 4);  // dO in the backward pass
+        keys = take(slots * sh.key_heads * 2 * planes * (key_cols / 64) * DR_BLOCK), unit = take(units * DR_UNIT);
+        x = back_x = z = back_z = back_out = 0;
+        if (backward) {
+            x = take(units * states(nullptr, 0, 0).bytes()), back_x = take(units * 32);
+            z = take(units * kept(nullptr, 0, 0).bytes()), back_z = take(units * 32);
+            back_out = take(units * 32);
         }
         bytes = max(at, (size_t)256);
     }
-    DrPrepared prepared(void* temp) const {
-        char* const t = (char*)temp;
-        return DrPrepared{(__nv_bfloat16*)(t + inverse), (__nv_bfloat16*)(t + read), (float*)(t + gates)};
-    }
+    DrImage states(void* room, size_t at, size_t back) const { return DrImage{(uint8_t*)room + at, (float*)((char*)room + back), key_cols / 64, rows}; }
+    DrImage kept(void* room, size_t at, size_t back) const { return DrImage{(uint8_t*)room + at, (float*)((char*)room + back), 1, rows}; }
+    // What the forward call saves: S0 and w.
+    size_t saved_w() const { return align_up(units * states(nullptr, 0, 0).bytes(), 256); }
+    size_t saved_back() const { return saved_w() + align_up(units * kept(nullptr, 0, 0).bytes(), 256); }
+    size_t saved_bytes() const { return saved_back() + 2 * align_up(units * 32, 256); }
+    DrImage saved_states(void* saved) const { return states(saved, 0, saved_back()); }
+    DrImage saved_kept(void* saved) const { return kept(saved, saved_w(), saved_back() + align_up(units * 32, 256)); }
 };
 
-// Rows of bf16 that can be copied in pieces of 16 bytes.
-static bool dr_direct(const void* p, uint64_t stride, uint64_t rows, uint32_t dim) {
-    return (uintptr_t)p % 16 == 0 && dim % 8 == 0 && (rows <= 1 || stride % 8 == 0);
-}
-
-template <typename T>
-static lcpp_status dr_operand(const DrShape& sh, const DrLayout& l, const void* from, uint64_t stride, uint32_t heads, uint32_t dim,
-                              uint64_t pitch, void* room, DrOperand* to, cudaStream_t s) {
-    if (!from) {
-        *to = DrOperand{};
-        return LCPP_OK;
-    }
-    if (!l.packed) {
-        *to = DrOperand{(const __nv_bfloat16*)from, stride, 0, dim, dim, false};
-        return LCPP_OK;
-    }
-    const uint64_t plane = l.slots * DR_CHUNK * heads * pitch;
-    *to = DrOperand{(const __nv_bfloat16*)room, heads * pitch, plane, (uint32_t)pitch, (uint32_t)pitch, true};
-    ProfScope prof("dr_pack", s);
-    dr_pack_kernel<T><<<(unsigned)l.slots, 256, 0, s>>>(sh, (const T*)from, stride, heads, dim, (__nv_bfloat16*)room, plane, (uint32_t)pitch);
-    count_launch();
-    return check_launch();
+// Rows that are whole pieces of 16 bytes on 16 bytes.
+static bool dr_wide(const void* p, uint64_t stride, uint64_t rows, uint32_t dim, size_t element) {
+    return (uintptr_t)p % 16 == 0 && dim * element % 16 == 0 && (rows <= 1 || stride * element % 16 == 0);
 }
 
 // Allows KERNEL `smem` bytes of shared memory on the current device.
@@ -1260,34 +1534,41 @@ static bool dr_sized(size_t smem) {
     sized.fetch_or(bit, std::memory_order_relaxed);
     return true;
 }
-template <auto KERNEL, typename... A>
-static lcpp_status dr_launch(const char* name, uint64_t grid, unsigned threads, size_t smem, cudaStream_t s, const A&... args) {
+template <auto KERNEL, typename A>
+static lcpp_status dr_launch(const char* name, uint64_t grid, unsigned threads, size_t smem, cudaStream_t s, const A& args) {
     if (grid > 0x7fffffffull) return LCPP_ERR_INVALID_ARG;
     if (!dr_sized<KERNEL>(smem)) return check_launch();
     ProfScope prof(name, s);
-    KERNEL<<<(unsigned)grid, threads, smem, s>>>(args...);
+    KERNEL<<<(unsigned)grid, threads, smem, s>>>(args);
     count_launch();
     return check_launch();
 }
 
 // How many warps a CTA of the chain has, 16 value dimensions each: fewer where that spreads the states over more SMs.
-// Two planes of 128 key columns leave shared memory for 4 warps' values.
-static int dr_warps(const lcpp_delta_shape& sh, bool packed) {
+static int dr_warps(const lcpp_delta_shape& sh) {
     const uint64_t states = sh.num_sequences * sh.heads, sms = device_info().sms;
-    int warps = packed ? 4 : 8;
+    int warps = 8;
     while (warps > 2 && (warps * 8u >= sh.value_dim || states * ceil_div(sh.value_dim, warps * 16) * 2 <= sms)) warps /= 2;
     return warps;
 }
-
-template <typename T, typename F>
-static lcpp_status dr_dispatch(const lcpp_delta_shape& sh, bool packed, F&& f) {
-    auto planes = [&](auto dk) -> lcpp_status {
-        if constexpr (std::is_same_v<T, __nv_bfloat16>) {
-            if (!packed) return f(dk, std::integral_constant<int, 1>{});
-        }
-        return f(dk, std::integral_constant<int, 2>{});
+template <typename F>
+static lcpp_status dr_dispatch(const lcpp_delta_shape& sh, F&& f) {
+    return sh.key_dim <= 64 ? f(std::integral_constant<int, 64>{}) : f(std::integral_constant<int, 128>{});
+}
+template <typename T, int DK, bool BACKWARD>
+static lcpp_status dr_chain(const lcpp_delta_shape& sh, const DrChain& p, cudaStream_t s) {
+    auto chain = [&](auto warps) {
+        constexpr int WARPS = decltype(warps)::value;
+        const uint64_t grid = sh.num_sequences * sh.heads * ceil_div(sh.value_dim, WARPS * 16);
+        constexpr size_t smem = sizeof(DrChainSmem<T, DK, WARPS>);
+        static_assert(smem <= 227 * 1024, "shared memory of a CTA");
+        if constexpr (BACKWARD) return dr_launch<dr_backward_kernel<T, DK, WARPS>>("dr_backward", grid, WARPS * 32, smem, s, p);
+        else return dr_launch<dr_forward_kernel<T, DK, WARPS>>("dr_forward", grid, WARPS * 32, smem, s, p);
     };
-    return sh.key_dim <= 64 ? planes(std::integral_constant<int, 64>{}) : planes(std::integral_constant<int, 128>{});
+    const int warps = dr_warps(sh);
+    if (warps == 8) return chain(std::integral_constant<int, 8>{});
+    if (warps == 4) return chain(std::integral_constant<int, 4>{});
+    return chain(std::integral_constant<int, 2>{});
 }
 
 // Everything that a call reads, and its checks.
@@ -1328,9 +1609,11 @@ struct DrCall {
     bool apart(const Region& w, bool init_too = true) const {
         return w.apart(q(), k(), v(), decay(), beta(), offsets()) && (!init_too || w.apart(states(in.init)));
     }
-    bool direct() const {
-        return dtype == LCPP_BF16 && dr_direct(in.q, in.q_stride, sh.rows, sh.key_dim) &&
-               dr_direct(in.k, in.k_stride, sh.rows, sh.key_dim) && dr_direct(in.v, in.v_stride, sh.rows, sh.value_dim);
+    DrPrepare prepare(const DrShape& shape, const DrLayout& l, void* temp) const {
+        return DrPrepare{shape, in.q, in.k, in.q_stride, in.k_stride, in.decay, in.beta, in.decay_stride, in.beta_stride,
+                         sh.key_dim % 8 == 0 && dr_wide(in.q, in.q_stride, sh.rows, sh.key_dim, element()) &&
+                             dr_wide(in.k, in.k_stride, sh.rows, sh.key_dim, element()),
+                         (uint8_t*)temp + l.keys, (uint8_t*)temp + l.unit};
     }
 };
 
@@ -1346,17 +1629,12 @@ static lcpp_status dr_padding(const DrShape& sh, const DrFills& fills, cudaStrea
 
 using namespace lcpp;
 
-extern "C" size_t lcpp_delta_rule_temp_bytes(int dtype, const lcpp_delta_shape* shape, int backward, int aligned) {
-    if (dr_check(dtype, shape) != LCPP_OK) return 0;
-    const bool pack = dtype != LCPP_BF16 || !aligned || shape->key_dim % 8 || shape->value_dim % 8;
-    return DrLayout(*shape, backward != 0, pack).bytes;
+extern "C" size_t lcpp_delta_rule_temp_bytes(int dtype, const lcpp_delta_shape* shape, int backward) {
+    return dr_check(dtype, shape) == LCPP_OK ? DrLayout(dtype, *shape, backward != 0).bytes : 0;
 }
 
 extern "C" size_t lcpp_delta_rule_saved_bytes(const lcpp_delta_shape* shape) {
-    if (dr_check(LCPP_F32, shape) != LCPP_OK) return 0;
-    const DrLayout l(*shape, false, false);
-    const uint64_t units = l.slots * shape->heads;
-    return align_up(units * 2 * l.state * 2, 256) + align_up(units * 2 * l.value * 2, 256);
+    return dr_check(LCPP_F32, shape) == LCPP_OK ? DrLayout(LCPP_F32, *shape, false).saved_bytes() : 0;
 }
 
 extern "C" lcpp_status lcpp_delta_rule_forward(int dtype, const lcpp_delta_shape* shape, const lcpp_delta_inputs* inputs, void* out,
@@ -1370,8 +1648,7 @@ extern "C" lcpp_status lcpp_delta_rule_forward(int dtype, const lcpp_delta_shape
     if (!elements_aligned(dtype, out) || !elements_aligned(LCPP_F32, last) || (uintptr_t)saved % 16 ||
         (shape->rows && (!out || !DrCall::stride_ok(out_stride, shape->rows, c.values()))))
         return LCPP_ERR_INVALID_ARG;
-    const bool packed = !c.direct();
-    const DrLayout l(*shape, false, packed);
+    const DrLayout l(dtype, *shape, false);
     if (!temp || temp_bytes < l.bytes) return LCPP_ERR_TEMP_TOO_SMALL;
     if ((uintptr_t)temp % 16) return LCPP_ERR_INVALID_ARG;
     const Region ro = c.matrix(out, out_stride, c.values(), c.element()), rl = c.states(last), rt(temp, l.bytes),
@@ -1387,38 +1664,19 @@ extern "C" lcpp_status lcpp_delta_rule_forward(int dtype, const lcpp_delta_shape
     if (status != LCPP_OK || !shape->num_sequences) return status;
     return dispatch_float(dtype, [&](auto type) -> lcpp_status {
         using T = decltype(type);
+        const DrPrepare pr = c.prepare(sh, l, temp);
         DrChain p{};
-        p.sh = sh, p.prepared = l.prepared(temp), p.from = inputs->init, p.to = last, p.out = out, p.out_stride = out_stride;
-        p.key_cols = (uint32_t)dr_key_cols(*shape);
-        char* const t = (char*)temp;
-        lcpp_status status = dr_operand<T>(sh, l, inputs->q, inputs->q_stride, sh.key_heads, sh.key_dim, l.key_pitch, t + l.q, &p.q, s);
-        if (status == LCPP_OK) status = dr_operand<T>(sh, l, inputs->k, inputs->k_stride, sh.key_heads, sh.key_dim, l.key_pitch, t + l.k, &p.k, s);
-        if (status == LCPP_OK) status = dr_operand<T>(sh, l, inputs->v, inputs->v_stride, sh.heads, sh.value_dim, l.value_pitch, t + l.v, &p.v, s);
-        if (status != LCPP_OK) return status;
-        if (saved) {
-            p.states = DrPlanes{(__nv_bfloat16*)saved, l.state};
-            p.values = DrPlanes{(__nv_bfloat16*)((char*)saved + align_up(l.slots * sh.heads * 2 * l.state * 2, 256)), l.value};
-        }
-        return dr_dispatch<T>(*shape, packed, [&](auto dk, auto planes) -> lcpp_status {
-            constexpr int DK = decltype(dk)::value, PLANES = decltype(planes)::value;
+        p.sh = sh, p.keys = pr.keys, p.units = pr.units, p.values = inputs->v, p.value_stride = inputs->v_stride;
+        p.wide = dr_wide(inputs->v, inputs->v_stride, sh.rows, sh.value_dim, sizeof(T));
+        p.from = inputs->init, p.to = last, p.out = out, p.out_stride = out_stride;
+        if (saved) p.states = l.saved_states(saved), p.kept = l.saved_kept(saved);
+        return dr_dispatch(*shape, [&](auto dk) -> lcpp_status {
+            constexpr int DK = decltype(dk)::value, PLANES = sizeof(T) == 4 ? 2 : 1;
             lcpp_status status = LCPP_OK;
             if (sh.rows)
-                status = dr_launch<dr_prepare_kernel<DK, PLANES, false>>("dr_prepare", l.slots * sh.key_heads, DR_PREPARE_THREADS,
-                                                                         sizeof(DrPrepareSmem<DK, PLANES>), s, sh, p.q, p.k, inputs->decay,
-                                                                         inputs->decay_stride, inputs->beta, inputs->beta_stride, p.prepared);
-            if (status != LCPP_OK) return status;
-            auto chain = [&](auto warps) {
-                constexpr int WARPS = decltype(warps)::value;
-                const uint64_t grid = (uint64_t)sh.sequences * sh.heads * ceil_div(sh.value_dim, WARPS * 16);
-                return dr_launch<dr_forward_kernel<T, DK, PLANES, WARPS>>("dr_forward", grid, WARPS * 32,
-                                                                          sizeof(DrChainSmem<DK, PLANES, WARPS>), s, p);
-            };
-            const int warps = dr_warps(*shape, packed);
-            if constexpr (PLANES == 1) {
-                if (warps == 8) return chain(std::integral_constant<int, 8>{});
-            }
-            if (warps == 4) return chain(std::integral_constant<int, 4>{});
-            return chain(std::integral_constant<int, 2>{});
+                status = dr_launch<dr_prepare_kernel<T, DK, false>>("dr_prepare", l.slots * sh.key_heads, DR_PREPARE_THREADS,
+                                                                    sizeof(DrPrepareSmem<DK, PLANES>), s, pr);
+            return status != LCPP_OK ? status : dr_chain<T, DK, false>(*shape, p, s);
         });
     });
 }
@@ -1437,8 +1695,7 @@ extern "C" lcpp_status lcpp_delta_rule_backward(int dtype, const lcpp_delta_shap
     if (shape->rows && (!saved || !grads->q || !grads->k || !grads->v || !grads->beta ||
                         (grads->out && !DrCall::stride_ok(grads->out_stride, shape->rows, c.values()))))
         return LCPP_ERR_INVALID_ARG;
-    const bool packed = !c.direct() || (grads->out && !dr_direct(grads->out, grads->out_stride, shape->rows, shape->value_dim));
-    const DrLayout l(*shape, true, packed);
+    const DrLayout l(dtype, *shape, true);
     if (!temp || temp_bytes < l.bytes) return LCPP_ERR_TEMP_TOO_SMALL;
     if ((uintptr_t)temp % 16) return LCPP_ERR_INVALID_ARG;
     const uint64_t e = c.element(), rows = shape->rows;
@@ -1462,48 +1719,32 @@ extern "C" lcpp_status lcpp_delta_rule_backward(int dtype, const lcpp_delta_shap
     if (status != LCPP_OK || !shape->num_sequences) return status;
     return dispatch_float(dtype, [&](auto type) -> lcpp_status {
         using T = decltype(type);
+        const DrPrepare pr = c.prepare(sh, l, temp);
         DrChain p{};
-        p.sh = sh, p.prepared = l.prepared(temp), p.from = grads->last, p.to = grads->init;
-        p.key_cols = (uint32_t)dr_key_cols(*shape);
-        char* const t = (char*)temp;
-        p.states = DrPlanes{(__nv_bfloat16*)(t + l.x), l.state}, p.values = DrPlanes{(__nv_bfloat16*)(t + l.z), l.value};
-        lcpp_status status = dr_operand<T>(sh, l, inputs->q, inputs->q_stride, sh.key_heads, sh.key_dim, l.key_pitch, t + l.q, &p.q, s);
-        if (status == LCPP_OK) status = dr_operand<T>(sh, l, inputs->k, inputs->k_stride, sh.key_heads, sh.key_dim, l.key_pitch, t + l.k, &p.k, s);
-        if (status == LCPP_OK) status = dr_operand<T>(sh, l, grads->out, grads->out_stride, sh.heads, sh.value_dim, l.value_pitch, t + l.v, &p.v, s);
-        if (status != LCPP_OK) return status;
+        p.sh = sh, p.keys = pr.keys, p.units = pr.units, p.values = grads->out, p.value_stride = grads->out_stride;
+        p.wide = dr_wide(grads->out, grads->out_stride, sh.rows, sh.value_dim, sizeof(T));
+        p.from = grads->last, p.to = grads->init;
+        p.states = l.states(temp, l.x, l.back_x), p.kept = l.kept(temp, l.z, l.back_z);
+        p.back_values = (float*)((char*)temp + l.back_out);
         DrGradient gr{};
-        gr.sh = sh, gr.q = p.q, gr.k = p.k, gr.go = p.v, gr.prepared = p.prepared, gr.decay = inputs->decay, gr.decay_stride = inputs->decay_stride;
-        gr.s = DrPlanes{(__nv_bfloat16*)saved, l.state};
-        gr.w = DrPlanes{(__nv_bfloat16*)((char*)saved + align_up(l.slots * sh.heads * 2 * l.state * 2, 256)), l.value};
-        gr.x = p.states, gr.z = p.values, gr.key_cols = p.key_cols;
+        gr.sh = sh, gr.keys = pr.keys, gr.units = pr.units, gr.out = p.values, gr.out_stride = p.value_stride, gr.wide = p.wide;
+        gr.s = l.saved_states((void*)saved), gr.w = l.saved_kept((void*)saved), gr.x = p.states, gr.z = p.kept, gr.back_out = p.back_values;
         gr.dq = grads->q, gr.dk = grads->k, gr.dv = grads->v, gr.ddecay = grads->decay, gr.dbeta = grads->beta;
         gr.pairs_k = sh.key_dim % 2 == 0 && ((uintptr_t)grads->q | (uintptr_t)grads->k) % (2 * sizeof(T)) == 0;
         gr.pairs_v = sh.value_dim % 2 == 0 && (uintptr_t)grads->v % (2 * sizeof(T)) == 0;
-        return dr_dispatch<T>(*shape, packed, [&](auto dk, auto planes) -> lcpp_status {
-            constexpr int DK = decltype(dk)::value, PLANES = decltype(planes)::value;
+        return dr_dispatch(*shape, [&](auto dk) -> lcpp_status {
+            constexpr int DK = decltype(dk)::value, PLANES = sizeof(T) == 4 ? 2 : 1;
+            constexpr size_t smem = sizeof(DrGradientSmem<T, DK>);
+            static_assert(smem <= 227 * 1024, "shared memory of a CTA");
             lcpp_status status = LCPP_OK;
             if (sh.rows)
-                status = dr_launch<dr_prepare_kernel<DK, PLANES, true>>("dr_prepare", l.slots * sh.key_heads, DR_PREPARE_THREADS,
-                                                                        sizeof(DrPrepareSmem<DK, PLANES>), s, sh, p.q, p.k, inputs->decay,
-                                                                        inputs->decay_stride, inputs->beta, inputs->beta_stride, p.prepared);
-            if (status != LCPP_OK) return status;
-            auto chain = [&](auto warps) {
-                constexpr int WARPS = decltype(warps)::value;
-                const uint64_t grid = (uint64_t)sh.sequences * sh.heads * ceil_div(sh.value_dim, WARPS * 16);
-                return dr_launch<dr_backward_kernel<DK, PLANES, WARPS>>("dr_backward", grid, WARPS * 32,
-                                                                        sizeof(DrChainSmem<DK, PLANES, WARPS>), s, p);
-            };
-            const int warps = dr_warps(*shape, packed);
-            if (PLANES == 1 && warps == 8) {
-                if constexpr (PLANES == 1) status = chain(std::integral_constant<int, 8>{});
-            } else if (warps == 4) {
-                status = chain(std::integral_constant<int, 4>{});
-            } else {
-                status = chain(std::integral_constant<int, 2>{});
-            }
+                status = dr_launch<dr_prepare_kernel<T, DK, true>>("dr_prepare", l.slots * sh.key_heads, DR_PREPARE_THREADS,
+                                                                   sizeof(DrPrepareSmem<DK, PLANES>), s, pr);
+            if (status == LCPP_OK) status = dr_chain<T, DK, true>(*shape, p, s);
             if (status != LCPP_OK || !sh.rows) return status;
-            return dr_launch<dr_gradient_kernel<T, DK, PLANES>>("dr_gradient", l.slots * sh.key_heads, DR_GRAD_THREADS,
-                                                                sizeof(DrGradientSmem<DK, PLANES>), s, gr);
+            const uint64_t grid = l.slots * sh.key_heads;
+            if (sh.heads > sh.key_heads) return dr_launch<dr_gradient_kernel<T, DK, true>>("dr_gradient", grid, DR_GRAD_THREADS, smem, s, gr);
+            return dr_launch<dr_gradient_kernel<T, DK, false>>("dr_gradient", grid, DR_GRAD_THREADS, smem, s, gr);
         });
     });
 }

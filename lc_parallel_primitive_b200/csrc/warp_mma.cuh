@@ -1,42 +1,39 @@
-// Warp-level products of 16-bit tiles in shared memory (ldmatrix, mma.sync
-// m16n8k16 bf16), and the split of float32 values into two bf16 parts.
+// Warp-level products of float16 tiles in shared memory (ldmatrix, mma.sync m16n8k16) and float32 values as pairs of
+// float16.
 //
-// A tile has rows of COLS bf16 elements (64 or 128); its 16-byte pieces are
-// permuted within a row by the row's number modulo 8, so that 8 rows at the
-// same column lie in different banks.
+// Tiles are made of blocks with rows of 64 elements (128 bytes); the 16-byte pieces of a row are permuted by the row's
+// number modulo 8, so that 8 rows at the same column lie in different banks.  The same image lies in global memory, so
+// that a block is one bulk copy.
+//
+// A float32 value x enters a product as hi + lo: hi = f16(x s), lo = f16(x s - hi), with a power of two s that brings
+// the largest value of the matrix to 2^14 .. 2^15.  That leaves 2^-23 of a value, or 2^-39 of the largest where lo is
+// subnormal; hi hi + hi lo + lo hi leaves out 2^-22.  bf16 pairs would need no scale, but leave 2^-17.
 #pragma once
-#include <cuda_bf16.h>
+#include <cuda_fp16.h>
 #include "bulk.cuh"
 #include "common.cuh"
 
 namespace lcpp {
 
-template <int COLS>
-__device__ __forceinline__ uint32_t tile_at(uint32_t tile, int row, int piece) {
-    return tile + row * (COLS * 2) + ((piece ^ (row & 7)) << 4);
-}
-// The pair of elements (row, col), (row, col + 1), col even.
-template <int COLS>
-__device__ __forceinline__ uint32_t tile_word(uint32_t tile, int row, int col) {
-    uint32_t v;
-    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(tile_at<COLS>(tile, row, col >> 3) + (col & 7) * 2));
-    return v;
+constexpr int BLOCK_COLS = 64, BLOCK_ROW = 128;  // elements and bytes of a row
+
+// Byte of element (row, col) within a block.
+__host__ __device__ __forceinline__ uint32_t block_at(uint32_t row, uint32_t col) {
+    return row * BLOCK_ROW + ((((col >> 3) ^ row) & 7) << 4) + (col & 7) * 2;
 }
 
-// 16-byte copy to shared memory; `bytes` 0 writes zeros and reads nothing.
-__device__ __forceinline__ void cp_async16_fill(uint32_t dst, const void* src, uint32_t bytes) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-// rows x COLS elements from rows `stride` elements apart; zeros beyond `have_rows` and `have_cols` (a multiple of 8).
-template <int COLS>
-__device__ __forceinline__ void tile_load(uint32_t tile, const __nv_bfloat16* from, uint64_t stride, int rows, int have_rows,
-                                          int have_cols, int thread, int threads) {
-    for (int i = thread; i < rows * (COLS / 8); i += threads) {
-        const int r = i / (COLS / 8), c = i % (COLS / 8);
-        const bool have = r < have_rows && c * 8 < have_cols;
-        cp_async16_fill(tile_at<COLS>(tile, r, c), have ? from + r * stride + c * 8 : from, have ? 16 : 0);
+// What a lane adds to a block's address and its first row's for 16 x 16 elements at columns 16 j (j = 0 .. 3).
+struct LaneOffsets {
+    uint32_t rows[4];   // a stored [m][k], b stored [k][n] (transposed on the way)
+    uint32_t cols[4];   // b stored [n][k], a stored [k][m] (transposed on the way)
+    __device__ __forceinline__ explicit LaneOffsets(int lane) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            rows[j] = (((2 * j + (lane >> 4)) ^ (lane & 7)) << 4) + (lane & 15) * BLOCK_ROW;
+            cols[j] = (((2 * j + ((lane >> 3) & 1)) ^ (lane & 7)) << 4) + ((lane & 7) + (lane >> 4) * 8) * BLOCK_ROW;
+        }
     }
-}
+};
 
 __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -50,48 +47,93 @@ __device__ __forceinline__ void ldmatrix4_t(uint32_t (&r)[4], uint32_t addr) {
                  : "r"(addr)
                  : "memory");
 }
-// 16 x 16 pieces of a tile as operands.  (row, piece): the first row and 16-byte piece of the block.
-// A fragment (m16 k16): a stored [m][k], a_t stored [k][m].
-template <int COLS>
-__device__ __forceinline__ void load_a(uint32_t (&r)[4], uint32_t tile, int row, int piece, int lane) {
-    ldmatrix4(r, tile_at<COLS>(tile, row + (lane & 15), piece + (lane >> 4)));
+// Fragments of the 16 x 16 elements at (row, 16 j) of a block: A (m16 k16), or two of B (k16 n8 each: r[0], r[1] and
+// r[2], r[3]); _t where the block holds the operand's transpose.
+__device__ __forceinline__ void load_a(uint32_t (&r)[4], uint32_t block, int row, int j, const LaneOffsets& o) {
+    ldmatrix4(r, block + row * BLOCK_ROW + o.rows[j]);
 }
-template <int COLS>
-__device__ __forceinline__ void load_a_t(uint32_t (&r)[4], uint32_t tile, int row, int piece, int lane) {
-    ldmatrix4_t(r, tile_at<COLS>(tile, row + (lane & 7) + (lane >> 4) * 8, piece + ((lane >> 3) & 1)));
+__device__ __forceinline__ void load_a_t(uint32_t (&r)[4], uint32_t block, int row, int j, const LaneOffsets& o) {
+    ldmatrix4_t(r, block + row * BLOCK_ROW + o.cols[j]);
 }
-// Two B fragments (k16 n8 each: r[0], r[1] and r[2], r[3]): b stored [n][k], b_t stored [k][n].
-template <int COLS>
-__device__ __forceinline__ void load_b(uint32_t (&r)[4], uint32_t tile, int row, int piece, int lane) {
-    ldmatrix4(r, tile_at<COLS>(tile, row + (lane & 7) + (lane >> 4) * 8, piece + ((lane >> 3) & 1)));
+__device__ __forceinline__ void load_b(uint32_t (&r)[4], uint32_t block, int row, int j, const LaneOffsets& o) {
+    ldmatrix4(r, block + row * BLOCK_ROW + o.cols[j]);
 }
-template <int COLS>
-__device__ __forceinline__ void load_b_t(uint32_t (&r)[4], uint32_t tile, int row, int piece, int lane) {
-    ldmatrix4_t(r, tile_at<COLS>(tile, row + (lane & 15), piece + (lane >> 4)));
+__device__ __forceinline__ void load_b_t(uint32_t (&r)[4], uint32_t block, int row, int j, const LaneOffsets& o) {
+    ldmatrix4_t(r, block + row * BLOCK_ROW + o.rows[j]);
 }
 
-__device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-
-// (x, y) as pairs of bf16: hi the roundings, lo what they leave, itself rounded (the sum is off by 2^-18 at most).
-__device__ __forceinline__ void split_bf16(float x, float y, uint32_t& hi, uint32_t& lo) {
-    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(hi) : "f"(y), "f"(x));
-    const float rx = x - __uint_as_float(hi << 16), ry = y - __uint_as_float(hi & 0xffff0000u);
-    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(lo) : "f"(ry), "f"(rx));
+// Both halves of a pair of B fragments.
+__device__ __forceinline__ void mma_f16_2(float (&c0)[4], float (&c1)[4], const uint32_t (&a)[4], const uint32_t (&b)[4]) {
+    mma_f16(c0, a, b[0], b[1]);
+    mma_f16(c1, a, b[2], b[3]);
 }
-__device__ __forceinline__ float bf16_low(uint32_t v) { return __uint_as_float(v << 16); }
-__device__ __forceinline__ float bf16_high(uint32_t v) { return __uint_as_float(v & 0xffff0000u); }
+
+// ---- scales ------------------------------------------------------------------------------------------
+// A power of two and its inverse.
+struct Scale {
+    float by, back;
+};
+// For the largest absolute value `most`: most * by is in [2^14, 2^15), by <= 2^45 (1 for zeros).
+__device__ __forceinline__ Scale scale_for(float most) {
+    const int e = __float_as_int(most) >> 23 & 255;
+    const int field = e == 0 ? 127 : min(268 - e, 172);
+    return Scale{__int_as_float(field << 23), __int_as_float((254 - field) << 23)};
+}
+__device__ __forceinline__ float warp_max(float v) {  // of values >= 0
+    return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(v)));
+}
+template <int N>
+__device__ __forceinline__ float max_abs(const float (&c)[N][4]) {  // of the warp's accumulators
+    float m = 0.0f;
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) m = fmaxf(m, fabsf(c[n][j]));
+    return warp_max(m);
+}
+
+__device__ __forceinline__ uint32_t pack_f16(float x, float y) {
+    uint32_t v;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(v) : "f"(y), "f"(x));
+    return v;
+}
+__device__ __forceinline__ float2 unpack_f16(uint32_t v) { return __half22float2(*(const __half2*)&v); }
+__device__ __forceinline__ void split_f16(float x, float y, float s, uint32_t& hi, uint32_t& lo) {
+    hi = pack_f16(x * s, y * s);
+    const float2 h = unpack_f16(hi);
+    lo = pack_f16(fmaf(x, s, -h.x), fmaf(y, s, -h.y));
+}
 // Accumulators of two neighbouring 16 x 8 tiles as the fragment of the 16 x 16 block they are: as A (m = rows), and as
 // two B fragments with n = rows: (f[0], f[2]) rows 0-7, (f[1], f[3]) rows 8-15.
-__device__ __forceinline__ void split_block(const float (&c0)[4], const float (&c1)[4], uint32_t (&hi)[4], uint32_t (&lo)[4]) {
-    split_bf16(c0[0], c0[1], hi[0], lo[0]);
-    split_bf16(c0[2], c0[3], hi[1], lo[1]);
-    split_bf16(c1[0], c1[1], hi[2], lo[2]);
-    split_bf16(c1[2], c1[3], hi[3], lo[3]);
+__device__ __forceinline__ void split_block(const float (&c0)[4], const float (&c1)[4], float s, uint32_t (&hi)[4], uint32_t (&lo)[4]) {
+    split_f16(c0[0], c0[1], s, hi[0], lo[0]);
+    split_f16(c0[2], c0[3], s, hi[1], lo[1]);
+    split_f16(c1[0], c1[1], s, hi[2], lo[2]);
+    split_f16(c1[2], c1[3], s, hi[3], lo[3]);
+}
+__device__ __forceinline__ void scale_f16(uint32_t (&r)[4], __half2 by) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const __half2 v = __hmul2(*(const __half2*)&r[j], by);
+        r[j] = *(const uint32_t*)&v;
+    }
+}
+
+__device__ __forceinline__ uint32_t lds32(uint32_t addr) {
+    uint32_t v;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ void sts32(uint32_t addr, uint32_t v) { asm volatile("st.shared.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory"); }
+// 16-byte asynchronous copy to shared memory; `bytes` 0 writes zeros and reads nothing.
+__device__ __forceinline__ void cp_async16_fill(uint32_t dst, const void* src, uint32_t bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 
 }  // namespace lcpp

@@ -273,13 +273,12 @@ class DeviceDeltaRule(_Recorded):
 
     @staticmethod
     def GetTempStorageBytes(num_rows: int, num_sequences: int, heads: int, key_heads: int, key_dim: int, value_dim: int,
-                            dtype=torch.bfloat16, backward: bool = True, aligned: bool = True) -> int:
-        """For Forward, or for both calls; aligned=False: rows of d_q, d_k, d_v or d_grad_out may start off a 16-byte
-        boundary."""
+                            dtype=torch.bfloat16, backward: bool = True) -> int:
+        """For Forward, or (backward) for both calls."""
         if dtype not in _FLOATS:
             raise TypeError(f"unsupported element type {dtype}")
         shape = DeviceDeltaRule._shape(num_rows, num_sequences, heads, key_heads, key_dim, value_dim)
-        return int(L.lib().lcpp_delta_rule_temp_bytes(_FLOATS[dtype], shape, backward, aligned))
+        return int(L.lib().lcpp_delta_rule_temp_bytes(_FLOATS[dtype], shape, backward))
 
     @staticmethod
     def GetSavedStateBytes(num_rows: int, num_sequences: int, heads: int, key_heads: int, key_dim: int, value_dim: int) -> int:
