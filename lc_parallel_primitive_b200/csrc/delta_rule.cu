@@ -95,19 +95,22 @@ __device__ __forceinline__ void dr_store(uint8_t* image, uint32_t blocks, uint32
 }
 
 // ---- what does not depend on the state ------------------------------------------------------------
-constexpr int DR_PREPARE_THREADS = 128;
+constexpr int DR_PREPARE_THREADS = 256;  // warps: 4 blocks of 16 rows x 2 halves of the columns
 constexpr int DR_PITCH = 68;
 struct DrInvert {
     float m[64 * DR_PITCH], inv[64 * DR_PITCH], tmp[32 * 36];
 };
+// The keys' blocks, then a head's triangular matrix and its inverse, then the blocks of the head's unit, one after the other
+// in the same memory.
 template <int DK, int PLANES>
 struct DrPrepareSmem {
     union alignas(128) {
         uint8_t keys[2 * DR_KEYS<DK, PLANES>];
         DrInvert invert;
+        uint8_t blocks[4 * DR_BLOCK];
     };
-    alignas(128) uint8_t unit[DR_UNIT];
-    float most[2][4];
+    alignas(128) DrGates gates;
+    float most[2][8];
 };
 
 __device__ __forceinline__ void dr_fma4(float (&v)[4], float a, const float* b) {
@@ -118,68 +121,81 @@ __device__ __forceinline__ void dr_fma4(float (&v)[4], float a, const float* b) 
 // lane, then blocks below from ones above: [X 0; -Y m21 X, Y].
 __device__ __forceinline__ void dr_invert(DrInvert& s) {
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
-    if (lane < 16) {
-        const int b = warp * 16;
-        float x[16];
+    if (warp < 4) {
+        if (lane < 16) {
+            const int b = warp * 16;
+            float x[16];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            float v = i == lane ? 1.0f : 0.0f;
+            for (int i = 0; i < 16; ++i) {
+                float v = i == lane ? 1.0f : 0.0f;
 #pragma unroll
-            for (int k = 0; k < i; k += 4) {
-                const float4 m = *(const float4*)&s.m[(b + i) * DR_PITCH + b + k];
-                v = fmaf(-m.x, x[k], v);
-                if (k + 1 < i) v = fmaf(-m.y, x[k + 1], v);
-                if (k + 2 < i) v = fmaf(-m.z, x[k + 2], v);
-                if (k + 3 < i) v = fmaf(-m.w, x[k + 3], v);
+                for (int k = 0; k < i; k += 4) {
+                    const float4 m = *(const float4*)&s.m[(b + i) * DR_PITCH + b + k];
+                    v = fmaf(-m.x, x[k], v);
+                    if (k + 1 < i) v = fmaf(-m.y, x[k + 1], v);
+                    if (k + 2 < i) v = fmaf(-m.z, x[k + 2], v);
+                    if (k + 3 < i) v = fmaf(-m.w, x[k + 3], v);
+                }
+                x[i] = v;
             }
-            x[i] = v;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s.inv[(b + i) * DR_PITCH + b + lane] = x[i];
         }
-#pragma unroll
-        for (int i = 0; i < 16; ++i) s.inv[(b + i) * DR_PITCH + b + lane] = x[i];
-    }
-    for (int i = t; i < 64 * 16; i += DR_PREPARE_THREADS) {  // above the diagonal blocks
-        const int r = i >> 4, c = (i & 15) * 4;
-        if ((c >> 4) > (r >> 4)) *(float4*)&s.inv[r * DR_PITCH + c] = make_float4(0, 0, 0, 0);
+    } else {
+        for (int i = t - 128; i < 64 * 16; i += 128) {  // above the diagonal blocks
+            const int r = i >> 4, c = (i & 15) * 4;
+            if ((c >> 4) > (r >> 4)) *(float4*)&s.inv[r * DR_PITCH + c] = make_float4(0, 0, 0, 0);
+        }
     }
     __syncthreads();
     {
-        const int half = t >> 6, b = half * 32, r = (t & 63) >> 2, c = (t & 3) * 4;  // blocks (16, 0) and (48, 32)
-        float v[4] = {0, 0, 0, 0};
+        const int half = t >> 7, b = half * 32, r = (t & 127) >> 3, c = (t & 7) * 2;  // blocks (16, 0) and (48, 32)
+        float v0 = 0.0f, v1 = 0.0f;
 #pragma unroll
-        for (int k = 0; k < 16; ++k) dr_fma4(v, s.m[(b + 16 + r) * DR_PITCH + b + k], &s.inv[(b + k) * DR_PITCH + b + c]);
-        *(float4*)&s.tmp[(half * 16 + r) * 36 + c] = make_float4(v[0], v[1], v[2], v[3]);
+        for (int k = 0; k < 16; ++k) {
+            const float a = s.m[(b + 16 + r) * DR_PITCH + b + k];
+            const float2 x = *(const float2*)&s.inv[(b + k) * DR_PITCH + b + c];
+            v0 = fmaf(a, x.x, v0), v1 = fmaf(a, x.y, v1);
+        }
+        *(float2*)&s.tmp[(half * 16 + r) * 36 + c] = make_float2(v0, v1);
         __syncthreads();
-        v[0] = v[1] = v[2] = v[3] = 0.0f;
+        v0 = v1 = 0.0f;
 #pragma unroll
-        for (int k = 0; k < 16; ++k) dr_fma4(v, s.inv[(b + 16 + r) * DR_PITCH + b + 16 + k], &s.tmp[(half * 16 + k) * 36 + c]);
-        *(float4*)&s.inv[(b + 16 + r) * DR_PITCH + b + c] = make_float4(-v[0], -v[1], -v[2], -v[3]);
+        for (int k = 0; k < 16; ++k) {
+            const float a = s.inv[(b + 16 + r) * DR_PITCH + b + 16 + k];
+            const float2 x = *(const float2*)&s.tmp[(half * 16 + k) * 36 + c];
+            v0 = fmaf(a, x.x, v0), v1 = fmaf(a, x.y, v1);
+        }
+        *(float2*)&s.inv[(b + 16 + r) * DR_PITCH + b + c] = make_float2(-v0, -v1);
     }
     __syncthreads();
     {
-        const int r = t >> 2, c = (t & 3) * 4;  // block (32, 0), columns c .. and 16 + c ..
-        float v[4] = {0, 0, 0, 0}, u[4] = {0, 0, 0, 0};
-#pragma unroll 8
-        for (int k = 0; k < 32; ++k) {
-            const float a = s.m[(32 + r) * DR_PITCH + k];
-            dr_fma4(v, a, &s.inv[k * DR_PITCH + c]), dr_fma4(u, a, &s.inv[k * DR_PITCH + 16 + c]);
+        const int r = t >> 3, c = (t & 7) * 4;  // block (32, 0)
+        float v[4] = {0, 0, 0, 0};
+#pragma unroll 4
+        for (int k = 0; k < 32; k += 4) {
+            const float4 a = *(const float4*)&s.m[(32 + r) * DR_PITCH + k];
+            const float* const b = &s.inv[k * DR_PITCH + c];
+            dr_fma4(v, a.x, b), dr_fma4(v, a.y, b + DR_PITCH), dr_fma4(v, a.z, b + 2 * DR_PITCH), dr_fma4(v, a.w, b + 3 * DR_PITCH);
         }
         *(float4*)&s.tmp[r * 36 + c] = make_float4(v[0], v[1], v[2], v[3]);
-        *(float4*)&s.tmp[r * 36 + 16 + c] = make_float4(u[0], u[1], u[2], u[3]);
         __syncthreads();
-        v[0] = v[1] = v[2] = v[3] = u[0] = u[1] = u[2] = u[3] = 0.0f;
-#pragma unroll 8
-        for (int k = 0; k < 32; ++k) {
-            const float a = s.inv[(32 + r) * DR_PITCH + 32 + k];
-            dr_fma4(v, a, &s.tmp[k * 36 + c]), dr_fma4(u, a, &s.tmp[k * 36 + 16 + c]);
+        v[0] = v[1] = v[2] = v[3] = 0.0f;
+#pragma unroll 4
+        for (int k = 0; k < 32; k += 4) {
+            const float4 a = *(const float4*)&s.inv[(32 + r) * DR_PITCH + 32 + k];
+            const float* const b = &s.tmp[k * 36 + c];
+            dr_fma4(v, a.x, b), dr_fma4(v, a.y, b + 36), dr_fma4(v, a.z, b + 72), dr_fma4(v, a.w, b + 108);
         }
         *(float4*)&s.inv[(32 + r) * DR_PITCH + c] = make_float4(-v[0], -v[1], -v[2], -v[3]);
-        *(float4*)&s.inv[(32 + r) * DR_PITCH + 16 + c] = make_float4(-u[0], -u[1], -u[2], -u[3]);
     }
     __syncthreads();
 }
 
-// The largest of the CTA's values >= 0; `room` 4 floats, between barriers of the caller.
-__device__ __forceinline__ float dr_max4(const float* room) { return fmaxf(fmaxf(room[0], room[1]), fmaxf(room[2], room[3])); }
+// The largest of the warps' values >= 0.
+__device__ __forceinline__ float dr_max8(const float* of) {
+    return fmaxf(fmaxf(fmaxf(of[0], of[1]), fmaxf(of[2], of[3])), fmaxf(fmaxf(of[4], of[5]), fmaxf(of[6], of[7])));
+}
 
 struct DrPrepare {
     DrShape sh;
@@ -192,7 +208,7 @@ struct DrPrepare {
 };
 
 template <typename T, int DK, bool BACKWARD>
-__global__ void __launch_bounds__(DR_PREPARE_THREADS)
+__global__ void __launch_bounds__(DR_PREPARE_THREADS, sizeof(T) == 4 ? 2 : 3)
 dr_prepare_kernel(const __grid_constant__ DrPrepare p) {
     constexpr int PLANES = sizeof(T) == 4 ? 2 : 1, NB = DK / 64, ITEMS = DR_CHUNK * DK / 8 / DR_PREPARE_THREADS;
     extern __shared__ __align__(128) uint8_t dr_smem[];
@@ -202,26 +218,44 @@ dr_prepare_kernel(const __grid_constant__ DrPrepare p) {
     const uint32_t hk = blockIdx.x % sh.key_heads, group = sh.heads / sh.key_heads;
     const DrChunk c(sh, slot);
     if (!c.rows) return;
-    const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+    const int t = threadIdx.x, lane = t & 31, warp = t >> 5, rb = warp >> 1, ch = warp & 1;
     const LaneOffsets o(lane);
     // K and Q into blocks, each with a scale
     Scale scale[2];
     {
         alignas(16) T raw[2][ITEMS][8];
+        auto from = [&](int x, uint32_t r, uint32_t d) {
+            return (const T*)(x ? p.q : p.k) + (c.row + r) * (x ? p.q_stride : p.k_stride) + (uint64_t)hk * sh.key_dim + d;
+        };
+        if (p.wide) {  // all loads before the first use: rows and columns that do not exist are read from others and cleared
 #pragma unroll
-        for (int x = 0; x < 2; ++x)
+            for (int x = 0; x < 2; ++x)
+#pragma unroll
+                for (int i = 0; i < ITEMS; ++i) {
+                    const uint32_t item = i * DR_PREPARE_THREADS + t, r = item / (DK / 8), d = item % (DK / 8) * 8;
+                    const T* const at = from(x, min(r, c.rows - 1), d < sh.key_dim ? d : 0);
+#pragma unroll
+                    for (int j = 0; j < (int)sizeof(T) / 2; ++j) ((uint4*)raw[x][i])[j] = __ldg((const uint4*)at + j);
+                }
 #pragma unroll
             for (int i = 0; i < ITEMS; ++i) {
                 const uint32_t item = i * DR_PREPARE_THREADS + t, r = item / (DK / 8), d = item % (DK / 8) * 8;
-                const T* const from = (const T*)(x ? p.q : p.k) + (c.row + r) * (x ? p.q_stride : p.k_stride) + (uint64_t)hk * sh.key_dim + d;
-                if (p.wide && r < c.rows && d < sh.key_dim) {
+                if (r < c.rows && d < sh.key_dim) continue;
 #pragma unroll
-                    for (int j = 0; j < (int)sizeof(T) / 2; ++j) ((uint4*)raw[x][i])[j] = ((const uint4*)from)[j];
-                } else {
+                for (int x = 0; x < 2; ++x)
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) raw[x][i][j] = r < c.rows && d + j < sh.key_dim ? from[j] : narrow<T>(0.0f);
-                }
+                    for (int j = 0; j < (int)sizeof(T) / 2; ++j) ((uint4*)raw[x][i])[j] = make_uint4(0, 0, 0, 0);
             }
+        } else {
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+#pragma unroll
+                for (int i = 0; i < ITEMS; ++i) {
+                    const uint32_t item = i * DR_PREPARE_THREADS + t, r = item / (DK / 8), d = item % (DK / 8) * 8;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) raw[x][i][j] = r < c.rows && d + j < sh.key_dim ? *from(x, r, d + j) : narrow<T>(0.0f);
+                }
+        }
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
             float most = 0.0f;
@@ -235,7 +269,7 @@ dr_prepare_kernel(const __grid_constant__ DrPrepare p) {
         __syncthreads();
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-            scale[x] = scale_for(dr_max4(s.most[x]));
+            scale[x] = scale_for(dr_max8(s.most[x]));
 #pragma unroll
             for (int i = 0; i < ITEMS; ++i) {
                 const uint32_t item = i * DR_PREPARE_THREADS + t, r = item / (DK / 8), d = item % (DK / 8) * 8;
@@ -254,36 +288,37 @@ dr_prepare_kernel(const __grid_constant__ DrPrepare p) {
         bulk_store(p.keys + (slot * sh.key_heads + hk) * (2 * DR_KEYS<DK, PLANES>), s.keys, 2 * DR_KEYS<DK, PLANES>);
         bulk_commit();
     }
-    float nr[8][4] = {}, rd[8][4] = {};  // k_i.k_j and q_i.k_j: 16 rows a warp
+    float nr[4][4] = {}, rd[4][4] = {};  // k_i.k_j and q_i.k_j: 16 rows and 32 columns a warp
     const uint32_t kt = smem_u32(s.keys), qt = kt + DR_KEYS<DK, PLANES>;
 #pragma unroll
     for (int kk = 0; kk < DK / 16; ++kk) {
+        if (ch * 2 > rb) break;  // columns past the warp's rows are masked
         const uint32_t block = (kk >> 2) * DR_BLOCK;
         uint32_t ak[PLANES][4], aq[PLANES][4];
 #pragma unroll
         for (int i = 0; i < PLANES; ++i) {
-            load_a(ak[i], kt + i * NB * DR_BLOCK + block, warp * 16, kk & 3, o);
-            load_a(aq[i], qt + i * NB * DR_BLOCK + block, warp * 16, kk & 3, o);
+            load_a(ak[i], kt + i * NB * DR_BLOCK + block, rb * 16, kk & 3, o);
+            load_a(aq[i], qt + i * NB * DR_BLOCK + block, rb * 16, kk & 3, o);
         }
 #pragma unroll
-        for (int n = 0; n < 4; ++n) {
-            if (n > warp) break;  // columns past the warp's rows are masked
+        for (int n = 0; n < 2; ++n) {
+            if (ch * 2 + n > rb) break;
 #pragma unroll
             for (int i = 0; i < PLANES; ++i) {
                 uint32_t b[4];
-                load_b(b, kt + i * NB * DR_BLOCK + block, n * 16, kk & 3, o);
+                load_b(b, kt + i * NB * DR_BLOCK + block, (ch * 2 + n) * 16, kk & 3, o);
 #pragma unroll
                 for (int l = 0; l < PLANES - i; ++l) mma_f16_2(nr[2 * n], nr[2 * n + 1], ak[l], b), mma_f16_2(rd[2 * n], rd[2 * n + 1], aq[l], b);
             }
         }
     }
-    const int r0 = warp * 16 + (lane >> 2), col = (lane & 3) * 2;
+    const int r0 = rb * 16 + (lane >> 2), col = ch * 32 + (lane & 3) * 2;
     const float back_near = scale[0].back * scale[0].back, back_read = scale[0].back * scale[1].back * sh.scale;
 #pragma unroll
-    for (int n = 0; n < 8; ++n)
+    for (int n = 0; n < 4; ++n)
 #pragma unroll
         for (int j = 0; j < 4; ++j) nr[n][j] *= back_near, rd[n][j] *= back_read;
-    DrGates& gates = *(DrGates*)(s.unit + 4 * DR_BLOCK);
+    DrGates& gates = s.gates;
     for (uint32_t h = hk * group; h < (hk + 1) * group; ++h) {
         if (t == 0) bulk_wait_read_all();  // the keys, the head before's unit
         __syncthreads();
@@ -308,31 +343,36 @@ dr_prepare_kernel(const __grid_constant__ DrPrepare p) {
             for (int j = 0; j < 2; ++j) {
                 const int r = lane * 2 + j;
                 gates.total[r] = (float)total[j], gates.rest[r] = (float)(total[j] - (float)total[j]);
-                gates.g[r] = expf((float)total[j]), gates.e[r] = expf((float)(last - total[j]));
+                gates.g[r] = __expf((float)total[j]), gates.e[r] = __expf((float)(last - total[j]));
             }
             if (lane == 0) gates.back_k = scale[0].back, gates.back_q = scale[1].back;
         }
         __syncthreads();
-        float a[8][4], most = 0.0f;
+        float a[4][4], most = 0.0f;
 #pragma unroll
-        for (int n = 0; n < 8; ++n)
+        for (int n = 0; n < 4; ++n) {
+            if (ch * 4 + n <= 2 * rb + 1) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int r = r0 + (j >> 1) * 8, cc = n * 8 + col + (j & 1);
-                const float d = cc <= r ? expf((gates.total[r] - gates.total[cc]) + (gates.rest[r] - gates.rest[cc])) : 0.0f;
-                a[n][j] = cc <= r ? d * rd[n][j] : 0.0f;
-                most = fmaxf(most, fabsf(a[n][j]));
-                s.invert.m[r * DR_PITCH + cc] = cc < r ? d * nr[n][j] * gates.beta[BACKWARD ? r : cc] : 0.0f;
+                for (int j = 0; j < 4; ++j) {
+                    const int r = r0 + (j >> 1) * 8, cc = n * 8 + col + (j & 1);
+                    const float d = __expf((gates.total[r] - gates.total[cc]) + (gates.rest[r] - gates.rest[cc]));
+                    a[n][j] = cc <= r ? d * rd[n][j] : 0.0f;
+                    most = fmaxf(most, fabsf(a[n][j]));
+                    s.invert.m[r * DR_PITCH + cc] = cc < r ? d * nr[n][j] * gates.beta[BACKWARD ? r : cc] : 0.0f;
+                }
+            } else {  // the inversion does not look above the blocks of the diagonal
+                a[n][0] = a[n][1] = a[n][2] = a[n][3] = 0.0f;
             }
+        }
         most = warp_max(most);
         if (lane == 0) s.most[0][warp] = most;
         __syncthreads();
         dr_invert(s.invert);
-        const Scale read = scale_for(dr_max4(s.most[0]));
-        float v[8][4];
+        const Scale read = scale_for(dr_max8(s.most[0]));
+        float v[4][4];
         most = 0.0f;
 #pragma unroll
-        for (int n = 0; n < 8; ++n)
+        for (int n = 0; n < 4; ++n)
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 const float2 x = *(const float2*)&s.invert.inv[(r0 + j * 8) * DR_PITCH + n * 8 + col];
@@ -342,14 +382,14 @@ dr_prepare_kernel(const __grid_constant__ DrPrepare p) {
         most = warp_max(most);
         if (lane == 0) s.most[1][warp] = most;
         __syncthreads();
-        const Scale inverse = scale_for(dr_max4(s.most[1]));
+        const Scale inverse = scale_for(dr_max8(s.most[1]));
         if (t == 0) gates.back_inverse = inverse.back, gates.back_read = read.back;
 #pragma unroll
-        for (int n = 0; n < 8; ++n)
+        for (int n = 0; n < 4; ++n)
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 uint32_t hi, lo;
-                uint8_t* const at = s.unit + block_at(r0 + j * 8, n * 8 + col);
+                uint8_t* const at = s.blocks + block_at(r0 + j * 8, n * 8 + col);
                 split_f16(v[n][2 * j], v[n][2 * j + 1], inverse.by, hi, lo);
                 *(uint32_t*)at = hi, *(uint32_t*)(at + DR_BLOCK) = lo;
                 split_f16(a[n][2 * j], a[n][2 * j + 1], read.by, hi, lo);
@@ -358,7 +398,9 @@ dr_prepare_kernel(const __grid_constant__ DrPrepare p) {
         fence_proxy_async_smem();
         __syncthreads();
         if (t == 0) {
-            bulk_store(p.units + (slot * sh.heads + h) * DR_UNIT, s.unit, DR_UNIT);
+            uint8_t* const to = p.units + (slot * sh.heads + h) * DR_UNIT;
+            bulk_store(to, s.blocks, 4 * DR_BLOCK);
+            bulk_store(to + 4 * DR_BLOCK, &s.gates, sizeof(DrGates));
             bulk_commit();
         }
     }
@@ -628,7 +670,7 @@ dr_forward_kernel(const __grid_constant__ DrChain p) {
         const uint64_t unit = cta.unit(it);
         // r = S0 K^T (value x token) and out = Q S0^T (token x value)
         float r[8][4] = {}, y[4][2][4] = {};
-        const Scale ss = scale_for(max_abs(s));
+        const Scale ss = coarse_scale_for(max_abs(s));
         uint8_t* const states = p.states.at ? p.states.of(unit) : nullptr;
         if (states) cta.keep_back(p.states.back, unit, ss.back * back_domain);
 #pragma unroll
@@ -682,7 +724,7 @@ dr_forward_kernel(const __grid_constant__ DrChain p) {
         }
         const float back_w = sr.back * gt.back_inverse;
         if (p.kept.at) {
-            const Scale sw = scale_for(max_abs(w));
+            const Scale sw = coarse_scale_for(max_abs(w));
             uint8_t* const kept = p.kept.of(unit);
             cta.keep_back(p.kept.back, unit, sw.back * back_w);
 #pragma unroll
@@ -794,7 +836,7 @@ dr_backward_kernel(const __grid_constant__ DrChain p) {
         const uint32_t raw = smem_u32(cta.sm.raw[warp][it & 1]);
         // du = e X K^T (value x token)
         float du[8][4] = {};
-        const Scale sx = scale_for(max_abs(x));
+        const Scale sx = coarse_scale_for(max_abs(x));
         uint8_t* const states = p.states.of(unit);
         cta.keep_back(p.states.back, unit, sx.back * back_domain);
 #pragma unroll
@@ -819,7 +861,7 @@ dr_backward_kernel(const __grid_constant__ DrChain p) {
                 }
             }
         }
-        const Scale so = scale_for(warp_max(most)), sg = scale_for(warp_max(most_g) * fabsf(p.sh.scale));
+        const Scale so = coarse_scale_for(warp_max(most)), sg = scale_for(warp_max(most_g) * fabsf(p.sh.scale));
         cta.keep_back(p.back_values, unit, so.back);
         {
             const float back = sx.back * back_domain * gt.back_k * so.by * __frcp_rn(gt.back_read);
@@ -868,7 +910,7 @@ dr_backward_kernel(const __grid_constant__ DrChain p) {
         }
         const float back_z = sd.back * gt.back_inverse * so.back * gt.back_read;
         {
-            const Scale sz = scale_for(max_abs(z));
+            const Scale sz = coarse_scale_for(max_abs(z));
             uint8_t* const kept = p.kept.of(unit);
             cta.keep_back(p.kept.back, unit, sz.back * back_z);
 #pragma unroll
@@ -926,7 +968,7 @@ dr_backward_kernel(const __grid_constant__ DrChain p) {
 }
 
 // ---- gradients of the inputs ------------------------------------------------------------------------
-constexpr int DR_GRAD_THREADS = 256;  // warps: 4 blocks of 16 tokens x 2 halves of the key columns
+constexpr int DR_GRAD_THREADS = 512;  // warps: 4 blocks of 16 tokens x 4 parts of the key columns
 // 64 tokens x 32 of the value dimensions of dO: rows of 64 bytes with permuted pieces, float32 rows of 144 bytes.
 template <typename T>
 constexpr int DR_SLAB_ROW = sizeof(T) == 4 ? 144 : 64;
@@ -946,9 +988,10 @@ struct DrGradientSmem {
     uint8_t dn[2 * DR_BLOCK];
     DrGates gates;
     float factor[5][8], back[5], own[4][8];  // of 16 value dimensions: shares of the largest scale; scales; of S, X, w, z
+    uint32_t uneven[5];                      // whether not all factors of a product are 1
     float by_out[8];                         // scales of dO
-    alignas(16) float dbeta[4][DR_CHUNK];  // also read and written in pairs
-    float dot[2][DR_CHUNK], carry[2][DR_CHUNK], most[2][8], sx[8];
+    float dbeta[DR_CHUNK];
+    float dot[4][DR_CHUNK], carry[4][DR_CHUNK], most[2][16], sx[16];
     uint64_t full[2], keys_full;
 };
 
@@ -969,7 +1012,7 @@ template <typename T, int DK, bool SHARED>  // SHARED: several heads a key head
 __global__ void __launch_bounds__(DR_GRAD_THREADS, 1)
 dr_gradient_kernel(const __grid_constant__ DrGradient p) {
     using Smem = DrGradientSmem<T, DK>;
-    constexpr int PLANES = Smem::PLANES, NB = Smem::NB, NT = DK / 16, NP = DK / 32;  // (pairs of) tiles of 8 key columns a warp has
+    constexpr int PLANES = Smem::PLANES, NB = Smem::NB, NT = DK / 32, NP = DK / 64;  // (pairs of) tiles of 8 key columns a warp has
     constexpr bool EXACT = sizeof(T) == 2;
     extern __shared__ __align__(128) uint8_t dr_smem[];
     auto& sm = *(Smem*)dr_smem;
@@ -978,7 +1021,7 @@ dr_gradient_kernel(const __grid_constant__ DrGradient p) {
     const uint32_t hk = blockIdx.x % sh.key_heads, group = sh.heads / sh.key_heads, h0 = hk * group;
     const DrChunk c(sh, slot);
     if (!c.rows) return;
-    const int t = threadIdx.x, lane = t & 31, warp = t >> 5, rb = warp >> 1, ch = warp & 1, g = lane >> 2, col = (lane & 3) * 2;
+    const int t = threadIdx.x, lane = t & 31, warp = t >> 5, rb = warp >> 2, cq = warp & 3, g = lane >> 2, col = (lane & 3) * 2;
     const LaneOffsets o(lane);
     const uint32_t limit = g_spin_limit, groups = (sh.value_dim + 15) / 16, steps = (groups + 1) / 2, total = steps * group;
     bool ok = true;
@@ -997,9 +1040,8 @@ dr_gradient_kernel(const __grid_constant__ DrGradient p) {
         constexpr int E = 16 / sizeof(T), PIECES = 32 / E;
         const uint32_t v0 = it % steps * 32, slab = smem_u32(sm.slab[it & 1]);
         const T* const from = (const T*)p.out + c.row * p.out_stride + (uint64_t)(h0 + it / steps) * sh.value_dim + v0;
-#pragma unroll
-        for (int i = 0; i < DR_CHUNK * PIECES / DR_GRAD_THREADS; ++i) {
-            const uint32_t item = i * DR_GRAD_THREADS + t, r = item / PIECES, e = item % PIECES * E;
+        for (int item = t; item < DR_CHUNK * PIECES; item += DR_GRAD_THREADS) {
+            const uint32_t r = item / PIECES, e = item % PIECES * E;
             const uint32_t at = dr_slab_at<T>(slab, r, item % PIECES);
             if (p.wide) {
                 const bool have = r < c.rows && v0 + e < sh.value_dim;
@@ -1041,12 +1083,13 @@ dr_gradient_kernel(const __grid_constant__ DrGradient p) {
 #pragma unroll
             for (int i = 4; i > 0; i >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffu, most, i));
             sm.factor[warp][lane] = most > 0.0f ? mine / most : 0.0f;
-            if (lane == 0) sm.back[warp] = most;
+            const bool uneven = __any_sync(0xffu, have && mine != most);
+            if (lane == 0) sm.back[warp] = most, sm.uneven[warp] = uneven;
             if (warp == 4) sm.own[0][lane] = s, sm.own[1][lane] = x, sm.own[2][lane] = w, sm.own[3][lane] = z;
             if (warp == 0) sm.by_out[lane] = go > 0.0f ? 1.0f / go : 0.0f;
         }
-        float dq[NT][4] = {}, er[NT][4] = {}, wr[NT][4] = {}, a[4][4] = {}, n[4][4] = {};
-        float sx = 0.0f, db0 = 0.0f, db1 = 0.0f;
+        float dq[NT][4] = {}, er[NT][4] = {}, wr[NT][4] = {}, a[2][4] = {}, n[2][4] = {};
+        float sx = 0.0f;
         for (uint32_t v = 0; v < steps; ++v, ++it) {
             cp_async_wait_all();
             __syncthreads();  // dO is there, and the buffers of the step before are free
@@ -1058,16 +1101,20 @@ dr_gradient_kernel(const __grid_constant__ DrGradient p) {
             if (it == 0) ok = mbar_wait(&sm.keys_full, 0, limit) && ok;
             ok = mbar_wait(&sm.full[it & 1], (it >> 1) & 1, limit) && ok;
             const uint8_t* const step = sm.step[it & 1];
+            const float beta0 = sm.gates.beta[token], beta1 = sm.gates.beta[token + 8];
+            T* const dv0 = (T*)p.dv + ((c.row + token) * sh.heads + h) * sh.value_dim;
+            T* const dv1 = dv0 + 8ull * sh.heads * sh.value_dim;
             const uint32_t s = smem_u32(step), x = s + Smem::STATE, w = x + Smem::STATE, z = w + Smem::KEPT,
                            slab = smem_u32(sm.slab[it & 1]);
 #pragma unroll
             for (int kt = 0; kt < 2; ++kt) {
                 const uint32_t at = v * 2 + kt;  // 16 value dimensions
                 if (at >= groups) break;
-                uint32_t gs[2][4], gw[2][4], aw[2][4], zs[2][4], zw[2][4];
+                // dO (and z below) against S0, and against w: shares of the scales differ
+                uint32_t go[2][4], aw[2][4], zt[2][4];
                 if (p.out) {
                     const float by = sm.by_out[at];
-                    if constexpr (sizeof(T) == 2) {
+                    if constexpr (EXACT) {
                         uint32_t r[4];
                         ldmatrix4(r, dr_slab_at<T>(slab, rb * 16 + (lane & 15), kt * 2 + (lane >> 4)));
 #pragma unroll
@@ -1075,135 +1122,148 @@ dr_gradient_kernel(const __grid_constant__ DrGradient p) {
                             float2 f;
                             if constexpr (std::is_same_v<T, __half>) f = unpack_f16(r[j]);
                             else f = make_float2(__uint_as_float(r[j] << 16), __uint_as_float(r[j] & 0xffff0000u));
-                            gs[0][j] = gw[0][j] = pack_f16(f.x * by, f.y * by);
+                            go[0][j] = pack_f16(f.x * by, f.y * by);
                         }
                     } else {
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
                             const uint32_t f = slab + (rb * 16 + g + (j & 1) * 8) * 144 + (kt * 16 + (j >> 1) * 8 + col) * 4;
-                            split_f16(__uint_as_float(lds32(f)), __uint_as_float(lds32(f + 4)), by, gs[0][j], gs[1][j]);
-                            gw[0][j] = gs[0][j], gw[1][j] = gs[1][j];
+                            split_f16(__uint_as_float(lds32(f)), __uint_as_float(lds32(f + 4)), by, go[0][j], go[1][j]);
                         }
                     }
-#pragma unroll
-                    for (int i = 0; i < (EXACT ? 1 : 2); ++i)
-                        scale_f16(gs[i], __float2half2_rn(sm.factor[0][at])), scale_f16(gw[i], __float2half2_rn(sm.factor[3][at]));
                 }
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     load_a_t(aw[i], w + i * DR_PIECE, kt * 16, rb, o);
-                    load_a_t(zs[i], z + i * DR_PIECE, kt * 16, rb, o);
+                    load_a_t(zt[i], z + i * DR_PIECE, kt * 16, rb, o);
                 }
-                if (ch == 0) {  // dv = beta z
-                    T* const to = (T*)p.dv + (c.row * sh.heads + h) * sh.value_dim;
+                if (cq == (int)(at & 3)) {  // dv = beta z
                     const float back = sm.own[3][at];
+                    const uint32_t vcol = at * 16 + col;
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         const uint32_t r = token + (j & 1) * 8;
-                        const float b = sm.gates.beta[r] * back;
-                        const float2 hi = unpack_f16(zs[0][j]), lo = unpack_f16(zs[1][j]);
+                        const float b = (j & 1 ? beta1 : beta0) * back;
+                        const float2 hi = unpack_f16(zt[0][j]), lo = unpack_f16(zt[1][j]);
                         if (r < c.rows)
-                            dr_store_pair(to + (uint64_t)r * sh.heads * sh.value_dim, at * 16 + (j >> 1) * 8 + col, sh.value_dim, p.pairs_v,
-                                          b * (hi.x + lo.x), b * (hi.y + lo.y));
+                            dr_store_pair((j & 1) ? dv1 : dv0, vcol + (j >> 1) * 8, sh.value_dim, p.pairs_v, b * (hi.x + lo.x), b * (hi.y + lo.y));
                     }
                 }
+                if (sm.uneven[2]) {
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
+                    for (int i = 0; i < 2; ++i) scale_f16(aw[i], __float2half2_rn(sm.factor[2][at]));
+                }
+                {  // against w first, as they are; then scaled on to what S0 wants
+                    uint32_t gw[2][4], zw[2][4];
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) zw[i][j] = zs[i][j];
-                    scale_f16(zs[i], __float2half2_rn(sm.factor[1][at])), scale_f16(zw[i], __float2half2_rn(sm.factor[4][at]));
-                    scale_f16(aw[i], __float2half2_rn(sm.factor[2][at]));
+                    for (int i = 0; i < 2; ++i)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) gw[i][j] = go[i][j], zw[i][j] = zt[i][j];
+                    if (sm.uneven[3] && p.out) {
+#pragma unroll
+                        for (int i = 0; i < (EXACT ? 1 : 2); ++i) scale_f16(gw[i], __float2half2_rn(sm.factor[3][at]));
+                    }
+                    if (sm.uneven[4]) {
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) scale_f16(zw[i], __float2half2_rn(sm.factor[4][at]));
+                    }
+                    if (cq <= rb) {  // 16 of the other tokens
+                        uint32_t b[4];
+                        load_b_t(b, w, kt * 16, cq, o);
+                        if (p.out) {
+                            mma_f16_2(a[0], a[1], gw[0], b);
+                            if constexpr (!EXACT) mma_f16_2(a[0], a[1], gw[1], b);
+                        }
+                        mma_f16_2(n[0], n[1], zw[0], b);
+                        mma_f16_2(n[0], n[1], zw[1], b);
+                        load_b_t(b, w + DR_PIECE, kt * 16, cq, o);
+                        if (p.out) mma_f16_2(a[0], a[1], gw[0], b);
+                        mma_f16_2(n[0], n[1], zw[0], b);
+                    }
+                }
+                if (sm.uneven[0] && p.out) {
+#pragma unroll
+                    for (int i = 0; i < (EXACT ? 1 : 2); ++i) scale_f16(go[i], __float2half2_rn(sm.factor[0][at]));
+                }
+                if (sm.uneven[1]) {
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) scale_f16(zt[i], __float2half2_rn(sm.factor[1][at]));
                 }
 #pragma unroll
                 for (int j = 0; j < NP; ++j) {
-                    const int first = ch * (DK / 2) + j * 16, block = first / 64 * DR_PIECE, jj = first % 64 / 16;
+                    const int first = cq * (DK / 4) + j * 16, block = first / 64 * DR_PIECE, jj = first % 64 / 16;
                     uint32_t b[4];
                     load_b_t(b, s + block, kt * 16, jj, o);
                     if (p.out) {
-                        mma_f16_2(dq[2 * j], dq[2 * j + 1], gs[0], b);
-                        if constexpr (!EXACT) mma_f16_2(dq[2 * j], dq[2 * j + 1], gs[1], b);
+                        mma_f16_2(dq[2 * j], dq[2 * j + 1], go[0], b);
+                        if constexpr (!EXACT) mma_f16_2(dq[2 * j], dq[2 * j + 1], go[1], b);
                     }
-                    mma_f16_2(er[2 * j], er[2 * j + 1], zs[0], b);
-                    mma_f16_2(er[2 * j], er[2 * j + 1], zs[1], b);
+                    mma_f16_2(er[2 * j], er[2 * j + 1], zt[0], b);
+                    mma_f16_2(er[2 * j], er[2 * j + 1], zt[1], b);
                     load_b_t(b, s + NB * DR_PIECE + block, kt * 16, jj, o);
-                    if (p.out) mma_f16_2(dq[2 * j], dq[2 * j + 1], gs[0], b);
-                    mma_f16_2(er[2 * j], er[2 * j + 1], zs[0], b);
+                    if (p.out) mma_f16_2(dq[2 * j], dq[2 * j + 1], go[0], b);
+                    mma_f16_2(er[2 * j], er[2 * j + 1], zt[0], b);
                     load_b_t(b, x + block, kt * 16, jj, o);
                     mma_f16_2(wr[2 * j], wr[2 * j + 1], aw[0], b);
                     mma_f16_2(wr[2 * j], wr[2 * j + 1], aw[1], b);
                     load_b_t(b, x + NB * DR_PIECE + block, kt * 16, jj, o);
                     mma_f16_2(wr[2 * j], wr[2 * j + 1], aw[0], b);
                 }
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {  // 32 of the other tokens, if there are earlier ones among them
-                    if (ch * 2 + j > rb) break;
-                    uint32_t b[4];
-                    load_b_t(b, w, kt * 16, ch * 2 + j, o);
-                    if (p.out) {
-                        mma_f16_2(a[2 * j], a[2 * j + 1], gw[0], b);
-                        if constexpr (!EXACT) mma_f16_2(a[2 * j], a[2 * j + 1], gw[1], b);
-                    }
-                    mma_f16_2(n[2 * j], n[2 * j + 1], zw[0], b);
-                    mma_f16_2(n[2 * j], n[2 * j + 1], zw[1], b);
-                    load_b_t(b, w + DR_PIECE, kt * 16, ch * 2 + j, o);
-                    if (p.out) mma_f16_2(a[2 * j], a[2 * j + 1], gw[0], b);
-                    mma_f16_2(n[2 * j], n[2 * j + 1], zw[0], b);
+            }
+            // <S0, X> of the step's 32 rows: the diagonal of S0 X^T, 16 rows and 16 key columns a warp
+            if (warp < DK / 8) {
+                const int kt = warp & 1, first = (warp >> 1) * 16;
+                const uint32_t at = v * 2 + kt, block = first / 64 * DR_PIECE;
+                if (at < groups) {
+                    float d[2][4] = {};  // the diagonal's 8 x 8 blocks
+                    uint32_t s0[4], s1[4], x0[4], x1[4];
+                    const int j = first % 64 / 16;
+                    const uint32_t rows = ((2 * j + (lane >> 4)) ^ (lane & 7)) * 16 + (lane & 15) * BLOCK_ROW,
+                                   cols = ((2 * j + (lane >> 3 & 1)) ^ (lane & 7)) * 16 + ((lane & 7) + (lane >> 4) * 8) * BLOCK_ROW;
+                    ldmatrix4(s0, s + block + kt * 2048 + rows), ldmatrix4(s1, s + NB * DR_PIECE + block + kt * 2048 + rows);
+                    ldmatrix4(x0, x + block + kt * 2048 + cols), ldmatrix4(x1, x + NB * DR_PIECE + block + kt * 2048 + cols);
+                    mma_f16_2(d[0], d[1], s0, x0), mma_f16_2(d[0], d[1], s1, x0), mma_f16_2(d[0], d[1], s0, x1);
+                    // rows g (d[0]) and g + 8 (d[1]) against columns col, col + 1 of their block
+                    const float mine = g == col ? d[0][0] + d[1][2] : g == col + 1 ? d[0][1] + d[1][3] : 0.0f;
+                    sx = fmaf(mine, sm.own[0][at] * sm.own[1][at], sx);
                 }
-                // <S0, X>
-                const float both = sm.own[0][at] * sm.own[1][at];
-                float sum = 0.0f;
-#pragma unroll
-                for (int i = 0; i < NB * 16 * 32 / DR_GRAD_THREADS; ++i) {
-                    const uint32_t word = i * DR_GRAD_THREADS + t, off = word / 512 * DR_PIECE + kt * 2048 + word % 512 * 4;
-                    const float2 s0 = unpack_f16(lds32(s + off)), s1 = unpack_f16(lds32(s + NB * DR_PIECE + off)),
-                                 x0 = unpack_f16(lds32(x + off)), x1 = unpack_f16(lds32(x + NB * DR_PIECE + off));
-                    sum = fmaf(s0.x + s1.x, x0.x + x1.x, sum);
-                    sum = fmaf(s0.y + s1.y, x0.y + x1.y, sum);
-                }
-                sx = fmaf(sum, both, sx);
-                // w.z of two tokens a lane, 2 of the value dimensions a warp
-                const float wz = sm.own[2][at] * sm.own[3][at];
-                float d0 = 0.0f, d1 = 0.0f;
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const uint32_t off = block_at(kt * 16 + warp * 2 + i, lane * 2);
-                    const float2 w0 = unpack_f16(lds32(w + off)), w1 = unpack_f16(lds32(w + DR_PIECE + off)), z0 = unpack_f16(lds32(z + off)),
-                                 z1 = unpack_f16(lds32(z + DR_PIECE + off));
-                    d0 = fmaf(w0.x + w1.x, z0.x + z1.x, d0);
-                    d1 = fmaf(w0.y + w1.y, z0.y + z1.y, d1);
-                }
-                db0 = fmaf(d0, wz, db0), db1 = fmaf(d1, wz, db1);
             }
         }
+        // dbeta_i = w_i.z_i is the diagonal of n
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int m = 0; m < 4; ++m)
+                if (cq * 16 + j * 8 + col + (m & 1) == (int)token + (m >> 1) * 8) sm.dbeta[token + (m >> 1) * 8] = n[j][m] * sm.back[4];
         // scale D dA and D dN: dA_ij = beta_j a_ij, dN_ij = -beta_i beta_j n_ij
         float most_a = 0.0f, most_n = 0.0f;
         {
             const float back_a = sm.back[3] * sh.scale, back_n = -sm.back[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
+            for (int j = 0; j < 2; ++j) {
+                if (cq > rb) break;  // zeros
 #pragma unroll
                 for (int m = 0; m < 4; ++m) {
-                    const int i = token + (m >> 1) * 8, cc = ch * 32 + j * 8 + col + (m & 1);
-                    const float d = cc <= i ? expf((sm.gates.total[i] - sm.gates.total[cc]) + (sm.gates.rest[i] - sm.gates.rest[cc])) * sm.gates.beta[cc] : 0.0f;
+                    const int i = token + (m >> 1) * 8, cc = cq * 16 + j * 8 + col + (m & 1);
+                    const float d = __expf((sm.gates.total[i] - sm.gates.total[cc]) + (sm.gates.rest[i] - sm.gates.rest[cc])) * sm.gates.beta[cc];
                     a[j][m] = cc <= i ? a[j][m] * back_a * d : 0.0f;
                     n[j][m] = cc < i ? n[j][m] * back_n * d * sm.gates.beta[i] : 0.0f;
                     most_a = fmaxf(most_a, fabsf(a[j][m])), most_n = fmaxf(most_n, fabsf(n[j][m]));
                 }
+            }
         }
         most_a = warp_max(most_a), most_n = warp_max(most_n);
         if (lane == 0) sm.most[0][warp] = most_a, sm.most[1][warp] = most_n;
-        if ((warp & 1) == 0) *(float2*)&sm.dbeta[warp >> 1][lane * 2] = make_float2(db0, db1);
         __syncthreads();
-        if ((warp & 1) == 1) sm.dbeta[warp >> 1][lane * 2] += db0, sm.dbeta[warp >> 1][lane * 2 + 1] += db1;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) most_a = fmaxf(most_a, sm.most[0][i]), most_n = fmaxf(most_n, sm.most[1][i]);
+        for (int i = 0; i < 16; ++i) most_a = fmaxf(most_a, sm.most[0][i]), most_n = fmaxf(most_n, sm.most[1][i]);
         const Scale sa = scale_for(most_a), sn = scale_for(most_n);
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int j = 0; j < 2; ++j)
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
                 uint32_t hi, lo;
-                const uint32_t off = block_at(token + half * 8, ch * 32 + j * 8 + col);
+                const uint32_t off = block_at(token + half * 8, cq * 16 + j * 8 + col);
                 split_f16(a[j][half * 2], a[j][half * 2 + 1], sa.by, hi, lo);
                 sts32(da + off, hi), sts32(da + DR_BLOCK + off, lo);
                 split_f16(n[j][half * 2], n[j][half * 2 + 1], sn.by, hi, lo);
@@ -1221,7 +1281,7 @@ dr_gradient_kernel(const __grid_constant__ DrGradient p) {
             const float fq = g0 * sh.scale * sm.back[0] * into_q, fe = -g0 * b * sm.back[1] * into_n, fw = sm.gates.e[i] * b * sm.back[2];
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
-                const int first = ch * (DK / 2) + j * 8 + col;
+                const int first = cq * (DK / 4) + j * 8 + col;
                 const uint32_t off = first / 64 * DR_BLOCK + block_at(i, first % 64);
                 float2 kv = unpack_f16(lds32(k + off));
                 if constexpr (PLANES == 2) {
@@ -1258,7 +1318,7 @@ dr_gradient_kernel(const __grid_constant__ DrGradient p) {
                 }
 #pragma unroll
                 for (int j = 0; j < NP; ++j) {
-                    const int first = ch * (DK / 2) + j * 16, block = first / 64 * DR_BLOCK, jj = first % 64 / 16;
+                    const int first = cq * (DK / 4) + j * 16, block = first / 64 * DR_BLOCK, jj = first % 64 / 16;
 #pragma unroll
                     for (int i = 0; i < PLANES; ++i) {
                         uint32_t b[4];
@@ -1281,7 +1341,7 @@ dr_gradient_kernel(const __grid_constant__ DrGradient p) {
             float dot = 0.0f;
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
-                const int first = ch * (DK / 2) + j * 8 + col;
+                const int first = cq * (DK / 4) + j * 8 + col;
                 const uint32_t off = first / 64 * DR_BLOCK + block_at(i, first % 64);
                 float kv[2] = {0, 0}, qv[2] = {0, 0};
 #pragma unroll
@@ -1303,7 +1363,7 @@ dr_gradient_kernel(const __grid_constant__ DrGradient p) {
                 dot += __shfl_xor_sync(0xffffffffu, dot, i2);
                 carry[half] += __shfl_xor_sync(0xffffffffu, carry[half], i2);
             }
-            if ((lane & 3) == 0) sm.dot[ch][i] = dot, sm.carry[ch][i] = carry[half];
+            if ((lane & 3) == 0) sm.dot[cq][i] = dot, sm.carry[cq][i] = carry[half];
         }
         sx = warp_reduce<OpSum>(sx);
         if (lane == 0) sm.sx[warp] = sx;
@@ -1315,7 +1375,7 @@ dr_gradient_kernel(const __grid_constant__ DrGradient p) {
                 const uint64_t to = ((c.row + i) * sh.key_heads + hk) * sh.key_dim;
 #pragma unroll
                 for (int j = 0; j < NT; ++j) {
-                    const uint32_t cc = ch * (DK / 2) + j * 8 + col;
+                    const uint32_t cc = cq * (DK / 4) + j * 8 + col;
                     const float* const fq = SHARED ? all_q[SHARED ? j : 0] : dq[j];
                     const float* const fk = SHARED ? all_k[SHARED ? j : 0] : er[j];
                     dr_store_pair((T*)p.dq + to, cc, sh.key_dim, p.pairs_k, fq[half * 2], fq[half * 2 + 1]);
@@ -1329,10 +1389,10 @@ dr_gradient_kernel(const __grid_constant__ DrGradient p) {
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 const int r = lane * 2 + j;
-                d[j] = (double)sm.dot[0][r] + sm.dot[1][r];
-                extra += (double)sm.carry[0][r] + sm.carry[1][r];
+                d[j] = ((double)sm.dot[0][r] + sm.dot[1][r]) + ((double)sm.dot[2][r] + sm.dot[3][r]);
+                extra += ((double)sm.carry[0][r] + sm.carry[1][r]) + ((double)sm.carry[2][r] + sm.carry[3][r]);
             }
-            if (lane < 8) extra += (double)sm.sx[lane] * sm.gates.g[DR_CHUNK - 1];
+            if (lane < 16) extra += (double)sm.sx[lane] * sm.gates.g[DR_CHUNK - 1];
 #pragma unroll
             for (int i = 16; i > 0; i >>= 1) extra += __shfl_xor_sync(0xffffffffu, extra, i);
             double sum = d[0] + d[1];  // from the lane's rows to the end
@@ -1348,7 +1408,7 @@ dr_gradient_kernel(const __grid_constant__ DrGradient p) {
                 if (r < c.rows) {
                     const uint64_t to = (c.row + r) * sh.heads + h;
                     if (p.ddecay) p.ddecay[to] = (float)v[j];
-                    p.dbeta[to] = (sm.dbeta[0][r] + sm.dbeta[1][r]) + (sm.dbeta[2][r] + sm.dbeta[3][r]);
+                    p.dbeta[to] = sm.dbeta[r];
                 }
             }
         }

@@ -85,6 +85,12 @@ __device__ __forceinline__ Scale scale_for(float most) {
     const int field = e == 0 ? 127 : min(268 - e, 172);
     return Scale{__int_as_float(field << 23), __int_as_float((254 - field) << 23)};
 }
+// With an exponent that is a multiple of 8, so that most * by is in [2^7, 2^15): matrices of like size share it.
+__device__ __forceinline__ Scale coarse_scale_for(float most) {
+    const int e = __float_as_int(most) >> 23 & 255;
+    const int field = e == 0 ? 127 : min((268 - e - 127 + 1024) / 8 * 8 - 1024 + 127, 167);
+    return Scale{__int_as_float(field << 23), __int_as_float((254 - field) << 23)};
+}
 __device__ __forceinline__ float warp_max(float v) {  // of values >= 0
     return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(v)));
 }
