@@ -96,9 +96,9 @@ __device__ __forceinline__ void dr_store(uint8_t* image, uint32_t blocks, uint32
 
 // ---- what does not depend on the state ------------------------------------------------------------
 constexpr int DR_PREPARE_THREADS = 256;  // warps: 4 blocks of 16 rows x 2 halves of the columns
-constexpr int DR_PITCH = 68;
+constexpr int DR_PITCH = 68, DR_TMP_PITCH = 40;
 struct DrInvert {
-    float m[64 * DR_PITCH], inv[64 * DR_PITCH], tmp[32 * 36];
+    float m[64 * DR_PITCH], inv[64 * DR_PITCH], tmp[32 * DR_TMP_PITCH];
 };
 // The keys' blocks, then a head's triangular matrix and its inverse, then the blocks of the head's unit, one after the other
 // in the same memory.
@@ -113,10 +113,39 @@ struct DrPrepareSmem {
     float most[2][8];
 };
 
-__device__ __forceinline__ void dr_fma4(float (&v)[4], float a, const float* b) {
-    const float4 x = *(const float4*)b;
-    v[0] = fmaf(a, x.x, v[0]), v[1] = fmaf(a, x.y, v[1]), v[2] = fmaf(a, x.z, v[2]), v[3] = fmaf(a, x.w, v[3]);
+// c (16 x 8) += a (16 x 8 steps, rows `ap` floats apart) b (8 steps x 8, rows `bp` apart), all float32 in shared memory: each
+// factor as two tf32 (hi hi + hi lo + lo hi: 2^-21 is left out), which have float32's range.
+__device__ __forceinline__ uint32_t dr_tf32(float v) {
+    uint32_t r;
+    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(v));
+    return r;
 }
+__device__ __forceinline__ void dr_mma_tf32(float (&c)[4], const uint32_t (&a)[4], const uint32_t (&b)[2]) {
+    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
+}
+template <int STEPS>
+__device__ __forceinline__ void dr_product(float (&c)[4], const float* a, int ap, const float* b, int bp, int lane) {
+    const int g = lane >> 2, t = lane & 3;
+    a += g * ap + t, b += t * bp + g;
+#pragma unroll
+    for (int k = 0; k < STEPS; ++k) {
+        const float av[4] = {a[k * 8], a[k * 8 + 8 * ap], a[k * 8 + 4], a[k * 8 + 8 * ap + 4]}, bv[2] = {b[k * 8 * bp], b[(k * 8 + 4) * bp]};
+        uint32_t ah[4], al[4], bh[2], bl[2];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) ah[i] = dr_tf32(av[i]), al[i] = dr_tf32(av[i] - __uint_as_float(ah[i]));
+#pragma unroll
+        for (int i = 0; i < 2; ++i) bh[i] = dr_tf32(bv[i]), bl[i] = dr_tf32(bv[i] - __uint_as_float(bh[i]));
+        dr_mma_tf32(c, ah, bl), dr_mma_tf32(c, al, bh), dr_mma_tf32(c, ah, bh);
+    }
+}
+__device__ __forceinline__ void dr_put(float* to, int pitch, const float (&c)[4], float by, int lane) {
+    to += (lane >> 2) * pitch + (lane & 3) * 2;
+    *(float2*)to = make_float2(c[0] * by, c[1] * by);
+    *(float2*)(to + 8 * pitch) = make_float2(c[2] * by, c[3] * by);
+}
+
 // inv = (I + m)^-1 of a strictly lower triangular m: the 16 x 16 blocks of the diagonal by substitution, a column a
 // lane, then blocks below from ones above: [X 0; -Y m21 X, Y].
 __device__ __forceinline__ void dr_invert(DrInvert& s) {
@@ -148,46 +177,29 @@ __device__ __forceinline__ void dr_invert(DrInvert& s) {
         }
     }
     __syncthreads();
-    {
-        const int half = t >> 7, b = half * 32, r = (t & 127) >> 3, c = (t & 7) * 2;  // blocks (16, 0) and (48, 32)
-        float v0 = 0.0f, v1 = 0.0f;
-#pragma unroll
-        for (int k = 0; k < 16; ++k) {
-            const float a = s.m[(b + 16 + r) * DR_PITCH + b + k];
-            const float2 x = *(const float2*)&s.inv[(b + k) * DR_PITCH + b + c];
-            v0 = fmaf(a, x.x, v0), v1 = fmaf(a, x.y, v1);
+    {  // blocks (16, 0) and (48, 32): 8 of their columns a warp
+        const int b = (warp >> 1 & 1) * 32, n = (warp & 1) * 8;
+        float* const tmp = s.tmp + (warp >> 1 & 1) * 16 * DR_TMP_PITCH + n;
+        if (warp < 4) {
+            float c[4] = {0, 0, 0, 0};
+            dr_product<2>(c, &s.m[(b + 16) * DR_PITCH + b], DR_PITCH, &s.inv[b * DR_PITCH + b + n], DR_PITCH, lane);
+            dr_put(tmp, DR_TMP_PITCH, c, 1.0f, lane);
+            __syncwarp();  // a column of the product needs its own columns only
+            c[0] = c[1] = c[2] = c[3] = 0.0f;
+            dr_product<2>(c, &s.inv[(b + 16) * DR_PITCH + b + 16], DR_PITCH, tmp, DR_TMP_PITCH, lane);
+            dr_put(&s.inv[(b + 16) * DR_PITCH + b + n], DR_PITCH, c, -1.0f, lane);
         }
-        *(float2*)&s.tmp[(half * 16 + r) * 36 + c] = make_float2(v0, v1);
-        __syncthreads();
-        v0 = v1 = 0.0f;
-#pragma unroll
-        for (int k = 0; k < 16; ++k) {
-            const float a = s.inv[(b + 16 + r) * DR_PITCH + b + 16 + k];
-            const float2 x = *(const float2*)&s.tmp[(half * 16 + k) * 36 + c];
-            v0 = fmaf(a, x.x, v0), v1 = fmaf(a, x.y, v1);
-        }
-        *(float2*)&s.inv[(b + 16 + r) * DR_PITCH + b + c] = make_float2(-v0, -v1);
     }
     __syncthreads();
-    {
-        const int r = t >> 3, c = (t & 7) * 4;  // block (32, 0)
-        float v[4] = {0, 0, 0, 0};
-#pragma unroll 4
-        for (int k = 0; k < 32; k += 4) {
-            const float4 a = *(const float4*)&s.m[(32 + r) * DR_PITCH + k];
-            const float* const b = &s.inv[k * DR_PITCH + c];
-            dr_fma4(v, a.x, b), dr_fma4(v, a.y, b + DR_PITCH), dr_fma4(v, a.z, b + 2 * DR_PITCH), dr_fma4(v, a.w, b + 3 * DR_PITCH);
-        }
-        *(float4*)&s.tmp[r * 36 + c] = make_float4(v[0], v[1], v[2], v[3]);
+    {  // block (32, 0): 16 x 8 of it a warp
+        const int r = (warp >> 2) * 16, n = (warp & 3) * 8;
+        float c[4] = {0, 0, 0, 0};
+        dr_product<4>(c, &s.m[(32 + r) * DR_PITCH], DR_PITCH, &s.inv[n], DR_PITCH, lane);
+        dr_put(s.tmp + r * DR_TMP_PITCH + n, DR_TMP_PITCH, c, 1.0f, lane);
         __syncthreads();
-        v[0] = v[1] = v[2] = v[3] = 0.0f;
-#pragma unroll 4
-        for (int k = 0; k < 32; k += 4) {
-            const float4 a = *(const float4*)&s.inv[(32 + r) * DR_PITCH + 32 + k];
-            const float* const b = &s.tmp[k * 36 + c];
-            dr_fma4(v, a.x, b), dr_fma4(v, a.y, b + 36), dr_fma4(v, a.z, b + 72), dr_fma4(v, a.w, b + 108);
-        }
-        *(float4*)&s.inv[(32 + r) * DR_PITCH + c] = make_float4(-v[0], -v[1], -v[2], -v[3]);
+        c[0] = c[1] = c[2] = c[3] = 0.0f;
+        dr_product<4>(c, &s.inv[(32 + r) * DR_PITCH + 32], DR_PITCH, s.tmp + n, DR_TMP_PITCH, lane);
+        dr_put(&s.inv[(32 + r) * DR_PITCH + n], DR_PITCH, c, -1.0f, lane);
     }
     __syncthreads();
 }
@@ -480,36 +492,17 @@ struct DrChain {
     const void* values;  // V forward, dO backward (null: zeros)
     uint64_t value_stride;
     bool wide;           // rows of values are whole 16-byte pieces
-    const float* from;   // states before the first chunk (forward), gradients of the last ones (backward)
-    float* to;           // the states after; gradients of the first
+    // States before the first chunk (forward), gradients of the last ones (backward), and the states after (gradients of
+    // the first), of the sequences' parts one after the other; parts > 1: `to` is of whole sequences, the end part's.
+    const float* from;
+    float* to;
+    uint32_t parts;      // of a sequence, with about as many chunks each
+    float *local, *map;  // DR_STATES: what a part makes of no state, and of each row of the unit matrix
     void* out;           // forward
     uint64_t out_stride;
     DrImage states, kept;  // S0 and w (forward, if saved), X and z (backward)
     float* back_values;    // backward: inverse scales of dO
 };
-
-// The state's 16 rows of this warp, from or to float32 [value_dim][key_dim].
-template <int NT>
-__device__ __forceinline__ void dr_state_in(float (&s)[NT][4], const float* from, uint32_t row, uint32_t rows, uint32_t cols, int col) {
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const uint32_t r = row + (j >> 1) * 8, c = n * 8 + col + (j & 1);
-            s[n][j] = from && r < rows && c < cols ? from[(uint64_t)r * cols + c] : 0.0f;
-        }
-}
-template <int NT>
-__device__ __forceinline__ void dr_state_out(const float (&s)[NT][4], float by, float* to, uint32_t row, uint32_t rows, uint32_t cols, int col) {
-    if (!to) return;
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const uint32_t r = row + (j >> 1) * 8, c = n * 8 + col + (j & 1);
-            if (r < rows && c < cols) to[(uint64_t)r * cols + c] = s[n][j] * by;
-        }
-}
 
 template <typename T>
 __device__ __forceinline__ void dr_store_pair(T* to, uint32_t col, uint32_t cols, bool pairs, float x, float y) {
@@ -523,8 +516,13 @@ __device__ __forceinline__ void dr_store_pair(T* to, uint32_t col, uint32_t cols
     }
 }
 
+// What a chain writes: everything, or only the states at the end of its part, for sequences in parts: part p's states
+// are those before it times a key_dim x key_dim matrix plus what it makes of none.  The matrix comes from the same
+// recurrence, with the unit matrix's rows for a state and without values.
+enum { DR_ALL, DR_STATES };
+
 // What both directions share: where a CTA's warps are, the copies of the chunks' images, and products with them.
-template <typename T, int DK, int WARPS>
+template <typename T, int DK, int WARPS, bool BACKWARD, int WHAT>
 struct DrChainCta {
     using Smem = DrChainSmem<T, DK, WARPS>;
     static constexpr int PLANES = Smem::PLANES, NB = DK / 64, NT = DK / 8, STAGES = Smem::STAGES, KEYS = DR_KEYS<DK, PLANES>;
@@ -532,29 +530,77 @@ struct DrChainCta {
     Smem& sm;
     const int lane, warp, g, col;
     const LaneOffsets o;
-    uint32_t h, hk, seq, v0, live, row, limit;
-    uint64_t start, end, base, state;
-    uint32_t chunks;
-    bool ok = true;
+    uint32_t h, hk, seq, v0, live, row, limit, dim;  // dim: rows of the state
+    uint64_t start, end, base;
+    uint32_t first, chunks;  // the part's
+    const T* values;
+    bool unit_rows = false, ok = true;
+    const float* from;
+    float* to;
 
     __device__ __forceinline__ DrChainCta(const DrChain& p_, Smem& sm_)
         : p(p_), sm(sm_), lane(threadIdx.x & 31), warp(threadIdx.x >> 5), g((threadIdx.x & 31) >> 2), col((threadIdx.x & 3) * 2),
           o(threadIdx.x & 31) {
         const DrShape& sh = p.sh;
-        const uint32_t slices = (sh.value_dim + WARPS * 16 - 1) / (WARPS * 16);
-        h = blockIdx.x / slices % sh.heads, seq = blockIdx.x / slices / sh.heads;
-        hk = h / (sh.heads / sh.key_heads), v0 = blockIdx.x % slices * WARPS * 16;
-        live = min((uint32_t)WARPS, (sh.value_dim - v0 + 15) / 16);
+        const uint32_t value_slices = (sh.value_dim + WARPS * 16 - 1) / (WARPS * 16),
+                       slices = value_slices + (WHAT == DR_STATES ? (sh.key_dim + WARPS * 16 - 1) / (WARPS * 16) : 0);
+        const uint32_t parts = WHAT == DR_STATES ? p.parts - 1 : p.parts;  // nothing follows on the end part
+        uint32_t slice = blockIdx.x % slices, rest = blockIdx.x / slices;
+        h = rest % sh.heads, rest /= sh.heads;
+        const uint32_t part = rest % parts + (WHAT == DR_STATES && BACKWARD ? 1 : 0);
+        seq = rest / parts, hk = h / (sh.heads / sh.key_heads);
+        unit_rows = slice >= value_slices;
+        if (unit_rows) slice -= value_slices;
+        dim = unit_rows ? sh.key_dim : sh.value_dim;
+        v0 = slice * WARPS * 16;
+        live = min((uint32_t)WARPS, (dim - v0 + 15) / 16);
         row = v0 + warp * 16 + g;
         start = sh.start(seq), end = min(sh.start(seq + 1), sh.rows), base = sh.base(seq);
-        chunks = end > start ? (uint32_t)((end - start + DR_CHUNK - 1) / DR_CHUNK) : 0;
-        state = ((uint64_t)seq * sh.heads + h) * sh.value_dim * sh.key_dim;
+        const uint32_t all = end > start ? (uint32_t)((end - start + DR_CHUNK - 1) / DR_CHUNK) : 0, each = (all + p.parts - 1) / p.parts;
+        first = min(part * each, all), chunks = min(all - first, each);
+        values = unit_rows ? nullptr : (const T*)p.values;
+        const uint64_t state = (uint64_t)sh.value_dim * sh.key_dim, stream = (uint64_t)seq * sh.heads + h, piece = stream * p.parts + part;
+        if (WHAT == DR_STATES) {
+            from = nullptr;
+            to = unit_rows ? p.map + piece * sh.key_dim * sh.key_dim : p.local + piece * state;
+        } else {
+            from = p.from ? p.from + piece * state : nullptr;
+            to = p.to && part == (BACKWARD ? 0 : p.parts - 1) ? p.to + stream * state : nullptr;
+        }
         limit = g_spin_limit;
         if (threadIdx.x == 0) {
             for (int i = 0; i < STAGES; ++i) mbar_init(&sm.full[i], 1), mbar_init(&sm.empty[i], live);
             fence_mbar_init();
         }
         __syncthreads();
+    }
+    __device__ __forceinline__ uint32_t order(uint32_t it) const { return first + (BACKWARD ? chunks - 1 - it : it); }
+    // The first images and values, and the state that they meet.
+    __device__ __forceinline__ void open(float (&s)[NT][4]) {
+        if (warp == 0 && lane == 0)
+            for (uint32_t i = 0; i < (uint32_t)STAGES && i < chunks; ++i) load(i, order(i));
+        __syncwarp();
+        if (chunks) load_values(0, order(0));
+        cp_async_commit();
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t r = row + (j >> 1) * 8, c = n * 8 + col + (j & 1);
+                s[n][j] = from && r < dim && c < p.sh.key_dim ? from[(uint64_t)r * p.sh.key_dim + c] : 0.0f;
+                if (WHAT == DR_STATES && unit_rows && r == c && r < dim) s[n][j] = 1.0f;
+            }
+    }
+    __device__ __forceinline__ void close(const float (&s)[NT][4], float by) {
+        if (!ok) set_error(LCPP_ERR_LOOKBACK_TIMEOUT);
+        if (!to) return;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t r = row + (j >> 1) * 8, c = n * 8 + col + (j & 1);
+                if (r < dim && c < p.sh.key_dim) to[(uint64_t)r * p.sh.key_dim + c] = s[n][j] * by;
+            }
     }
     __device__ __forceinline__ uint64_t unit(uint32_t chunk) const { return (base + chunk) * p.sh.heads + h; }
     __device__ __forceinline__ uint32_t rows(uint32_t chunk) const {
@@ -566,13 +612,12 @@ struct DrChainCta {
         bulk_load(sm.stage[stage] + 2 * KEYS, p.units + unit(chunk) * DR_UNIT, DR_UNIT, &sm.full[stage]);
     }
     __device__ __forceinline__ void load_values(uint32_t buffer, uint32_t chunk) {
-        if (!p.values) return;
-        const T* const from = (const T*)p.values + (start + (uint64_t)chunk * DR_CHUNK) * p.value_stride + (uint64_t)h * p.sh.value_dim + v0 + warp * 16;
-        dr_raw_load<T>(smem_u32(sm.raw[warp][buffer]), from, p.value_stride, rows(chunk), (int)(p.sh.value_dim - v0) - warp * 16, p.wide, lane);
+        if (!values) return;
+        const T* const at = values + (start + (uint64_t)chunk * DR_CHUNK) * p.value_stride + (uint64_t)h * p.sh.value_dim + v0 + warp * 16;
+        dr_raw_load<T>(smem_u32(sm.raw[warp][buffer]), at, p.value_stride, rows(chunk), (int)(p.sh.value_dim - v0) - warp * 16, p.wide, lane);
     }
-    // Step `it` is chunk order(it).  Waits for its images, then for its values, and starts the next ones.
-    template <typename F>
-    __device__ __forceinline__ bool begin(uint32_t it, F&& order) {
+    // Step `it` is chunk order(it).  Waits for its values and images, and asks for the next values.
+    __device__ __forceinline__ bool begin(uint32_t it) {
         cp_async_wait_all();
         __syncwarp();
         if (it + 1 < chunks) load_values((it + 1) & 1, order(it + 1));
@@ -581,16 +626,14 @@ struct DrChainCta {
         return ok;
     }
     // Two stages: the next images are asked for amid a step, when the other warps have left the step before.
-    template <typename F>
-    __device__ __forceinline__ void ahead(uint32_t it, F&& order) {
+    __device__ __forceinline__ void ahead(uint32_t it) {
         if (STAGES == 2 && warp == 0 && lane == 0 && it + 1 < chunks && it >= 1) {
             if (mbar_wait(&sm.empty[(it + 1) & 1], ((it - 1) / 2) & 1, limit)) load((it + 1) & 1, order(it + 1));
             else set_error(LCPP_ERR_LOOKBACK_TIMEOUT);
         }
         __syncwarp();
     }
-    template <typename F>
-    __device__ __forceinline__ void finish(uint32_t it, F&& order) {
+    __device__ __forceinline__ void finish(uint32_t it) {
         __syncwarp();
         if (lane == 0) {
             asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&sm.empty[it % STAGES])) : "memory");
@@ -640,10 +683,11 @@ struct DrChainCta {
     }
 };
 
-template <typename T, int DK, int WARPS>
+template <typename T, int DK, int WARPS, int WHAT>
 __global__ void __launch_bounds__(WARPS * 32, 1)
 dr_forward_kernel(const __grid_constant__ DrChain p) {
-    using Cta = DrChainCta<T, DK, WARPS>;
+    using Cta = DrChainCta<T, DK, WARPS, false, WHAT>;
+    constexpr bool ALL = WHAT == DR_ALL;
     constexpr int NT = Cta::NT, NB = Cta::NB, PLANES = Cta::PLANES, KEYS = Cta::KEYS;
     constexpr bool FINE = !std::is_same_v<T, __nv_bfloat16>;  // outputs of 8 bits need one part of the state and of u (11 bits)
     extern __shared__ __align__(128) uint8_t dr_smem[];
@@ -651,27 +695,21 @@ dr_forward_kernel(const __grid_constant__ DrChain p) {
     const int lane = cta.lane, warp = cta.warp, g = cta.g, col = cta.col;
     const LaneOffsets& o = cta.o;
     if (warp >= (int)cta.live) return;
-    auto order = [](uint32_t it) { return it; };
-    if (warp == 0 && lane == 0)
-        for (uint32_t i = 0; i < (uint32_t)Cta::STAGES && i < cta.chunks; ++i) cta.load(i, i);
-    __syncwarp();
-    if (cta.chunks) cta.load_values(0, 0);
-    cp_async_commit();
     float s[NT][4];  // the state times a power of two
     float back_domain = 1.0f;
-    dr_state_in<NT>(s, p.from ? p.from + cta.state : nullptr, cta.row, p.sh.value_dim, p.sh.key_dim, col);
+    cta.open(s);
     T* const out = (T*)p.out + (uint64_t)cta.h * p.sh.value_dim;
     const bool pairs = ((uintptr_t)p.out | p.out_stride * sizeof(T) | p.sh.value_dim * sizeof(T)) % (2 * sizeof(T)) == 0;
     for (uint32_t it = 0; it < cta.chunks; ++it) {
-        if (!cta.begin(it, order)) break;
+        if (!cta.begin(it)) break;
         const uint32_t stage = smem_u32(cta.sm.stage[it % Cta::STAGES]), k = stage, q = stage + KEYS, inv = stage + 2 * KEYS,
                        rd = inv + 2 * DR_BLOCK;
         const DrGates& gt = *(const DrGates*)(cta.sm.stage[it % Cta::STAGES] + 2 * KEYS + 4 * DR_BLOCK);
-        const uint64_t unit = cta.unit(it);
+        const uint64_t unit = cta.unit(cta.order(it));
         // r = S0 K^T (value x token) and out = Q S0^T (token x value)
         float r[8][4] = {}, y[4][2][4] = {};
         const Scale ss = coarse_scale_for(max_abs(s));
-        uint8_t* const states = p.states.at ? p.states.of(unit) : nullptr;
+        uint8_t* const states = ALL && p.states.at ? p.states.of(unit) : nullptr;
         if (states) cta.keep_back(p.states.back, unit, ss.back * back_domain);
 #pragma unroll
         for (int kk = 0; kk < DK / 16; ++kk) {
@@ -680,7 +718,7 @@ dr_forward_kernel(const __grid_constant__ DrChain p) {
             if (states) cta.keep_state(states, hi, lo, kk);
             cta.times_keys(r, hi, lo, k, kk);
 #pragma unroll
-            for (int i = 0; i < PLANES; ++i)
+            for (int i = 0; ALL && i < PLANES; ++i)
 #pragma unroll
                 for (int m = 0; m < 4; ++m) {
                     uint32_t a[4];
@@ -695,8 +733,8 @@ dr_forward_kernel(const __grid_constant__ DrChain p) {
         const float back_r = -back_state * gt.back_k;
 #pragma unroll
         for (int n = 0; n < 4; ++n) {
-            float v[4][2];
-            dr_raw_get<T>(v, raw, n * 16, lane);
+            float v[4][2] = {};
+            if (ALL || cta.values) dr_raw_get<T>(v, raw, n * 16, lane);
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
                 const float2 gate = *(const float2*)&gt.g[n * 16 + (x >> 1) * 8 + col];
@@ -704,7 +742,7 @@ dr_forward_kernel(const __grid_constant__ DrChain p) {
                 d[0] = fmaf(gate.x * back_r, d[0], v[x][0]), d[1] = fmaf(gate.y * back_r, d[1], v[x][1]);
             }
         }
-        cta.ahead(it, order);
+        cta.ahead(it);
         // w = r inverse^T
         const Scale sr = scale_for(max_abs(r));
         float w[8][4] = {};
@@ -723,7 +761,7 @@ dr_forward_kernel(const __grid_constant__ DrChain p) {
             }
         }
         const float back_w = sr.back * gt.back_inverse;
-        if (p.kept.at) {
+        if (ALL && p.kept.at) {
             const Scale sw = coarse_scale_for(max_abs(w));
             uint8_t* const kept = p.kept.of(unit);
             cta.keep_back(p.kept.back, unit, sw.back * back_w);
@@ -739,47 +777,48 @@ dr_forward_kernel(const __grid_constant__ DrChain p) {
             const float2 b = *(const float2*)&gt.beta[n * 8 + col];
             w[n][0] *= b.x * back_w, w[n][1] *= b.y * back_w, w[n][2] *= b.x * back_w, w[n][3] *= b.y * back_w;
         }
-        // out = scale g out + A u
-        const Scale su = scale_for(max_abs(w));
-        {
-            const float by = p.sh.scale * back_state * gt.back_q, into = su.by * __frcp_rn(gt.back_read);
+        if constexpr (ALL) {  // out = scale g out + A u
+            const Scale su = scale_for(max_abs(w));
+            {
+                const float by = p.sh.scale * back_state * gt.back_q, into = su.by * __frcp_rn(gt.back_read);
 #pragma unroll
-            for (int m = 0; m < 4; ++m) {
-                const float g0 = gt.g[m * 16 + g] * by * into, g1 = gt.g[m * 16 + g + 8] * by * into;
+                for (int m = 0; m < 4; ++m) {
+                    const float g0 = gt.g[m * 16 + g] * by * into, g1 = gt.g[m * 16 + g + 8] * by * into;
 #pragma unroll
-                for (int n = 0; n < 2; ++n) y[m][n][0] *= g0, y[m][n][1] *= g0, y[m][n][2] *= g1, y[m][n][3] *= g1;
+                    for (int n = 0; n < 2; ++n) y[m][n][0] *= g0, y[m][n][1] *= g0, y[m][n][2] *= g1, y[m][n][3] *= g1;
+                }
             }
-        }
 #pragma unroll
-        for (int kt = 0; kt < 4; ++kt) {
-            uint32_t hi[4], lo[4];
-            split_block(w[2 * kt], w[2 * kt + 1], su.by, hi, lo);
+            for (int kt = 0; kt < 4; ++kt) {
+                uint32_t hi[4], lo[4];
+                split_block(w[2 * kt], w[2 * kt + 1], su.by, hi, lo);
 #pragma unroll
-            for (int m = kt; m < 4; ++m) {
-                uint32_t a[4];
-                load_a(a, rd, m * 16, kt, o);
-                mma_f16(y[m][0], a, hi[0], hi[2]), mma_f16(y[m][1], a, hi[1], hi[3]);
-                if constexpr (FINE) {
-                    mma_f16(y[m][0], a, lo[0], lo[2]), mma_f16(y[m][1], a, lo[1], lo[3]);
-                    load_a(a, rd + DR_BLOCK, m * 16, kt, o);
+                for (int m = kt; m < 4; ++m) {
+                    uint32_t a[4];
+                    load_a(a, rd, m * 16, kt, o);
                     mma_f16(y[m][0], a, hi[0], hi[2]), mma_f16(y[m][1], a, hi[1], hi[3]);
+                    if constexpr (FINE) {
+                        mma_f16(y[m][0], a, lo[0], lo[2]), mma_f16(y[m][1], a, lo[1], lo[3]);
+                        load_a(a, rd + DR_BLOCK, m * 16, kt, o);
+                        mma_f16(y[m][0], a, hi[0], hi[2]), mma_f16(y[m][1], a, hi[1], hi[3]);
+                    }
                 }
             }
-        }
-        {
-            const float back = su.back * gt.back_read;
-            const uint32_t have = cta.rows(it);
-            T* const first = out + (cta.start + (uint64_t)it * DR_CHUNK + g) * p.out_stride;
+            {
+                const float back = su.back * gt.back_read;
+                const uint32_t have = cta.rows(cta.order(it));
+                T* const first = out + (cta.start + (uint64_t)cta.order(it) * DR_CHUNK + g) * p.out_stride;
 #pragma unroll
-            for (int m = 0; m < 4; ++m)
+                for (int m = 0; m < 4; ++m)
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    if (m * 16 + j * 8 + g >= have) continue;
-                    T* const to = first + (m * 16 + j * 8) * p.out_stride;
+                    for (int j = 0; j < 2; ++j) {
+                        if (m * 16 + j * 8 + g >= have) continue;
+                        T* const to = first + (m * 16 + j * 8) * p.out_stride;
 #pragma unroll
-                    for (int n = 0; n < 2; ++n)
-                        dr_store_pair(to, cta.v0 + warp * 16 + n * 8 + col, p.sh.value_dim, pairs, y[m][n][2 * j] * back, y[m][n][2 * j + 1] * back);
-                }
+                        for (int n = 0; n < 2; ++n)
+                            dr_store_pair(to, cta.v0 + warp * 16 + n * 8 + col, p.sh.value_dim, pairs, y[m][n][2 * j] * back, y[m][n][2 * j + 1] * back);
+                    }
+            }
         }
         // S = g_64 S + (e u)^T K, in the domain of the product
 #pragma unroll
@@ -800,16 +839,16 @@ dr_forward_kernel(const __grid_constant__ DrChain p) {
             split_block(w[2 * kt], w[2 * kt + 1], se.by, hi, lo);
             cta.template add_outer<false>(s, hi, lo, k, kt);
         }
-        cta.finish(it, order);
+        cta.finish(it);
     }
-    if (!cta.ok) set_error(LCPP_ERR_LOOKBACK_TIMEOUT);
-    dr_state_out<NT>(s, back_domain, p.to ? p.to + cta.state : nullptr, cta.row, p.sh.value_dim, p.sh.key_dim, col);
+    cta.close(s, back_domain);
 }
 
-template <typename T, int DK, int WARPS>
+template <typename T, int DK, int WARPS, int WHAT>
 __global__ void __launch_bounds__(WARPS * 32, 1)
 dr_backward_kernel(const __grid_constant__ DrChain p) {
-    using Cta = DrChainCta<T, DK, WARPS>;
+    using Cta = DrChainCta<T, DK, WARPS, true, WHAT>;
+    constexpr bool ALL = WHAT == DR_ALL;
     constexpr int NT = Cta::NT, KEYS = Cta::KEYS;
     constexpr bool EXACT = sizeof(T) == 2;  // dO in one part
     extern __shared__ __align__(128) uint8_t dr_smem[];
@@ -817,38 +856,31 @@ dr_backward_kernel(const __grid_constant__ DrChain p) {
     const int lane = cta.lane, warp = cta.warp, col = cta.col;
     const LaneOffsets& o = cta.o;
     if (warp >= (int)cta.live) return;
-    const uint32_t last = cta.chunks - 1;
-    auto order = [last](uint32_t it) { return last - it; };
-    if (warp == 0 && lane == 0)
-        for (uint32_t i = 0; i < (uint32_t)Cta::STAGES && i < cta.chunks; ++i) cta.load(i, order(i));
-    __syncwarp();
-    if (cta.chunks) cta.load_values(0, last);
-    cp_async_commit();
     float x[NT][4];  // the state's gradient times a power of two
     float back_domain = 1.0f;
-    dr_state_in<NT>(x, p.from ? p.from + cta.state : nullptr, cta.row, p.sh.value_dim, p.sh.key_dim, col);
+    cta.open(x);
     for (uint32_t it = 0; it < cta.chunks; ++it) {
-        if (!cta.begin(it, order)) break;
+        if (!cta.begin(it)) break;
         const uint32_t stage = smem_u32(cta.sm.stage[it % Cta::STAGES]), k = stage, q = stage + KEYS, inv = stage + 2 * KEYS,
                        rd = inv + 2 * DR_BLOCK;
         const DrGates& gt = *(const DrGates*)(cta.sm.stage[it % Cta::STAGES] + 2 * KEYS + 4 * DR_BLOCK);
-        const uint64_t unit = cta.unit(order(it));
+        const uint64_t unit = cta.unit(cta.order(it));
         const uint32_t raw = smem_u32(cta.sm.raw[warp][it & 1]);
         // du = e X K^T (value x token)
         float du[8][4] = {};
         const Scale sx = coarse_scale_for(max_abs(x));
-        uint8_t* const states = p.states.of(unit);
-        cta.keep_back(p.states.back, unit, sx.back * back_domain);
+        uint8_t* const states = ALL ? p.states.of(unit) : nullptr;
+        if constexpr (ALL) cta.keep_back(p.states.back, unit, sx.back * back_domain);
 #pragma unroll
         for (int kk = 0; kk < DK / 16; ++kk) {
             uint32_t hi[4], lo[4];
             split_block(x[2 * kk], x[2 * kk + 1], sx.by, hi, lo);
-            cta.keep_state(states, hi, lo, kk);
+            if constexpr (ALL) cta.keep_state(states, hi, lo, kk);
             cta.times_keys(du, hi, lo, k, kk);
         }
         // ... + dO^T A
         float most = 0.0f, most_g = 0.0f;
-        if (p.values) {
+        if (cta.values) {
 #pragma unroll
             for (int kt = 0; kt < 4; ++kt) {
                 float v[4][2];
@@ -862,7 +894,7 @@ dr_backward_kernel(const __grid_constant__ DrChain p) {
             }
         }
         const Scale so = coarse_scale_for(warp_max(most)), sg = scale_for(warp_max(most_g) * fabsf(p.sh.scale));
-        cta.keep_back(p.back_values, unit, so.back);
+        if constexpr (ALL) cta.keep_back(p.back_values, unit, so.back);
         {
             const float back = sx.back * back_domain * gt.back_k * so.by * __frcp_rn(gt.back_read);
 #pragma unroll
@@ -871,7 +903,7 @@ dr_backward_kernel(const __grid_constant__ DrChain p) {
                 du[n][0] *= e.x * back, du[n][1] *= e.y * back, du[n][2] *= e.x * back, du[n][3] *= e.y * back;
             }
         }
-        if (p.values) {
+        if (cta.values) {
 #pragma unroll
             for (int kt = 0; kt < 4; ++kt) {
                 float v[4][2];
@@ -890,7 +922,7 @@ dr_backward_kernel(const __grid_constant__ DrChain p) {
                 }
             }
         }
-        cta.ahead(it, order);
+        cta.ahead(it);
         // z = du inverse
         const Scale sd = scale_for(max_abs(du));
         float z[8][4] = {};
@@ -909,7 +941,7 @@ dr_backward_kernel(const __grid_constant__ DrChain p) {
             }
         }
         const float back_z = sd.back * gt.back_inverse * so.back * gt.back_read;
-        {
+        if constexpr (ALL) {
             const Scale sz = coarse_scale_for(max_abs(z));
             uint8_t* const kept = p.kept.of(unit);
             cta.keep_back(p.kept.back, unit, sz.back * back_z);
@@ -922,7 +954,7 @@ dr_backward_kernel(const __grid_constant__ DrChain p) {
         }
         // X = g_64 X + (scale g dO)^T Q - (g beta z)^T K, each in the domain of its product
         float into = gt.g[DR_CHUNK - 1] * back_domain;
-        if (p.values) {
+        if (cta.values) {
             into *= sg.by * __frcp_rn(gt.back_q);
 #pragma unroll
             for (int n = 0; n < NT; ++n)
@@ -961,10 +993,49 @@ dr_backward_kernel(const __grid_constant__ DrChain p) {
             split_block(z[2 * kt], z[2 * kt + 1], sy.by, hi, lo);
             cta.template add_outer<false>(x, hi, lo, k, kt);
         }
-        cta.finish(it, order);
+        cta.finish(it);
     }
-    if (!cta.ok) set_error(LCPP_ERR_LOOKBACK_TIMEOUT);
-    dr_state_out<NT>(x, back_domain, p.to ? p.to + cta.state : nullptr, cta.row, p.sh.value_dim, p.sh.key_dim, col);
+    cta.close(x, back_domain);
+}
+
+// The states before each part of a sequence: through the parts in order, a CTA with 8 rows of a state and all its columns.
+constexpr int DR_JOIN_ROWS = 8;
+struct DrJoin {
+    const float *first, *local, *map;  // first: null for zeros
+    float* before;
+    uint32_t heads, key_dim, value_dim, parts, slices;
+    bool backward;  // the end part first
+};
+__global__ void __launch_bounds__(128) dr_join_kernel(const __grid_constant__ DrJoin p) {
+    __shared__ float s[DR_JOIN_ROWS][DR_MAX_DIM];
+    const uint32_t slice = blockIdx.x % p.slices, r0 = slice * DR_JOIN_ROWS, c = threadIdx.x;
+    const uint64_t stream = blockIdx.x / p.slices, size = (uint64_t)p.value_dim * p.key_dim;
+    float mine[DR_JOIN_ROWS];
+#pragma unroll
+    for (int i = 0; i < DR_JOIN_ROWS; ++i)
+        mine[i] = p.first && c < p.key_dim && r0 + i < p.value_dim ? p.first[stream * size + (uint64_t)(r0 + i) * p.key_dim + c] : 0.0f;
+    for (uint32_t k = 0; k < p.parts; ++k) {
+        const uint64_t piece = stream * p.parts + (p.backward ? p.parts - 1 - k : k);
+#pragma unroll
+        for (int i = 0; i < DR_JOIN_ROWS; ++i)
+            if (c < p.key_dim && r0 + i < p.value_dim) p.before[piece * size + (uint64_t)(r0 + i) * p.key_dim + c] = mine[i];
+        if (k + 1 == p.parts) break;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < DR_JOIN_ROWS; ++i) s[i][c] = mine[i];
+        __syncthreads();
+        if (c < p.key_dim) {
+#pragma unroll
+            for (int i = 0; i < DR_JOIN_ROWS; ++i) mine[i] = r0 + i < p.value_dim ? p.local[piece * size + (uint64_t)(r0 + i) * p.key_dim + c] : 0.0f;
+            const float* const map = p.map + piece * p.key_dim * p.key_dim + c;
+#pragma unroll 16
+            for (uint32_t j = 0; j < p.key_dim; ++j) {
+                const float m = map[(uint64_t)j * p.key_dim];
+#pragma unroll
+                for (int i = 0; i < DR_JOIN_ROWS; ++i) mine[i] = fmaf(s[i][j], m, mine[i]);
+            }
+        }
+    }
 }
 
 // ---- gradients of the inputs ------------------------------------------------------------------------
@@ -1547,10 +1618,29 @@ static DrShape dr_shape(const lcpp_delta_shape& sh) {
                    sh.key_dim, sh.value_dim, sh.scale};
 }
 
+// Into how many parts the sequences are cut, so that the chains have work for all SMs: the number with the least time, by
+// the sequences' average length and the waves of CTAs with 8 warps (16 value dimensions each) that both passes take.  A
+// chunk takes such a CTA 5.8 us in the second pass, 3.9 us in the first, and a chain of 2 warps alone on its SM 5.1 us
+// (bf16, 128 dimensions).  A part has 8 chunks at least.
+static uint64_t dr_parts(const lcpp_delta_shape& sh) {
+    const uint64_t sms = device_info().sms, streams = sh.num_sequences * sh.heads;
+    if (!streams || streams * ceil_div(sh.value_dim, 32) > sms) return 1;
+    const uint64_t chunks = ceil_div(sh.rows / sh.num_sequences, DR_CHUNK), values = ceil_div(sh.value_dim, 128), keys = ceil_div(sh.key_dim, 128);
+    uint64_t best = 1;
+    double least = 5.1 * chunks;
+    for (uint64_t parts = 2; parts <= 64 && parts * 8 <= chunks; ++parts) {
+        const double each = (double)ceil_div(chunks, parts), first = (double)ceil_div(streams * (parts - 1) * (values + keys), sms),
+                     second = (double)ceil_div(streams * parts * values, sms), time = each * (3.9 * first + 5.8 * second) + 4.0 * parts;
+        if (time < 0.9 * least) best = parts, least = time;
+    }
+    return best;
+}
+
 struct DrLayout {
     uint64_t slots, units;
     uint32_t planes, key_cols, rows;  // rows of an image
-    size_t keys, unit, x, back_x, z, back_z, back_out, bytes;
+    uint64_t parts;                   // of a sequence
+    size_t keys, unit, x, back_x, z, back_z, back_out, local, map, before, bytes;
     DrLayout(int dtype, const lcpp_delta_shape& sh, bool backward) {
         slots = sh.rows / DR_CHUNK + sh.num_sequences, units = slots * sh.heads;
         planes = dtype == LCPP_F32 ? 2 : 1, key_cols = sh.key_dim <= 64 ? 64 : 128, rows = (uint32_t)align_up(sh.value_dim, 32);
@@ -1566,6 +1656,11 @@ struct DrLayout {
             x = take(units * states(nullptr, 0, 0).bytes()), back_x = take(units * 32);
             z = take(units * kept(nullptr, 0, 0).bytes()), back_z = take(units * 32);
             back_out = take(units * 32);
+        }
+        parts = dr_parts(sh), local = map = before = 0;
+        if (parts > 1) {
+            const uint64_t pieces = sh.num_sequences * sh.heads * parts, state = (uint64_t)sh.value_dim * sh.key_dim;
+            local = take(pieces * state * 4), map = take(pieces * sh.key_dim * sh.key_dim * 4), before = take(pieces * state * 4);
         }
         bytes = max(at, (size_t)256);
     }
@@ -1604,31 +1699,51 @@ static lcpp_status dr_launch(const char* name, uint64_t grid, unsigned threads, 
     return check_launch();
 }
 
-// How many warps a CTA of the chain has, 16 value dimensions each: fewer where that spreads the states over more SMs.
-static int dr_warps(const lcpp_delta_shape& sh) {
-    const uint64_t states = sh.num_sequences * sh.heads, sms = device_info().sms;
+// How many warps a CTA of the chain has, 16 value dimensions each: fewer where that spreads `streams` over more SMs.
+static int dr_warps(uint64_t streams, uint32_t dim) {
+    const uint64_t sms = device_info().sms;
     int warps = 8;
-    while (warps > 2 && (warps * 8u >= sh.value_dim || states * ceil_div(sh.value_dim, warps * 16) * 2 <= sms)) warps /= 2;
+    while (warps > 2 && (warps * 8u >= dim || streams * ceil_div(dim, warps * 16) * 2 <= sms)) warps /= 2;
     return warps;
 }
 template <typename F>
 static lcpp_status dr_dispatch(const lcpp_delta_shape& sh, F&& f) {
     return sh.key_dim <= 64 ? f(std::integral_constant<int, 64>{}) : f(std::integral_constant<int, 128>{});
 }
-template <typename T, int DK, bool BACKWARD>
-static lcpp_status dr_chain(const lcpp_delta_shape& sh, const DrChain& p, cudaStream_t s) {
+template <typename T, int DK, bool BACKWARD, int WHAT>
+static lcpp_status dr_chain_pass(const DrChain& p, cudaStream_t s) {
+    const uint64_t streams = (uint64_t)p.sh.sequences * p.sh.heads * (WHAT == DR_STATES ? p.parts - 1 : p.parts);
     auto chain = [&](auto warps) {
         constexpr int WARPS = decltype(warps)::value;
-        const uint64_t grid = sh.num_sequences * sh.heads * ceil_div(sh.value_dim, WARPS * 16);
+        const uint64_t grid = streams * (ceil_div(p.sh.value_dim, WARPS * 16) + (WHAT == DR_STATES ? ceil_div(p.sh.key_dim, WARPS * 16) : 0));
         constexpr size_t smem = sizeof(DrChainSmem<T, DK, WARPS>);
         static_assert(smem <= 227 * 1024, "shared memory of a CTA");
-        if constexpr (BACKWARD) return dr_launch<dr_backward_kernel<T, DK, WARPS>>("dr_backward", grid, WARPS * 32, smem, s, p);
-        else return dr_launch<dr_forward_kernel<T, DK, WARPS>>("dr_forward", grid, WARPS * 32, smem, s, p);
+        if constexpr (BACKWARD) return dr_launch<dr_backward_kernel<T, DK, WARPS, WHAT>>(WHAT == DR_ALL ? "dr_backward" : "dr_states", grid, WARPS * 32, smem, s, p);
+        else return dr_launch<dr_forward_kernel<T, DK, WARPS, WHAT>>(WHAT == DR_ALL ? "dr_forward" : "dr_states", grid, WARPS * 32, smem, s, p);
     };
-    const int warps = dr_warps(sh);
-    if (warps == 8) return chain(std::integral_constant<int, 8>{});
-    if (warps == 4) return chain(std::integral_constant<int, 4>{});
-    return chain(std::integral_constant<int, 2>{});
+    if constexpr (WHAT == DR_STATES) return chain(std::integral_constant<int, 8>{});  // there are parts enough
+    else {
+        const int warps = dr_warps(streams, p.sh.value_dim);
+        if (warps == 8) return chain(std::integral_constant<int, 8>{});
+        if (warps == 4) return chain(std::integral_constant<int, 4>{});
+        return chain(std::integral_constant<int, 2>{});
+    }
+}
+template <typename T, int DK, bool BACKWARD>
+static lcpp_status dr_chain(DrChain p, const DrLayout& l, void* temp, cudaStream_t s) {
+    p.parts = (uint32_t)l.parts;
+    if (l.parts > 1) {
+        char* const t = (char*)temp;
+        p.local = (float*)(t + l.local), p.map = (float*)(t + l.map);
+        lcpp_status status = dr_chain_pass<T, DK, BACKWARD, DR_STATES>(p, s);
+        if (status != LCPP_OK) return status;
+        const DrJoin j{p.from, p.local, p.map, (float*)(t + l.before), p.sh.heads, p.sh.key_dim, p.sh.value_dim, p.parts,
+                       (uint32_t)ceil_div(p.sh.value_dim, DR_JOIN_ROWS), BACKWARD};
+        status = dr_launch<dr_join_kernel>("dr_join", (uint64_t)p.sh.sequences * p.sh.heads * j.slices, 128, 0, s, j);
+        if (status != LCPP_OK) return status;
+        p.from = j.before;
+    }
+    return dr_chain_pass<T, DK, BACKWARD, DR_ALL>(p, s);
 }
 
 // Everything that a call reads, and its checks.
@@ -1736,7 +1851,7 @@ extern "C" lcpp_status lcpp_delta_rule_forward(int dtype, const lcpp_delta_shape
             if (sh.rows)
                 status = dr_launch<dr_prepare_kernel<T, DK, false>>("dr_prepare", l.slots * sh.key_heads, DR_PREPARE_THREADS,
                                                                     sizeof(DrPrepareSmem<DK, PLANES>), s, pr);
-            return status != LCPP_OK ? status : dr_chain<T, DK, false>(*shape, p, s);
+            return status != LCPP_OK ? status : dr_chain<T, DK, false>(p, l, temp, s);
         });
     });
 }
@@ -1800,7 +1915,7 @@ extern "C" lcpp_status lcpp_delta_rule_backward(int dtype, const lcpp_delta_shap
             if (sh.rows)
                 status = dr_launch<dr_prepare_kernel<T, DK, true>>("dr_prepare", l.slots * sh.key_heads, DR_PREPARE_THREADS,
                                                                    sizeof(DrPrepareSmem<DK, PLANES>), s, pr);
-            if (status == LCPP_OK) status = dr_chain<T, DK, true>(*shape, p, s);
+            if (status == LCPP_OK) status = dr_chain<T, DK, true>(p, l, temp, s);
             if (status != LCPP_OK || !sh.rows) return status;
             const uint64_t grid = l.slots * sh.key_heads;
             if (sh.heads > sh.key_heads) return dr_launch<dr_gradient_kernel<T, DK, true>>("dr_gradient", grid, DR_GRAD_THREADS, smem, s, gr);
