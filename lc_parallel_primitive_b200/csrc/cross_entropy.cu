@@ -44,15 +44,23 @@ constexpr int CE_STAGE_BYTES = 2 * CE_HALF_BYTES;    // both operands
 constexpr int CE_EPILOGUE_WARPS = 8;
 constexpr int CE_THREADS = 64 + 32 * CE_EPILOGUE_WARPS;  // a loading warp, a warp that issues products, the epilogue
 constexpr float CE_LOG2E = 1.44269504088896f;
-// f16: G is kept as a share of the largest gradient of the loss times 2^14, or small probabilities would vanish.
-constexpr float CE_F16_GAIN = 16384.0f;
+// G is kept for gradients of the loss as shares of the largest, which the sums are multiplied by in the end: for a mean's
+// equal gradients the shares are 1, and an entry's rounding is that of the probability alone (-1 for an unlikely target is
+// exact, where rounding 1 / rows would be off the same way in all rows).  float16 times 2^14, or small probabilities
+// would vanish.
+template <typename T>
+constexpr float CE_GAIN = std::is_same_v<T, __half> ? 16384.0f : 1.0f;
 
 enum { CE_LOGSUM, CE_GRAD, CE_HIDDEN, CE_WEIGHT };
+
+// The next kernel may start; the one before has ended.
+__device__ __forceinline__ void ce_let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void ce_wait_for_last() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 // What the rows that take part are, in packed order; written by ce_plan_kernel.
 struct CePlan {
     uint32_t* count;   // rows that take part
-    float* largest;    // largest |grad_loss| of them
+    float* largest;    // largest finite |grad_loss| of them
     int32_t* slot;     // of a row, or -1
     uint32_t* row;     // of a slot
     int32_t* target;
@@ -75,7 +83,7 @@ struct CeGemm {
     uint64_t sum_stride;
     void* out;                // CE_WEIGHT: gradient of the weight
     uint64_t out_stride;
-    uint32_t out_wide;        // its rows start on 16 bytes
+    uint32_t grad_wide, out_wide;  // bytes that the rows of G and out start on: 32, 16 or 1
 };
 
 struct CeBarriers {
@@ -106,12 +114,17 @@ struct CeTiles {
     __device__ __forceinline__ uint64_t units() const { return (uint64_t)m * n * parts; }
     // Bands of 8 tiles along M, M fastest: the tiles under way share operands in L2.
     __device__ __forceinline__ void at(uint64_t unit, uint32_t* mt, uint32_t* nt, uint32_t* first, uint32_t* end) const {
-        const uint32_t part = (uint32_t)(unit % parts);
-        const uint64_t tile = unit / parts;
-        const uint32_t band = (uint32_t)(tile / (8ull * n)), height = min(8u, m - band * 8);
+        const uint64_t tile = parts > 1 ? unit / parts : unit;
+        // 64-bit division takes a thread some hundred cycles
+        const uint32_t band = tile >> 32 || n >> 29 ? (uint32_t)(tile / (8ull * n)) : (uint32_t)tile / (8 * n), height = min(8u, m - band * 8);
         const uint32_t in = (uint32_t)(tile - band * 8ull * n);
         *mt = band * 8 + in % height, *nt = in / height;
-        *first = (uint32_t)((uint64_t)steps * part / parts), *end = (uint32_t)((uint64_t)steps * (part + 1) / parts);
+        range(part(unit), first, end);
+    }
+    __device__ __forceinline__ uint32_t part(uint64_t unit) const { return parts > 1 ? (uint32_t)unit % parts : 0; }
+    // Steps along K of a part; parts <= 32 and steps < 2^26.
+    __device__ __forceinline__ void range(uint32_t part, uint32_t* first, uint32_t* end) const {
+        *first = steps * part / parts, *end = steps * (part + 1) / parts;
     }
 };
 
@@ -131,10 +144,29 @@ __device__ __forceinline__ float ce_exp2(float v) {
     return r;
 }
 
-// 32 values of a row, `width` of which exist.
+// 32 bytes, a whole sector, on a 32-byte boundary.
+__device__ __forceinline__ void ce_store_sector(void* to, const uint32_t (&v)[8]) {
+    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(to), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]),
+                 "r"(v[5]), "r"(v[6]), "r"(v[7])
+                 : "memory");
+}
+// 32 values of a row, `width` of which exist; rows start on `wide` bytes.  A lane has a row of its own, so that a warp's
+// store meets 32 rows: whole sectors are half the transactions of 16-byte stores.
 template <typename T>
-__device__ __forceinline__ void ce_store32(T* to, const float (&v)[32], uint32_t width, bool wide) {
-    if (wide && width >= 32) {
+__device__ __forceinline__ void ce_store32(T* to, const float (&v)[32], uint32_t width, uint32_t wide) {
+    if (wide >= 32 && width >= 32) {
+        constexpr int E = 32 / sizeof(T);
+#pragma unroll
+        for (int i = 0; i < 32 / E; ++i) {
+            uint32_t w[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                if constexpr (sizeof(T) == 4) w[j] = __float_as_uint(v[i * E + j]);
+                else w[j] = ce_pack2<T>(v[i * E + 2 * j], v[i * E + 2 * j + 1]);
+            }
+            ce_store_sector(to + i * E, w);
+        }
+    } else if (wide >= 16 && width >= 32) {
         if constexpr (sizeof(T) == 4) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) ((float4*)to)[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
@@ -197,7 +229,7 @@ __device__ __forceinline__ void ce_epilogue(const CeGemm& p, uint32_t tmem, uint
         const int64_t target = live ? (int64_t)p.plan.target[m] - (int64_t)p.vocab0 - n0 : -1;
         const float shift = live ? p.plan.logsum[m] * CE_LOG2E : 0.0f;
         float gain = live ? p.plan.gain[m] : 0.0f;
-        if (std::is_same_v<T, __half> && live && gain != 0.0f) gain = gain / *p.plan.largest * CE_F16_GAIN;
+        if (live && gain != 0.0f) gain = gain / *p.plan.largest * CE_GAIN<T>;
         E* const to = (E*)p.grad + (uint64_t)m * p.grad_stride + n0;
 #pragma unroll 1
         for (int c = 0; c < CE_BN / 2; c += 32) {
@@ -220,11 +252,11 @@ __device__ __forceinline__ void ce_epilogue(const CeGemm& p, uint32_t tmem, uint
                     if (i >= real) v[i] = 0.0f;
             }
             if constexpr (sizeof(T) == 2) {
-                ce_store32<E>(to + c, v, width, true);
+                ce_store32<E>(to + c, v, width, p.grad_wide);
             } else {  // three parts of 8 bits
 #pragma unroll
                 for (int plane = 0; plane < 3; ++plane) {
-                    ce_store32<E>(to + plane * (uint64_t)p.padded * p.grad_stride + c, v, width, true);
+                    ce_store32<E>(to + plane * (uint64_t)p.padded * p.grad_stride + c, v, width, p.grad_wide);
 #pragma unroll
                     for (int i = 0; i < 32; ++i) v[i] -= widen(narrow<E>(v[i]));
                 }
@@ -253,7 +285,7 @@ __device__ __forceinline__ void ce_epilogue(const CeGemm& p, uint32_t tmem, uint
         }
     } else {
         const bool live = m < p.vocab;
-        const float unit = std::is_same_v<T, __half> ? *p.plan.largest / CE_F16_GAIN : 1.0f;
+        const float unit = *p.plan.largest / CE_GAIN<T>;
         T* const to = (T*)p.out + (uint64_t)(p.vocab0 + m) * p.out_stride + n0;
 #pragma unroll 1
         for (int c = 0; c < CE_BN / 2; c += 32) {
@@ -293,6 +325,8 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     cluster_sync();
     tmem_fence_after();
     const uint32_t tmem = bar.tmem;
+    ce_let_next_start();
+    ce_wait_for_last();
     const uint32_t count = *p.plan.count;
     const CeTiles<EPI> tl(p, count);
     const uint32_t pairs = ce_pairs(p.planes), groups = gridDim.x / 2, group = blockIdx.x / 2;
@@ -347,8 +381,8 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
             constexpr uint32_t step_a = A_MN ? 2048 : 32, step_b = B_MN ? 2048 : 32;  // bytes of 16 along K
             uint32_t it = 0, sums = 0;
             for (uint64_t unit = group; ok && unit < tl.units(); unit += groups, ++sums) {
-                uint32_t mt, nt, first, end;
-                tl.at(unit, &mt, &nt, &first, &end);
+                uint32_t first, end;
+                tl.range(tl.part(unit), &first, &end);
                 const uint32_t d = sums & 1;
                 if (sums >= 2 && !mbar_poll(&bar.sum_empty[d], (sums / 2 - 1) & 1, limit)) {
                     ok = false;
@@ -386,7 +420,7 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
             tmem_fence_after();
             ce_epilogue<T, EPI>(p, tmem + d * CE_BN + half * (CE_BN / 2) + (quarter * 32 << 16),
                                 rank * 128 + quarter * 32 + (threadIdx.x & 31), count, mt, nt, half, first == end,
-                                (uint32_t)(unit % tl.parts));
+                                tl.part(unit));
             tmem_fence_before();
             __syncwarp();
             if (elect_one()) mbar_arrive_cluster(cluster_smem(smem_u32(&bar.sum_empty[d]), 0));
@@ -408,38 +442,53 @@ ce_plan_kernel(const int32_t* targets, const float* grad_loss, uint64_t grad_str
                uint32_t vocab, CePlan plan) {
     __shared__ uint32_t sums[32];
     __shared__ float tops[32];
+    ce_let_next_start();
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     uint32_t base = 0;
     float most = 0.0f;
-    for (uint64_t r0 = 0; r0 < rows; r0 += CE_PLAN_THREADS) {
-        const uint64_t r = r0 + threadIdx.x;
-        int32_t t = r < rows ? targets[r] : -1;
-        if (t >= 0 && (uint32_t)t >= vocab) {
-            set_error(LCPP_ERR_INVALID_ARG);
-            t = -1;
+    for (uint64_t r0 = 0; r0 < rows; r0 += CE_PLAN_THREADS * 4) {  // 128 rows a warp
+        int32_t t[4];
+        uint32_t ballot[4], mine = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint64_t r = r0 + warp * 128 + i * 32 + lane;
+            t[i] = r < rows ? targets[r] : -1;
         }
-        const uint32_t ballot = __ballot_sync(0xffffffffu, t >= 0);
-        if (lane == 0) sums[warp] = __popc(ballot);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (t[i] >= 0 && (uint32_t)t[i] >= vocab) {
+                set_error(LCPP_ERR_INVALID_ARG);
+                t[i] = -1;
+            }
+            ballot[i] = __ballot_sync(0xffffffffu, t[i] >= 0);
+            mine += __popc(ballot[i]);
+        }
+        if (lane == 0) sums[warp] = mine;
         __syncthreads();
-        uint32_t before = 0, all = 0;
+        uint32_t before = base, all = 0;
 #pragma unroll
         for (uint32_t w = 0; w < 32; ++w) {
             if (w < warp) before += sums[w];
             all += sums[w];
         }
-        if (r < rows) {
-            const uint32_t slot = base + before + __popc(ballot & lanemask_lt());
-            plan.slot[r] = t >= 0 ? (int32_t)slot : -1;
-            if (t >= 0) {
-                plan.row[slot] = (uint32_t)r;
-                plan.target[slot] = t;
-                if (grad_loss) {
-                    const float g = grad_loss[r * grad_stride];
-                    plan.gain[slot] = g;
-                    plan.logsum[slot] = logsum[r];
-                    most = fmaxf(most, fabsf(g));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint64_t r = r0 + warp * 128 + i * 32 + lane;
+            if (r < rows) {
+                const uint32_t slot = before + __popc(ballot[i] & lanemask_lt());
+                plan.slot[r] = t[i] >= 0 ? (int32_t)slot : -1;
+                if (t[i] >= 0) {
+                    plan.row[slot] = (uint32_t)r;
+                    plan.target[slot] = t[i];
+                    if (grad_loss) {
+                        const float g = grad_loss[r * grad_stride];
+                        plan.gain[slot] = g;
+                        plan.logsum[slot] = logsum[r];
+                        if (fabsf(g) < INFINITY) most = fmaxf(most, fabsf(g));
+                    }
                 }
             }
+            before += __popc(ballot[i]);
         }
         base += all;
         __syncthreads();
@@ -461,16 +510,28 @@ __global__ void __launch_bounds__(256)
 ce_pack_kernel(const T* from, uint64_t from_stride, const uint32_t* row, const uint32_t* count, uint32_t rows,
                uint32_t channels, void* to, uint64_t to_stride, uint64_t plane) {
     using E = std::conditional_t<sizeof(T) == 4, __nv_bfloat16, T>;
+    ce_let_next_start();
+    ce_wait_for_last();
     const uint32_t have = count ? *count : rows, last = count ? (have + CE_BM - 1) / CE_BM * CE_BM : rows;
     const uint32_t words = (uint32_t)(to_stride / 8);
     const bool wide = ((uintptr_t)from | from_stride * sizeof(T)) % 16 == 0;
-    for (uint64_t r = blockIdx.x; r < last; r += gridDim.x) {
+    const uint32_t lane = threadIdx.x & 31;
+    for (uint64_t r = (uint64_t)blockIdx.x * 8 + (threadIdx.x >> 5); r < last; r += (uint64_t)gridDim.x * 8) {  // a warp a row
         const T* const source = r < have ? from + (row ? row[r] : r) * from_stride : nullptr;
-        for (uint32_t w = threadIdx.x; w < words; w += blockDim.x) {
+#pragma unroll 4
+        for (uint32_t w = lane; w < words; w += 32) {
             alignas(16) T v[8];
             if (source && wide && w * 8 + 8 <= channels) {
 #pragma unroll
                 for (int i = 0; i < (int)sizeof(v) / 16; ++i) ((uint4*)v)[i] = ((const uint4*)(source + w * 8))[i];
+            } else if (sizeof(T) == 2 && source && w && w * 8 + 8 < channels) {  // neighbours on both sides: words
+                const uint32_t* const words = (const uint32_t*)((uintptr_t)(source + w * 8) & ~(uintptr_t)3);
+                const uint32_t shift = (uintptr_t)(source + w * 8) & 2 ? 16 : 0;
+                uint32_t x[5];
+#pragma unroll
+                for (int i = 0; i < 5; ++i) x[i] = words[i];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) ((uint32_t*)v)[i] = __funnelshift_r(x[i], x[i + 1], shift);
             } else {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) v[i] = source && w * 8 + i < channels ? source[w * 8 + i] : narrow<T>(0.0f);
@@ -497,11 +558,14 @@ ce_pack_kernel(const T* from, uint64_t from_stride, const uint32_t* row, const u
     }
 }
 
-// 32 slots a CTA, 8 warps over the parts of the vocabulary: logsum and loss.
-__global__ void __launch_bounds__(256)
+// 32 rows a CTA, its warps over the parts of the vocabulary: logsum and loss.
+constexpr int CE_LOSS_WARPS = 32;
+__global__ void __launch_bounds__(CE_LOSS_WARPS * 32)
 ce_loss_kernel(const float2* part, uint32_t parts, const float* right, CePlan plan, uint32_t rows, uint32_t padded, float* loss,
                float* logsum) {
-    __shared__ float2 joined[8][32];
+    __shared__ float2 joined[CE_LOSS_WARPS][32];
+    ce_let_next_start();
+    ce_wait_for_last();
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const uint64_t r = (uint64_t)blockIdx.x * 32 + lane;
     const int32_t slot = r < rows ? plan.slot[r] : -1;
@@ -511,12 +575,21 @@ ce_loss_kernel(const float2* part, uint32_t parts, const float* right, CePlan pl
         sum = sum * ce_exp2(top - shift) + v.y * ce_exp2(v.x - shift);
         top = base;
     };
-    if (slot >= 0)
-        for (uint32_t i = warp; i < parts; i += 8) join(part[(uint64_t)i * padded + slot]);
+    if (slot >= 0) {
+        uint32_t i = warp;
+        for (; i + 3 * CE_LOSS_WARPS < parts; i += 4 * CE_LOSS_WARPS) {
+            float2 v[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = part[(uint64_t)(i + j * CE_LOSS_WARPS) * padded + slot];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) join(v[j]);
+        }
+        for (; i < parts; i += CE_LOSS_WARPS) join(part[(uint64_t)i * padded + slot]);
+    }
     joined[warp][lane] = make_float2(top, sum);
     __syncthreads();
     if (warp == 0 && r < rows) {
-        for (int w = 1; w < 8; ++w) join(joined[w][lane]);
+        for (int w = 1; w < CE_LOSS_WARPS; ++w) join(joined[w][lane]);
         const float total = (top + log2f(sum)) * 0.693147180559945f;
         if (loss) loss[r] = slot >= 0 ? total - right[slot] : 0.0f;
         if (logsum) logsum[r] = slot >= 0 ? total : 0.0f;
@@ -528,7 +601,9 @@ template <typename T>
 __global__ void __launch_bounds__(256)
 ce_hidden_kernel(const float* sums, uint64_t stride, uint32_t padded, uint32_t splits, CePlan plan, uint32_t rows,
                  uint32_t channels, T* out, uint64_t out_stride, bool wide) {
-    const float unit = std::is_same_v<T, __half> ? *plan.largest / CE_F16_GAIN : 1.0f;
+    ce_let_next_start();
+    ce_wait_for_last();
+    const float unit = *plan.largest / CE_GAIN<T>;
     for (uint64_t r = blockIdx.x; r < rows; r += gridDim.x) {
         const int32_t slot = plan.slot[r];
         T* const to = out + r * out_stride;
@@ -569,10 +644,8 @@ struct CeLayout {
         sum_pitch = align_up(channels, 4);
         const uint64_t widest = max(CE_PIECE_BYTES / (planes * padded * 2) / CE_BN * CE_BN, (uint64_t)CE_BN);
         const uint64_t pieces = ceil_div(vocab, widest);
-        piece = min(align_up(ceil_div(vocab, pieces), CE_BN), align_up(vocab, 8));
-        // sums over K in as many parts as there are pairs of CTAs for the tiles
-        const uint64_t tiles = padded / CE_BM * ceil_div(channels, CE_BN);
-        splits = max(min((uint64_t)device_info().sms / 2 / tiles, piece / 1024), (uint64_t)1);
+        piece = min(align_up(ceil_div(vocab, pieces), CE_BN), align_up(vocab, 16));  // rows of G on 32 bytes
+        splits = best_splits(padded, channels, piece);
         size_t at = 0;
         auto take = [&](uint64_t n) {
             const size_t here = at;
@@ -592,6 +665,18 @@ struct CeLayout {
             part = take(parts * padded * 8);
         }
         bytes = at;
+    }
+    // Parts of the hidden gradient's sum over the vocabulary: the number with the least time, of whole waves of tiles (a step
+    // of 64 takes 0.33 us) and of the parts' sums (float32, written and read once a piece).
+    static uint64_t best_splits(uint64_t padded, uint64_t channels, uint64_t piece) {
+        const uint64_t pairs = device_info().sms / 2, tiles = padded / CE_BM * ceil_div(channels, CE_BN), steps = ceil_div(piece, CE_BK);
+        uint64_t best = 1;
+        double least = 0;
+        for (uint64_t n = 1; n <= 32 && n * 16 <= max(steps, (uint64_t)16); ++n) {
+            const double time = (double)ceil_div(tiles * n, pairs) * ceil_div(steps, n) * 0.33 + (double)n * padded * channels * 8 / 6e6;
+            if (n == 1 || time < least) best = n, least = time;
+        }
+        return best;
     }
     CePlan plan(void* temp) const {
         char* const t = (char*)temp;
@@ -629,12 +714,27 @@ struct CeCall {
     }
 };
 
-template <typename K, typename... A>
-static lcpp_status ce_launch(const char* name, K kernel, uint64_t grid, unsigned threads, cudaStream_t s, A... args) {
+// A call's kernels but the first start while the one before ends (programmatic dependent launch): each lets the next
+// one in when it starts itself, and waits for the end of the one before ahead of its first access to memory.
+template <typename... P, typename... A>
+static lcpp_status ce_launch(const char* name, void (*kernel)(P...), uint64_t grid, unsigned threads, size_t smem, bool first, cudaStream_t s,
+                             const A&... args) {
+    cudaLaunchAttribute how[1];
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)grid);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cfg.attrs = how;
+    if (!first) {
+        how[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        how[0].val.programmaticStreamSerializationAllowed = 1;
+        cfg.numAttrs = 1;
+    }
     ProfScope prof(name, s);
-    kernel<<<(unsigned)grid, threads, 0, s>>>(args...);
+    if (cudaLaunchKernelEx(&cfg, kernel, P(args)...) != cudaSuccess) return check_launch();
     count_launch();
-    return check_launch();
+    return LCPP_OK;
 }
 
 template <typename T, int EPI>
@@ -650,10 +750,7 @@ static lcpp_status ce_gemm(const char* name, const CUtensorMap& a, const CUtenso
         sized.fetch_or(bit, std::memory_order_relaxed);
     }
     const uint64_t pairs = min(units, (uint64_t)device.sms / 2);
-    ProfScope prof(name, s);
-    ce_gemm_kernel<T, EPI><<<(unsigned)pairs * 2, CE_THREADS, smem, s>>>(a, b, p);
-    count_launch();
-    return check_launch();
+    return ce_launch(name, ce_gemm_kernel<T, EPI>, pairs * 2, CE_THREADS, smem, false, s, a, b, p);
 }
 
 struct CeMaps {
@@ -666,18 +763,18 @@ static lcpp_status ce_begin(const CeCall& c, const CeLayout& l, const float* gra
                             const float* logsum, CeMaps* maps) {
     const CePlan plan = l.plan(c.temp);
     char* const t = (char*)c.temp;
-    lcpp_status ok = ce_launch("ce_plan", ce_plan_kernel, 1, CE_PLAN_THREADS, c.stream, c.targets, grad_loss, grad_stride,
+    lcpp_status ok = ce_launch("ce_plan", ce_plan_kernel, 1, CE_PLAN_THREADS, 0, true, c.stream, c.targets, grad_loss, grad_stride,
                                logsum, (uint32_t)c.rows, (uint32_t)c.vocab, plan);
     if (ok != LCPP_OK) return ok;
     const uint64_t most = (uint64_t)device_info().sms * 16;
-    ok = ce_launch("ce_pack", ce_pack_kernel<T>, min(l.padded, most), 256, c.stream, (const T*)c.hidden, c.hidden_stride,
+    ok = ce_launch("ce_pack", ce_pack_kernel<T>, min(ceil_div(l.padded, 8), most), 256, 0, false, c.stream, (const T*)c.hidden, c.hidden_stride,
                    plan.row, plan.count, (uint32_t)c.rows, (uint32_t)c.channels, t + l.hidden, l.pitch, l.padded * l.pitch);
     if (ok != LCPP_OK) return ok;
     const void* weight = c.weight;
     uint64_t weight_pitch = c.weight_stride;
     if (l.weight) {
         weight = t + l.weight, weight_pitch = l.pitch;
-        ok = ce_launch("ce_pack", ce_pack_kernel<T>, min(c.vocab, most), 256, c.stream, (const T*)c.weight, c.weight_stride,
+        ok = ce_launch("ce_pack", ce_pack_kernel<T>, min(ceil_div(c.vocab, 8), most), 256, 0, false, c.stream, (const T*)c.weight, c.weight_stride,
                        nullptr, nullptr, (uint32_t)c.vocab, (uint32_t)c.channels, t + l.weight, l.pitch, c.vocab * l.pitch);
         if (ok != LCPP_OK) return ok;
     } else if (c.vocab == 1) {
@@ -738,7 +835,7 @@ extern "C" lcpp_status lcpp_cross_entropy_forward(int dtype, const void* hidden,
         p.part = (float2*)((char*)temp + l.part), p.right = (float*)((char*)temp + l.right);
         ok = ce_gemm<T, CE_LOGSUM>("ce_logsum", maps.hidden_k, maps.weight_k, p, l.padded / CE_BM * ceil_div(vocab, CE_BN), c.stream);
         if (ok != LCPP_OK) return ok;
-        return ce_launch("ce_loss", ce_loss_kernel, ceil_div(rows, 32), 256, c.stream, (const float2*)p.part, (uint32_t)l.parts,
+        return ce_launch("ce_loss", ce_loss_kernel, ceil_div(rows, 32), CE_LOSS_WARPS * 32, 0, false, c.stream, (const float2*)p.part, (uint32_t)l.parts,
                          (const float*)p.right, p.plan, (uint32_t)rows, (uint32_t)l.padded, loss, logsum);
     });
 }
@@ -783,10 +880,11 @@ extern "C" lcpp_status lcpp_cross_entropy_backward(int dtype, const void* hidden
         p.plan = l.plan(temp);
         p.planes = (uint32_t)l.planes, p.rows = (uint32_t)rows, p.channels = (uint32_t)channels;
         p.padded = (uint32_t)l.padded, p.splits = (uint32_t)l.splits;
-        p.grad = (char*)temp + l.grad, p.grad_stride = l.piece;
+        p.grad = (char*)temp + l.grad, p.grad_stride = l.piece, p.grad_wide = (uintptr_t)p.grad % 32 == 0 ? 32 : 16;
         p.sums = (float*)((char*)temp + l.sums), p.sum_stride = l.sum_pitch;
         p.out = grad_weight, p.out_stride = grad_weight_stride;
-        p.out_wide = ((uintptr_t)grad_weight | (vocab > 1 ? grad_weight_stride * sizeof(T) : 0)) % 16 == 0;
+        const uintptr_t starts = (uintptr_t)grad_weight | (vocab > 1 ? grad_weight_stride * sizeof(T) : 0);
+        p.out_wide = starts % 32 == 0 ? 32 : starts % 16 == 0 ? 16 : 1;
         const uint64_t mt = l.padded / CE_BM, dt = ceil_div(channels, CE_BN);
         for (uint64_t v0 = 0; v0 < vocab; v0 += l.piece) {
             p.vocab0 = (uint32_t)v0, p.vocab = (uint32_t)min(l.piece, vocab - v0), p.add = v0 > 0;
@@ -799,7 +897,7 @@ extern "C" lcpp_status lcpp_cross_entropy_backward(int dtype, const void* hidden
         }
         if (!grad_hidden) return LCPP_OK;
         const bool wide = ((uintptr_t)grad_hidden | (rows > 1 ? grad_hidden_stride * sizeof(T) : 0)) % 16 == 0;
-        return ce_launch("ce_hidden_out", ce_hidden_kernel<T>, min(rows, (uint64_t)device_info().sms * 16), 256, c.stream,
+        return ce_launch("ce_hidden_out", ce_hidden_kernel<T>, min(rows, (uint64_t)device_info().sms * 16), 256, 0, false, c.stream,
                          (const float*)p.sums, l.sum_pitch, (uint32_t)l.padded, (uint32_t)l.splits, p.plan, (uint32_t)rows,
                          (uint32_t)channels, (T*)grad_hidden, grad_hidden_stride, wide);
     });
