@@ -150,6 +150,12 @@ __device__ __forceinline__ void ce_store_sector(void* to, const uint32_t (&v)[8]
                  "r"(v[5]), "r"(v[6]), "r"(v[7])
                  : "memory");
 }
+__device__ __forceinline__ void ce_load_sector(uint32_t (&v)[8], const void* from) {
+    asm volatile("ld.global.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
+                 : "l"(from)
+                 : "memory");
+}
 // 32 values of a row, `width` of which exist; rows start on `wide` bytes.  A lane has a row of its own, so that a warp's
 // store meets 32 rows: whole sectors are half the transactions of 16-byte stores.
 template <typename T>
@@ -271,17 +277,19 @@ __device__ __forceinline__ void ce_epilogue(const CeGemm& p, uint32_t tmem, uint
             if (width <= 0) break;
 #pragma unroll
             for (int i = 0; i < 32; ++i) v[i] = empty ? 0.0f : v[i];
-            if (p.add) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    if (4 * i < width) {
-                        const float4 a = ((const float4*)(to + c))[i];
-                        v[4 * i] += a.x, v[4 * i + 1] += a.y, v[4 * i + 2] += a.z, v[4 * i + 3] += a.w;
-                    }
+            for (int i = 0; i < 4; ++i) {
+                if (8 * i >= width) break;
+                uint32_t w[8];
+                if (p.add) {
+                    ce_load_sector(w, to + c + 8 * i);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) v[8 * i + j] += __uint_as_float(w[j]);
+                }
+#pragma unroll
+                for (int j = 0; j < 8; ++j) w[j] = __float_as_uint(v[8 * i + j]);
+                ce_store_sector(to + c + 8 * i, w);
             }
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (4 * i < width) ((float4*)(to + c))[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
         }
     } else {
         const bool live = m < p.vocab;
@@ -629,7 +637,7 @@ ce_hidden_kernel(const float* sums, uint64_t stride, uint32_t padded, uint32_t s
 
 // ---- host ------------------------------------------------------------------------------------
 constexpr uint64_t CE_MAX_ROWS = 1ull << 24, CE_MAX_CHANNELS = 1ull << 20, CE_MAX_VOCAB = 1ull << 30;
-constexpr uint64_t CE_PIECE_BYTES = 256ull << 20;  // of G
+constexpr uint64_t CE_PIECE_BYTES = 512ull << 20;  // of G
 
 // The pieces of the temp buffer.
 struct CeLayout {
@@ -641,7 +649,7 @@ struct CeLayout {
         padded = align_up(rows, CE_BM);
         pitch = align_up(channels, 8);
         parts = ceil_div(vocab, CE_BN) * 2;
-        sum_pitch = align_up(channels, 4);
+        sum_pitch = align_up(channels, 8);
         const uint64_t widest = max(CE_PIECE_BYTES / (planes * padded * 2) / CE_BN * CE_BN, (uint64_t)CE_BN);
         const uint64_t pieces = ceil_div(vocab, widest);
         piece = min(align_up(ceil_div(vocab, pieces), CE_BN), align_up(vocab, 16));  // rows of G on 32 bytes
@@ -819,7 +827,7 @@ extern "C" lcpp_status lcpp_cross_entropy_forward(int dtype, const void* hidden,
     if ((!loss && !logsum) || !elements_aligned(LCPP_F32, loss, logsum)) return LCPP_ERR_INVALID_ARG;
     const CeLayout l(dtype, rows, channels, vocab, false, !ce_direct(dtype, weight, vocab > 1 ? weight_stride : 0));
     if (!temp || temp_bytes < l.bytes) return LCPP_ERR_TEMP_TOO_SMALL;
-    if ((uintptr_t)temp % 16) return LCPP_ERR_INVALID_ARG;
+    if ((uintptr_t)temp % 32) return LCPP_ERR_INVALID_ARG;
     const Region rh = c.r_hidden(), rw = c.r_weight(), rg(targets, rows * 4), rl(loss, rows * 4), rs(logsum, rows * 4),
                  rt(temp, l.bytes);
     if (!rl.apart(rh, rw, rg, rs, rt) || !rs.apart(rh, rw, rg, rt) || !rt.apart(rh, rw, rg)) return LCPP_ERR_INVALID_ARG;
@@ -863,7 +871,7 @@ extern "C" lcpp_status lcpp_cross_entropy_backward(int dtype, const void* hidden
         return LCPP_ERR_INVALID_ARG;
     const CeLayout l(dtype, rows, channels, vocab, true, !ce_direct(dtype, weight, vocab > 1 ? weight_stride : 0));
     if (!temp || temp_bytes < l.bytes) return LCPP_ERR_TEMP_TOO_SMALL;
-    if ((uintptr_t)temp % 16) return LCPP_ERR_INVALID_ARG;
+    if ((uintptr_t)temp % 32) return LCPP_ERR_INVALID_ARG;
     const uint64_t e = c.element();
     const Region rh = c.r_hidden(), rw = c.r_weight(), rg(targets, rows * 4), rs(logsum, rows * 4),
                  rl(grad_loss, grad_loss_stride ? rows : 1, grad_loss_stride * 4, 4), rt(temp, l.bytes),
@@ -880,7 +888,7 @@ extern "C" lcpp_status lcpp_cross_entropy_backward(int dtype, const void* hidden
         p.plan = l.plan(temp);
         p.planes = (uint32_t)l.planes, p.rows = (uint32_t)rows, p.channels = (uint32_t)channels;
         p.padded = (uint32_t)l.padded, p.splits = (uint32_t)l.splits;
-        p.grad = (char*)temp + l.grad, p.grad_stride = l.piece, p.grad_wide = (uintptr_t)p.grad % 32 == 0 ? 32 : 16;
+        p.grad = (char*)temp + l.grad, p.grad_stride = l.piece, p.grad_wide = 32;
         p.sums = (float*)((char*)temp + l.sums), p.sum_stride = l.sum_pitch;
         p.out = grad_weight, p.out_stride = grad_weight_stride;
         const uintptr_t starts = (uintptr_t)grad_weight | (vocab > 1 ? grad_weight_stride * sizeof(T) : 0);

@@ -95,6 +95,9 @@ __device__ __forceinline__ void dr_store(uint8_t* image, uint32_t blocks, uint32
 }
 
 // ---- what does not depend on the state ------------------------------------------------------------
+__device__ __forceinline__ void dr_let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void dr_wait_for_last() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 constexpr int DR_PREPARE_THREADS = 256;  // warps: 4 blocks of 16 rows x 2 halves of the columns
 constexpr int DR_PITCH = 68, DR_TMP_PITCH = 40;
 struct DrInvert {
@@ -226,6 +229,8 @@ dr_prepare_kernel(const __grid_constant__ DrPrepare p) {
     extern __shared__ __align__(128) uint8_t dr_smem[];
     auto& s = *(DrPrepareSmem<DK, PLANES>*)dr_smem;
     const DrShape& sh = p.sh;
+    dr_let_next_start();
+    dr_wait_for_last();
     const uint64_t slot = blockIdx.x / sh.key_heads;
     const uint32_t hk = blockIdx.x % sh.key_heads, group = sh.heads / sh.key_heads;
     const DrChunk c(sh, slot);
@@ -542,6 +547,7 @@ struct DrChainCta {
         : p(p_), sm(sm_), lane(threadIdx.x & 31), warp(threadIdx.x >> 5), g((threadIdx.x & 31) >> 2), col((threadIdx.x & 3) * 2),
           o(threadIdx.x & 31) {
         const DrShape& sh = p.sh;
+        dr_let_next_start();
         const uint32_t value_slices = (sh.value_dim + WARPS * 16 - 1) / (WARPS * 16),
                        slices = value_slices + (WHAT == DR_STATES ? (sh.key_dim + WARPS * 16 - 1) / (WARPS * 16) : 0);
         const uint32_t parts = WHAT == DR_STATES ? p.parts - 1 : p.parts;  // nothing follows on the end part
@@ -577,6 +583,7 @@ struct DrChainCta {
     __device__ __forceinline__ uint32_t order(uint32_t it) const { return first + (BACKWARD ? chunks - 1 - it : it); }
     // The first images and values, and the state that they meet.
     __device__ __forceinline__ void open(float (&s)[NT][4]) {
+        dr_wait_for_last();
         if (warp == 0 && lane == 0)
             for (uint32_t i = 0; i < (uint32_t)STAGES && i < chunks; ++i) load(i, order(i));
         __syncwarp();
@@ -1008,6 +1015,8 @@ struct DrJoin {
 };
 __global__ void __launch_bounds__(128) dr_join_kernel(const __grid_constant__ DrJoin p) {
     __shared__ float s[DR_JOIN_ROWS][DR_MAX_DIM];
+    dr_let_next_start();
+    dr_wait_for_last();
     const uint32_t slice = blockIdx.x % p.slices, r0 = slice * DR_JOIN_ROWS, c = threadIdx.x;
     const uint64_t stream = blockIdx.x / p.slices, size = (uint64_t)p.value_dim * p.key_dim;
     float mine[DR_JOIN_ROWS];
@@ -1088,6 +1097,8 @@ dr_gradient_kernel(const __grid_constant__ DrGradient p) {
     extern __shared__ __align__(128) uint8_t dr_smem[];
     auto& sm = *(Smem*)dr_smem;
     const DrShape& sh = p.sh;
+    dr_let_next_start();
+    dr_wait_for_last();
     const uint64_t slot = blockIdx.x / sh.key_heads;
     const uint32_t hk = blockIdx.x % sh.key_heads, group = sh.heads / sh.key_heads, h0 = hk * group;
     const DrChunk c(sh, slot);
@@ -1497,6 +1508,7 @@ struct DrFills {
     DrFill f[5];
 };
 __global__ void __launch_bounds__(256) dr_padding_kernel(DrShape sh, DrFills fills) {
+    dr_let_next_start();
     const uint64_t first = min((uint64_t)sh.offsets[0], sh.rows), last = min((uint64_t)sh.offsets[sh.sequences], sh.rows);
     const uint64_t outside = first + (sh.rows - last);
     for (uint64_t i = blockIdx.x; i < outside; i += gridDim.x) {
@@ -1689,14 +1701,28 @@ static bool dr_sized(size_t smem) {
     sized.fetch_or(bit, std::memory_order_relaxed);
     return true;
 }
+// follows: the kernel starts while the call's one before ends (programmatic dependent launch); every kernel lets the next
+// one in when it starts itself, and waits for the end of the one before ahead of its first access to memory.
 template <auto KERNEL, typename A>
-static lcpp_status dr_launch(const char* name, uint64_t grid, unsigned threads, size_t smem, cudaStream_t s, const A& args) {
+static lcpp_status dr_launch(const char* name, uint64_t grid, unsigned threads, size_t smem, bool follows, cudaStream_t s, const A& args) {
     if (grid > 0x7fffffffull) return LCPP_ERR_INVALID_ARG;
     if (!dr_sized<KERNEL>(smem)) return check_launch();
+    cudaLaunchAttribute how[1];
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)grid);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cfg.attrs = how;
+    if (follows) {
+        how[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        how[0].val.programmaticStreamSerializationAllowed = 1;
+        cfg.numAttrs = 1;
+    }
     ProfScope prof(name, s);
-    KERNEL<<<(unsigned)grid, threads, smem, s>>>(args);
+    if (cudaLaunchKernelEx(&cfg, KERNEL, args) != cudaSuccess) return check_launch();
     count_launch();
-    return check_launch();
+    return LCPP_OK;
 }
 
 // How many warps a CTA of the chain has, 16 value dimensions each: fewer where that spreads `streams` over more SMs.
@@ -1718,8 +1744,8 @@ static lcpp_status dr_chain_pass(const DrChain& p, cudaStream_t s) {
         const uint64_t grid = streams * (ceil_div(p.sh.value_dim, WARPS * 16) + (WHAT == DR_STATES ? ceil_div(p.sh.key_dim, WARPS * 16) : 0));
         constexpr size_t smem = sizeof(DrChainSmem<T, DK, WARPS>);
         static_assert(smem <= 227 * 1024, "shared memory of a CTA");
-        if constexpr (BACKWARD) return dr_launch<dr_backward_kernel<T, DK, WARPS, WHAT>>(WHAT == DR_ALL ? "dr_backward" : "dr_states", grid, WARPS * 32, smem, s, p);
-        else return dr_launch<dr_forward_kernel<T, DK, WARPS, WHAT>>(WHAT == DR_ALL ? "dr_forward" : "dr_states", grid, WARPS * 32, smem, s, p);
+        if constexpr (BACKWARD) return dr_launch<dr_backward_kernel<T, DK, WARPS, WHAT>>(WHAT == DR_ALL ? "dr_backward" : "dr_states", grid, WARPS * 32, smem, p.sh.rows > 0, s, p);
+        else return dr_launch<dr_forward_kernel<T, DK, WARPS, WHAT>>(WHAT == DR_ALL ? "dr_forward" : "dr_states", grid, WARPS * 32, smem, p.sh.rows > 0, s, p);
     };
     if constexpr (WHAT == DR_STATES) return chain(std::integral_constant<int, 8>{});  // there are parts enough
     else {
@@ -1739,7 +1765,7 @@ static lcpp_status dr_chain(DrChain p, const DrLayout& l, void* temp, cudaStream
         if (status != LCPP_OK) return status;
         const DrJoin j{p.from, p.local, p.map, (float*)(t + l.before), p.sh.heads, p.sh.key_dim, p.sh.value_dim, p.parts,
                        (uint32_t)ceil_div(p.sh.value_dim, DR_JOIN_ROWS), BACKWARD};
-        status = dr_launch<dr_join_kernel>("dr_join", (uint64_t)p.sh.sequences * p.sh.heads * j.slices, 128, 0, s, j);
+        status = dr_launch<dr_join_kernel>("dr_join", (uint64_t)p.sh.sequences * p.sh.heads * j.slices, 128, 0, true, s, j);
         if (status != LCPP_OK) return status;
         p.from = j.before;
     }
@@ -1850,7 +1876,7 @@ extern "C" lcpp_status lcpp_delta_rule_forward(int dtype, const lcpp_delta_shape
             lcpp_status status = LCPP_OK;
             if (sh.rows)
                 status = dr_launch<dr_prepare_kernel<T, DK, false>>("dr_prepare", l.slots * sh.key_heads, DR_PREPARE_THREADS,
-                                                                    sizeof(DrPrepareSmem<DK, PLANES>), s, pr);
+                                                                    sizeof(DrPrepareSmem<DK, PLANES>), sh.offsets != nullptr, s, pr);
             return status != LCPP_OK ? status : dr_chain<T, DK, false>(p, l, temp, s);
         });
     });
@@ -1914,12 +1940,12 @@ extern "C" lcpp_status lcpp_delta_rule_backward(int dtype, const lcpp_delta_shap
             lcpp_status status = LCPP_OK;
             if (sh.rows)
                 status = dr_launch<dr_prepare_kernel<T, DK, true>>("dr_prepare", l.slots * sh.key_heads, DR_PREPARE_THREADS,
-                                                                   sizeof(DrPrepareSmem<DK, PLANES>), s, pr);
+                                                                   sizeof(DrPrepareSmem<DK, PLANES>), sh.offsets != nullptr, s, pr);
             if (status == LCPP_OK) status = dr_chain<T, DK, true>(p, l, temp, s);
             if (status != LCPP_OK || !sh.rows) return status;
             const uint64_t grid = l.slots * sh.key_heads;
-            if (sh.heads > sh.key_heads) return dr_launch<dr_gradient_kernel<T, DK, true>>("dr_gradient", grid, DR_GRAD_THREADS, smem, s, gr);
-            return dr_launch<dr_gradient_kernel<T, DK, false>>("dr_gradient", grid, DR_GRAD_THREADS, smem, s, gr);
+            if (sh.heads > sh.key_heads) return dr_launch<dr_gradient_kernel<T, DK, true>>("dr_gradient", grid, DR_GRAD_THREADS, smem, true, s, gr);
+            return dr_launch<dr_gradient_kernel<T, DK, false>>("dr_gradient", grid, DR_GRAD_THREADS, smem, true, s, gr);
         });
     });
 }
