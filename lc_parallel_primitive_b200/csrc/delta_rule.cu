@@ -651,17 +651,22 @@ struct DrChainCta {
         }
         __syncwarp();
     }
+    // A sum takes its next product some 24 cycles after the last, three issues of products: all tiles take one before any
+    // takes the next.
     // c (16 x 64: value x token) += s (16 x 16 kk .. 16 kk + 16) K^T
     __device__ __forceinline__ void times_keys(float (&c)[8][4], const uint32_t (&hi)[4], const uint32_t (&lo)[4], uint32_t k, int kk) const {
 #pragma unroll
-        for (int i = 0; i < PLANES; ++i)
+        for (int i = 0; i < PLANES; ++i) {
+            uint32_t b[4][4];
 #pragma unroll
-            for (int n = 0; n < 4; ++n) {
-                uint32_t b[4];
-                load_b(b, k + (i * NB + (kk >> 2)) * DR_BLOCK, n * 16, kk & 3, o);
-                mma_f16_2(c[2 * n], c[2 * n + 1], hi, b);
-                if (i == 0) mma_f16_2(c[2 * n], c[2 * n + 1], lo, b);
+            for (int n = 0; n < 4; ++n) load_b(b[n], k + (i * NB + (kk >> 2)) * DR_BLOCK, n * 16, kk & 3, o);
+#pragma unroll
+            for (int n = 0; n < 4; ++n) mma_f16_2(c[2 * n], c[2 * n + 1], hi, b[n]);
+            if (i == 0) {
+#pragma unroll
+                for (int n = 0; n < 4; ++n) mma_f16_2(c[2 * n], c[2 * n + 1], lo, b[n]);
             }
+        }
     }
     // s (16 x DK) += a (16 x tokens 16 kt .. 16 kt + 16) times the rows of K or Q
     template <bool EXACT>
@@ -669,11 +674,16 @@ struct DrChainCta {
 #pragma unroll
         for (int i = 0; i < PLANES; ++i)
 #pragma unroll
-            for (int n = 0; n < DK / 16; ++n) {
-                uint32_t b[4];
-                load_b_t(b, tile + (i * NB + (n >> 2)) * DR_BLOCK, kt * 16, n & 3, o);
-                mma_f16_2(s[2 * n], s[2 * n + 1], hi, b);
-                if (i == 0 && !EXACT) mma_f16_2(s[2 * n], s[2 * n + 1], lo, b);
+            for (int m = 0; m < DK / 64; ++m) {
+                uint32_t b[4][4];
+#pragma unroll
+                for (int n = 0; n < 4; ++n) load_b_t(b[n], tile + (i * NB + m) * DR_BLOCK, kt * 16, n, o);
+#pragma unroll
+                for (int n = 0; n < 4; ++n) mma_f16_2(s[8 * m + 2 * n], s[8 * m + 2 * n + 1], hi, b[n]);
+                if (i == 0 && !EXACT) {
+#pragma unroll
+                    for (int n = 0; n < 4; ++n) mma_f16_2(s[8 * m + 2 * n], s[8 * m + 2 * n + 1], lo, b[n]);
+                }
             }
     }
     // The state's fragment kk to an image.
@@ -725,14 +735,17 @@ dr_forward_kernel(const __grid_constant__ DrChain p) {
             if (states) cta.keep_state(states, hi, lo, kk);
             cta.times_keys(r, hi, lo, k, kk);
 #pragma unroll
-            for (int i = 0; ALL && i < PLANES; ++i)
+            for (int i = 0; ALL && i < PLANES; ++i) {
+                uint32_t a[4][4];
 #pragma unroll
-                for (int m = 0; m < 4; ++m) {
-                    uint32_t a[4];
-                    load_a(a, q + (i * NB + (kk >> 2)) * DR_BLOCK, m * 16, kk & 3, o);
-                    mma_f16(y[m][0], a, hi[0], hi[2]), mma_f16(y[m][1], a, hi[1], hi[3]);
-                    if (FINE && i == 0) mma_f16(y[m][0], a, lo[0], lo[2]), mma_f16(y[m][1], a, lo[1], lo[3]);
+                for (int m = 0; m < 4; ++m) load_a(a[m], q + (i * NB + (kk >> 2)) * DR_BLOCK, m * 16, kk & 3, o);
+#pragma unroll
+                for (int m = 0; m < 4; ++m) mma_f16(y[m][0], a[m], hi[0], hi[2]), mma_f16(y[m][1], a[m], hi[1], hi[3]);
+                if (FINE && i == 0) {
+#pragma unroll
+                    for (int m = 0; m < 4; ++m) mma_f16(y[m][0], a[m], lo[0], lo[2]), mma_f16(y[m][1], a[m], lo[1], lo[3]);
                 }
+            }
         }
         const float back_state = ss.back * back_domain;
         // r = V - g S0 K^T
@@ -757,15 +770,17 @@ dr_forward_kernel(const __grid_constant__ DrChain p) {
         for (int kt = 0; kt < 4; ++kt) {
             uint32_t hi[4], lo[4];
             split_block(r[2 * kt], r[2 * kt + 1], sr.by, hi, lo);
+            uint32_t b[4][4];
 #pragma unroll
-            for (int n = kt; n < 4; ++n) {
-                uint32_t b[4];
-                load_b(b, inv, n * 16, kt, o);
-                mma_f16_2(w[2 * n], w[2 * n + 1], hi, b);
-                mma_f16_2(w[2 * n], w[2 * n + 1], lo, b);
-                load_b(b, inv + DR_BLOCK, n * 16, kt, o);
-                mma_f16_2(w[2 * n], w[2 * n + 1], hi, b);
-            }
+            for (int n = kt; n < 4; ++n) load_b(b[n], inv, n * 16, kt, o);
+#pragma unroll
+            for (int n = kt; n < 4; ++n) mma_f16_2(w[2 * n], w[2 * n + 1], hi, b[n]);
+#pragma unroll
+            for (int n = kt; n < 4; ++n) mma_f16_2(w[2 * n], w[2 * n + 1], lo, b[n]);
+#pragma unroll
+            for (int n = kt; n < 4; ++n) load_b(b[n], inv + DR_BLOCK, n * 16, kt, o);
+#pragma unroll
+            for (int n = kt; n < 4; ++n) mma_f16_2(w[2 * n], w[2 * n + 1], hi, b[n]);
         }
         const float back_w = sr.back * gt.back_inverse;
         if (ALL && p.kept.at) {
@@ -799,16 +814,18 @@ dr_forward_kernel(const __grid_constant__ DrChain p) {
             for (int kt = 0; kt < 4; ++kt) {
                 uint32_t hi[4], lo[4];
                 split_block(w[2 * kt], w[2 * kt + 1], su.by, hi, lo);
+                uint32_t a[4][4];
 #pragma unroll
-                for (int m = kt; m < 4; ++m) {
-                    uint32_t a[4];
-                    load_a(a, rd, m * 16, kt, o);
-                    mma_f16(y[m][0], a, hi[0], hi[2]), mma_f16(y[m][1], a, hi[1], hi[3]);
-                    if constexpr (FINE) {
-                        mma_f16(y[m][0], a, lo[0], lo[2]), mma_f16(y[m][1], a, lo[1], lo[3]);
-                        load_a(a, rd + DR_BLOCK, m * 16, kt, o);
-                        mma_f16(y[m][0], a, hi[0], hi[2]), mma_f16(y[m][1], a, hi[1], hi[3]);
-                    }
+                for (int m = kt; m < 4; ++m) load_a(a[m], rd, m * 16, kt, o);
+#pragma unroll
+                for (int m = kt; m < 4; ++m) mma_f16(y[m][0], a[m], hi[0], hi[2]), mma_f16(y[m][1], a[m], hi[1], hi[3]);
+                if constexpr (FINE) {
+#pragma unroll
+                    for (int m = kt; m < 4; ++m) mma_f16(y[m][0], a[m], lo[0], lo[2]), mma_f16(y[m][1], a[m], lo[1], lo[3]);
+#pragma unroll
+                    for (int m = kt; m < 4; ++m) load_a(a[m], rd + DR_BLOCK, m * 16, kt, o);
+#pragma unroll
+                    for (int m = kt; m < 4; ++m) mma_f16(y[m][0], a[m], hi[0], hi[2]), mma_f16(y[m][1], a[m], hi[1], hi[3]);
                 }
             }
             {
@@ -918,15 +935,19 @@ dr_backward_kernel(const __grid_constant__ DrChain p) {
                 dr_raw_get<T>(v, raw, kt * 16, lane);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) split_f16(v[j][0], v[j][1], so.by, hi[j], lo[j]);
+                uint32_t b[4][4];
 #pragma unroll
-                for (int n = 0; n <= kt; ++n) {
-                    uint32_t b[4];
-                    load_b_t(b, rd, kt * 16, n, o);
-                    mma_f16_2(du[2 * n], du[2 * n + 1], hi, b);
-                    if constexpr (!EXACT) mma_f16_2(du[2 * n], du[2 * n + 1], lo, b);
-                    load_b_t(b, rd + DR_BLOCK, kt * 16, n, o);
-                    mma_f16_2(du[2 * n], du[2 * n + 1], hi, b);
+                for (int n = 0; n <= kt; ++n) load_b_t(b[n], rd, kt * 16, n, o);
+#pragma unroll
+                for (int n = 0; n <= kt; ++n) mma_f16_2(du[2 * n], du[2 * n + 1], hi, b[n]);
+                if constexpr (!EXACT) {
+#pragma unroll
+                    for (int n = 0; n <= kt; ++n) mma_f16_2(du[2 * n], du[2 * n + 1], lo, b[n]);
                 }
+#pragma unroll
+                for (int n = 0; n <= kt; ++n) load_b_t(b[n], rd + DR_BLOCK, kt * 16, n, o);
+#pragma unroll
+                for (int n = 0; n <= kt; ++n) mma_f16_2(du[2 * n], du[2 * n + 1], hi, b[n]);
             }
         }
         cta.ahead(it);
@@ -937,15 +958,17 @@ dr_backward_kernel(const __grid_constant__ DrChain p) {
         for (int kt = 0; kt < 4; ++kt) {
             uint32_t hi[4], lo[4];
             split_block(du[2 * kt], du[2 * kt + 1], sd.by, hi, lo);
+            uint32_t b[4][4];
 #pragma unroll
-            for (int n = 0; n <= kt; ++n) {
-                uint32_t b[4];
-                load_b_t(b, inv, kt * 16, n, o);
-                mma_f16_2(z[2 * n], z[2 * n + 1], hi, b);
-                mma_f16_2(z[2 * n], z[2 * n + 1], lo, b);
-                load_b_t(b, inv + DR_BLOCK, kt * 16, n, o);
-                mma_f16_2(z[2 * n], z[2 * n + 1], hi, b);
-            }
+            for (int n = 0; n <= kt; ++n) load_b_t(b[n], inv, kt * 16, n, o);
+#pragma unroll
+            for (int n = 0; n <= kt; ++n) mma_f16_2(z[2 * n], z[2 * n + 1], hi, b[n]);
+#pragma unroll
+            for (int n = 0; n <= kt; ++n) mma_f16_2(z[2 * n], z[2 * n + 1], lo, b[n]);
+#pragma unroll
+            for (int n = 0; n <= kt; ++n) load_b_t(b[n], inv + DR_BLOCK, kt * 16, n, o);
+#pragma unroll
+            for (int n = 0; n <= kt; ++n) mma_f16_2(z[2 * n], z[2 * n + 1], hi, b[n]);
         }
         const float back_z = sd.back * gt.back_inverse * so.back * gt.back_read;
         if constexpr (ALL) {
