@@ -36,6 +36,7 @@ constexpr float DR_LEAST_DECAY = -150.0f;       // exp of less is 0 in float32 a
 struct DrShape {
     uint64_t rows, length;
     const uint32_t* offsets;
+    const uint32_t* order;  // of the chains: the sequences' numbers, long ones first (null: as they come)
     uint32_t sequences, heads, key_heads, key_dim, value_dim;
     float scale;
     __device__ __forceinline__ uint64_t start(uint32_t s) const { return offsets ? offsets[s] : s * length; }
@@ -555,6 +556,8 @@ struct DrChainCta {
         h = rest % sh.heads, rest /= sh.heads;
         const uint32_t part = rest % parts + (WHAT == DR_STATES && BACKWARD ? 1 : 0);
         seq = rest / parts, hk = h / (sh.heads / sh.key_heads);
+        dr_wait_for_last();
+        if (sh.order) seq = sh.order[seq];
         unit_rows = slice >= value_slices;
         if (unit_rows) slice -= value_slices;
         dim = unit_rows ? sh.key_dim : sh.value_dim;
@@ -583,7 +586,6 @@ struct DrChainCta {
     __device__ __forceinline__ uint32_t order(uint32_t it) const { return first + (BACKWARD ? chunks - 1 - it : it); }
     // The first images and values, and the state that they meet.
     __device__ __forceinline__ void open(float (&s)[NT][4]) {
-        dr_wait_for_last();
         if (warp == 0 && lane == 0)
             for (uint32_t i = 0; i < (uint32_t)STAGES && i < chunks; ++i) load(i, order(i));
         __syncwarp();
@@ -1545,6 +1547,36 @@ __global__ void __launch_bounds__(256) dr_padding_kernel(DrShape sh, DrFills fil
     }
 }
 
+// Sequences by their numbers of chunks, the longest first (by powers of two): a chain takes as long as its sequence, and a
+// long one that starts last is waited for.  One CTA; which order equals have changes no result.
+constexpr int DR_ORDER_THREADS = 1024;
+struct DrOrder {
+    DrShape sh;
+    uint32_t* order;
+};
+__global__ void __launch_bounds__(DR_ORDER_THREADS) dr_order_kernel(const __grid_constant__ DrOrder p) {
+    __shared__ uint32_t next[33];
+    dr_let_next_start();
+    dr_wait_for_last();
+    auto size = [&](uint32_t s) -> uint32_t {  // 0 the longest
+        const uint64_t from = p.sh.start(s), to = p.sh.start(s + 1);
+        return to > from ? __clz((uint32_t)((to - from + DR_CHUNK - 1) / DR_CHUNK)) : 32;
+    };
+    if (threadIdx.x < 33) next[threadIdx.x] = 0;
+    __syncthreads();
+    for (uint32_t s = threadIdx.x; s < p.sh.sequences; s += DR_ORDER_THREADS) atomicAdd(&next[size(s)], 1u);
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        uint32_t sum = 0;
+        for (int i = 0; i < 33; ++i) {
+            const uint32_t n = next[i];
+            next[i] = sum, sum += n;
+        }
+    }
+    __syncthreads();
+    for (uint32_t s = threadIdx.x; s < p.sh.sequences; s += DR_ORDER_THREADS) p.order[atomicAdd(&next[size(s)], 1u)] = s;
+}
+
 // ---- one token ------------------------------------------------------------------------------------
 constexpr int DR_STEP_WARPS = 4;
 // A warp takes 8 rows of a state (value dimensions) at a time: a lane holds 4 key columns of each.
@@ -1649,7 +1681,7 @@ static lcpp_status dr_check(int dtype, const lcpp_delta_shape* sh) {
     return LCPP_OK;
 }
 static DrShape dr_shape(const lcpp_delta_shape& sh) {
-    return DrShape{sh.rows, sh.offsets ? 0 : sh.length, sh.offsets, (uint32_t)sh.num_sequences, sh.heads, sh.key_heads,
+    return DrShape{sh.rows, sh.offsets ? 0 : sh.length, sh.offsets, nullptr, (uint32_t)sh.num_sequences, sh.heads, sh.key_heads,
                    sh.key_dim, sh.value_dim, sh.scale};
 }
 
@@ -1675,7 +1707,7 @@ struct DrLayout {
     uint64_t slots, units;
     uint32_t planes, key_cols, rows;  // rows of an image
     uint64_t parts;                   // of a sequence
-    size_t keys, unit, x, back_x, z, back_z, back_out, local, map, before, bytes;
+    size_t keys, unit, x, back_x, z, back_z, back_out, local, map, before, order, bytes;
     DrLayout(int dtype, const lcpp_delta_shape& sh, bool backward) {
         slots = sh.rows / DR_CHUNK + sh.num_sequences, units = slots * sh.heads;
         planes = dtype == LCPP_F32 ? 2 : 1, key_cols = sh.key_dim <= 64 ? 64 : 128, rows = (uint32_t)align_up(sh.value_dim, 32);
@@ -1692,6 +1724,7 @@ struct DrLayout {
             z = take(units * kept(nullptr, 0, 0).bytes()), back_z = take(units * 32);
             back_out = take(units * 32);
         }
+        order = take(sh.num_sequences * 4);
         parts = dr_parts(sh), local = map = before = 0;
         if (parts > 1) {
             const uint64_t pieces = sh.num_sequences * sh.heads * parts, state = (uint64_t)sh.value_dim * sh.key_dim;
@@ -1781,6 +1814,13 @@ static lcpp_status dr_chain_pass(const DrChain& p, cudaStream_t s) {
 template <typename T, int DK, bool BACKWARD>
 static lcpp_status dr_chain(DrChain p, const DrLayout& l, void* temp, cudaStream_t s) {
     p.parts = (uint32_t)l.parts;
+    // more chains than SMs, of different lengths: the order matters
+    if (p.sh.offsets && p.sh.sequences > 1 && (uint64_t)p.sh.sequences * p.sh.heads * ceil_div(p.sh.value_dim, 128) > (uint64_t)device_info().sms) {
+        const DrOrder o{p.sh, (uint32_t*)((char*)temp + l.order)};
+        const lcpp_status status = dr_launch<dr_order_kernel>("dr_order", 1, DR_ORDER_THREADS, 0, true, s, o);
+        if (status != LCPP_OK) return status;
+        p.sh.order = o.order;
+    }
     if (l.parts > 1) {
         char* const t = (char*)temp;
         p.local = (float*)(t + l.local), p.map = (float*)(t + l.map);

@@ -292,7 +292,7 @@ class DeviceDeltaRule(_Recorded):
         pq, sq, rows, key_heads, key_dim = _heads(d_q, "d_q")
         pk, sk, rk, hk, dk = _heads(d_k, "d_k")
         pv, sv, rv, heads, value_dim = _heads(d_v, "d_v")
-        if (rk, hk, dk) != (rows, key_heads, key_dim):
+        if rk != rows or hk != key_heads or dk != key_dim:
             raise ValueError("d_q and d_k must have the same shape")
         if rv != rows:
             raise ValueError("d_v must have the rows of d_q")
@@ -300,12 +300,8 @@ class DeviceDeltaRule(_Recorded):
             raise ValueError(f"{heads} heads are no whole number for each of {key_heads} key heads")
         if key_dim > 128 or value_dim > 128 or not key_dim or not value_dim:
             raise ValueError("key_dim and value_dim must be from 1 to 128")
-        if d_beta.dtype != torch.float32 or (d_decay is not None and d_decay.dtype != torch.float32):
-            raise TypeError("d_decay and d_beta must have the element type torch.float32")
-        pb, sb, rb, hb = _matrix(d_beta, "d_beta")
-        pd, sd, rd, hd = (None, 0, rb, hb) if d_decay is None else _matrix(d_decay, "d_decay")
-        if (rb, hb) != (rows, heads) or (rd, hd) != (rows, heads):
-            raise ValueError(f"d_decay and d_beta must have the shape {(rows, heads)}")
+        pb, sb = _gates(d_beta, rows, heads)
+        pd, sd = (None, 0) if d_decay is None else _gates(d_decay, rows, heads)
         return L.DeltaInputs(pq, pk, pv, sq, sk, sv, pd, pb, sd, sb, None), rows, heads, key_heads, key_dim, value_dim
 
     def _sequences(self, inputs, offsets_or_length, rows, heads, key_heads, key_dim, value_dim, d_init, scale):
@@ -386,22 +382,44 @@ class DeviceDeltaRule(_Recorded):
         keep = (d_q, d_k, d_v, d_decay, d_beta, d_states_in, d_states_out, d_out, d_parents)
         _one_device(*keep)
         inputs, rows, heads, key_heads, key_dim, value_dim = self._inputs(d_q, d_k, d_v, d_decay, d_beta)
-        rows_in = 0 if d_states_in is None else d_states_in.shape[0]
-        inputs.init = _dense(d_states_in, (rows_in, heads, value_dim, key_dim), _F32, "d_states_in")
-        pn = _dense(d_states_out, (rows, heads, value_dim, key_dim), _F32, "d_states_out")
+        state = (heads, value_dim, key_dim)
+        rows_in = 0
+        if d_states_in is not None:
+            rows_in = d_states_in.shape[0]
+            inputs.init = _dense(d_states_in, (rows_in, *state), _F32, "d_states_in")
+        pn = _dense(d_states_out, (rows, *state), _F32, "d_states_out")
         pp = _dense(d_parents, (rows,), _I32, "d_parents")
-        po, so, *like = _heads(d_out, "d_out")
-        if like != [rows, heads, value_dim]:
+        po, so, r, h, d = _heads(d_out, "d_out")
+        if r != rows or h != heads or d != value_dim:
             raise ValueError("d_out must have the shape of d_v")
-        shape = self._shape(rows, 0, heads, key_heads, key_dim, value_dim, scale=key_dim ** -0.5 if scale is None else scale)
+        if scale is None:
+            scale = key_dim ** -0.5
+        shape = L.DeltaShape(rows, 0, 0, None, heads, key_heads, key_dim, value_dim, scale)
         self._call(cmdlist, L.lib().lcpp_delta_rule_step, (dt, shape, inputs, rows_in, pp, pn, po, so), keep,
                    "DeviceDeltaRule.Step")
+
+
+def _gates(t, rows, heads):
+    """(pointer, row stride) of decays or strengths."""
+    if t.dtype != torch.float32:
+        raise TypeError("d_decay and d_beta must have the element type torch.float32")
+    shape = t.shape
+    if len(shape) == 2 and shape[0] == rows and shape[1] == heads and t.is_contiguous():  # the usual one
+        return t.data_ptr(), heads
+    pointer, row, r, h = _matrix(t, "d_decay and d_beta")
+    if r != rows or h != heads:
+        raise ValueError(f"d_decay and d_beta must have the shape {(rows, heads)}")
+    return pointer, row
 
 
 def _heads(t, name):
     """(pointer, row stride, rows, heads, dim) of a (rows, heads, dim) or (batch, time, heads, dim) tensor whose rows are
     one stride apart and whose heads are adjacent."""
-    shape, stride = t.shape, t.stride()
+    shape = t.shape
+    if len(shape) == 3 and t.is_contiguous():  # the usual one
+        rows, heads, dim = shape
+        return t.data_ptr(), heads * dim, rows, heads, dim
+    stride = t.stride()
     if len(shape) == 4:
         batch, time, heads, dim = shape
         rows, row = batch * time, stride[1]
