@@ -88,13 +88,6 @@ struct DrImage {
     __device__ __forceinline__ uint8_t* of(uint64_t unit) const { return at + unit * bytes(); }
 };
 
-// Stores elements (row, col), (row, col + 1), col even, of a matrix with `blocks` blocks in its rows.
-__device__ __forceinline__ void dr_store(uint8_t* image, uint32_t blocks, uint32_t row, uint32_t col, uint32_t hi, uint32_t lo) {
-    uint8_t* const at = image + ((row >> 5) * 2 * blocks + (col >> 6)) * DR_PIECE + block_at(row & 31, col & 63);
-    *(uint32_t*)at = hi;
-    *(uint32_t*)(at + blocks * DR_PIECE) = lo;
-}
-
 // ---- what does not depend on the state ------------------------------------------------------------
 __device__ __forceinline__ void dr_let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void dr_wait_for_last() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
@@ -688,14 +681,21 @@ struct DrChainCta {
                 }
             }
     }
-    // The state's fragment kk to an image.
-    __device__ __forceinline__ void keep_state(uint8_t* image, const uint32_t (&hi)[4], const uint32_t (&lo)[4], int kk) const {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) dr_store(image, NB, row + (j & 1) * 8, kk * 16 + (j >> 1) * 8 + col, hi[j], lo[j]);
+    // Where the thread's elements of an image with `blocks` blocks a row lie, but for the piece of 8 columns, whose number's
+    // bits 4 .. 6 are exclusive or-ed with (its rows g and g + 8 permute alike).
+    __device__ __forceinline__ uint8_t* mine(uint8_t* image, uint32_t blocks) const {
+        return image + (row >> 5) * (2 * blocks * DR_PIECE) + (row & 31) * BLOCK_ROW + (g << 4) + col * 2;
     }
-    __device__ __forceinline__ void keep_values(uint8_t* image, const uint32_t (&hi)[4], const uint32_t (&lo)[4], int kt) const {
+    static __device__ __forceinline__ uint32_t* piece(uint8_t* at, int number) { return (uint32_t*)((uintptr_t)at ^ (uintptr_t)(number << 4)); }
+    // The fragment of columns 16 kk .. of the warp's 16 rows to an image, from mine().
+    template <int BLOCKS>
+    static __device__ __forceinline__ void keep(uint8_t* at, const uint32_t (&hi)[4], const uint32_t (&lo)[4], int kk) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) dr_store(image, 1, row + (j & 1) * 8, kt * 16 + (j >> 1) * 8 + col, hi[j], lo[j]);
+        for (int j = 0; j < 4; ++j) {
+            uint32_t* const to = piece(at, (kk & 3) * 2 + (j >> 1)) + ((kk >> 2) * DR_PIECE + (j & 1) * 8 * BLOCK_ROW) / 4;
+            to[0] = hi[j];
+            to[BLOCKS * DR_PIECE / 4] = lo[j];
+        }
     }
     __device__ __forceinline__ void keep_back(float* back, uint64_t unit, float v) const {
         if (lane == 0) back[unit * 8 + (v0 >> 4) + warp] = v;
@@ -728,13 +728,13 @@ dr_forward_kernel(const __grid_constant__ DrChain p) {
         // r = S0 K^T (value x token) and out = Q S0^T (token x value)
         float r[8][4] = {}, y[4][2][4] = {};
         const Scale ss = coarse_scale_for(max_abs(s));
-        uint8_t* const states = ALL && p.states.at ? p.states.of(unit) : nullptr;
+        uint8_t* const states = ALL && p.states.at ? cta.mine(p.states.of(unit), NB) : nullptr;
         if (states) cta.keep_back(p.states.back, unit, ss.back * back_domain);
 #pragma unroll
         for (int kk = 0; kk < DK / 16; ++kk) {
             uint32_t hi[4], lo[4];
             split_block(s[2 * kk], s[2 * kk + 1], ss.by, hi, lo);
-            if (states) cta.keep_state(states, hi, lo, kk);
+            if (states) Cta::template keep<NB>(states, hi, lo, kk);
             cta.times_keys(r, hi, lo, k, kk);
 #pragma unroll
             for (int i = 0; ALL && i < PLANES; ++i) {
@@ -761,7 +761,7 @@ dr_forward_kernel(const __grid_constant__ DrChain p) {
             for (int x = 0; x < 4; ++x) {
                 const float2 gate = *(const float2*)&gt.g[n * 16 + (x >> 1) * 8 + col];
                 float* const d = &r[2 * n + (x >> 1)][(x & 1) * 2];
-                d[0] = fmaf(gate.x * back_r, d[0], v[x][0]), d[1] = fmaf(gate.y * back_r, d[1], v[x][1]);
+                pair_split(pair_fma(pair_mul(pair_of(gate.x, gate.y), pair_of(back_r, back_r)), pair_of(d[0], d[1]), pair_of(v[x][0], v[x][1])), d[0], d[1]);
             }
         }
         cta.ahead(it);
@@ -787,19 +787,20 @@ dr_forward_kernel(const __grid_constant__ DrChain p) {
         const float back_w = sr.back * gt.back_inverse;
         if (ALL && p.kept.at) {
             const Scale sw = coarse_scale_for(max_abs(w));
-            uint8_t* const kept = p.kept.of(unit);
+            uint8_t* const kept = cta.mine(p.kept.of(unit), 1);
             cta.keep_back(p.kept.back, unit, sw.back * back_w);
 #pragma unroll
             for (int kt = 0; kt < 4; ++kt) {
                 uint32_t hi[4], lo[4];
                 split_block(w[2 * kt], w[2 * kt + 1], sw.by, hi, lo);
-                cta.keep_values(kept, hi, lo, kt);
+                Cta::template keep<1>(kept, hi, lo, kt);
             }
         }
 #pragma unroll
         for (int n = 0; n < 8; ++n) {  // u
             const float2 b = *(const float2*)&gt.beta[n * 8 + col];
-            w[n][0] *= b.x * back_w, w[n][1] *= b.y * back_w, w[n][2] *= b.x * back_w, w[n][3] *= b.y * back_w;
+            const uint64_t by = pair_mul(pair_of(b.x, b.y), pair_of(back_w, back_w));
+            scale_pair(w[n][0], w[n][1], by), scale_pair(w[n][2], w[n][3], by);
         }
         if constexpr (ALL) {  // out = scale g out + A u
             const Scale su = scale_for(max_abs(w));
@@ -809,7 +810,7 @@ dr_forward_kernel(const __grid_constant__ DrChain p) {
                 for (int m = 0; m < 4; ++m) {
                     const float g0 = gt.g[m * 16 + g] * by * into, g1 = gt.g[m * 16 + g + 8] * by * into;
 #pragma unroll
-                    for (int n = 0; n < 2; ++n) y[m][n][0] *= g0, y[m][n][1] *= g0, y[m][n][2] *= g1, y[m][n][3] *= g1;
+                    for (int n = 0; n < 2; ++n) scale_pair(y[m][n][0], y[m][n][1], pair_of(g0, g0)), scale_pair(y[m][n][2], y[m][n][3], pair_of(g1, g1));
                 }
             }
 #pragma unroll
@@ -850,15 +851,12 @@ dr_forward_kernel(const __grid_constant__ DrChain p) {
 #pragma unroll
         for (int n = 0; n < 8; ++n) {
             const float2 e = *(const float2*)&gt.e[n * 8 + col];
-            w[n][0] *= e.x, w[n][1] *= e.y, w[n][2] *= e.x, w[n][3] *= e.y;
+            scale_pair(w[n][0], w[n][1], pair_of(e.x, e.y)), scale_pair(w[n][2], w[n][3], pair_of(e.x, e.y));
         }
         const Scale se = scale_for(max_abs(w));
         const float into = se.by * __frcp_rn(gt.back_k), whole = gt.g[DR_CHUNK - 1] * back_domain * into;
         back_domain = se.back * gt.back_k;
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) s[n][j] *= whole;
+        scale_all(s, whole);
 #pragma unroll
         for (int kt = 0; kt < 4; ++kt) {
             uint32_t hi[4], lo[4];
@@ -895,13 +893,13 @@ dr_backward_kernel(const __grid_constant__ DrChain p) {
         // du = e X K^T (value x token)
         float du[8][4] = {};
         const Scale sx = coarse_scale_for(max_abs(x));
-        uint8_t* const states = ALL ? p.states.of(unit) : nullptr;
+        uint8_t* const states = ALL ? cta.mine(p.states.of(unit), Cta::NB) : nullptr;
         if constexpr (ALL) cta.keep_back(p.states.back, unit, sx.back * back_domain);
 #pragma unroll
         for (int kk = 0; kk < DK / 16; ++kk) {
             uint32_t hi[4], lo[4];
             split_block(x[2 * kk], x[2 * kk + 1], sx.by, hi, lo);
-            if constexpr (ALL) cta.keep_state(states, hi, lo, kk);
+            if constexpr (ALL) Cta::template keep<Cta::NB>(states, hi, lo, kk);
             cta.times_keys(du, hi, lo, k, kk);
         }
         // ... + dO^T A
@@ -926,7 +924,8 @@ dr_backward_kernel(const __grid_constant__ DrChain p) {
 #pragma unroll
             for (int n = 0; n < 8; ++n) {
                 const float2 e = *(const float2*)&gt.e[n * 8 + col];
-                du[n][0] *= e.x * back, du[n][1] *= e.y * back, du[n][2] *= e.x * back, du[n][3] *= e.y * back;
+                const uint64_t by = pair_mul(pair_of(e.x, e.y), pair_of(back, back));
+                scale_pair(du[n][0], du[n][1], by), scale_pair(du[n][2], du[n][3], by);
             }
         }
         if (cta.values) {
@@ -975,23 +974,20 @@ dr_backward_kernel(const __grid_constant__ DrChain p) {
         const float back_z = sd.back * gt.back_inverse * so.back * gt.back_read;
         if constexpr (ALL) {
             const Scale sz = coarse_scale_for(max_abs(z));
-            uint8_t* const kept = p.kept.of(unit);
+            uint8_t* const kept = cta.mine(p.kept.of(unit), 1);
             cta.keep_back(p.kept.back, unit, sz.back * back_z);
 #pragma unroll
             for (int kt = 0; kt < 4; ++kt) {
                 uint32_t hi[4], lo[4];
                 split_block(z[2 * kt], z[2 * kt + 1], sz.by, hi, lo);
-                cta.keep_values(kept, hi, lo, kt);
+                Cta::template keep<1>(kept, hi, lo, kt);
             }
         }
         // X = g_64 X + (scale g dO)^T Q - (g beta z)^T K, each in the domain of its product
         float into = gt.g[DR_CHUNK - 1] * back_domain;
         if (cta.values) {
             into *= sg.by * __frcp_rn(gt.back_q);
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) x[n][j] *= into;
+            scale_all(x, into);
 #pragma unroll
             for (int kt = 0; kt < 4; ++kt) {
                 float v[4][2];
@@ -1009,16 +1005,13 @@ dr_backward_kernel(const __grid_constant__ DrChain p) {
 #pragma unroll
         for (int n = 0; n < 8; ++n) {
             const float2 gate = *(const float2*)&gt.g[n * 8 + col], b = *(const float2*)&gt.beta[n * 8 + col];
-            const float y0 = -gate.x * b.x * back_z, y1 = -gate.y * b.y * back_z;
-            z[n][0] *= y0, z[n][1] *= y1, z[n][2] *= y0, z[n][3] *= y1;
+            const uint64_t by = pair_of(-gate.x * b.x * back_z, -gate.y * b.y * back_z);
+            scale_pair(z[n][0], z[n][1], by), scale_pair(z[n][2], z[n][3], by);
         }
         const Scale sy = scale_for(max_abs(z));
         into *= sy.by * __frcp_rn(gt.back_k);
         back_domain = sy.back * gt.back_k;
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) x[n][j] *= into;
+        scale_all(x, into);
 #pragma unroll
         for (int kt = 0; kt < 4; ++kt) {
             uint32_t hi[4], lo[4];

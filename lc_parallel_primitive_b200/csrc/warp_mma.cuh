@@ -94,14 +94,48 @@ __device__ __forceinline__ Scale coarse_scale_for(float most) {
 __device__ __forceinline__ float warp_max(float v) {  // of values >= 0
     return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(v)));
 }
+__device__ __forceinline__ float max3_abs(float m, float x, float y) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(m), "f"(fabsf(x)), "f"(fabsf(y)));
+    return r;
+}
 template <int N>
 __device__ __forceinline__ float max_abs(const float (&c)[N][4]) {  // of the warp's accumulators
-    float m = 0.0f;
+    float m0 = 0.0f, m1 = 0.0f;
 #pragma unroll
-    for (int n = 0; n < N; ++n)
+    for (int n = 0; n < N; ++n) m0 = max3_abs(m0, c[n][0], c[n][1]), m1 = max3_abs(m1, c[n][2], c[n][3]);
+    return warp_max(fmaxf(m0, m1));
+}
+
+// ---- two float32 at a time -------------------------------------------------------------------------
+__device__ __forceinline__ uint64_t pair_of(float x, float y) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ void pair_split(uint64_t v, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v)); }
+__device__ __forceinline__ uint64_t pair_mul(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t pair_sub(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("sub.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t pair_fma(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+// (x, y) *= (a, b)
+__device__ __forceinline__ void scale_pair(float& x, float& y, uint64_t by) { pair_split(pair_mul(pair_of(x, y), by), x, y); }
+template <int N>
+__device__ __forceinline__ void scale_all(float (&c)[N][4], float by) {
+    const uint64_t b = pair_of(by, by);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) m = fmaxf(m, fabsf(c[n][j]));
-    return warp_max(m);
+    for (int n = 0; n < N; ++n) scale_pair(c[n][0], c[n][1], b), scale_pair(c[n][2], c[n][3], b);
 }
 
 __device__ __forceinline__ uint32_t pack_f16(float x, float y) {
@@ -111,9 +145,13 @@ __device__ __forceinline__ uint32_t pack_f16(float x, float y) {
 }
 __device__ __forceinline__ float2 unpack_f16(uint32_t v) { return __half22float2(*(const __half2*)&v); }
 __device__ __forceinline__ void split_f16(float x, float y, float s, uint32_t& hi, uint32_t& lo) {
-    hi = pack_f16(x * s, y * s);
+    const uint64_t v = pair_mul(pair_of(x, y), pair_of(s, s));  // exact but where it is far below the largest
+    float a, b;
+    pair_split(v, a, b);
+    hi = pack_f16(a, b);
     const float2 h = unpack_f16(hi);
-    lo = pack_f16(fmaf(x, s, -h.x), fmaf(y, s, -h.y));
+    pair_split(pair_sub(v, pair_of(h.x, h.y)), a, b);
+    lo = pack_f16(a, b);
 }
 // Accumulators of two neighbouring 16 x 8 tiles as the fragment of the 16 x 16 block they are: as A (m = rows), and as
 // two B fragments with n = rows: (f[0], f[2]) rows 0-7, (f[1], f[3]) rows 8-15.
