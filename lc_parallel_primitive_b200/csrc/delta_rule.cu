@@ -805,7 +805,7 @@ dr_forward_kernel(const __grid_constant__ DrChain p) {
         if constexpr (ALL) {  // out = scale g out + A u
             const Scale su = scale_for(max_abs(w));
             {
-                const float by = p.sh.scale * back_state * gt.back_q, into = su.by * __frcp_rn(gt.back_read);
+                const float by = p.sh.scale * back_state * gt.back_q, into = su.by * power_inverse(gt.back_read);
 #pragma unroll
                 for (int m = 0; m < 4; ++m) {
                     const float g0 = gt.g[m * 16 + g] * by * into, g1 = gt.g[m * 16 + g + 8] * by * into;
@@ -854,7 +854,7 @@ dr_forward_kernel(const __grid_constant__ DrChain p) {
             scale_pair(w[n][0], w[n][1], pair_of(e.x, e.y)), scale_pair(w[n][2], w[n][3], pair_of(e.x, e.y));
         }
         const Scale se = scale_for(max_abs(w));
-        const float into = se.by * __frcp_rn(gt.back_k), whole = gt.g[DR_CHUNK - 1] * back_domain * into;
+        const float into = se.by * power_inverse(gt.back_k), whole = gt.g[DR_CHUNK - 1] * back_domain * into;
         back_domain = se.back * gt.back_k;
         scale_all(s, whole);
 #pragma unroll
@@ -920,7 +920,7 @@ dr_backward_kernel(const __grid_constant__ DrChain p) {
         const Scale so = coarse_scale_for(warp_max(most)), sg = scale_for(warp_max(most_g) * fabsf(p.sh.scale));
         if constexpr (ALL) cta.keep_back(p.back_values, unit, so.back);
         {
-            const float back = sx.back * back_domain * gt.back_k * so.by * __frcp_rn(gt.back_read);
+            const float back = sx.back * back_domain * gt.back_k * so.by * power_inverse(gt.back_read);
 #pragma unroll
             for (int n = 0; n < 8; ++n) {
                 const float2 e = *(const float2*)&gt.e[n * 8 + col];
@@ -986,7 +986,7 @@ dr_backward_kernel(const __grid_constant__ DrChain p) {
         // X = g_64 X + (scale g dO)^T Q - (g beta z)^T K, each in the domain of its product
         float into = gt.g[DR_CHUNK - 1] * back_domain;
         if (cta.values) {
-            into *= sg.by * __frcp_rn(gt.back_q);
+            into *= sg.by * power_inverse(gt.back_q);
             scale_all(x, into);
 #pragma unroll
             for (int kt = 0; kt < 4; ++kt) {
@@ -1009,7 +1009,7 @@ dr_backward_kernel(const __grid_constant__ DrChain p) {
             scale_pair(z[n][0], z[n][1], by), scale_pair(z[n][2], z[n][3], by);
         }
         const Scale sy = scale_for(max_abs(z));
-        into *= sy.by * __frcp_rn(gt.back_k);
+        into *= sy.by * power_inverse(gt.back_k);
         back_domain = sy.back * gt.back_k;
         scale_all(x, into);
 #pragma unroll
@@ -1090,7 +1090,7 @@ struct DrGradientSmem {
     float by_out[8];                         // scales of dO
     float dbeta[DR_CHUNK];
     float dot[4][DR_CHUNK], carry[4][DR_CHUNK], most[2][16], sx[16];
-    uint64_t full[2], keys_full;
+    uint64_t full[2], empty[2], keys_full;
 };
 
 struct DrGradient {
@@ -1154,16 +1154,23 @@ dr_gradient_kernel(const __grid_constant__ DrGradient p) {
                 asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(q.x), "r"(q.y), "r"(q.z), "r"(q.w) : "memory");
             }
         }
+        // arrives when the thread's copies have landed, or now that it has stored
+        const uint32_t bar = smem_u32(&sm.full[it & 1]);
+        if (p.wide) asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+        else asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
     };
     if (t == 0) {
-        mbar_init(&sm.full[0], 1), mbar_init(&sm.full[1], 1), mbar_init(&sm.keys_full, 1);
+        for (int i = 0; i < 2; ++i) mbar_init(&sm.full[i], 1 + (p.out ? DR_GRAD_THREADS : 0)), mbar_init(&sm.empty[i], DR_GRAD_THREADS / 32);
+        mbar_init(&sm.keys_full, 1);
         fence_mbar_init();
+    }
+    __syncthreads();
+    if (t == 0) {
         mbar_arrive_expect_tx(&sm.keys_full, 2 * DR_KEYS<DK, PLANES>);
         bulk_load(sm.keys, p.keys + (slot * sh.key_heads + hk) * (2 * DR_KEYS<DK, PLANES>), 2 * DR_KEYS<DK, PLANES>, &sm.keys_full);
         load(0);
     }
     load_out(0);
-    cp_async_commit();
     const uint32_t k = smem_u32(sm.keys), q = k + DR_KEYS<DK, PLANES>, da = smem_u32(sm.da), dn = smem_u32(sm.dn);
     float all_q[SHARED ? NT : 1][4] = {}, all_k[SHARED ? NT : 1][4] = {};  // sums over the key head's heads
     const uint32_t token = rb * 16 + g;
@@ -1188,16 +1195,15 @@ dr_gradient_kernel(const __grid_constant__ DrGradient p) {
             if (warp == 4) sm.own[0][lane] = s, sm.own[1][lane] = x, sm.own[2][lane] = w, sm.own[3][lane] = z;
             if (warp == 0) sm.by_out[lane] = go > 0.0f ? 1.0f / go : 0.0f;
         }
+        __syncthreads();
         float dq[NT][4] = {}, er[NT][4] = {}, wr[NT][4] = {}, a[2][4] = {}, n[2][4] = {};
         float sx = 0.0f;
         for (uint32_t v = 0; v < steps; ++v, ++it) {
-            cp_async_wait_all();
-            __syncthreads();  // dO is there, and the buffers of the step before are free
-            if (it + 1 < total) {
+            if (it + 1 < total) {  // into the buffers that the warps left a step ago
+                if (it) ok = mbar_wait(&sm.empty[(it + 1) & 1], ((it - 1) >> 1) & 1, limit) && ok;
                 if (t == 0) load(it + 1);
                 load_out(it + 1);
             }
-            cp_async_commit();
             if (it == 0) ok = mbar_wait(&sm.keys_full, 0, limit) && ok;
             ok = mbar_wait(&sm.full[it & 1], (it >> 1) & 1, limit) && ok;
             const uint8_t* const step = sm.step[it & 1];
@@ -1328,6 +1334,8 @@ dr_gradient_kernel(const __grid_constant__ DrGradient p) {
                     sx = fmaf(mine, sm.own[0][at] * sm.own[1][at], sx);
                 }
             }
+            __syncwarp();
+            if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&sm.empty[it & 1])) : "memory");
         }
         // dbeta_i = w_i.z_i is the diagonal of n
 #pragma unroll
@@ -1372,7 +1380,7 @@ dr_gradient_kernel(const __grid_constant__ DrGradient p) {
         // row factors of the products with the states, into the domains of the products that follow; k.(e u X) is needed by
         // itself
         const float back_k = sm.gates.back_k, back_q = sm.gates.back_q;
-        const float by_k = __frcp_rn(back_k), into_q = sa.by * by_k, into_n = sn.by * by_k;
+        const float by_k = power_inverse(back_k), into_q = sa.by * by_k, into_n = sn.by * by_k;
         float carry[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
@@ -1400,7 +1408,7 @@ dr_gradient_kernel(const __grid_constant__ DrGradient p) {
 #pragma unroll
         for (int part = 0; part < 3; ++part) {
             if (part == 2) {
-                const float turn = sa.by * __frcp_rn(back_q) * sn.back * back_k;
+                const float turn = sa.by * power_inverse(back_q) * sn.back * back_k;
 #pragma unroll
                 for (int j = 0; j < NT; ++j)
 #pragma unroll

@@ -79,6 +79,8 @@ __device__ __forceinline__ void mma_f16_2(float (&c0)[4], float (&c1)[4], const 
 struct Scale {
     float by, back;
 };
+// 1 / v for a power of two between 2^-126 and 2^126.
+__device__ __forceinline__ float power_inverse(float v) { return __int_as_float(0x7f000000 - __float_as_int(v)); }
 // For the largest absolute value `most`: most * by is in [2^14, 2^15), by <= 2^45 (1 for zeros).
 __device__ __forceinline__ Scale scale_for(float most) {
     const int e = __float_as_int(most) >> 23 & 255;
