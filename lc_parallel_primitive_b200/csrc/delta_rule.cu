@@ -1084,12 +1084,12 @@ struct DrGradientSmem {
     alignas(128) uint8_t slab[2][DR_CHUNK * DR_SLAB_ROW<T>];
     alignas(128) uint8_t da[2 * DR_BLOCK];  // two planes
     uint8_t dn[2 * DR_BLOCK];
-    DrGates gates;
-    float factor[5][8], back[5], own[4][8];  // of 16 value dimensions: shares of the largest scale; scales; of S, X, w, z
-    uint32_t uneven[5];                      // whether not all factors of a product are 1
-    float by_out[8];                         // scales of dO
-    float dbeta[DR_CHUNK];
-    float dot[4][DR_CHUNK], carry[4][DR_CHUNK], most[2][16], sx[16];
+    alignas(128) DrGates gates[2];     // of a head and the next
+    alignas(32) float back[2][5][8];   // inverse scales of S, X, w, z and dO by 16 value dimensions
+    float dbeta[2][DR_CHUNK];
+    float scales[16][5];               // of a warp's products
+    float dot[4][DR_CHUNK], carry[4][DR_CHUNK], sx[16];
+    alignas(16) float most[2][16];
     uint64_t full[2], empty[2], keys_full;
 };
 
@@ -1129,7 +1129,15 @@ dr_gradient_kernel(const __grid_constant__ DrGradient p) {
         const uint64_t unit = slot * sh.heads + h0 + it / steps;
         const uint32_t v = it % steps;
         uint8_t* const to = sm.step[it & 1];
-        mbar_arrive_expect_tx(&sm.full[it & 1], Smem::STEP);
+        const bool first = v == 0;  // the head's gates and scales come along
+        mbar_arrive_expect_tx(&sm.full[it & 1], Smem::STEP + (first ? (uint32_t)sizeof(DrGates) + 5 * 32 : 0));
+        if (first) {
+            const uint32_t at = it / steps & 1;
+            bulk_load(&sm.gates[at], p.units + unit * DR_UNIT + 4 * DR_BLOCK, sizeof(DrGates), &sm.full[it & 1]);
+            const float* const back[5] = {p.s.back, p.x.back, p.w.back, p.z.back, p.back_out};
+#pragma unroll
+            for (int i = 0; i < 5; ++i) bulk_load(sm.back[at][i], back[i] + unit * 8, 32, &sm.full[it & 1]);
+        }
         bulk_load(to, p.s.of(unit) + v * Smem::STATE, Smem::STATE, &sm.full[it & 1]);
         bulk_load(to + Smem::STATE, p.x.of(unit) + v * Smem::STATE, Smem::STATE, &sm.full[it & 1]);
         bulk_load(to + 2 * Smem::STATE, p.w.of(unit) + v * Smem::KEPT, Smem::KEPT, &sm.full[it & 1]);
@@ -1176,26 +1184,11 @@ dr_gradient_kernel(const __grid_constant__ DrGradient p) {
     const uint32_t token = rb * 16 + g;
     uint32_t it = 0;
     for (uint32_t h = h0; h < h0 + group; ++h) {
-        const uint64_t unit = slot * sh.heads + h;
-        // the heads' gates and scales; what the head before read is read (barriers of its end)
-        for (int i = t; i < (int)sizeof(DrGates) / 4; i += DR_GRAD_THREADS)
-            ((float*)&sm.gates)[i] = ((const float*)(p.units + unit * DR_UNIT + 4 * DR_BLOCK))[i];
-        if (warp < 5 && lane < 8) {
-            const bool have = lane < (int)groups;
-            const float s = have ? p.s.back[unit * 8 + lane] : 0.0f, x = have ? p.x.back[unit * 8 + lane] : 0.0f,
-                        w = have ? p.w.back[unit * 8 + lane] : 0.0f, z = have ? p.z.back[unit * 8 + lane] : 0.0f,
-                        go = have ? p.back_out[unit * 8 + lane] : 0.0f;
-            const float mine = warp == 0 ? go * s : warp == 1 ? z * s : warp == 2 ? w * x : warp == 3 ? go * w : z * w;
-            float most = mine;
-#pragma unroll
-            for (int i = 4; i > 0; i >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffu, most, i));
-            sm.factor[warp][lane] = most > 0.0f ? mine / most : 0.0f;
-            const bool uneven = __any_sync(0xffu, have && mine != most);
-            if (lane == 0) sm.back[warp] = most, sm.uneven[warp] = uneven;
-            if (warp == 4) sm.own[0][lane] = s, sm.own[1][lane] = x, sm.own[2][lane] = w, sm.own[3][lane] = z;
-            if (warp == 0) sm.by_out[lane] = go > 0.0f ? 1.0f / go : 0.0f;
-        }
-        __syncthreads();
+        const DrGates& gates = sm.gates[(h - h0) & 1];
+        const float(&back)[5][8] = sm.back[(h - h0) & 1];
+        enum { S, X, W, Z, GO };
+        float* const most = sm.scales[warp];  // of dO S0, z S0, w X, dO w and z w: the largest of the value dimensions'
+        uint32_t uneven = 0;  // which of them have others, too
         float dq[NT][4] = {}, er[NT][4] = {}, wr[NT][4] = {}, a[2][4] = {}, n[2][4] = {};
         float sx = 0.0f;
         for (uint32_t v = 0; v < steps; ++v, ++it) {
@@ -1206,8 +1199,23 @@ dr_gradient_kernel(const __grid_constant__ DrGradient p) {
             }
             if (it == 0) ok = mbar_wait(&sm.keys_full, 0, limit) && ok;
             ok = mbar_wait(&sm.full[it & 1], (it >> 1) & 1, limit) && ok;
+            if (v == 0) {
+                const int at = lane & 7;
+                const bool have = at < (int)groups;
+                const float mine[5] = {back[GO][at] * back[S][at], back[Z][at] * back[S][at], back[W][at] * back[X][at], back[GO][at] * back[W][at],
+                                       back[Z][at] * back[W][at]};
+#pragma unroll
+                for (int i = 0; i < 5; ++i) {
+                    const float largest = warp_max(have ? mine[i] : 0.0f);
+                    if (lane == 0) most[i] = largest;
+                    uneven |= (uint32_t)__any_sync(0xffffffffu, have && mine[i] != largest) << i;
+                }
+                __syncwarp();
+            }
+            // a product's share of the largest scale
+            auto share = [&](int i, float x, float y) { return __float2half2_rn(x * y * power_inverse(most[i])); };
             const uint8_t* const step = sm.step[it & 1];
-            const float beta0 = sm.gates.beta[token], beta1 = sm.gates.beta[token + 8];
+            const float beta0 = gates.beta[token], beta1 = gates.beta[token + 8];
             T* const dv0 = (T*)p.dv + ((c.row + token) * sh.heads + h) * sh.value_dim;
             T* const dv1 = dv0 + 8ull * sh.heads * sh.value_dim;
             const uint32_t s = smem_u32(step), x = s + Smem::STATE, w = x + Smem::STATE, z = w + Smem::KEPT,
@@ -1219,7 +1227,7 @@ dr_gradient_kernel(const __grid_constant__ DrGradient p) {
                 // dO (and z below) against S0, and against w: shares of the scales differ
                 uint32_t go[2][4], aw[2][4], zt[2][4];
                 if (p.out) {
-                    const float by = sm.by_out[at];
+                    const float by = power_inverse(back[GO][at]);
                     if constexpr (EXACT) {
                         uint32_t r[4];
                         ldmatrix4(r, dr_slab_at<T>(slab, rb * 16 + (lane & 15), kt * 2 + (lane >> 4)));
@@ -1244,20 +1252,20 @@ dr_gradient_kernel(const __grid_constant__ DrGradient p) {
                     load_a_t(zt[i], z + i * DR_PIECE, kt * 16, rb, o);
                 }
                 if (cq == (int)(at & 3)) {  // dv = beta z
-                    const float back = sm.own[3][at];
+                    const float back_z = back[Z][at];
                     const uint32_t vcol = at * 16 + col;
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         const uint32_t r = token + (j & 1) * 8;
-                        const float b = (j & 1 ? beta1 : beta0) * back;
+                        const float b = (j & 1 ? beta1 : beta0) * back_z;
                         const float2 hi = unpack_f16(zt[0][j]), lo = unpack_f16(zt[1][j]);
                         if (r < c.rows)
                             dr_store_pair((j & 1) ? dv1 : dv0, vcol + (j >> 1) * 8, sh.value_dim, p.pairs_v, b * (hi.x + lo.x), b * (hi.y + lo.y));
                     }
                 }
-                if (sm.uneven[2]) {
+                if (uneven & 4) {
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) scale_f16(aw[i], __float2half2_rn(sm.factor[2][at]));
+                    for (int i = 0; i < 2; ++i) scale_f16(aw[i], share(2, back[W][at], back[X][at]));
                 }
                 {  // against w first, as they are; then scaled on to what S0 wants
                     uint32_t gw[2][4], zw[2][4];
@@ -1265,13 +1273,13 @@ dr_gradient_kernel(const __grid_constant__ DrGradient p) {
                     for (int i = 0; i < 2; ++i)
 #pragma unroll
                         for (int j = 0; j < 4; ++j) gw[i][j] = go[i][j], zw[i][j] = zt[i][j];
-                    if (sm.uneven[3] && p.out) {
+                    if (uneven & 8 && p.out) {
 #pragma unroll
-                        for (int i = 0; i < (EXACT ? 1 : 2); ++i) scale_f16(gw[i], __float2half2_rn(sm.factor[3][at]));
+                        for (int i = 0; i < (EXACT ? 1 : 2); ++i) scale_f16(gw[i], share(3, back[GO][at], back[W][at]));
                     }
-                    if (sm.uneven[4]) {
+                    if (uneven & 16) {
 #pragma unroll
-                        for (int i = 0; i < 2; ++i) scale_f16(zw[i], __float2half2_rn(sm.factor[4][at]));
+                        for (int i = 0; i < 2; ++i) scale_f16(zw[i], share(4, back[Z][at], back[W][at]));
                     }
                     if (cq <= rb) {  // 16 of the other tokens
                         uint32_t b[4];
@@ -1287,13 +1295,13 @@ dr_gradient_kernel(const __grid_constant__ DrGradient p) {
                         mma_f16_2(n[0], n[1], zw[0], b);
                     }
                 }
-                if (sm.uneven[0] && p.out) {
+                if (uneven & 1 && p.out) {
 #pragma unroll
-                    for (int i = 0; i < (EXACT ? 1 : 2); ++i) scale_f16(go[i], __float2half2_rn(sm.factor[0][at]));
+                    for (int i = 0; i < (EXACT ? 1 : 2); ++i) scale_f16(go[i], share(0, back[GO][at], back[S][at]));
                 }
-                if (sm.uneven[1]) {
+                if (uneven & 2) {
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) scale_f16(zt[i], __float2half2_rn(sm.factor[1][at]));
+                    for (int i = 0; i < 2; ++i) scale_f16(zt[i], share(1, back[Z][at], back[S][at]));
                 }
 #pragma unroll
                 for (int j = 0; j < NP; ++j) {
@@ -1331,7 +1339,7 @@ dr_gradient_kernel(const __grid_constant__ DrGradient p) {
                     mma_f16_2(d[0], d[1], s0, x0), mma_f16_2(d[0], d[1], s1, x0), mma_f16_2(d[0], d[1], s0, x1);
                     // rows g (d[0]) and g + 8 (d[1]) against columns col, col + 1 of their block
                     const float mine = g == col ? d[0][0] + d[1][2] : g == col + 1 ? d[0][1] + d[1][3] : 0.0f;
-                    sx = fmaf(mine, sm.own[0][at] * sm.own[1][at], sx);
+                    sx = fmaf(mine, back[S][at] * back[X][at], sx);
                 }
             }
             __syncwarp();
@@ -1342,20 +1350,20 @@ dr_gradient_kernel(const __grid_constant__ DrGradient p) {
         for (int j = 0; j < 2; ++j)
 #pragma unroll
             for (int m = 0; m < 4; ++m)
-                if (cq * 16 + j * 8 + col + (m & 1) == (int)token + (m >> 1) * 8) sm.dbeta[token + (m >> 1) * 8] = n[j][m] * sm.back[4];
+                if (cq * 16 + j * 8 + col + (m & 1) == (int)token + (m >> 1) * 8) sm.dbeta[(h - h0) & 1][token + (m >> 1) * 8] = n[j][m] * most[4];
         // scale D dA and D dN: dA_ij = beta_j a_ij, dN_ij = -beta_i beta_j n_ij
         float most_a = 0.0f, most_n = 0.0f;
         {
-            const float back_a = sm.back[3] * sh.scale, back_n = -sm.back[4];
+            const float back_a = most[3] * sh.scale, back_n = -most[4];
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 if (cq > rb) break;  // zeros
 #pragma unroll
                 for (int m = 0; m < 4; ++m) {
                     const int i = token + (m >> 1) * 8, cc = cq * 16 + j * 8 + col + (m & 1);
-                    const float d = __expf((sm.gates.total[i] - sm.gates.total[cc]) + (sm.gates.rest[i] - sm.gates.rest[cc])) * sm.gates.beta[cc];
+                    const float d = __expf((gates.total[i] - gates.total[cc]) + (gates.rest[i] - gates.rest[cc])) * gates.beta[cc];
                     a[j][m] = cc <= i ? a[j][m] * back_a * d : 0.0f;
-                    n[j][m] = cc < i ? n[j][m] * back_n * d * sm.gates.beta[i] : 0.0f;
+                    n[j][m] = cc < i ? n[j][m] * back_n * d * gates.beta[i] : 0.0f;
                     most_a = fmaxf(most_a, fabsf(a[j][m])), most_n = fmaxf(most_n, fabsf(n[j][m]));
                 }
             }
@@ -1364,7 +1372,10 @@ dr_gradient_kernel(const __grid_constant__ DrGradient p) {
         if (lane == 0) sm.most[0][warp] = most_a, sm.most[1][warp] = most_n;
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < 16; ++i) most_a = fmaxf(most_a, sm.most[0][i]), most_n = fmaxf(most_n, sm.most[1][i]);
+        for (int i = 0; i < 16; i += 4) {
+            const float4 x = *(const float4*)&sm.most[0][i], y = *(const float4*)&sm.most[1][i];
+            most_a = fmaxf(fmaxf(fmaxf(most_a, x.x), fmaxf(x.y, x.z)), x.w), most_n = fmaxf(fmaxf(fmaxf(most_n, y.x), fmaxf(y.y, y.z)), y.w);
+        }
         const Scale sa = scale_for(most_a), sn = scale_for(most_n);
 #pragma unroll
         for (int j = 0; j < 2; ++j)
@@ -1379,14 +1390,14 @@ dr_gradient_kernel(const __grid_constant__ DrGradient p) {
             }
         // row factors of the products with the states, into the domains of the products that follow; k.(e u X) is needed by
         // itself
-        const float back_k = sm.gates.back_k, back_q = sm.gates.back_q;
+        const float back_k = gates.back_k, back_q = gates.back_q;
         const float by_k = power_inverse(back_k), into_q = sa.by * by_k, into_n = sn.by * by_k;
         float carry[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
             const int i = token + half * 8;
-            const float g0 = sm.gates.g[i], b = sm.gates.beta[i];
-            const float fq = g0 * sh.scale * sm.back[0] * into_q, fe = -g0 * b * sm.back[1] * into_n, fw = sm.gates.e[i] * b * sm.back[2];
+            const float g0 = gates.g[i], b = gates.beta[i];
+            const float fq = g0 * sh.scale * most[0] * into_q, fe = -g0 * b * most[1] * into_n, fw = gates.e[i] * b * most[2];
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
                 const int first = cq * (DK / 4) + j * 8 + col;
@@ -1493,34 +1504,34 @@ dr_gradient_kernel(const __grid_constant__ DrGradient p) {
         }
         __syncthreads();
         if (warp == 0) {
-            double d[2], extra = 0.0;
+            float d[2], extra = 0.0f;
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 const int r = lane * 2 + j;
-                d[j] = ((double)sm.dot[0][r] + sm.dot[1][r]) + ((double)sm.dot[2][r] + sm.dot[3][r]);
-                extra += ((double)sm.carry[0][r] + sm.carry[1][r]) + ((double)sm.carry[2][r] + sm.carry[3][r]);
+                d[j] = (sm.dot[0][r] + sm.dot[1][r]) + (sm.dot[2][r] + sm.dot[3][r]);
+                extra += (sm.carry[0][r] + sm.carry[1][r]) + (sm.carry[2][r] + sm.carry[3][r]);
             }
-            if (lane < 16) extra += (double)sm.sx[lane] * sm.gates.g[DR_CHUNK - 1];
-#pragma unroll
-            for (int i = 16; i > 0; i >>= 1) extra += __shfl_xor_sync(0xffffffffu, extra, i);
-            double sum = d[0] + d[1];  // from the lane's rows to the end
+            if (lane < 16) extra = fmaf(sm.sx[lane], gates.g[DR_CHUNK - 1], extra);
+            extra = warp_reduce<OpSum>(extra);
+            float sum = d[0] + d[1];  // from the lane's rows to the end
 #pragma unroll
             for (int i = 1; i < 32; i <<= 1) {
-                const double down = __shfl_down_sync(0xffffffffu, sum, i);
+                const float down = __shfl_down_sync(0xffffffffu, sum, i);
                 if (lane + i < 32) sum += down;
             }
-            const double v[2] = {sum + extra, sum - d[0] + extra};
+            const float after = __shfl_down_sync(0xffffffffu, sum, 1), rest = lane < 31 ? after : 0.0f;
+            const float v[2] = {sum + extra, (d[1] + rest) + extra};
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 const uint32_t r = lane * 2 + j;
                 if (r < c.rows) {
                     const uint64_t to = (c.row + r) * sh.heads + h;
-                    if (p.ddecay) p.ddecay[to] = (float)v[j];
-                    p.dbeta[to] = sm.dbeta[r];
+                    if (p.ddecay) p.ddecay[to] = v[j];
+                    p.dbeta[to] = sm.dbeta[(h - h0) & 1][r];
                 }
             }
         }
-        if (SHARED) __syncthreads();  // the gates and scales may be replaced
+        // the next head's first barrier comes before it writes anything that is read here, but for its gates, scales and dbeta
     }
     if (!ok) set_error(LCPP_ERR_LOOKBACK_TIMEOUT);
 }
