@@ -328,8 +328,10 @@ lcpp_status lcpp_beam_reorder(const void* in, uint64_t in_layer_bytes, uint64_t 
  * decay (log of the factor, <= 0; -inf: the state starts anew; NULL: 0) and beta [rows][heads] float32, each with a
  * row stride in elements; head h reads key head h / (heads / key_heads).  key_dim and value_dim <= 128.  Sequences are
  * as above (length, or offsets); rows outside them give zeros.  init and last are [num_sequences][heads][value_dim]
- * [key_dim] (init NULL: zeros, last NULL: not wanted; last may be init).  The work goes by chunks of 64 rows, so a value
- * that is not finite reaches the rows of its sequence up to 63 before it, too, but no other sequence or head. */
+ * [key_dim] (init NULL: zeros, last NULL: not wanted; last may be init).  Inputs are finite: the
+ * work goes by chunks of 64 rows and 16 value dimensions, so a value that is not reaches rows of its sequence up to 63
+ * before it, too, and value dimensions beside it, but no other sequence or head (a key or query: its key head's).  Rows
+ * outside all sequences may hold anything. */
 typedef struct {
     uint64_t rows, num_sequences, length; /* length: of every sequence, where offsets is NULL */
     const uint32_t* offsets;              /* num_sequences + 1 ascending row offsets */
@@ -377,7 +379,8 @@ lcpp_status lcpp_delta_rule_step(int dtype, const lcpp_delta_shape* shape, const
  * as three bf16 parts each, products to about 2^-24).  A row with a negative target takes no part: its loss, logsum and
  * gradient are 0, it adds nothing to the weight's gradient, and its hidden state may hold anything; a target >= vocab
  * does the same and leaves LCPP_ERR_INVALID_ARG in the device error word.  loss or logsum may be NULL.
- * rows <= 2^24, vocab <= 2^30.  What is written, temp included, must not overlap anything else.
+ * rows <= 2^24, vocab <= 2^30; temp is refused where it is not 32-byte aligned.  What is written, temp included, must
+ * not overlap anything else.
  * temp bytes: for the forward call, or (backward != 0) for both; aligned = 0 where a row of weight may start off a
  * 16-byte boundary (it is copied then, as it is for channels that are no multiple of 8 and for float32). */
 size_t      lcpp_cross_entropy_temp_bytes(int dtype, uint64_t rows, uint64_t channels, uint64_t vocab, int backward,
@@ -489,7 +492,10 @@ lcpp_status lcpp_lookback_probe(const uint64_t* descriptors, uint64_t tile,
  * and returns, for one kernel kind ("reduce", "scan", "rs_memset",
  * "rs_histogram", "rs_bins_scan", "rs_onesweep", "seg_warp", "seg_block",
  * "lr_prepare", "lr_forward", "lr_backward", "lr_step", "beam_cluster",
- * "beam_rows", "beam_merge", "beam_reorder"),
+ * "beam_rows", "beam_merge", "beam_reorder", "dr_padding", "dr_prepare",
+ * "dr_order", "dr_states", "dr_join", "dr_forward", "dr_backward",
+ * "dr_gradient", "dr_step", "ce_plan", "ce_pack", "ce_logsum", "ce_loss",
+ * "ce_grad", "ce_hidden", "ce_weight", "ce_hidden_out"),
  * the number of timed launches and their summed duration in ms. */
 lcpp_status lcpp_profile_enable(int on);
 lcpp_status lcpp_profile_read(const char* kernel, uint64_t* launches, double* total_ms);

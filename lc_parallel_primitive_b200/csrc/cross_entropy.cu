@@ -43,6 +43,7 @@ constexpr int CE_HALF_BYTES = 128 * CE_BK * 2;       // one CTA's half of an ope
 constexpr int CE_STAGE_BYTES = 2 * CE_HALF_BYTES;    // both operands
 constexpr int CE_EPILOGUE_WARPS = 8;
 constexpr int CE_THREADS = 64 + 32 * CE_EPILOGUE_WARPS;  // a loading warp, a warp that issues products, the epilogue
+constexpr uint32_t CE_WAIT_LIMIT = 1u << 22;  // polls of at most a microsecond before a wait gives up
 constexpr float CE_LOG2E = 1.44269504088896f;
 // G is kept for gradients of the loss as shares of the largest, which the sums are multiplied by in the end: for a mean's
 // equal gradients the shares are 1, and an entry's rounding is that of the probability alone (-1 for an unlikely target is
@@ -319,7 +320,7 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     __shared__ CeBarriers bar;
     const uint32_t tiles = (smem_u32(ce_smem) + 1023) & ~1023u;  // swizzled boxes start on 1024 bytes
     const uint32_t warp = threadIdx.x >> 5, rank = cluster_rank();
-    const uint32_t limit = g_spin_limit;
+    constexpr uint32_t limit = CE_WAIT_LIMIT;
     if (warp == 0 && elect_one()) {
         tma_prefetch_map(&map_a);
         tma_prefetch_map(&map_b);

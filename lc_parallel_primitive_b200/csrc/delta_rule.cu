@@ -31,6 +31,7 @@ namespace lcpp {
 constexpr int DR_CHUNK = 64;
 constexpr int DR_MAX_DIM = 128;
 constexpr int DR_BLOCK = DR_CHUNK * BLOCK_ROW;  // bytes of a 64 x 64 block
+constexpr uint32_t DR_WAIT_LIMIT = 1u << 24;     // polls before a wait for a copy gives up, a second or so
 constexpr float DR_LEAST_DECAY = -150.0f;       // exp of less is 0 in float32 anyway, and -inf has no differences
 
 struct DrShape {
@@ -280,7 +281,7 @@ dr_prepare_kernel(const __grid_constant__ DrPrepare p) {
         __syncthreads();
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-            scale[x] = scale_for(dr_max8(s.most[x]));
+            scale[x] = scale_for<40>(dr_max8(s.most[x]));
 #pragma unroll
             for (int i = 0; i < ITEMS; ++i) {
                 const uint32_t item = i * DR_PREPARE_THREADS + t, r = item / (DK / 8), d = item % (DK / 8) * 8;
@@ -379,7 +380,7 @@ dr_prepare_kernel(const __grid_constant__ DrPrepare p) {
         if (lane == 0) s.most[0][warp] = most;
         __syncthreads();
         dr_invert(s.invert);
-        const Scale read = scale_for(dr_max8(s.most[0]));
+        const Scale read = scale_for<40>(dr_max8(s.most[0]));
         float v[4][4];
         most = 0.0f;
 #pragma unroll
@@ -393,7 +394,7 @@ dr_prepare_kernel(const __grid_constant__ DrPrepare p) {
         most = warp_max(most);
         if (lane == 0) s.most[1][warp] = most;
         __syncthreads();
-        const Scale inverse = scale_for(dr_max8(s.most[1]));
+        const Scale inverse = scale_for<40>(dr_max8(s.most[1]));
         if (t == 0) gates.back_inverse = inverse.back, gates.back_read = read.back;
 #pragma unroll
         for (int n = 0; n < 4; ++n)
@@ -529,7 +530,8 @@ struct DrChainCta {
     Smem& sm;
     const int lane, warp, g, col;
     const LaneOffsets o;
-    uint32_t h, hk, seq, v0, live, row, limit, dim;  // dim: rows of the state
+    uint32_t h, hk, seq, v0, live, row, dim;  // dim: rows of the state
+    static constexpr uint32_t limit = DR_WAIT_LIMIT;
     uint64_t start, end, base;
     uint32_t first, chunks;  // the part's
     const T* values;
@@ -569,7 +571,6 @@ struct DrChainCta {
             from = p.from ? p.from + piece * state : nullptr;
             to = p.to && part == (BACKWARD ? 0 : p.parts - 1) ? p.to + stream * state : nullptr;
         }
-        limit = g_spin_limit;
         if (threadIdx.x == 0) {
             for (int i = 0; i < STAGES; ++i) mbar_init(&sm.full[i], 1), mbar_init(&sm.empty[i], live);
             fence_mbar_init();
@@ -603,6 +604,11 @@ struct DrChainCta {
                 const uint32_t r = row + (j >> 1) * 8, c = n * 8 + col + (j & 1);
                 if (r < dim && c < p.sh.key_dim) to[(uint64_t)r * p.sh.key_dim + c] = s[n][j] * by;
             }
+    }
+    // What is added to a state need not be finer than 2^-45 of it, and must not be much finer, or the state would not fit
+    // the domain: a limit of its scale, from the state's largest value (times a domain) and that domain.
+    static __device__ __forceinline__ float finest(float top, float back) {
+        return top > 0.0f ? power_inverse(back) * 1073741824.0f : __int_as_float(0x7f000000);  // 2^30 times its scale; any
     }
     __device__ __forceinline__ uint64_t unit(uint32_t chunk) const { return (base + chunk) * p.sh.heads + h; }
     __device__ __forceinline__ uint32_t rows(uint32_t chunk) const {
@@ -727,7 +733,8 @@ dr_forward_kernel(const __grid_constant__ DrChain p) {
         const uint64_t unit = cta.unit(cta.order(it));
         // r = S0 K^T (value x token) and out = Q S0^T (token x value)
         float r[8][4] = {}, y[4][2][4] = {};
-        const Scale ss = coarse_scale_for(max_abs(s));
+        const float top = max_abs(s);
+        const Scale ss = coarse_scale_for(top);
         uint8_t* const states = ALL && p.states.at ? cta.mine(p.states.of(unit), NB) : nullptr;
         if (states) cta.keep_back(p.states.back, unit, ss.back * back_domain);
 #pragma unroll
@@ -749,7 +756,7 @@ dr_forward_kernel(const __grid_constant__ DrChain p) {
                 }
             }
         }
-        const float back_state = ss.back * back_domain;
+        const float back_state = ss.back * back_domain, finest = Cta::finest(top, back_state);
         // r = V - g S0 K^T
         const uint32_t raw = smem_u32(cta.sm.raw[warp][it & 1]);
         const float back_r = -back_state * gt.back_k;
@@ -803,7 +810,7 @@ dr_forward_kernel(const __grid_constant__ DrChain p) {
             scale_pair(w[n][0], w[n][1], by), scale_pair(w[n][2], w[n][3], by);
         }
         if constexpr (ALL) {  // out = scale g out + A u
-            const Scale su = scale_for(max_abs(w));
+            const Scale su = scale_up_to(scale_for(max_abs(w)), finest);
             {
                 const float by = p.sh.scale * back_state * gt.back_q, into = su.by * power_inverse(gt.back_read);
 #pragma unroll
@@ -853,8 +860,8 @@ dr_forward_kernel(const __grid_constant__ DrChain p) {
             const float2 e = *(const float2*)&gt.e[n * 8 + col];
             scale_pair(w[n][0], w[n][1], pair_of(e.x, e.y)), scale_pair(w[n][2], w[n][3], pair_of(e.x, e.y));
         }
-        const Scale se = scale_for(max_abs(w));
-        const float into = se.by * power_inverse(gt.back_k), whole = gt.g[DR_CHUNK - 1] * back_domain * into;
+        const Scale se = scale_up_to(scale_for(max_abs(w)), finest);
+        const float into = se.by * power_inverse(gt.back_k), whole = gt.g[DR_CHUNK - 1] * (back_domain * into);
         back_domain = se.back * gt.back_k;
         scale_all(s, whole);
 #pragma unroll
@@ -892,7 +899,9 @@ dr_backward_kernel(const __grid_constant__ DrChain p) {
         const uint32_t raw = smem_u32(cta.sm.raw[warp][it & 1]);
         // du = e X K^T (value x token)
         float du[8][4] = {};
-        const Scale sx = coarse_scale_for(max_abs(x));
+        const float top = max_abs(x);
+        const Scale sx = coarse_scale_for(top);
+        const float finest = Cta::finest(top, sx.back * back_domain);
         uint8_t* const states = ALL ? cta.mine(p.states.of(unit), Cta::NB) : nullptr;
         if constexpr (ALL) cta.keep_back(p.states.back, unit, sx.back * back_domain);
 #pragma unroll
@@ -917,10 +926,10 @@ dr_backward_kernel(const __grid_constant__ DrChain p) {
                 }
             }
         }
-        const Scale so = coarse_scale_for(warp_max(most)), sg = scale_for(warp_max(most_g) * fabsf(p.sh.scale));
+        const Scale so = scale_up_to(coarse_scale_for(warp_max(most)), finest), sg = scale_up_to(scale_for(warp_max(most_g) * fabsf(p.sh.scale)), finest);
         if constexpr (ALL) cta.keep_back(p.back_values, unit, so.back);
         {
-            const float back = sx.back * back_domain * gt.back_k * so.by * power_inverse(gt.back_read);
+            const float back = (sx.back * back_domain * gt.back_k) * (so.by * power_inverse(gt.back_read));
 #pragma unroll
             for (int n = 0; n < 8; ++n) {
                 const float2 e = *(const float2*)&gt.e[n * 8 + col];
@@ -984,9 +993,9 @@ dr_backward_kernel(const __grid_constant__ DrChain p) {
             }
         }
         // X = g_64 X + (scale g dO)^T Q - (g beta z)^T K, each in the domain of its product
-        float into = gt.g[DR_CHUNK - 1] * back_domain;
+        float into = back_domain;
         if (cta.values) {
-            into *= sg.by * power_inverse(gt.back_q);
+            into = gt.g[DR_CHUNK - 1] * (into * (sg.by * power_inverse(gt.back_q)));
             scale_all(x, into);
 #pragma unroll
             for (int kt = 0; kt < 4; ++kt) {
@@ -1008,8 +1017,9 @@ dr_backward_kernel(const __grid_constant__ DrChain p) {
             const uint64_t by = pair_of(-gate.x * b.x * back_z, -gate.y * b.y * back_z);
             scale_pair(z[n][0], z[n][1], by), scale_pair(z[n][2], z[n][3], by);
         }
-        const Scale sy = scale_for(max_abs(z));
+        const Scale sy = scale_up_to(scale_for(max_abs(z)), finest);
         into *= sy.by * power_inverse(gt.back_k);
+        if (!cta.values) into *= gt.g[DR_CHUNK - 1];
         back_domain = sy.back * gt.back_k;
         scale_all(x, into);
 #pragma unroll
@@ -1123,7 +1133,8 @@ dr_gradient_kernel(const __grid_constant__ DrGradient p) {
     if (!c.rows) return;
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5, rb = warp >> 2, cq = warp & 3, g = lane >> 2, col = (lane & 3) * 2;
     const LaneOffsets o(lane);
-    const uint32_t limit = g_spin_limit, groups = (sh.value_dim + 15) / 16, steps = (groups + 1) / 2, total = steps * group;
+    constexpr uint32_t limit = DR_WAIT_LIMIT;
+    const uint32_t groups = (sh.value_dim + 15) / 16, steps = (groups + 1) / 2, total = steps * group;
     bool ok = true;
     auto load = [&](uint32_t it) {  // one thread
         const uint64_t unit = slot * sh.heads + h0 + it / steps;

@@ -81,17 +81,25 @@ struct Scale {
 };
 // 1 / v for a power of two between 2^-126 and 2^126.
 __device__ __forceinline__ float power_inverse(float v) { return __int_as_float(0x7f000000 - __float_as_int(v)); }
-// For the largest absolute value `most`: most * by is in [2^14, 2^15), by <= 2^45 (1 for zeros).
-__device__ __forceinline__ Scale scale_for(float most) {
-    const int e = __float_as_int(most) >> 23 & 255;
-    const int field = e == 0 ? 127 : min(268 - e, 172);
+// For the largest absolute value `most`: most * by is in [2^14, 2^15), by <= 2^LIMIT (1 for zeros).  The limits keep
+// products of two scales, and a scale times a value that is not of its own matrix, within float32.  An infinity among the values
+// would leave nothing of the others: all become NaN.
+__device__ __forceinline__ Scale scale_of_field(int e, int field) {
+    if (e == 255) return Scale{__int_as_float(0x7fffffff), __int_as_float(0x7fffffff)};
+    if (e == 0) field = 127;
     return Scale{__int_as_float(field << 23), __int_as_float((254 - field) << 23)};
 }
+template <int LIMIT = 80>
+__device__ __forceinline__ Scale scale_for(float most) {
+    const int e = __float_as_int(most) >> 23 & 255;
+    return scale_of_field(e, min(268 - e, 127 + LIMIT));
+}
+// The scale, or `by` if that is less.
+__device__ __forceinline__ Scale scale_up_to(Scale s, float by) { return s.by > by ? Scale{by, power_inverse(by)} : s; }
 // With an exponent that is a multiple of 8, so that most * by is in [2^7, 2^15): matrices of like size share it.
 __device__ __forceinline__ Scale coarse_scale_for(float most) {
     const int e = __float_as_int(most) >> 23 & 255;
-    const int field = e == 0 ? 127 : min((268 - e - 127 + 1024) / 8 * 8 - 1024 + 127, 167);
-    return Scale{__int_as_float(field << 23), __int_as_float((254 - field) << 23)};
+    return scale_of_field(e, min((268 - e - 127 + 1024) / 8 * 8 - 1024 + 127, 207));
 }
 __device__ __forceinline__ float warp_max(float v) {  // of values >= 0
     return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(v)));

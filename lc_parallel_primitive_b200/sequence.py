@@ -264,7 +264,8 @@ class DeviceDeltaRule(_Recorded):
     of the factor, <= 0; None: 0) and d_beta: float32 (rows, heads), any row stride.  Dimensions up to 128.  scale:
     None for 1 / sqrt(key_dim).  offsets_or_length as in DeviceLinearRecurrence; states are contiguous float32
     (sequences, heads, value_dim, key_dim).  temp_storage is contiguous and 16-byte aligned, as temp_buffer's is.
-    Inputs are finite: the work goes by 64 rows, so a NaN reaches up to 63 rows of its sequence and head before it too.
+    Inputs are finite: the work goes by 64 rows and 16 value dimensions, so a NaN reaches up to 63 rows of its sequence
+    before it and value dimensions beside it, too, but no other sequence or head.
     """
 
     @staticmethod
