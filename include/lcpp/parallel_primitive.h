@@ -12,3 +12,5 @@
 #include "lcpp/device/device_multi_gpu.h"
 #include "lcpp/device/device_linear_recurrence.h"
 #include "lcpp/device/device_beam_search.h"
+#include "lcpp/device/device_delta_rule.h"
+#include "lcpp/device/device_cross_entropy.h"
