@@ -382,22 +382,52 @@ class DeviceDeltaRule(_Recorded):
         dt = _float_dtype(d_q, d_k, d_v, d_out)
         keep = (d_q, d_k, d_v, d_decay, d_beta, d_states_in, d_states_out, d_out, d_parents)
         _one_device(*keep)
-        inputs, rows, heads, key_heads, key_dim, value_dim = self._inputs(d_q, d_k, d_v, d_decay, d_beta)
-        state = (heads, value_dim, key_dim)
-        rows_in = 0
-        if d_states_in is not None:
-            rows_in = d_states_in.shape[0]
-            inputs.init = _dense(d_states_in, (rows_in, *state), _F32, "d_states_in")
-        pn = _dense(d_states_out, (rows, *state), _F32, "d_states_out")
+        usual = self._usual_step(d_q, d_k, d_v, d_decay, d_beta, d_states_in, d_states_out, d_out)
+        if usual is not None:
+            inputs, rows, heads, key_heads, key_dim, value_dim, rows_in, pn, po = usual
+            so = heads * value_dim
+        else:
+            inputs, rows, heads, key_heads, key_dim, value_dim = self._inputs(d_q, d_k, d_v, d_decay, d_beta)
+            state = (heads, value_dim, key_dim)
+            rows_in = 0
+            if d_states_in is not None:
+                rows_in = d_states_in.shape[0]
+                inputs.init = _dense(d_states_in, (rows_in, *state), _F32, "d_states_in")
+            pn = _dense(d_states_out, (rows, *state), _F32, "d_states_out")
+            po, so, r, h, d = _heads(d_out, "d_out")
+            if r != rows or h != heads or d != value_dim:
+                raise ValueError("d_out must have the shape of d_v")
         pp = _dense(d_parents, (rows,), _I32, "d_parents")
-        po, so, r, h, d = _heads(d_out, "d_out")
-        if r != rows or h != heads or d != value_dim:
-            raise ValueError("d_out must have the shape of d_v")
         if scale is None:
             scale = key_dim ** -0.5
         shape = L.DeltaShape(rows, 0, 0, None, heads, key_heads, key_dim, value_dim, scale)
         self._call(cmdlist, L.lib().lcpp_delta_rule_step, (dt, shape, inputs, rows_in, pp, pn, po, so), keep,
                    "DeviceDeltaRule.Step")
+
+    @staticmethod
+    def _usual_step(d_q, d_k, d_v, d_decay, d_beta, d_states_in, d_states_out, d_out):
+        """What Step passes on, for contiguous tensors of the shapes (rows, ...) that all fit; else None."""
+        q, v, n = d_q.shape, d_v.shape, d_states_out.shape
+        if len(q) != 3 or len(v) != 3 or len(n) != 4 or d_states_in is None or d_decay is None:
+            return None
+        rows, key_heads, key_dim = q
+        r, heads, value_dim = v
+        gates = d_beta.shape
+        before = d_states_in.shape
+        if (r != rows or d_k.shape != q or d_out.shape != v or not 0 < key_dim <= 128 or not 0 < value_dim <= 128 or not key_heads
+                or heads % key_heads or len(gates) != 2 or gates[0] != rows or gates[1] != heads or d_decay.shape != gates
+                or n[0] != rows or n[1] != heads or n[2] != value_dim or n[3] != key_dim or before[1:] != n[1:]):
+            return None
+        f32 = torch.float32
+        if d_decay.dtype != f32 or d_beta.dtype != f32 or d_states_in.dtype != f32 or d_states_out.dtype != f32:
+            return None
+        if not (d_q.is_contiguous() and d_k.is_contiguous() and d_v.is_contiguous() and d_decay.is_contiguous()
+                and d_beta.is_contiguous() and d_states_in.is_contiguous() and d_states_out.is_contiguous() and d_out.is_contiguous()):
+            return None
+        keys, values = key_heads * key_dim, heads * value_dim
+        return (L.DeltaInputs(d_q.data_ptr(), d_k.data_ptr(), d_v.data_ptr(), keys, keys, values, d_decay.data_ptr(), d_beta.data_ptr(),
+                              heads, heads, d_states_in.data_ptr()),
+                rows, heads, key_heads, key_dim, value_dim, before[0], d_states_out.data_ptr(), d_out.data_ptr())
 
 
 def _gates(t, rows, heads):
