@@ -72,10 +72,11 @@ struct CeGemm {
     CePlan plan;
     uint32_t planes;          // 1, or 3 for float32 operands in three bf16 parts
     uint32_t vocab0, vocab;   // the piece [vocab0, vocab0 + vocab)
-    uint32_t rows, channels;  // rows: as given, not packed
+    uint32_t channels;
     uint32_t padded;          // rows of the packed buffers
     uint32_t splits;          // CE_HIDDEN: parts of K, each with its own sum
-    uint32_t add;             // CE_HIDDEN: add to the sums
+    uint32_t row0, row_end;   // CE_WEIGHT: the slots to sum over, of those that there are
+    uint32_t add;             // add to what is there
     float2* part;             // CE_LOGSUM: (maximum, sum of 2^(z log2 e - maximum)) by 128 columns and slot
     float* right;             // CE_LOGSUM: the targets' logits by slot
     void* grad;               // CE_GRAD: G (planes, padded, grad_stride)
@@ -109,7 +110,9 @@ struct CeTiles {
             m = (count + CE_BM - 1) / CE_BM, n = (p.channels + CE_BN - 1) / CE_BN, steps = (p.vocab + CE_BK - 1) / CE_BK;
             parts = p.splits;
         } else {
-            m = (p.vocab + CE_BM - 1) / CE_BM, n = (p.channels + CE_BN - 1) / CE_BN, steps = (count + CE_BK - 1) / CE_BK;
+            m = (p.vocab + CE_BM - 1) / CE_BM, n = (p.channels + CE_BN - 1) / CE_BN;
+            const uint32_t end = min(count, p.row_end);
+            steps = end > p.row0 ? (end - p.row0 + CE_BK - 1) / CE_BK : 0;
         }
     }
     __device__ __forceinline__ uint64_t units() const { return (uint64_t)m * n * parts; }
@@ -187,6 +190,23 @@ __device__ __forceinline__ void ce_store32(T* to, const float (&v)[32], uint32_t
 #pragma unroll
         for (int i = 0; i < 32; ++i)
             if (i < width) to[i] = narrow<T>(v[i]);
+    }
+}
+
+// v += the row's
+__device__ __forceinline__ void ce_add32(float (&v)[32], const float* from, uint32_t width, uint32_t wide) {
+    if (wide >= 32 && width >= 32) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            uint32_t w[8];
+            ce_load_sector(w, from + i * 8);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[i * 8 + j] += __uint_as_float(w[j]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+            if (i < width) v[i] += from[i];
     }
 }
 
@@ -303,6 +323,9 @@ __device__ __forceinline__ void ce_epilogue(const CeGemm& p, uint32_t tmem, uint
             if (width <= 0) break;
 #pragma unroll
             for (int i = 0; i < 32; ++i) v[i] = empty ? 0.0f : v[i] * unit;
+            if constexpr (sizeof(T) == 4) {
+                if (p.add && live) ce_add32(v, to + c, width, p.out_wide);
+            }
             if (live) ce_store32<T>(to + c, v, width, p.out_wide);
         }
     }
@@ -361,13 +384,13 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                         const uint32_t full = cluster_smem(smem_u32(&bar.full[s]), 0);
                         const int m0 = mt * CE_BM + rank * 128, n0 = nt * CE_BN + rank * 128, k0 = k * CE_BK;
                         if constexpr (A_MN) {
-                            tma_load_3d(&map_a, a, full, m0, k0, pa);
-                            tma_load_3d(&map_a, a + CE_HALF_BYTES / 2, full, m0 + 64, k0, pa);
+                            tma_load_3d(&map_a, a, full, m0, p.row0 + k0, pa);
+                            tma_load_3d(&map_a, a + CE_HALF_BYTES / 2, full, m0 + 64, p.row0 + k0, pa);
                         } else {
                             tma_load_3d(&map_a, a, full, k0, m0, pa);
                         }
                         if constexpr (B_MN) {
-                            const int y = k0 + (EPI == CE_HIDDEN ? p.vocab0 : 0);
+                            const int y = k0 + (EPI == CE_HIDDEN ? p.vocab0 : p.row0);
                             tma_load_3d(&map_b, b, full, n0, y, pb);
                             tma_load_3d(&map_b, b + CE_HALF_BYTES / 2, full, n0 + 64, y, pb);
                         } else {
@@ -639,6 +662,10 @@ ce_hidden_kernel(const float* sums, uint64_t stride, uint32_t padded, uint32_t s
 // ---- host ------------------------------------------------------------------------------------
 constexpr uint64_t CE_MAX_ROWS = 1ull << 24, CE_MAX_CHANNELS = 1ull << 20, CE_MAX_VOCAB = 1ull << 30;
 constexpr uint64_t CE_PIECE_BYTES = 512ull << 20;  // of G
+// The tensor cores' sums are cut off, not rounded, at every step: they come out too small by about 1.2e-9 of themselves a
+// term.  Beside the roundings of 16-bit gradients that is nothing, but float32 ones take this many terms a sum at most, and
+// add the sums in float32 (weight gradient of 16384 rows in one sum: error 1.9e-5, so 4.8e-6).
+constexpr uint64_t CE_EXACT_TERMS = 4096;
 
 // The pieces of the temp buffer.
 struct CeLayout {
@@ -676,12 +703,10 @@ struct CeLayout {
         bytes = at;
     }
     // Parts of the hidden gradient's sum over the vocabulary: the number with the least time, of whole waves of tiles (a step
-    // of 64 takes 0.33 us) and of the parts' sums (float32, written and read once a piece).  The tensor cores' sums are cut off,
-    // not rounded, at every step, so that float32 gradients take 4096 tokens of the vocabulary a part at most (2048 x 512
-    // x 32000 in one part: error 9.5e-6, here 2e-6).
+    // of 64 takes 0.33 us) and of the parts' sums (float32, written and read once a piece).
     static uint64_t best_splits(uint64_t padded, uint64_t channels, uint64_t piece, uint64_t planes) {
         const uint64_t pairs = device_info().sms / 2, tiles = padded / CE_BM * ceil_div(channels, CE_BN), steps = ceil_div(piece, CE_BK);
-        const uint64_t fewest = planes == 1 ? 1 : min(ceil_div(steps, 64), (uint64_t)64);
+        const uint64_t fewest = planes == 1 ? 1 : min(ceil_div(piece, CE_EXACT_TERMS), (uint64_t)64);
         uint64_t best = fewest;
         double least = 0;
         for (uint64_t n = fewest; n <= max(fewest, (uint64_t)32) && (n == fewest || n * 16 <= steps); ++n) {
@@ -842,7 +867,7 @@ extern "C" lcpp_status lcpp_cross_entropy_forward(int dtype, const void* hidden,
         if (ok != LCPP_OK) return ok;
         CeGemm p{};
         p.plan = l.plan(temp);
-        p.planes = (uint32_t)l.planes, p.vocab = (uint32_t)vocab, p.rows = (uint32_t)rows, p.channels = (uint32_t)channels;
+        p.planes = (uint32_t)l.planes, p.vocab = (uint32_t)vocab, p.channels = (uint32_t)channels;
         p.padded = (uint32_t)l.padded, p.splits = 1;
         p.part = (float2*)((char*)temp + l.part), p.right = (float*)((char*)temp + l.right);
         ok = ce_gemm<T, CE_LOGSUM>("ce_logsum", maps.hidden_k, maps.weight_k, p, l.padded / CE_BM * ceil_div(vocab, CE_BN), c.stream);
@@ -890,7 +915,7 @@ extern "C" lcpp_status lcpp_cross_entropy_backward(int dtype, const void* hidden
         if (ok != LCPP_OK) return ok;
         CeGemm p{};
         p.plan = l.plan(temp);
-        p.planes = (uint32_t)l.planes, p.rows = (uint32_t)rows, p.channels = (uint32_t)channels;
+        p.planes = (uint32_t)l.planes, p.channels = (uint32_t)channels;
         p.padded = (uint32_t)l.padded, p.splits = (uint32_t)l.splits;
         p.grad = (char*)temp + l.grad, p.grad_stride = l.piece, p.grad_wide = 32;
         p.sums = (float*)((char*)temp + l.sums), p.sum_stride = l.sum_pitch;
@@ -900,11 +925,16 @@ extern "C" lcpp_status lcpp_cross_entropy_backward(int dtype, const void* hidden
         const uint64_t mt = l.padded / CE_BM, dt = ceil_div(channels, CE_BN);
         for (uint64_t v0 = 0; v0 < vocab; v0 += l.piece) {
             p.vocab0 = (uint32_t)v0, p.vocab = (uint32_t)min(l.piece, vocab - v0), p.add = v0 > 0;
+            p.row0 = 0;
             ok = ce_gemm<T, CE_GRAD>("ce_grad", maps.hidden_k, maps.weight_k, p, mt * ceil_div(p.vocab, CE_BN), c.stream);
             if (ok != LCPP_OK) return ok;
             if (grad_hidden) ok = ce_gemm<T, CE_HIDDEN>("ce_hidden", maps.grad_k, maps.weight_n, p, mt * dt * l.splits, c.stream);
             if (ok != LCPP_OK) return ok;
-            if (grad_weight) ok = ce_gemm<T, CE_WEIGHT>("ce_weight", maps.grad_m, maps.hidden_n, p, ceil_div(p.vocab, CE_BM) * dt, c.stream);
+            const uint64_t part = sizeof(T) == 4 ? CE_EXACT_TERMS : l.padded;  // rows
+            for (uint64_t row = 0; grad_weight && ok == LCPP_OK && row < rows; row += part) {
+                p.row0 = (uint32_t)row, p.row_end = (uint32_t)(row + part), p.add = row > 0;
+                ok = ce_gemm<T, CE_WEIGHT>("ce_weight", maps.grad_m, maps.hidden_n, p, ceil_div(p.vocab, CE_BM) * dt, c.stream);
+            }
             if (ok != LCPP_OK) return ok;
         }
         if (!grad_hidden) return LCPP_OK;

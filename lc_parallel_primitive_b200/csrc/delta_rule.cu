@@ -670,7 +670,6 @@ struct DrChainCta {
         }
     }
     // s (16 x DK) += a (16 x tokens 16 kt .. 16 kt + 16) times the rows of K or Q
-    template <bool EXACT>
     __device__ __forceinline__ void add_outer(float (&s)[NT][4], const uint32_t (&hi)[4], const uint32_t (&lo)[4], uint32_t tile, int kt) const {
 #pragma unroll
         for (int i = 0; i < PLANES; ++i)
@@ -681,7 +680,7 @@ struct DrChainCta {
                 for (int n = 0; n < 4; ++n) load_b_t(b[n], tile + (i * NB + m) * DR_BLOCK, kt * 16, n, o);
 #pragma unroll
                 for (int n = 0; n < 4; ++n) mma_f16_2(s[8 * m + 2 * n], s[8 * m + 2 * n + 1], hi, b[n]);
-                if (i == 0 && !EXACT) {
+                if (i == 0) {
 #pragma unroll
                     for (int n = 0; n < 4; ++n) mma_f16_2(s[8 * m + 2 * n], s[8 * m + 2 * n + 1], lo, b[n]);
                 }
@@ -868,7 +867,7 @@ dr_forward_kernel(const __grid_constant__ DrChain p) {
         for (int kt = 0; kt < 4; ++kt) {
             uint32_t hi[4], lo[4];
             split_block(w[2 * kt], w[2 * kt + 1], se.by, hi, lo);
-            cta.template add_outer<false>(s, hi, lo, k, kt);
+            cta.add_outer(s, hi, lo, k, kt);
         }
         cta.finish(it);
     }
@@ -1007,7 +1006,7 @@ dr_backward_kernel(const __grid_constant__ DrChain p) {
                     const float2 gate = *(const float2*)&gt.g[kt * 16 + (j >> 1) * 8 + col];
                     split_f16(v[j][0] * (gate.x * p.sh.scale), v[j][1] * (gate.y * p.sh.scale), sg.by, hi[j], lo[j]);
                 }
-                cta.template add_outer<false>(x, hi, lo, q, kt);
+                cta.add_outer(x, hi, lo, q, kt);
             }
             into = sg.back * gt.back_q;
         }
@@ -1026,7 +1025,7 @@ dr_backward_kernel(const __grid_constant__ DrChain p) {
         for (int kt = 0; kt < 4; ++kt) {
             uint32_t hi[4], lo[4];
             split_block(z[2 * kt], z[2 * kt + 1], sy.by, hi, lo);
-            cta.template add_outer<false>(x, hi, lo, k, kt);
+            cta.add_outer(x, hi, lo, k, kt);
         }
         cta.finish(it);
     }

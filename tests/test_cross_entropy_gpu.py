@@ -163,6 +163,19 @@ def test_pieces_of_the_vocabulary(cuda, dtype, rows, vocab):
     Case(rows, 40, vocab, dtype, seed=4).check()
 
 
+@pytest.mark.parametrize("pad,shift", [(0, 0), (3, 1)])
+def test_weight_gradient_of_many_rows(cuda, pad, shift):
+    """Sums over up to 4096 rows are cut off at each of 256 steps, by up to 2u of what they have come to, half of the whole on
+    average: 256 u; the roundings of G, of the parts' sums and the smaller products' cuts add less than 16 u."""
+    c = Case(40000, 64, 300, "f32", seed=19, ignored=0.0, gain=1 / 40000, pad=pad, shift=shift)
+    c.run()
+    h, w = c.hidden.double(), c.weight.double()
+    p = (h @ w.t()).softmax(1)
+    p[range(40000), c.targets.long()] -= 1
+    want = p.t() @ h / 40000
+    assert float((c.grad_weight.double() - want).norm() / want.norm()) <= (256 + 16) * U
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_sum_over_the_vocabulary_in_parts(cuda, dtype):
     # few tiles of the hidden gradient: several parts of the sum, each with its own
