@@ -11,6 +11,7 @@
 // epilogue's result (CE_GRAD), G W (CE_HIDDEN) and G^T H (CE_WEIGHT).
 #include "float_types.cuh"
 #include "tcgen05.cuh"
+#include "warp_mma.cuh"
 
 namespace lcpp {
 
@@ -70,7 +71,7 @@ struct CePlan {
 
 struct CeGemm {
     CePlan plan;
-    uint32_t planes;          // 1, or 3 for float32 operands in three bf16 parts
+    const float *hidden_back, *weight_back;  // logits of float32: inverse scales by slot and token
     uint32_t vocab0, vocab;   // the piece [vocab0, vocab0 + vocab)
     uint32_t channels;
     uint32_t padded;          // rows of the packed buffers
@@ -93,11 +94,21 @@ struct CeBarriers {
     uint32_t tmem;
 };
 
-// Products of planes (a, b) that make up a float32 product to about 2^-24: a = a0 + a1 + a2 with 8 bits each.
-__device__ __forceinline__ uint32_t ce_pairs(uint32_t planes) { return planes == 1 ? 1 : 6; }
+// Float32 operands are sums of 16-bit planes.  Logits: two of float16, with a scale for each row, which leave 2^-23 of a
+// value (2^-39 of its row's largest where that is more): 3 products (2^-22 is left out).  Gradients: three of bf16, 6 products to
+// about 2^-24; G has probabilities of any size, and what a row of G or a column of it has in common is no scale of a sum
+// over it.  With 6 products for the logits too, loss and gradients of 2048 x 512 x 32000 took 1352 us
+// instead of 1160.
+template <typename T, int EPI>
+constexpr int CE_PAIRS = sizeof(T) == 2 ? 1 : EPI == CE_LOGSUM || EPI == CE_GRAD ? 3 : 6;
+template <typename T, int EPI>
+constexpr bool CE_BF16 = sizeof(T) == 4 ? CE_PAIRS<T, EPI> == 6 : !std::is_same_v<T, __half>;
+// The planes of a's and b's i-th product, small products first.
+template <int PAIRS>
 __device__ __forceinline__ void ce_pair(uint32_t i, uint32_t* a, uint32_t* b) {
-    *a = 0x010120 >> (4 * i) & 15;  // small products first: (0,2) (2,0) (1,1) (0,1) (1,0) (0,0)
-    *b = 0x001102 >> (4 * i) & 15;
+    if constexpr (PAIRS == 3) *a = i == 1, *b = i == 0;  // (0,1) (1,0) (0,0)
+    else if constexpr (PAIRS == 6) *a = 0x010120 >> (4 * i) & 15, *b = 0x001102 >> (4 * i) & 15;  // (0,2) (2,0) (1,1) (0,1) (1,0) (0,0)
+    else *a = *b = 0;
 }
 
 template <int EPI>
@@ -210,6 +221,18 @@ __device__ __forceinline__ void ce_add32(float (&v)[32], const float* from, uint
     }
 }
 
+// Logits of float32 out of their scales: the row's, and those of 32 tokens from `back` on.
+template <typename T>
+__device__ __forceinline__ void ce_unscale(float (&v)[32], float row, const float* back) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < 32; i += 4) {
+            const float4 b = *(const float4*)(back + i);
+            v[i] *= row * b.x, v[i + 1] *= row * b.y, v[i + 2] *= row * b.z, v[i + 3] *= row * b.w;
+        }
+    }
+}
+
 // T: the element type of hidden states and weight.
 template <typename T, int EPI>
 __device__ __forceinline__ void ce_epilogue(const CeGemm& p, uint32_t tmem, uint32_t lane_row, uint32_t count, uint32_t mt,
@@ -221,9 +244,11 @@ __device__ __forceinline__ void ce_epilogue(const CeGemm& p, uint32_t tmem, uint
         float top = -INFINITY, sum = 0.0f, right = 0.0f;
         const bool live = m < count;
         const int64_t target = live ? (int64_t)p.plan.target[m] - (int64_t)p.vocab0 - n0 : -1;
+        const float back = sizeof(T) == 4 && live ? p.hidden_back[m] : 0.0f;
 #pragma unroll 1
         for (int c = 0; c < CE_BN / 2; c += 32) {
             tmem_load32(tmem + c, v);
+            ce_unscale<T>(v, back, p.weight_back + n0 + c);
             const int width = (int)p.vocab - (int)n0 - c;
             if (width < 32) {
 #pragma unroll
@@ -257,12 +282,14 @@ __device__ __forceinline__ void ce_epilogue(const CeGemm& p, uint32_t tmem, uint
         const float shift = live ? p.plan.logsum[m] * CE_LOG2E : 0.0f;
         float gain = live ? p.plan.gain[m] : 0.0f;
         if (live && gain != 0.0f) gain = gain / *p.plan.largest * CE_GAIN<T>;
+        const float back = sizeof(T) == 4 && live ? p.hidden_back[m] : 0.0f;
         E* const to = (E*)p.grad + (uint64_t)m * p.grad_stride + n0;
 #pragma unroll 1
         for (int c = 0; c < CE_BN / 2; c += 32) {
             tmem_load32(tmem + c, v);
             const int width = (int)p.grad_stride - (int)n0 - c;
             if (width <= 0) break;
+            ce_unscale<T>(v, back, p.weight_back + p.vocab0 + n0 + c);
 #pragma unroll
             for (int i = 0; i < 32; ++i) v[i] = ce_exp2(fmaf(v[i], CE_LOG2E, -shift));
             if (target >= c && target < c + 32) {
@@ -338,7 +365,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(CE_THREADS, 1)
 ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                const __grid_constant__ CeGemm p) {
     constexpr bool A_MN = EPI == CE_WEIGHT, B_MN = EPI == CE_HIDDEN || EPI == CE_WEIGHT;
-    constexpr bool BF16 = !std::is_same_v<T, __half>;
+    constexpr uint32_t PAIRS = CE_PAIRS<T, EPI>;
     extern __shared__ uint8_t ce_smem[];
     __shared__ CeBarriers bar;
     const uint32_t tiles = (smem_u32(ce_smem) + 1023) & ~1023u;  // swizzled boxes start on 1024 bytes
@@ -361,7 +388,7 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     ce_wait_for_last();
     const uint32_t count = *p.plan.count;
     const CeTiles<EPI> tl(p, count);
-    const uint32_t pairs = ce_pairs(p.planes), groups = gridDim.x / 2, group = blockIdx.x / 2;
+    const uint32_t groups = gridDim.x / 2, group = blockIdx.x / 2;
     bool ok = true;
 
     if (warp == 0) {
@@ -370,9 +397,9 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
             for (uint64_t unit = group; ok && unit < tl.units(); unit += groups) {
                 uint32_t mt, nt, first, end;
                 tl.at(unit, &mt, &nt, &first, &end);
-                for (uint32_t pair = 0; ok && pair < pairs; ++pair) {
-                    uint32_t pa = 0, pb = 0;
-                    if (pairs > 1) ce_pair(pair, &pa, &pb);
+                for (uint32_t pair = 0; ok && pair < PAIRS; ++pair) {
+                    uint32_t pa, pb;
+                    ce_pair<PAIRS>(pair, &pa, &pb);
                     for (uint32_t k = first; k < end; ++k, ++it) {
                         const uint32_t s = it % CE_STAGES;
                         if (it >= CE_STAGES && !mbar_poll(&bar.empty[s], (it / CE_STAGES - 1) & 1, limit)) {
@@ -408,7 +435,7 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         __syncwarp();
     } else if (warp == 1) {
         if (rank == 0 && elect_one()) {
-            constexpr uint32_t instruction = mma_instruction(BF16, A_MN, B_MN, CE_BM, CE_BN);
+            constexpr uint32_t instruction = mma_instruction(CE_BF16<T, EPI>, A_MN, B_MN, CE_BM, CE_BN);
             constexpr uint32_t lead_a = A_MN ? CE_HALF_BYTES / 2 : 16, lead_b = B_MN ? CE_HALF_BYTES / 2 : 16;
             constexpr uint32_t step_a = A_MN ? 2048 : 32, step_b = B_MN ? 2048 : 32;  // bytes of 16 along K
             uint32_t it = 0, sums = 0;
@@ -421,7 +448,7 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                     break;
                 }
                 tmem_fence_after();
-                const uint32_t steps = (end - first) * pairs;
+                const uint32_t steps = (end - first) * PAIRS;
                 for (uint32_t k = 0; k < steps; ++k, ++it) {
                     const uint32_t s = it % CE_STAGES;
                     if (!mbar_poll(&bar.full[s], (it / CE_STAGES) & 1, limit)) {
@@ -535,56 +562,97 @@ ce_plan_kernel(const int32_t* targets, const float* grad_loss, uint64_t grad_str
     }
 }
 
-// Rows of 16-bit elements on 16-byte boundaries, float32 ones as three planes of bf16; to row s from row[s] (null: s),
-// zeros from row `count` on up to the next multiple of 256.
+// Elements [8 w, 8 w + 8) of a row; zeros from `channels` on.  wide: rows start on 16 bytes.
+template <typename T>
+__device__ __forceinline__ void ce_load8(T (&v)[8], const T* source, bool wide, uint32_t w, uint32_t channels) {
+    if (wide && w * 8 + 8 <= channels) {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(v) / 16; ++i) ((uint4*)v)[i] = ((const uint4*)(source + w * 8))[i];
+    } else if (sizeof(T) == 2 && w && w * 8 + 8 < channels) {  // neighbours on both sides: words
+        const uint32_t* const words = (const uint32_t*)((uintptr_t)(source + w * 8) & ~(uintptr_t)3);
+        const uint32_t shift = (uintptr_t)(source + w * 8) & 2 ? 16 : 0;
+        uint32_t x[5];
+#pragma unroll
+        for (int i = 0; i < 5; ++i) x[i] = words[i];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) ((uint32_t*)v)[i] = __funnelshift_r(x[i], x[i + 1], shift);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = w * 8 + i < channels ? source[w * 8 + i] : narrow<T>(0.0f);
+    }
+}
+
+// Rows of 16-bit elements on 16-byte boundaries; to row s from row[s] (null: s), zeros from row `count` on up to the next
+// multiple of 256.  A warp a row.
 template <typename T>
 __global__ void __launch_bounds__(256)
 ce_pack_kernel(const T* from, uint64_t from_stride, const uint32_t* row, const uint32_t* count, uint32_t rows,
-               uint32_t channels, void* to, uint64_t to_stride, uint64_t plane) {
-    using E = std::conditional_t<sizeof(T) == 4, __nv_bfloat16, T>;
+               uint32_t channels, void* to, uint64_t to_stride) {
     ce_let_next_start();
     ce_wait_for_last();
     const uint32_t have = count ? *count : rows, last = count ? (have + CE_BM - 1) / CE_BM * CE_BM : rows;
     const uint32_t words = (uint32_t)(to_stride / 8);
     const bool wide = ((uintptr_t)from | from_stride * sizeof(T)) % 16 == 0;
     const uint32_t lane = threadIdx.x & 31;
-    for (uint64_t r = (uint64_t)blockIdx.x * 8 + (threadIdx.x >> 5); r < last; r += (uint64_t)gridDim.x * 8) {  // a warp a row
+    for (uint64_t r = (uint64_t)blockIdx.x * 8 + (threadIdx.x >> 5); r < last; r += (uint64_t)gridDim.x * 8) {
         const T* const source = r < have ? from + (row ? row[r] : r) * from_stride : nullptr;
 #pragma unroll 4
         for (uint32_t w = lane; w < words; w += 32) {
-            alignas(16) T v[8];
-            if (source && wide && w * 8 + 8 <= channels) {
+            alignas(16) T v[8] = {};
+            if (source) ce_load8(v, source, wide, w, channels);
+            *(uint4*)((T*)to + r * to_stride + w * 8) = *(const uint4*)v;
+        }
+    }
+}
+
+// Float32 rows, likewise: as two planes of float16 by a power of two that brings the row's largest finite value to 2^14 ..
+// 2^15, whose inverse goes to back[], and (null: not) as three planes of bf16.
+struct CeSplit {
+    const float* from;
+    uint64_t from_stride;
+    const uint32_t *row, *count;
+    uint32_t rows, channels;
+    __half* halves;
+    __nv_bfloat16* parts;
+    float* back;
+    uint64_t to_stride, plane;
+};
+__global__ void __launch_bounds__(256) ce_split_kernel(const CeSplit p) {
+    ce_let_next_start();
+    ce_wait_for_last();
+    const uint32_t have = p.count ? *p.count : p.rows, last = p.count ? (have + CE_BM - 1) / CE_BM * CE_BM : p.rows;
+    const uint32_t words = (uint32_t)(p.to_stride / 8), lane = threadIdx.x & 31;
+    const bool wide = ((uintptr_t)p.from | p.from_stride * 4) % 16 == 0;
+    for (uint64_t r = (uint64_t)blockIdx.x * 8 + (threadIdx.x >> 5); r < last; r += (uint64_t)gridDim.x * 8) {
+        const float* const source = r < have ? p.from + (p.row ? p.row[r] : r) * p.from_stride : nullptr;
+        float most = 0.0f;
+        if (source) {
+#pragma unroll 4
+            for (uint32_t w = lane; w < words; w += 32) {
+                alignas(16) float v[8];
+                ce_load8(v, source, wide, w, p.channels);
 #pragma unroll
-                for (int i = 0; i < (int)sizeof(v) / 16; ++i) ((uint4*)v)[i] = ((const uint4*)(source + w * 8))[i];
-            } else if (sizeof(T) == 2 && source && w && w * 8 + 8 < channels) {  // neighbours on both sides: words
-                const uint32_t* const words = (const uint32_t*)((uintptr_t)(source + w * 8) & ~(uintptr_t)3);
-                const uint32_t shift = (uintptr_t)(source + w * 8) & 2 ? 16 : 0;
-                uint32_t x[5];
-#pragma unroll
-                for (int i = 0; i < 5; ++i) x[i] = words[i];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) ((uint32_t*)v)[i] = __funnelshift_r(x[i], x[i + 1], shift);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] = source && w * 8 + i < channels ? source[w * 8 + i] : narrow<T>(0.0f);
+                for (int i = 0; i < 8; ++i) most = fabsf(v[i]) < INFINITY ? fmaxf(most, fabsf(v[i])) : most;
             }
-            E* const at = (E*)to + r * to_stride + w * 8;
-            if constexpr (sizeof(T) == 2) {
-                *(uint4*)at = *(const uint4*)v;
-            } else {
-                float f[8];
+        }
+        const Scale scale = scale_for<120>(warp_max(most));
+        if (lane == 0) p.back[r] = scale.back;
+#pragma unroll 2
+        for (uint32_t w = lane; w < words; w += 32) {
+            alignas(16) float v[8] = {};
+            if (source) ce_load8(v, source, wide, w, p.channels);
+            alignas(16) uint32_t hi[4], lo[4];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) f[i] = v[i];
+            for (int i = 0; i < 4; ++i) split_f16(v[2 * i], v[2 * i + 1], scale.by, hi[i], lo[i]);
+            const uint64_t at = r * p.to_stride + w * 8;
+            *(uint4*)(p.halves + at) = *(const uint4*)hi, *(uint4*)(p.halves + p.plane + at) = *(const uint4*)lo;
+            if (!p.parts) continue;
 #pragma unroll
-                for (int p = 0; p < 3; ++p) {
-                    alignas(16) E e[8];
+            for (int plane = 0; plane < 3; ++plane) {
+                alignas(16) __nv_bfloat16 e[8];
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        e[i] = narrow<E>(f[i]);
-                        f[i] -= widen(e[i]);
-                    }
-                    *(uint4*)(at + p * plane) = *(const uint4*)e;
-                }
+                for (int i = 0; i < 8; ++i) e[i] = narrow<__nv_bfloat16>(v[i]), v[i] -= widen(e[i]);
+                *(uint4*)(p.parts + plane * p.plane + at) = *(const uint4*)e;
             }
         }
     }
@@ -669,9 +737,10 @@ constexpr uint64_t CE_EXACT_TERMS = 4096;
 
 // The pieces of the temp buffer.
 struct CeLayout {
-    uint64_t planes, padded, pitch;       // planes of operands; packed rows; elements of a packed row
+    uint64_t planes, padded, pitch;       // planes of G, and of operands for gradients; packed rows; elements of a packed row
     uint64_t parts, piece, splits, sum_pitch;
     size_t count, slot, row, target, logsum, gain, right, hidden, weight, part, grad, sums, bytes;
+    size_t hidden_halves, weight_halves, hidden_back, weight_back;  // float32: what the logits are made of
     CeLayout(int dtype, uint64_t rows, uint64_t channels, uint64_t vocab, bool backward, bool pack_weight) {
         planes = dtype == LCPP_F32 ? 3 : 1;
         padded = align_up(rows, CE_BM);
@@ -690,8 +759,15 @@ struct CeLayout {
         };
         count = take(8), slot = take(rows * 4), row = take(padded * 4), target = take(padded * 4);
         logsum = take(padded * 4), gain = take(padded * 4);
-        hidden = take(planes * padded * pitch * 2);
-        weight = pack_weight ? take(planes * vocab * pitch * 2) : 0;
+        hidden = weight = hidden_halves = weight_halves = hidden_back = weight_back = 0;
+        if (planes == 1 || backward) {
+            hidden = take(planes * padded * pitch * 2);
+            weight = pack_weight ? take(planes * vocab * pitch * 2) : 0;
+        }
+        if (planes > 1) {
+            hidden_halves = take(2 * padded * pitch * 2), weight_halves = take(2 * vocab * pitch * 2);
+            hidden_back = take(padded * 4), weight_back = take(align_up(vocab, CE_BN) * 4);  // read by whole tiles
+        }
         right = part = grad = sums = 0;
         if (backward) {
             grad = take(planes * padded * piece * 2);
@@ -803,31 +879,37 @@ static lcpp_status ce_begin(const CeCall& c, const CeLayout& l, const float* gra
     lcpp_status ok = ce_launch("ce_plan", ce_plan_kernel, 1, CE_PLAN_THREADS, 0, true, c.stream, c.targets, grad_loss, grad_stride,
                                logsum, (uint32_t)c.rows, (uint32_t)c.vocab, plan);
     if (ok != LCPP_OK) return ok;
-    const uint64_t most = (uint64_t)device_info().sms * 16;
-    ok = ce_launch("ce_pack", ce_pack_kernel<T>, min(ceil_div(l.padded, 8), most), 256, 0, false, c.stream, (const T*)c.hidden, c.hidden_stride,
-                   plan.row, plan.count, (uint32_t)c.rows, (uint32_t)c.channels, t + l.hidden, l.pitch, l.padded * l.pitch);
-    if (ok != LCPP_OK) return ok;
-    const void* weight = c.weight;
-    uint64_t weight_pitch = c.weight_stride;
-    if (l.weight) {
-        weight = t + l.weight, weight_pitch = l.pitch;
-        ok = ce_launch("ce_pack", ce_pack_kernel<T>, min(ceil_div(c.vocab, 8), most), 256, 0, false, c.stream, (const T*)c.weight, c.weight_stride,
-                       nullptr, nullptr, (uint32_t)c.vocab, (uint32_t)c.channels, t + l.weight, l.pitch, c.vocab * l.pitch);
+    const uint64_t most = (uint64_t)device_info().sms * 16, hidden_grid = min(ceil_div(l.padded, 8), most), weight_grid = min(ceil_div(c.vocab, 8), most);
+    const uint32_t rows = (uint32_t)c.rows, channels = (uint32_t)c.channels, vocab = (uint32_t)c.vocab;
+    const void* weight = l.weight ? t + l.weight : c.weight;
+    const uint64_t weight_pitch = l.weight || c.vocab == 1 ? l.pitch : c.weight_stride;
+    if constexpr (sizeof(T) == 4) {
+        const CeSplit hidden{(const float*)c.hidden, c.hidden_stride, plan.row, plan.count, rows, channels, (__half*)(t + l.hidden_halves),
+                             (__nv_bfloat16*)(l.hidden ? t + l.hidden : nullptr), (float*)(t + l.hidden_back), l.pitch, l.padded * l.pitch};
+        ok = ce_launch("ce_pack", ce_split_kernel, hidden_grid, 256, 0, false, c.stream, hidden);
         if (ok != LCPP_OK) return ok;
-    } else if (c.vocab == 1) {
-        weight_pitch = l.pitch;
+        const CeSplit tokens{(const float*)c.weight, c.weight_stride, nullptr, nullptr, vocab, channels, (__half*)(t + l.weight_halves),
+                             (__nv_bfloat16*)(l.weight ? t + l.weight : nullptr), (float*)(t + l.weight_back), l.pitch, c.vocab * l.pitch};
+        ok = ce_launch("ce_pack", ce_split_kernel, weight_grid, 256, 0, false, c.stream, tokens);
+    } else {
+        ok = ce_launch("ce_pack", ce_pack_kernel<T>, hidden_grid, 256, 0, false, c.stream, (const T*)c.hidden, c.hidden_stride, plan.row,
+                       plan.count, rows, channels, t + l.hidden, l.pitch);
+        if (ok == LCPP_OK && l.weight)
+            ok = ce_launch("ce_pack", ce_pack_kernel<T>, weight_grid, 256, 0, false, c.stream, (const T*)c.weight, c.weight_stride, nullptr, nullptr,
+                           vocab, channels, t + l.weight, l.pitch);
     }
-    constexpr bool bf16 = !std::is_same_v<T, __half>;
-    auto map = [&](CUtensorMap* m, const void* base, uint64_t inner, uint64_t rows, uint64_t pitch, uint32_t box) {
-        return make_tensor_map(m, bf16, base, inner, rows, l.planes, pitch * 2, (l.planes > 1 ? rows : 1) * pitch * 2, box);
+    if (ok != LCPP_OK) return ok;
+    auto map = [&](CUtensorMap* m, bool bf16, uint64_t planes, const void* base, uint64_t inner, uint64_t rows, uint64_t pitch, uint32_t box) {
+        return make_tensor_map(m, bf16, base, inner, rows, planes, pitch * 2, (planes > 1 ? rows : 1) * pitch * 2, box);
     };
-    if (!map(&maps->hidden_k, t + l.hidden, c.channels, l.padded, l.pitch, 128) ||
-        !map(&maps->weight_k, weight, c.channels, c.vocab, weight_pitch, 128))
+    constexpr bool FINE = sizeof(T) == 4, LOGITS_BF16 = CE_BF16<T, CE_LOGSUM>, GRAD_BF16 = CE_BF16<T, CE_HIDDEN>;
+    if (!map(&maps->hidden_k, LOGITS_BF16, FINE ? 2 : 1, t + (FINE ? l.hidden_halves : l.hidden), c.channels, l.padded, l.pitch, 128) ||
+        !map(&maps->weight_k, LOGITS_BF16, FINE ? 2 : 1, FINE ? t + l.weight_halves : weight, c.channels, c.vocab, FINE ? l.pitch : weight_pitch, 128))
         return LCPP_ERR_CUDA;
-    if (l.grad && (!map(&maps->hidden_n, t + l.hidden, c.channels, l.padded, l.pitch, 64) ||
-                   !map(&maps->weight_n, weight, c.channels, c.vocab, weight_pitch, 64) ||
-                   !map(&maps->grad_k, t + l.grad, l.piece, l.padded, l.piece, 128) ||
-                   !map(&maps->grad_m, t + l.grad, l.piece, l.padded, l.piece, 64)))
+    if (l.grad && (!map(&maps->hidden_n, GRAD_BF16, l.planes, t + l.hidden, c.channels, l.padded, l.pitch, 64) ||
+                   !map(&maps->weight_n, GRAD_BF16, l.planes, weight, c.channels, c.vocab, weight_pitch, 64) ||
+                   !map(&maps->grad_k, GRAD_BF16, l.planes, t + l.grad, l.piece, l.padded, l.piece, 128) ||
+                   !map(&maps->grad_m, GRAD_BF16, l.planes, t + l.grad, l.piece, l.padded, l.piece, 64)))
         return LCPP_ERR_CUDA;
     return LCPP_OK;
 }
@@ -867,7 +949,8 @@ extern "C" lcpp_status lcpp_cross_entropy_forward(int dtype, const void* hidden,
         if (ok != LCPP_OK) return ok;
         CeGemm p{};
         p.plan = l.plan(temp);
-        p.planes = (uint32_t)l.planes, p.vocab = (uint32_t)vocab, p.channels = (uint32_t)channels;
+        p.hidden_back = (const float*)((char*)temp + l.hidden_back), p.weight_back = (const float*)((char*)temp + l.weight_back);
+        p.vocab = (uint32_t)vocab, p.channels = (uint32_t)channels;
         p.padded = (uint32_t)l.padded, p.splits = 1;
         p.part = (float2*)((char*)temp + l.part), p.right = (float*)((char*)temp + l.right);
         ok = ce_gemm<T, CE_LOGSUM>("ce_logsum", maps.hidden_k, maps.weight_k, p, l.padded / CE_BM * ceil_div(vocab, CE_BN), c.stream);
@@ -915,7 +998,8 @@ extern "C" lcpp_status lcpp_cross_entropy_backward(int dtype, const void* hidden
         if (ok != LCPP_OK) return ok;
         CeGemm p{};
         p.plan = l.plan(temp);
-        p.planes = (uint32_t)l.planes, p.channels = (uint32_t)channels;
+        p.hidden_back = (const float*)((char*)temp + l.hidden_back), p.weight_back = (const float*)((char*)temp + l.weight_back);
+        p.channels = (uint32_t)channels;
         p.padded = (uint32_t)l.padded, p.splits = (uint32_t)l.splits;
         p.grad = (char*)temp + l.grad, p.grad_stride = l.piece, p.grad_wide = 32;
         p.sums = (float*)((char*)temp + l.sums), p.sum_stride = l.sum_pitch;

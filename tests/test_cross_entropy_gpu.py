@@ -1,8 +1,8 @@
 """DeviceCrossEntropy on the GPU against float64, with element-wise bounds.
 
-u = 2^-24.  A logit is a sum of products that are exact (16-bit operands; float32 ones in three bf16 parts leave out 2^-24 of
-a product) in float32, cut off at every step of 16 products: off by z_err = (channels / 16 * pairs + 4) 2u sum_d |h_d w_d|
-with pairs 1, or 6 for float32.  logsum is off by the largest z_err and the sum's roundings (exp2 2 ulp of the term, its
+u = 2^-24.  A logit is a sum of products that are exact (16-bit operands) in float32, cut off at every step of 16 products: off
+by z_err = (channels / 16 * pairs + 4) 2u sum_d |h_d w_d| with pairs 1, or 6 for float32: its operands in two float16 parts
+take 3 products, leave 2^-23 of each factor and leave out the lower parts' product, 2^-22, together 8u.  logsum is off by the largest z_err and the sum's roundings (exp2 2 ulp of the term, its
 argument |z| u, log2 and the last product 4 u |logsum|), the loss by that and one z_err more.
 G = g (p - [target]), p = exp(z - logsum): off by g p times the errors of z and of logsum (which is the row's, of its
 largest logits) and (|z| + |logsum|) 2u + 8u of the argument's and exp2's roundings, and, rounded between the products, by r |G| with r half an ulp of
