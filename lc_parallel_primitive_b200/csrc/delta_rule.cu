@@ -22,7 +22,15 @@
 //
 // Products are of float16 with float32 sums, and a float32 value enters as two float16 with a power of two taken out
 // (warp_mma.cuh), so that states, which live for a whole sequence, and gradients keep float32's order of error.  q and k
-// of 16 bits are exact in one float16 but for the scale of their tile; float32 ones are split too (PLANES 2).
+// of 16 bits are exact in one float16 but for the scale of their tile; float32 ones are split too (PLANES 2).  Pairs of
+// bf16, which need no scale, left errors of 5e-6 to 2e-5, these leave 2e-7 to 3e-6.
+//
+// mma.sync and not tcgen05: a chain's products are 16 x 64 x 16 to 16 x 128 x 16 a warp, and each needs the last one's
+// result; in registers that is the next operand at once, where an accumulator in tensor memory would have to be read,
+// split and written to shared memory between any two.
+//
+// Times at 8 sequences of 2048 tokens, 16 heads, 128 dimensions, bf16 (4096 chunks and heads): preparation 126 us, forward
+// with what the backward pass wants 269, backward chain 259, gradients 592; 1379 us in all.
 #include "float_types.cuh"
 #include "warp_mma.cuh"
 
@@ -217,6 +225,10 @@ struct DrPrepare {
     uint8_t *keys, *units;
 };
 
+// A CTA a chunk and key head, the heads of which it takes in turn.  Bound by shared memory (45 % of its pipe's cycles; issue
+// slots 51 %) and by the barriers between its short steps; 3 CTAs an SM (2 for float32's two planes) fill most of the
+// gaps, 4 with fewer registers took the same time.  The inverse is by substitution only in its 16 x 16 diagonal blocks:
+// 64 rows of it took 3 times as long as the products that join blocks.
 template <typename T, int DK, bool BACKWARD>
 __global__ void __launch_bounds__(DR_PREPARE_THREADS, sizeof(T) == 4 ? 2 : 3)
 dr_prepare_kernel(const __grid_constant__ DrPrepare p) {
@@ -707,6 +719,10 @@ struct DrChainCta {
     }
 };
 
+// Bound by latency: a warp's products wait for the last ones' sums (13 ns each) and for their operands, with one or two warps
+// a scheduler.  Counters with 8 warps: issue slots 37 %, tensor pipe 31 %, shared memory 40 %; with 2: 29 and 12 %.  Two
+// CTAs an SM, for which 64 key columns leave room with one stage of images each, took 523 us instead of 450 over 256
+// packed sequences: the copies are no longer ahead.
 template <typename T, int DK, int WARPS, int WHAT>
 __global__ void __launch_bounds__(WARPS * 32, 1)
 dr_forward_kernel(const __grid_constant__ DrChain p) {
@@ -874,6 +890,7 @@ dr_forward_kernel(const __grid_constant__ DrChain p) {
     cta.close(s, back_domain);
 }
 
+// As the forward chain (issue slots 35 %, tensor pipe 36 %).
 template <typename T, int DK, int WARPS, int WHAT>
 __global__ void __launch_bounds__(WARPS * 32, 1)
 dr_backward_kernel(const __grid_constant__ DrChain p) {
@@ -1033,6 +1050,8 @@ dr_backward_kernel(const __grid_constant__ DrChain p) {
 }
 
 // The states before each part of a sequence: through the parts in order, a CTA with 8 rows of a state and all its columns.
+// The maps come from L2, 16 loads ahead: 16 heads of one sequence of 65536 tokens 78 us (32 loads ahead in registers of
+// their own 141; rows of the state by 16-byte reads 113).
 constexpr int DR_JOIN_ROWS = 8;
 struct DrJoin {
     const float *first, *local, *map;  // first: null for zeros
@@ -1115,6 +1134,11 @@ struct DrGradient {
     bool pairs_k, pairs_v;  // elements 2 i and 2 i + 1 of a row can be stored together: of dq and dk, of dv
 };
 
+// A CTA a chunk and key head: 32 value dimensions a step with the next step's images on their way (a step's two buffers are
+// handed over by barriers in memory, so that warps need not meet), then what the key columns need of all of them.  Bound by
+// shared memory (46 % of its pipe's cycles), the tensor pipe (32 %) and what each warp waits between: about 235 us of
+// the 592 are outside the steps.  8 warps with twice the columns each took 565 us where 16 took 596, but 1515 us instead
+// of 1424 for the whole pass before the buffers were handed over so.
 template <typename T, int DK, bool SHARED>  // SHARED: several heads a key head
 __global__ void __launch_bounds__(DR_GRAD_THREADS, 1)
 dr_gradient_kernel(const __grid_constant__ DrGradient p) {
@@ -1601,7 +1625,9 @@ __global__ void __launch_bounds__(DR_ORDER_THREADS) dr_order_kernel(const __grid
 
 // ---- one token ------------------------------------------------------------------------------------
 constexpr int DR_STEP_WARPS = 4;
-// A warp takes 8 rows of a state (value dimensions) at a time: a lane holds 4 key columns of each.
+// A warp takes 8 rows of a state (value dimensions) at a time: a lane holds 4 key columns of each.  All loads come before the
+// first sum, and one pass serves S' k and S' q, since S q = S' q + u (k.q).  Bound by HBM: 256 rows of 32 heads of
+// 128 x 128, 1.07 GB read and written, in 150 us, 7.1 TB/s.
 template <typename T, bool WIDE>
 __global__ void __launch_bounds__(DR_STEP_WARPS * 32)
 dr_step_kernel(DrShape sh, const T* q, uint64_t q_stride, const T* k, uint64_t k_stride, const T* v, uint64_t v_stride,
