@@ -221,7 +221,7 @@ struct DrPrepare {
     uint64_t q_stride, k_stride;
     const float *decay, *beta;
     uint64_t decay_stride, beta_stride;
-    bool wide;  // rows of q and k are whole pieces of 8 elements on 16 bytes
+    bool wide;  // rows of q and k are whole pieces of 16 bytes on 16 bytes
     uint8_t *keys, *units;
 };
 
@@ -257,18 +257,21 @@ dr_prepare_kernel(const __grid_constant__ DrPrepare p) {
 #pragma unroll
                 for (int i = 0; i < ITEMS; ++i) {
                     const uint32_t item = i * DR_PREPARE_THREADS + t, r = item / (DK / 8), d = item % (DK / 8) * 8;
-                    const T* const at = from(x, min(r, c.rows - 1), d < sh.key_dim ? d : 0);
 #pragma unroll
-                    for (int j = 0; j < (int)sizeof(T) / 2; ++j) ((uint4*)raw[x][i])[j] = __ldg((const uint4*)at + j);
+                    for (int j = 0; j < (int)sizeof(T) / 2; ++j) {
+                        const uint32_t e = d + j * 16 / (int)sizeof(T);
+                        ((uint4*)raw[x][i])[j] = __ldg((const uint4*)from(x, min(r, c.rows - 1), e < sh.key_dim ? e : 0));
+                    }
                 }
 #pragma unroll
             for (int i = 0; i < ITEMS; ++i) {
                 const uint32_t item = i * DR_PREPARE_THREADS + t, r = item / (DK / 8), d = item % (DK / 8) * 8;
-                if (r < c.rows && d < sh.key_dim) continue;
 #pragma unroll
-                for (int x = 0; x < 2; ++x)
+                for (int j = 0; j < (int)sizeof(T) / 2; ++j) {
+                    if (r < c.rows && d + j * 16 / (int)sizeof(T) < sh.key_dim) continue;
 #pragma unroll
-                    for (int j = 0; j < (int)sizeof(T) / 2; ++j) ((uint4*)raw[x][i])[j] = make_uint4(0, 0, 0, 0);
+                    for (int x = 0; x < 2; ++x) ((uint4*)raw[x][i])[j] = make_uint4(0, 0, 0, 0);
+                }
             }
         } else {
 #pragma unroll
@@ -1923,7 +1926,7 @@ struct DrCall {
     }
     DrPrepare prepare(const DrShape& shape, const DrLayout& l, void* temp) const {
         return DrPrepare{shape, in.q, in.k, in.q_stride, in.k_stride, in.decay, in.beta, in.decay_stride, in.beta_stride,
-                         sh.key_dim % 8 == 0 && dr_wide(in.q, in.q_stride, sh.rows, sh.key_dim, element()) &&
+                         dr_wide(in.q, in.q_stride, sh.rows, sh.key_dim, element()) &&
                              dr_wide(in.k, in.k_stride, sh.rows, sh.key_dim, element()),
                          (uint8_t*)temp + l.keys, (uint8_t*)temp + l.unit};
     }
