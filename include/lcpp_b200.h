@@ -243,11 +243,13 @@ lcpp_status lcpp_reduce_by_key(int op, int key_dtype, int value_dtype, const voi
  * No counterpart in the reference, whose scans and sorts are over scalars:
  * the scan a recurrent language model is made of, with its gradient and its
  * single-token form, and the selection and state reordering that decode such
- * a model with beams.  dtype: LCPP_F32, LCPP_F16 or LCPP_BF16; states, scores
+ * a model with beams; and the same of a matrix state (gated delta rule), and
+ * the loss that such models are trained with.  dtype: LCPP_F32, LCPP_F16 or LCPP_BF16; states, scores
  * and every sum are float32.  Matrices are row-major with unit element stride
  * and a row stride in elements (>= channels, < 2^31; any value for one row);
  * no alignment beyond the element's own is required, and any other address is
- * refused.  temp is refused where it is not 16-byte (selection: 8-byte) aligned.
+ * refused.  temp is refused where it is not 16-byte (selection: 8-byte, cross
+ * entropy: 32-byte) aligned.
  * Matrices may be columns of one buffer; two of different strides whose bounds
  * meet count as overlapping.
  *
@@ -376,7 +378,8 @@ lcpp_status lcpp_delta_rule_step(int dtype, const lcpp_delta_shape* shape, const
 /* Softmax cross entropy over a vocabulary from hidden states, without the logits in memory:
  *   z = hidden weight^T,  logsum[i] = log sum_v exp(z_iv),  loss[i] = logsum[i] - z_i,targets[i]
  * hidden is [rows][channels], weight [vocab][channels], both of dtype; products are summed in float32 (float32 operands
- * as three bf16 parts each, products to about 2^-24).  A row with a negative target takes no part: its loss, logsum and
+ * in parts: of two float16 with a scale for each row in the logits, 2^-22 of a product, or 2^-39 of its rows' largest
+ * values where that is more; of three bf16 in the gradients, about 2^-24).  A row with a negative target takes no part: its loss, logsum and
  * gradient are 0, it adds nothing to the weight's gradient, and its hidden state may hold anything; a target >= vocab
  * does the same and leaves LCPP_ERR_INVALID_ARG in the device error word.  loss or logsum may be NULL.
  * rows <= 2^24, vocab <= 2^30; temp is refused where it is not 32-byte aligned.  What is written, temp included, must
@@ -391,7 +394,10 @@ lcpp_status lcpp_cross_entropy_forward(int dtype, const void* hidden, uint64_t h
                                        void* stream);
 /* Gradients from those of loss (grad_loss[i * grad_loss_stride]; stride 0: one for all rows), given the forward call's
  * logsum: grad_hidden [rows][channels] and grad_weight [vocab][channels] (NULL: not wanted), both of dtype.  The
- * logits' gradient is rounded to dtype between the two products (float32: to three bf16 parts). */
+ * logits' gradient, as a share of the largest finite |grad_loss|, is rounded to dtype between the two products (float32:
+ * to three bf16 parts; float16 shares below 2^-39 vanish).  Float32 sums go over 4096 terms at a time, which come out too
+ * small by up to 5e-6 of themselves, since the tensor cores cut sums off; sums of the 16-bit types go on longer, 1.2e-9 of
+ * themselves a term. */
 lcpp_status lcpp_cross_entropy_backward(int dtype, const void* hidden, uint64_t hidden_stride, const void* weight,
                                         uint64_t weight_stride, const int32_t* targets, const float* logsum,
                                         const float* grad_loss, uint64_t grad_loss_stride, void* grad_hidden,

@@ -2,7 +2,8 @@
 
 Native code: liblcpp_b200.so (CUDA kernels + C ABI, include/lcpp_b200.h).
 Python host mirror of the reference's Device* classes: primitives.py; operators
-over sequences (gated linear recurrence, beam search): sequence.py.
+over sequences (gated linear recurrence, gated delta rule, beam search, cross
+entropy over a vocabulary): sequence.py.
 """
 from ._lib import LcppError, check, lib  # noqa: F401
 from .primitives import (  # noqa: F401

@@ -1,7 +1,9 @@
 """Operators over sequences, in the manner of the Device* classes: the gated
 linear recurrence with its backward pass and single-token step
-(DeviceLinearRecurrence), and beam search's selection and reordering of states
-(DeviceBeamSearch).
+(DeviceLinearRecurrence), the gated delta rule, whose states are matrices,
+likewise (DeviceDeltaRule), beam search's selection and reordering of states
+(DeviceBeamSearch), and the cross entropy over a vocabulary from hidden states
+with its gradients (DeviceCrossEntropy).
 
 The reference has no counterpart.  Buffers are CUDA torch tensors of float32,
 float16 or bfloat16 (states and scores float32); calls are recorded into a
@@ -530,7 +532,7 @@ class DeviceCrossEntropy(_Recorded):
     loss[i] = log sum_v exp(z_iv) - z_i,target(i) with z = d_hidden d_weight^T.  d_hidden: (rows, channels) or
     (batch, time, channels), any row stride; d_weight: (vocab, channels) of the same type; d_targets: int32, one for
     each row.  A row with a negative target takes no part: loss, logsum and gradient 0, whatever its hidden state
-    holds.  Sums are float32; float32 operands are multiplied in three bf16 parts.
+    holds.  Sums are float32; float32 operands are multiplied in two float16 or three bf16 parts.
     """
 
     @staticmethod
