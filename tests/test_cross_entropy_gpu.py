@@ -163,6 +163,30 @@ def test_pieces_of_the_vocabulary(cuda, dtype, rows, vocab):
     Case(rows, 40, vocab, dtype, seed=4).check()
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_rows_and_tokens_of_any_size(cuda, dtype):
+    import torch
+
+    c = Case(300, 72, 700, dtype, seed=18)
+    c.hidden *= (10.0 ** -torch.linspace(0, 18, 300, device="cuda"))[:, None].to(c.hidden.dtype)
+    c.weight *= (10.0 ** -torch.linspace(0, 15, 700, device="cuda"))[torch.randperm(700, device="cuda")][:, None].to(c.weight.dtype)
+    c.hidden[40], c.weight[50] = 0, 0
+    c.check()
+
+
+def test_an_infinity_of_float32_stays_in_its_row(cuda):
+    import torch
+
+    rows, row = 300, 7
+    c = Case(rows, 72, 700, "f32", seed=17, ignored=0.0)
+    want = [t.clone() for t in c.run()]
+    c.hidden[row, 3] = float("inf")
+    loss, logsum, gh, gw = c.run()
+    rest = torch.arange(rows, device="cuda") != row
+    assert not loss[row].isfinite() and not gh[row].isfinite().any()
+    assert torch.equal(loss[rest], want[0][rest]) and torch.equal(logsum[rest], want[1][rest]) and torch.equal(gh[rest], want[2][rest])
+
+
 @pytest.mark.parametrize("pad,shift", [(0, 0), (3, 1)])
 def test_weight_gradient_of_many_rows(cuda, pad, shift):
     """Sums over up to 4096 rows are cut off at each of 256 steps, by up to 2u of what they have come to, half of the whole on
