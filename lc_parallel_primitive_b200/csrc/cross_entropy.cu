@@ -580,14 +580,17 @@ __device__ __forceinline__ void ce_load8(T (&v)[8], const T* source, bool wide, 
     if (wide && w * 8 + 8 <= channels) {
 #pragma unroll
         for (int i = 0; i < (int)sizeof(v) / 16; ++i) ((uint4*)v)[i] = ((const uint4*)(source + w * 8))[i];
-    } else if (sizeof(T) == 2 && w && w * 8 + 8 < channels) {  // neighbours on both sides: words
-        const uint32_t* const words = (const uint32_t*)((uintptr_t)(source + w * 8) & ~(uintptr_t)3);
-        const uint32_t shift = (uintptr_t)(source + w * 8) & 2 ? 16 : 0;
-        uint32_t x[5];
+    } else if (sizeof(T) == 2 && w && w * 8 + 16 <= channels) {  // neighbours on both sides: two pieces on 16 bytes
+        const uint4* const pieces = (const uint4*)((uintptr_t)(source + w * 8) & ~(uintptr_t)15);
+        const uint4 a = pieces[0], b = pieces[1];
+        const uint32_t phase = (uint32_t)(uintptr_t)source & 15, shift = phase & 2 ? 16 : 0;  // the same along a row
+        const uint32_t x[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
 #pragma unroll
-        for (int i = 0; i < 5; ++i) x[i] = words[i];
+        for (uint32_t first = 0; first < 4; ++first) {
+            if (phase >> 2 != first) continue;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) ((uint32_t*)v)[i] = __funnelshift_r(x[i], x[i + 1], shift);
+            for (int i = 0; i < 4; ++i) ((uint32_t*)v)[i] = __funnelshift_r(x[first + i], x[first + i + 1], shift);
+        }
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = w * 8 + i < channels ? source[w * 8 + i] : narrow<T>(0.0f);
