@@ -580,17 +580,6 @@ __device__ __forceinline__ void ce_load8(T (&v)[8], const T* source, bool wide, 
     if (wide && w * 8 + 8 <= channels) {
 #pragma unroll
         for (int i = 0; i < (int)sizeof(v) / 16; ++i) ((uint4*)v)[i] = ((const uint4*)(source + w * 8))[i];
-    } else if (sizeof(T) == 2 && w && w * 8 + 16 <= channels) {  // neighbours on both sides: two pieces on 16 bytes
-        const uint4* const pieces = (const uint4*)((uintptr_t)(source + w * 8) & ~(uintptr_t)15);
-        const uint4 a = pieces[0], b = pieces[1];
-        const uint32_t phase = (uint32_t)(uintptr_t)source & 15, shift = phase & 2 ? 16 : 0;  // the same along a row
-        const uint32_t x[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-#pragma unroll
-        for (uint32_t first = 0; first < 4; ++first) {
-            if (phase >> 2 != first) continue;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) ((uint32_t*)v)[i] = __funnelshift_r(x[first + i], x[first + i + 1], shift);
-        }
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = w * 8 + i < channels ? source[w * 8 + i] : narrow<T>(0.0f);
@@ -611,12 +600,41 @@ ce_pack_kernel(const T* from, uint64_t from_stride, const uint32_t* row, const u
     const uint32_t lane = threadIdx.x & 31;
     for (uint64_t r = (uint64_t)blockIdx.x * 8 + (threadIdx.x >> 5); r < last; r += (uint64_t)gridDim.x * 8) {
         const T* const source = r < have ? from + (row ? row[r] : r) * from_stride : nullptr;
-#pragma unroll 4
-        for (uint32_t w = lane; w < words; w += 32) {
+        uint4* const out = (uint4*)((T*)to + r * to_stride);
+        auto copy = [&](uint32_t w) {
             alignas(16) T v[8] = {};
             if (source) ce_load8(v, source, wide, w, channels);
-            *(uint4*)((T*)to + r * to_stride + w * 8) = *(const uint4*)v;
+            out[w] = *(const uint4*)v;
+        };
+        if (wide || !source) {
+#pragma unroll 4
+            for (uint32_t w = lane; w < words; w += 32) copy(w);
+            continue;
         }
+        // Pieces with neighbours on both sides: put together from the two on 16 bytes that they lie in, four at a time.
+        const uint32_t end = max(channels / 8, 2u) - 1;  // 8 end + 8 <= channels; from 1 on
+        const uint32_t phase = (uint32_t)(uintptr_t)source & 15, shift = phase & 2 ? 16 : 0;
+        const uint4* const pieces = (const uint4*)((uintptr_t)source & ~(uintptr_t)15);
+        for (uint32_t w0 = 1 + lane; w0 < end; w0 += 128) {
+            uint4 a[4], b[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (w0 + i * 32 < end) a[i] = pieces[w0 + i * 32], b[i] = pieces[w0 + i * 32 + 1];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t x[8] = {a[i].x, a[i].y, a[i].z, a[i].w, b[i].x, b[i].y, b[i].z, b[i].w};
+                uint32_t v[4];
+#pragma unroll
+                for (uint32_t first = 0; first < 4; ++first) {
+                    if (phase >> 2 != first) continue;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) v[j] = __funnelshift_r(x[first + j], x[first + j + 1], shift);
+                }
+                if (w0 + i * 32 < end) out[w0 + i * 32] = make_uint4(v[0], v[1], v[2], v[3]);
+            }
+        }
+        if (lane == 0) copy(0);
+        for (uint32_t w = end + lane; w < words; w += 32) copy(w);
     }
 }
 
