@@ -752,9 +752,9 @@ dr_forward_kernel(const __grid_constant__ DrChain p) {
         // r = S0 K^T (value x token) and out = Q S0^T (token x value)
         float r[8][4] = {}, y[4][2][4] = {};
         const float top = max_abs(s);
-        const Scale ss = coarse_scale_for(top);
+        const Scale ss = coarse_scale_for(top, back_domain);
         uint8_t* const states = ALL && p.states.at ? cta.mine(p.states.of(unit), NB) : nullptr;
-        if (states) cta.keep_back(p.states.back, unit, ss.back * back_domain);
+        if (states) cta.keep_back(p.states.back, unit, kept_back(top, ss.back * back_domain));
 #pragma unroll
         for (int kk = 0; kk < DK / 16; ++kk) {
             uint32_t hi[4], lo[4];
@@ -811,9 +811,10 @@ dr_forward_kernel(const __grid_constant__ DrChain p) {
         }
         const float back_w = sr.back * gt.back_inverse;
         if (ALL && p.kept.at) {
-            const Scale sw = coarse_scale_for(max_abs(w));
+            const float most = max_abs(w);
+            const Scale sw = coarse_scale_for(most, back_w);
             uint8_t* const kept = cta.mine(p.kept.of(unit), 1);
-            cta.keep_back(p.kept.back, unit, sw.back * back_w);
+            cta.keep_back(p.kept.back, unit, kept_back(most, sw.back * back_w));
 #pragma unroll
             for (int kt = 0; kt < 4; ++kt) {
                 uint32_t hi[4], lo[4];
@@ -919,10 +920,10 @@ dr_backward_kernel(const __grid_constant__ DrChain p) {
         // du = e X K^T (value x token)
         float du[8][4] = {};
         const float top = max_abs(x);
-        const Scale sx = coarse_scale_for(top);
+        const Scale sx = coarse_scale_for(top, back_domain);
         const float finest = Cta::finest(top, sx.back * back_domain);
         uint8_t* const states = ALL ? cta.mine(p.states.of(unit), Cta::NB) : nullptr;
-        if constexpr (ALL) cta.keep_back(p.states.back, unit, sx.back * back_domain);
+        if constexpr (ALL) cta.keep_back(p.states.back, unit, kept_back(top, sx.back * back_domain));
 #pragma unroll
         for (int kk = 0; kk < DK / 16; ++kk) {
             uint32_t hi[4], lo[4];
@@ -945,8 +946,9 @@ dr_backward_kernel(const __grid_constant__ DrChain p) {
                 }
             }
         }
-        const Scale so = scale_up_to(coarse_scale_for(warp_max(most)), finest), sg = scale_up_to(scale_for(warp_max(most_g) * fabsf(p.sh.scale)), finest);
-        if constexpr (ALL) cta.keep_back(p.back_values, unit, so.back);
+        most = warp_max(most);
+        const Scale so = scale_up_to(coarse_scale_for(most), finest), sg = scale_up_to(scale_for(warp_max(most_g) * fabsf(p.sh.scale)), finest);
+        if constexpr (ALL) cta.keep_back(p.back_values, unit, kept_back(most, so.back));
         {
             const float back = (sx.back * back_domain * gt.back_k) * (so.by * power_inverse(gt.back_read));
 #pragma unroll
@@ -1001,9 +1003,10 @@ dr_backward_kernel(const __grid_constant__ DrChain p) {
         }
         const float back_z = sd.back * gt.back_inverse * so.back * gt.back_read;
         if constexpr (ALL) {
-            const Scale sz = coarse_scale_for(max_abs(z));
+            const float most_z = max_abs(z);
+            const Scale sz = coarse_scale_for(most_z, back_z);
             uint8_t* const kept = cta.mine(p.kept.of(unit), 1);
-            cta.keep_back(p.kept.back, unit, sz.back * back_z);
+            cta.keep_back(p.kept.back, unit, kept_back(most_z, sz.back * back_z));
 #pragma unroll
             for (int kt = 0; kt < 4; ++kt) {
                 uint32_t hi[4], lo[4];
@@ -1118,7 +1121,7 @@ struct DrGradientSmem {
     alignas(128) DrGates gates[2];     // of a head and the next
     alignas(32) float back[2][5][8];   // inverse scales of S, X, w, z and dO by 16 value dimensions
     float dbeta[2][DR_CHUNK];
-    float scales[16][5];               // of a warp's products
+    float scales[16][5];               // of a warp's products over the value dimensions
     float dot[4][DR_CHUNK], carry[4][DR_CHUNK], sx[16];
     alignas(16) float most[2][16];
     uint64_t full[2], empty[2], keys_full;
@@ -1224,8 +1227,10 @@ dr_gradient_kernel(const __grid_constant__ DrGradient p) {
         const DrGates& gates = sm.gates[(h - h0) & 1];
         const float(&back)[5][8] = sm.back[(h - h0) & 1];
         enum { S, X, W, Z, GO };
-        float* const most = sm.scales[warp];  // of dO S0, z S0, w X, dO w and z w: the largest of the value dimensions'
-        uint32_t uneven = 0;  // which of them have others, too
+        // The scales of dO S0, z S0, w X, dO w and z w: that of all 16 value dimensions which have any, or 1 where they differ
+        // (uneven): their products are added in float32 then, each by its own.
+        float* const unit = sm.scales[warp];
+        uint32_t uneven = 0;
         float dq[NT][4] = {}, er[NT][4] = {}, wr[NT][4] = {}, a[2][4] = {}, n[2][4] = {};
         float sx = 0.0f;
         for (uint32_t v = 0; v < steps; ++v, ++it) {
@@ -1239,18 +1244,29 @@ dr_gradient_kernel(const __grid_constant__ DrGradient p) {
             if (v == 0) {
                 const int at = lane & 7;
                 const bool have = at < (int)groups;
-                const float mine[5] = {back[GO][at] * back[S][at], back[Z][at] * back[S][at], back[W][at] * back[X][at], back[GO][at] * back[W][at],
-                                       back[Z][at] * back[W][at]};
+                const float x[5] = {back[GO][at], back[Z][at], back[W][at], back[GO][at], back[Z][at]},
+                            y[5] = {back[S][at], back[S][at], back[X][at], back[W][at], back[W][at]};
 #pragma unroll
                 for (int i = 0; i < 5; ++i) {
-                    const float largest = warp_max(have ? mine[i] : 0.0f);
-                    if (lane == 0) most[i] = largest;
-                    uneven |= (uint32_t)__any_sync(0xffffffffu, have && mine[i] != largest) << i;
+                    const float mine = x[i] * y[i], largest = warp_max(have ? mine : 0.0f);
+                    const bool differ = __any_sync(0xffffffffu, have && x[i] != 0.0f && y[i] != 0.0f && mine != largest);
+                    if (lane == 0) unit[i] = differ ? 1.0f : largest;
+                    uneven |= (uint32_t)differ << i;
                 }
                 __syncwarp();
             }
-            // a product's share of the largest scale
-            auto share = [&](int i, float x, float y) { return __float2half2_rn(x * y * power_inverse(most[i])); };
+            // c0, c1 += the i-th product over the value dimensions 16 at .. with the scales of x and y
+            auto add = [&](int i, float (&c0)[4], float (&c1)[4], int x, int y, uint32_t at, auto&& products) {
+                if (!(uneven >> i & 1)) {
+                    products(c0, c1);
+                    return;
+                }
+                float d0[4] = {}, d1[4] = {};
+                products(d0, d1);
+                const float by = back[x][at], then = back[y][at];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) c0[j] = fmaf(d0[j] * by, then, c0[j]), c1[j] = fmaf(d1[j] * by, then, c1[j]);
+            };
             const uint8_t* const step = sm.step[it & 1];
             const float beta0 = gates.beta[token], beta1 = gates.beta[token + 8];
             T* const dv0 = (T*)p.dv + ((c.row + token) * sh.heads + h) * sh.value_dim;
@@ -1261,7 +1277,6 @@ dr_gradient_kernel(const __grid_constant__ DrGradient p) {
             for (int kt = 0; kt < 2; ++kt) {
                 const uint32_t at = v * 2 + kt;  // 16 value dimensions
                 if (at >= groups) break;
-                // dO (and z below) against S0, and against w: shares of the scales differ
                 uint32_t go[2][4], aw[2][4], zt[2][4];
                 if (p.out) {
                     const float by = power_inverse(back[GO][at]);
@@ -1300,65 +1315,46 @@ dr_gradient_kernel(const __grid_constant__ DrGradient p) {
                             dr_store_pair((j & 1) ? dv1 : dv0, vcol + (j >> 1) * 8, sh.value_dim, p.pairs_v, b * (hi.x + lo.x), b * (hi.y + lo.y));
                     }
                 }
-                if (uneven & 4) {
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) scale_f16(aw[i], share(2, back[W][at], back[X][at]));
-                }
-                {  // against w first, as they are; then scaled on to what S0 wants
-                    uint32_t gw[2][4], zw[2][4];
-#pragma unroll
-                    for (int i = 0; i < 2; ++i)
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) gw[i][j] = go[i][j], zw[i][j] = zt[i][j];
-                    if (uneven & 8 && p.out) {
-#pragma unroll
-                        for (int i = 0; i < (EXACT ? 1 : 2); ++i) scale_f16(gw[i], share(3, back[GO][at], back[W][at]));
-                    }
-                    if (uneven & 16) {
-#pragma unroll
-                        for (int i = 0; i < 2; ++i) scale_f16(zw[i], share(4, back[Z][at], back[W][at]));
-                    }
-                    if (cq <= rb) {  // 16 of the other tokens
-                        uint32_t b[4];
-                        load_b_t(b, w, kt * 16, cq, o);
-                        if (p.out) {
-                            mma_f16_2(a[0], a[1], gw[0], b);
-                            if constexpr (!EXACT) mma_f16_2(a[0], a[1], gw[1], b);
-                        }
-                        mma_f16_2(n[0], n[1], zw[0], b);
-                        mma_f16_2(n[0], n[1], zw[1], b);
-                        load_b_t(b, w + DR_PIECE, kt * 16, cq, o);
-                        if (p.out) mma_f16_2(a[0], a[1], gw[0], b);
-                        mma_f16_2(n[0], n[1], zw[0], b);
-                    }
-                }
-                if (uneven & 1 && p.out) {
-#pragma unroll
-                    for (int i = 0; i < (EXACT ? 1 : 2); ++i) scale_f16(go[i], share(0, back[GO][at], back[S][at]));
-                }
-                if (uneven & 2) {
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) scale_f16(zt[i], share(1, back[Z][at], back[S][at]));
+                if (cq <= rb) {  // 16 of the other tokens
+                    uint32_t b[2][4];
+                    load_b_t(b[0], w, kt * 16, cq, o);
+                    load_b_t(b[1], w + DR_PIECE, kt * 16, cq, o);
+                    if (p.out)
+                        add(3, a[0], a[1], GO, W, at, [&](float(&c0)[4], float(&c1)[4]) {
+                            mma_f16_2(c0, c1, go[0], b[0]);
+                            if constexpr (!EXACT) mma_f16_2(c0, c1, go[1], b[0]);
+                            mma_f16_2(c0, c1, go[0], b[1]);
+                        });
+                    add(4, n[0], n[1], Z, W, at, [&](float(&c0)[4], float(&c1)[4]) {
+                        mma_f16_2(c0, c1, zt[0], b[0]);
+                        mma_f16_2(c0, c1, zt[1], b[0]);
+                        mma_f16_2(c0, c1, zt[0], b[1]);
+                    });
                 }
 #pragma unroll
                 for (int j = 0; j < NP; ++j) {
                     const int first = cq * (DK / 4) + j * 16, block = first / 64 * DR_PIECE, jj = first % 64 / 16;
-                    uint32_t b[4];
-                    load_b_t(b, s + block, kt * 16, jj, o);
-                    if (p.out) {
-                        mma_f16_2(dq[2 * j], dq[2 * j + 1], go[0], b);
-                        if constexpr (!EXACT) mma_f16_2(dq[2 * j], dq[2 * j + 1], go[1], b);
-                    }
-                    mma_f16_2(er[2 * j], er[2 * j + 1], zt[0], b);
-                    mma_f16_2(er[2 * j], er[2 * j + 1], zt[1], b);
-                    load_b_t(b, s + NB * DR_PIECE + block, kt * 16, jj, o);
-                    if (p.out) mma_f16_2(dq[2 * j], dq[2 * j + 1], go[0], b);
-                    mma_f16_2(er[2 * j], er[2 * j + 1], zt[0], b);
-                    load_b_t(b, x + block, kt * 16, jj, o);
-                    mma_f16_2(wr[2 * j], wr[2 * j + 1], aw[0], b);
-                    mma_f16_2(wr[2 * j], wr[2 * j + 1], aw[1], b);
-                    load_b_t(b, x + NB * DR_PIECE + block, kt * 16, jj, o);
-                    mma_f16_2(wr[2 * j], wr[2 * j + 1], aw[0], b);
+                    uint32_t b[2][4];
+                    load_b_t(b[0], s + block, kt * 16, jj, o);
+                    load_b_t(b[1], s + NB * DR_PIECE + block, kt * 16, jj, o);
+                    if (p.out)
+                        add(0, dq[2 * j], dq[2 * j + 1], GO, S, at, [&](float(&c0)[4], float(&c1)[4]) {
+                            mma_f16_2(c0, c1, go[0], b[0]);
+                            if constexpr (!EXACT) mma_f16_2(c0, c1, go[1], b[0]);
+                            mma_f16_2(c0, c1, go[0], b[1]);
+                        });
+                    add(1, er[2 * j], er[2 * j + 1], Z, S, at, [&](float(&c0)[4], float(&c1)[4]) {
+                        mma_f16_2(c0, c1, zt[0], b[0]);
+                        mma_f16_2(c0, c1, zt[1], b[0]);
+                        mma_f16_2(c0, c1, zt[0], b[1]);
+                    });
+                    load_b_t(b[0], x + block, kt * 16, jj, o);
+                    load_b_t(b[1], x + NB * DR_PIECE + block, kt * 16, jj, o);
+                    add(2, wr[2 * j], wr[2 * j + 1], W, X, at, [&](float(&c0)[4], float(&c1)[4]) {
+                        mma_f16_2(c0, c1, aw[0], b[0]);
+                        mma_f16_2(c0, c1, aw[1], b[0]);
+                        mma_f16_2(c0, c1, aw[0], b[1]);
+                    });
                 }
             }
             // <S0, X> of the step's 32 rows: the diagonal of S0 X^T, 16 rows and 16 key columns a warp
@@ -1387,11 +1383,11 @@ dr_gradient_kernel(const __grid_constant__ DrGradient p) {
         for (int j = 0; j < 2; ++j)
 #pragma unroll
             for (int m = 0; m < 4; ++m)
-                if (cq * 16 + j * 8 + col + (m & 1) == (int)token + (m >> 1) * 8) sm.dbeta[(h - h0) & 1][token + (m >> 1) * 8] = n[j][m] * most[4];
+                if (cq * 16 + j * 8 + col + (m & 1) == (int)token + (m >> 1) * 8) sm.dbeta[(h - h0) & 1][token + (m >> 1) * 8] = n[j][m] * unit[4];
         // scale D dA and D dN: dA_ij = beta_j a_ij, dN_ij = -beta_i beta_j n_ij
         float most_a = 0.0f, most_n = 0.0f;
         {
-            const float back_a = most[3] * sh.scale, back_n = -most[4];
+            const float back_a = unit[3] * sh.scale, back_n = -unit[4];
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 if (cq > rb) break;  // zeros
@@ -1434,7 +1430,7 @@ dr_gradient_kernel(const __grid_constant__ DrGradient p) {
         for (int half = 0; half < 2; ++half) {
             const int i = token + half * 8;
             const float g0 = gates.g[i], b = gates.beta[i];
-            const float fq = g0 * sh.scale * most[0] * into_q, fe = -g0 * b * most[1] * into_n, fw = gates.e[i] * b * most[2];
+            const float fq = g0 * sh.scale * unit[0] * into_q, fe = -g0 * b * unit[1] * into_n, fw = gates.e[i] * b * unit[2];
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
                 const int first = cq * (DK / 4) + j * 8 + col;

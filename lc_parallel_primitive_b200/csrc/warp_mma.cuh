@@ -96,11 +96,15 @@ __device__ __forceinline__ Scale scale_for(float most) {
 }
 // The scale, or `by` if that is less.
 __device__ __forceinline__ Scale scale_up_to(Scale s, float by) { return s.by > by ? Scale{by, power_inverse(by)} : s; }
-// With an exponent that is a multiple of 8, so that most * by is in [2^7, 2^15): matrices of like size share it.
-__device__ __forceinline__ Scale coarse_scale_for(float most) {
-    const int e = __float_as_int(most) >> 23 & 255;
-    return scale_of_field(e, min((268 - e - 127 + 1024) / 8 * 8 - 1024 + 127, 207));
+// Of values that are `back` times smaller or larger than they stand here (a power of two): by / back is a power of 2^8, so that
+// matrices of like size share it, and most * by is in [2^7, 2^15).
+__device__ __forceinline__ Scale coarse_scale_for(float most, float back = 1.0f) {
+    const int e = __float_as_int(most) >> 23 & 255, own = (__float_as_int(back) >> 23 & 255) - 127;
+    return scale_of_field(e, own + ((min(141 - e, 80) - own) >> 3) * 8 + 127);
 }
+// The inverse scale of what is kept as float16: 0 of nothing (or of what is below float32's normal numbers, of which by = 1
+// leaves nothing), which says nothing of the sizes beside it.
+__device__ __forceinline__ float kept_back(float most, float back) { return most < 1.17549435e-38f ? 0.0f : back; }
 __device__ __forceinline__ float warp_max(float v) {  // of values >= 0
     return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(v)));
 }
@@ -171,14 +175,6 @@ __device__ __forceinline__ void split_block(const float (&c0)[4], const float (&
     split_f16(c1[0], c1[1], s, hi[2], lo[2]);
     split_f16(c1[2], c1[3], s, hi[3], lo[3]);
 }
-__device__ __forceinline__ void scale_f16(uint32_t (&r)[4], __half2 by) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const __half2 v = __hmul2(*(const __half2*)&r[j], by);
-        r[j] = *(const uint32_t*)&v;
-    }
-}
-
 __device__ __forceinline__ uint32_t lds32(uint32_t addr) {
     uint32_t v;
     asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
