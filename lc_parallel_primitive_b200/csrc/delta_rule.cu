@@ -947,8 +947,9 @@ dr_backward_kernel(const __grid_constant__ DrChain p) {
             }
         }
         most = warp_max(most);
-        const Scale so = scale_up_to(coarse_scale_for(most), finest), sg = scale_up_to(scale_for(warp_max(most_g) * fabsf(p.sh.scale)), finest);
-        if constexpr (ALL) cta.keep_back(p.back_values, unit, kept_back(most, so.back));
+        // beside X only what may be added to it counts; the gradients of q, which have dO alone, want its own scale
+        const Scale own = coarse_scale_for(most), so = scale_up_to(own, finest), sg = scale_up_to(scale_for(warp_max(most_g) * fabsf(p.sh.scale)), finest);
+        if constexpr (ALL) cta.keep_back(p.back_values, unit, kept_back(most, own.back));
         {
             const float back = (sx.back * back_domain * gt.back_k) * (so.by * power_inverse(gt.back_read));
 #pragma unroll

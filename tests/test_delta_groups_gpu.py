@@ -2,7 +2,8 @@
 import numpy as np
 import pytest
 
-from tests.test_delta_gpu import Case
+from tests import delta_reference as R
+from tests.test_delta_gpu import Case, host
 
 pytestmark = pytest.mark.gpu
 
@@ -60,3 +61,23 @@ def test_groups_of_different_sizes(cuda, dtype, step, names, heads, key_heads, d
         for n in names:
             grouped(c, n, f)
         c.check(use_last="grad_last" in names, use_out="grad_out" in names or "v" in names)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("size", [1e-10, 1e-18, 1e-24])
+def test_small_gradients_of_outputs_beside_large_ones_of_states(cuda, dtype, size):
+    """grad_q is made of grad_out alone: its bound is that of tests.delta_reference.bounds without the states' gradient, of
+    scale |grad_out| M, with the largest gradient of the sequence for each value dimension."""
+    c = Case([130, 70], 2, 1, 64, 48, dtype, seed=33)
+    c.grad_out.mul_(size)
+    f = c.reference()
+    c.run()
+    got, want = c.back(), R.backward(f, host(c.grad_out), host(c.grad_last))
+    bound = np.zeros((c.rows, c.heads, 1))
+    go = np.abs(host(c.grad_out))
+    for s in range(2):
+        a, b = c.offsets[s], c.offsets[s + 1]
+        unit = R.UNIT * np.sqrt(-(-(b - a) // 64))
+        bound[a:b] = 2 * unit * f.scale * np.sqrt(((go[a:b].max(0) * f.most[s]) ** 2).sum(1))[:, None]
+    bound = bound.reshape(c.rows, 1, 2, 1).sum(2)
+    R.assert_within(host(got.q), want.q, bound, dtype, "grad q")
