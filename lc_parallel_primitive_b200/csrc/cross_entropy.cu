@@ -83,7 +83,7 @@ struct CeGemm {
     uint32_t splits;          // CE_HIDDEN: parts of K, each with its own sum
     uint32_t row0, row_end;   // CE_WEIGHT: the slots to sum over, of those that there are
     uint32_t add;             // add to what is there
-    float2* part;             // CE_LOGSUM: (maximum, sum of 2^(z log2 e - maximum)) by 128 columns and slot
+    float2* part;             // CE_LOGSUM: (maximum, sum of exp(z - maximum)) by 128 columns and slot
     float* right;             // CE_LOGSUM: the targets' logits by slot
     void* grad;               // CE_GRAD: G (planes, padded, grad_stride)
     uint64_t grad_stride;
@@ -166,6 +166,15 @@ __device__ __forceinline__ float ce_exp2(float v) {
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
     return r;
+}
+// v = exp(v - shift): the difference is taken first, so that a row's largest logit gives exactly 1.
+__device__ __forceinline__ void ce_exp32(float (&v)[32], float shift) {
+    const uint64_t s = pair_of(shift, shift), by = pair_of(CE_LOG2E, CE_LOG2E);
+#pragma unroll
+    for (int i = 0; i < 32; i += 2) {
+        pair_split(pair_mul(pair_sub(pair_of(v[i], v[i + 1]), s), by), v[i], v[i + 1]);
+        v[i] = ce_exp2(v[i]), v[i + 1] = ce_exp2(v[i + 1]);
+    }
 }
 
 // 32 bytes, a whole sector, on a 32-byte boundary.
@@ -272,12 +281,12 @@ __device__ __forceinline__ void ce_epilogue(const CeGemm& p, uint32_t tmem, uint
             float most = v[0];
 #pragma unroll
             for (int i = 1; i < 32; ++i) most = fmaxf(most, v[i]);
-            most *= CE_LOG2E;
             const float base = fmaxf(top, most), shift = base == -INFINITY ? 0.0f : base;
             float s[4] = {0, 0, 0, 0};
+            ce_exp32(v, shift);
 #pragma unroll
-            for (int i = 0; i < 32; ++i) s[i & 3] += ce_exp2(fmaf(v[i], CE_LOG2E, -shift));
-            sum = sum * ce_exp2(top - shift) + ((s[0] + s[1]) + (s[2] + s[3]));
+            for (int i = 0; i < 32; ++i) s[i & 3] += v[i];
+            sum = sum * ce_exp2((top - shift) * CE_LOG2E) + ((s[0] + s[1]) + (s[2] + s[3]));
             top = base;
         }
         if (live) {
@@ -288,7 +297,7 @@ __device__ __forceinline__ void ce_epilogue(const CeGemm& p, uint32_t tmem, uint
         using E = std::conditional_t<std::is_same_v<T, __half>, __half, __nv_bfloat16>;
         const bool live = m < count;
         const int64_t target = live ? (int64_t)p.plan.target[m] - (int64_t)p.vocab0 - n0 : -1;
-        const float shift = live ? p.plan.logsum[m] * CE_LOG2E : 0.0f;
+        const float logsum = live ? p.plan.logsum[m] : 0.0f;
         float gain = live ? p.plan.gain[m] : 0.0f;
         if (live && gain != 0.0f) gain = gain / *p.plan.largest * CE_GAIN<T>;
         const float back = sizeof(T) == 4 && live ? p.hidden_back[m] : 0.0f;
@@ -299,8 +308,7 @@ __device__ __forceinline__ void ce_epilogue(const CeGemm& p, uint32_t tmem, uint
             const int width = (int)p.grad_stride - (int)n0 - c;
             if (width <= 0) break;
             ce_unscale<T>(v, back, p.weight_back + p.vocab0 + n0 + c);
-#pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = ce_exp2(fmaf(v[i], CE_LOG2E, -shift));
+            ce_exp32(v, logsum);
             if (target >= c && target < c + 32) {
 #pragma unroll
                 for (int i = 0; i < 32; ++i)
@@ -705,7 +713,7 @@ ce_loss_kernel(const float2* part, uint32_t parts, const float* right, CePlan pl
     float top = -INFINITY, sum = 0.0f;
     auto join = [&](float2 v) {
         const float base = fmaxf(top, v.x), shift = base == -INFINITY ? 0.0f : base;
-        sum = sum * ce_exp2(top - shift) + v.y * ce_exp2(v.x - shift);
+        sum = sum * ce_exp2((top - shift) * CE_LOG2E) + v.y * ce_exp2((v.x - shift) * CE_LOG2E);
         top = base;
     };
     if (slot >= 0) {
@@ -723,9 +731,9 @@ ce_loss_kernel(const float2* part, uint32_t parts, const float* right, CePlan pl
     __syncthreads();
     if (warp == 0 && r < rows) {
         for (int w = 1; w < CE_LOSS_WARPS; ++w) join(joined[w][lane]);
-        const float total = (top + log2f(sum)) * 0.693147180559945f;
-        if (loss) loss[r] = slot >= 0 ? total - right[slot] : 0.0f;
-        if (logsum) logsum[r] = slot >= 0 ? total : 0.0f;
+        const float rest = logf(sum);  // sum >= 1, right <= top: the loss is never negative
+        if (loss) loss[r] = slot >= 0 ? (top - right[slot]) + rest : 0.0f;
+        if (logsum) logsum[r] = slot >= 0 ? top + rest : 0.0f;
     }
 }
 
