@@ -17,7 +17,8 @@ class DeviceCrossEntropy : public LuisaModule {
         m_debug_stream = debug_stream;
     }
 
-    // For Forward, or (backward) for both calls; aligned false: d_weight may start off a 16-byte boundary.
+    // For Forward, or (backward) for both calls, with so many rows or fewer; aligned false: d_weight may start off a
+    // 16-byte boundary.
     template <SequenceFloatT T>
     static size_t GetTempStorageBytes(size_t num_rows, size_t num_channels, size_t vocab, bool backward = true, bool aligned = true) {
         return lcpp_cross_entropy_temp_bytes(lcpp_float_dtype_of<T>(), num_rows, num_channels, vocab, backward, aligned);

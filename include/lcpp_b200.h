@@ -384,7 +384,7 @@ lcpp_status lcpp_delta_rule_step(int dtype, const lcpp_delta_shape* shape, const
  * does the same and leaves LCPP_ERR_INVALID_ARG in the device error word.  loss or logsum may be NULL.
  * rows <= 2^24, vocab <= 2^30; temp is refused where it is not 32-byte aligned.  What is written, temp included, must
  * not overlap anything else.
- * temp bytes: for the forward call, or (backward != 0) for both; aligned = 0 where a row of weight may start off a
+ * temp bytes: for the forward call, or (backward != 0) for both, with so many rows or fewer; aligned = 0 where a row of weight may start off a
  * 16-byte boundary (it is copied then, as it is for channels that are no multiple of 8 and for float32). */
 size_t      lcpp_cross_entropy_temp_bytes(int dtype, uint64_t rows, uint64_t channels, uint64_t vocab, int backward,
                                           int aligned);

@@ -965,8 +965,12 @@ extern "C" size_t lcpp_cross_entropy_temp_bytes(int dtype, uint64_t rows, uint64
     if (!rows || !channels || !vocab) return 256;
     // with gradients the loss's own buffer may be wanted too
     const bool pack = dtype == LCPP_F32 || !aligned || channels % 8;
-    const size_t loss = CeLayout(dtype, rows, channels, vocab, false, pack).bytes;
-    return backward ? max(loss, CeLayout(dtype, rows, channels, vocab, true, pack).bytes) : loss;
+    size_t most = CeLayout(dtype, rows, channels, vocab, false, pack).bytes;
+    if (!backward) return most;
+    // Fewer rows may want more, with larger pieces of G or more splits: the buffer serves any number up to this one.
+    most = max(most, CeLayout(dtype, rows, channels, vocab, true, pack).bytes);
+    for (uint64_t fewer = CE_BM; fewer < rows; fewer += CE_BM) most = max(most, CeLayout(dtype, fewer, channels, vocab, true, pack).bytes);
+    return most;
 }
 
 extern "C" lcpp_status lcpp_cross_entropy_forward(int dtype, const void* hidden, uint64_t hidden_stride, const void* weight,

@@ -538,7 +538,8 @@ class DeviceCrossEntropy(_Recorded):
     @staticmethod
     def GetTempStorageBytes(num_rows: int, num_channels: int, vocab: int, dtype=torch.bfloat16, backward: bool = True,
                             aligned: bool = True) -> int:
-        """For Forward, or for both calls; aligned=False: rows of d_weight may start off a 16-byte boundary."""
+        """For Forward, or for both calls, with so many rows or fewer; aligned=False: rows of d_weight may start off a
+        16-byte boundary."""
         if dtype not in _FLOATS:
             raise TypeError(f"unsupported element type {dtype}")
         return int(L.lib().lcpp_cross_entropy_temp_bytes(_FLOATS[dtype], num_rows, num_channels, vocab, backward, aligned))

@@ -38,3 +38,16 @@ def test_losses_are_not_negative(cuda, dtype):
     c.run(grads="")
     assert float(c.loss.min()) >= 0.0 and (c.loss <= 1e-3).sum() > 100
     assert not torch.isnan(c.loss).any() and np.isfinite(float(c.loss.max()))
+
+
+@pytest.mark.parametrize("dtype,channels,vocab,rows,more", [("bf16", 256, 5000, 6144, 6400), ("f32", 40, 33000, 2560, 2816)])
+def test_a_buffer_for_more_rows(cuda, dtype, channels, vocab, rows, more):
+    # these fewer rows take more pieces or splits of their own
+    import torch
+    from lc_parallel_primitive_b200 import DeviceCrossEntropy, temp_buffer
+    from tests.test_cross_entropy_gpu import torch_dtype
+
+    c = Case(rows, channels, vocab, dtype, seed=43)
+    want = [t.clone() for t in c.run()]
+    got = c.run(temp=temp_buffer(DeviceCrossEntropy.GetTempStorageBytes(more, channels, vocab, torch_dtype(dtype))))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
