@@ -379,13 +379,16 @@ lcpp_status lcpp_delta_rule_step(int dtype, const lcpp_delta_shape* shape, const
  *   z = hidden weight^T,  logsum[i] = log sum_v exp(z_iv),  loss[i] = logsum[i] - z_i,targets[i]
  * hidden is [rows][channels], weight [vocab][channels], both of dtype; products are summed in float32 (float32 operands
  * in parts: of two float16 with a scale for each row in the logits, 2^-22 of a product, or 2^-39 of its rows' largest
- * values where that is more; of three bf16 in the gradients, about 2^-24).  A row with a negative target takes no part: its loss, logsum and
+ * values where that is more; of three bf16 in the gradients, about 2^-24).  The tensor cores cut sums off, so that a logit
+ * comes out too small by up to 1.2e-9 of itself a channel, 5e-6 for 4096.  A loss is never negative.
+ * A row with a negative target takes no part: its loss, logsum and
  * gradient are 0, it adds nothing to the weight's gradient, and its hidden state may hold anything; a target >= vocab
  * does the same and leaves LCPP_ERR_INVALID_ARG in the device error word.  loss or logsum may be NULL.
  * rows <= 2^24, vocab <= 2^30; temp is refused where it is not 32-byte aligned.  What is written, temp included, must
  * not overlap anything else.
- * temp bytes: for the forward call, or (backward != 0) for both, with so many rows or fewer; aligned = 0 where a row of weight may start off a
- * 16-byte boundary (it is copied then, as it is for channels that are no multiple of 8 and for float32). */
+ * temp bytes: for the forward call, or (backward != 0) for both, with so many rows or fewer; aligned = 0 where a row of
+ * weight may start off a 16-byte boundary (it is copied then, as it is for channels that are no multiple of 8 and for
+ * float32). */
 size_t      lcpp_cross_entropy_temp_bytes(int dtype, uint64_t rows, uint64_t channels, uint64_t vocab, int backward,
                                           int aligned);
 lcpp_status lcpp_cross_entropy_forward(int dtype, const void* hidden, uint64_t hidden_stride, const void* weight,

@@ -146,7 +146,7 @@ struct CeTiles {
         if (parts == 1) return 0;
         return unit >> 32 ? (uint32_t)(unit / ((uint64_t)m * n)) : (uint32_t)unit / (m * n);  // m n < 2^28
     }
-    // Steps along K of a part; parts <= 64 and steps <= 2^24.
+    // Steps along K of a part; parts <= CE_MAX_SPLITS and steps <= 2^24.
     __device__ __forceinline__ void range(uint32_t part, uint32_t* first, uint32_t* end) const {
         *first = steps * part / parts, *end = steps * (part + 1) / parts;
     }
@@ -774,7 +774,8 @@ constexpr uint64_t CE_PIECE_BYTES = 512ull << 20;  // of G
 // The tensor cores' sums are cut off, not rounded, at every step: they come out too small by about 1.2e-9 of themselves a
 // term.  Beside the roundings of 16-bit gradients that is nothing, but float32 ones take this many terms a sum at most, and
 // add the sums in float32 (weight gradient of 16384 rows in one sum: error 1.9e-5, so 4.8e-6).
-constexpr uint64_t CE_EXACT_TERMS = 4096;
+constexpr uint64_t CE_EXACT_TERMS = 4096, CE_MAX_SPLITS = 64;
+static_assert(CE_EXACT_TERMS % CE_BK == 0, "splits are whole steps");
 
 // The pieces of the temp buffer.
 struct CeLayout {
@@ -788,7 +789,8 @@ struct CeLayout {
         pitch = align_up(channels, 8);
         parts = ceil_div(vocab, CE_BN) * 2;
         sum_pitch = align_up(channels, 8);
-        const uint64_t widest = max(CE_PIECE_BYTES / (planes * padded * 2) / CE_BN * CE_BN, (uint64_t)CE_BN);
+        uint64_t widest = max(CE_PIECE_BYTES / (planes * padded * 2) / CE_BN * CE_BN, (uint64_t)CE_BN);
+        if (planes > 1) widest = min(widest, CE_MAX_SPLITS * CE_EXACT_TERMS);
         const uint64_t pieces = ceil_div(vocab, widest);
         piece = min(align_up(ceil_div(vocab, pieces), CE_BN), align_up(vocab, 16));  // rows of G on 32 bytes
         splits = best_splits(padded, channels, piece, planes);
@@ -823,7 +825,7 @@ struct CeLayout {
     // of 64 takes 0.33 us) and of the parts' sums (float32, written and read once a piece).
     static uint64_t best_splits(uint64_t padded, uint64_t channels, uint64_t piece, uint64_t planes) {
         const uint64_t pairs = device_info().sms / 2, tiles = padded / CE_BM * ceil_div(channels, CE_BN), steps = ceil_div(piece, CE_BK);
-        const uint64_t fewest = planes == 1 ? 1 : min(ceil_div(piece, CE_EXACT_TERMS), (uint64_t)64);
+        const uint64_t fewest = planes == 1 ? 1 : ceil_div(piece, CE_EXACT_TERMS);
         uint64_t best = fewest;
         double least = 0;
         for (uint64_t n = fewest; n <= max(fewest, (uint64_t)32) && (n == fewest || n * 16 <= steps); ++n) {

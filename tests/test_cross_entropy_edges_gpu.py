@@ -51,3 +51,8 @@ def test_a_buffer_for_more_rows(cuda, dtype, channels, vocab, rows, more):
     want = [t.clone() for t in c.run()]
     got = c.run(temp=temp_buffer(DeviceCrossEntropy.GetTempStorageBytes(more, channels, vocab, torch_dtype(dtype))))
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_float32_sums_over_a_large_vocabulary(cuda):
+    # two pieces of the vocabulary, the hidden gradient's sums in parts of 4096 tokens at most
+    Case(16, 40, 300001, "f32", seed=44).check()
