@@ -28,13 +28,13 @@ class DeviceDeltaRule : public LuisaModule {
         m_debug_stream = debug_stream;
     }
 
-    // For Forward, or (backward) for both calls.
+    // For Forward, or (backward) for both calls, with so many rows and sequences or fewer.
     template <SequenceFloatT T>
     static size_t GetTempStorageBytes(size_t num_rows, size_t num_sequences, DeltaHeads heads, bool backward = true) {
         const lcpp_delta_shape shape = of(num_rows, Sequences::of_length(num_sequences, 0), heads, 0);
         return lcpp_delta_rule_temp_bytes(lcpp_float_dtype_of<T>(), &shape, backward);
     }
-    // Bytes of d_saved, which Forward fills for Backward.
+    // Bytes of d_saved, which Forward fills for Backward; for so many rows and sequences or fewer.
     static size_t GetSavedStateBytes(size_t num_rows, size_t num_sequences, DeltaHeads heads) {
         const lcpp_delta_shape shape = of(num_rows, Sequences::of_length(num_sequences, 0), heads, 0);
         return lcpp_delta_rule_saved_bytes(&shape);

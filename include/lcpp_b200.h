@@ -347,7 +347,8 @@ typedef struct {
     uint64_t decay_stride, beta_stride;
     const float* init;
 } lcpp_delta_inputs;
-/* Only rows, num_sequences and the heads and dimensions of the shape are looked at.  backward != 0: for both calls. */
+/* Only rows, num_sequences and the heads and dimensions of the shape are looked at.  backward != 0: for both calls.  Buffers
+ * for so many rows and sequences serve fewer. */
 size_t      lcpp_delta_rule_temp_bytes(int dtype, const lcpp_delta_shape* shape, int backward);
 size_t      lcpp_delta_rule_saved_bytes(const lcpp_delta_shape* shape);
 /* saved (16-byte aligned; NULL: no backward pass follows) is filled for the backward call.  What is written must not

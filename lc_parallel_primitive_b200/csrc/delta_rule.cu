@@ -1756,7 +1756,9 @@ struct DrLayout {
     uint32_t planes, key_cols, rows;  // rows of an image
     uint64_t parts;                   // of a sequence
     size_t keys, unit, x, back_x, z, back_z, back_out, local, map, before, order, bytes;
-    DrLayout(int dtype, const lcpp_delta_shape& sh, bool backward) {
+    // room: bytes that there are.  A buffer for more rows and sequences serves fewer, which may want more parts than it holds:
+    // they get those that it does.
+    DrLayout(int dtype, const lcpp_delta_shape& sh, bool backward, size_t room = SIZE_MAX) {
         slots = sh.rows / DR_CHUNK + sh.num_sequences, units = slots * sh.heads;
         planes = dtype == LCPP_F32 ? 2 : 1, key_cols = sh.key_dim <= 64 ? 64 : 128, rows = (uint32_t)align_up(sh.value_dim, 32);
         size_t at = 0;
@@ -1773,10 +1775,14 @@ struct DrLayout {
             back_out = take(units * 32);
         }
         order = take(sh.num_sequences * 4);
-        parts = dr_parts(sh), local = map = before = 0;
-        if (parts > 1) {
-            const uint64_t pieces = sh.num_sequences * sh.heads * parts, state = (uint64_t)sh.value_dim * sh.key_dim;
-            local = take(pieces * state * 4), map = take(pieces * sh.key_dim * sh.key_dim * 4), before = take(pieces * state * 4);
+        const size_t whole = at;
+        for (parts = dr_parts(sh);; --parts) {
+            local = map = before = 0, at = whole;
+            if (parts > 1) {
+                const uint64_t pieces = sh.num_sequences * sh.heads * parts, state = (uint64_t)sh.value_dim * sh.key_dim;
+                local = take(pieces * state * 4), map = take(pieces * sh.key_dim * sh.key_dim * 4), before = take(pieces * state * 4);
+            }
+            if (parts == 1 || at <= room) break;
         }
         bytes = max(at, (size_t)256);
     }
@@ -1960,7 +1966,7 @@ extern "C" lcpp_status lcpp_delta_rule_forward(int dtype, const lcpp_delta_shape
     if (!elements_aligned(dtype, out) || !elements_aligned(LCPP_F32, last) || (uintptr_t)saved % 16 ||
         (shape->rows && (!out || !DrCall::stride_ok(out_stride, shape->rows, c.values()))))
         return LCPP_ERR_INVALID_ARG;
-    const DrLayout l(dtype, *shape, false);
+    const DrLayout l(dtype, *shape, false, temp_bytes);
     if (!temp || temp_bytes < l.bytes) return LCPP_ERR_TEMP_TOO_SMALL;
     if ((uintptr_t)temp % 16) return LCPP_ERR_INVALID_ARG;
     const Region ro = c.matrix(out, out_stride, c.values(), c.element()), rl = c.states(last), rt(temp, l.bytes),
@@ -2007,7 +2013,7 @@ extern "C" lcpp_status lcpp_delta_rule_backward(int dtype, const lcpp_delta_shap
     if (shape->rows && (!saved || !grads->q || !grads->k || !grads->v || !grads->beta ||
                         (grads->out && !DrCall::stride_ok(grads->out_stride, shape->rows, c.values()))))
         return LCPP_ERR_INVALID_ARG;
-    const DrLayout l(dtype, *shape, true);
+    const DrLayout l(dtype, *shape, true, temp_bytes);
     if (!temp || temp_bytes < l.bytes) return LCPP_ERR_TEMP_TOO_SMALL;
     if ((uintptr_t)temp % 16) return LCPP_ERR_INVALID_ARG;
     const uint64_t e = c.element(), rows = shape->rows;

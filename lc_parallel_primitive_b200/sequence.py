@@ -277,7 +277,7 @@ class DeviceDeltaRule(_Recorded):
     @staticmethod
     def GetTempStorageBytes(num_rows: int, num_sequences: int, heads: int, key_heads: int, key_dim: int, value_dim: int,
                             dtype=torch.bfloat16, backward: bool = True) -> int:
-        """For Forward, or (backward) for both calls."""
+        """For Forward, or (backward) for both calls, with so many rows and sequences or fewer."""
         if dtype not in _FLOATS:
             raise TypeError(f"unsupported element type {dtype}")
         shape = DeviceDeltaRule._shape(num_rows, num_sequences, heads, key_heads, key_dim, value_dim)
@@ -285,7 +285,7 @@ class DeviceDeltaRule(_Recorded):
 
     @staticmethod
     def GetSavedStateBytes(num_rows: int, num_sequences: int, heads: int, key_heads: int, key_dim: int, value_dim: int) -> int:
-        """Bytes of d_saved, which Forward fills for Backward."""
+        """Bytes of d_saved, which Forward fills for Backward; for so many rows and sequences or fewer."""
         shape = DeviceDeltaRule._shape(num_rows, num_sequences, heads, key_heads, key_dim, value_dim)
         return int(L.lib().lcpp_delta_rule_saved_bytes(shape))
 
