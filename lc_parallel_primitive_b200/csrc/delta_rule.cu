@@ -39,7 +39,7 @@ namespace lcpp {
 constexpr int DR_CHUNK = 64;
 constexpr int DR_MAX_DIM = 128;
 constexpr int DR_BLOCK = DR_CHUNK * BLOCK_ROW;  // bytes of a 64 x 64 block
-constexpr uint32_t DR_WAIT_LIMIT = 1u << 24;     // polls before a wait for a copy gives up, a second or so
+constexpr uint32_t DR_DRAIN_LIMIT = 1u << 14;    // polls of 32 ns and more that a CTA which gave up waits for its own copies
 constexpr float DR_LEAST_DECAY = -150.0f;       // exp of less is 0 in float32 anyway, and -inf has no differences
 
 struct DrShape {
@@ -96,6 +96,11 @@ struct DrImage {
     __host__ __device__ uint64_t bytes() const { return (uint64_t)rows / 32 * 2 * blocks * DR_PIECE; }
     __device__ __forceinline__ uint8_t* of(uint64_t unit) const { return at + unit * bytes(); }
 };
+
+// Wait for a barrier's phase with the library's cap of polls, which is read when the first poll fails.
+__device__ __forceinline__ bool dr_wait(uint64_t* bar, uint32_t parity) {
+    return mbar_wait(bar, parity, 1) || mbar_wait(bar, parity, g_spin_limit - 1);
+}
 
 // ---- what does not depend on the state ------------------------------------------------------------
 __device__ __forceinline__ void dr_let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
@@ -546,7 +551,7 @@ struct DrChainCta {
     const int lane, warp, g, col;
     const LaneOffsets o;
     uint32_t h, hk, seq, v0, live, row, dim;  // dim: rows of the state
-    static constexpr uint32_t limit = DR_WAIT_LIMIT;
+    uint32_t asked = 0;  // stages' copies so far, by the thread that asks for them
     uint64_t start, end, base;
     uint32_t first, chunks;  // the part's
     const T* values;
@@ -610,7 +615,11 @@ struct DrChainCta {
             }
     }
     __device__ __forceinline__ void close(const float (&s)[NT][4], float by) {
-        if (!ok) set_error(LCPP_ERR_LOOKBACK_TIMEOUT);
+        if (!ok) {  // copies under way land before the CTA's memory is another's
+            cp_async_wait_all();
+            for (uint32_t i = asked - min(asked, (uint32_t)STAGES); i < asked; ++i) mbar_wait(&sm.full[i % STAGES], (i / STAGES) & 1, DR_DRAIN_LIMIT);
+            set_error(LCPP_ERR_LOOKBACK_TIMEOUT);
+        }
         if (!to) return;
 #pragma unroll
         for (int n = 0; n < NT; ++n)
@@ -630,6 +639,7 @@ struct DrChainCta {
         return (uint32_t)min((uint64_t)DR_CHUNK, end - start - (uint64_t)chunk * DR_CHUNK);
     }
     __device__ __forceinline__ void load(uint32_t stage, uint32_t chunk) {  // one thread
+        ++asked;
         mbar_arrive_expect_tx(&sm.full[stage], Smem::STAGE);
         bulk_load(sm.stage[stage], p.keys + ((base + chunk) * p.sh.key_heads + hk) * (2 * KEYS), 2 * KEYS, &sm.full[stage]);
         bulk_load(sm.stage[stage] + 2 * KEYS, p.units + unit(chunk) * DR_UNIT, DR_UNIT, &sm.full[stage]);
@@ -645,13 +655,13 @@ struct DrChainCta {
         __syncwarp();
         if (it + 1 < chunks) load_values((it + 1) & 1, order(it + 1));
         cp_async_commit();
-        ok = __all_sync(0xffffffffu, mbar_wait(&sm.full[it % STAGES], (it / STAGES) & 1, limit));
+        ok = __all_sync(0xffffffffu, dr_wait(&sm.full[it % STAGES], (it / STAGES) & 1));
         return ok;
     }
     // Two stages: the next images are asked for amid a step, when the other warps have left the step before.
     __device__ __forceinline__ void ahead(uint32_t it) {
         if (STAGES == 2 && warp == 0 && lane == 0 && it + 1 < chunks && it >= 1) {
-            if (mbar_wait(&sm.empty[(it + 1) & 1], ((it - 1) / 2) & 1, limit)) load((it + 1) & 1, order(it + 1));
+            if (dr_wait(&sm.empty[(it + 1) & 1], ((it - 1) / 2) & 1)) load((it + 1) & 1, order(it + 1));
             else set_error(LCPP_ERR_LOOKBACK_TIMEOUT);
         }
         __syncwarp();
@@ -661,7 +671,7 @@ struct DrChainCta {
         if (lane == 0) {
             asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&sm.empty[it % STAGES])) : "memory");
             if (STAGES == 1 && warp == 0 && it + 1 < chunks) {
-                if (mbar_wait(&sm.empty[0], it & 1, limit)) load(0, order(it + 1));
+                if (dr_wait(&sm.empty[0], it & 1)) load(0, order(it + 1));
                 else set_error(LCPP_ERR_LOOKBACK_TIMEOUT);
             }
         }
@@ -1126,6 +1136,7 @@ struct DrGradientSmem {
     float dot[4][DR_CHUNK], carry[4][DR_CHUNK], sx[16];
     alignas(16) float most[2][16];
     uint64_t full[2], empty[2], keys_full;
+    uint32_t asked;  // steps whose copies were asked for
 };
 
 struct DrGradient {
@@ -1163,13 +1174,13 @@ dr_gradient_kernel(const __grid_constant__ DrGradient p) {
     if (!c.rows) return;
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5, rb = warp >> 2, cq = warp & 3, g = lane >> 2, col = (lane & 3) * 2;
     const LaneOffsets o(lane);
-    constexpr uint32_t limit = DR_WAIT_LIMIT;
     const uint32_t groups = (sh.value_dim + 15) / 16, steps = (groups + 1) / 2, total = steps * group;
     bool ok = true;
     auto load = [&](uint32_t it) {  // one thread
         const uint64_t unit = slot * sh.heads + h0 + it / steps;
         const uint32_t v = it % steps;
         uint8_t* const to = sm.step[it & 1];
+        sm.asked = it + 1;
         const bool first = v == 0;  // the head's gates and scales come along
         mbar_arrive_expect_tx(&sm.full[it & 1], Smem::STEP + (first ? (uint32_t)sizeof(DrGates) + 5 * 32 : 0));
         if (first) {
@@ -1236,12 +1247,15 @@ dr_gradient_kernel(const __grid_constant__ DrGradient p) {
         float sx = 0.0f;
         for (uint32_t v = 0; v < steps; ++v, ++it) {
             if (it + 1 < total) {  // into the buffers that the warps left a step ago
-                if (it) ok = mbar_wait(&sm.empty[(it + 1) & 1], ((it - 1) >> 1) & 1, limit) && ok;
-                if (t == 0) load(it + 1);
-                load_out(it + 1);
+                if (it) ok = ok && dr_wait(&sm.empty[(it + 1) & 1], ((it - 1) >> 1) & 1);
+                if (ok) {  // a thread that gave up asks for nothing more and waits for nothing; the others give up in their turn
+                    if (t == 0) load(it + 1);
+                    load_out(it + 1);
+                }
             }
-            if (it == 0) ok = mbar_wait(&sm.keys_full, 0, limit) && ok;
-            ok = mbar_wait(&sm.full[it & 1], (it >> 1) & 1, limit) && ok;
+            if (it == 0) ok = ok && dr_wait(&sm.keys_full, 0);
+            ok = ok && dr_wait(&sm.full[it & 1], (it >> 1) & 1);
+            __syncwarp();
             if (v == 0) {
                 const int at = lane & 7;
                 const bool have = at < (int)groups;
@@ -1567,7 +1581,14 @@ dr_gradient_kernel(const __grid_constant__ DrGradient p) {
         }
         // the next head's first barrier comes before it writes anything that is read here, but for its gates, scales and dbeta
     }
-    if (!ok) set_error(LCPP_ERR_LOOKBACK_TIMEOUT);
+    if (!ok) {  // copies under way land before the CTA's memory is another's
+        cp_async_wait_all();
+        if (t == 0) {
+            mbar_wait(&sm.keys_full, 0, DR_DRAIN_LIMIT);
+            for (uint32_t i = sm.asked - min(sm.asked, 2u); i < sm.asked; ++i) mbar_wait(&sm.full[i & 1], (i >> 1) & 1, DR_DRAIN_LIMIT);
+        }
+        set_error(LCPP_ERR_LOOKBACK_TIMEOUT);
+    }
 }
 
 // Rows outside all sequences: zeros.
