@@ -49,7 +49,7 @@ constexpr int CE_HALF_BYTES = 128 * CE_BK * 2;       // one CTA's half of an ope
 constexpr int CE_STAGE_BYTES = 2 * CE_HALF_BYTES;    // both operands
 constexpr int CE_EPILOGUE_WARPS = 8;
 constexpr int CE_THREADS = 64 + 32 * CE_EPILOGUE_WARPS;  // a loading warp, a warp that issues products, the epilogue
-constexpr uint32_t CE_WAIT_LIMIT = 1u << 22;  // polls of at most a microsecond before a wait gives up
+constexpr uint32_t CE_DRAIN_LIMIT = 1u << 14;  // polls of at most a microsecond that a CTA waits for its own copies in the end
 constexpr float CE_LOG2E = 1.44269504088896f;
 // G is kept for gradients of the loss as shares of the largest, which the sums are multiplied by in the end: for a mean's
 // equal gradients the shares are 1, and an entry's rounding is that of the probability alone (-1 for an unlikely target is
@@ -390,7 +390,7 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     __shared__ CeBarriers bar;
     const uint32_t tiles = (smem_u32(ce_smem) + 1023) & ~1023u;  // swizzled boxes start on 1024 bytes
     const uint32_t warp = threadIdx.x >> 5, rank = cluster_rank();
-    constexpr uint32_t limit = CE_WAIT_LIMIT;
+    const uint32_t limit = g_spin_limit;  // polls of at most a microsecond
     if (warp == 0 && elect_one()) {
         tma_prefetch_map(&map_a);
         tma_prefetch_map(&map_b);
@@ -446,10 +446,11 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                     }
                 }
             }
-            // every copy has landed before the CTA may leave: its stage was read
+            // Every copy has landed before the CTA may leave: its stage was read.  Stages that nothing reads any more, since a
+            // wait gave up, are waited for as long as a copy can take.
             for (uint32_t back = 0; back < CE_STAGES && back < it; ++back) {
                 const uint32_t last = it - 1 - back;
-                if (!mbar_poll(&bar.empty[last % CE_STAGES], (last / CE_STAGES) & 1, limit)) break;
+                if (!mbar_poll(&bar.empty[last % CE_STAGES], (last / CE_STAGES) & 1, CE_DRAIN_LIMIT)) break;
             }
         }
         __syncwarp();
@@ -485,6 +486,8 @@ ce_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
                 }
                 if (ok) mma_commit_pair(&bar.sum_full[d]);
             }
+            // and so have the products' last arrivals, also where the epilogue does not wait for them any more
+            if (sums) mbar_poll(&bar.sum_full[(sums - 1) & 1], ((sums - 1) / 2) & 1, CE_DRAIN_LIMIT);
         }
         __syncwarp();
     } else {

@@ -47,3 +47,22 @@ def test_delta_rule(one_poll, dtype, lengths, heads, dk, dv):
     got += [g.q, g.k, g.v, g.decay, g.beta, g.init]
     assert all(torch.equal(a, b) for a, b in zip(got, want))
     assert all(np.isfinite(host(t)).all() for t in got)
+
+
+def test_cross_entropy(one_poll):
+    """The products of a tile of 4096 channels take longer than a poll of a microsecond."""
+    import torch
+    from lc_parallel_primitive_b200 import last_device_error
+    from tests.test_cross_entropy_gpu import Case as Loss
+
+    lib = L.lib()
+    L.check(lib.lcpp_set_spin_limit(0))
+    c = Loss(600, 4096, 2000, "bf16", seed=62)
+    want = [t.clone() for t in c.run()]
+    L.check(lib.lcpp_set_spin_limit(1))
+    for _ in range(3):
+        c.run(check=False)
+        torch.cuda.synchronize()
+        assert last_device_error() == L.ERR_LOOKBACK_TIMEOUT
+    L.check(lib.lcpp_set_spin_limit(0))
+    assert all(torch.equal(a, b) for a, b in zip(c.run(), want))
