@@ -97,9 +97,21 @@ struct DrImage {
     __device__ __forceinline__ uint8_t* of(uint64_t unit) const { return at + unit * bytes(); }
 };
 
-// Wait for a barrier's phase with the library's cap of polls, which is read when the first poll fails.
+// Wait for a barrier's phase, with the library's cap of polls of at most a microsecond (read when the first one fails).
+__device__ __forceinline__ bool dr_poll(uint64_t* bar, uint32_t parity) {
+    uint32_t done;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 1000;\n selp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(done)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    return done;
+}
 __device__ __forceinline__ bool dr_wait(uint64_t* bar, uint32_t parity) {
-    return mbar_wait(bar, parity, 1) || mbar_wait(bar, parity, g_spin_limit - 1);
+    bool done = dr_poll(bar, parity);
+    if (!done)
+        for (uint32_t left = g_spin_limit; --left && !done;) done = dr_poll(bar, parity);
+    return done;
 }
 
 // ---- what does not depend on the state ------------------------------------------------------------
