@@ -1469,10 +1469,9 @@ dr_gradient_kernel(const __grid_constant__ DrGradient p) {
                 }
 #pragma unroll
                 for (int m = half * 2; m < half * 2 + 2; ++m) dq[j][m] *= fq, er[j][m] *= fe, wr[j][m] *= fw;
-                carry[half] = fmaf(kv.x, wr[j][half * 2], fmaf(kv.y, wr[j][half * 2 + 1], carry[half]));
+                carry[half] = fmaf(kv.x * back_k, wr[j][half * 2], fmaf(kv.y * back_k, wr[j][half * 2 + 1], carry[half]));
                 wr[j][half * 2] *= into_n, wr[j][half * 2 + 1] *= into_n;
             }
-            carry[half] *= back_k;
         }
         __syncthreads();
         // rows of dA and dN against the keys before; then columns against the later ones: dN^T K, and in dA^T Q's domain that
