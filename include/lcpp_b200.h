@@ -333,7 +333,14 @@ lcpp_status lcpp_beam_reorder(const void* in, uint64_t in_layer_bytes, uint64_t 
  * [key_dim] (init NULL: zeros, last NULL: not wanted; last may be init).  Inputs are finite: the
  * work goes by chunks of 64 rows and 16 value dimensions, so a value that is not reaches rows of its sequence up to 63
  * before it, too, and value dimensions beside it, but no other sequence or head (a key or query: its key head's).  Rows
- * outside all sequences may hold anything. */
+ * outside all sequences may hold anything.
+ * Precision (the step is float32 throughout): sums are float32; what is multiplied enters as two float16 parts with a power
+ * of two taken out, which leaves out 2^-22 of a product (16-bit q and k as one part, exact).  q and k share a power with
+ * the 64 rows of their chunk and head, and count to 2^-39 (16 bits: whole down to 2^-28) of the largest of these; values, states
+ * and their gradients share it with their 16 value dimensions, and count to 2^-32 of the largest.  Powers have limits: q and k of
+ * 2^-42 and the others of 2^-75 and more keep all their bits, below 2^-65 and 2^-98 nothing is left.  What the rows of a chunk
+ * bring to its outputs counts to 2^-62 of the state before it.  bf16 outputs are made of one part (11 bits) of the state, of
+ * u and of q k^T: off by 2^-12 of the terms of their sums, and then rounded. */
 typedef struct {
     uint64_t rows, num_sequences, length; /* length: of every sequence, where offsets is NULL */
     const uint32_t* offsets;              /* num_sequences + 1 ascending row offsets */
@@ -483,8 +490,9 @@ size_t      lcpp_lookback_temp_bytes(uint64_t num_tiles);
 lcpp_status lcpp_lookback_tiles(const uint32_t* aggregates, uint32_t* exclusive_out,
                                 uint32_t* inclusive_out, uint64_t num_tiles,
                                 void* temp, size_t temp_bytes, void* stream);
-/* Caps every look-back wait at `iterations` polls (0 restores the default,
- * about one second) on the current device. */
+/* Caps every wait within a kernel (look-back, copies, products) at
+ * `iterations` polls (0 restores the default, a second or so; a few in the
+ * delta rule and the cross entropy) on the current device. */
 lcpp_status lcpp_set_spin_limit(uint32_t iterations);
 /* One warp runs the look-back of tile `tile` against the caller's descriptor
  * array (num_tiles 64-bit words, status in the high half: 0 = not yet

@@ -10,10 +10,10 @@
 // sum for each row and 128 columns), and, for a piece of the vocabulary at a time, the logits again with G as the
 // epilogue's result (CE_GRAD), G W (CE_HIDDEN) and G^T H (CE_WEIGHT).
 //
-// Times: 8192 rows of 4096 bf16 channels over 128000 tokens: logits 5.4 ms (1.59 PFLOP/s), and 5.5, 6.1 and 5.7 ms in four
-// pieces for the gradients; 34 TFLOP in 22.4 to 23.1 ms, 1.49 to 1.54 PFLOP/s, with the power limit's clocks.  The logits are
-// computed twice, a quarter of the work: kept for the backward pass they would take 2 bytes each (2.1 GB here), and
-// rounded to 8 bits they would be off by more than the probabilities may be.
+// Times: 8192 rows of 4096 bf16 channels over 128000 tokens, 7373 of which take part (29 tiles): logits 5.8 ms (1.34 PFLOP/s of
+// what the tiles take), and 5.9, 6.5 and 6.1 ms in four pieces for the gradients; 31 TFLOP in 23.4 ms, 1.33 PFLOP/s, with
+// the power limit's clocks.  The logits are computed twice, a quarter of the work: kept for the backward pass they would take
+// 2 bytes each (2.1 GB here), and rounded to 8 bits they would be off by more than the probabilities may be.
 #include "float_types.cuh"
 #include "tcgen05.cuh"
 #include "warp_mma.cuh"
@@ -375,7 +375,7 @@ __device__ __forceinline__ void ce_epilogue(const CeGemm& p, uint32_t tmem, uint
     }
 }
 
-// Bound by the tensor cores: 4096 rows x 2048 x 65536 bf16, tensor pipe 95 % of the cycles for the logits and for G, 94 % for
+// Bound by the tensor cores: 4096 rows (3686 that take part) x 2048 x 65536 bf16, tensor pipe 95 % of the cycles for the logits and for G, 94 % for
 // G^T H, 87 % for G W with its 1.7 waves of tiles and parts; DRAM 11 to 20 % (G W 30 %), L2 50 %.  Long runs of it meet the power limit,
 // so that bytes not moved are time too.  2 CTAs a tile halve what shared memory and L2 pass on for the same products.
 // One pair of CTAs makes tiles of 256 x 256: each CTA holds 128 rows of A and 128 rows of B (as K-major) and has 128

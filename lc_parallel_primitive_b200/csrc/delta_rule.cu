@@ -30,7 +30,7 @@
 // split and written to shared memory between any two.
 //
 // Times at 8 sequences of 2048 tokens, 16 heads, 128 dimensions, bf16 (4096 chunks and heads): preparation 126 us, forward
-// with what the backward pass wants 269, backward chain 259, gradients 592; 1379 us in all.
+// with what the backward pass wants 261, backward chain 254, gradients 579; 1353 us in all.
 #include "float_types.cuh"
 #include "warp_mma.cuh"
 
@@ -1166,9 +1166,10 @@ struct DrGradient {
 
 // A CTA a chunk and key head: 32 value dimensions a step with the next step's images on their way (a step's two buffers are
 // handed over by barriers in memory, so that warps need not meet), then what the key columns need of all of them.  Bound by
-// shared memory (46 % of its pipe's cycles), the tensor pipe (32 %) and what each warp waits between: about 235 us of
-// the 592 are outside the steps.  8 warps with twice the columns each took 565 us where 16 took 596, but 1515 us instead
-// of 1424 for the whole pass before the buffers were handed over so.
+// shared memory (46 % of its pipe's cycles), the tensor pipe (32 %) and what each warp waits between: 579 us for 8 x 2048
+// tokens and 16 heads of 128 x 128, of which about 235 are outside the steps.  16 warps were chosen when warps met after each
+// step (1424 us for the whole pass, 1515 with 8 warps of twice the columns); as the buffers are handed over now 8 have not been
+// compared.
 template <typename T, int DK, bool SHARED>  // SHARED: several heads a key head
 __global__ void __launch_bounds__(DR_GRAD_THREADS, 1)
 dr_gradient_kernel(const __grid_constant__ DrGradient p) {
@@ -1768,7 +1769,7 @@ static DrShape dr_shape(const lcpp_delta_shape& sh) {
 // Into how many parts the sequences are cut, so that the chains have work for all SMs: the number with the least time, by
 // the sequences' average length and the waves of CTAs with 8 warps (16 value dimensions each) that both passes take.  A
 // chunk takes such a CTA 5.8 us in the second pass, 3.9 us in the first, and a chain of 2 warps alone on its SM 5.1 us
-// (bf16, 128 dimensions).  A part has 8 chunks at least.
+// (bf16, 128 dimensions; other types and sizes, whose times were not taken, go by the same).  A part has 8 chunks at least.
 static uint64_t dr_parts(const lcpp_delta_shape& sh) {
     const uint64_t sms = device_info().sms, streams = sh.num_sequences * sh.heads;
     if (!streams || streams * ceil_div(sh.value_dim, 32) > sms) return 1;

@@ -267,7 +267,8 @@ class DeviceDeltaRule(_Recorded):
     None for 1 / sqrt(key_dim).  offsets_or_length as in DeviceLinearRecurrence; states are contiguous float32
     (sequences, heads, value_dim, key_dim).  temp_storage is contiguous and 16-byte aligned, as temp_buffer's is.
     Inputs are finite: the work goes by 64 rows and 16 value dimensions, so a NaN reaches up to 63 rows of its sequence
-    before it and value dimensions beside it, too, but no other sequence or head.
+    before it and value dimensions beside it, too, but no other sequence or head.  float32 values enter products in two
+    float16 parts, bf16 outputs are made of 11 bits of the state; include/lcpp_b200.h states precision and range.
     """
 
     @staticmethod
