@@ -334,13 +334,14 @@ lcpp_status lcpp_beam_reorder(const void* in, uint64_t in_layer_bytes, uint64_t 
  * work goes by chunks of 64 rows and 16 value dimensions, so a value that is not reaches rows of its sequence up to 63
  * before it, too, and value dimensions beside it, but no other sequence or head (a key or query: its key head's).  Rows
  * outside all sequences may hold anything.
- * Precision (the step is float32 throughout): sums are float32; what is multiplied enters as two float16 parts with a power
- * of two taken out, which leaves out 2^-22 of a product (16-bit q and k as one part, exact).  q and k share a power with
- * the 64 rows of their chunk and head, and count to 2^-39 (16 bits: whole down to 2^-28) of the largest of these; values, states
- * and their gradients share it with their 16 value dimensions, and count to 2^-32 of the largest.  Powers have limits: q and k of
- * 2^-42 and the others of 2^-75 and more keep all their bits, below 2^-65 and 2^-98 nothing is left.  What the rows of a chunk
- * bring to its outputs counts to 2^-62 of the state before it.  bf16 outputs are made of one part (11 bits) of the state, of
- * u and of q k^T: off by 2^-12 of the terms of their sums, and then rounded. */
+ * Precision (the step is float32 throughout): sums are float32; what is multiplied enters as two float16 parts with
+ * a power of two taken out, which leaves out 2^-22 of a product (16-bit q and k as one part, exact).  q and k share
+ * a power with the 64 rows of their chunk and head, and count to 2^-39 (16 bits: whole down to 2^-28) of the largest
+ * of these; values, states and their gradients share it with their 16 value dimensions, and count to 2^-32 of the
+ * largest.  Powers have limits: q and k of 2^-42 and the others of 2^-75 and more keep all their bits, below 2^-65
+ * and 2^-98 nothing is left.  What the rows of a chunk bring to its outputs counts to 2^-62 of the state before it.
+ * bf16 outputs are made of one part (11 bits) of the state, of u and of q k^T: off by 2^-12 of the terms of their
+ * sums, and then rounded. */
 typedef struct {
     uint64_t rows, num_sequences, length; /* length: of every sequence, where offsets is NULL */
     const uint32_t* offsets;              /* num_sequences + 1 ascending row offsets */
@@ -389,9 +390,9 @@ lcpp_status lcpp_delta_rule_step(int dtype, const lcpp_delta_shape* shape, const
  * in parts: of two float16 with a scale for each row in the logits, 2^-22 of a product, or 2^-39 of its rows' largest
  * values where that is more; of three bf16 in the gradients, about 2^-24).  The tensor cores cut sums off, so that a logit
  * comes out too small by up to 1.2e-9 of itself a channel, 5e-6 for 4096.  A loss is never negative.
- * A row with a negative target takes no part: its loss, logsum and
- * gradient are 0, it adds nothing to the weight's gradient, and its hidden state may hold anything; a target >= vocab
- * does the same and leaves LCPP_ERR_INVALID_ARG in the device error word.  loss or logsum may be NULL.
+ * A row with a negative target takes no part: its loss, logsum and gradient are 0, it adds nothing to the weight's
+ * gradient, and its hidden state may hold anything; a target >= vocab does the same and leaves LCPP_ERR_INVALID_ARG
+ * in the device error word.  loss or logsum may be NULL.
  * rows <= 2^24, vocab <= 2^30; temp is refused where it is not 32-byte aligned.  What is written, temp included, must
  * not overlap anything else.
  * temp bytes: for the forward call, or (backward != 0) for both, with so many rows or fewer; aligned = 0 where a row of
